@@ -9,12 +9,19 @@ holds positions 64e..64e+63 (all-keys group) or, in a window group, the position
 p with (p // 64) % ring_pages == e: a ring of ring_pages = ceil(window / 64) pages
 that is written round and round.
 
+With `need.bits` 4 the arrays are uint8 [n_pages, n_kv_heads, ops.tile4_bytes(head_dim)]:
+codes of 4 bits with a scale and a middle per 64 numbers (parts/attention4.py).
+
+Slots may share pages (a forked sequence begins with the pages of the one it comes
+from): a page counts its holders, and `grow` gives a slot that is about to write
+into a page with other holders a page of its own with the same contents first.
+
 The host keeps the table and the lengths; `flush()` copies changed rows to the
 device before a step runs.
 """
 from __future__ import annotations
 
-from typing import Dict, List
+from typing import Dict, List, Optional, Sequence
 
 import torch
 
@@ -39,17 +46,27 @@ class KVGroup:
         full_entries = (max_seq_len + PAGE - 1) // PAGE
         self.table_stride = max(1, min(full_entries, self.ring_pages) if self.ring_pages else full_entries)
         self.pages = IdPool(n_pages, "page")
-        shape = (n_pages, need.n_kv_heads, PAGE, need.head_dim)
+        if need.bits is not None:
+            from ..parts import attention4
+            if need.bits != 4 or need.keys_only or (need.v_head_dim or need.head_dim) != need.head_dim or not attention4.supports(need.head_dim):
+                raise CacheError(f"no cache in {need.bits} bits for heads of {need.head_dim} numbers: 4 bits are offered for keys and "
+                                 f"values of {attention4.GROUP} to {attention4.MAX_HEAD_DIM} numbers, a multiple of {attention4.GROUP}")
+            dtype = torch.uint8
+            shape = v_shape = (n_pages, need.n_kv_heads, ops.tile4_bytes(need.head_dim))
+        else:
+            shape = (n_pages, need.n_kv_heads, PAGE, need.head_dim)
+            v_shape = (n_pages, need.n_kv_heads, PAGE, need.v_head_dim or need.head_dim)
         # zero-filled once: a page's unwritten rows are never selected by a mask, but they
         # are multiplied by zero weights, and 0 * NaN would not be 0
         self.k = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(n_entries)]
-        v_shape = (n_pages, need.n_kv_heads, PAGE, need.v_head_dim or need.head_dim)
         self.v = [None if need.keys_only else torch.zeros(v_shape, dtype=dtype, device=device) for _ in range(n_entries)]
         self.table_host = torch.zeros((n_slots, self.table_stride), dtype=torch.int32)
         self._table_np = self.table_host.numpy()       # the same memory: an entry is written without a tensor operation
         self.table_dev = torch.zeros((n_slots, self.table_stride), dtype=torch.int32, device=device)
         self._slot_pages: Dict[int, List[int]] = {}
+        self._holders: Dict[int, int] = {}             # pages that several slots hold -> how many
         self._dirty: set = set()
+        self._arrays: Optional[torch.Tensor] = None    # what ops.copy_pages wants of the arrays, made at the first copy
 
     def chunk_room(self):
         """The most tokens a sequence may bring in one step that attends over this group's
@@ -67,14 +84,45 @@ class KVGroup:
             raise CacheError(f"slot {slot} is opened twice")
         self._slot_pages[slot] = []
 
-    def grow(self, slot: int, new_len: int) -> None:
-        """Make sure the slot has pages for positions < new_len."""
+    def shared_before(self, slot: int, old_len: int, new_len: int) -> List[int]:
+        """Table entries of the slot that positions old_len..new_len-1 are written to and whose pages others hold too."""
+        if not self._holders or new_len <= old_len:
+            return []
+        held, first, last = self._slot_pages[slot], old_len // PAGE, (new_len - 1) // PAGE
+        if self.ring_pages:
+            entries = {p % self.ring_pages for p in range(max(first, last - self.ring_pages + 1), last + 1)}
+        else:
+            entries = range(first, last + 1)
+        return [e for e in sorted(entries) if e < len(held) and held[e] in self._holders]
+
+    def more_pages(self, slots: Sequence[int], old_lens: Sequence[int], new_lens: Sequence[int]) -> int:
+        """Pages that `grow` takes for these slots, one after another: of a shared page the last holder needs no copy."""
+        more, copied = 0, {}
+        for slot, old, new in zip(slots, old_lens, new_lens):
+            more += max(0, self.pages_for(new) - len(self._slot_pages[slot]))
+            for e in self.shared_before(slot, old, new):
+                page = self._slot_pages[slot][e]
+                copied[page] = min(copied.get(page, 0) + 1, self._holders[page] - 1)
+        return more + sum(copied.values())
+
+    def grow(self, slot: int, new_len: int, old_len: Optional[int] = None) -> None:
+        """Make sure the slot has pages for positions < new_len, and that no other slot holds those that positions from old_len on
+        are written to."""
         held = self._slot_pages[slot]
         want = self.pages_for(new_len)
         if self.ring_pages == 0 and (new_len + PAGE - 1) // PAGE > self.table_stride:
             raise CacheError(f"a sequence of {new_len} tokens is longer than the cache's tables "
                              f"hold ({self.table_stride * PAGE})")
         row = self._table_np[slot]
+        shared = self.shared_before(slot, new_len if old_len is None else old_len, new_len)
+        if shared:
+            olds = [held[e] for e in shared]
+            news = [self.pages.take() for _ in shared]
+            self._copy_listed(olds, news)
+            for e, old, new in zip(shared, olds, news):
+                row[e] = held[e] = new
+                self._let_go(old)
+            self._dirty.add(slot)
         while len(held) < want:
             page = self.pages.take()
             row[len(held)] = page
@@ -83,7 +131,70 @@ class KVGroup:
 
     def close_slot(self, slot: int) -> None:
         for page in self._slot_pages.pop(slot):
+            self._let_go(page)
+
+    def _let_go(self, page: int) -> None:
+        """One holder less; the last one gives the page back."""
+        n = self._holders.pop(page, 1)
+        if n == 1:
             self.pages.give_back(page)
+        elif n > 2:
+            self._holders[page] = n - 1
+
+    def share(self, slot: int, new_slot: int, length: int) -> None:
+        """The (open, empty) new slot holds the pages of the slot's first `length` positions too."""
+        pages = self._slot_pages[slot][:self.pages_for(length)]
+        for page in pages:
+            self._holders[page] = self._holders.get(page, 1) + 1
+        self._slot_pages[new_slot] = list(pages)
+        self._table_np[new_slot, :len(pages)] = pages
+        self._dirty.add(new_slot)
+
+    def compact(self) -> int:
+        """Move the held pages to the front of the arrays; the number of them."""
+        n = self.pages.n_held
+        olds = sorted(p for p in self.pages.held() if p >= n)
+        news = self.pages.move_down(olds)
+        if olds:
+            self._copy_listed(olds, news)
+            to = dict(zip(olds, news))
+            self._holders = {to.get(p, p): k for p, k in self._holders.items()}
+            for slot, held in self._slot_pages.items():
+                if any(p in to for p in held):
+                    held[:] = [to.get(p, p) for p in held]
+                    self._table_np[slot, :len(held)] = held
+                    self._dirty.add(slot)
+        return n
+
+    def resize(self, n_pages: int) -> None:
+        """Arrays of n_pages pages with what the held pages hold (they must fit); the old arrays' memory goes back."""
+        if self.compact() > n_pages:
+            raise CacheError(f"{self.pages.n_held} pages are held: they do not fit into {n_pages}")
+        keep = min(n_pages, self.pages.n)
+        for arrays in (self.k, self.v):
+            for i, old in enumerate(arrays):
+                if old is not None:
+                    arrays[i] = new = torch.zeros((n_pages,) + tuple(old.shape[1:]), dtype=old.dtype, device=old.device)
+                    new[:keep].copy_(old[:keep])
+        self.pages.resize(n_pages)
+        self._arrays = None
+
+    def copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:
+        """Page src[i] to page dst[i] (int32, on the cache's device) in the arrays of all entries, in one launch; pairs with a page
+        outside the arrays copy nothing.  No page may be written twice, or read and written, in one call."""
+        arrays = self.k + [v for v in self.v if v is not None]
+        if self._arrays is None:
+            page = [a[0].numel() * a.element_size() for a in arrays]
+            self._arrays = torch.tensor([[a.data_ptr(), b] for a, b in zip(arrays, page)], dtype=torch.int64).to(arrays[0].device), max(page)
+        ops.copy_pages(self._arrays[0], self._arrays[1], src, dst, self.pages.n)
+
+    def _copy_listed(self, src: Sequence[int], dst: Sequence[int]) -> None:
+        if self.table_dev.device.type != "cuda":            # the bookkeeping without a GPU
+            for a in self.k + [v for v in self.v if v is not None]:
+                a[list(dst)] = a[list(src)]
+            return
+        pairs = torch.tensor([list(src), list(dst)], dtype=torch.int32).pin_memory().to(self.table_dev.device, non_blocking=True)
+        self.copy_pages(pairs[0], pairs[1])
 
     def flush(self) -> None:
         """Changed rows of the table go to the device: staged in pinned memory (the host may change the
@@ -105,9 +216,11 @@ class KVGroup:
 
     def view(self, entry: int) -> ops.PagedKVArgs:
         return ops.PagedKVArgs(self.k[entry], self.v[entry], self.table_dev, self.ring_pages,
-                               self.need.n_kv_heads, self.need.head_dim, self.need.v_head_dim or 0)
+                               self.need.n_kv_heads, self.need.head_dim, self.need.v_head_dim or 0, self.need.bits)
 
     def bytes_per_token(self) -> int:
+        if self.need.bits is not None:
+            return self.n_entries * 2 * self.need.n_kv_heads * ops.tile4_bytes(self.need.head_dim) // PAGE
         e = self.k[0].element_size()
         per_head = self.need.head_dim + (0 if self.need.keys_only else (self.need.v_head_dim or self.need.head_dim))
         return self.n_entries * self.need.n_kv_heads * per_head * e

@@ -10,6 +10,9 @@ group.
     slots = cache.admit(lengths)         # one slot per sequence, pages for its prompt
     cache.extend(slot, new_len)          # before a step that lengthens the sequence
     cache.release(slot)                  # the sequence has ended: slot and pages go back
+    cache.fork(slot, n)                  # n sequences that go on from where this one is; pages are shared until one writes
+    cache.compact()                      # held pages to the front of the arrays
+    cache.resize(max_tokens)             # and arrays of another size
 
 Per-sequence state of fixed size lives beside the keys and values, a row per slot,
 zeroed when a sequence is admitted to the slot: the record (`record`, int32
@@ -23,6 +26,7 @@ from the record.
 """
 from __future__ import annotations
 
+from collections import Counter
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
@@ -71,9 +75,11 @@ class CacheManager:
                 placed[e] = (len(self.groups), j)
             self.groups.append(g)
         self.stores: List[CallStore] = []
+        self._placed: List[Optional[Tuple[int, int]]] = []      # entry -> (group, index in group) of what it reads
         for i, need in enumerate(kv_needs):
             src = cache_from[i]
             kv, owns = None, True
+            self._placed.append(None)
             if need is not None:
                 owner = i if src is None else src
                 if owner not in placed:
@@ -83,6 +89,7 @@ class CacheManager:
                     raise CacheError(f"entry {i} reads the cache of entry {src}, whose keys have "
                                      f"another shape or window")
                 kv, owns = self.groups[gi].view(j), src is None
+                self._placed[-1] = (gi, j)
             state = {s.name: torch.zeros((self.n_slots,) + tuple(s.shape), dtype=s.dtype,
                                          device=self.device) for s in state_needs[i]}
             self.stores.append(CallStore(kv, owns, state))
@@ -154,12 +161,12 @@ class CacheManager:
             raise CacheError(f"a sequence of {new_len} tokens is longer than the cache holds "
                              f"({self.max_seq_len})")
         for g in self.groups:          # all or nothing: look before taking
-            more = g.pages_for(new_len) - len(g._slot_pages[slot])
+            more = g.more_pages([slot], [self.lengths[slot]], [new_len])
             if more > g.pages.n_free:
                 raise CacheError(f"the cache has no free page left for slot {slot} to reach "
                                  f"{new_len} tokens ({more} wanted, {g.pages.n_free} free)")
         for g in self.groups:
-            g.grow(slot, new_len)
+            g.grow(slot, new_len, self.lengths[slot])
         self.lengths[slot] = max(self.lengths[slot], new_len)
 
     def extend_all(self, slots: Sequence[int], new_lens: Sequence[int]) -> None:
@@ -172,13 +179,13 @@ class CacheManager:
                 raise CacheError(f"a sequence of {n} tokens is longer than the cache holds "
                                  f"({self.max_seq_len})")
         for g in self.groups:
-            more = sum(max(0, g.pages_for(n) - len(g._slot_pages[slot])) for slot, n in zip(slots, new_lens))
+            more = g.more_pages(slots, [self.lengths[s] for s in slots], new_lens)
             if more > g.pages.n_free:
                 raise CacheError(f"the cache has no free pages left for this step ({more} wanted, "
                                  f"{g.pages.n_free} free of {g.pages.n})")
         for slot, n in zip(slots, new_lens):
             for g in self.groups:
-                g.grow(slot, n)
+                g.grow(slot, n, self.lengths[slot])
             self.lengths[slot] = max(self.lengths[slot], n)
 
     def chunk_room(self) -> Optional[int]:
@@ -186,6 +193,46 @@ class CacheManager:
         the smallest room of the window groups' rings."""
         rooms = [r for r in (g.chunk_room() for g in self.groups) if r is not None]
         return min(rooms) if rooms else None
+
+    def fork(self, slot: int, n: int = 1) -> List[int]:
+        """n new slots whose sequences are, for now, the slot's: the same length, the same pages (a page is copied when one of its
+        holders is about to write into it), a copy of the state of fixed size and of the record.  All or nothing."""
+        if slot not in self.lengths:
+            raise CacheError(f"slot {slot} holds no sequence")
+        if n < 0 or n > self.slots.n_free:
+            raise CacheError(f"the cache has {self.slots.n_free} free slots, {n} wanted")
+        out = [self.slots.take() for _ in range(n)]
+        for new in out:
+            self.lengths[new] = self.lengths[slot]
+            for g in self.groups:
+                g.open_slot(new)
+                g.share(slot, new, self.lengths[slot])
+            for t in [self.record, self.recent] + self.state_tensors():
+                t[new].copy_(t[slot])
+        return out
+
+    def compact(self) -> None:
+        """Move every group's held pages to the front of its arrays."""
+        for g in self.groups:
+            g.compact()
+
+    def resize(self, max_tokens: int) -> None:
+        """Pages for max_tokens tokens from now on (see the class): a smaller cache gives memory back, a larger one takes more.  The
+        sequences held must fit; slots, and the longest sequence that the page tables have room for, stay as they were made.  The
+        arrays are new ones: graphs captured before must not be replayed."""
+        if max_tokens <= 0:
+            raise CacheError("the cache must hold at least one token")
+        n_pages = (max_tokens + PAGE - 1) // PAGE
+        for g in self.groups:
+            if g.pages.n_held > n_pages:
+                raise CacheError(f"{g.pages.n_held} pages are held: they do not fit into {n_pages}")
+        self.n_pages = n_pages
+        for g in self.groups:
+            g.resize(n_pages)
+        for store, place in zip(self.stores, self._placed):
+            if place is not None:
+                view = self.groups[place[0]].view(place[1])
+                store.kv.k_pages, store.kv.v_pages = view.k_pages, view.v_pages
 
     def release(self, slot: int) -> None:
         if slot not in self.lengths:
@@ -207,7 +254,10 @@ class CacheManager:
         for g in self.groups:
             g.pages.check()
             owned = [p for pages in g._slot_pages.values() for p in pages]
-            if len(owned) != len(set(owned)):
+            counts = Counter(owned)
+            if any(len(set(pages)) != len(pages) for pages in g._slot_pages.values()):
+                raise CacheError("a page is held twice by one sequence")
+            if {p: k for p, k in counts.items() if k > 1} != g._holders:
                 raise CacheError("a page is held by two sequences")
             if set(owned) != g.pages.held():
                 raise CacheError("held pages and the sequences' pages differ")

@@ -52,6 +52,22 @@ class IdPool:
                 hi = mid
         self._free.insert(lo, i)
 
+    def move_down(self, ids: List[int]) -> List[int]:
+        """Hold the lowest free ids in the place of these held ones; the new ids, in the same order."""
+        new = [self._free.pop() for _ in ids]
+        for i in ids:
+            self._held.remove(i)
+        self._held.update(new)
+        self._free = sorted(set(range(self.n)) - self._held, reverse=True)
+        return new
+
+    def resize(self, n: int) -> None:
+        """Ids 0..n-1 from now on; none of the held ones may be n or above."""
+        if any(i >= n for i in self._held):
+            raise CacheError(f"a held {self.what} does not fit into {n}")
+        self.n = n
+        self._free = sorted(set(range(n)) - self._held, reverse=True)
+
     def check(self) -> None:
         """Every id is free or held, never both, never neither."""
         free = set(self._free)

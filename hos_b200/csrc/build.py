@@ -26,6 +26,8 @@ Libraries and what needs them:
   mixers      a norm after the residual sum, the norm-and-gate of a mixer's heads, and the
               matrix-state recurrences with a decay per head (constant, or per token with the
               delta rule and short convolutions) or per key channel, hyper-connections
+  fourbit     products with 4-bit weights, keys and values in 4-bit pages and attention over them,
+              copies of pages (a forked sequence, a compacted cache)
 A model builds only the libraries whose parts it has.
 """
 from __future__ import annotations
@@ -58,6 +60,7 @@ _STATIC_LIBS: Dict[str, Tuple[List[str], List[str]]] = {
     "blocks": (["latent_attention.cu", "latent_prompt.cu", "wkv.cu"], []),
     "gated_attn": (["gated_attention.cu", "gated_attention_mma.cu"], []),
     "mixers": (["postnorm.cu", "state_scan.cu", "hyper.cu"], []),
+    "fourbit": (["weights4.cu", "attention4.cu", "pages.cu"], []),
 }
 
 _loaded: Dict[str, ctypes.CDLL] = {}

@@ -10,6 +10,7 @@ Prompts are token ids separated by commas (tokenizers are not part of this libra
 be given several times, which makes a batch.  The model is `-m`, else $HOS_MODEL
 (src/main.rs:3419-3425).  `--fp32` runs everything in true 32-bit; `--random <config.json>`
 runs that configuration with random weights from `--seed` instead of a model folder.
+`--weight-bits 4` holds attention projections and gated feed-forwards in 4 bits, `--cache-bits 4` keys and values.
 stdout carries token ids only; everything else goes to stderr with the reference's `[hos]`
 prefix.  An unknown option ends with status 2 (src/main.rs:3547-3554).
 """
@@ -26,6 +27,7 @@ USAGE = """usage: hos -m model_dir -p "id,id,..." [-n 64] [--temp 0.0] [--seed 4
        hos -m model_dir --perplexity "id,id,..." # score a token sequence
 options: --top-k 40 --top-p 0.95 --repeat-penalty 1.1 --repeat-last-n 64 --no-echo --fp32
          --random config.json (random weights from --seed instead of -m)
+         --weight-bits 4 --cache-bits 4 (matrices, keys and values in 4 bits)
          --ctx C (longest sequence the cache is sized for)
          --bench: --batch B sequences of --prompt-len T fixed ids each (default: one prompt of 16)"""
 
@@ -48,6 +50,8 @@ class Args:
         self.perplexity: Optional[List[int]] = None
         self.random: Optional[str] = None
         self.batch, self.prompt_len, self.ctx = 1, 16, None
+        self.weight_bits: Optional[int] = None
+        self.cache_bits: Optional[int] = None
 
 
 def parse_args(argv: List[str]) -> Args:
@@ -91,6 +95,10 @@ def parse_args(argv: List[str]) -> Args:
             a.random = value(arg)
         elif arg == "--perplexity":
             a.perplexity = parse_ids(value(arg))
+        elif arg == "--weight-bits":
+            a.weight_bits = int(value(arg))
+        elif arg == "--cache-bits":
+            a.cache_bits = int(value(arg))
         elif arg == "--batch":
             a.batch = max(1, int(value(arg)))
         elif arg == "--prompt-len":
@@ -125,9 +133,9 @@ def main(argv: Optional[List[str]] = None) -> int:
     from .engine import Engine
     dtype = "float32" if args.fp32 else "bfloat16"
     n_seqs = max(1, len(args.prompts), args.batch if args.bench else 1)
-    size = {}
+    size = dict(weight_bits=args.weight_bits, cache_bits=args.cache_bits)
     if args.ctx is not None:
-        size = dict(max_seq_len=args.ctx, max_tokens=n_seqs * ((args.ctx + 63) // 64 * 64))
+        size.update(max_seq_len=args.ctx, max_tokens=n_seqs * ((args.ctx + 63) // 64 * 64))
     try:
         if args.random:
             from .. import models  # noqa: F401

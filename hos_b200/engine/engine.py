@@ -78,11 +78,14 @@ class Engine:
     dtype       "bfloat16" (the fast kernels) or "float32" (everything in true 32-bit)
     max_batch   most sequences generated side by side
     max_tokens  tokens the cache holds (default: max_batch full contexts, at most 8192 each)
+    weight_bits 4: attention projections and gated feed-forwards in 4 bits (None: as `dtype` says)
+    cache_bits  4: keys and values in 4 bits
     """
 
     def __init__(self, path: Optional[str] = None, gpu: bool = True, dtype: str = "bfloat16",
                  max_batch: int = 8, max_tokens: Optional[int] = None,
-                 max_seq_len: Optional[int] = None, _runner: Optional[Runner] = None):
+                 max_seq_len: Optional[int] = None, weight_bits: Optional[int] = None,
+                 cache_bits: Optional[int] = None, _runner: Optional[Runner] = None):
         self.max_batch = max_batch
         if _runner is not None:
             self.runner = _runner
@@ -95,7 +98,8 @@ class Engine:
             cfg = config_from_dict(read_config_json(path))
             self.runner = Runner.from_folder(path, dtype=dtype, max_seq_len=max_seq_len,
                                              max_tokens=self._default_tokens(cfg, max_batch, max_tokens,
-                                                                             max_seq_len))
+                                                                             max_seq_len),
+                                             weight_bits=weight_bits, cache_bits=cache_bits)
         self.config = self.runner.config
         self.stop_ids: Tuple[int, ...] = tuple(self.runner.plan.stop_token_ids)
 
@@ -109,9 +113,10 @@ class Engine:
     @classmethod
     def from_config(cls, config: ModelConfig, seed: int = 0, dtype: str = "bfloat16",
                     max_batch: int = 8, max_tokens: Optional[int] = None,
-                    max_seq_len: Optional[int] = None) -> "Engine":
+                    max_seq_len: Optional[int] = None, weight_bits: Optional[int] = None,
+                    cache_bits: Optional[int] = None) -> "Engine":
         """A model with random weights made on the device (no files)."""
-        runner = Runner.from_random(config, seed, dtype=dtype, max_seq_len=max_seq_len,
+        runner = Runner.from_random(config, seed, dtype=dtype, max_seq_len=max_seq_len, weight_bits=weight_bits, cache_bits=cache_bits,
                                     max_tokens=cls._default_tokens(config, max_batch, max_tokens,
                                                                    max_seq_len))
         return cls(max_batch=max_batch, _runner=runner)
@@ -288,6 +293,15 @@ class Conversation:
     def _check_open(self) -> None:
         if self.slot is None:
             raise HosError("this conversation is closed")
+
+    def fork(self, n: int = 1) -> List["Conversation"]:
+        """n conversations that go on, each for itself, from where this one is: they share its keys and values until one of them
+        writes into a page that others hold (several answers to one prompt cost one prompt)."""
+        self._check_open()
+        out = [Conversation(self.engine, s) for s in self.engine.runner.fork(self.slot, n)]
+        for c in out:
+            c.position, c.pending = self.position, self.pending
+        return out
 
     def reset(self) -> None:
         """Forget everything: the next call starts at position 0 (pages go back, the slot stays)."""

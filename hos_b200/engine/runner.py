@@ -44,17 +44,28 @@ def _device() -> torch.device:
 class Runner:
     def __init__(self, config: ModelConfig, source, dtype: str = "bfloat16", max_tokens: int = 8192,
                  max_seq_len: Optional[int] = None, max_slots: Optional[int] = None,
-                 device: Optional[torch.device] = None, chunk_tokens: int = 2048):
+                 device: Optional[torch.device] = None, chunk_tokens: int = 2048,
+                 weight_bits: Optional[int] = None, cache_bits: Optional[int] = None):
         """`chunk_tokens`: the most tokens a step adds in one pass to a sequence that is under way
         (layers that keep a window of keys make their ring of pages that much longer; a step
-        that brings more is run as several passes)."""
+        that brings more is run as several passes).  `weight_bits` 4: the projections of softmax attention and the matrices of
+        gated feed-forwards are held in 4 bits; `cache_bits` 4: the keys and values are (every mixer that keeps keys must offer it)."""
         if dtype not in DTYPES:
             raise HosError(f"dtype must be one of {sorted(DTYPES)}, found {dtype!r}")
         self.config = config
         self.device = device or _device()
-        self.rt = Runtime(self.device, DTYPES[dtype])
+        for what, bits in (("weight_bits", weight_bits), ("cache_bits", cache_bits)):
+            if bits not in (None, 4):
+                raise HosError(f"{what} must be None or 4, found {bits!r}")
+        self.rt = Runtime(self.device, DTYPES[dtype], weight_bits, cache_bits)
         self.plan = plan_for(config)
         self.model = Model(self.plan, self.rt)
+        if weight_bits and not any(p.takes_weight_bits for p in self.model.all_parts()):
+            raise HosError("weight_bits: no part of this model holds its matrices in 4 bits")
+        if cache_bits:
+            needs = [m for layer in self.model.layers for m in [layer.mixer.kv_need()] if m is not None]
+            if not needs or any(m.bits != cache_bits for m in needs):
+                raise HosError("cache_bits: a mixer of this model does not keep its keys and values in 4 bits")
         tensors = load_tensors(self.model.weight_specs(), source, self.device)
         self.model.bind(tensors)
         del tensors
@@ -89,6 +100,17 @@ class Runner:
 
     def release(self, slot: int) -> None:
         self.cache.release(slot)
+
+    def fork(self, slot: int, n: int = 1) -> List[int]:
+        """n slots with sequences that go on from where this one is; pages are shared until one of them writes."""
+        return self.cache.fork(slot, n)
+
+    def resize_cache(self, max_tokens: int) -> None:
+        """A cache for max_tokens tokens that holds the live sequences as they are: held pages move to the front, the rest of the
+        memory goes back (or more is taken).  Captured steps are captured anew."""
+        torch.cuda.synchronize(self.device)          # a step under way reads the arrays that go back
+        self._sessions.clear()
+        self.cache.resize(max_tokens)
 
     def length(self, slot: int) -> int:
         return self.cache.lengths[slot]

@@ -282,6 +282,7 @@ class PagedKVArgs:
     n_kv_heads: int
     head_dim: int
     v_head_dim: int = 0          # 0: values are as wide as keys
+    bits: Optional[int] = None   # 4: uint8 [n_pages, n_kv_heads, tile4_bytes(head_dim)] tiles (csrc/fourbit.cuh)
 
     @property
     def table_stride(self) -> int:
@@ -452,6 +453,8 @@ def attn_plain(q: torch.Tensor, q_stride: int, out: torch.Tensor, token_pos, tok
     """Either (k_rows, v_rows, cu_seqlens): keys of this step's own rows, sequences
     from position 0; or (cache, seq_slot): keys from the paged cache."""
     paged = cache is not None
+    if paged and cache.bits is not None:
+        raise KernelError("attention over a cache in 4 bits goes through parts/attention4.py")
     _check(out, "attention output", q.dtype, 2)
     core().call("hos_attn_plain", dtype_code(q.dtype), int(paged), _ptr(q), q_stride,
                 _ptr(k_rows), _ptr(v_rows), kv_stride, _ptr(out), out.shape[1],
@@ -1384,3 +1387,49 @@ def channel_decay(rows: torch.Tensor, col: int, rank: int, w: torch.Tensor, b: t
         raise KernelError("channel_decay: sizes disagree")
     mixers().call("hos_channel_decay", _at(rows, col), rows.shape[1], _ptr(w), _ptr(b), int(rank), float(tau), _ptr(out), n, int(c),
                   _stream())
+
+
+# ---- 4-bit weights, 4-bit keys and values, pages (csrc/weights4.cu, attention4.cu, pages.cu) -----------------------------
+_fourbit: Optional[Library] = None
+
+
+def fourbit() -> Library:
+    global _fourbit
+    if _fourbit is None:
+        _fourbit = Library("fourbit")
+    return _fourbit
+
+
+def tile4_bytes(head_dim: int) -> int:
+    """Bytes of a page's tile of one kv head in 4 bits: 64 positions of head_dim codes, and 4 bytes for every 64 of them."""
+    return 36 * head_dim
+
+
+def _check_rows(t: torch.Tensor, what: str, dtype=None) -> None:
+    """Rows [n, width] whose numbers lie side by side, any number of numbers apart."""
+    if not t.is_cuda:
+        raise KernelError(f"{what} must be on the GPU")
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        raise KernelError(f"{what} must be rows of neighbouring numbers, found shape {tuple(t.shape)} and strides {t.stride()}")
+    if dtype is not None and t.dtype != dtype:
+        raise KernelError(f"{what} must be {dtype}, found {t.dtype}")
+
+
+def product4(x: torch.Tensor, codes: torch.Tensor, records: torch.Tensor, out: torch.Tensor, group: int, zeros: bool, gated: bool,
+             act: int = 0, limit: float = 0.0) -> None:
+    """out[M, N] = x[M, K] . W^T with W in 4 bits as parts/weights4.py lays it out; gated: W is a gate's and an up's N rows and
+    out = act(gate) * up."""
+    core4 = fourbit()
+    core4.call("hos_product4", _ptr(x), dtype_code(x.dtype), x.stride(0), _ptr(codes), _ptr(records), _ptr(out), dtype_code(out.dtype), out.stride(0),
+               x.shape[0], out.shape[1], x.shape[1], int(group), int(zeros), int(gated), int(act), float(limit), _stream())
+
+
+def copy_pages(table: torch.Tensor, most_bytes: int, src: torch.Tensor, dst: torch.Tensor, n_pages: int) -> None:
+    """Pages src[p] copied to dst[p] in every array of `table` (int64 [arrays, 2]: address, bytes of a page, on the device); a pair
+    with a page outside 0..n_pages-1 copies nothing.  No page may be written twice, or read and written, in one call."""
+    _check(table, "table of arrays", torch.int64, 2)
+    _check(src, "source pages", torch.int32, 1)
+    _check(dst, "destination pages", torch.int32, 1)
+    if src.shape != dst.shape:
+        raise KernelError(f"copy_pages: {src.shape[0]} source pages and {dst.shape[0]} destinations")
+    fourbit().call("hos_copy_pages", _ptr(table), table.shape[0], int(most_bytes), _ptr(src), _ptr(dst), src.shape[0], int(n_pages), _stream())

@@ -7,7 +7,9 @@ of the last W keys, softmax, weighted values, output projection
 Every size and constant is a parameter: width, n_heads, n_kv_heads, head_dim,
 scale, softcap (0 = off), window (None = all keys), and the position encoding
 (a PartSpec of category "position").  The mixer asks the cache for keys and
-values of [n_kv_heads, head_dim] per position, all of them or a window.
+values of [n_kv_heads, head_dim] per position, all of them or a window; with the
+runtime's `cache_bits` 4 they are held in 4 bits (parts/attention4.py), and with
+`weight_bits` 4 the projections are (parts/weights4.py).
 
 A sequence that starts at position 0 attends over its own freshly projected rows
 and only stores to the cache; a sequence that goes on (by one token or by many)
@@ -24,12 +26,14 @@ import torch
 from .. import ops
 from ..errors import KernelError, SpecError
 from ..registry import part_impl, register_part
-from . import linear
+from . import attention4, linear
 from .base import CallStore, KVNeed, Mixer, StepInfo, WeightSpec
+from .weights4 import Weight4
 
 
 class SoftmaxAttention(Mixer):
     graph_safe = True
+    takes_weight_bits = True
 
     def __init__(self, spec, rt):
         super().__init__(spec, rt)
@@ -62,12 +66,15 @@ class SoftmaxAttention(Mixer):
         q, k, v = (self._matrix(tensors[w[r]]) for r in ("q", "k", "v"))
         if not (q.dtype == k.dtype == v.dtype):
             q, k, v = q.float(), k.float(), v.float()
-        self.w_qkv = torch.cat([q, k, v], dim=0).contiguous()    # one product for q, k and v
-        self.w_q = self.w_qkv[: self.q_dim]                      # a view: rows of q alone
-        self.w_o = self._matrix(tensors[w["o"]])
+        self.w_qkv = self._product_matrix(torch.cat([q, k, v], dim=0).contiguous())    # one product for q, k and v
+        if isinstance(self.w_qkv, Weight4):
+            self.w_q = self.w_qkv.first_rows(self.q_dim) or self._product_matrix(q)
+        else:
+            self.w_q = self.w_qkv[: self.q_dim]                  # a view: rows of q alone
+        self.w_o = self._product_matrix(self._matrix(tensors[w["o"]]))
 
     def kv_need(self) -> KVNeed:
-        return KVNeed(self.n_kv_heads, self.head_dim, self.window)
+        return KVNeed(self.n_kv_heads, self.head_dim, self.window, bits=self.rt.cache_bits)
 
     def forward(self, h: torch.Tensor, step: StepInfo, store: CallStore) -> torch.Tensor:
         return self._run(h, step, store, False)
@@ -86,28 +93,34 @@ class SoftmaxAttention(Mixer):
         w = self.w_qkv if store.owns_kv else self.w_q
         n_kv = self.n_kv_heads if store.owns_kv else 0
         from . import gemm_skinny, gemm_tc
-        if not linear.plain_forced() and gemm_skinny.can_fuse_qkv_rope(h, w, self.head_dim, rotary_dim):
+        four = cache.bits == 4
+        stored = cache if store.owns_kv and not four else None      # where the rotation's kernel puts keys and values
+        fuse = not linear.plain_forced() and not isinstance(w, Weight4)
+        if fuse and gemm_skinny.can_fuse_qkv_rope(h, w, self.head_dim, rotary_dim):
             # a handful of rows: projection, rotation and cache write in one kernel
             qkv = torch.empty((n, w.shape[0]), dtype=h.dtype, device=h.device)
             gemm_skinny.qkv_rope(h, w, qkv, self.n_heads, n_kv, self.head_dim, step, inv_freq, rotary_dim, style,
-                                 cache if store.owns_kv else None)
-        elif not linear.plain_forced() and gemm_tc.can_fuse_qkv_rope(h, w, self.head_dim, rotary_dim, style, inv_freq):
+                                 stored)
+        elif fuse and gemm_tc.can_fuse_qkv_rope(h, w, self.head_dim, rotary_dim, style, inv_freq):
             # many rows: the same on the tensor cores (tiles of 256 columns hold whole heads)
             qkv = torch.empty((n, w.shape[0]), dtype=h.dtype, device=h.device)
-            gemm_tc.qkv_rope(h, w, qkv, self.n_heads, n_kv, self.head_dim, step, inv_freq,
-                             cache if store.owns_kv else None)
+            gemm_tc.qkv_rope(h, w, qkv, self.n_heads, n_kv, self.head_dim, step, inv_freq, stored)
         elif store.owns_kv:
             qkv = linear.matmul_or_partials(h, w)
             parts = None
             if qkv.dim() == 3:       # partial sums: the rotate-and-store kernel adds them
                 parts, qkv = qkv, torch.empty(qkv.shape[1:], dtype=h.dtype, device=h.device)
             ops.rope_kv_write(qkv, self.n_heads, step.token_pos, step.token_seq, step.seq_slot,
-                              step.seq_len_after, inv_freq, rotary_dim, style, cache,
+                              step.seq_len_after, inv_freq, rotary_dim, style, stored,
                               self.n_kv_heads, self.head_dim, partials=parts)
         else:
             qkv = linear.matmul(h, w)
             ops.rope_kv_write(qkv, self.n_heads, step.token_pos, step.token_seq, step.seq_slot,
                               step.seq_len_after, inv_freq, rotary_dim, style, None, 0, self.head_dim)
+        if four and store.owns_kv:
+            # the step's own rows become what the pages hold: prompts see the keys and values that later steps see
+            kv_rows = qkv[:, self.q_dim:]
+            attention4.store(kv_rows, step, cache, held=kv_rows)
         att = torch.empty((n, self.q_dim), dtype=h.dtype, device=h.device)
         if step.from_zero and store.owns_kv:
             self._attend(qkv, att, step, cache, True)          # whole prompts: over the step's own rows
@@ -127,6 +140,9 @@ class SoftmaxAttention(Mixer):
                             f"keeps a window of {self.window} keys in a ring of "
                             f"{cache.ring_pages * ops.PAGE_TOKENS}: at most {room} fit without overwriting "
                             f"keys that the step still reads")
+                if four:
+                    attention4.attend(qkv[nf:, :self.q_dim], att[nf:], rest, cache, self.n_heads, self.scale, self.softcap, self.window)
+                    return linear.matmul_or_partials(att, self.w_o) if partial_ok else linear.matmul(att, self.w_o)
                 # sequences that bring many tokens: a kernel that takes 64 queries per key tile; the few-token
                 # tail (decoding rows that share the step): the kernel that splits one query's keys over the GPU
                 nt, st = rest.tail_tokens, rest.tail_seqs

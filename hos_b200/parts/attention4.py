@@ -1,0 +1,66 @@
+"""Keys and values held in 4 bits (a cache group whose need says `bits=4`): rows put into the pages, attention over them.
+
+Per 64 neighbouring numbers of a head a scale s and a middle m in bfloat16 and codes -8..7; what is held is code * s + m
+(csrc/attention4.cu has the rounding).  Head sizes 64, 128, 192 and 256; rows in bfloat16 or in 32 bits."""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from .. import ops
+from ..errors import KernelError
+
+GROUP = 64                     # numbers of a head that share a scale
+MAX_HEAD_DIM = 256
+
+
+def supports(head_dim: int) -> bool:
+    return head_dim % GROUP == 0 and 0 < head_dim <= MAX_HEAD_DIM
+
+
+def _check_cache(cache: ops.PagedKVArgs) -> None:
+    if cache.bits != 4:
+        raise KernelError("a cache in 4 bits is wanted (KVNeed(bits=4))")
+
+
+def _check_step(n: int, step, what: str) -> None:
+    if step.n_tokens != n:
+        raise KernelError(f"{what}: {n} rows for a step of {step.n_tokens} tokens")
+
+
+def store(rows: torch.Tensor, step, cache: ops.PagedKVArgs, held: Optional[torch.Tensor] = None) -> None:
+    """Put the rows [N, 2 * n_kv_heads * head_dim] (keys, then values, rotated) into the pages at the step's places.  `held` (like
+    rows, or rows itself) receives what the pages then hold, rounded to its type: prompts attend over that, so that they see
+    the keys and values that later steps see.  Padding rows store nothing."""
+    _check_cache(cache)
+    ops._check_rows(rows, "rows of keys and values")
+    n, width = rows.shape
+    if width != 2 * cache.n_kv_heads * cache.head_dim:
+        raise KernelError(f"rows of {width} numbers for {cache.n_kv_heads} kv heads of {cache.head_dim}")
+    _check_step(n, step, "store")
+    if held is not None:
+        ops._check_rows(held, "what is held", rows.dtype)
+        if held.shape != rows.shape:
+            raise KernelError("what is held and the rows differ in size")
+    ops.fourbit().call("hos_store4", ops._ptr(rows), ops.dtype_code(rows.dtype), rows.stride(0), ops._ptr(held), held.stride(0) if held is not None else 0,
+                       ops._ptr(step.token_pos), ops._ptr(step.token_seq), ops._ptr(step.seq_slot), ops._ptr(step.seq_len_after), ops._ptr(cache.k_pages),
+                       ops._ptr(cache.v_pages), ops._ptr(cache.page_table), cache.table_stride, cache.ring_pages, cache.n_kv_heads, cache.head_dim, n,
+                       ops._stream())
+
+
+def attend(q: torch.Tensor, out: torch.Tensor, step, cache: ops.PagedKVArgs, n_heads: int, scale: float, softcap: float = 0.0,
+           window: Optional[int] = None) -> None:
+    """out[N, n_heads * head_dim] = softmax attention of the step's rows, each at its own position, over what the pages hold up to
+    and with that position (the last `window` of it).  Padding rows become zeros."""
+    _check_cache(cache)
+    ops._check_rows(q, "queries")
+    ops._check_rows(out, "attention output", q.dtype)
+    n = q.shape[0]
+    if q.shape[1] != n_heads * cache.head_dim or out.shape != q.shape:
+        raise KernelError(f"queries {tuple(q.shape)} and output {tuple(out.shape)} for {n_heads} heads of {cache.head_dim}")
+    _check_step(n, step, "attend")
+    ops.fourbit().call("hos_attend4", ops._ptr(q), ops.dtype_code(q.dtype), q.stride(0), ops._ptr(out), out.stride(0), ops._ptr(step.token_pos),
+                       ops._ptr(step.token_seq), ops._ptr(step.seq_slot), ops._ptr(cache.k_pages), ops._ptr(cache.v_pages), ops._ptr(cache.page_table),
+                       cache.table_stride, cache.ring_pages, cache.n_kv_heads, cache.head_dim, n, n_heads, float(scale), float(softcap),
+                       int(window) if window else 0, ops._stream())

@@ -49,6 +49,7 @@ class KVNeed:
     keys_only: bool = False          # True: one array per entry instead of two (a mixer whose values are a part
                                      # of what it keeps as keys, e.g. a shared latent row per position)
     v_head_dim: Optional[int] = None # values of another size than the keys (None: head_dim)
+    bits: Optional[int] = None       # None: the model's data type; 4: codes of 4 bits with a scale and a middle per 64 numbers
 
 
 @dataclass(frozen=True)
@@ -60,13 +61,17 @@ class StateNeed:
 
 
 class Runtime:
-    """Where and in what precision a model runs."""
+    """Where and in what precision a model runs.  `weight_bits` 4: the matrices of the parts that offer it (`Part.takes_weight_bits`)
+    are held in 4 bits; `cache_bits` 4: so are the keys and values of the mixers whose `KVNeed` says so."""
 
-    def __init__(self, device: torch.device, dtype: torch.dtype):
+    def __init__(self, device: torch.device, dtype: torch.dtype, weight_bits: Optional[int] = None, cache_bits: Optional[int] = None):
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"compute dtype must be float32 or bfloat16, found {dtype}")
+        if weight_bits not in (None, 4) or cache_bits not in (None, 4):
+            raise ValueError(f"weights and cache are held in the compute dtype (None) or in 4 bits, found {weight_bits} and {cache_bits}")
         self.device = torch.device(device)
         self.dtype = dtype
+        self.weight_bits, self.cache_bits = weight_bits, cache_bits
 
     @property
     def is_fp32(self) -> bool:
@@ -177,6 +182,7 @@ class Part:
     # say so are captured in a CUDA graph and replayed.  A part that loops over
     # `step.slots_host` or the like leaves it False and is run step by step.
     graph_safe = False
+    takes_weight_bits = False       # True if bind() holds its matrices as the runtime's weight_bits says
 
     def __init__(self, spec: PartSpec, rt: Runtime):
         self.spec = spec
@@ -203,6 +209,13 @@ class Part:
         if t.dtype == torch.float16:
             return t.to(torch.bfloat16).contiguous()
         return t.contiguous()
+
+    def _product_matrix(self, t: torch.Tensor, blocks: int = 1):
+        """A matrix (or `blocks` of them, row after row) for `linear.matmul`: as it is, or in 4 bits if the runtime says so."""
+        if self.rt.weight_bits is None:
+            return t
+        from .weights4 import Weight4
+        return Weight4.from_matrix(t, blocks=blocks)
 
     @staticmethod
     def _vector32(t: torch.Tensor) -> torch.Tensor:

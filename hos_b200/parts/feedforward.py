@@ -25,6 +25,7 @@ from .base import FeedForward, StepInfo, WeightSpec
 
 class GatedMLP(FeedForward):
     graph_safe = True
+    takes_weight_bits = True
     fused = True          # tests switch it off to compare the clamped form's two ways
 
     def __init__(self, spec, rt):
@@ -51,8 +52,10 @@ class GatedMLP(FeedForward):
         g, u = self._matrix(tensors[w["gate"]]), self._matrix(tensors[w["up"]])
         if g.dtype != u.dtype:
             g, u = g.float(), u.float()
-        self.w_gate_up = torch.cat([g, u], dim=0).contiguous()    # gate rows, then up rows
-        self.w_down = self._matrix(tensors[w["down"]])
+        fused = not self.clamped or (self.alpha == ops.SWISH_ALPHA and self.up_shift == ops.SWISH_SHIFT)
+        both = torch.cat([g, u], dim=0).contiguous()              # gate rows, then up rows
+        self.w_gate_up = self._product_matrix(both, blocks=2) if fused else both
+        self.w_down = self._product_matrix(self._matrix(tensors[w["down"]]))
 
     def _inner(self, h: torch.Tensor) -> torch.Tensor:
         if not self.clamped:

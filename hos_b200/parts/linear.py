@@ -10,6 +10,7 @@ from typing import Optional
 import torch
 
 from .. import ops
+from .weights4 import Weight4
 
 _force_plain = False
 
@@ -36,6 +37,8 @@ def matmul(x: torch.Tensor, w: torch.Tensor, out_dtype: Optional[torch.dtype] = 
            out: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """out[M, N] = x[M, K] . w[N or 2N, K]^T (2N rows with the gated epilogue; with its clamped activation the limit
     rides in `cap`; the bias epilogue adds `bias` ([N] float32, or None) and applies `act`, one of ops.BIAS_ACTIVATIONS)."""
+    if isinstance(w, Weight4):
+        return w.product(x, out_dtype, epilogue, cap, act, out, bias)
     m = x.shape[0]
     n = w.shape[0] // 2 if epilogue == ops.EPI_GATED else w.shape[0]
     if out is None:
@@ -58,6 +61,8 @@ def matmul_or_partials(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
     """x . w^T for a consumer that can add partial sums: either the product [M, N] in the
     activation type, or float32 partial sums [parts, M, N] when the tensor-core kernel splits K
     (few rows, few output tiles: decoding).  No epilogue."""
+    if isinstance(w, Weight4):
+        return matmul(x, w)
     if (not _force_plain and x.dtype == torch.bfloat16 and w.dtype == torch.bfloat16 and x.shape[0] > 0):
         from . import gemm_skinny, gemm_tc
         if gemm_skinny.enabled and x.shape[0] <= gemm_skinny.MAX_ROWS:

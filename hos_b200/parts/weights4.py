@@ -1,0 +1,113 @@
+"""A matrix held in 4 bits: codes 0..15, a scale (bfloat16) and, if it has them, a zero code per `group` neighbouring weights of a
+row; W[n, k] = (code - zero) * scale, zero 8 where there are none.  Products with it go through `linear.matmul` like those with any
+other matrix, with rows in bfloat16 or in 32 bits.
+
+`from_codes` takes what a quantised checkpoint holds, `from_matrix` rounds a matrix.  Both lay the codes out once, as the
+operand registers of the tensor cores want them (csrc/fourbit.cuh)."""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from .. import ops
+from ..errors import KernelError, SpecError
+
+ROWS, COLS = 16, 64             # of a block of codes
+
+
+class Weight4:
+    def __init__(self, codes: torch.Tensor, records: torch.Tensor, n: int, k: int, group: int, blocks: int, zeros: bool):
+        self.codes, self.records = codes, records
+        self.n, self.k, self.group, self.blocks, self.zeros = n, k, group, blocks, zeros
+
+    @property
+    def shape(self):
+        return torch.Size((self.blocks * self.n, self.k))
+
+    def nbytes(self) -> int:
+        return self.codes.numel() + 2 * self.records.numel()
+
+    @classmethod
+    def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor], group: int, blocks: int = 1) -> "Weight4":
+        """codes: uint8 [rows, k], 0..15; scales: [rows, ceil(k / group)], kept in bfloat16; zeros: uint8 like the scales, or None.
+        `blocks`: the rows are that many matrices one after another (2: gate and up of a gated feed-forward)."""
+        if group != 32 and (group < 64 or group % 64):
+            raise SpecError(f"groups of {group} weights: 32 or a multiple of 64 is wanted")
+        if codes.dim() != 2 or codes.dtype != torch.uint8:
+            raise SpecError(f"codes must be uint8 [rows, k], found {codes.dtype} {tuple(codes.shape)}")
+        rows, k = codes.shape
+        want = (rows, -(-k // group))
+        if k == 0 or rows == 0 or blocks < 1 or rows % blocks:
+            raise SpecError(f"{rows} x {k} codes are not {blocks} matrices")
+        if tuple(scales.shape) != want or not scales.is_floating_point():
+            raise SpecError(f"scales must be floating-point numbers {want}, found {scales.dtype} {tuple(scales.shape)}")
+        if zeros is not None and (tuple(zeros.shape) != want or zeros.dtype != torch.uint8):
+            raise SpecError(f"zero codes must be uint8 {want}, found {zeros.dtype} {tuple(zeros.shape)}")
+        if int(codes.max()) > 15 or (zeros is not None and int(zeros.max()) > 15):
+            raise SpecError("codes and zero codes must be 0..15")
+        n = rows // blocks
+        tiles, k_blocks = -(-n // ROWS), -(-k // COLS)
+        groups = -(-k_blocks * COLS // group)
+        padded = codes.new_zeros((blocks, tiles * ROWS, k_blocks * COLS))
+        padded[:, :n, :k] = codes.view(blocks, n, k)
+        # a row 8 hi + g, a number 16 t + 8 w + 2 r + h of a block: byte (g, t, hi, w, h, r / 2), nibble r % 2
+        p = padded.view(blocks * tiles, 2, 8, k_blocks, 4, 2, 4, 2).permute(0, 3, 2, 4, 1, 5, 7, 6)
+        packed = (p[..., 0::2] | (p[..., 1::2] << 4)).contiguous().view(blocks * tiles, k_blocks, 512)
+
+        def records(t):                                      # [blocks * tiles, groups, 8, 2]: rows g and g + 8 side by side
+            r = t.new_zeros((blocks, tiles * ROWS, groups), dtype=torch.bfloat16)
+            r[:, :n, :want[1]] = t.view(blocks, n, want[1]).to(torch.bfloat16)
+            return r.view(blocks * tiles, 2, 8, groups).permute(0, 3, 2, 1)
+        parts = [records(scales)]
+        if zeros is not None:
+            parts.append(records(zeros.to(torch.int32) + 128))
+        return cls(packed, torch.stack(parts, dim=3).contiguous(), n, k, group, blocks, zeros is not None)
+
+    @classmethod
+    def from_matrix(cls, w: torch.Tensor, group: int = 64, zeros: bool = False, blocks: int = 1) -> "Weight4":
+        """The matrix [rows, k] rounded: scale (max - min) / 15 and the zero code nearest to 0's place (`zeros`), or largest
+        magnitude / 7, per group; the scale is rounded to bfloat16 before the codes are taken."""
+        if w.dim() != 2 or not w.is_floating_point():
+            raise SpecError(f"a matrix is wanted, found {w.dtype} {tuple(w.shape)}")
+        rows, k = w.shape
+        g = torch.nn.functional.pad(w.float(), (0, -k % group)).view(rows, -1, group)
+        if not bool(torch.isfinite(g).all()):
+            raise SpecError("a matrix with infinities or NaN cannot be held in 4 bits")
+        if zeros:
+            lo, hi = g.amin(-1).clamp(max=0), g.amax(-1).clamp(min=0)
+            s = ((hi - lo) / 15).to(torch.bfloat16)
+            z = torch.round(-lo / torch.where(s > 0, s.float(), 1.0)).clamp(0, 15)
+        else:
+            s = (g.abs().amax(-1) / 7).to(torch.bfloat16)
+            z = torch.full_like(s, 8.0, dtype=torch.float32)
+        inner = g / torch.where(s > 0, s.float(), 1.0)[..., None] + z[..., None]
+        codes = torch.round(inner).clamp_(0, 15).to(torch.uint8).view(rows, -1)[:, :k].contiguous()
+        return cls.from_codes(codes, s, z.to(torch.uint8) if zeros else None, group, blocks)
+
+    def first_rows(self, n: int) -> Optional["Weight4"]:
+        """The first n rows (a view), or None where n cuts a block."""
+        if self.blocks != 1 or n % ROWS or n > self.n:
+            return None
+        return Weight4(self.codes[:n // ROWS], self.records[:n // ROWS], n, self.k, self.group, 1, self.zeros)
+
+    def product(self, x: torch.Tensor, out_dtype: Optional[torch.dtype] = None, epilogue: int = ops.EPI_NONE, cap: float = 0.0, act: int = 0,
+                out: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """x . W^T as `linear.matmul` describes it; epilogues: none, gated."""
+        gated = epilogue == ops.EPI_GATED
+        if epilogue not in (ops.EPI_NONE, ops.EPI_GATED) or bias is not None:
+            raise KernelError("products with 4-bit weights have no epilogue but the gated one")
+        if gated != (self.blocks == 2):
+            raise KernelError(f"a {'gated' if gated else 'plain'} product is asked of {self.blocks} matrices")
+        ops._check_rows(x, "left operand")
+        if x.shape[1] != self.k:
+            raise KernelError(f"product with 4-bit weights: rows of {x.shape[1]} numbers, weights of {self.k}")
+        if out is None:
+            out = torch.empty((x.shape[0], self.n), dtype=out_dtype or x.dtype, device=x.device)
+        else:
+            ops._check_rows(out, "product")
+            if tuple(out.shape) != (x.shape[0], self.n):
+                raise KernelError(f"product with 4-bit weights: the output is {tuple(out.shape)}, not {(x.shape[0], self.n)}")
+        if x.shape[0]:
+            ops.product4(x, self.codes, self.records, out, self.group, self.zeros, gated, act, cap)
+        return out
