@@ -2,13 +2,15 @@
 //
 // A block is 16 rows x 64 numbers in 512 bytes, 16 to a lane of the warp that multiplies it: with g = lane / 4 and
 // t = lane % 4 the MMA wants of its 16 x 16 operand the rows g and g + 8 and four columns a lane, and since a dot product does not
-// care in which order its terms come, the four MMA steps of a block take the lane's 16 neighbouring numbers of a row four by four
+// care in which order its terms come, the four MMA steps of a block take a lane's 16 numbers of a row four by four
 // (the other operand is read in the same order).  A 32-bit word holds eight codes; shifted right by 4 r its low nibbles of the two
 // halves are the two codes of the operand's register r, so that a register costs a shift and one logical instruction, which also
 // sets the bits that make 128 + c of a code c in bfloat16, and one subtraction, exact, that takes the 128 and the zero code away.
 //
-// Rows of numbers (weights: features x k; keys: positions x numbers of a head), "by row": word ((row / 8) % 2) * 2 + (d / 8) % 2 of
-// lane (row % 8) * 4 + d / 16, code d % 8 of the word.  A token's eight neighbouring numbers are one word of its own.
+// Keys (positions x numbers of a head), "by row": word ((row / 8) % 2) * 2 + (d / 8) % 2 of lane (row % 8) * 4 + d / 16, code d % 8
+// of the word.  A token's eight neighbouring numbers are one word of its own.
+// Weights (features x k) the same with d / 32 in the place of (d / 8) % 2 and (d / 8) % 4 in that of d / 16: a word's step lies in
+// one group of 32.
 // Values, which the MMA takes transposed (numbers of a head x positions), "by column": word d / 16 of lane (d % 8) * 4 +
 // (row % 8) / 2, byte (row % 2) * 2 + row / 8, the low nibble where (d / 8) % 2 is 0.  A byte belongs to one token.
 #pragma once

@@ -51,8 +51,8 @@ class Weight4:
         groups = -(-k_blocks * COLS // group)
         padded = codes.new_zeros((blocks, tiles * ROWS, k_blocks * COLS))
         padded[:, :n, :k] = codes.view(blocks, n, k)
-        # a row 8 hi + g, a number 16 t + 8 w + 2 r + h of a block: byte (g, t, hi, w, h, r / 2), nibble r % 2
-        p = padded.view(blocks * tiles, 2, 8, k_blocks, 4, 2, 4, 2).permute(0, 3, 2, 4, 1, 5, 7, 6)
+        # a row 8 hi + g, a number 32 w + 8 t + 2 r + h of a block: byte (g, t, hi, w, h, r / 2), nibble r % 2
+        p = padded.view(blocks * tiles, 2, 8, k_blocks, 2, 4, 4, 2).permute(0, 3, 2, 5, 1, 4, 7, 6)
         packed = (p[..., 0::2] | (p[..., 1::2] << 4)).contiguous().view(blocks * tiles, k_blocks, 512)
 
         def records(t):                                      # [blocks * tiles, groups, 8, 2]: rows g and g + 8 side by side
