@@ -37,12 +37,17 @@ __host__ __device__ __forceinline__ int by_column_byte(int row, int d) {
 __host__ __device__ __forceinline__ int tile4_codes(int dim) { return 32 * dim; }
 __host__ __device__ __forceinline__ int tile4_bytes(int dim) { return 36 * dim; }
 
-// The four operand registers of a word: codes minus `zero` ((128 + zero) twice in bfloat16), exact.
+// The four operand registers of a word: 128 + code, or (SUBTRACT) the codes minus `zero` ((128 + zero) twice in bfloat16), exact.
+template <bool SUBTRACT = true>
 __device__ __forceinline__ void codes_to_bf16(uint32_t w, uint32_t zero, uint32_t (&r)[4]) {
     const __nv_bfloat162 z = *reinterpret_cast<const __nv_bfloat162*>(&zero);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const uint32_t v = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+        if (!SUBTRACT) {
+            r[i] = v;
+            continue;
+        }
         const __nv_bfloat162 c = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), z);
         r[i] = *reinterpret_cast<const uint32_t*>(&c);
     }

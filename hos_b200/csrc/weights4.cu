@@ -16,6 +16,9 @@
 
 namespace hos {
 
+struct TrueTag4 { static constexpr bool value = true; };
+struct FalseTag4 { static constexpr bool value = false; };
+
 __device__ __forceinline__ float gate_times(int act, float gate, float up, float limit, bool fast) {
     if (fast) return act == 2 ? clamped_swish_fast(gate, up, limit) : (act == 0 ? gelu_tanh_fast(gate) : silu_fast(gate)) * up;
     if (act == 2) return clamped_swish(gate, up, limit);
@@ -23,9 +26,11 @@ __device__ __forceinline__ float gate_times(int act, float gate, float up, float
 }
 
 // A lane's 16 numbers of a row of x, 8 from p on and 8 from p + 32 on, as operand registers: pair j holds the numbers 2 j and 2 j + 1.
+// `left`: how many numbers the row still has from p on; WHOLE: 16-byte pieces may be read, K is made of them and p begins on one.
 struct Row16 { uint32_t v[8]; };
-__device__ __forceinline__ void load_row(Row16 (&r)[1], const bf16* p, int left, bool vec) {
-    if (vec) {                                   // whole 16-byte pieces: K is a multiple of 8 and the rows begin on 16 bytes
+template <bool WHOLE>
+__device__ __forceinline__ void load_row(Row16 (&r)[1], const bf16* p, int left) {
+    if (WHOLE) {
         const uint4 zero = make_uint4(0, 0, 0, 0);
         const uint4 a = left > 0 ? __ldg((const uint4*)p) : zero, b = left > 32 ? __ldg((const uint4*)(p + 32)) : zero;
         r[0] = Row16{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
@@ -38,9 +43,10 @@ __device__ __forceinline__ void load_row(Row16 (&r)[1], const bf16* p, int left,
         r[0].v[j] = (at < left ? (uint32_t)__ldg(u + at) : 0u) | (at + 1 < left ? (uint32_t)__ldg(u + at + 1) << 16 : 0u);
     }
 }
-__device__ __forceinline__ void load_row(Row16 (&r)[3], const float* p, int left, bool vec) {
+template <bool WHOLE>
+__device__ __forceinline__ void load_row(Row16 (&r)[3], const float* p, int left) {
     float f[16];
-    if (vec) {
+    if (WHOLE) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int at = 4 * i + (i < 2 ? 0 : 24);
@@ -67,40 +73,62 @@ __device__ __forceinline__ void load_row(Row16 (&r)[3], const float* p, int left
     }
 }
 
-// MT: tiles of 8 rows of x; T: tiles of 16 features a warp (2: gated); SUB: scales a block of 64 (2: groups of 32).
-template <typename XT, typename OutT, int MT, int T, int SUB, bool ZEROS, int WARPS>
+// MT: tiles of 8 rows of x; T: tiles of 16 features a warp (the first half of them gate's, the other up's, if GATED); SUB: scales a
+// block of 64 (2: groups of 32); ring_of: blocks of T tiles that a warp's ring holds.
+template <int T> struct ring_of { static constexpr int value = T == 1 ? 8 : (T == 2 ? 6 : 4); };
+template <typename XT, int MT, int T, bool GATED, int SUB, bool ZEROS, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS)
-product4_kernel(const XT* __restrict__ x, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ records, OutT* __restrict__ out, int M, int N,
-                int K, long long ldx, long long ldo, int group, int act, float limit, int vec) {
+product4_kernel(const XT* __restrict__ x, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ records, void* __restrict__ out, int out_f32,
+                int M, int N, int K, long long ldx, long long ldo, int group_blocks, int act, float limit, int whole) {
     constexpr int kTerms = sizeof(XT) == 4 ? 3 : 1;
-    constexpr int kRing = T == 1 ? 8 : 5;
+    // For rows in bfloat16 the codes go in as 128 + c and (128 + z) sum x, which a product with ones gives for all of the warp's tiles
+    // at once, is where the sums start: a quarter of the instructions that form the operands.  The sums lose 2^-24 of 136 sum |x|, far
+    // below the rounding of the result; 32-bit rows subtract first.
+    constexpr bool kLate = kTerms == 1;
+    constexpr int kRing = ring_of<T>::value;
     constexpr int kRecord = ZEROS ? 64 : 32;                       // bytes of a tile's records of a group
     constexpr int kTile = kBlockBytes + SUB * kRecord, kStage = T * kTile;
     constexpr int kSums = T * MT * 16 * 9;
+    constexpr int kWide = GATED ? T / 2 : T;                       // tiles of features of the result
     extern __shared__ __align__(16) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-    const int tiles = (N + 15) / 16, k_blocks = (K + 63) / 64, groups = (k_blocks * 64 + group - 1) / group;
+    const int tiles = (N + 15) / 16, k_blocks = (K + 63) / 64;
+    const int groups = SUB == 2 ? 2 * k_blocks : (k_blocks + group_blocks - 1) / group_blocks;
     const int per_way = (k_blocks + WARPS - 1) / WARPS, kb0 = min(k_blocks, warp * per_way), kb1 = min(k_blocks, kb0 + per_way);
     const int m0 = blockIdx.y * 8 * MT;
     uint8_t* ring = smem + warp * kRing * kStage;
     const uint32_t ring_at = smem_u32(ring);
 
-    auto fetch = [&](int kb) {
-        if (kb < kb1) {
-            const uint32_t to = ring_at + (kb - kb0) % kRing * kStage;
+    // where the next block to be fetched is; a tile beyond the last reads the last one, and its sums are dropped
+    const uint8_t *code_at[T], *record_at[T];
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+        const size_t tile = (size_t)(t / kWide) * tiles + min((int)blockIdx.x * kWide + t % kWide, tiles - 1);
+        code_at[t] = codes + (tile * k_blocks + kb0) * kBlockBytes + lane * 16;
+        record_at[t] = records + (tile * groups + (SUB == 2 ? 2 * kb0 : kb0 / group_blocks)) * kRecord + lane * 16;
+    }
+    int to_fetch = kb1 - kb0, in_group = SUB == 2 ? 1 : group_blocks - kb0 % group_blocks;
+    auto fetch = [&](uint32_t to) {
+        if (to_fetch > 0) {
+            const bool has_record = lane < SUB * kRecord / 16;
 #pragma unroll
             for (int t = 0; t < T; ++t) {
-                const size_t tile = (size_t)t * tiles + blockIdx.x;
-                copy16_async(to + t * kTile + lane * 16, codes + (tile * k_blocks + kb) * kBlockBytes + lane * 16);
-                if (lane < SUB * kRecord / 16)
-                    copy16_async(to + t * kTile + kBlockBytes + lane * 16, records + (tile * groups + (SUB == 2 ? 2 * kb : kb * 64 / group)) * kRecord + lane * 16);
+                copy16_async(to + t * kTile + lane * 16, code_at[t]);
+                if (has_record) copy16_async(to + t * kTile + kBlockBytes + lane * 16, record_at[t]);
+                code_at[t] += kBlockBytes;
+            }
+            if (--in_group == 0) {
+                in_group = SUB == 2 ? 1 : group_blocks;
+#pragma unroll
+                for (int t = 0; t < T; ++t) record_at[t] += SUB * kRecord;
             }
         }
+        --to_fetch;
         copies_commit();
     };
     // W is nothing that a kernel before this one writes
 #pragma unroll
-    for (int i = 0; i < kRing - 1; ++i) fetch(kb0 + i);
+    for (int i = 0; i < kRing - 1; ++i) fetch(ring_at + i * kStage);
     pdl_wait();
     pdl_launch_dependents();
 
@@ -111,77 +139,118 @@ product4_kernel(const XT* __restrict__ x, const uint8_t* __restrict__ codes, con
         for (int m = 0; m < MT; ++m) acc[t][m][0] = acc[t][m][1] = acc[t][m][2] = acc[t][m][3] = 0.f;
     const XT* row[MT];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) row[m] = x + (size_t)min(m0 + 8 * m + g, M - 1) * ldx + 8 * t4;
+    for (int m = 0; m < MT; ++m) row[m] = x + (size_t)min(m0 + 8 * m + g, M - 1) * ldx + 8 * t4 + (size_t)kb0 * 64;   // rows beyond M: sums dropped
+    int left = K - kb0 * 64 - 8 * t4;
 
-    auto rows_of = [&](int kb, int m, Row16 (&r)[kTerms]) {
-        const int left = m0 + 8 * m + g < M ? K - (kb * 64 + 8 * t4) : 0;
-        load_row(r, row[m] + kb * 64, left, vec != 0);
-    };
-    Row16 next[kTerms];
-    if (MT == 1 && kb0 < kb1) rows_of(kb0, 0, next);
-    for (int kb = kb0; kb < kb1; ++kb) {
-        copies_wait<kRing - 2>();
-        __syncwarp();
-        const uint32_t at = ring_at + (kb - kb0) % kRing * kStage;
-        uint32_t a[T][4][4];
-        float s[T][SUB][2];
+    auto walk = [&](auto whole_tag) {
+        constexpr bool kWhole = decltype(whole_tag)::value;
+        int slot = 0, before = (kRing - 1) * kStage;                // this block's place in the ring, and the one before it
+        Row16 next[kTerms];
+        if (MT == 1 && kb0 < kb1) load_row<kWhole>(next, row[0], left);
+        for (int n = kb1 - kb0; n > 0; --n) {
+            copies_wait<kRing - 2>();
+            __syncwarp();
+            fetch(ring_at + before);                                // the place that the last block has left
+            // the rows of a tile of 8 with the sums of x over a group, columns 2 t and 2 t + 1 (kLate), where the products start
+            auto rows_of = [&](int m, Row16 (&r)[kTerms], float (&start)[SUB][2]) {
+                if (MT == 1) {
 #pragma unroll
-        for (int t = 0; t < T; ++t) {
-            const uint4 w = lds16(at + t * kTile + lane * 16);
-            uint32_t lo[4], hi[4];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {                          // two MMA steps to a word
-                uint32_t z0 = kZero8, z1 = kZero8;
-                const uint8_t* rec = ring + (kb - kb0) % kRing * kStage + t * kTile + kBlockBytes + (SUB == 2 ? h : 0) * kRecord + g * (kRecord / 8);
-                if (h < SUB) {
-                    const uint32_t two = *(const uint32_t*)rec;
-                    s[t][h][0] = bf16_lo(two);
-                    s[t][h][1] = bf16_hi(two);
+                    for (int i = 0; i < kTerms; ++i) r[i] = next[i];
+                    if (n > 1) load_row<kWhole>(next, row[0] + 64, left - 64);
+                } else {
+                    load_row<kWhole>(r, row[m], left);
                 }
-                if (ZEROS) {
-                    const uint32_t two = *(const uint32_t*)(rec + 4);
-                    z0 = __byte_perm(two, 0, 0x1010);
-                    z1 = __byte_perm(two, 0, 0x3232);
+                row[m] += 64;
+                if (kLate) {
+                    const uint32_t ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+#pragma unroll
+                    for (int sub = 0; sub < SUB; ++sub) {
+                        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int st = 4 / SUB * sub; st < 4 / SUB * (sub + 1); ++st) mma_bf16(sum, ones, r[0].v[2 * st], r[0].v[2 * st + 1]);
+                        start[sub][0] = ZEROS ? sum[0] : -136.f * sum[0];
+                        start[sub][1] = ZEROS ? sum[1] : -136.f * sum[1];
+                    }
                 }
-                codes_to_bf16(h == 0 ? w.x : w.y, z0, lo);
-                codes_to_bf16(h == 0 ? w.z : w.w, z1, hi);
+            };
+            struct Tile { uint32_t a[4][4]; float s[SUB][2], z[SUB][2]; };
+            auto operands_of = [&](int t, Tile& f) {
+                const uint4 w = lds16(ring_at + slot + t * kTile + lane * 16);
+                const uint8_t* rec = ring + slot + t * kTile + kBlockBytes + g * (kRecord / 8);
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    a[t][2 * h + e][0] = lo[2 * e];
-                    a[t][2 * h + e][1] = hi[2 * e];
-                    a[t][2 * h + e][2] = lo[2 * e + 1];
-                    a[t][2 * h + e][3] = hi[2 * e + 1];
+                for (int h = 0; h < 2; ++h) {                       // two MMA steps to a word
+                    const int sub = SUB == 2 ? h : 0;
+                    uint32_t z0 = kZero8, z1 = kZero8;
+                    if (h < SUB) {
+                        const uint32_t two = *(const uint32_t*)(rec + sub * kRecord);
+                        f.s[sub][0] = bf16_lo(two);
+                        f.s[sub][1] = bf16_hi(two);
+                    }
+                    if (ZEROS) {
+                        const uint32_t two = *(const uint32_t*)(rec + sub * kRecord + 4);
+                        z0 = __byte_perm(two, 0, 0x1010);
+                        z1 = __byte_perm(two, 0, 0x3232);
+                        f.z[sub][0] = -bf16_lo(two);
+                        f.z[sub][1] = -bf16_hi(two);
+                    }
+                    uint32_t lo[4], hi[4];
+                    codes_to_bf16<!kLate>(h == 0 ? w.x : w.y, z0, lo);
+                    codes_to_bf16<!kLate>(h == 0 ? w.z : w.w, z1, hi);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        f.a[2 * h + e][0] = lo[2 * e];
+                        f.a[2 * h + e][1] = hi[2 * e];
+                        f.a[2 * h + e][2] = lo[2 * e + 1];
+                        f.a[2 * h + e][3] = hi[2 * e + 1];
+                    }
                 }
-            }
-        }
-        fetch(kb + kRing - 1);
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            Row16 r[kTerms];
-            if (MT == 1) {
-#pragma unroll
-                for (int i = 0; i < kTerms; ++i) r[i] = next[i];
-                if (kb + 1 < kb1) rows_of(kb + 1, 0, next);
-            } else {
-                rows_of(kb, m, r);
-            }
-#pragma unroll
-            for (int t = 0; t < T; ++t) {
+            };
+            auto multiply = [&](int t, int m, const Tile& f, const Row16 (&r)[kTerms], const float (&start)[SUB][2]) {
 #pragma unroll
                 for (int sub = 0; sub < SUB; ++sub) {
                     float part[4] = {0.f, 0.f, 0.f, 0.f};
+                    if (kLate) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) part[c] = ZEROS ? f.z[sub][c >> 1] * start[sub][c & 1] : start[sub][c & 1];
+                    }
 #pragma unroll
                     for (int i = kTerms - 1; i >= 0; --i)           // the small terms first
 #pragma unroll
-                        for (int st = 4 / SUB * sub; st < 4 / SUB * (sub + 1); ++st) mma_bf16(part, a[t][st], r[i].v[2 * st], r[i].v[2 * st + 1]);
-                    acc[t][m][0] = fmaf(s[t][sub][0], part[0], acc[t][m][0]);
-                    acc[t][m][1] = fmaf(s[t][sub][0], part[1], acc[t][m][1]);
-                    acc[t][m][2] = fmaf(s[t][sub][1], part[2], acc[t][m][2]);
-                    acc[t][m][3] = fmaf(s[t][sub][1], part[3], acc[t][m][3]);
+                        for (int st = 4 / SUB * sub; st < 4 / SUB * (sub + 1); ++st) mma_bf16(part, f.a[st], r[i].v[2 * st], r[i].v[2 * st + 1]);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) acc[t][m][c] = fmaf(f.s[sub][c >> 1], part[c], acc[t][m][c]);
+                }
+            };
+            if (MT == 1) {                                          // the rows stay while the tiles go by
+                Row16 r[kTerms];
+                float start[SUB][2];
+                rows_of(0, r, start);
+#pragma unroll
+                for (int t = 0; t < T; ++t) {
+                    Tile f;
+                    operands_of(t, f);
+                    multiply(t, 0, f, r, start);
+                }
+            } else {                                                // and the other way round
+                Tile f[T];
+#pragma unroll
+                for (int t = 0; t < T; ++t) operands_of(t, f[t]);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    Row16 r[kTerms];
+                    float start[SUB][2];
+                    rows_of(m, r, start);
+#pragma unroll
+                    for (int t = 0; t < T; ++t) multiply(t, m, f[t], r, start);
                 }
             }
+            left -= 64;
+            before = slot;
+            slot = slot == (kRing - 1) * kStage ? 0 : slot + kStage;
         }
-    }
+    };
+    if (whole) walk(TrueTag4{});
+    else walk(FalseTag4{});
     copies_wait<0>();
     __syncthreads();                             // the rings are done with: the sums go where they were
     float* sums = (float*)smem;
@@ -196,27 +265,29 @@ product4_kernel(const XT* __restrict__ x, const uint8_t* __restrict__ codes, con
             p[(g + 8) * 9 + 2 * t4 + 1] = acc[t][m][3];
         }
     __syncthreads();
-    for (int i = threadIdx.x; i < MT * 8 * 16; i += WARPS * 32) {
-        const int tok = i / 16, r = i % 16, n = blockIdx.x * 16 + r;      // consecutive threads: consecutive features
+    for (int i = threadIdx.x; i < MT * 8 * 16 * kWide; i += WARPS * 32) {
+        const int tok = i / (16 * kWide), r = i % (16 * kWide), n = blockIdx.x * 16 * kWide + r;      // consecutive threads: consecutive features
         if (m0 + tok >= M || n >= N) continue;
-        float v[T];
+        float v[GATED ? 2 : 1];
 #pragma unroll
-        for (int t = 0; t < T; ++t) {
-            v[t] = 0.f;
+        for (int h = 0; h < (GATED ? 2 : 1); ++h) {
+            v[h] = 0.f;
 #pragma unroll
-            for (int w = 0; w < WARPS; ++w) v[t] += sums[w * kSums + (t * MT + tok / 8) * 144 + r * 9 + tok % 8];
+            for (int w = 0; w < WARPS; ++w) v[h] += sums[w * kSums + ((h * kWide + r / 16) * MT + tok / 8) * 144 + (r & 15) * 9 + tok % 8];
         }
-        out[(size_t)(m0 + tok) * ldo + n] = from_float<OutT>(T == 2 ? gate_times(act, v[0], v[T - 1], limit, kTerms == 1) : v[0]);
+        const float y = GATED ? gate_times(act, v[0], v[GATED ? 1 : 0], limit, kTerms == 1) : v[0];
+        const size_t at = (size_t)(m0 + tok) * ldo + n;
+        if (kTerms == 3 || out_f32) ((float*)out)[at] = y;
+        else ((bf16*)out)[at] = __float2bfloat16_rn(y);
     }
 }
 
-template <typename XT, typename OutT, int MT, int T, int SUB, bool ZEROS, int WARPS>
-int launch_product4(const void* x, const void* codes, const void* records, void* out, int M, int N, int K, long long ldx, long long ldo, int group,
-                    int act, float limit, int vec, cudaStream_t stream) {
-    constexpr int ring = T == 1 ? 8 : 5, stage = T * (kBlockBytes + SUB * (ZEROS ? 64 : 32));
-    constexpr int sums = T * MT * 144 * 4;
-    constexpr int smem = WARPS * (ring * stage > sums ? ring * stage : sums);
-    auto kernel = product4_kernel<XT, OutT, MT, T, SUB, ZEROS, WARPS>;
+template <typename XT, int MT, int T, bool GATED, int SUB, bool ZEROS, int WARPS>
+int launch_product4(const void* x, const void* codes, const void* records, void* out, int out_f32, int M, int N, int K, long long ldx, long long ldo, int group,
+                    int act, float limit, int whole, cudaStream_t stream) {
+    constexpr int ring = ring_of<T>::value * T * (kBlockBytes + SUB * (ZEROS ? 64 : 32)), sums = T * MT * 144 * 4;
+    constexpr int smem = WARPS * (ring > sums ? ring : sums), wide = 16 * (GATED ? T / 2 : T);
+    auto kernel = product4_kernel<XT, MT, T, GATED, SUB, ZEROS, WARPS>;
     if (smem > 48 * 1024) {
         static bool set = false;                 // once per kernel: the attribute stays
         if (!set) {
@@ -224,8 +295,8 @@ int launch_product4(const void* x, const void* codes, const void* records, void*
             set = true;
         }
     }
-    launch_pdl(kernel, dim3((unsigned)((N + 15) / 16), (unsigned)((M + 8 * MT - 1) / (8 * MT))), dim3(WARPS * 32), smem, stream, (const XT*)x,
-               (const uint8_t*)codes, (const uint8_t*)records, (OutT*)out, M, N, K, ldx, ldo, group, act, limit, vec);
+    launch_pdl(kernel, dim3((unsigned)((N + wide - 1) / wide), (unsigned)((M + 8 * MT - 1) / (8 * MT))), dim3(WARPS * 32), smem, stream, (const XT*)x,
+               (const uint8_t*)codes, (const uint8_t*)records, out, out_f32, M, N, K, ldx, ldo, group / 64, act, limit, whole);
     return check_launch("product4");
 }
 
@@ -244,17 +315,17 @@ extern "C" int hos_product4(const void* x, int x_dtype, long long ldx, const voi
     if (M > 65535 * 8) HOS_REFUSE("product4: %d rows", M);
     if (x_dtype == kF32 ? out_dtype != kF32 : x_dtype != kBF16 || (out_dtype != kF32 && out_dtype != kBF16))
         HOS_REFUSE("product4: no product of type %d into type %d", x_dtype, out_dtype);
-    const int piece = x_dtype == kF32 ? 4 : 8, vec = K % piece == 0 && ldx % piece == 0 && (uintptr_t)x % 16 == 0;
-    const int sm = sm_count_cached(), ctas = (N + 15) / 16;
-    // the warps that share a CTA's K: as few as fill the SMs with 16 warps each
-    const int ways = ctas >= 4 * sm ? 4 : (ctas >= 2 * sm ? 8 : 16);
-#define HOS_P4(X, O, MT, T, SUB, Z, W) return launch_product4<X, O, MT, T, SUB, Z, W>(x, codes, records, out, M, N, K, ldx, ldo, group, act, limit, vec, stream)
-#define HOS_P4_W(X, O, MT, T, SUB, Z) do { if (ways == 4) HOS_P4(X, O, MT, T, SUB, Z, 4); else if (ways == 8) HOS_P4(X, O, MT, T, SUB, Z, 8); else HOS_P4(X, O, MT, T, SUB, Z, 16); } while (0)
-#define HOS_P4_M(X, O, T, SUB, Z) do { if (M <= 8) HOS_P4_W(X, O, 1, T, SUB, Z); else if (M <= 16) HOS_P4_W(X, O, 2, T, SUB, Z); else HOS_P4_W(X, O, 4, T, SUB, Z); } while (0)
-#define HOS_P4_S(X, O, T, Z) do { if (group == 32) HOS_P4_M(X, O, T, 2, Z); else HOS_P4_M(X, O, T, 1, Z); } while (0)
-#define HOS_P4_G(X, O, Z) do { if (gated) HOS_P4_S(X, O, 2, Z); else HOS_P4_S(X, O, 1, Z); } while (0)
-#define HOS_P4_Z(X, O) do { if (zeros) HOS_P4_G(X, O, true); else HOS_P4_G(X, O, false); } while (0)
-    if (x_dtype == kF32) HOS_P4_Z(float, float);
-    else if (out_dtype == kBF16) HOS_P4_Z(bf16, bf16);
-    else HOS_P4_Z(bf16, float);
+    const int piece = x_dtype == kF32 ? 4 : 8, whole = K % piece == 0 && ldx % piece == 0 && (uintptr_t)x % 16 == 0;
+    // 16 features to a CTA and 16 warps that share K where that makes few CTAs; more features to a warp (they share its rows of x) and
+    // fewer warps to a CTA where there are enough to fill the SMs with 16 warps each
+    const int sm = sm_count_cached(), tiles = (N + 15) / 16;
+    const int shape = tiles >= 8 * sm ? 2 : (tiles >= 2 * sm ? 1 : 0);
+#define HOS_P4(X, MT, T, G, SUB, Z, W) return launch_product4<X, MT, T, G, SUB, Z, W>(x, codes, records, out, out_dtype == kF32, M, N, K, ldx, ldo, group, act, limit, whole, stream)
+#define HOS_P4_W(X, MT, G, SUB, Z) do { if (shape == 2) HOS_P4(X, MT, ((G ? 2 : 1) * (MT == 1 ? 2 : 1)), G, SUB, Z, 4); else if (shape == 1) HOS_P4(X, MT, (G ? 2 : 1), G, SUB, Z, 8); else HOS_P4(X, MT, (G ? 2 : 1), G, SUB, Z, 16); } while (0)
+#define HOS_P4_M(X, G, SUB, Z) do { if (M <= 8) HOS_P4_W(X, 1, G, SUB, Z); else if (M <= 16) HOS_P4_W(X, 2, G, SUB, Z); else HOS_P4_W(X, 4, G, SUB, Z); } while (0)
+#define HOS_P4_S(X, G, Z) do { if (group == 32) HOS_P4_M(X, G, 2, Z); else HOS_P4_M(X, G, 1, Z); } while (0)
+#define HOS_P4_G(X, Z) do { if (gated) HOS_P4_S(X, true, Z); else HOS_P4_S(X, false, Z); } while (0)
+#define HOS_P4_Z(X) do { if (zeros) HOS_P4_G(X, true); else HOS_P4_G(X, false); } while (0)
+    if (x_dtype == kF32) HOS_P4_Z(float);
+    else HOS_P4_Z(bf16);
 }
