@@ -43,7 +43,8 @@ __device__ __forceinline__ void codes_to_bf16(uint32_t w, uint32_t zero, uint32_
     const __nv_bfloat162 z = *reinterpret_cast<const __nv_bfloat162*>(&zero);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const uint32_t v = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+        uint32_t v;                                            // (w >> 4 i) & mask | bits in one instruction
+        asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(w >> (4 * i)), "r"(0x000f000fu), "r"(0x43004300u));
         if (!SUBTRACT) {
             r[i] = v;
             continue;

@@ -25,14 +25,21 @@ __device__ __forceinline__ float gate_times(int act, float gate, float up, float
     return (act == 0 ? gelu_tanh(gate) : gate / (1.f + expf(-gate))) * up;
 }
 
+// d = a . b + c: not volatile and with sums of its own to start from, so that the products of several tiles may be woven into one
+// another.
+__device__ __forceinline__ void mma_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+
 // A lane's 16 numbers of a row of x, 8 from p on and 8 from p + 32 on, as operand registers: pair j holds the numbers 2 j and 2 j + 1.
-// `left`: how many numbers the row still has from p on; WHOLE: 16-byte pieces may be read, K is made of them and p begins on one.
+// WHOLE: all of them are there and 16-byte pieces may be read; else `left` says how many numbers the row still has from p on.
 struct Row16 { uint32_t v[8]; };
 template <bool WHOLE>
 __device__ __forceinline__ void load_row(Row16 (&r)[1], const bf16* p, int left) {
     if (WHOLE) {
-        const uint4 zero = make_uint4(0, 0, 0, 0);
-        const uint4 a = left > 0 ? __ldg((const uint4*)p) : zero, b = left > 32 ? __ldg((const uint4*)(p + 32)) : zero;
+        const uint4 a = __ldg((const uint4*)p), b = __ldg((const uint4*)(p + 32));
         r[0] = Row16{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
         return;
     }
@@ -50,7 +57,7 @@ __device__ __forceinline__ void load_row(Row16 (&r)[3], const float* p, int left
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int at = 4 * i + (i < 2 ? 0 : 24);
-            const float4 a = left > at ? __ldg((const float4*)(p + at)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            const float4 a = __ldg((const float4*)(p + at));
             f[4 * i] = a.x; f[4 * i + 1] = a.y; f[4 * i + 2] = a.z; f[4 * i + 3] = a.w;
         }
     } else {
@@ -142,115 +149,131 @@ product4_kernel(const XT* __restrict__ x, const uint8_t* __restrict__ codes, con
     for (int m = 0; m < MT; ++m) row[m] = x + (size_t)min(m0 + 8 * m + g, M - 1) * ldx + 8 * t4 + (size_t)kb0 * 64;   // rows beyond M: sums dropped
     int left = K - kb0 * 64 - 8 * t4;
 
-    auto walk = [&](auto whole_tag) {
+    // One block: WHOLE as load_row's, AHEAD: the next block's rows may be asked for whole.
+    Row16 next[kTerms];
+    auto block = [&](uint32_t slot, auto whole_tag, int ahead) {
         constexpr bool kWhole = decltype(whole_tag)::value;
-        int slot = 0, before = (kRing - 1) * kStage;                // this block's place in the ring, and the one before it
-        Row16 next[kTerms];
-        if (MT == 1 && kb0 < kb1) load_row<kWhole>(next, row[0], left);
-        for (int n = kb1 - kb0; n > 0; --n) {
-            copies_wait<kRing - 2>();
-            __syncwarp();
-            fetch(ring_at + before);                                // the place that the last block has left
-            // the rows of a tile of 8 with the sums of x over a group, columns 2 t and 2 t + 1 (kLate), where the products start
-            auto rows_of = [&](int m, Row16 (&r)[kTerms], float (&start)[SUB][2]) {
-                if (MT == 1) {
+        // the rows of a tile of 8 with the sums of x over a group, columns 2 t and 2 t + 1 (kLate), where the products start
+        auto rows_of = [&](int m, Row16 (&r)[kTerms], float (&start)[SUB][2]) {
+            if (MT == 1) {
 #pragma unroll
-                    for (int i = 0; i < kTerms; ++i) r[i] = next[i];
-                    if (n > 1) load_row<kWhole>(next, row[0] + 64, left - 64);
-                } else {
-                    load_row<kWhole>(r, row[m], left);
-                }
-                row[m] += 64;
-                if (kLate) {
-                    const uint32_t ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
-#pragma unroll
-                    for (int sub = 0; sub < SUB; ++sub) {
-                        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int st = 4 / SUB * sub; st < 4 / SUB * (sub + 1); ++st) mma_bf16(sum, ones, r[0].v[2 * st], r[0].v[2 * st + 1]);
-                        start[sub][0] = ZEROS ? sum[0] : -136.f * sum[0];
-                        start[sub][1] = ZEROS ? sum[1] : -136.f * sum[1];
-                    }
-                }
-            };
-            struct Tile { uint32_t a[4][4]; float s[SUB][2], z[SUB][2]; };
-            auto operands_of = [&](int t, Tile& f) {
-                const uint4 w = lds16(ring_at + slot + t * kTile + lane * 16);
-                const uint8_t* rec = ring + slot + t * kTile + kBlockBytes + g * (kRecord / 8);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {                       // two MMA steps to a word
-                    const int sub = SUB == 2 ? h : 0;
-                    uint32_t z0 = kZero8, z1 = kZero8;
-                    if (h < SUB) {
-                        const uint32_t two = *(const uint32_t*)(rec + sub * kRecord);
-                        f.s[sub][0] = bf16_lo(two);
-                        f.s[sub][1] = bf16_hi(two);
-                    }
-                    if (ZEROS) {
-                        const uint32_t two = *(const uint32_t*)(rec + sub * kRecord + 4);
-                        z0 = __byte_perm(two, 0, 0x1010);
-                        z1 = __byte_perm(two, 0, 0x3232);
-                        f.z[sub][0] = -bf16_lo(two);
-                        f.z[sub][1] = -bf16_hi(two);
-                    }
-                    uint32_t lo[4], hi[4];
-                    codes_to_bf16<!kLate>(h == 0 ? w.x : w.y, z0, lo);
-                    codes_to_bf16<!kLate>(h == 0 ? w.z : w.w, z1, hi);
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        f.a[2 * h + e][0] = lo[2 * e];
-                        f.a[2 * h + e][1] = hi[2 * e];
-                        f.a[2 * h + e][2] = lo[2 * e + 1];
-                        f.a[2 * h + e][3] = hi[2 * e + 1];
-                    }
-                }
-            };
-            auto multiply = [&](int t, int m, const Tile& f, const Row16 (&r)[kTerms], const float (&start)[SUB][2]) {
+                for (int i = 0; i < kTerms; ++i) r[i] = next[i];
+                if (ahead == 2) load_row<true>(next, row[0] + 64, 0);
+                else if (ahead == 1) load_row<false>(next, row[0] + 64, left - 64);
+            } else {
+                load_row<kWhole>(r, row[m], left);
+            }
+            row[m] += 64;
+            if (kLate) {
+                const uint32_t ones[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
 #pragma unroll
                 for (int sub = 0; sub < SUB; ++sub) {
-                    float part[4] = {0.f, 0.f, 0.f, 0.f};
-                    if (kLate) {
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) part[c] = ZEROS ? f.z[sub][c >> 1] * start[sub][c & 1] : start[sub][c & 1];
-                    }
-#pragma unroll
-                    for (int i = kTerms - 1; i >= 0; --i)           // the small terms first
-#pragma unroll
-                        for (int st = 4 / SUB * sub; st < 4 / SUB * (sub + 1); ++st) mma_bf16(part, f.a[st], r[i].v[2 * st], r[i].v[2 * st + 1]);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) acc[t][m][c] = fmaf(f.s[sub][c >> 1], part[c], acc[t][m][c]);
-                }
-            };
-            if (MT == 1) {                                          // the rows stay while the tiles go by
-                Row16 r[kTerms];
-                float start[SUB][2];
-                rows_of(0, r, start);
-#pragma unroll
-                for (int t = 0; t < T; ++t) {
-                    Tile f;
-                    operands_of(t, f);
-                    multiply(t, 0, f, r, start);
-                }
-            } else {                                                // and the other way round
-                Tile f[T];
-#pragma unroll
-                for (int t = 0; t < T; ++t) operands_of(t, f[t]);
-#pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    Row16 r[kTerms];
-                    float start[SUB][2];
-                    rows_of(m, r, start);
-#pragma unroll
-                    for (int t = 0; t < T; ++t) multiply(t, m, f[t], r, start);
+                    for (int st = 4 / SUB * sub; st < 4 / SUB * (sub + 1); ++st) mma_from(sum, ones, r[0].v[2 * st], r[0].v[2 * st + 1], sum);
+                    start[sub][0] = ZEROS ? sum[0] : -136.f * sum[0];
+                    start[sub][1] = ZEROS ? sum[1] : -136.f * sum[1];
                 }
             }
-            left -= 64;
-            before = slot;
-            slot = slot == (kRing - 1) * kStage ? 0 : slot + kStage;
+        };
+        struct Tile { uint32_t a[4][4]; float s[SUB][2], z[SUB][2]; };
+        auto operands_of = [&](int t, Tile& f) {
+            const uint4 w = lds16(ring_at + slot + t * kTile + lane * 16);
+            const uint8_t* rec = ring + slot + t * kTile + kBlockBytes + g * (kRecord / 8);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {                       // two MMA steps to a word
+                const int sub = SUB == 2 ? h : 0;
+                uint32_t z0 = kZero8, z1 = kZero8;
+                if (h < SUB) {
+                    const uint32_t two = *(const uint32_t*)(rec + sub * kRecord);
+                    f.s[sub][0] = bf16_lo(two);
+                    f.s[sub][1] = bf16_hi(two);
+                }
+                if (ZEROS) {
+                    const uint32_t two = *(const uint32_t*)(rec + sub * kRecord + 4);
+                    z0 = __byte_perm(two, 0, 0x1010);
+                    z1 = __byte_perm(two, 0, 0x3232);
+                    f.z[sub][0] = -bf16_lo(two);
+                    f.z[sub][1] = -bf16_hi(two);
+                }
+                uint32_t lo[4], hi[4];
+                codes_to_bf16<!kLate>(h == 0 ? w.x : w.y, z0, lo);
+                codes_to_bf16<!kLate>(h == 0 ? w.z : w.w, z1, hi);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    f.a[2 * h + e][0] = lo[2 * e];
+                    f.a[2 * h + e][1] = hi[2 * e];
+                    f.a[2 * h + e][2] = lo[2 * e + 1];
+                    f.a[2 * h + e][3] = hi[2 * e + 1];
+                }
+            }
+        };
+        auto multiply = [&](int t, int m, const Tile& f, const Row16 (&r)[kTerms], const float (&start)[SUB][2]) {
+#pragma unroll
+            for (int sub = 0; sub < SUB; ++sub) {
+                float part[4] = {0.f, 0.f, 0.f, 0.f};
+                if (kLate) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) part[c] = ZEROS ? f.z[sub][c >> 1] * start[sub][c & 1] : start[sub][c & 1];
+                }
+#pragma unroll
+                for (int i = kTerms - 1; i >= 0; --i)           // the small terms first
+#pragma unroll
+                    for (int st = 4 / SUB * sub; st < 4 / SUB * (sub + 1); ++st) mma_from(part, f.a[st], r[i].v[2 * st], r[i].v[2 * st + 1], part);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[t][m][c] = fmaf(f.s[sub][c >> 1], part[c], acc[t][m][c]);
+            }
+        };
+        if (MT == 1) {                                          // the rows stay while the tiles go by
+            Row16 r[kTerms];
+            float start[SUB][2];
+            rows_of(0, r, start);
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+                Tile f;
+                operands_of(t, f);
+                multiply(t, 0, f, r, start);
+            }
+        } else {                                                // and the other way round
+            Tile f[T];
+#pragma unroll
+            for (int t = 0; t < T; ++t) operands_of(t, f[t]);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                Row16 r[kTerms];
+                float start[SUB][2];
+                rows_of(m, r, start);
+#pragma unroll
+                for (int t = 0; t < T; ++t) multiply(t, m, f[t], r, start);
+            }
         }
+        left -= 64;
     };
-    if (whole) walk(TrueTag4{});
-    else walk(FalseTag4{});
+    // Blocks whose numbers are all there are read whole; a last one that is not, or all of them where rows are not made of 16-byte
+    // pieces, number by number.
+    const int n = kb1 - kb0, n_whole = !whole ? 0 : (kb1 * 64 > K ? n - 1 : n);
+    if (MT == 1 && n > 0) {
+        if (n_whole > 0) load_row<true>(next, row[0], 0);
+        else load_row<false>(next, row[0], left);
+    }
+    uint32_t slot = 0, before = (kRing - 1) * kStage;              // this block's place in the ring, and the one before it
+    int i = 0;
+    for (; i < n_whole; ++i) {
+        copies_wait<kRing - 2>();
+        __syncwarp();
+        fetch(ring_at + before);                                    // the place that the last block has left
+        block(slot, TrueTag4{}, i + 1 < n_whole ? 2 : (i + 1 < n ? 1 : 0));
+        before = slot;
+        slot = slot == (kRing - 1) * kStage ? 0 : slot + kStage;
+    }
+    for (; i < n; ++i) {
+        copies_wait<kRing - 2>();
+        __syncwarp();
+        fetch(ring_at + before);
+        block(slot, FalseTag4{}, i + 1 < n ? 1 : 0);
+        before = slot;
+        slot = slot == (kRing - 1) * kStage ? 0 : slot + kStage;
+    }
     copies_wait<0>();
     __syncthreads();                             // the rings are done with: the sums go where they were
     float* sums = (float*)smem;
