@@ -339,12 +339,21 @@ extern "C" int hos_product4(const void* x, int x_dtype, long long ldx, const voi
     if (x_dtype == kF32 ? out_dtype != kF32 : x_dtype != kBF16 || (out_dtype != kF32 && out_dtype != kBF16))
         HOS_REFUSE("product4: no product of type %d into type %d", x_dtype, out_dtype);
     const int piece = x_dtype == kF32 ? 4 : 8, whole = K % piece == 0 && ldx % piece == 0 && (uintptr_t)x % 16 == 0;
-    // 16 features to a CTA and 16 warps that share K where that makes few CTAs; more features to a warp (they share its rows of x) and
-    // fewer warps to a CTA where there are enough to fill the SMs with 16 warps each
-    const int sm = sm_count_cached(), tiles = (N + 15) / 16;
-    const int shape = tiles >= 8 * sm ? 2 : (tiles >= 2 * sm ? 1 : 0);
+    // How many tiles of 16 rows of W a warp takes (they share its rows of x), and how many warps of a CTA share K: what makes one wave of
+    // CTAs with 16 warps an SM, more tiles before fewer warps.  Of rows of more than 8 a warp's sums leave room for two tiles.  (us, 8 rows,
+    // with 16 features a warp and 8 or 16 warps / by this rule: 9216 x 2304 gated 10.4 / 9.3, 36864 x 4608 28.5 / 22.3, 4608 x 36864 32.9 / 28.9.)
+    const int units = (N + 15) / 16 * (gated ? 2 : 1), sm = sm_count_cached();
+    const int shape = units <= sm && !gated ? 0 : (units <= 2 * sm ? 1 : (units <= 4 * sm ? 2 : (units <= 8 * sm ? 3 : 4)));
 #define HOS_P4(X, MT, T, G, SUB, Z, W) return launch_product4<X, MT, T, G, SUB, Z, W>(x, codes, records, out, out_dtype == kF32, M, N, K, ldx, ldo, group, act, limit, whole, stream)
-#define HOS_P4_W(X, MT, G, SUB, Z) do { if (shape == 2) HOS_P4(X, MT, ((G ? 2 : 1) * (MT == 1 ? 2 : 1)), G, SUB, Z, 4); else if (shape == 1) HOS_P4(X, MT, (G ? 2 : 1), G, SUB, Z, 8); else HOS_P4(X, MT, (G ? 2 : 1), G, SUB, Z, 16); } while (0)
+#define HOS_P4_W(X, MT, G, SUB, Z)                                       \
+    do {                                                                 \
+        constexpr int kMost = MT == 1 ? 4 : 2;                           \
+        if (shape == 4) HOS_P4(X, MT, kMost, G, SUB, Z, 4);              \
+        else if (shape == 3) HOS_P4(X, MT, kMost, G, SUB, Z, 8);         \
+        else if (shape == 2) HOS_P4(X, MT, kMost, G, SUB, Z, 16);        \
+        else if (shape == 1) HOS_P4(X, MT, 2, G, SUB, Z, 16);            \
+        else HOS_P4(X, MT, (G ? 2 : 1), G, SUB, Z, 16);                  \
+    } while (0)
 #define HOS_P4_M(X, G, SUB, Z) do { if (M <= 8) HOS_P4_W(X, 1, G, SUB, Z); else if (M <= 16) HOS_P4_W(X, 2, G, SUB, Z); else HOS_P4_W(X, 4, G, SUB, Z); } while (0)
 #define HOS_P4_S(X, G, Z) do { if (group == 32) HOS_P4_M(X, G, 2, Z); else HOS_P4_M(X, G, 1, Z); } while (0)
 #define HOS_P4_G(X, Z) do { if (gated) HOS_P4_S(X, true, Z); else HOS_P4_S(X, false, Z); } while (0)
