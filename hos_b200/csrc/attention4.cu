@@ -8,6 +8,7 @@
 #include "common.cuh"
 #include "fourbit.cuh"
 #include "kv_layout.cuh"
+#include "mma_utils.cuh"
 
 namespace hos {
 
@@ -106,53 +107,377 @@ store4_kernel(const T* rows, long long stride, T* held, long long held_stride, c
     }
 }
 
-// One warp per (row, query head); a lane takes the words lane, lane + 32 of a key.
+// d += a . b, free to be woven into its neighbours.
+__device__ __forceinline__ void mma_plain(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// ---- attention of single rows --------------------------------------------------------------------------------------
+// Bound by reading the held keys and values once, and close behind by the instructions that make operands of codes.
+//
+// Scores: S^T = K Q^T with 16 keys as the MMA's rows and up to 8 query heads of a kv head as its columns.  The score of a key is
+// sum_g (s_g (sum_{d in g} q c') - 136 s_g sum q + m_g sum q) over its groups of 64, c' = 128 + c + 8 the operand as codes_to_bf16 makes
+// it without subtracting: a group's product starts at -136 sum q and is multiplied by the key's scale, in 32 bits; neither scale nor
+// middle is rounded into an operand.  Values: O^T = V^T P^T with 16 numbers of a head as rows, P times the value's scale rounded to
+// bfloat16 (the one rounding, 2^-9 of a weight, beside the 2^-9 of the result), the codes exact, and the middles' sum, one number a
+// group and head, in 32 bits beside it.  The scores' registers, transposed eight by eight, are P's operand.
+// Rows in 32 bits: q, and p times the scale, are three bfloat16 numbers each, exactly, and the codes are subtracted first.
+//
+// A CTA takes a share of the pages of one (row, kv head, 8 heads); its warps take 16 keys in turn, each through a ring of its own that
+// cp.async fills, so that no barrier stands in the walk.  Running maxima are a warp's own and are raised when a score passes them by
+// 2^8.  The warps merge through shared memory, the shares through a workspace and attend4_merge_kernel.
+constexpr int kAttendWarps = 8, kMaxSharePages = 256;
+
+template <int DIM> struct Attend4 {
+    static constexpr int kGroups = DIM / 64;
+    static constexpr int kCodes = kGroups * kBlockBytes, kMeta = 64 * kGroups;          // of 16 keys, or values
+    static constexpr int kStage = 2 * (kCodes + kMeta);
+    static constexpr int kRing = DIM >= 192 ? 3 : (DIM == 128 ? 5 : 8);
+    static constexpr int kPitch = DIM + 4;                                              // floats of a head's sums in shared memory
+    static constexpr int kRingBytes = kAttendWarps * kRing * kStage, kSumBytes = kAttendWarps * 8 * kPitch * 4;
+    static constexpr int kShared = kRingBytes > kSumBytes ? kRingBytes : kSumBytes;
+};
+
+template <int GROUPS>
+__device__ __forceinline__ void load_meta(uint32_t at, uint32_t (&m)[GROUPS]) {
+    if (GROUPS == 4) {
+        const uint4 v = lds16(at);
+        m[0] = v.x; m[1 % GROUPS] = v.y; m[2 % GROUPS] = v.z; m[3 % GROUPS] = v.w;
+    } else if (GROUPS == 2) {
+        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(m[0]), "=r"(m[1 % GROUPS]) : "r"(at));
+    } else {
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(m[i]) : "r"(at + 4 * i));
+    }
+}
+
+// The pages of a row's keys, first and one past the last, and how many make a share: more than planned where the row is longer than
+// the plan thought.
+struct KeySpan { int first, pos, page0, page1, share; };
+__device__ __forceinline__ KeySpan key_span(int pos, int window, int share, int splits) {
+    KeySpan k;
+    k.pos = pos;
+    k.first = window > 0 ? max(0, pos - window + 1) : 0;
+    k.page0 = k.first / kPageTokens;
+    k.page1 = pos / kPageTokens + 1;
+    k.share = max(share, (k.page1 - k.page0 + splits - 1) / splits);
+    return k;
+}
+
 template <typename T, int DIM>
-__global__ void __launch_bounds__(128)
-attend4_plain_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out, long long out_stride, const int* __restrict__ token_pos,
-                     const int* __restrict__ token_seq, const int* __restrict__ seq_slot, Paged4 c, int n_tokens, int n_heads, float scale, float cap,
-                     int window) {
+__global__ void __launch_bounds__(kAttendWarps * 32, 2)
+attend4_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out, long long out_stride, const int* __restrict__ token_pos,
+               const int* __restrict__ token_seq, const int* __restrict__ seq_slot, Paged4 c, int n_heads, float scale, float cap, int window, int share, int splits,
+               float* __restrict__ part_o, float2* __restrict__ part_ml) {
+    using A = Attend4<DIM>;
+    constexpr int G = A::kGroups, kTerms = sizeof(T) == 4 ? 3 : 1, kTiles = DIM / 16;
+    constexpr bool kExact = kTerms == 3;
+    extern __shared__ __align__(16) uint8_t ring_bytes[];
+    __shared__ __align__(16) uint4 q_frag[kTerms][G][2][32];
+    __shared__ float q_sum[G][8];
+    __shared__ int ids[kMaxSharePages];
+    __shared__ float2 warp_ml[kAttendWarps][8];
+    __shared__ float warp_f[kAttendWarps][8];
+    __shared__ float2 cta_ml[8];
     pdl_enter();
-    constexpr int kWords = DIM / 8, kPer = (kWords + 31) / 32;
-    const int lane = threadIdx.x & 31;
-    const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (item >= (long long)n_tokens * n_heads) return;
-    const int n = (int)(item / n_heads), h = (int)(item % n_heads), kvh = h / (n_heads / c.n_kv_heads);
-    const int seq = token_seq[n], pos = token_pos[n];
-    float qv[kPer][8], acc[kPer][8] = {}, best = -INFINITY, sum = 0.f;
-    for (int i = 0; i < kPer; ++i)
-        for (int j = 0; j < 8; ++j) qv[i][j] = (lane + 32 * i < kWords) ? to_float(q[(size_t)n * q_stride + h * DIM + (lane + 32 * i) * 8 + j]) : 0.f;
-    const int first = (seq < 0) ? pos + 1 : (window > 0 ? max(0, pos - window + 1) : 0);
-    for (int p = first; p <= pos; ++p) {
-        const int page = page4_of(c, seq_slot[seq], p), row = p % kPageTokens;
-        const size_t at = ((size_t)page * c.n_kv_heads + kvh) * tile4_bytes(DIM);
-        const uint8_t *kt = c.k_pages + at, *vt = c.v_pages + at;
-        float dot = 0.f;
-        for (int i = 0; i < kPer; ++i) {
-            const int d = (lane + 32 * i) * 8, g = d / 64;
-            if (d >= DIM) break;
-            const uint32_t w = *(const uint32_t*)(kt + ((row >> 4) * (DIM / 64) + g) * kBlockBytes + by_row_word(row & 15, d & 63));
-            const uint32_t sm = *(const uint32_t*)(kt + tile4_codes(DIM) + (row * (DIM / 64) + g) * 4);
-            for (int j = 0; j < 8; ++j) dot = fmaf(qv[i][j], fmaf((float)((w >> code_shift(j)) & 15u) - 8.f, bf16_lo(sm), bf16_hi(sm)), dot);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+    const int n = blockIdx.x / splits, split = blockIdx.x % splits;
+    const int per = n_heads / c.n_kv_heads, chunks = (per + 7) / 8, kvh = blockIdx.y / chunks, chunk = blockIdx.y % chunks;
+    const int h0 = kvh * per + chunk * 8, nh = min(8, per - chunk * 8);
+    const int seq = token_seq[n];
+    if (seq < 0) {                                             // padding: zeros (the merge writes them where there are shares)
+        if (splits == 1)
+            for (int i = threadIdx.x; i < nh * DIM; i += blockDim.x) out[(size_t)n * out_stride + (size_t)h0 * DIM + i] = from_float<T>(0.f);
+        return;
+    }
+    const KeySpan span = key_span(token_pos[n], window, share, splits);
+    const int p0 = span.page0 + split * span.share, p1 = min(span.page1, p0 + span.share);
+    if (p0 >= p1) return;
+    const int* table = c.page_table + (size_t)seq_slot[seq] * c.table_stride;
+    auto page_of = [&](int p) { return table[c.ring_pages > 0 ? p % c.ring_pages : p]; };
+    for (int i = threadIdx.x; i < min(p1 - p0, kMaxSharePages); i += blockDim.x) ids[i] = page_of(p0 + i);
+    // the heads' numbers as operands, and their sums over 64
+    const T* q_row = q + (size_t)n * q_stride + (size_t)h0 * DIM;
+    for (int i = threadIdx.x; i < G * 64; i += blockDim.x) {
+        const int l = i & 31, half = (i >> 5) & 1, grp = i >> 6, head = l >> 2, d = grp * 64 + (l & 3) * 16 + half * 8;
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = head < nh ? to_float(q_row[head * DIM + d + j]) : 0.f;
+#pragma unroll
+        for (int term = 0; term < kTerms; ++term) {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                w[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+                v[2 * j] -= bf16_lo(w[j]);
+                v[2 * j + 1] -= bf16_hi(w[j]);
+            }
+            q_frag[term][grp][half][l] = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        const float score = softcap_precise(warp_sum(dot) * scale, cap), top = fmaxf(best, score);
-        const float old = expf(best - top), e = expf(score - top);
-        best = top;
-        sum = sum * old + e;
-        for (int i = 0; i < kPer; ++i) {
-            const int d = (lane + 32 * i) * 8, g = d / 64;
-            if (d >= DIM) break;
-            const uint32_t sm = *(const uint32_t*)(vt + tile4_codes(DIM) + (row * (DIM / 64) + g) * 4);
-            for (int j = 0; j < 8; ++j) {
-                const int dd = (d & 63) + j;
-                const uint8_t b = vt[((row >> 4) * (DIM / 64) + g) * kBlockBytes + by_column_byte(row & 15, dd & ~8)];
-                acc[i][j] = acc[i][j] * old + e * fmaf((float)((b >> ((dd & 8) ? 4 : 0)) & 15) - 8.f, bf16_lo(sm), bf16_hi(sm));
+    }
+    for (int i = warp; i < G * 8; i += kAttendWarps) {
+        const int head = i & 7, grp = i >> 3;
+        float v = head < nh ? to_float(q_row[head * DIM + grp * 64 + lane]) + to_float(q_row[head * DIM + grp * 64 + 32 + lane]) : 0.f;
+        v = warp_sum(v);
+        if (lane == 0) q_sum[grp][head] = v;
+    }
+    __syncthreads();
+
+    const int b0 = max(span.first, p0 * kPageTokens) >> 4, b1 = min(span.pos, p1 * kPageTokens - 1) >> 4;      // blocks of 16 keys, b1 the last
+    const uint32_t ring = smem_u32(ring_bytes) + warp * A::kRing * A::kStage;
+    int to_fetch = b0 + warp;
+    auto fetch = [&](uint32_t to) {
+        if (to_fetch <= b1) {
+            const int p = to_fetch >> 2;
+            const size_t tile = ((size_t)(p - p0 < kMaxSharePages ? ids[p - p0] : page_of(p)) * c.n_kv_heads + kvh) * tile4_bytes(DIM);
+            const int in = to_fetch & 3;
+            const uint8_t *k = c.k_pages + tile, *v = c.v_pages + tile;
+#pragma unroll
+            for (int i = 0; i < G; ++i) {
+                copy16_async(to + i * kBlockBytes + lane * 16, k + (in * G + i) * kBlockBytes + lane * 16);
+                copy16_async(to + A::kCodes + A::kMeta + i * kBlockBytes + lane * 16, v + (in * G + i) * kBlockBytes + lane * 16);
+            }
+            if ((lane & 15) < 4 * G) {
+                const uint8_t* src = (lane < 16 ? k : v) + tile4_codes(DIM) + in * A::kMeta + (lane & 15) * 16;
+                copy16_async(to + A::kCodes + (lane < 16 ? 0 : A::kCodes + A::kMeta) + (lane & 15) * 16, src);
+            }
+        }
+        to_fetch += kAttendWarps;
+        copies_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < A::kRing - 1; ++i) fetch(ring + i * A::kStage);
+
+    float o[kTiles][4], mid[G][2], best[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+#pragma unroll
+    for (int i = 0; i < G; ++i) mid[i][0] = mid[i][1] = 0.f;
+    const float scale2 = scale * 1.44269504f, cap2 = cap * 1.44269504f, in_cap = cap > 0.f ? 2.f * scale2 / cap : 0.f;
+    uint32_t slot = ring, before = ring + (A::kRing - 1) * A::kStage;
+    for (int b = b0 + warp; b <= b1; b += kAttendWarps) {
+        copies_wait<A::kRing - 2>();
+        __syncwarp();
+        fetch(before);                                         // the place that the last block has left
+        uint32_t km[2][G], vm[2][G];                           // of the keys g and g + 8
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            load_meta<G>(slot + A::kCodes + (g + 8 * r) * 4 * G, km[r]);
+            load_meta<G>(slot + 2 * A::kCodes + A::kMeta + (g + 8 * r) * 4 * G, vm[r]);
+        }
+        const int key = b * 16 + g;
+        const bool edge = b * 16 < span.first || b * 16 + 15 > span.pos;
+        bool hidden[2] = {false, false};
+        if (edge) {                                            // what is hidden may be anything: its scales and middles become zeros
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                hidden[r] = key + 8 * r < span.first || key + 8 * r > span.pos;
+#pragma unroll
+                for (int i = 0; i < G; ++i) {
+                    if (hidden[r]) km[r][i] = vm[r][i] = 0u;
+                }
+            }
+        }
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+            const uint4 w = lds16(slot + i * kBlockBytes + lane * 16);
+            uint32_t lo[2][4], hi[2][4];                       // the key g's, and g + 8's
+            codes_to_bf16<kExact>(w.x, kZero8, lo[0]);
+            codes_to_bf16<kExact>(w.y, kZero8, lo[1]);
+            codes_to_bf16<kExact>(w.z, kZero8, hi[0]);
+            codes_to_bf16<kExact>(w.w, kZero8, hi[1]);
+            const float2 qs = *(const float2*)&q_sum[i][2 * t4];
+            float part[4] = {0.f, 0.f, 0.f, 0.f};
+            if (!kExact) {
+                part[0] = part[2] = -136.f * qs.x;
+                part[1] = part[3] = -136.f * qs.y;
+            }
+#pragma unroll
+            for (int term = kTerms - 1; term >= 0; --term) {
+                const uint4 qa = q_frag[term][i][0][lane], qb = q_frag[term][i][1][lane];
+                const uint32_t qf[8] = {qa.x, qa.y, qa.z, qa.w, qb.x, qb.y, qb.z, qb.w};
+#pragma unroll
+                for (int st = 0; st < 4; ++st) {
+                    const uint32_t a[4] = {lo[st >> 1][2 * (st & 1)], hi[st >> 1][2 * (st & 1)], lo[st >> 1][2 * (st & 1) + 1], hi[st >> 1][2 * (st & 1) + 1]};
+                    mma_plain(part, a, qf[2 * st], qf[2 * st + 1]);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t sm = km[e >> 1][i];
+                s[e] = fmaf(bf16_lo(sm), part[e], fmaf(bf16_hi(sm), (e & 1) ? qs.y : qs.x, s[e]));
+            }
+        }
+        // scores in units of log 2
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (cap > 0.f) {
+                if (kExact) s[e] = cap2 * tanhf(s[e] * scale / cap);
+                else s[e] = cap2 * (1.f - 2.f * rcp_approx(1.f + ex2_approx(s[e] * in_cap)));
+            } else {
+                s[e] *= scale2;
+            }
+            if (hidden[e >> 1]) s[e] = -INFINITY;
+        }
+        float top[2] = {fmaxf(s[0], s[2]), fmaxf(s[1], s[3])};
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) {
+            top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], off));
+            top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], off));
+        }
+        if (__any_sync(0xffffffffu, top[0] > best[0] + 8.f || top[1] > best[1] + 8.f)) {
+            float f[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float m = fmaxf(best[h], top[h]);
+                f[h] = best[h] == m ? 1.f : ex2_approx(best[h] - m);
+                best[h] = m;
+                sum[h] *= f[h];
+#pragma unroll
+                for (int i = 0; i < G; ++i) mid[i][h] *= f[h];
+            }
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) {
+                o[i][0] *= f[0]; o[i][1] *= f[1]; o[i][2] *= f[0]; o[i][3] *= f[1];
+            }
+        }
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[e] = ex2_approx(s[e] - best[e & 1]);
+        sum[0] += p[0] + p[2];
+        sum[1] += p[1] + p[3];
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+            float w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t sm = vm[e >> 1][i];
+                w[e] = p[e] * bf16_lo(sm);
+                mid[i][e & 1] = fmaf(p[e], bf16_hi(sm), mid[i][e & 1]);
+            }
+            uint32_t pb[kTerms][2];
+#pragma unroll
+            for (int term = 0; term < kTerms; ++term) {
+                const uint32_t a = pack_bf16(w[0], w[1]), b8 = pack_bf16(w[2], w[3]);
+                pb[term][0] = transposed_8x8(a);
+                pb[term][1] = transposed_8x8(b8);
+                w[0] -= bf16_lo(a); w[1] -= bf16_hi(a); w[2] -= bf16_lo(b8); w[3] -= bf16_hi(b8);
+            }
+            const uint4 v = lds16(slot + A::kCodes + A::kMeta + i * kBlockBytes + lane * 16);
+            const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int mt = 0; mt < 4; ++mt) {
+                uint32_t a[4];
+                codes_to_bf16<true>(words[mt], kZero8, a);
+#pragma unroll
+                for (int term = kTerms - 1; term >= 0; --term) mma_plain(o[4 * i + mt], a, pb[term][0], pb[term][1]);
+            }
+        }
+        before = slot;
+        slot = slot == ring + (A::kRing - 1) * A::kStage ? ring : slot + A::kStage;
+    }
+    copies_wait<0>();
+    // a lane's sums over its keys, added up over the lanes of its heads
+#pragma unroll
+    for (int off = 4; off < 32; off <<= 1) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], off);
+#pragma unroll
+            for (int i = 0; i < G; ++i) mid[i][h] += __shfl_xor_sync(0xffffffffu, mid[i][h], off);
+        }
+    }
+    if (g == 0) {
+        warp_ml[warp][2 * t4] = make_float2(best[0], sum[0]);
+        warp_ml[warp][2 * t4 + 1] = make_float2(best[1], sum[1]);
+    }
+    __syncthreads();                                           // the rings are done with: the sums go where they were
+    float* sums = (float*)ring_bytes;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        if (2 * t4 + h < nh) {
+            float* to = sums + (warp * 8 + 2 * t4 + h) * A::kPitch;
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) {
+                to[i * 16 + g] = o[i][h] + mid[i / 4][h];
+                to[i * 16 + g + 8] = o[i][2 + h] + mid[i / 4][h];
             }
         }
     }
-    for (int i = 0; i < kPer; ++i)
-        for (int j = 0; j < 8; ++j)
-            if (lane + 32 * i < kWords) out[(size_t)n * out_stride + h * DIM + (lane + 32 * i) * 8 + j] = from_float<T>(sum > 0.f ? acc[i][j] / sum : 0.f);
+    if (threadIdx.x < 8) {
+        float m = -INFINITY, l = 0.f;
+        for (int w = 0; w < kAttendWarps; ++w) m = fmaxf(m, warp_ml[w][threadIdx.x].x);
+        for (int w = 0; w < kAttendWarps; ++w) {
+            const float2 ml = warp_ml[w][threadIdx.x];
+            const float f = ml.x == m ? 1.f : ex2_approx(ml.x - m);       // a warp without keys: 2^(-inf)
+            warp_f[w][threadIdx.x] = f;
+            l += f * ml.y;
+        }
+        cta_ml[threadIdx.x] = make_float2(m, l);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < nh * DIM; i += blockDim.x) {
+        const int h = i / DIM, d = i % DIM;
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < kAttendWarps; ++w) v = fmaf(warp_f[w][h], sums[(w * 8 + h) * A::kPitch + d], v);
+        if (splits == 1) {
+            out[(size_t)n * out_stride + (size_t)(h0 + h) * DIM + d] = from_float<T>(v / cta_ml[h].y);
+        } else {
+            const size_t at = ((size_t)n * n_heads + h0 + h) * splits + split;
+            part_o[at * DIM + d] = v;
+            if (d == 0) part_ml[at] = cta_ml[h];
+        }
+    }
+}
+
+// The shares of a (row, head) added up: DIM threads, one a number.
+template <typename T, int DIM>
+__global__ void __launch_bounds__(DIM)
+attend4_merge_kernel(T* __restrict__ out, long long out_stride, const int* __restrict__ token_pos, const int* __restrict__ token_seq, int n_heads, int window,
+                     int share, int splits, const float* __restrict__ part_o, const float2* __restrict__ part_ml) {
+    pdl_enter();
+    const int n = blockIdx.x / n_heads, h = blockIdx.x % n_heads, d = threadIdx.x;
+    T* to = out + (size_t)n * out_stride + (size_t)h * DIM + d;
+    if (token_seq[n] < 0) {
+        *to = from_float<T>(0.f);
+        return;
+    }
+    const KeySpan span = key_span(token_pos[n], window, share, splits);
+    const int parts = (span.page1 - span.page0 + span.share - 1) / span.share;
+    const size_t at = (size_t)blockIdx.x * splits;
+    float m = -INFINITY, l = 0.f, v = 0.f;
+    for (int s = 0; s < parts; ++s) m = fmaxf(m, part_ml[at + s].x);
+    for (int s = 0; s < parts; ++s) {
+        const float2 ml = part_ml[at + s];
+        const float f = ml.x == m ? 1.f : ex2_approx(ml.x - m);
+        l = fmaf(f, ml.y, l);
+        v = fmaf(f, part_o[(at + s) * DIM + d], v);
+    }
+    *to = from_float<T>(v / l);
+}
+
+template <typename T, int DIM>
+int launch_attend4(const void* q, long long q_stride, void* out, long long out_stride, const int* token_pos, const int* token_seq, const int* seq_slot,
+                   const Paged4& c, int n_tokens, int n_heads, float scale, float cap, int window, int share, int splits, float* part_o, float2* part_ml,
+                   cudaStream_t stream) {
+    constexpr int smem = Attend4<DIM>::kShared;
+    auto kernel = attend4_kernel<T, DIM>;
+    static bool set = false;                                   // once per kernel: the attribute stays
+    if (!set) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return check_launch("attend4");
+        set = true;
+    }
+    const int per = n_heads / c.n_kv_heads, chunks = (per + 7) / 8;
+    launch_pdl(kernel, dim3((unsigned)((long long)n_tokens * splits), (unsigned)(c.n_kv_heads * chunks)), dim3(kAttendWarps * 32), smem, stream, (const T*)q,
+               q_stride, (T*)out, out_stride, token_pos, token_seq, seq_slot, c, n_heads, scale, cap, window, share, splits, part_o, part_ml);
+    if (splits > 1)
+        launch_pdl(attend4_merge_kernel<T, DIM>, dim3((unsigned)((long long)n_tokens * n_heads)), dim3(DIM), 0, stream, (T*)out, out_stride, token_pos, token_seq,
+                   n_heads, window, share, splits, (const float*)part_o, (const float2*)part_ml);
+    return check_launch("attend4");
 }
 
 }  // namespace hos
@@ -178,16 +503,20 @@ extern "C" int hos_store4(const void* rows, int dtype, long long stride, void* h
     return check_launch("store4");
 }
 
+// Every row alone over its pages, `share` of them to a CTA: `splits` shares cover the longest row's.  More than one: part_o and part_ml
+// hold n_tokens * n_heads * splits * head_dim and that many pairs of 32-bit numbers.
 extern "C" int hos_attend4(const void* q, int dtype, long long q_stride, void* out, long long out_stride, const int* token_pos, const int* token_seq,
                            const int* seq_slot, void* k_pages, void* v_pages, const int* page_table, int table_stride, int ring_pages, int n_kv_heads,
-                           int head_dim, int n_tokens, int n_heads, float scale, float cap, int window, cudaStream_t stream) {
+                           int head_dim, int n_tokens, int n_heads, float scale, float cap, int window, int share, int splits, float* part_o, float* part_ml,
+                           cudaStream_t stream) {
     if (n_tokens <= 0) return 0;
     HOS_CHECK_PAGED4("attend4");
     if (n_heads <= 0 || n_heads % n_kv_heads) HOS_REFUSE("attend4: %d query heads over %d kv heads", n_heads, n_kv_heads);
-    const dim3 grid((unsigned)(((long long)n_tokens * n_heads + 3) / 4));
-#define HOS_A4(T, D) launch_pdl(attend4_plain_kernel<T, D>, grid, dim3(128), 0, stream, (const T*)q, q_stride, (T*)out, out_stride, token_pos, token_seq, seq_slot, c, n_tokens, n_heads, scale, cap, window)
+    if (share < 1 || share > kMaxSharePages || splits < 1) HOS_REFUSE("attend4: %d shares of %d pages (1..%d)", splits, share, kMaxSharePages);
+    if (splits > 1 && (part_o == nullptr || part_ml == nullptr)) HOS_REFUSE("attend4: shares need a workspace");
+    if ((long long)n_tokens * splits > 0x7fffffffll || (long long)n_tokens * n_heads > 0x7fffffffll) HOS_REFUSE("attend4: %d rows in %d shares", n_tokens, splits);
+#define HOS_A4(T, D) return launch_attend4<T, D>(q, q_stride, out, out_stride, token_pos, token_seq, seq_slot, c, n_tokens, n_heads, scale, cap, window, share, splits, part_o, (float2*)part_ml, stream)
 #define HOS_A4_D(T) do { if (head_dim == 64) HOS_A4(T, 64); else if (head_dim == 128) HOS_A4(T, 128); else if (head_dim == 192) HOS_A4(T, 192); else HOS_A4(T, 256); } while (0)
     if (dtype == kF32) HOS_A4_D(float);
     else HOS_A4_D(bf16);
-    return check_launch("attend4");
 }

@@ -49,6 +49,25 @@ def store(rows: torch.Tensor, step, cache: ops.PagedKVArgs, held: Optional[torch
                        ops._stream())
 
 
+MAX_SHARE_PAGES = 256          # page numbers that a CTA keeps
+
+
+def shares(rows: int, kv_items: int, longest: int, window: Optional[int], fill: float = 1.0):
+    """(pages of a share, shares of a row): `rows` rows times `kv_items` (kv heads, times the eights of query heads that share one) over
+    up to `longest` keys.  Two CTAs fit an SM: rows that leave CTAs free are cut into as many shares as fill them; many rows of
+    unequal lengths (`fill`: the sum of the keys over rows * the longest) into shares of up to 32 pages, which CTAs take as they come free."""
+    span = min(longest, window) if window else longest
+    pages = max(1, -(-span // ops.PAGE_TOKENS) + (1 if window and longest > window else 0))
+    places, items = 2 * ops.sm_count(), max(1, rows * kv_items)
+    if items * fill < places:
+        splits = max(1, int(places // max(1.0, items * fill)))
+        share = -(-pages // splits)
+    else:
+        share = pages if fill > 0.9 and items % places == 0 else 32
+    share = max(1, min(share, pages, MAX_SHARE_PAGES))
+    return share, -(-pages // share)
+
+
 def attend(q: torch.Tensor, out: torch.Tensor, step, cache: ops.PagedKVArgs, n_heads: int, scale: float, softcap: float = 0.0,
            window: Optional[int] = None) -> None:
     """out[N, n_heads * head_dim] = softmax attention of the step's rows, each at its own position, over what the pages hold up to
@@ -60,7 +79,13 @@ def attend(q: torch.Tensor, out: torch.Tensor, step, cache: ops.PagedKVArgs, n_h
     if q.shape[1] != n_heads * cache.head_dim or out.shape != q.shape:
         raise KernelError(f"queries {tuple(q.shape)} and output {tuple(out.shape)} for {n_heads} heads of {cache.head_dim}")
     _check_step(n, step, "attend")
+    kv, dim = cache.n_kv_heads, cache.head_dim
+    share, splits = shares(n, kv * -(-(n_heads // kv) // 8), step.max_len_after, window, step.fill_for(window))
+    part_o = part_ml = None
+    if splits > 1:
+        part_o = torch.empty(n * n_heads * splits * dim, dtype=torch.float32, device=q.device)
+        part_ml = torch.empty(n * n_heads * splits * 2, dtype=torch.float32, device=q.device)
     ops.fourbit().call("hos_attend4", ops._ptr(q), ops.dtype_code(q.dtype), q.stride(0), ops._ptr(out), out.stride(0), ops._ptr(step.token_pos),
                        ops._ptr(step.token_seq), ops._ptr(step.seq_slot), ops._ptr(cache.k_pages), ops._ptr(cache.v_pages), ops._ptr(cache.page_table),
-                       cache.table_stride, cache.ring_pages, cache.n_kv_heads, cache.head_dim, n, n_heads, float(scale), float(softcap),
-                       int(window) if window else 0, ops._stream())
+                       cache.table_stride, cache.ring_pages, kv, dim, n, n_heads, float(scale), float(softcap),
+                       int(window) if window else 0, share, splits, ops._ptr(part_o), ops._ptr(part_ml), ops._stream())
