@@ -232,7 +232,7 @@ class CacheManager:
         for store, place in zip(self.stores, self._placed):
             if place is not None:
                 view = self.groups[place[0]].view(place[1])
-                store.kv.k_pages, store.kv.v_pages = view.k_pages, view.v_pages
+                store.kv.k_pages, store.kv.v_pages, store.kv.four = view.k_pages, view.v_pages, None
 
     def release(self, slot: int) -> None:
         if slot not in self.lengths:

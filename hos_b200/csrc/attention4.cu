@@ -12,6 +12,7 @@
 
 namespace hos {
 
+// One call's view of the pages, as the host hands it over (ops.Paged4).
 struct Paged4 {
     uint8_t* k_pages;
     uint8_t* v_pages;
@@ -485,13 +486,13 @@ int launch_attend4(const void* q, long long q_stride, void* out, long long out_s
 using namespace hos;
 
 #define HOS_CHECK_PAGED4(what)                                                                                            \
+    const Paged4 c = *(const Paged4*)cache;                                                                                \
+    const int head_dim = c.head_dim, n_kv_heads = c.n_kv_heads;                                                            \
     if (head_dim % 64 || head_dim < 64 || head_dim > 256) HOS_REFUSE(what ": head size %d (64, 128, 192 or 256)", head_dim);     \
-    if (n_kv_heads <= 0) HOS_REFUSE(what ": %d kv heads", n_kv_heads);                                                         \
-    const Paged4 c{(uint8_t*)k_pages, (uint8_t*)v_pages, page_table, table_stride, ring_pages, n_kv_heads, head_dim}
+    if (n_kv_heads <= 0) HOS_REFUSE(what ": %d kv heads", n_kv_heads)
 
 extern "C" int hos_store4(const void* rows, int dtype, long long stride, void* held, long long held_stride, const int* token_pos, const int* token_seq,
-                          const int* seq_slot, const int* seq_len_after, void* k_pages, void* v_pages, const int* page_table, int table_stride, int ring_pages,
-                          int n_kv_heads, int head_dim, int n_tokens, cudaStream_t stream) {
+                          const int* seq_slot, const int* seq_len_after, const void* cache, int n_tokens, cudaStream_t stream) {
     if (n_tokens <= 0) return 0;
     HOS_CHECK_PAGED4("store4");
     const long long items = (long long)n_tokens * 2 * n_kv_heads * (head_dim / 64);
@@ -503,19 +504,21 @@ extern "C" int hos_store4(const void* rows, int dtype, long long stride, void* h
     return check_launch("store4");
 }
 
-// Every row alone over its pages, `share` of them to a CTA: `splits` shares cover the longest row's.  More than one: part_o and part_ml
-// hold n_tokens * n_heads * splits * head_dim and that many pairs of 32-bit numbers.
+// Every row alone over its pages, `share` of them to a CTA: `splits` shares cover the longest row's.  More than one: `parts`
+// holds n_tokens * n_heads * splits * (head_dim + 2) 32-bit numbers.
 extern "C" int hos_attend4(const void* q, int dtype, long long q_stride, void* out, long long out_stride, const int* token_pos, const int* token_seq,
-                           const int* seq_slot, void* k_pages, void* v_pages, const int* page_table, int table_stride, int ring_pages, int n_kv_heads,
-                           int head_dim, int n_tokens, int n_heads, float scale, float cap, int window, int share, int splits, float* part_o, float* part_ml,
-                           cudaStream_t stream) {
+                           const int* seq_slot, const void* cache, int n_tokens, int n_heads, float scale, float cap, int window, int share, int splits,
+                           float* parts, cudaStream_t stream) {
     if (n_tokens <= 0) return 0;
     HOS_CHECK_PAGED4("attend4");
     if (n_heads <= 0 || n_heads % n_kv_heads) HOS_REFUSE("attend4: %d query heads over %d kv heads", n_heads, n_kv_heads);
     if (share < 1 || share > kMaxSharePages || splits < 1) HOS_REFUSE("attend4: %d shares of %d pages (1..%d)", splits, share, kMaxSharePages);
-    if (splits > 1 && (part_o == nullptr || part_ml == nullptr)) HOS_REFUSE("attend4: shares need a workspace");
+    if (splits > 1 && parts == nullptr) HOS_REFUSE("attend4: shares need a workspace");
     if ((long long)n_tokens * splits > 0x7fffffffll || (long long)n_tokens * n_heads > 0x7fffffffll) HOS_REFUSE("attend4: %d rows in %d shares", n_tokens, splits);
-#define HOS_A4(T, D) return launch_attend4<T, D>(q, q_stride, out, out_stride, token_pos, token_seq, seq_slot, c, n_tokens, n_heads, scale, cap, window, share, splits, part_o, (float2*)part_ml, stream)
+    const size_t n_parts = (size_t)n_tokens * n_heads * splits;
+    float2* part_ml = (float2*)parts;                          // pairs first: they want 8 bytes' alignment
+    float* part_o = parts == nullptr ? nullptr : parts + 2 * n_parts;
+#define HOS_A4(T, D) return launch_attend4<T, D>(q, q_stride, out, out_stride, token_pos, token_seq, seq_slot, c, n_tokens, n_heads, scale, cap, window, share, splits, part_o, part_ml, stream)
 #define HOS_A4_D(T) do { if (head_dim == 64) HOS_A4(T, 64); else if (head_dim == 128) HOS_A4(T, 128); else if (head_dim == 192) HOS_A4(T, 192); else HOS_A4(T, 256); } while (0)
     if (dtype == kF32) HOS_A4_D(float);
     else HOS_A4_D(bf16);

@@ -329,9 +329,18 @@ using namespace hos;
 
 extern "C" const char* hos_last_error() { return error_buffer(); }
 
-// Rows of x are ldx numbers apart, rows of out ldo; gated: W has 2 N rows, gate's 16-row tiles first, then up's.
-extern "C" int hos_product4(const void* x, int x_dtype, long long ldx, const void* codes, const void* records, void* out, int out_dtype, long long ldo,
-                            int M, int N, int K, int group, int zeros, int gated, int act, float limit, cudaStream_t stream) {
+// A matrix as the host hands it over (ops.Matrix4): N features (gated: of gate, and as many of up, gate's 16-row tiles first).
+struct Matrix4 {
+    const uint8_t *codes, *records;
+    int n, k, group, zeros, gated;
+};
+
+// Rows of x are ldx numbers apart, rows of out ldo.
+extern "C" int hos_product4(const void* x, int x_dtype, long long ldx, const void* matrix, void* out, int out_dtype, long long ldo, int M, int act, float limit,
+                            cudaStream_t stream) {
+    const Matrix4 w = *(const Matrix4*)matrix;
+    const int N = w.n, K = w.k, group = w.group, zeros = w.zeros, gated = w.gated;
+    const void *codes = w.codes, *records = w.records;
     if (M <= 0 || N <= 0) return 0;
     if (K <= 0) HOS_REFUSE("product4: K %d", K);
     if (group < 32 || (group != 32 && group % 64)) HOS_REFUSE("product4: groups of %d weights (32, or a multiple of 64)", group);

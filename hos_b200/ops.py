@@ -283,6 +283,7 @@ class PagedKVArgs:
     head_dim: int
     v_head_dim: int = 0          # 0: values are as wide as keys
     bits: Optional[int] = None   # 4: uint8 [n_pages, n_kv_heads, tile4_bytes(head_dim)] tiles (csrc/fourbit.cuh)
+    four: Optional[tuple] = None # what paged4() made of the fields
 
     @property
     def table_stride(self) -> int:
@@ -1409,19 +1410,37 @@ def _check_rows(t: torch.Tensor, what: str, dtype=None) -> None:
     """Rows [n, width] whose numbers lie side by side, any number of numbers apart."""
     if not t.is_cuda:
         raise KernelError(f"{what} must be on the GPU")
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        raise KernelError(f"{what} must be rows of neighbouring numbers, found shape {tuple(t.shape)} and strides {t.stride()}")
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 2 or (strides[1] != 1 and shape[1] > 1) or (strides[0] < shape[1] and shape[0] > 1):
+        raise KernelError(f"{what} must be rows of neighbouring numbers, found shape {tuple(shape)} and strides {strides}")
     if dtype is not None and t.dtype != dtype:
         raise KernelError(f"{what} must be {dtype}, found {t.dtype}")
 
 
-def product4(x: torch.Tensor, codes: torch.Tensor, records: torch.Tensor, out: torch.Tensor, group: int, zeros: bool, gated: bool,
-             act: int = 0, limit: float = 0.0) -> None:
-    """out[M, N] = x[M, K] . W^T with W in 4 bits as parts/weights4.py lays it out; gated: W is a gate's and an up's N rows and
-    out = act(gate) * up."""
-    core4 = fourbit()
-    core4.call("hos_product4", _ptr(x), dtype_code(x.dtype), x.stride(0), _ptr(codes), _ptr(records), _ptr(out), dtype_code(out.dtype), out.stride(0),
-               x.shape[0], out.shape[1], x.shape[1], int(group), int(zeros), int(gated), int(act), float(limit), _stream())
+class Matrix4(ctypes.Structure):
+    """A matrix in 4 bits as csrc/weights4.cu takes it."""
+    _fields_ = [("codes", _p), ("records", _p), ("n", _i), ("k", _i), ("group", _i), ("zeros", _i), ("gated", _i)]
+
+
+class Paged4(ctypes.Structure):
+    """A view of 4-bit pages as csrc/attention4.cu takes it."""
+    _fields_ = [("k_pages", _p), ("v_pages", _p), ("page_table", _p), ("table_stride", _i), ("ring_pages", _i), ("n_kv_heads", _i), ("head_dim", _i)]
+
+
+def paged4(cache: PagedKVArgs) -> int:
+    """Address of the view's description, made once for as long as the view's arrays stay."""
+    d = cache.four
+    if d is None:
+        d = Paged4(cache.k_pages.data_ptr(), cache.v_pages.data_ptr(), cache.page_table.data_ptr(), cache.table_stride, cache.ring_pages,
+                   cache.n_kv_heads, cache.head_dim)
+        cache.four = d = (d, ctypes.addressof(d))
+    return d[1]
+
+
+def product4(x: torch.Tensor, matrix: int, out: torch.Tensor, act: int = 0, limit: float = 0.0) -> None:
+    """out[M, N] = x[M, K] . W^T with the matrix in 4 bits that `matrix` (the address of a Matrix4) describes; gated: out = act(gate) * up."""
+    fourbit().call("hos_product4", x.data_ptr(), dtype_code(x.dtype), x.stride(0), matrix, out.data_ptr(), dtype_code(out.dtype), out.stride(0), x.shape[0],
+                   act, limit, _stream())
 
 
 def copy_pages(table: torch.Tensor, most_bytes: int, src: torch.Tensor, dst: torch.Tensor, n_pages: int) -> None:
@@ -1432,4 +1451,4 @@ def copy_pages(table: torch.Tensor, most_bytes: int, src: torch.Tensor, dst: tor
     _check(dst, "destination pages", torch.int32, 1)
     if src.shape != dst.shape:
         raise KernelError(f"copy_pages: {src.shape[0]} source pages and {dst.shape[0]} destinations")
-    fourbit().call("hos_copy_pages", _ptr(table), table.shape[0], int(most_bytes), _ptr(src), _ptr(dst), src.shape[0], int(n_pages), _stream())
+    fourbit().call("hos_copy_pages", table.data_ptr(), table.shape[0], most_bytes, src.data_ptr(), dst.data_ptr(), src.shape[0], n_pages, _stream())

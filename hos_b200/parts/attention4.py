@@ -43,10 +43,9 @@ def store(rows: torch.Tensor, step, cache: ops.PagedKVArgs, held: Optional[torch
         ops._check_rows(held, "what is held", rows.dtype)
         if held.shape != rows.shape:
             raise KernelError("what is held and the rows differ in size")
-    ops.fourbit().call("hos_store4", ops._ptr(rows), ops.dtype_code(rows.dtype), rows.stride(0), ops._ptr(held), held.stride(0) if held is not None else 0,
-                       ops._ptr(step.token_pos), ops._ptr(step.token_seq), ops._ptr(step.seq_slot), ops._ptr(step.seq_len_after), ops._ptr(cache.k_pages),
-                       ops._ptr(cache.v_pages), ops._ptr(cache.page_table), cache.table_stride, cache.ring_pages, cache.n_kv_heads, cache.head_dim, n,
-                       ops._stream())
+    ops.fourbit().call("hos_store4", rows.data_ptr(), ops.dtype_code(rows.dtype), rows.stride(0), held.data_ptr() if held is not None else None,
+                       held.stride(0) if held is not None else 0, step.token_pos.data_ptr(), step.token_seq.data_ptr(), step.seq_slot.data_ptr(),
+                       step.seq_len_after.data_ptr(), ops.paged4(cache), n, ops._stream())
 
 
 MAX_SHARE_PAGES = 256          # page numbers that a CTA keeps
@@ -79,13 +78,15 @@ def attend(q: torch.Tensor, out: torch.Tensor, step, cache: ops.PagedKVArgs, n_h
     if q.shape[1] != n_heads * cache.head_dim or out.shape != q.shape:
         raise KernelError(f"queries {tuple(q.shape)} and output {tuple(out.shape)} for {n_heads} heads of {cache.head_dim}")
     _check_step(n, step, "attend")
-    kv, dim = cache.n_kv_heads, cache.head_dim
-    share, splits = shares(n, kv * -(-(n_heads // kv) // 8), step.max_len_after, window, step.fill_for(window))
-    part_o = part_ml = None
+    kv = cache.n_kv_heads
+    key = ("shares of 4-bit pages", n, n_heads, kv, window, step.row_offset)
+    plan = step.shared.get(key)                      # once per step and kind of layer
+    if plan is None:
+        plan = step.shared[key] = shares(n, kv * -(-(n_heads // kv) // 8), step.max_len_after, window, step.fill_for(window))
+    share, splits = plan
+    parts = None
     if splits > 1:
-        part_o = torch.empty(n * n_heads * splits * dim, dtype=torch.float32, device=q.device)
-        part_ml = torch.empty(n * n_heads * splits * 2, dtype=torch.float32, device=q.device)
-    ops.fourbit().call("hos_attend4", ops._ptr(q), ops.dtype_code(q.dtype), q.stride(0), ops._ptr(out), out.stride(0), ops._ptr(step.token_pos),
-                       ops._ptr(step.token_seq), ops._ptr(step.seq_slot), ops._ptr(cache.k_pages), ops._ptr(cache.v_pages), ops._ptr(cache.page_table),
-                       cache.table_stride, cache.ring_pages, kv, dim, n, n_heads, float(scale), float(softcap),
-                       int(window) if window else 0, share, splits, ops._ptr(part_o), ops._ptr(part_ml), ops._stream())
+        parts = torch.empty(n * n_heads * splits * (cache.head_dim + 2), dtype=torch.float32, device=q.device)
+    ops.fourbit().call("hos_attend4", q.data_ptr(), ops.dtype_code(q.dtype), q.stride(0), out.data_ptr(), out.stride(0), step.token_pos.data_ptr(),
+                       step.token_seq.data_ptr(), step.seq_slot.data_ptr(), ops.paged4(cache), n, n_heads, scale, softcap, window or 0, share, splits,
+                       parts.data_ptr() if parts is not None else None, ops._stream())

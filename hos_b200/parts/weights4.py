@@ -6,6 +6,7 @@ other matrix, with rows in bfloat16 or in 32 bits.
 operand registers of the tensor cores want them (csrc/fourbit.cuh)."""
 from __future__ import annotations
 
+import ctypes
 from typing import Optional
 
 import torch
@@ -20,6 +21,8 @@ class Weight4:
     def __init__(self, codes: torch.Tensor, records: torch.Tensor, n: int, k: int, group: int, blocks: int, zeros: bool):
         self.codes, self.records = codes, records
         self.n, self.k, self.group, self.blocks, self.zeros = n, k, group, blocks, zeros
+        self._matrix = ops.Matrix4(codes.data_ptr(), records.data_ptr(), n, k, group, int(zeros), int(blocks == 2))
+        self._address = ctypes.addressof(self._matrix)
 
     @property
     def shape(self):
@@ -97,17 +100,16 @@ class Weight4:
         gated = epilogue == ops.EPI_GATED
         if epilogue not in (ops.EPI_NONE, ops.EPI_GATED) or bias is not None:
             raise KernelError("products with 4-bit weights have no epilogue but the gated one")
-        if gated != (self.blocks == 2):
+        if self.blocks != (2 if gated else 1):
             raise KernelError(f"a {'gated' if gated else 'plain'} product is asked of {self.blocks} matrices")
         ops._check_rows(x, "left operand")
         if x.shape[1] != self.k:
             raise KernelError(f"product with 4-bit weights: rows of {x.shape[1]} numbers, weights of {self.k}")
         if out is None:
-            out = torch.empty((x.shape[0], self.n), dtype=out_dtype or x.dtype, device=x.device)
+            out = x.new_empty((x.shape[0], self.n), dtype=out_dtype or x.dtype)
         else:
             ops._check_rows(out, "product")
             if tuple(out.shape) != (x.shape[0], self.n):
                 raise KernelError(f"product with 4-bit weights: the output is {tuple(out.shape)}, not {(x.shape[0], self.n)}")
-        if x.shape[0]:
-            ops.product4(x, self.codes, self.records, out, self.group, self.zeros, gated, act, cap)
+        ops.product4(x, self._address, out, act, cap)
         return out
