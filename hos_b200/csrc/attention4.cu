@@ -128,14 +128,15 @@ __device__ __forceinline__ void mma_plain(float (&d)[4], const uint32_t (&a)[4],
 //
 // A CTA takes a share of the pages of one (row, kv head, 8 heads); its warps take 16 keys in turn, each through a ring of its own that
 // cp.async fills, so that no barrier stands in the walk.  Running maxima are a warp's own and are raised when a score passes them by
-// 2^8.  The warps merge through shared memory, the shares through a workspace and attend4_merge_kernel.
-constexpr int kAttendWarps = 8, kMaxSharePages = 256;
+// 2^8.  The warps merge through shared memory; up to 8 shares are a cluster and merge through its shared memory, more through a
+// workspace and attend4_merge_kernel.
+constexpr int kAttendWarps = 8, kMaxSharePages = 256, kMaxShares = 1024, kClusterShares = 8;
 
 template <int DIM> struct Attend4 {
     static constexpr int kGroups = DIM / 64;
     static constexpr int kCodes = kGroups * kBlockBytes, kMeta = 64 * kGroups;          // of 16 keys, or values
     static constexpr int kStage = 2 * (kCodes + kMeta);
-    static constexpr int kRing = DIM >= 192 ? 3 : (DIM == 128 ? 5 : 8);
+    static constexpr int kRing = DIM == 256 ? 2 : (DIM == 192 ? 3 : (DIM == 128 ? 4 : 8));      // two CTAs to an SM
     static constexpr int kPitch = DIM + 4;                                              // floats of a head's sums in shared memory
     static constexpr int kRingBytes = kAttendWarps * kRing * kStage, kSumBytes = kAttendWarps * 8 * kPitch * 4;
     static constexpr int kShared = kRingBytes > kSumBytes ? kRingBytes : kSumBytes;
@@ -152,6 +153,20 @@ __device__ __forceinline__ void load_meta(uint32_t at, uint32_t (&m)[GROUPS]) {
 #pragma unroll
         for (int i = 0; i < GROUPS; ++i) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(m[i]) : "r"(at + 4 * i));
     }
+}
+
+__device__ __forceinline__ uint32_t peer_at(uint32_t at, int rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float peer_float(uint32_t at) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ void cluster_meet() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // The pages of a row's keys, first and one past the last, and how many make a share: more than planned where the row is longer than
@@ -188,14 +203,18 @@ attend4_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out,
     const int per = n_heads / c.n_kv_heads, chunks = (per + 7) / 8, kvh = blockIdx.y / chunks, chunk = blockIdx.y % chunks;
     const int h0 = kvh * per + chunk * 8, nh = min(8, per - chunk * 8);
     const int seq = token_seq[n];
-    if (seq < 0) {                                             // padding: zeros (the merge writes them where there are shares)
-        if (splits == 1)
-            for (int i = threadIdx.x; i < nh * DIM; i += blockDim.x) out[(size_t)n * out_stride + (size_t)h0 * DIM + i] = from_float<T>(0.f);
-        return;
-    }
     const KeySpan span = key_span(token_pos[n], window, share, splits);
-    const int p0 = span.page0 + split * span.share, p1 = min(span.page1, p0 + span.share);
-    if (p0 >= p1) return;
+    const int p0 = span.page0 + split * span.share, p1 = seq < 0 ? p0 : min(span.page1, p0 + span.share);      // a padding row has no pages
+    const bool clustered = splits > 1 && part_o == nullptr;
+    float* sums = (float*)ring_bytes;                          // once the walk is over
+    if (p0 >= p1) {
+        if (!clustered) {
+            if (splits == 1)                                   // padding: zeros (the merge writes them where there are shares)
+                for (int i = threadIdx.x; i < nh * DIM; i += blockDim.x) out[(size_t)n * out_stride + (size_t)h0 * DIM + i] = from_float<T>(0.f);
+            return;
+        }
+        if (threadIdx.x < 8) cta_ml[threadIdx.x] = make_float2(-INFINITY, 0.f);
+    } else {
     const int* table = c.page_table + (size_t)seq_slot[seq] * c.table_stride;
     auto page_of = [&](int p) { return table[c.ring_pages > 0 ? p % c.ring_pages : p]; };
     for (int i = threadIdx.x; i < min(p1 - p0, kMaxSharePages); i += blockDim.x) ids[i] = page_of(p0 + i);
@@ -396,7 +415,6 @@ attend4_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out,
         warp_ml[warp][2 * t4 + 1] = make_float2(best[1], sum[1]);
     }
     __syncthreads();                                           // the rings are done with: the sums go where they were
-    float* sums = (float*)ring_bytes;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         if (2 * t4 + h < nh) {
@@ -427,12 +445,32 @@ attend4_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out,
         for (int w = 0; w < kAttendWarps; ++w) v = fmaf(warp_f[w][h], sums[(w * 8 + h) * A::kPitch + d], v);
         if (splits == 1) {
             out[(size_t)n * out_stride + (size_t)(h0 + h) * DIM + d] = from_float<T>(v / cta_ml[h].y);
+        } else if (clustered) {
+            sums[h * A::kPitch + d] = v;                       // nobody else reads the first warp's
         } else {
             const size_t at = ((size_t)n * n_heads + h0 + h) * splits + split;
             part_o[at * DIM + d] = v;
             if (d == 0) part_ml[at] = cta_ml[h];
         }
     }
+    }
+    if (!clustered) return;
+    cluster_meet();
+    for (int i = split * blockDim.x + threadIdx.x; i < nh * DIM; i += splits * blockDim.x) {
+        const int h = i / DIM, d = i % DIM;
+        const uint32_t ml_at = smem_u32(&cta_ml[h]), v_at = smem_u32(&sums[h * A::kPitch + d]);
+        float m = -INFINITY, l = 0.f, v = 0.f;
+        for (int s = 0; s < splits; ++s) m = fmaxf(m, peer_float(peer_at(ml_at, s)));
+        for (int s = 0; s < splits; ++s) {
+            const float pm = peer_float(peer_at(ml_at, s)), pl = peer_float(peer_at(ml_at + 4, s));
+            if (pl == 0.f) continue;                           // a share without keys: its sums are not there
+            const float f = pm == m ? 1.f : ex2_approx(pm - m);
+            l = fmaf(f, pl, l);
+            v = fmaf(f, peer_float(peer_at(v_at, s)), v);
+        }
+        out[(size_t)n * out_stride + (size_t)(h0 + h) * DIM + d] = from_float<T>(seq < 0 ? 0.f : v / l);
+    }
+    cluster_meet();                                            // nobody leaves while its sums are read
 }
 
 // The shares of a (row, head) added up: DIM threads, one a number.
@@ -440,6 +478,8 @@ template <typename T, int DIM>
 __global__ void __launch_bounds__(DIM)
 attend4_merge_kernel(T* __restrict__ out, long long out_stride, const int* __restrict__ token_pos, const int* __restrict__ token_seq, int n_heads, int window,
                      int share, int splits, const float* __restrict__ part_o, const float2* __restrict__ part_ml) {
+    __shared__ float factor[kMaxShares];
+    __shared__ float in_total;
     pdl_enter();
     const int n = blockIdx.x / n_heads, h = blockIdx.x % n_heads, d = threadIdx.x;
     T* to = out + (size_t)n * out_stride + (size_t)h * DIM + d;
@@ -450,15 +490,24 @@ attend4_merge_kernel(T* __restrict__ out, long long out_stride, const int* __res
     const KeySpan span = key_span(token_pos[n], window, share, splits);
     const int parts = (span.page1 - span.page0 + span.share - 1) / span.share;
     const size_t at = (size_t)blockIdx.x * splits;
-    float m = -INFINITY, l = 0.f, v = 0.f;
-    for (int s = 0; s < parts; ++s) m = fmaxf(m, part_ml[at + s].x);
-    for (int s = 0; s < parts; ++s) {
-        const float2 ml = part_ml[at + s];
-        const float f = ml.x == m ? 1.f : ex2_approx(ml.x - m);
-        l = fmaf(f, ml.y, l);
-        v = fmaf(f, part_o[(at + s) * DIM + d], v);
+    if (d < 32) {                                              // one warp: every share's weight
+        float m = -INFINITY, l = 0.f;
+        for (int s = d; s < parts; s += 32) m = fmaxf(m, part_ml[at + s].x);
+        m = warp_max(m);
+        for (int s = d; s < parts; s += 32) {
+            const float2 ml = part_ml[at + s];
+            const float f = ml.x == m ? 1.f : ex2_approx(ml.x - m);
+            factor[s] = f;
+            l = fmaf(f, ml.y, l);
+        }
+        l = warp_sum(l);
+        if (d == 0) in_total = 1.f / l;
     }
-    *to = from_float<T>(v / l);
+    __syncthreads();
+    float v = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < parts; ++s) v = fmaf(factor[s], part_o[(at + s) * DIM + d], v);
+    *to = from_float<T>(v * in_total);
 }
 
 template <typename T, int DIM>
@@ -473,9 +522,22 @@ int launch_attend4(const void* q, long long q_stride, void* out, long long out_s
         set = true;
     }
     const int per = n_heads / c.n_kv_heads, chunks = (per + 7) / 8;
-    launch_pdl(kernel, dim3((unsigned)((long long)n_tokens * splits), (unsigned)(c.n_kv_heads * chunks)), dim3(kAttendWarps * 32), smem, stream, (const T*)q,
-               q_stride, (T*)out, out_stride, token_pos, token_seq, seq_slot, c, n_heads, scale, cap, window, share, splits, part_o, part_ml);
-    if (splits > 1)
+    const bool clustered = splits > 1 && part_o == nullptr;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((long long)n_tokens * splits), (unsigned)(c.n_kv_heads * chunks));
+    cfg.blockDim = dim3(kAttendWarps * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim = {(unsigned)splits, 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = clustered ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, kernel, (const T*)q, q_stride, (T*)out, out_stride, token_pos, token_seq, seq_slot, c, n_heads, scale, cap, window, share, splits,
+                       part_o, part_ml);
+    if (splits > 1 && !clustered)
         launch_pdl(attend4_merge_kernel<T, DIM>, dim3((unsigned)((long long)n_tokens * n_heads)), dim3(DIM), 0, stream, (T*)out, out_stride, token_pos, token_seq,
                    n_heads, window, share, splits, (const float*)part_o, (const float2*)part_ml);
     return check_launch("attend4");
@@ -504,16 +566,16 @@ extern "C" int hos_store4(const void* rows, int dtype, long long stride, void* h
     return check_launch("store4");
 }
 
-// Every row alone over its pages, `share` of them to a CTA: `splits` shares cover the longest row's.  More than one: `parts`
-// holds n_tokens * n_heads * splits * (head_dim + 2) 32-bit numbers.
+// Every row alone over its pages, `share` of them to a CTA: `splits` shares cover the longest row's.  2 to 8 without
+// `parts` are a cluster; else more than one need `parts`, n_tokens * n_heads * splits * (head_dim + 2) 32-bit numbers.
 extern "C" int hos_attend4(const void* q, int dtype, long long q_stride, void* out, long long out_stride, const int* token_pos, const int* token_seq,
                            const int* seq_slot, const void* cache, int n_tokens, int n_heads, float scale, float cap, int window, int share, int splits,
                            float* parts, cudaStream_t stream) {
     if (n_tokens <= 0) return 0;
     HOS_CHECK_PAGED4("attend4");
     if (n_heads <= 0 || n_heads % n_kv_heads) HOS_REFUSE("attend4: %d query heads over %d kv heads", n_heads, n_kv_heads);
-    if (share < 1 || share > kMaxSharePages || splits < 1) HOS_REFUSE("attend4: %d shares of %d pages (1..%d)", splits, share, kMaxSharePages);
-    if (splits > 1 && parts == nullptr) HOS_REFUSE("attend4: shares need a workspace");
+    if (share < 1 || splits < 1 || splits > kMaxShares) HOS_REFUSE("attend4: %d shares of %d pages (1..%d shares)", splits, share, kMaxShares);
+    if (splits > kClusterShares && parts == nullptr) HOS_REFUSE("attend4: %d shares need a workspace", splits);
     if ((long long)n_tokens * splits > 0x7fffffffll || (long long)n_tokens * n_heads > 0x7fffffffll) HOS_REFUSE("attend4: %d rows in %d shares", n_tokens, splits);
     const size_t n_parts = (size_t)n_tokens * n_heads * splits;
     float2* part_ml = (float2*)parts;                          // pairs first: they want 8 bytes' alignment

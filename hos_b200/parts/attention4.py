@@ -48,23 +48,29 @@ def store(rows: torch.Tensor, step, cache: ops.PagedKVArgs, held: Optional[torch
                        step.seq_len_after.data_ptr(), ops.paged4(cache), n, ops._stream())
 
 
-MAX_SHARE_PAGES = 256          # page numbers that a CTA keeps
+MAX_SHARES, CLUSTER_SHARES = 1024, 8
 
 
 def shares(rows: int, kv_items: int, longest: int, window: Optional[int], fill: float = 1.0):
-    """(pages of a share, shares of a row): `rows` rows times `kv_items` (kv heads, times the eights of query heads that share one) over
-    up to `longest` keys.  Two CTAs fit an SM: rows that leave CTAs free are cut into as many shares as fill them; many rows of
-    unequal lengths (`fill`: the sum of the keys over rows * the longest) into shares of up to 32 pages, which CTAs take as they come free."""
+    """(pages of a share, shares of a row, whether the shares are a cluster): `rows` rows times `kv_items` (kv heads, times the eights of
+    query heads that share one) over up to `longest` keys.  Two CTAs fit an SM: rows that leave CTAs free are cut into as many shares
+    as fill them; many rows of unequal lengths (`fill`: the sum of the keys over rows * the longest) into shares of up to 32 pages,
+    which CTAs take as they come free, not as clusters, whose CTAs without keys would wait for the others.  Up to 8 shares of few rows
+    merge as a cluster; more cost a second kernel, about the time of 4 pages, and have to save that."""
     span = min(longest, window) if window else longest
     pages = max(1, -(-span // ops.PAGE_TOKENS) + (1 if window and longest > window else 0))
     places, items = 2 * ops.sm_count(), max(1, rows * kv_items)
-    if items * fill < places:
-        splits = max(1, int(places // max(1.0, items * fill)))
-        share = -(-pages // splits)
+    few = items * fill < places
+    if few:
+        share = -(-pages // max(1, int(places // max(1.0, items * fill))))
     else:
         share = pages if fill > 0.9 and items % places == 0 else 32
-    share = max(1, min(share, pages, MAX_SHARE_PAGES))
-    return share, -(-pages // share)
+    share = max(1, min(share, pages), -(-pages // MAX_SHARES))
+    least = -(-pages // CLUSTER_SHARES)
+    if few and share < least <= share + 4:
+        share = least
+    splits = -(-pages // share)
+    return share, splits, few and 1 < splits <= CLUSTER_SHARES
 
 
 def attend(q: torch.Tensor, out: torch.Tensor, step, cache: ops.PagedKVArgs, n_heads: int, scale: float, softcap: float = 0.0,
@@ -83,9 +89,9 @@ def attend(q: torch.Tensor, out: torch.Tensor, step, cache: ops.PagedKVArgs, n_h
     plan = step.shared.get(key)                      # once per step and kind of layer
     if plan is None:
         plan = step.shared[key] = shares(n, kv * -(-(n_heads // kv) // 8), step.max_len_after, window, step.fill_for(window))
-    share, splits = plan
+    share, splits, cluster = plan
     parts = None
-    if splits > 1:
+    if splits > 1 and not cluster:
         parts = torch.empty(n * n_heads * splits * (cache.head_dim + 2), dtype=torch.float32, device=q.device)
     ops.fourbit().call("hos_attend4", q.data_ptr(), ops.dtype_code(q.dtype), q.stride(0), out.data_ptr(), out.stride(0), step.token_pos.data_ptr(),
                        step.token_seq.data_ptr(), step.seq_slot.data_ptr(), ops.paged4(cache), n, n_heads, scale, softcap, window or 0, share, splits,
