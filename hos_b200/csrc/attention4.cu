@@ -118,7 +118,8 @@ __device__ __forceinline__ void mma_plain(float (&d)[4], const uint32_t (&a)[4],
 // ---- attention of single rows --------------------------------------------------------------------------------------
 // Bound by reading the held keys and values once, and close behind by the instructions that make operands of codes.
 //
-// Scores: S^T = K Q^T with 16 keys as the MMA's rows and up to 8 query heads of a kv head as its columns.  The score of a key is
+// Scores: S^T = K Q^T with 16 keys as the MMA's rows and up to 8 query heads of a kv head as its columns (fewer heads: of several
+// neighbouring rows of a sequence, each with its own mask).  The score of a key is
 // sum_g (s_g (sum_{d in g} q c') - 136 s_g sum q + m_g sum q) over its groups of 64, c' = 128 + c + 8 the operand as codes_to_bf16 makes
 // it without subtracting: a group's product starts at -136 sum q and is multiplied by the key's scale, in 32 bits; neither scale nor
 // middle is rounded into an operand.  Values: O^T = V^T P^T with 16 numbers of a head as rows, P times the value's scale rounded to
@@ -126,7 +127,7 @@ __device__ __forceinline__ void mma_plain(float (&d)[4], const uint32_t (&a)[4],
 // group and head, in 32 bits beside it.  The scores' registers, transposed eight by eight, are P's operand.
 // Rows in 32 bits: q, and p times the scale, are three bfloat16 numbers each, exactly, and the codes are subtracted first.
 //
-// A CTA takes a share of the pages of one (row, kv head, 8 heads); its warps take 16 keys in turn, each through a ring of its own that
+// A CTA takes a share of the pages of one (row or neighbouring rows, kv head, 8 heads); its warps take 16 keys in turn, each through a ring of its own that
 // cp.async fills, so that no barrier stands in the walk.  Running maxima are a warp's own and are raised when a score passes them by
 // 2^8.  The warps merge through shared memory; up to 8 shares are a cluster and merge through its shared memory, more through a
 // workspace and attend4_merge_kernel.
@@ -169,24 +170,12 @@ __device__ __forceinline__ void cluster_meet() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// The pages of a row's keys, first and one past the last, and how many make a share: more than planned where the row is longer than
-// the plan thought.
-struct KeySpan { int first, pos, page0, page1, share; };
-__device__ __forceinline__ KeySpan key_span(int pos, int window, int share, int splits) {
-    KeySpan k;
-    k.pos = pos;
-    k.first = window > 0 ? max(0, pos - window + 1) : 0;
-    k.page0 = k.first / kPageTokens;
-    k.page1 = pos / kPageTokens + 1;
-    k.share = max(share, (k.page1 - k.page0 + splits - 1) / splits);
-    return k;
-}
-
-template <typename T, int DIM>
+// GROUPS: rows come as groups (row_groups); without, column j is simply head h0 + j of the row.
+template <typename T, int DIM, bool GROUPS>
 __global__ void __launch_bounds__(kAttendWarps * 32, 2)
 attend4_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out, long long out_stride, const int* __restrict__ token_pos,
-               const int* __restrict__ token_seq, const int* __restrict__ seq_slot, Paged4 c, int n_heads, float scale, float cap, int window, int share, int splits,
-               float* __restrict__ part_o, float2* __restrict__ part_ml) {
+               const int* __restrict__ token_seq, const int* __restrict__ seq_slot, const int* __restrict__ token_slot, const int2* __restrict__ row_groups, Paged4 c,
+               int n_heads, float scale, float cap, int window, int share, int splits, float* __restrict__ part_o, float2* __restrict__ part_ml) {
     using A = Attend4<DIM>;
     constexpr int G = A::kGroups, kTerms = sizeof(T) == 4 ? 3 : 1, kTiles = DIM / 16;
     constexpr bool kExact = kTerms == 3;
@@ -199,60 +188,40 @@ attend4_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out,
     __shared__ float2 cta_ml[8];
     pdl_enter();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-    const int n = blockIdx.x / splits, split = blockIdx.x % splits;
-    const int per = n_heads / c.n_kv_heads, chunks = (per + 7) / 8, kvh = blockIdx.y / chunks, chunk = blockIdx.y % chunks;
-    const int h0 = kvh * per + chunk * 8, nh = min(8, per - chunk * 8);
-    const int seq = token_seq[n];
-    const KeySpan span = key_span(token_pos[n], window, share, splits);
-    const int p0 = span.page0 + split * span.share, p1 = seq < 0 ? p0 : min(span.page1, p0 + span.share);      // a padding row has no pages
+    const int split = blockIdx.x % splits;
+    const int2 rows = GROUPS ? row_groups[blockIdx.x / splits] : make_int2(blockIdx.x / splits, 1);      // the first, and how many
+    const int n = rows.x, per = n_heads / c.n_kv_heads, chunks = (per + 7) / 8, kvh = blockIdx.y / chunks, chunk = blockIdx.y % chunks;
+    const int h0 = kvh * per + chunk * 8, nh = min(8, per - chunk * 8), columns = nh * rows.y;
+    auto row_at = [&](int column) { return GROUPS ? column / nh : 0; };                     // column j: head h0 + j % nh of row n + j / nh
+    auto head_at = [&](int column) { return GROUPS ? column % nh : column; };
+    const int seq = token_seq[n], known_slot = token_slot != nullptr ? token_slot[n] : -1;
+    const int pos0 = token_pos[n], last = pos0 + rows.y - 1, first = window > 0 ? max(0, pos0 - window + 1) : 0;
+    // the pages of the keys, from page0 to before page1; where there are more than planned a share is longer
+    const int page0 = first / kPageTokens, page1 = last / kPageTokens + 1, pages = max(share, (page1 - page0 + splits - 1) / splits);
+    const int p0 = page0 + split * pages, p1 = seq < 0 ? p0 : min(page1, p0 + pages);      // a padding row has no pages
     const bool clustered = splits > 1 && part_o == nullptr;
     float* sums = (float*)ring_bytes;                          // once the walk is over
-    if (p0 >= p1) {
-        if (!clustered) {
-            if (splits == 1)                                   // padding: zeros (the merge writes them where there are shares)
-                for (int i = threadIdx.x; i < nh * DIM; i += blockDim.x) out[(size_t)n * out_stride + (size_t)h0 * DIM + i] = from_float<T>(0.f);
+    if (p0 >= p1) {                                            // a share without keys says so; a padding row becomes zeros
+        if (splits == 1) {
+            for (int i = threadIdx.x; i < nh * DIM; i += blockDim.x) out[(size_t)n * out_stride + (size_t)h0 * DIM + i] = from_float<T>(0.f);
             return;
         }
         if (threadIdx.x < 8) cta_ml[threadIdx.x] = make_float2(-INFINITY, 0.f);
-    } else {
-    const int* table = c.page_table + (size_t)seq_slot[seq] * c.table_stride;
-    auto page_of = [&](int p) { return table[c.ring_pages > 0 ? p % c.ring_pages : p]; };
-    for (int i = threadIdx.x; i < min(p1 - p0, kMaxSharePages); i += blockDim.x) ids[i] = page_of(p0 + i);
-    // the heads' numbers as operands, and their sums over 64
-    const T* q_row = q + (size_t)n * q_stride + (size_t)h0 * DIM;
-    for (int i = threadIdx.x; i < G * 64; i += blockDim.x) {
-        const int l = i & 31, half = (i >> 5) & 1, grp = i >> 6, head = l >> 2, d = grp * 64 + (l & 3) * 16 + half * 8;
-        float v[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = head < nh ? to_float(q_row[head * DIM + d + j]) : 0.f;
-#pragma unroll
-        for (int term = 0; term < kTerms; ++term) {
-            uint32_t w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                w[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
-                v[2 * j] -= bf16_lo(w[j]);
-                v[2 * j + 1] -= bf16_hi(w[j]);
-            }
-            q_frag[term][grp][half][l] = make_uint4(w[0], w[1], w[2], w[3]);
+        if (!clustered) {
+            if (threadIdx.x < columns)
+                part_ml[((size_t)(n + row_at(threadIdx.x)) * n_heads + h0 + head_at(threadIdx.x)) * splits + split] = make_float2(-INFINITY, 0.f);
+            return;
         }
-    }
-    for (int i = warp; i < G * 8; i += kAttendWarps) {
-        const int head = i & 7, grp = i >> 3;
-        float v = head < nh ? to_float(q_row[head * DIM + grp * 64 + lane]) + to_float(q_row[head * DIM + grp * 64 + 32 + lane]) : 0.f;
-        v = warp_sum(v);
-        if (lane == 0) q_sum[grp][head] = v;
-    }
-    __syncthreads();
-
-    const int b0 = max(span.first, p0 * kPageTokens) >> 4, b1 = min(span.pos, p1 * kPageTokens - 1) >> 4;      // blocks of 16 keys, b1 the last
+    } else {
+    const int* table = c.page_table + (size_t)(token_slot != nullptr ? known_slot : seq_slot[seq]) * c.table_stride;
+    auto page_of = [&](int p) { return table[c.ring_pages > 0 ? p % c.ring_pages : p]; };
+    const int b0 = max(first, p0 * kPageTokens) >> 4, b1 = min(last, p1 * kPageTokens - 1) >> 4;      // blocks of 16 keys, b1 the last
     const uint32_t ring = smem_u32(ring_bytes) + warp * A::kRing * A::kStage;
     int to_fetch = b0 + warp;
-    auto fetch = [&](uint32_t to) {
+    auto fetch = [&](uint32_t to, bool known) {
         if (to_fetch <= b1) {
-            const int p = to_fetch >> 2;
-            const size_t tile = ((size_t)(p - p0 < kMaxSharePages ? ids[p - p0] : page_of(p)) * c.n_kv_heads + kvh) * tile4_bytes(DIM);
-            const int in = to_fetch & 3;
+            const int p = to_fetch >> 2, in = to_fetch & 3;
+            const size_t tile = ((size_t)(known && p - p0 < kMaxSharePages ? ids[p - p0] : page_of(p)) * c.n_kv_heads + kvh) * tile4_bytes(DIM);
             const uint8_t *k = c.k_pages + tile, *v = c.v_pages + tile;
 #pragma unroll
             for (int i = 0; i < G; ++i) {
@@ -268,19 +237,48 @@ attend4_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out,
         copies_commit();
     };
 #pragma unroll
-    for (int i = 0; i < A::kRing - 1; ++i) fetch(ring + i * A::kStage);
+    for (int i = 0; i < A::kRing - 1; ++i) fetch(ring + i * A::kStage, false);      // before the page numbers are in shared memory
+    for (int i = threadIdx.x; i < min(p1 - p0, kMaxSharePages); i += blockDim.x) ids[i] = page_of(p0 + i);
+    // the columns' numbers as operands, and their sums over 64
+    const T* q_row = q + (size_t)n * q_stride + (size_t)h0 * DIM;
+    for (int i = threadIdx.x; i < G * 64; i += blockDim.x) {
+        const int l = i & 31, half = (i >> 5) & 1, grp = i >> 6, head = l >> 2, d = grp * 64 + (l & 3) * 16 + half * 8;
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = head < columns ? to_float(q_row[row_at(head) * q_stride + head_at(head) * DIM + d + j]) : 0.f;
+#pragma unroll
+        for (int term = 0; term < kTerms; ++term) {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                w[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+                v[2 * j] -= bf16_lo(w[j]);
+                v[2 * j + 1] -= bf16_hi(w[j]);
+            }
+            q_frag[term][grp][half][l] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+    for (int i = warp; i < G * 8; i += kAttendWarps) {
+        const int head = i & 7, grp = i >> 3;
+        const T* from = q_row + row_at(head) * q_stride + head_at(head) * DIM + grp * 64 + lane;
+        float v = head < columns ? to_float(from[0]) + to_float(from[32]) : 0.f;
+        v = warp_sum(v);
+        if (lane == 0) q_sum[grp][head] = v;
+    }
+    __syncthreads();
 
     float o[kTiles][4], mid[G][2], best[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 #pragma unroll
     for (int i = 0; i < G; ++i) mid[i][0] = mid[i][1] = 0.f;
+    const int row_of[2] = {row_at(2 * t4), row_at(2 * t4 + 1)};     // of a lane's columns
     const float scale2 = scale * 1.44269504f, cap2 = cap * 1.44269504f, in_cap = cap > 0.f ? 2.f * scale2 / cap : 0.f;
     uint32_t slot = ring, before = ring + (A::kRing - 1) * A::kStage;
     for (int b = b0 + warp; b <= b1; b += kAttendWarps) {
         copies_wait<A::kRing - 2>();
         __syncwarp();
-        fetch(before);                                         // the place that the last block has left
+        fetch(before, true);                                   // the place that the last block has left
         uint32_t km[2][G], vm[2][G];                           // of the keys g and g + 8
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
@@ -288,16 +286,14 @@ attend4_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out,
             load_meta<G>(slot + 2 * A::kCodes + A::kMeta + (g + 8 * r) * 4 * G, vm[r]);
         }
         const int key = b * 16 + g;
-        const bool edge = b * 16 < span.first || b * 16 + 15 > span.pos;
-        bool hidden[2] = {false, false};
-        if (edge) {                                            // what is hidden may be anything: its scales and middles become zeros
+        // some column does not see some of these keys: what is hidden from a column may be anything
+        const bool edge = b * 16 + 15 > pos0 || (window > 0 && b * 16 <= last - window);
+        bool hidden[4] = {false, false, false, false};
+        if (edge) {
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                hidden[r] = key + 8 * r < span.first || key + 8 * r > span.pos;
-#pragma unroll
-                for (int i = 0; i < G; ++i) {
-                    if (hidden[r]) km[r][i] = vm[r][i] = 0u;
-                }
+            for (int e = 0; e < 4; ++e) {
+                const int at = key + 8 * (e >> 1), mine = pos0 + (GROUPS ? row_of[e & 1] : 0);
+                hidden[e] = at > mine || (window > 0 && at <= mine - window);
             }
         }
         float s[4] = {0.f, 0.f, 0.f, 0.f};
@@ -340,15 +336,15 @@ attend4_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out,
             } else {
                 s[e] *= scale2;
             }
-            if (hidden[e >> 1]) s[e] = -INFINITY;
+            if (hidden[e]) s[e] = -INFINITY;
         }
         float top[2] = {fmaxf(s[0], s[2]), fmaxf(s[1], s[3])};
-#pragma unroll
-        for (int off = 4; off < 32; off <<= 1) {
-            top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], off));
-            top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], off));
-        }
         if (__any_sync(0xffffffffu, top[0] > best[0] + 8.f || top[1] > best[1] + 8.f)) {
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) {
+                top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], off));
+                top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], off));
+            }
             float f[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -366,7 +362,7 @@ attend4_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out,
         }
         float p[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) p[e] = ex2_approx(s[e] - best[e & 1]);
+        for (int e = 0; e < 4; ++e) p[e] = hidden[e] ? 0.f : ex2_approx(s[e] - best[e & 1]);      // a column may not have seen a key yet
         sum[0] += p[0] + p[2];
         sum[1] += p[1] + p[3];
 #pragma unroll
@@ -375,8 +371,8 @@ attend4_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out,
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const uint32_t sm = vm[e >> 1][i];
-                w[e] = p[e] * bf16_lo(sm);
-                mid[i][e & 1] = fmaf(p[e], bf16_hi(sm), mid[i][e & 1]);
+                w[e] = hidden[e] ? 0.f : p[e] * bf16_lo(sm);
+                mid[i][e & 1] = hidden[e] ? mid[i][e & 1] : fmaf(p[e], bf16_hi(sm), mid[i][e & 1]);
             }
             uint32_t pb[kTerms][2];
 #pragma unroll
@@ -417,7 +413,7 @@ attend4_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out,
     __syncthreads();                                           // the rings are done with: the sums go where they were
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        if (2 * t4 + h < nh) {
+        if (2 * t4 + h < columns) {
             float* to = sums + (warp * 8 + 2 * t4 + h) * A::kPitch;
 #pragma unroll
             for (int i = 0; i < kTiles; ++i) {
@@ -438,17 +434,18 @@ attend4_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out,
         cta_ml[threadIdx.x] = make_float2(m, l);
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < nh * DIM; i += blockDim.x) {
+    for (int i = threadIdx.x; i < columns * DIM; i += blockDim.x) {
         const int h = i / DIM, d = i % DIM;
+        const size_t row = n + row_at(h), head = h0 + head_at(h);
         float v = 0.f;
 #pragma unroll
         for (int w = 0; w < kAttendWarps; ++w) v = fmaf(warp_f[w][h], sums[(w * 8 + h) * A::kPitch + d], v);
         if (splits == 1) {
-            out[(size_t)n * out_stride + (size_t)(h0 + h) * DIM + d] = from_float<T>(v / cta_ml[h].y);
+            out[row * out_stride + head * DIM + d] = from_float<T>(v / cta_ml[h].y);
         } else if (clustered) {
             sums[h * A::kPitch + d] = v;                       // nobody else reads the first warp's
         } else {
-            const size_t at = ((size_t)n * n_heads + h0 + h) * splits + split;
+            const size_t at = (row * n_heads + head) * splits + split;
             part_o[at * DIM + d] = v;
             if (d == 0) part_ml[at] = cta_ml[h];
         }
@@ -456,7 +453,7 @@ attend4_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out,
     }
     if (!clustered) return;
     cluster_meet();
-    for (int i = split * blockDim.x + threadIdx.x; i < nh * DIM; i += splits * blockDim.x) {
+    for (int i = split * blockDim.x + threadIdx.x; i < columns * DIM; i += splits * blockDim.x) {
         const int h = i / DIM, d = i % DIM;
         const uint32_t ml_at = smem_u32(&cta_ml[h]), v_at = smem_u32(&sums[h * A::kPitch + d]);
         float m = -INFINITY, l = 0.f, v = 0.f;
@@ -468,7 +465,7 @@ attend4_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out,
             l = fmaf(f, pl, l);
             v = fmaf(f, peer_float(peer_at(v_at, s)), v);
         }
-        out[(size_t)n * out_stride + (size_t)(h0 + h) * DIM + d] = from_float<T>(seq < 0 ? 0.f : v / l);
+        out[(size_t)(n + row_at(h)) * out_stride + (size_t)(h0 + head_at(h)) * DIM + d] = from_float<T>(seq < 0 ? 0.f : v / l);
     }
     cluster_meet();                                            // nobody leaves while its sums are read
 }
@@ -476,46 +473,41 @@ attend4_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out,
 // The shares of a (row, head) added up: DIM threads, one a number.
 template <typename T, int DIM>
 __global__ void __launch_bounds__(DIM)
-attend4_merge_kernel(T* __restrict__ out, long long out_stride, const int* __restrict__ token_pos, const int* __restrict__ token_seq, int n_heads, int window,
-                     int share, int splits, const float* __restrict__ part_o, const float2* __restrict__ part_ml) {
+attend4_merge_kernel(T* __restrict__ out, long long out_stride, int n_heads, int splits, const float* __restrict__ part_o, const float2* __restrict__ part_ml) {
     __shared__ float factor[kMaxShares];
-    __shared__ float in_total;
+    __shared__ float total;
     pdl_enter();
     const int n = blockIdx.x / n_heads, h = blockIdx.x % n_heads, d = threadIdx.x;
-    T* to = out + (size_t)n * out_stride + (size_t)h * DIM + d;
-    if (token_seq[n] < 0) {
-        *to = from_float<T>(0.f);
-        return;
-    }
-    const KeySpan span = key_span(token_pos[n], window, share, splits);
-    const int parts = (span.page1 - span.page0 + span.share - 1) / span.share;
     const size_t at = (size_t)blockIdx.x * splits;
-    if (d < 32) {                                              // one warp: every share's weight
+    if (d < 32) {                                              // one warp: every share's weight, 0 for one without keys
         float m = -INFINITY, l = 0.f;
-        for (int s = d; s < parts; s += 32) m = fmaxf(m, part_ml[at + s].x);
+        for (int s = d; s < splits; s += 32) m = fmaxf(m, part_ml[at + s].x);
         m = warp_max(m);
-        for (int s = d; s < parts; s += 32) {
+        for (int s = d; s < splits; s += 32) {
             const float2 ml = part_ml[at + s];
-            const float f = ml.x == m ? 1.f : ex2_approx(ml.x - m);
+            const float f = ml.y == 0.f ? 0.f : (ml.x == m ? 1.f : ex2_approx(ml.x - m));
             factor[s] = f;
             l = fmaf(f, ml.y, l);
         }
         l = warp_sum(l);
-        if (d == 0) in_total = 1.f / l;
+        if (d == 0) total = l;
     }
     __syncthreads();
     float v = 0.f;
 #pragma unroll 8
-    for (int s = 0; s < parts; ++s) v = fmaf(factor[s], part_o[(at + s) * DIM + d], v);
-    *to = from_float<T>(v * in_total);
+    for (int s = 0; s < splits; ++s) {
+        const float f = factor[s];
+        if (f != 0.f) v = fmaf(f, part_o[(at + s) * DIM + d], v);
+    }
+    out[(size_t)n * out_stride + (size_t)h * DIM + d] = from_float<T>(total == 0.f ? 0.f : v / total);      // a padding row has no share with keys
 }
 
-template <typename T, int DIM>
+template <typename T, int DIM, bool GROUPS>
 int launch_attend4(const void* q, long long q_stride, void* out, long long out_stride, const int* token_pos, const int* token_seq, const int* seq_slot,
-                   const Paged4& c, int n_tokens, int n_heads, float scale, float cap, int window, int share, int splits, float* part_o, float2* part_ml,
+                   const int* token_slot, const int2* row_groups, int n_groups, const Paged4& c, int n_tokens, int n_heads, float scale, float cap, int window, int share, int splits, float* part_o, float2* part_ml,
                    cudaStream_t stream) {
     constexpr int smem = Attend4<DIM>::kShared;
-    auto kernel = attend4_kernel<T, DIM>;
+    auto kernel = attend4_kernel<T, DIM, GROUPS>;
     static bool set = false;                                   // once per kernel: the attribute stays
     if (!set) {
         if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return check_launch("attend4");
@@ -524,7 +516,7 @@ int launch_attend4(const void* q, long long q_stride, void* out, long long out_s
     const int per = n_heads / c.n_kv_heads, chunks = (per + 7) / 8;
     const bool clustered = splits > 1 && part_o == nullptr;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((long long)n_tokens * splits), (unsigned)(c.n_kv_heads * chunks));
+    cfg.gridDim = dim3((unsigned)((long long)n_groups * splits), (unsigned)(c.n_kv_heads * chunks));
     cfg.blockDim = dim3(kAttendWarps * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
@@ -535,11 +527,11 @@ int launch_attend4(const void* q, long long q_stride, void* out, long long out_s
     attr[1].val.clusterDim = {(unsigned)splits, 1, 1};
     cfg.attrs = attr;
     cfg.numAttrs = clustered ? 2 : 1;
-    cudaLaunchKernelEx(&cfg, kernel, (const T*)q, q_stride, (T*)out, out_stride, token_pos, token_seq, seq_slot, c, n_heads, scale, cap, window, share, splits,
-                       part_o, part_ml);
+    cudaLaunchKernelEx(&cfg, kernel, (const T*)q, q_stride, (T*)out, out_stride, token_pos, token_seq, seq_slot, token_slot, row_groups, c, n_heads, scale, cap,
+                       window, share, splits, part_o, part_ml);
     if (splits > 1 && !clustered)
-        launch_pdl(attend4_merge_kernel<T, DIM>, dim3((unsigned)((long long)n_tokens * n_heads)), dim3(DIM), 0, stream, (T*)out, out_stride, token_pos, token_seq,
-                   n_heads, window, share, splits, (const float*)part_o, (const float2*)part_ml);
+        launch_pdl(attend4_merge_kernel<T, DIM>, dim3((unsigned)((long long)n_tokens * n_heads)), dim3(DIM), 0, stream, (T*)out, out_stride, n_heads,
+                   splits, (const float*)part_o, (const float2*)part_ml);
     return check_launch("attend4");
 }
 
@@ -566,11 +558,12 @@ extern "C" int hos_store4(const void* rows, int dtype, long long stride, void* h
     return check_launch("store4");
 }
 
-// Every row alone over its pages, `share` of them to a CTA: `splits` shares cover the longest row's.  2 to 8 without
+// token_slot: seq_slot[token_seq] of every row, or null.  row_groups: [n_groups][2], all rows as groups of neighbours (the first, how
+// many) of one sequence at consecutive positions, as many as times the heads of a kv head are at most 8; null: every row alone.  A group over its pages, `share` of them to a CTA: `splits` shares cover the longest row's.  2 to 8 without
 // `parts` are a cluster; else more than one need `parts`, n_tokens * n_heads * splits * (head_dim + 2) 32-bit numbers.
 extern "C" int hos_attend4(const void* q, int dtype, long long q_stride, void* out, long long out_stride, const int* token_pos, const int* token_seq,
-                           const int* seq_slot, const void* cache, int n_tokens, int n_heads, float scale, float cap, int window, int share, int splits,
-                           float* parts, cudaStream_t stream) {
+                           const int* seq_slot, const int* token_slot, const int* row_groups, int n_groups, const void* cache, int n_tokens, int n_heads, float scale, float cap, int window,
+                           int share, int splits, float* parts, cudaStream_t stream) {
     if (n_tokens <= 0) return 0;
     HOS_CHECK_PAGED4("attend4");
     if (n_heads <= 0 || n_heads % n_kv_heads) HOS_REFUSE("attend4: %d query heads over %d kv heads", n_heads, n_kv_heads);
@@ -580,7 +573,7 @@ extern "C" int hos_attend4(const void* q, int dtype, long long q_stride, void* o
     const size_t n_parts = (size_t)n_tokens * n_heads * splits;
     float2* part_ml = (float2*)parts;                          // pairs first: they want 8 bytes' alignment
     float* part_o = parts == nullptr ? nullptr : parts + 2 * n_parts;
-#define HOS_A4(T, D) return launch_attend4<T, D>(q, q_stride, out, out_stride, token_pos, token_seq, seq_slot, c, n_tokens, n_heads, scale, cap, window, share, splits, part_o, part_ml, stream)
+#define HOS_A4(T, D) return (row_groups != nullptr ? launch_attend4<T, D, true> : launch_attend4<T, D, false>)(q, q_stride, out, out_stride, token_pos, token_seq, seq_slot, token_slot, (const int2*)row_groups, row_groups != nullptr ? n_groups : n_tokens, c, n_tokens, n_heads, scale, cap, window, share, splits, part_o, part_ml, stream)
 #define HOS_A4_D(T) do { if (head_dim == 64) HOS_A4(T, 64); else if (head_dim == 128) HOS_A4(T, 128); else if (head_dim == 192) HOS_A4(T, 192); else HOS_A4(T, 256); } while (0)
     if (dtype == kF32) HOS_A4_D(float);
     else HOS_A4_D(bf16);

@@ -55,8 +55,9 @@ def shares(rows: int, kv_items: int, longest: int, window: Optional[int], fill: 
     """(pages of a share, shares of a row, whether the shares are a cluster): `rows` rows times `kv_items` (kv heads, times the eights of
     query heads that share one) over up to `longest` keys.  Two CTAs fit an SM: rows that leave CTAs free are cut into as many shares
     as fill them; many rows of unequal lengths (`fill`: the sum of the keys over rows * the longest) into shares of up to 32 pages,
-    which CTAs take as they come free, not as clusters, whose CTAs without keys would wait for the others.  Up to 8 shares of few rows
-    merge as a cluster; more cost a second kernel, about the time of 4 pages, and have to save that."""
+    which CTAs take as they come free.  Up to 8 shares of few rows of like lengths merge as a cluster (of unlike lengths the CTAs
+    without keys would wait for the others: 32 rows of up to 4,000 keys 19 us, through the workspace 15); more cost a second kernel,
+    about the time of 4 pages, and have to save that."""
     span = min(longest, window) if window else longest
     pages = max(1, -(-span // ops.PAGE_TOKENS) + (1 if window and longest > window else 0))
     places, items = 2 * ops.sm_count(), max(1, rows * kv_items)
@@ -70,7 +71,7 @@ def shares(rows: int, kv_items: int, longest: int, window: Optional[int], fill: 
     if few and share < least <= share + 4:
         share = least
     splits = -(-pages // share)
-    return share, splits, few and 1 < splits <= CLUSTER_SHARES
+    return share, splits, few and fill > 0.8 and 1 < splits <= CLUSTER_SHARES
 
 
 def attend(q: torch.Tensor, out: torch.Tensor, step, cache: ops.PagedKVArgs, n_heads: int, scale: float, softcap: float = 0.0,
@@ -85,14 +86,30 @@ def attend(q: torch.Tensor, out: torch.Tensor, step, cache: ops.PagedKVArgs, n_h
         raise KernelError(f"queries {tuple(q.shape)} and output {tuple(out.shape)} for {n_heads} heads of {cache.head_dim}")
     _check_step(n, step, "attend")
     kv = cache.n_kv_heads
-    key = ("shares of 4-bit pages", n, n_heads, kv, window, step.row_offset)
+    items = kv * -(-(n_heads // kv) // 8)
+    per = n_heads // kv
+    key = ("shares of 4-bit pages", n, items, per, window, step.row_offset)
     plan = step.shared.get(key)                      # once per step and kind of layer
     if plan is None:
-        plan = step.shared[key] = shares(n, kv * -(-(n_heads // kv) // 8), step.max_len_after, window, step.fill_for(window))
-    share, splits, cluster = plan
+        groups = _row_groups(step, n, per, q.device)
+        plan = step.shared[key] = (groups, *shares(n if groups is None else groups.shape[0], items, step.max_len_after, window, step.fill_for(window)))
+    groups, share, splits, cluster = plan
     parts = None
     if splits > 1 and not cluster:
         parts = torch.empty(n * n_heads * splits * (cache.head_dim + 2), dtype=torch.float32, device=q.device)
     ops.fourbit().call("hos_attend4", q.data_ptr(), ops.dtype_code(q.dtype), q.stride(0), out.data_ptr(), out.stride(0), step.token_pos.data_ptr(),
-                       step.token_seq.data_ptr(), step.seq_slot.data_ptr(), ops.paged4(cache), n, n_heads, scale, softcap, window or 0, share, splits,
-                       parts.data_ptr() if parts is not None else None, ops._stream())
+                       step.token_seq.data_ptr(), step.seq_slot.data_ptr(), step.token_slot.data_ptr() if step.token_slot is not None else None,
+                       groups.data_ptr() if groups is not None else None, groups.shape[0] if groups is not None else 0, ops.paged4(cache), n, n_heads,
+                       scale, softcap, window or 0, share, splits, parts.data_ptr() if parts is not None else None, ops._stream())
+
+
+def _row_groups(step, n: int, per: int, device):
+    """Rows of a sequence that share a walk over its keys, as many as the 8 columns of the kernel's products hold: [groups, 2] (the first
+    row, how many), or None where every row goes alone (also where which rows are whose is known on the device only)."""
+    together = 8 // per if per <= 8 else 1
+    if together < 2 or step.single_token or step.replayed or not step.cu_host:
+        return None
+    cu = step.cu_host
+    groups = [(row, min(together, cu[i + 1] - row)) for i in range(len(cu) - 1) for row in range(cu[i], cu[i + 1], together)]
+    groups += [(row, 1) for row in range(cu[-1], n)]              # padding rows
+    return torch.tensor(groups, dtype=torch.int32).pin_memory().to(device, non_blocking=True)
