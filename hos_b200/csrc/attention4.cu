@@ -25,86 +25,244 @@ __device__ __forceinline__ int page4_of(const Paged4& c, int slot, int pos) {
     return c.page_table[(size_t)slot * c.table_stride + (c.ring_pages > 0 ? lp % c.ring_pages : lp)];
 }
 
-__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+// ---- rows into pages ---------------------------------------------------------------------------------------------------
+// Four lanes hold 64 numbers of a row, 16 each.  Many rows are bound by reading them and writing what is held, and near that by the
+// dozen instructions a number costs.
+struct Numbers { float v[16]; };
+__device__ __forceinline__ Numbers load16(const float* p, bool vec) {
+    Numbers x;
+    if (vec) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = p[i];
+        for (int i = 0; i < 4; ++i) {
+            const float4 f = *(const float4*)(p + 4 * i);
+            x.v[4 * i] = f.x; x.v[4 * i + 1] = f.y; x.v[4 * i + 2] = f.z; x.v[4 * i + 3] = f.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x.v[i] = p[i];
+    }
+    return x;
 }
-__device__ __forceinline__ void load8(const bf16* p, float (&v)[8]) {
+__device__ __forceinline__ Numbers load16(const bf16* p, bool vec) {
+    Numbers x;
+    if (vec) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_float(p[i]);
+        for (int i = 0; i < 2; ++i) {
+            const uint4 w = *(const uint4*)(p + 8 * i);
+            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x.v[8 * i + 2 * j] = bf16_lo(u[j]);
+                x.v[8 * i + 2 * j + 1] = bf16_hi(u[j]);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x.v[i] = to_float(p[i]);
+    }
+    return x;
+}
+__device__ __forceinline__ void store16(float* p, const Numbers& x, bool vec) {
+    if (vec) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *(float4*)(p + 4 * i) = make_float4(x.v[4 * i], x.v[4 * i + 1], x.v[4 * i + 2], x.v[4 * i + 3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) p[i] = x.v[i];
+    }
+}
+__device__ __forceinline__ void store16(bf16* p, const Numbers& x, bool vec) {
+    if (vec) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            *(uint4*)(p + 8 * i) = make_uint4(pack_bf16(x.v[8 * i], x.v[8 * i + 1]), pack_bf16(x.v[8 * i + 2], x.v[8 * i + 3]),
+                                              pack_bf16(x.v[8 * i + 4], x.v[8 * i + 5]), pack_bf16(x.v[8 * i + 6], x.v[8 * i + 7]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) p[i] = from_float<bf16>(x.v[i]);
+    }
 }
 
-// Eight lanes hold 64 numbers, eight each: scale, middle and codes.
-__device__ __forceinline__ void quantise64(const float (&x)[8], float& s, float& m, int (&c)[8]) {
-    float lo = x[0], hi = x[0];
-    bool fine = true;
+// Scale and middle of 64 numbers that four lanes hold, their codes as words (eight codes each, as a word of keys holds them), and what
+// is held in the numbers' place.  The quotient by Markstein's correction (IA-64 and Elementary Functions, 2000): with r = 1 / s rounded and
+// q near y / s, q + (y - q s) r rounded once is y / s rounded, for numbers whose parts stay normal; others are divided.
+__device__ __forceinline__ void quantise64(Numbers& x, uint32_t& scale_middle, uint32_t (&w)[2]) {
+    float lo = x.v[0], hi = x.v[0], odd = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        lo = fminf(lo, x[i]);
-        hi = fmaxf(hi, x[i]);
-        fine = fine && isfinite(x[i]);
+    for (int i = 0; i < 16; ++i) {
+        lo = fminf(lo, x.v[i]);
+        hi = fmaxf(hi, x.v[i]);
+        odd = fmaf(x.v[i], 0.f, odd);                          // NaN after an infinity or a NaN
     }
-    float odd = fine ? 0.f : 1.f;
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        odd = fmaxf(odd, __shfl_xor_sync(0xffffffffu, odd, o));
-    }
-    s = to_float(__float2bfloat16_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f)));
-    if (!(s >= 1.17549435e-38f)) s = 0.f;            // subnormal or 0 (a NaN is caught below)
-    m = to_float(__float2bfloat16_rn(__fadd_rn(lo, 8.f * s)));
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, 1));
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, 1));
+    odd += __shfl_xor_sync(0xffffffffu, odd, 1);
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, 2));
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, 2));
+    odd += __shfl_xor_sync(0xffffffffu, odd, 2);
+    float s = to_float(__float2bfloat16_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.f)));
+    if (!(s >= 1.17549435e-38f)) s = 0.f;                      // subnormal or 0 (a NaN is caught below)
+    float m = to_float(__float2bfloat16_rn(__fadd_rn(lo, 8.f * s)));
     if (odd != 0.f || !isfinite(s) || !isfinite(m)) s = m = __int_as_float(0x7fffffff);
+    scale_middle = pack_bf16(s, m);
+    const float magic = 12582912.f;                            // 1.5 2^23: a sum with it is rounded to a whole number, ties to even
+    const int zero = 0x4b400000;                               // its bits
+    const bool none = !(s > 0.f), rough = s < 0x1p-100f || s > 0x1p100f;
+    const float r = none ? 0.f : __frcp_rn(s);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float q = (s > 0.f) ? rintf(__fdiv_rn(__fsub_rn(x[i], m), s)) : 0.f;      // NaN: not above 0
-        c[i] = (int)fminf(fmaxf(q, -8.f), 7.f);
+    for (int half = 0; half < 2; ++half) {
+        uint32_t word = 0u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float& v = x.v[8 * half + i];
+            const float y = __fsub_rn(v, m);
+            float q = __fmul_rn(y, r);
+            q = fmaf(fmaf(-q, s, y), r, q);
+            if (rough) q = none ? 0.f : __fdiv_rn(y, s);
+            q = none ? 0.f : fminf(fmaxf(q, -8.f), 7.f);
+            const float whole = __fadd_rn(q, magic);
+            word += (uint32_t)(__float_as_int(whole) - zero + 8) << code_shift(i);
+            v = fmaf(whole - magic, s, m);
+        }
+        w[half] = word;
     }
 }
 
-// Eight lanes per 64 numbers; a lane's word of keys, or with its neighbour's codes eight bytes of values.  A row is n_kv_heads * head_dim
-// numbers of keys, then as many of values.
+// The eight bytes that 16 values of a row are by column: byte j holds the numbers j and j + 8.
+__device__ __forceinline__ uint32_t column_byte(const uint32_t (&w)[2], int j) {
+    return ((w[0] >> code_shift(j)) & 15u) | (((w[1] >> code_shift(j)) & 15u) << 4);
+}
+
+// A few rows: four lanes a row and 64 numbers, straight into the pages.  A row is n_kv_heads * head_dim numbers of keys, then as many of
+// values.
 template <typename T>
-__global__ void __launch_bounds__(256)
-store4_kernel(const T* rows, long long stride, T* held, long long held_stride, const int* __restrict__ token_pos, const int* __restrict__ token_seq,
-              const int* __restrict__ seq_slot, const int* __restrict__ seq_len_after, Paged4 c, int n_tokens) {
+__global__ void __launch_bounds__(128)
+store4_few_kernel(const T* rows, long long stride, T* held, long long held_stride, const int* __restrict__ token_pos, const int* __restrict__ token_seq,
+                  const int* __restrict__ seq_slot, const int* __restrict__ seq_len_after, Paged4 c, int n_tokens, int vec) {
     pdl_enter();
     const int dim = c.head_dim, groups = dim / 64, per_row = 2 * c.n_kv_heads * groups;
-    const long long item = (long long)blockIdx.x * 32 + (threadIdx.x >> 3);
+    const long long item = (long long)blockIdx.x * 32 + (threadIdx.x >> 2);
     const bool live = item < (long long)n_tokens * per_row;
-    const int n = live ? (int)(item / per_row) : 0, r = live ? (int)(item % per_row) : 0, l = threadIdx.x & 7;
-    const bool value = r >= c.n_kv_heads * groups;
-    const int col = r * 64 + l * 8;                       // column of the row
-    float x[8], s, m;
-    int q[8];
-    load8(rows + (size_t)n * stride + col, x);
-    quantise64(x, s, m, q);
-    if (live && held != nullptr) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) held[(size_t)n * held_stride + col + i] = from_float<T>(fmaf((float)q[i], s, m));
-    }
-    uint32_t w = 0, other;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w |= (uint32_t)(q[i] + 8) << code_shift(i);
-    other = __shfl_xor_sync(0xffffffffu, w, 1);
-    if (!live) return;
+    const int n = live ? (int)(item / per_row) : 0, r = live ? (int)(item % per_row) : 0, l = threadIdx.x & 3, col = r * 64 + l * 16;
     const int seq = token_seq[n], pos = token_pos[n];
+    Numbers x = load16(rows + (size_t)n * stride + col, vec & 1);
+    uint32_t sm, w[2];
+    quantise64(x, sm, w);
+    if (!live) return;
+    if (held != nullptr) store16(held + (size_t)n * held_stride + col, x, vec & 2);
     if (seq < 0) return;
     if (c.ring_pages > 0 && pos + c.ring_pages * kPageTokens < seq_len_after[seq]) return;     // the same step writes over it
+    const bool value = r >= c.n_kv_heads * groups;
     const int head = (r - (value ? c.n_kv_heads * groups : 0)) / groups, g = r % groups, row = pos % kPageTokens;
     const int page = page4_of(c, seq_slot[seq], pos);
     uint8_t* tile = (value ? c.v_pages : c.k_pages) + ((size_t)page * c.n_kv_heads + head) * tile4_bytes(dim);
     uint8_t* block = tile + ((row >> 4) * groups + g) * kBlockBytes;
     if (!value) {
-        *(uint32_t*)(block + by_row_word(row & 15, l * 8)) = w;
-    } else if ((l & 1) == 0) {
+        *(uint2*)(block + by_row_word(row & 15, l * 16)) = make_uint2(w[0], w[1]);
+    } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            block[by_column_byte(row & 15, l * 8 + i)] = (uint8_t)(((w >> code_shift(i)) & 15u) | (((other >> code_shift(i)) & 15u) << 4));
+        for (int j = 0; j < 8; ++j) block[by_column_byte(row & 15, l * 16 + j)] = (uint8_t)column_byte(w, j);
     }
-    if (l == 0) {
-        const __nv_bfloat162 sm = __floats2bfloat162_rn(s, m);
-        *(__nv_bfloat162*)(tile + tile4_codes(dim) + (row * groups + g) * 4) = sm;
+    if (l == 0) *(uint32_t*)(tile + tile4_codes(dim) + (row * groups + g) * 4) = sm;
+}
+
+// Block `left` of the step's rows, cut into blocks of up to `size` rows of one sequence (begun anew where a position is a multiple of
+// size if `align` is size - 1, else, 0, at a sequence's first row), in order; after them come the padding rows, `size` at a time (seq
+// -1).  Every lane of a warp looks at a sequence, their numbers of blocks are added up.  count <= 0: there is no such block.
+struct RowBlock { int seq, row0, pos0, count; };
+__device__ __forceinline__ RowBlock find_rows(const int* __restrict__ cu_seqlens, int row_base, int n_seqs, const int* __restrict__ token_pos, int n_tokens,
+                                              int left, int size, int align) {
+    const int lane = threadIdx.x & 31;
+    for (int s0 = 0; s0 < n_seqs; s0 += 32) {
+        const int s = s0 + lane;
+        int first = 0, n = 0, pos = 0, nb = 0;
+        if (s < n_seqs) {
+            first = cu_seqlens[s] - row_base;
+            n = cu_seqlens[s + 1] - row_base - first;
+            pos = n > 0 ? token_pos[first] : 0;
+            nb = n > 0 ? ((pos & align) + n + size - 1) / size : 0;
+        }
+        int upto = nb;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        const uint32_t found = __ballot_sync(0xffffffffu, left < upto);
+        if (found != 0) {
+            const int who = __ffs(found) - 1, in = left - (__shfl_sync(0xffffffffu, upto, who) - __shfl_sync(0xffffffffu, nb, who));
+            first = __shfl_sync(0xffffffffu, first, who);
+            n = __shfl_sync(0xffffffffu, n, who);
+            pos = __shfl_sync(0xffffffffu, pos, who);
+            const int skip = in == 0 ? 0 : size * in - (pos & align);  // rows of the sequence before the block
+            return RowBlock{s0 + who, first + skip, pos + skip, min(size - ((pos + skip) & align), n - skip)};
+        }
+        left -= __shfl_sync(0xffffffffu, upto, 31);
+    }
+    const int row0 = cu_seqlens[n_seqs] - row_base + size * left;
+    return RowBlock{-1, row0, 0, min(size, n_tokens - row0)};
+}
+
+// Many rows: a warp takes 64 numbers of the up to 16 rows whose positions make a block of the pages, forms the block's 512 bytes in shared
+// memory and writes them at once (with positions missing, or written over by the same step, what is there only).  Blocks are the
+// sequences' in order, and after them the padding rows, 16 at a time, which store nothing but are handed back.
+template <typename T>
+__global__ void __launch_bounds__(256)
+store4_many_kernel(const T* rows, long long stride, T* held, long long held_stride, const int* __restrict__ token_pos, const int* __restrict__ cu_seqlens,
+                   int row_base, int n_seqs, const int* __restrict__ seq_slot, const int* __restrict__ seq_len_after, int seq_base, Paged4 c, int n_tokens,
+                   int vec) {
+    __shared__ __align__(16) uint8_t blocks[8][kBlockBytes];
+    pdl_enter();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane & 3, quad = lane >> 2;
+    const int dim = c.head_dim, groups = dim / 64, per_row = 2 * c.n_kv_heads * groups;
+    const RowBlock found = find_rows(cu_seqlens, row_base, n_seqs, token_pos, n_tokens, blockIdx.x, 16, 15);
+    const int seq = found.seq, row0 = found.row0, pos0 = found.pos0, count = found.count;
+    if (count <= 0) return;
+    const int r = blockIdx.y * 8 + warp;                       // which 64 numbers of a row
+    if (r >= per_row) return;
+    const bool value = r >= c.n_kv_heads * groups;
+    const int head = (r - (value ? c.n_kv_heads * groups : 0)) / groups, g = r % groups, at0 = pos0 & 15, page_row = pos0 & (kPageTokens - 1) & ~15;
+    uint8_t* tile = nullptr;
+    int kept = 0;                                              // the rows before this one are written over by the same step
+    if (seq >= 0) {
+        const int slot = seq_slot[seq_base + seq];
+        tile = (value ? c.v_pages : c.k_pages) + ((size_t)page4_of(c, slot, pos0) * c.n_kv_heads + head) * tile4_bytes(dim);
+        if (c.ring_pages > 0) kept = max(0, seq_len_after[seq_base + seq] - c.ring_pages * kPageTokens - pos0);
+    }
+#pragma unroll
+    for (int it = 0; it < 2; ++it) {
+        const int i = it * 8 + quad;                           // eight rows at a time
+        const T* from = rows + (size_t)(row0 + min(i, count - 1)) * stride + r * 64 + l * 16;
+        Numbers x = load16(from, vec & 1);
+        uint32_t sm, w[2];
+        quantise64(x, sm, w);
+        if (i < count) {
+            if (held != nullptr) store16(held + (size_t)(row0 + i) * held_stride + r * 64 + l * 16, x, vec & 2);
+            const int row = at0 + i;
+            if (tile != nullptr && i >= kept) {
+                if (l == 0) *(uint32_t*)(tile + tile4_codes(dim) + ((page_row + row) * groups + g) * 4) = sm;
+                if (!value) {
+                    *(uint2*)(blocks[warp] + by_row_word(row, l * 16)) = make_uint2(w[0], w[1]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) blocks[warp][by_column_byte(row, l * 16 + j)] = (uint8_t)column_byte(w, j);
+                }
+            }
+        }
+    }
+    __syncwarp();
+    if (tile == nullptr) return;
+    uint8_t* to = tile + ((page_row >> 4) * groups + g) * kBlockBytes + lane * 16;
+    const uint8_t* mine = blocks[warp] + lane * 16;
+    if (count == 16 && kept == 0) {
+        *(uint4*)to = *(const uint4*)mine;
+        return;
+    }
+    auto there = [&](int row) { return row >= at0 + kept && row < at0 + count; };
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int row = value ? 2 * (lane & 3) + ((i >> 1) & 1) + 8 * (i & 1) : (lane >> 2) + 8 * (i >> 3);
+        if (there(row)) to[i] = mine[i];
     }
 }
 
@@ -170,12 +328,12 @@ __device__ __forceinline__ void cluster_meet() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// GROUPS: rows come as groups (row_groups); without, column j is simply head h0 + j of the row.
+// GROUPS: a CTA takes up to 8 / (heads of a kv head) neighbouring rows of a sequence; without, column j is simply head h0 + j of a row.
 template <typename T, int DIM, bool GROUPS>
 __global__ void __launch_bounds__(kAttendWarps * 32, 2)
 attend4_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out, long long out_stride, const int* __restrict__ token_pos,
-               const int* __restrict__ token_seq, const int* __restrict__ seq_slot, const int* __restrict__ token_slot, const int2* __restrict__ row_groups, Paged4 c,
-               int n_heads, float scale, float cap, int window, int share, int splits, float* __restrict__ part_o, float2* __restrict__ part_ml) {
+               const int* __restrict__ token_seq, const int* __restrict__ seq_slot, const int* __restrict__ token_slot, const int* __restrict__ cu_seqlens, int row_base,
+               int n_seqs, int n_tokens, Paged4 c, int n_heads, float scale, float cap, int window, int share, int splits, float* __restrict__ part_o, float2* __restrict__ part_ml) {
     using A = Attend4<DIM>;
     constexpr int G = A::kGroups, kTerms = sizeof(T) == 4 ? 3 : 1, kTiles = DIM / 16;
     constexpr bool kExact = kTerms == 3;
@@ -189,13 +347,18 @@ attend4_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out,
     pdl_enter();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
     const int split = blockIdx.x % splits;
-    const int2 rows = GROUPS ? row_groups[blockIdx.x / splits] : make_int2(blockIdx.x / splits, 1);      // the first, and how many
-    const int n = rows.x, per = n_heads / c.n_kv_heads, chunks = (per + 7) / 8, kvh = blockIdx.y / chunks, chunk = blockIdx.y % chunks;
-    const int h0 = kvh * per + chunk * 8, nh = min(8, per - chunk * 8), columns = nh * rows.y;
+    const int per = n_heads / c.n_kv_heads;
+    RowBlock rows = {0, (int)blockIdx.x / splits, 0, 1};
+    if (GROUPS) {
+        rows = find_rows(cu_seqlens, row_base, n_seqs, token_pos, n_tokens, blockIdx.x / splits, 8 / per, 0);
+        if (rows.count <= 0) return;                           // all of a cluster's CTAs alike
+    }
+    const int n = rows.row0, chunks = (per + 7) / 8, kvh = blockIdx.y / chunks, chunk = blockIdx.y % chunks;
+    const int h0 = kvh * per + chunk * 8, nh = min(8, per - chunk * 8), columns = nh * rows.count;
     auto row_at = [&](int column) { return GROUPS ? column / nh : 0; };                     // column j: head h0 + j % nh of row n + j / nh
     auto head_at = [&](int column) { return GROUPS ? column % nh : column; };
     const int seq = token_seq[n], known_slot = token_slot != nullptr ? token_slot[n] : -1;
-    const int pos0 = token_pos[n], last = pos0 + rows.y - 1, first = window > 0 ? max(0, pos0 - window + 1) : 0;
+    const int pos0 = token_pos[n], last = pos0 + rows.count - 1, first = window > 0 ? max(0, pos0 - window + 1) : 0;
     // the pages of the keys, from page0 to before page1; where there are more than planned a share is longer
     const int page0 = first / kPageTokens, page1 = last / kPageTokens + 1, pages = max(share, (page1 - page0 + splits - 1) / splits);
     const int p0 = page0 + split * pages, p1 = seq < 0 ? p0 : min(page1, p0 + pages);      // a padding row has no pages
@@ -203,7 +366,8 @@ attend4_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out,
     float* sums = (float*)ring_bytes;                          // once the walk is over
     if (p0 >= p1) {                                            // a share without keys says so; a padding row becomes zeros
         if (splits == 1) {
-            for (int i = threadIdx.x; i < nh * DIM; i += blockDim.x) out[(size_t)n * out_stride + (size_t)h0 * DIM + i] = from_float<T>(0.f);
+            for (int i = threadIdx.x; i < columns * DIM; i += blockDim.x)
+                out[(size_t)(n + row_at(i / DIM)) * out_stride + (size_t)(h0 + head_at(i / DIM)) * DIM + i % DIM] = from_float<T>(0.f);
             return;
         }
         if (threadIdx.x < 8) cta_ml[threadIdx.x] = make_float2(-INFINITY, 0.f);
@@ -504,7 +668,7 @@ attend4_merge_kernel(T* __restrict__ out, long long out_stride, int n_heads, int
 
 template <typename T, int DIM, bool GROUPS>
 int launch_attend4(const void* q, long long q_stride, void* out, long long out_stride, const int* token_pos, const int* token_seq, const int* seq_slot,
-                   const int* token_slot, const int2* row_groups, int n_groups, const Paged4& c, int n_tokens, int n_heads, float scale, float cap, int window, int share, int splits, float* part_o, float2* part_ml,
+                   const int* token_slot, const int* cu_seqlens, int row_base, int n_seqs, const Paged4& c, int n_tokens, int n_heads, float scale, float cap, int window, int share, int splits, float* part_o, float2* part_ml,
                    cudaStream_t stream) {
     constexpr int smem = Attend4<DIM>::kShared;
     auto kernel = attend4_kernel<T, DIM, GROUPS>;
@@ -514,9 +678,10 @@ int launch_attend4(const void* q, long long q_stride, void* out, long long out_s
         set = true;
     }
     const int per = n_heads / c.n_kv_heads, chunks = (per + 7) / 8;
+    const long long n_groups = GROUPS ? (n_tokens + 8 / per - 1) / (8 / per) + n_seqs : n_tokens;      // a sequence's last may not be full
     const bool clustered = splits > 1 && part_o == nullptr;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((long long)n_groups * splits), (unsigned)(c.n_kv_heads * chunks));
+    cfg.gridDim = dim3((unsigned)(n_groups * splits), (unsigned)(c.n_kv_heads * chunks));
     cfg.blockDim = dim3(kAttendWarps * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
@@ -527,8 +692,8 @@ int launch_attend4(const void* q, long long q_stride, void* out, long long out_s
     attr[1].val.clusterDim = {(unsigned)splits, 1, 1};
     cfg.attrs = attr;
     cfg.numAttrs = clustered ? 2 : 1;
-    cudaLaunchKernelEx(&cfg, kernel, (const T*)q, q_stride, (T*)out, out_stride, token_pos, token_seq, seq_slot, token_slot, row_groups, c, n_heads, scale, cap,
-                       window, share, splits, part_o, part_ml);
+    cudaLaunchKernelEx(&cfg, kernel, (const T*)q, q_stride, (T*)out, out_stride, token_pos, token_seq, seq_slot, token_slot, cu_seqlens, row_base,
+                       n_seqs, n_tokens, c, n_heads, scale, cap, window, share, splits, part_o, part_ml);
     if (splits > 1 && !clustered)
         launch_pdl(attend4_merge_kernel<T, DIM>, dim3((unsigned)((long long)n_tokens * n_heads)), dim3(DIM), 0, stream, (T*)out, out_stride, n_heads,
                    splits, (const float*)part_o, (const float2*)part_ml);
@@ -545,24 +710,39 @@ using namespace hos;
     if (head_dim % 64 || head_dim < 64 || head_dim > 256) HOS_REFUSE(what ": head size %d (64, 128, 192 or 256)", head_dim);     \
     if (n_kv_heads <= 0) HOS_REFUSE(what ": %d kv heads", n_kv_heads)
 
+// Rows and `held` (or null) have their numbers side by side; sequences' rows are cu_seqlens[s] - row_base .. in order (their entries of
+// seq_slot and seq_len_after begin at seq_base), then padding rows.  single: the sequences bring a row each.
 extern "C" int hos_store4(const void* rows, int dtype, long long stride, void* held, long long held_stride, const int* token_pos, const int* token_seq,
-                          const int* seq_slot, const int* seq_len_after, const void* cache, int n_tokens, cudaStream_t stream) {
+                          const int* seq_slot, const int* seq_len_after, const int* cu_seqlens, int row_base, int n_seqs, int seq_base, int single,
+                          const void* cache, int n_tokens, cudaStream_t stream) {
     if (n_tokens <= 0) return 0;
     HOS_CHECK_PAGED4("store4");
-    const long long items = (long long)n_tokens * 2 * n_kv_heads * (head_dim / 64);
-    const dim3 grid((unsigned)((items + 31) / 32));
-    if (dtype == kF32)
-        launch_pdl(store4_kernel<float>, grid, dim3(256), 0, stream, (const float*)rows, stride, (float*)held, held_stride, token_pos, token_seq, seq_slot, seq_len_after, c, n_tokens);
-    else
-        launch_pdl(store4_kernel<bf16>, grid, dim3(256), 0, stream, (const bf16*)rows, stride, (bf16*)held, held_stride, token_pos, token_seq, seq_slot, seq_len_after, c, n_tokens);
+    const int per_row = 2 * n_kv_heads * (head_dim / 64), piece = dtype == kF32 ? 4 : 8;
+    const int vec = (stride % piece == 0 && (uintptr_t)rows % 16 == 0 ? 1 : 0) | (held_stride % piece == 0 && (uintptr_t)held % 16 == 0 ? 2 : 0);
+    const bool many = n_tokens >= 32 && !single;
+    const long long items = (long long)n_tokens * per_row;
+    // every sequence may begin and end inside a block
+    const dim3 few_grid((unsigned)((items + 31) / 32)), many_grid((unsigned)((n_tokens + 15) / 16 + 2 * n_seqs), (unsigned)((per_row + 7) / 8));
+    if (many && many_grid.y > 65535) HOS_REFUSE("store4: %d kv heads", n_kv_heads);
+#define HOS_S4(T)                                                                                                                                       \
+    do {                                                                                                                                                \
+        if (many)                                                                                                                                       \
+            launch_pdl(store4_many_kernel<T>, many_grid, dim3(256), 0, stream, (const T*)rows, stride, (T*)held, held_stride, token_pos, cu_seqlens,        \
+                       row_base, n_seqs, seq_slot, seq_len_after, seq_base, c, n_tokens, vec);                                                          \
+        else                                                                                                                                            \
+            launch_pdl(store4_few_kernel<T>, few_grid, dim3(128), 0, stream, (const T*)rows, stride, (T*)held, held_stride, token_pos, token_seq,           \
+                       seq_slot, seq_len_after, c, n_tokens, vec);                                                                                      \
+    } while (0)
+    if (dtype == kF32) HOS_S4(float);
+    else HOS_S4(bf16);
     return check_launch("store4");
 }
 
-// token_slot: seq_slot[token_seq] of every row, or null.  row_groups: [n_groups][2], all rows as groups of neighbours (the first, how
-// many) of one sequence at consecutive positions, as many as times the heads of a kv head are at most 8; null: every row alone.  A group over its pages, `share` of them to a CTA: `splits` shares cover the longest row's.  2 to 8 without
+// token_slot: seq_slot[token_seq] of every row, or null.  cu_seqlens: the sequences' rows (less row_base), n_seqs + 1 of
+// them, padding rows behind: neighbouring rows of a sequence share a walk if the kv heads have few heads; null: every row alone.  A walk over its pages, `share` of them to a CTA: `splits` shares cover the longest row's.  2 to 8 without
 // `parts` are a cluster; else more than one need `parts`, n_tokens * n_heads * splits * (head_dim + 2) 32-bit numbers.
 extern "C" int hos_attend4(const void* q, int dtype, long long q_stride, void* out, long long out_stride, const int* token_pos, const int* token_seq,
-                           const int* seq_slot, const int* token_slot, const int* row_groups, int n_groups, const void* cache, int n_tokens, int n_heads, float scale, float cap, int window,
+                           const int* seq_slot, const int* token_slot, const int* cu_seqlens, int row_base, int n_seqs, const void* cache, int n_tokens, int n_heads, float scale, float cap, int window,
                            int share, int splits, float* parts, cudaStream_t stream) {
     if (n_tokens <= 0) return 0;
     HOS_CHECK_PAGED4("attend4");
@@ -573,7 +753,8 @@ extern "C" int hos_attend4(const void* q, int dtype, long long q_stride, void* o
     const size_t n_parts = (size_t)n_tokens * n_heads * splits;
     float2* part_ml = (float2*)parts;                          // pairs first: they want 8 bytes' alignment
     float* part_o = parts == nullptr ? nullptr : parts + 2 * n_parts;
-#define HOS_A4(T, D) return (row_groups != nullptr ? launch_attend4<T, D, true> : launch_attend4<T, D, false>)(q, q_stride, out, out_stride, token_pos, token_seq, seq_slot, token_slot, (const int2*)row_groups, row_groups != nullptr ? n_groups : n_tokens, c, n_tokens, n_heads, scale, cap, window, share, splits, part_o, part_ml, stream)
+    const bool groups = cu_seqlens != nullptr && 2 * (n_heads / n_kv_heads) <= 8;
+#define HOS_A4(T, D) return (groups ? launch_attend4<T, D, true> : launch_attend4<T, D, false>)(q, q_stride, out, out_stride, token_pos, token_seq, seq_slot, token_slot, cu_seqlens, row_base, n_seqs, c, n_tokens, n_heads, scale, cap, window, share, splits, part_o, part_ml, stream)
 #define HOS_A4_D(T) do { if (head_dim == 64) HOS_A4(T, 64); else if (head_dim == 128) HOS_A4(T, 128); else if (head_dim == 192) HOS_A4(T, 192); else HOS_A4(T, 256); } while (0)
     if (dtype == kF32) HOS_A4_D(float);
     else HOS_A4_D(bf16);

@@ -45,7 +45,8 @@ def store(rows: torch.Tensor, step, cache: ops.PagedKVArgs, held: Optional[torch
             raise KernelError("what is held and the rows differ in size")
     ops.fourbit().call("hos_store4", rows.data_ptr(), ops.dtype_code(rows.dtype), rows.stride(0), held.data_ptr() if held is not None else None,
                        held.stride(0) if held is not None else 0, step.token_pos.data_ptr(), step.token_seq.data_ptr(), step.seq_slot.data_ptr(),
-                       step.seq_len_after.data_ptr(), ops.paged4(cache), n, ops._stream())
+                       step.seq_len_after.data_ptr(), step.cu_seqlens.data_ptr(), step.row_offset, step.n_seqs, step.seq_offset, int(step.single_token),
+                       ops.paged4(cache), n, ops._stream())
 
 
 MAX_SHARES, CLUSTER_SHARES = 1024, 8
@@ -87,29 +88,17 @@ def attend(q: torch.Tensor, out: torch.Tensor, step, cache: ops.PagedKVArgs, n_h
     _check_step(n, step, "attend")
     kv = cache.n_kv_heads
     items = kv * -(-(n_heads // kv) // 8)
-    per = n_heads // kv
-    key = ("shares of 4-bit pages", n, items, per, window, step.row_offset)
+    together = 1 if step.single_token else max(1, 8 // (n_heads // kv))      # rows of a sequence that share a walk
+    key = ("shares of 4-bit pages", n, items, together, window, step.row_offset)
     plan = step.shared.get(key)                      # once per step and kind of layer
     if plan is None:
-        groups = _row_groups(step, n, per, q.device)
-        plan = step.shared[key] = (groups, *shares(n if groups is None else groups.shape[0], items, step.max_len_after, window, step.fill_for(window)))
-    groups, share, splits, cluster = plan
+        walks = n if together == 1 else -(-n // together)
+        plan = step.shared[key] = shares(walks, items, step.max_len_after, window, step.fill_for(window))
+    share, splits, cluster = plan
     parts = None
     if splits > 1 and not cluster:
         parts = torch.empty(n * n_heads * splits * (cache.head_dim + 2), dtype=torch.float32, device=q.device)
     ops.fourbit().call("hos_attend4", q.data_ptr(), ops.dtype_code(q.dtype), q.stride(0), out.data_ptr(), out.stride(0), step.token_pos.data_ptr(),
                        step.token_seq.data_ptr(), step.seq_slot.data_ptr(), step.token_slot.data_ptr() if step.token_slot is not None else None,
-                       groups.data_ptr() if groups is not None else None, groups.shape[0] if groups is not None else 0, ops.paged4(cache), n, n_heads,
+                       step.cu_seqlens.data_ptr() if together > 1 else None, step.row_offset, step.n_seqs, ops.paged4(cache), n, n_heads,
                        scale, softcap, window or 0, share, splits, parts.data_ptr() if parts is not None else None, ops._stream())
-
-
-def _row_groups(step, n: int, per: int, device):
-    """Rows of a sequence that share a walk over its keys, as many as the 8 columns of the kernel's products hold: [groups, 2] (the first
-    row, how many), or None where every row goes alone (also where which rows are whose is known on the device only)."""
-    together = 8 // per if per <= 8 else 1
-    if together < 2 or step.single_token or step.replayed or not step.cu_host:
-        return None
-    cu = step.cu_host
-    groups = [(row, min(together, cu[i + 1] - row)) for i in range(len(cu) - 1) for row in range(cu[i], cu[i + 1], together)]
-    groups += [(row, 1) for row in range(cu[-1], n)]              # padding rows
-    return torch.tensor(groups, dtype=torch.int32).pin_memory().to(device, non_blocking=True)
