@@ -1,0 +1,346 @@
+// Products of many rows with weights in 4 bits on the 5th-generation tensor cores: out[M, N] = x[M, K] . W[N, K]^T in bfloat16.
+//
+// The weights are formed in bfloat16 on their way: (c - z) s, c - z exact and the product rounded once (2^-9 of a weight, as a matrix
+// kept in bfloat16 would be), straight into the operand's place in shared memory, so that they cross memory in 4 bits however many
+// rows there are.  A CTA takes 128 features (gated: 128 of gate and the same 128 of up) and up to 256 rows, tcgen05.mma with M = 128
+// features and N = rows: eight warps each form 16 features' 64 numbers a stage (from a ring of codes of their own that cp.async fills)
+// and bring the rows of x, a ninth issues the products.  Few tiles share K as a cluster, whose sums meet in shared memory.
+// Bound by the products where rows fill the tile (2 clocks a row and stage of 64 k), else by forming the weights (some 250 clocks a
+// stage): plan_tiles below chooses rows a tile and CTAs a cluster by these.
+#include "common.cuh"
+#include "fourbit.cuh"
+#include "mma_utils.cuh"
+#include "tcgen05_one.cuh"
+
+namespace hos {
+
+constexpr int kTcFeatures = 128, kTcRows = 256, kTcMakers = 8, kTcThreads = (kTcMakers + 1) * 32;
+constexpr int kTcShared = 226 * 1024, kTcWeights = kTcFeatures * 128;            // bytes of a stage's 128 features
+constexpr long long kProductWaitCycles = 1ll << 31;
+constexpr int kGiveUpProduct4 = 6;
+
+__device__ int* g_product4_error_host = nullptr;            // a word in pinned host memory, if the host gave one
+
+__device__ __forceinline__ void product4_give_up() {
+    int* w = g_product4_error_host;
+    if (w != nullptr) {
+        atomicExch_system(w, kGiveUpProduct4);
+        __threadfence_system();
+    }
+}
+
+struct Product4Args {
+    const bf16* x;
+    const uint8_t *codes, *records;
+    void* out;
+    long long ldx, ldo, wait_cycles;     // wait_cycles: the limit of every wait
+    int out_f32, M, N, K, group_blocks, act, tile_rows, shares, stages;
+    int stop_stage;                      // for tests of the give-up path: the stage at which the products' warp takes its wait as run out (-1: none)
+    float limit;
+};
+
+__host__ __device__ inline int stage_bytes(bool gated, int tile_rows) { return (gated ? 2 : 1) * kTcWeights + tile_rows * 128; }
+__host__ __device__ inline int codes_bytes(bool gated, int sub, bool zeros) { return (gated ? 2 : 1) * (kBlockBytes + sub * (zeros ? 64 : 32)); }
+
+__device__ __forceinline__ float peer_value(uint32_t at, int rank) {
+    uint32_t r;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(r));
+    return v;
+}
+__device__ __forceinline__ void shares_meet() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ float gated_value(int act, float gate, float up, float limit) {
+    return act == 2 ? clamped_swish_fast(gate, up, limit) : (act == 0 ? gelu_tanh_fast(gate) : silu_fast(gate)) * up;
+}
+
+// S: stages of operands, and of codes; SUB: scales a block of 64 (2: groups of 32).
+template <int S, bool GATED, int SUB, bool ZEROS>
+__global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(Product4Args p) {
+    constexpr int kAcc = GATED ? 2 : 1, kRecord = ZEROS ? 64 : 32, kTile = kBlockBytes + SUB * kRecord, kCodes = kAcc * kTile;
+    constexpr int P = S - 2;                                 // blocks asked for ahead: the products of the block before the last may still run
+    extern __shared__ unsigned char smem_unaligned[];
+    unsigned char* stages = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_unaligned) + 1023) & ~(uintptr_t)1023);
+    const int stage = stage_bytes(GATED, p.tile_rows);
+    unsigned char* rings = stages + S * stage;
+    __shared__ uint64_t full[S], empty[S], done;
+    __shared__ uint32_t tmem_base_smem;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+    const int columns = (p.tile_rows + 31) & ~31;           // of an accumulator
+    int tmem_columns = 32;
+    while (tmem_columns < kAcc * columns) tmem_columns *= 2;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) { mbar_init(&full[s], kTcMakers); mbar_init(&empty[s], 1); }
+        mbar_init(&done, 1);
+        mbar_fence_init();
+    }
+    if (warp == kTcMakers) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_smem)), "r"(tmem_columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem_base = tmem_base_smem;
+    pdl_enter();
+
+    const int k_blocks = (p.K + 63) / 64, tiles = (p.N + 15) / 16, feature_tiles = (p.N + kTcFeatures - 1) / kTcFeatures;
+    const int groups = SUB == 2 ? 2 * k_blocks : (k_blocks + p.group_blocks - 1) / p.group_blocks;
+    const int share = blockIdx.x % p.shares, tile = blockIdx.x / p.shares, f0 = tile % feature_tiles * kTcFeatures, m0 = tile / feature_tiles * p.tile_rows;
+    const int kb0 = (int)((long long)share * k_blocks / p.shares), n_k = (int)((long long)(share + 1) * k_blocks / p.shares) - kb0;
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_cycles(bar, parity, p.wait_cycles); };
+
+    if (warp < kTcMakers) {
+        const uint32_t ring = smem_u32(rings) + warp * S * kCodes;
+        const unsigned char* ring_ptr = rings + warp * S * kCodes;
+        const uint8_t *code_at[kAcc], *record_at[kAcc];
+#pragma unroll
+        for (int a = 0; a < kAcc; ++a) {                    // a tile beyond the last reads the last one: its sums are dropped
+            const size_t t = (size_t)a * tiles + min(f0 / 16 + warp, tiles - 1);
+            code_at[a] = p.codes + (t * k_blocks + kb0) * kBlockBytes + lane * 16;
+            record_at[a] = p.records + (t * groups + (SUB == 2 ? 2 * kb0 : kb0 / p.group_blocks)) * kRecord + lane * 16;
+        }
+        int in_group = SUB == 2 ? 1 : p.group_blocks - kb0 % p.group_blocks;
+        // the rows' 16-byte pieces that a thread brings: piece i of row j, j a step of 32 apart
+        const int piece = threadIdx.x & 7, first_row = threadIdx.x >> 3;
+        auto fetch = [&](int i) {                           // block i of this share into place i % S
+            if (i < n_k) {
+                const int s = i % S;
+#pragma unroll
+                for (int a = 0; a < kAcc; ++a) {
+                    const uint32_t to = ring + s * kCodes + a * kTile;
+                    copy16_async(to + lane * 16, code_at[a]);
+                    if (lane < SUB * kRecord / 16) copy16_async(to + kBlockBytes + lane * 16, record_at[a]);
+                    code_at[a] += kBlockBytes;
+                }
+                if (--in_group == 0) {
+                    in_group = SUB == 2 ? 1 : p.group_blocks;
+#pragma unroll
+                    for (int a = 0; a < kAcc; ++a) record_at[a] += SUB * kRecord;
+                }
+                const uint32_t b = smem_u32(stages + s * stage + kAcc * kTcWeights);
+                const int k = (kb0 + i) * 64 + piece * 8;
+                for (int j = first_row; j < p.tile_rows; j += 32) {
+                    const int m = m0 + j;
+                    const bool in = m < p.M && k < p.K;      // K is a multiple of 8: a piece is whole or not there
+                    copy16_async(b + j * 128 + ((piece ^ (j & 7)) << 4), p.x + (in ? (size_t)m * p.ldx + k : 0), in ? 16 : 0);
+                }
+            }
+            copies_commit();
+        };
+#pragma unroll 1
+        for (int i = 0; i < P; ++i) fetch(i);
+        for (int i = 0; i < n_k; ++i) {
+            const int s = i % S, ahead = i + P;
+            if (ahead >= S && ahead < n_k) {                // the place of the block that is asked for now
+                ok = lane != 0 || wait(&empty[ahead % S], ((ahead / S) - 1) & 1);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+            }
+            fetch(ahead);
+            copies_wait<P>();
+            __syncwarp();
+#pragma unroll
+            for (int a = 0; a < kAcc; ++a) {
+                const uint4 w = lds16(ring + s * kCodes + a * kTile + lane * 16);
+                const unsigned char* rec = ring_ptr + s * kCodes + a * kTile + kBlockBytes + g * (kRecord / 8);
+                unsigned char* to = stages + s * stage + a * kTcWeights + warp * 2048 + g * 128;
+                // the k below and from 32 on, in the other order for odd rows: eight lanes then fill all banks
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int half = h ^ (g & 1);
+                    const uint32_t lo = half ? w.y : w.x, hi = half ? w.w : w.z;
+                    const unsigned char* r = rec + (SUB == 2 ? half * kRecord : 0);
+                    const uint32_t two = *(const uint32_t*)r;
+                    uint32_t z0 = kZero8, z1 = kZero8;
+                    if (ZEROS) {
+                        const uint32_t zz = *(const uint32_t*)(r + 4);
+                        z0 = __byte_perm(zz, 0, 0x1010);
+                        z1 = __byte_perm(zz, 0, 0x3232);
+                    }
+                    const uint32_t s0 = __byte_perm(two, 0, 0x1010), s1 = __byte_perm(two, 0, 0x3232);
+                    const __nv_bfloat162 sc0 = *reinterpret_cast<const __nv_bfloat162*>(&s0), sc1 = *reinterpret_cast<const __nv_bfloat162*>(&s1);
+                    uint32_t v0[4], v1[4];
+                    codes_to_bf16<true>(lo, z0, v0);
+                    codes_to_bf16<true>(hi, z1, v1);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const __nv_bfloat162 y0 = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&v0[j]), sc0);
+                        const __nv_bfloat162 y1 = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&v1[j]), sc1);
+                        v0[j] = *reinterpret_cast<const uint32_t*>(&y0);
+                        v1[j] = *reinterpret_cast<const uint32_t*>(&y1);
+                    }
+                    const int chunk = ((4 * half + t4) ^ g) << 4;
+                    *reinterpret_cast<uint4*>(to + chunk) = make_uint4(v0[0], v0[1], v0[2], v0[3]);
+                    *reinterpret_cast<uint4*>(to + 1024 + chunk) = make_uint4(v1[0], v1[1], v1[2], v1[3]);
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[s]);
+        }
+        copies_wait<0>();
+    } else if (lane == 0) {
+        const uint32_t idesc = tc_idesc(kTcFeatures, p.tile_rows, 0);
+        for (int i = 0; i < n_k; ++i) {
+            const int s = i % S;
+            ok = wait(&full[s], (i / S) & 1) && i != p.stop_stage;
+            if (!ok) break;
+            tc_fence_after_sync();
+            const uint32_t at = smem_u32(stages + s * stage);
+            const uint64_t b_desc = desc_kmajor(at + kAcc * kTcWeights);
+#pragma unroll
+            for (int a = 0; a < kAcc; ++a) {
+                const uint64_t a_desc = desc_kmajor(at + a * kTcWeights);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) tc_mma(tmem_base + a * columns, a_desc + 2 * k, b_desc + 2 * k, idesc, (i > 0 || k > 0) ? 1u : 0u);
+            }
+            tc_commit(&empty[s]);
+        }
+        if (ok) tc_commit(&done);
+    }
+    __syncwarp();
+    if (warp < kTcMakers && ok) {
+        ok = lane != 0 || wait(&done, 0);
+        ok = __all_sync(0xffffffffu, ok);
+    }
+    tc_fence_after_sync();
+    float* sums = reinterpret_cast<float*>(stages);          // [kAcc][tile_rows][128] of a share, over operands that are done with
+    if (warp < kTcMakers && ok) {
+        const int quarter = warp & 3, feature = quarter * 32 + lane, n = f0 + feature;
+        const uint32_t from = tmem_base + ((uint32_t)(quarter * 32) << 16);
+#pragma unroll 1
+        for (int c0 = (warp >> 2) * 32; c0 < p.tile_rows; c0 += 64) {
+            uint32_t v[32], u[32];
+            tc_ld32(from + c0, v);
+            if (GATED) tc_ld32(from + columns + c0, u);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+                const int c = c0 + j, m = m0 + c;
+                if (p.shares > 1) {
+                    if (c < p.tile_rows) {
+                        sums[c * 128 + feature] = __uint_as_float(v[j]);
+                        if (GATED) sums[(p.tile_rows + c) * 128 + feature] = __uint_as_float(u[j]);
+                    }
+                } else if (c < p.tile_rows && m < p.M && n < p.N) {
+                    const float y = GATED ? gated_value(p.act, __uint_as_float(v[j]), __uint_as_float(u[j]), p.limit) : __uint_as_float(v[j]);
+                    if (p.out_f32) ((float*)p.out)[(size_t)m * p.ldo + n] = y;
+                    else ((bf16*)p.out)[(size_t)m * p.ldo + n] = __float2bfloat16_rn(y);
+                }
+            }
+        }
+    }
+    if (!ok && lane == 0) product4_give_up();
+    const bool gave_up = __syncthreads_or(!ok);
+    if (gave_up) let_work_under_way_end();
+    if (p.shares > 1) {
+        shares_meet();
+        if (warp < kTcMakers && !gave_up) {
+            const int feature = threadIdx.x & 127, n = f0 + feature;
+            const uint32_t at = smem_u32(sums);
+            for (int c = 2 * share + (threadIdx.x >> 7); c < p.tile_rows; c += 2 * p.shares) {
+                float v = 0.f, u = 0.f;
+                for (int s = 0; s < p.shares; ++s) {
+                    v += peer_value(at + (c * 128 + feature) * 4, s);
+                    if (GATED) u += peer_value(at + ((p.tile_rows + c) * 128 + feature) * 4, s);
+                }
+                const int m = m0 + c;
+                if (m < p.M && n < p.N) {
+                    const float y = GATED ? gated_value(p.act, v, u, p.limit) : v;
+                    if (p.out_f32) ((float*)p.out)[(size_t)m * p.ldo + n] = y;
+                    else ((bf16*)p.out)[(size_t)m * p.ldo + n] = __float2bfloat16_rn(y);
+                }
+            }
+        }
+        shares_meet();                                       // nobody leaves while its sums are read
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == kTcMakers) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(tmem_columns));
+}
+
+template <int S, bool GATED, int SUB, bool ZEROS>
+int launch_product4_tc(const Product4Args& p, int ctas, int smem, cudaStream_t stream) {
+    auto kernel = product4_tc_kernel<S, GATED, SUB, ZEROS>;
+    static bool set = false;                                 // once per kernel: the attribute stays
+    if (!set) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcShared) != cudaSuccess) return check_launch("product4_tc");
+        set = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(kTcThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim = {(unsigned)p.shares, 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = p.shares > 1 ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, kernel, p);
+    return check_launch("product4_tc");
+}
+
+// Rows of a tile and CTAs that share a tile's K: the least of waves x (stages x clocks a stage + what a tile costs besides), in clocks as
+// above.  Sums of shares have to fit where the operands were.
+static void plan_tiles(int M, int N, int K, bool gated, int& tile_rows, int& shares) {
+    const int sm = sm_count_cached(), acc = gated ? 2 : 1, feature_tiles = (N + kTcFeatures - 1) / kTcFeatures, k_blocks = (K + 63) / 64;
+    double best = 0.;
+    tile_rows = 0;
+    for (int row_tiles = (M + kTcRows - 1) / kTcRows; row_tiles <= (M + 15) / 16; ++row_tiles) {
+        const int rows = ((M + row_tiles - 1) / row_tiles + 15) / 16 * 16;
+        const long long n = (long long)feature_tiles * ((M + rows - 1) / rows);
+        for (int s = 1; s <= 8 && s <= k_blocks; s *= 2) {
+            if (s > 1 && (rows > 128 || n * s > sm)) break;
+            const double stage = acc * (rows * 2.1 > 250. ? rows * 2.1 : 250.), blocks = (k_blocks + s - 1) / s;
+            const double cost = (double)((n * s + sm - 1) / sm) * (blocks * stage + 5000. + rows * acc * 12. + (s > 1 ? 3000. : 0.));
+            if (tile_rows == 0 || cost < best) { best = cost; tile_rows = rows; shares = s; }
+        }
+        if (rows == 16) break;
+    }
+}
+
+}  // namespace hos
+
+using namespace hos;
+
+extern "C" int hos_product4_tc_set_error_word(void* word) {
+    return cudaMemcpyToSymbol(g_product4_error_host, &word, sizeof(word)) == cudaSuccess ? 0 : -1;
+}
+
+// As hos_product4 for bfloat16 rows that begin on 16 bytes, K and ldx multiples of 8.  tile_rows 0: chosen here, with shares.
+extern "C" int hos_product4_tc(const void* x, long long ldx, const void* matrix, void* out, int out_dtype, long long ldo, int M, int act, float limit,
+                               int tile_rows, int shares, long long wait_cycles, int stop_stage, cudaStream_t stream) {
+    struct Matrix4 { const uint8_t *codes, *records; int n, k, group, zeros, gated; };
+    const Matrix4 w = *(const Matrix4*)matrix;
+    if (M <= 0 || w.n <= 0) return 0;
+    if (w.k <= 0 || w.k % 8 || ldx % 8 || (uintptr_t)x % 16) HOS_REFUSE("product4_tc: rows must be 16-byte pieces (K %d, %lld apart)", w.k, ldx);
+    if (w.group < 32 || (w.group != 32 && w.group % 64)) HOS_REFUSE("product4_tc: groups of %d weights (32, or a multiple of 64)", w.group);
+    if (out_dtype != kF32 && out_dtype != kBF16) HOS_REFUSE("product4_tc: no product into type %d", out_dtype);
+    if (tile_rows == 0) plan_tiles(M, w.n, w.k, w.gated != 0, tile_rows, shares);
+    const int k_blocks = (w.k + 63) / 64, sub = w.group == 32 ? 2 : 1;
+    if (tile_rows < 16 || tile_rows > kTcRows || tile_rows % 16 || shares < 1 || shares > 8 || shares > k_blocks || (shares > 1 && tile_rows > 128))
+        HOS_REFUSE("product4_tc: tiles of %d rows in %d shares", tile_rows, shares);
+    Product4Args p = {};
+    p.x = (const bf16*)x; p.codes = w.codes; p.records = w.records; p.out = out; p.ldx = ldx; p.ldo = ldo;
+    p.wait_cycles = wait_cycles > 0 ? wait_cycles : kProductWaitCycles;
+    p.out_f32 = out_dtype == kF32; p.M = M; p.N = w.n; p.K = w.k; p.group_blocks = w.group / 64; p.act = act; p.limit = limit;
+    p.tile_rows = tile_rows; p.shares = shares; p.stop_stage = stop_stage;
+    const long long ctas = (long long)((w.n + kTcFeatures - 1) / kTcFeatures) * ((M + tile_rows - 1) / tile_rows) * shares;
+    if (ctas > 0x7fffffffll) HOS_REFUSE("product4_tc: %d rows", M);
+    const int a_stage = stage_bytes(w.gated, tile_rows) + kTcMakers * codes_bytes(w.gated, sub, w.zeros);
+    const int S = 6 * a_stage + 1024 <= kTcShared ? 6 : (4 * a_stage + 1024 <= kTcShared ? 4 : 3), smem = S * a_stage + 1024;
+#define HOS_PT(SS, G, U, Z) return launch_product4_tc<SS, G, U, Z>(p, (int)ctas, smem, stream)
+#define HOS_PT_S(G, U, Z) do { if (S == 6) HOS_PT(6, G, U, Z); else if (S == 4) HOS_PT(4, G, U, Z); else HOS_PT(3, G, U, Z); } while (0)
+#define HOS_PT_U(G, Z) do { if (sub == 2) HOS_PT_S(G, 2, Z); else HOS_PT_S(G, 1, Z); } while (0)
+#define HOS_PT_Z(G) do { if (w.zeros) HOS_PT_U(G, true); else HOS_PT_U(G, false); } while (0)
+    if (w.gated) HOS_PT_Z(true);
+    else HOS_PT_Z(false);
+}

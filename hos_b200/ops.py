@@ -168,9 +168,11 @@ def call_times() -> dict:
 _launch_ahead = False
 
 _ERROR_WORD_SETTERS = ("hos_gemm_tc_set_error_word", "hos_attn_decode_set_error_word",
-                       "hos_attn_prefill_tc_set_error_word", "hos_latent_prompt_set_error_word", "hos_moe_grouped_set_error_word")
+                       "hos_attn_prefill_tc_set_error_word", "hos_latent_prompt_set_error_word", "hos_moe_grouped_set_error_word",
+                       "hos_product4_tc_set_error_word")
 GIVE_UP_CODES = {1: "the tcgen05 matrix product", 2: "the decode attention", 3: "the tcgen05 prompt attention",
-                 4: "the tcgen05 prompt attention over latent rows", 5: "the tcgen05 products of the routed experts"}
+                 4: "the tcgen05 prompt attention over latent rows", 5: "the tcgen05 products of the routed experts",
+                 6: "the tcgen05 product with 4-bit weights"}
 _error_word_tensor: Optional[torch.Tensor] = None
 _after_give_up = []        # callables that put shared scratch state right after a kernel gave up
 
@@ -1441,6 +1443,14 @@ def product4(x: torch.Tensor, matrix: int, out: torch.Tensor, act: int = 0, limi
     """out[M, N] = x[M, K] . W^T with the matrix in 4 bits that `matrix` (the address of a Matrix4) describes; gated: out = act(gate) * up."""
     fourbit().call("hos_product4", x.data_ptr(), dtype_code(x.dtype), x.stride(0), matrix, out.data_ptr(), dtype_code(out.dtype), out.stride(0), x.shape[0],
                    act, limit, _stream())
+
+
+def product4_tc(x: torch.Tensor, matrix: int, out: torch.Tensor, act: int = 0, limit: float = 0.0, tile_rows: int = 0, shares: int = 1,
+                wait_cycles: int = 0, stop_stage: int = -1) -> None:
+    """As product4 for many bfloat16 rows, on the tcgen05 tensor cores; the weights are rounded to bfloat16.  tile_rows, shares: rows of a
+    tile (0: chosen by the kernel's library) and CTAs that share its k.  wait_cycles, stop_stage: for tests of a wait that runs out."""
+    fourbit().call("hos_product4_tc", x.data_ptr(), x.stride(0), matrix, out.data_ptr(), dtype_code(out.dtype), out.stride(0), x.shape[0], act, limit,
+                   tile_rows, shares, wait_cycles, stop_stage, _stream())
 
 
 def copy_pages(table: torch.Tensor, most_bytes: int, src: torch.Tensor, dst: torch.Tensor, n_pages: int) -> None:

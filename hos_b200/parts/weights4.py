@@ -15,6 +15,7 @@ from .. import ops
 from ..errors import KernelError, SpecError
 
 ROWS, COLS = 16, 64             # of a block of codes
+FEW_ROWS = 32                   # up to so many rows the codes are multiplied as they are, above the weights are rounded to bfloat16
 
 
 class Weight4:
@@ -111,5 +112,8 @@ class Weight4:
             ops._check_rows(out, "product")
             if tuple(out.shape) != (x.shape[0], self.n):
                 raise KernelError(f"product with 4-bit weights: the output is {tuple(out.shape)}, not {(x.shape[0], self.n)}")
-        ops.product4(x, self._address, out, act, cap)
+        if x.shape[0] > FEW_ROWS and x.dtype == torch.bfloat16 and self.k % 8 == 0 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0:
+            ops.product4_tc(x, self._address, out, act, cap)
+        else:
+            ops.product4(x, self._address, out, act, cap)
         return out
