@@ -3,10 +3,11 @@
 // The weights are formed in bfloat16 on their way: (c - z) s, c - z exact and the product rounded once (2^-9 of a weight, as a matrix
 // kept in bfloat16 would be), straight into the operand's place in shared memory, so that they cross memory in 4 bits however many
 // rows there are.  A CTA takes 128 features (gated: 128 of gate and the same 128 of up) and up to 256 rows, tcgen05.mma with M = 128
-// features and N = rows: eight warps each form 16 features' 64 numbers a stage (from a ring of codes of their own that cp.async fills)
-// and bring the rows of x, a ninth issues the products.  Few tiles share K as a cluster, whose sums meet in shared memory.
-// Bound by the products where rows fill the tile (2 clocks a row and stage of 64 k), else by forming the weights (some 250 clocks a
-// stage): plan_tiles below chooses rows a tile and CTAs a cluster by these.
+// features and N = rows.  Two groups of eight warps take the stages of 64 k in turn: each warp forms 16 features (its codes wait in
+// registers, asked for two of its turns ahead) and brings its part of the rows of x by cp.async; one more warp issues the products.
+// Few tiles share K as a cluster, whose sums meet in shared memory.
+// Bound by the products where rows fill the tile (2 clocks a row and stage), else by forming the weights: plan_tiles below chooses rows
+// a tile and CTAs a cluster by these.
 #include "common.cuh"
 #include "fourbit.cuh"
 #include "mma_utils.cuh"
@@ -14,8 +15,9 @@
 
 namespace hos {
 
-constexpr int kTcFeatures = 128, kTcRows = 256, kTcMakers = 8, kTcThreads = (kTcMakers + 1) * 32;
+constexpr int kTcFeatures = 128, kTcRows = 256, kTcGroup = 8, kTcMakers = 2 * kTcGroup, kTcThreads = (kTcMakers + 1) * 32;
 constexpr int kTcShared = 226 * 1024, kTcWeights = kTcFeatures * 128;            // bytes of a stage's 128 features
+constexpr double kClocksForm = 500., kClocksRow = 1.5;      // of a stage: 128 features formed, and brought a row
 constexpr long long kProductWaitCycles = 1ll << 31;
 constexpr int kGiveUpProduct4 = 6;
 
@@ -34,13 +36,13 @@ struct Product4Args {
     const uint8_t *codes, *records;
     void* out;
     long long ldx, ldo, wait_cycles;     // wait_cycles: the limit of every wait
-    int out_f32, M, N, K, group_blocks, act, tile_rows, shares, stages;
+    uint32_t group_magic;                // ceil(2^32 / blocks of 64 a group): the group of a block is a product's high half
+    int out_f32, M, N, K, group_blocks, act, tile_rows, shares;
     int stop_stage;                      // for tests of the give-up path: the stage at which the products' warp takes its wait as run out (-1: none)
     float limit;
 };
 
 __host__ __device__ inline int stage_bytes(bool gated, int tile_rows) { return (gated ? 2 : 1) * kTcWeights + tile_rows * 128; }
-__host__ __device__ inline int codes_bytes(bool gated, int sub, bool zeros) { return (gated ? 2 : 1) * (kBlockBytes + sub * (zeros ? 64 : 32)); }
 
 __device__ __forceinline__ float peer_value(uint32_t at, int rank) {
     uint32_t r;
@@ -57,15 +59,14 @@ __device__ __forceinline__ float gated_value(int act, float gate, float up, floa
     return act == 2 ? clamped_swish_fast(gate, up, limit) : (act == 0 ? gelu_tanh_fast(gate) : silu_fast(gate)) * up;
 }
 
-// S: stages of operands, and of codes; SUB: scales a block of 64 (2: groups of 32).
+// S: stages of operands; SUB: scales a block of 64 (2: groups of 32).
 template <int S, bool GATED, int SUB, bool ZEROS>
 __global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(Product4Args p) {
-    constexpr int kAcc = GATED ? 2 : 1, kRecord = ZEROS ? 64 : 32, kTile = kBlockBytes + SUB * kRecord, kCodes = kAcc * kTile;
-    constexpr int P = S - 2;                                 // blocks asked for ahead: the products of the block before the last may still run
+    constexpr int kAcc = GATED ? 2 : 1, kRecord = ZEROS ? 64 : 32;
+    constexpr int P = S >= 6 ? 2 : 1;                        // how many of a group's turns ahead the rows of x are asked for
     extern __shared__ unsigned char smem_unaligned[];
     unsigned char* stages = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_unaligned) + 1023) & ~(uintptr_t)1023);
     const int stage = stage_bytes(GATED, p.tile_rows);
-    unsigned char* rings = stages + S * stage;
     __shared__ uint64_t full[S], empty[S], done;
     __shared__ uint32_t tmem_base_smem;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
@@ -73,7 +74,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(Product4Args
     int tmem_columns = 32;
     while (tmem_columns < kAcc * columns) tmem_columns *= 2;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S; ++s) { mbar_init(&full[s], kTcMakers); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < S; ++s) { mbar_init(&full[s], kTcGroup); mbar_init(&empty[s], 1); }
         mbar_init(&done, 1);
         mbar_fence_init();
     }
@@ -95,70 +96,76 @@ __global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(Product4Args
     auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_cycles(bar, parity, p.wait_cycles); };
 
     if (warp < kTcMakers) {
-        const uint32_t ring = smem_u32(rings) + warp * S * kCodes;
-        const unsigned char* ring_ptr = rings + warp * S * kCodes;
+        const int group = warp / kTcGroup, mine = warp % kTcGroup;
+        struct Codes { uint4 w[kAcc]; uint32_t scale[kAcc][SUB], zero[kAcc][SUB]; };
         const uint8_t *code_at[kAcc], *record_at[kAcc];
 #pragma unroll
         for (int a = 0; a < kAcc; ++a) {                    // a tile beyond the last reads the last one: its sums are dropped
-            const size_t t = (size_t)a * tiles + min(f0 / 16 + warp, tiles - 1);
+            const size_t t = (size_t)a * tiles + min(f0 / 16 + mine, tiles - 1);
             code_at[a] = p.codes + (t * k_blocks + kb0) * kBlockBytes + lane * 16;
-            record_at[a] = p.records + (t * groups + (SUB == 2 ? 2 * kb0 : kb0 / p.group_blocks)) * kRecord + lane * 16;
+            record_at[a] = p.records + t * groups * kRecord + g * (kRecord / 8);
         }
-        int in_group = SUB == 2 ? 1 : p.group_blocks - kb0 % p.group_blocks;
-        // the rows' 16-byte pieces that a thread brings: piece i of row j, j a step of 32 apart
-        const int piece = threadIdx.x & 7, first_row = threadIdx.x >> 3;
-        auto fetch = [&](int i) {                           // block i of this share into place i % S
-            if (i < n_k) {
-                const int s = i % S;
-#pragma unroll
-                for (int a = 0; a < kAcc; ++a) {
-                    const uint32_t to = ring + s * kCodes + a * kTile;
-                    copy16_async(to + lane * 16, code_at[a]);
-                    if (lane < SUB * kRecord / 16) copy16_async(to + kBlockBytes + lane * 16, record_at[a]);
-                    code_at[a] += kBlockBytes;
-                }
-                if (--in_group == 0) {
-                    in_group = SUB == 2 ? 1 : p.group_blocks;
-#pragma unroll
-                    for (int a = 0; a < kAcc; ++a) record_at[a] += SUB * kRecord;
-                }
-                const uint32_t b = smem_u32(stages + s * stage + kAcc * kTcWeights);
-                const int k = (kb0 + i) * 64 + piece * 8;
-                for (int j = first_row; j < p.tile_rows; j += 32) {
-                    const int m = m0 + j;
-                    const bool in = m < p.M && k < p.K;      // K is a multiple of 8: a piece is whole or not there
-                    copy16_async(b + j * 128 + ((piece ^ (j & 7)) << 4), p.x + (in ? (size_t)m * p.ldx + k : 0), in ? 16 : 0);
-                }
-            }
-            copies_commit();
-        };
-#pragma unroll 1
-        for (int i = 0; i < P; ++i) fetch(i);
-        for (int i = 0; i < n_k; ++i) {
-            const int s = i % S, ahead = i + P;
-            if (ahead >= S && ahead < n_k) {                // the place of the block that is asked for now
-                ok = lane != 0 || wait(&empty[ahead % S], ((ahead / S) - 1) & 1);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-            }
-            fetch(ahead);
-            copies_wait<P>();
-            __syncwarp();
+        auto ask = [&](int i, Codes& c) {                   // the codes of block i of this share
+            if (i >= n_k) return;
+            const uint32_t record = (SUB == 2 ? 2u * (kb0 + i) : (p.group_blocks == 1 ? (uint32_t)(kb0 + i) : __umulhi((uint32_t)(kb0 + i), p.group_magic))) * kRecord;
 #pragma unroll
             for (int a = 0; a < kAcc; ++a) {
-                const uint4 w = lds16(ring + s * kCodes + a * kTile + lane * 16);
-                const unsigned char* rec = ring_ptr + s * kCodes + a * kTile + kBlockBytes + g * (kRecord / 8);
-                unsigned char* to = stages + s * stage + a * kTcWeights + warp * 2048 + g * 128;
+                c.w[a] = __ldg(reinterpret_cast<const uint4*>(code_at[a] + (uint32_t)(i * kBlockBytes)));
+#pragma unroll
+                for (int u = 0; u < SUB; ++u) {
+                    const uint8_t* r = record_at[a] + record + u * kRecord;
+                    if (ZEROS) {
+                        const uint2 v = __ldg(reinterpret_cast<const uint2*>(r));
+                        c.scale[a][u] = v.x;
+                        c.zero[a][u] = v.y;
+                    } else {
+                        c.scale[a][u] = __ldg(reinterpret_cast<const uint32_t*>(r));
+                    }
+                }
+            }
+        };
+        // the rows' 16-byte pieces that a thread of a group brings: one piece of every 32nd row, of which it has `mine_rows`; rows
+        // beyond the last are zeros
+        const int piece = threadIdx.x & 7, first_row = (threadIdx.x & 255) >> 3;
+        const int mine_rows = max(0, (p.tile_rows - first_row + 31) / 32), real_rows = max(0, min(mine_rows, (p.M - m0 - first_row + 31) / 32));
+        const uint32_t piece_to = smem_u32(stages) + kAcc * kTcWeights + first_row * 128 + ((piece ^ (first_row & 7)) << 4);
+        const bf16* row_at = p.x + (size_t)min(m0 + first_row, p.M - 1) * p.ldx + kb0 * 64 + piece * 8;
+        const int k_left = p.K - kb0 * 64 - piece * 8;      // K is a multiple of 8: a piece is whole or not there
+        int fetch_s = group % S, fetch_round = -1;          // the place of the block that fetch() is at, and how often it was used before
+        auto fetch = [&](int i) {                           // rows of block i, once its place is free
+            if (i < n_k) {
+                if (i >= S) {
+                    ok = lane != 0 || wait(&empty[fetch_s], fetch_round & 1);
+                    ok = __all_sync(0xffffffffu, ok);
+                }
+                if (ok) {
+                    const uint32_t to = piece_to + fetch_s * stage;
+                    const bf16* from = row_at + (size_t)(i * 64);
+                    const int bytes = i * 64 < k_left ? 16 : 0;
+                    for (int j = 0; j < mine_rows; ++j) {
+                        const bool in = j < real_rows && bytes != 0;
+                        copy16_async(to + j * 4096, in ? from : p.x, in ? 16 : 0);
+                        from += 32 * p.ldx;
+                    }
+                }
+            }
+            fetch_s += 2;
+            if (fetch_s >= S) { fetch_s -= S; ++fetch_round; }
+            copies_commit();
+        };
+        auto form = [&](int s, const Codes& c) {            // a block's weights into place s, which fetch() has waited for
+#pragma unroll
+            for (int a = 0; a < kAcc; ++a) {
+                unsigned char* to = stages + s * stage + a * kTcWeights + mine * 2048 + g * 128;
                 // the k below and from 32 on, in the other order for odd rows: eight lanes then fill all banks
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int half = h ^ (g & 1);
-                    const uint32_t lo = half ? w.y : w.x, hi = half ? w.w : w.z;
-                    const unsigned char* r = rec + (SUB == 2 ? half * kRecord : 0);
-                    const uint32_t two = *(const uint32_t*)r;
+                    const bool upper = h != (g & 1);
+                    const uint32_t lo = upper ? c.w[a].y : c.w[a].x, hi = upper ? c.w[a].w : c.w[a].z;
+                    const uint32_t two = SUB == 2 && upper ? c.scale[a][SUB - 1] : c.scale[a][0];
                     uint32_t z0 = kZero8, z1 = kZero8;
                     if (ZEROS) {
-                        const uint32_t zz = *(const uint32_t*)(r + 4);
+                        const uint32_t zz = SUB == 2 && upper ? c.zero[a][SUB - 1] : c.zero[a][0];
                         z0 = __byte_perm(zz, 0, 0x1010);
                         z1 = __byte_perm(zz, 0, 0x3232);
                     }
@@ -174,21 +181,39 @@ __global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(Product4Args
                         v0[j] = *reinterpret_cast<const uint32_t*>(&y0);
                         v1[j] = *reinterpret_cast<const uint32_t*>(&y1);
                     }
-                    const int chunk = ((4 * half + t4) ^ g) << 4;
+                    const int chunk = (((upper ? 4 : 0) + t4) ^ g) << 4;
                     *reinterpret_cast<uint4*>(to + chunk) = make_uint4(v0[0], v0[1], v0[2], v0[3]);
                     *reinterpret_cast<uint4*>(to + 1024 + chunk) = make_uint4(v1[0], v1[1], v1[2], v1[3]);
                 }
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&full[s]);
+        };
+        Codes codes[2];
+        ask(group, codes[0]);
+        ask(group + 2, codes[1]);
+#pragma unroll 1
+        for (int j = 0; j < P; ++j) fetch(group + 2 * j);
+        int form_s = group;
+        for (int i = group; i < n_k && ok; i += 4) {        // two turns, so that the codes' places are known
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int at = i + 2 * e;
+                if (at < n_k && ok) {
+                    form(form_s, codes[e]);
+                    ask(at + 4, codes[e]);
+                    copies_wait<P - 1>();                   // the block's rows
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&full[form_s]);
+                    form_s += form_s + 2 >= S ? 2 - S : 2;
+                    fetch(at + 2 * P);
+                }
+            }
         }
         copies_wait<0>();
     } else if (lane == 0) {
         const uint32_t idesc = tc_idesc(kTcFeatures, p.tile_rows, 0);
-        for (int i = 0; i < n_k; ++i) {
-            const int s = i % S;
-            ok = wait(&full[s], (i / S) & 1) && i != p.stop_stage;
+        for (int i = 0, s = 0, round = 0; i < n_k; ++i) {
+            ok = wait(&full[s], round & 1) && i != p.stop_stage;
             if (!ok) break;
             tc_fence_after_sync();
             const uint32_t at = smem_u32(stages + s * stage);
@@ -200,6 +225,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(Product4Args
                 for (int k = 0; k < 4; ++k) tc_mma(tmem_base + a * columns, a_desc + 2 * k, b_desc + 2 * k, idesc, (i > 0 || k > 0) ? 1u : 0u);
             }
             tc_commit(&empty[s]);
+            if (++s == S) { s = 0; ++round; }
         }
         if (ok) tc_commit(&done);
     }
@@ -214,7 +240,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(Product4Args
         const int quarter = warp & 3, feature = quarter * 32 + lane, n = f0 + feature;
         const uint32_t from = tmem_base + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll 1
-        for (int c0 = (warp >> 2) * 32; c0 < p.tile_rows; c0 += 64) {
+        for (int c0 = (warp >> 2) * 32; c0 < p.tile_rows; c0 += 128) {
             uint32_t v[32], u[32];
             tc_ld32(from + c0, v);
             if (GATED) tc_ld32(from + columns + c0, u);
@@ -243,7 +269,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(Product4Args
         if (warp < kTcMakers && !gave_up) {
             const int feature = threadIdx.x & 127, n = f0 + feature;
             const uint32_t at = smem_u32(sums);
-            for (int c = 2 * share + (threadIdx.x >> 7); c < p.tile_rows; c += 2 * p.shares) {
+            for (int c = 4 * share + (threadIdx.x >> 7); c < p.tile_rows; c += 4 * p.shares) {
                 float v = 0.f, u = 0.f;
                 for (int s = 0; s < p.shares; ++s) {
                     v += peer_value(at + (c * 128 + feature) * 4, s);
@@ -288,8 +314,33 @@ int launch_product4_tc(const Product4Args& p, int ctas, int smem, cudaStream_t s
     return check_launch("product4_tc");
 }
 
-// Rows of a tile and CTAs that share a tile's K: the least of waves x (stages x clocks a stage + what a tile costs besides), in clocks as
-// above.  Sums of shares have to fit where the operands were.
+// Clusters of `shares` CTAs, one to an SM, that run at once (asked once).
+static int clusters_at_once(int shares) {
+    static int known[9] = {};
+    if (known[shares] == 0) {
+        auto kernel = product4_tc_kernel<4, false, 1, false>;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(shares * 64));
+        cfg.blockDim = dim3(kTcThreads);
+        cfg.dynamicSmemBytes = 128 * 1024;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim = {(unsigned)shares, 1, 1};
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcShared) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
+            cudaGetLastError();
+            n = sm_count_cached() / shares / 2 + 1;
+        }
+        known[shares] = n;
+    }
+    return known[shares];
+}
+
+// Rows of a tile and CTAs that share a tile's K: the least of waves x (stages x clocks a stage + what a tile costs besides), in clocks.
+// Sums of shares have to fit where the operands were.
 static void plan_tiles(int M, int N, int K, bool gated, int& tile_rows, int& shares) {
     const int sm = sm_count_cached(), acc = gated ? 2 : 1, feature_tiles = (N + kTcFeatures - 1) / kTcFeatures, k_blocks = (K + 63) / 64;
     double best = 0.;
@@ -298,9 +349,11 @@ static void plan_tiles(int M, int N, int K, bool gated, int& tile_rows, int& sha
         const int rows = ((M + row_tiles - 1) / row_tiles + 15) / 16 * 16;
         const long long n = (long long)feature_tiles * ((M + rows - 1) / rows);
         for (int s = 1; s <= 8 && s <= k_blocks; s *= 2) {
-            if (s > 1 && (rows > 128 || n * s > sm)) break;
-            const double stage = acc * (rows * 2.1 > 250. ? rows * 2.1 : 250.), blocks = (k_blocks + s - 1) / s;
-            const double cost = (double)((n * s + sm - 1) / sm) * (blocks * stage + 5000. + rows * acc * 12. + (s > 1 ? 3000. : 0.));
+            if (s > 1 && rows > 128) break;
+            const int at_once = s == 1 ? sm : clusters_at_once(s);
+            if (s > 1 && n > at_once) break;
+            const double form = kClocksForm * acc + kClocksRow * rows, stage = rows * 2.1 * acc > form ? rows * 2.1 * acc : form;
+            const double cost = (double)((n + at_once - 1) / at_once) * ((k_blocks + s - 1) / s * stage + 5000. + rows * acc * 12. + (s > 1 ? 3000. : 0.));
             if (tile_rows == 0 || cost < best) { best = cost; tile_rows = rows; shares = s; }
         }
         if (rows == 16) break;
@@ -323,6 +376,7 @@ extern "C" int hos_product4_tc(const void* x, long long ldx, const void* matrix,
     if (M <= 0 || w.n <= 0) return 0;
     if (w.k <= 0 || w.k % 8 || ldx % 8 || (uintptr_t)x % 16) HOS_REFUSE("product4_tc: rows must be 16-byte pieces (K %d, %lld apart)", w.k, ldx);
     if (w.group < 32 || (w.group != 32 && w.group % 64)) HOS_REFUSE("product4_tc: groups of %d weights (32, or a multiple of 64)", w.group);
+    if (w.k > (1 << 21)) HOS_REFUSE("product4_tc: K %d", w.k);
     if (out_dtype != kF32 && out_dtype != kBF16) HOS_REFUSE("product4_tc: no product into type %d", out_dtype);
     if (tile_rows == 0) plan_tiles(M, w.n, w.k, w.gated != 0, tile_rows, shares);
     const int k_blocks = (w.k + 63) / 64, sub = w.group == 32 ? 2 : 1;
@@ -331,11 +385,12 @@ extern "C" int hos_product4_tc(const void* x, long long ldx, const void* matrix,
     Product4Args p = {};
     p.x = (const bf16*)x; p.codes = w.codes; p.records = w.records; p.out = out; p.ldx = ldx; p.ldo = ldo;
     p.wait_cycles = wait_cycles > 0 ? wait_cycles : kProductWaitCycles;
-    p.out_f32 = out_dtype == kF32; p.M = M; p.N = w.n; p.K = w.k; p.group_blocks = w.group / 64; p.act = act; p.limit = limit;
+    p.out_f32 = out_dtype == kF32; p.M = M; p.N = w.n; p.K = w.k; p.group_blocks = w.group / 64;
+    p.group_magic = p.group_blocks > 1 ? (uint32_t)(((1ull << 32) + p.group_blocks - 1) / p.group_blocks) : 0u; p.act = act; p.limit = limit;
     p.tile_rows = tile_rows; p.shares = shares; p.stop_stage = stop_stage;
     const long long ctas = (long long)((w.n + kTcFeatures - 1) / kTcFeatures) * ((M + tile_rows - 1) / tile_rows) * shares;
     if (ctas > 0x7fffffffll) HOS_REFUSE("product4_tc: %d rows", M);
-    const int a_stage = stage_bytes(w.gated, tile_rows) + kTcMakers * codes_bytes(w.gated, sub, w.zeros);
+    const int a_stage = stage_bytes(w.gated, tile_rows);
     const int S = 6 * a_stage + 1024 <= kTcShared ? 6 : (4 * a_stage + 1024 <= kTcShared ? 4 : 3), smem = S * a_stage + 1024;
 #define HOS_PT(SS, G, U, Z) return launch_product4_tc<SS, G, U, Z>(p, (int)ctas, smem, stream)
 #define HOS_PT_S(G, U, Z) do { if (S == 6) HOS_PT(6, G, U, Z); else if (S == 4) HOS_PT(4, G, U, Z); else HOS_PT(3, G, U, Z); } while (0)
