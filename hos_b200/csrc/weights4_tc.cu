@@ -3,8 +3,9 @@
 // The weights are formed in bfloat16 on their way: (c - z) s, c - z exact and the product rounded once (2^-9 of a weight, as a matrix
 // kept in bfloat16 would be), straight into the operand's place in shared memory, so that they cross memory in 4 bits however many
 // rows there are.  A CTA takes 128 features (gated: 128 of gate and the same 128 of up) and up to 256 rows, tcgen05.mma with M = 128
-// features and N = rows.  Two groups of eight warps take the stages of 64 k in turn: each warp forms 16 features (its codes wait in
-// registers, asked for two of its turns ahead) and brings its part of the rows of x by cp.async; one more warp issues the products.
+// features and N = rows.  Three groups of eight warps take the stages of 64 k in turn: each warp forms 16 features (its codes wait in
+// registers, asked for a turn ahead); one more warp brings the rows of x by TMA, and one issues the products.  (With the rows
+// brought by the makers' cp.async the fence behind what they form waited for those copies too: 2304 x 9216, 64 rows on one SM a tile 64 us.)
 // Few tiles share K as a cluster, whose sums meet in shared memory.
 // Bound by the products where rows fill the tile (2 clocks a row and stage), else by forming the weights: plan_tiles below chooses rows
 // a tile and CTAs a cluster by these.
@@ -15,7 +16,7 @@
 
 namespace hos {
 
-constexpr int kTcFeatures = 128, kTcRows = 256, kTcGroup = 8, kTcMakers = 2 * kTcGroup, kTcThreads = (kTcMakers + 1) * 32;
+constexpr int kTcFeatures = 128, kTcRows = 256, kTcGroup = 8, kTcGroups = 3, kTcMakers = kTcGroups * kTcGroup, kTcThreads = (kTcMakers + 2) * 32;
 constexpr int kTcShared = 226 * 1024, kTcWeights = kTcFeatures * 128;            // bytes of a stage's 128 features
 constexpr double kClocksForm = 500., kClocksRow = 1.5;      // of a stage: 128 features formed, and brought a row
 constexpr long long kProductWaitCycles = 1ll << 31;
@@ -32,10 +33,9 @@ __device__ __forceinline__ void product4_give_up() {
 }
 
 struct Product4Args {
-    const bf16* x;
     const uint8_t *codes, *records;
     void* out;
-    long long ldx, ldo, wait_cycles;     // wait_cycles: the limit of every wait
+    long long ldo, wait_cycles;     // wait_cycles: the limit of every wait
     uint32_t group_magic;                // ceil(2^32 / blocks of 64 a group): the group of a block is a product's high half
     int out_f32, M, N, K, group_blocks, act, tile_rows, shares;
     int stop_stage;                      // for tests of the give-up path: the stage at which the products' warp takes its wait as run out (-1: none)
@@ -43,6 +43,40 @@ struct Product4Args {
 };
 
 __host__ __device__ inline int stage_bytes(bool gated, int tile_rows) { return (gated ? 2 : 1) * kTcWeights + tile_rows * 128; }
+
+// As mbar_wait_cycles, asleep for up to two microseconds at a time: a warp that polls takes issue slots from those that form weights.
+__device__ __forceinline__ bool wait_asleep(uint64_t* bar, uint32_t parity, long long limit) {
+    const long long t0 = clock64();
+    do {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity), "r"(2000u)
+            : "memory");
+        if (ok != 0) return true;
+    } while (clock64() - t0 <= limit);
+    return false;
+}
+
+// Loads that stay where they are written, ahead of their use.
+__device__ __forceinline__ uint4 load_now16(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint2 load_now8(const void* p) {
+    uint2 v;
+    asm volatile("ld.global.nc.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t load_now4(const void* p) {
+    uint32_t v;
+    asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
 
 __device__ __forceinline__ float peer_value(uint32_t at, int rank) {
     uint32_t r;
@@ -61,9 +95,8 @@ __device__ __forceinline__ float gated_value(int act, float gate, float up, floa
 
 // S: stages of operands; SUB: scales a block of 64 (2: groups of 32).
 template <int S, bool GATED, int SUB, bool ZEROS>
-__global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(Product4Args p) {
+__global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(const __grid_constant__ CUtensorMap rows_map, Product4Args p) {
     constexpr int kAcc = GATED ? 2 : 1, kRecord = ZEROS ? 64 : 32;
-    constexpr int P = S >= 6 ? 2 : 1;                        // how many of a group's turns ahead the rows of x are asked for
     extern __shared__ unsigned char smem_unaligned[];
     unsigned char* stages = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_unaligned) + 1023) & ~(uintptr_t)1023);
     const int stage = stage_bytes(GATED, p.tile_rows);
@@ -74,7 +107,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(Product4Args
     int tmem_columns = 32;
     while (tmem_columns < kAcc * columns) tmem_columns *= 2;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S; ++s) { mbar_init(&full[s], kTcGroup); mbar_init(&empty[s], 1); }
+        for (int s = 0; s < S; ++s) { mbar_init(&full[s], kTcGroup + 1); mbar_init(&empty[s], 1); }
         mbar_init(&done, 1);
         mbar_fence_init();
     }
@@ -93,7 +126,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(Product4Args
     const int share = blockIdx.x % p.shares, tile = blockIdx.x / p.shares, f0 = tile % feature_tiles * kTcFeatures, m0 = tile / feature_tiles * p.tile_rows;
     const int kb0 = (int)((long long)share * k_blocks / p.shares), n_k = (int)((long long)(share + 1) * k_blocks / p.shares) - kb0;
     bool ok = true;
-    auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_cycles(bar, parity, p.wait_cycles); };
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_asleep(bar, parity, p.wait_cycles); };
 
     if (warp < kTcMakers) {
         const int group = warp / kTcGroup, mine = warp % kTcGroup;
@@ -110,50 +143,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(Product4Args
             const uint32_t record = (SUB == 2 ? 2u * (kb0 + i) : (p.group_blocks == 1 ? (uint32_t)(kb0 + i) : __umulhi((uint32_t)(kb0 + i), p.group_magic))) * kRecord;
 #pragma unroll
             for (int a = 0; a < kAcc; ++a) {
-                c.w[a] = __ldg(reinterpret_cast<const uint4*>(code_at[a] + (uint32_t)(i * kBlockBytes)));
+                c.w[a] = load_now16(code_at[a] + (uint32_t)(i * kBlockBytes));
 #pragma unroll
                 for (int u = 0; u < SUB; ++u) {
                     const uint8_t* r = record_at[a] + record + u * kRecord;
                     if (ZEROS) {
-                        const uint2 v = __ldg(reinterpret_cast<const uint2*>(r));
+                        const uint2 v = load_now8(r);
                         c.scale[a][u] = v.x;
                         c.zero[a][u] = v.y;
                     } else {
-                        c.scale[a][u] = __ldg(reinterpret_cast<const uint32_t*>(r));
+                        c.scale[a][u] = load_now4(r);
                     }
                 }
             }
         };
-        // the rows' 16-byte pieces that a thread of a group brings: one piece of every 32nd row, of which it has `mine_rows`; rows
-        // beyond the last are zeros
-        const int piece = threadIdx.x & 7, first_row = (threadIdx.x & 255) >> 3;
-        const int mine_rows = max(0, (p.tile_rows - first_row + 31) / 32), real_rows = max(0, min(mine_rows, (p.M - m0 - first_row + 31) / 32));
-        const uint32_t piece_to = smem_u32(stages) + kAcc * kTcWeights + first_row * 128 + ((piece ^ (first_row & 7)) << 4);
-        const bf16* row_at = p.x + (size_t)min(m0 + first_row, p.M - 1) * p.ldx + kb0 * 64 + piece * 8;
-        const int k_left = p.K - kb0 * 64 - piece * 8;      // K is a multiple of 8: a piece is whole or not there
-        int fetch_s = group % S, fetch_round = -1;          // the place of the block that fetch() is at, and how often it was used before
-        auto fetch = [&](int i) {                           // rows of block i, once its place is free
-            if (i < n_k) {
-                if (i >= S) {
-                    ok = lane != 0 || wait(&empty[fetch_s], fetch_round & 1);
-                    ok = __all_sync(0xffffffffu, ok);
-                }
-                if (ok) {
-                    const uint32_t to = piece_to + fetch_s * stage;
-                    const bf16* from = row_at + (size_t)(i * 64);
-                    const int bytes = i * 64 < k_left ? 16 : 0;
-                    for (int j = 0; j < mine_rows; ++j) {
-                        const bool in = j < real_rows && bytes != 0;
-                        copy16_async(to + j * 4096, in ? from : p.x, in ? 16 : 0);
-                        from += 32 * p.ldx;
-                    }
-                }
-            }
-            fetch_s += 2;
-            if (fetch_s >= S) { fetch_s -= S; ++fetch_round; }
-            copies_commit();
-        };
-        auto form = [&](int s, const Codes& c) {            // a block's weights into place s, which fetch() has waited for
+        auto form = [&](int s, const Codes& c) {            // a block's weights into place s
 #pragma unroll
             for (int a = 0; a < kAcc; ++a) {
                 unsigned char* to = stages + s * stage + a * kTcWeights + mine * 2048 + g * 128;
@@ -187,40 +191,44 @@ __global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(Product4Args
                 }
             }
         };
-        Codes codes[2];
-        ask(group, codes[0]);
-        ask(group + 2, codes[1]);
-#pragma unroll 1
-        for (int j = 0; j < P; ++j) fetch(group + 2 * j);
-        int form_s = group;
-        for (int i = group; i < n_k && ok; i += 4) {        // two turns, so that the codes' places are known
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int at = i + 2 * e;
-                if (at < n_k && ok) {
-                    form(form_s, codes[e]);
-                    ask(at + 4, codes[e]);
-                    copies_wait<P - 1>();                   // the block's rows
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&full[form_s]);
-                    form_s += form_s + 2 >= S ? 2 - S : 2;
-                    fetch(at + 2 * P);
-                }
+        Codes codes;
+        ask(group, codes);
+        int s = group % S, round = group / S - 1;           // the block's place, and how often it was used before
+        for (int i = group; i < n_k; i += kTcGroups) {
+            if (i >= S) {
+                ok = lane != 0 || wait(&empty[s], round & 1);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+            }
+            form(s, codes);
+            ask(i + kTcGroups, codes);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[s]);
+            s += kTcGroups;
+            if (s >= S) { s -= S; ++round; }
+        }
+    } else if (warp == kTcMakers + 1) {
+        if (lane == 0) {
+            for (int i = 0, s = 0, round = -1; i < n_k; ++i) {
+                if (i >= S) ok = wait(&empty[s], round & 1);
+                if (!ok) break;
+                mbar_expect_tx(&full[s], p.tile_rows * 128);
+                tc_tma_2d(stages + s * stage + kAcc * kTcWeights, &rows_map, (kb0 + i) * 64, m0, &full[s]);
+                if (++s == S) { s = 0; ++round; }
             }
         }
-        copies_wait<0>();
     } else if (lane == 0) {
         const uint32_t idesc = tc_idesc(kTcFeatures, p.tile_rows, 0);
+        const uint64_t weights0 = desc_kmajor(smem_u32(stages)), rows0 = desc_kmajor(smem_u32(stages) + kAcc * kTcWeights);
         for (int i = 0, s = 0, round = 0; i < n_k; ++i) {
             ok = wait(&full[s], round & 1) && i != p.stop_stage;
             if (!ok) break;
             tc_fence_after_sync();
-            const uint32_t at = smem_u32(stages + s * stage);
-            const uint64_t b_desc = desc_kmajor(at + kAcc * kTcWeights);
+            const uint64_t off = (uint32_t)(s * stage) >> 4, b_desc = rows0 + off;
 #pragma unroll
             for (int a = 0; a < kAcc; ++a) {
-                const uint64_t a_desc = desc_kmajor(at + a * kTcWeights);
+                const uint64_t a_desc = weights0 + off + a * (kTcWeights >> 4);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) tc_mma(tmem_base + a * columns, a_desc + 2 * k, b_desc + 2 * k, idesc, (i > 0 || k > 0) ? 1u : 0u);
             }
@@ -240,7 +248,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(Product4Args
         const int quarter = warp & 3, feature = quarter * 32 + lane, n = f0 + feature;
         const uint32_t from = tmem_base + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll 1
-        for (int c0 = (warp >> 2) * 32; c0 < p.tile_rows; c0 += 128) {
+        for (int c0 = (warp >> 2) * 32; c0 < p.tile_rows; c0 += kTcMakers * 8) {
             uint32_t v[32], u[32];
             tc_ld32(from + c0, v);
             if (GATED) tc_ld32(from + columns + c0, u);
@@ -269,7 +277,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(Product4Args
         if (warp < kTcMakers && !gave_up) {
             const int feature = threadIdx.x & 127, n = f0 + feature;
             const uint32_t at = smem_u32(sums);
-            for (int c = 4 * share + (threadIdx.x >> 7); c < p.tile_rows; c += 4 * p.shares) {
+            for (int c = kTcMakers / 4 * share + (threadIdx.x >> 7); c < p.tile_rows; c += kTcMakers / 4 * p.shares) {
                 float v = 0.f, u = 0.f;
                 for (int s = 0; s < p.shares; ++s) {
                     v += peer_value(at + (c * 128 + feature) * 4, s);
@@ -291,7 +299,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(Product4Args
 }
 
 template <int S, bool GATED, int SUB, bool ZEROS>
-int launch_product4_tc(const Product4Args& p, int ctas, int smem, cudaStream_t stream) {
+int launch_product4_tc(const CUtensorMap& rows_map, const Product4Args& p, int ctas, int smem, cudaStream_t stream) {
     auto kernel = product4_tc_kernel<S, GATED, SUB, ZEROS>;
     static bool set = false;                                 // once per kernel: the attribute stays
     if (!set) {
@@ -310,7 +318,7 @@ int launch_product4_tc(const Product4Args& p, int ctas, int smem, cudaStream_t s
     attr[1].val.clusterDim = {(unsigned)p.shares, 1, 1};
     cfg.attrs = attr;
     cfg.numAttrs = p.shares > 1 ? 2 : 1;
-    cudaLaunchKernelEx(&cfg, kernel, p);
+    cudaLaunchKernelEx(&cfg, kernel, rows_map, p);
     return check_launch("product4_tc");
 }
 
@@ -374,7 +382,7 @@ extern "C" int hos_product4_tc(const void* x, long long ldx, const void* matrix,
     struct Matrix4 { const uint8_t *codes, *records; int n, k, group, zeros, gated; };
     const Matrix4 w = *(const Matrix4*)matrix;
     if (M <= 0 || w.n <= 0) return 0;
-    if (w.k <= 0 || w.k % 8 || ldx % 8 || (uintptr_t)x % 16) HOS_REFUSE("product4_tc: rows must be 16-byte pieces (K %d, %lld apart)", w.k, ldx);
+    if (w.k < 64 || w.k % 8 || ldx % 8 || (uintptr_t)x % 16) HOS_REFUSE("product4_tc: rows must be 16-byte pieces (K %d, %lld apart)", w.k, ldx);
     if (w.group < 32 || (w.group != 32 && w.group % 64)) HOS_REFUSE("product4_tc: groups of %d weights (32, or a multiple of 64)", w.group);
     if (w.k > (1 << 21)) HOS_REFUSE("product4_tc: K %d", w.k);
     if (out_dtype != kF32 && out_dtype != kBF16) HOS_REFUSE("product4_tc: no product into type %d", out_dtype);
@@ -383,7 +391,9 @@ extern "C" int hos_product4_tc(const void* x, long long ldx, const void* matrix,
     if (tile_rows < 16 || tile_rows > kTcRows || tile_rows % 16 || shares < 1 || shares > 8 || shares > k_blocks || (shares > 1 && tile_rows > 128))
         HOS_REFUSE("product4_tc: tiles of %d rows in %d shares", tile_rows, shares);
     Product4Args p = {};
-    p.x = (const bf16*)x; p.codes = w.codes; p.records = w.records; p.out = out; p.ldx = ldx; p.ldo = ldo;
+    CUtensorMap rows_map;                                    // boxes of 64 numbers of tile_rows rows; what is beyond them reads as zeros
+    if (int rc = tc_make_map(&rows_map, x, M, w.k, (int)ldx, tile_rows)) return rc;
+    p.codes = w.codes; p.records = w.records; p.out = out; p.ldo = ldo;
     p.wait_cycles = wait_cycles > 0 ? wait_cycles : kProductWaitCycles;
     p.out_f32 = out_dtype == kF32; p.M = M; p.N = w.n; p.K = w.k; p.group_blocks = w.group / 64;
     p.group_magic = p.group_blocks > 1 ? (uint32_t)(((1ull << 32) + p.group_blocks - 1) / p.group_blocks) : 0u; p.act = act; p.limit = limit;
@@ -392,7 +402,7 @@ extern "C" int hos_product4_tc(const void* x, long long ldx, const void* matrix,
     if (ctas > 0x7fffffffll) HOS_REFUSE("product4_tc: %d rows", M);
     const int a_stage = stage_bytes(w.gated, tile_rows);
     const int S = 6 * a_stage + 1024 <= kTcShared ? 6 : (4 * a_stage + 1024 <= kTcShared ? 4 : 3), smem = S * a_stage + 1024;
-#define HOS_PT(SS, G, U, Z) return launch_product4_tc<SS, G, U, Z>(p, (int)ctas, smem, stream)
+#define HOS_PT(SS, G, U, Z) return launch_product4_tc<SS, G, U, Z>(rows_map, p, (int)ctas, smem, stream)
 #define HOS_PT_S(G, U, Z) do { if (S == 6) HOS_PT(6, G, U, Z); else if (S == 4) HOS_PT(4, G, U, Z); else HOS_PT(3, G, U, Z); } while (0)
 #define HOS_PT_U(G, Z) do { if (sub == 2) HOS_PT_S(G, 2, Z); else HOS_PT_S(G, 1, Z); } while (0)
 #define HOS_PT_Z(G) do { if (w.zeros) HOS_PT_U(G, true); else HOS_PT_U(G, false); } while (0)

@@ -112,7 +112,7 @@ class Weight4:
             ops._check_rows(out, "product")
             if tuple(out.shape) != (x.shape[0], self.n):
                 raise KernelError(f"product with 4-bit weights: the output is {tuple(out.shape)}, not {(x.shape[0], self.n)}")
-        if x.shape[0] > FEW_ROWS and x.dtype == torch.bfloat16 and self.k % 8 == 0 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0:
+        if x.shape[0] > FEW_ROWS and x.dtype == torch.bfloat16 and self.k >= COLS and self.k % 8 == 0 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0:
             ops.product4_tc(x, self._address, out, act, cap)
         else:
             ops.product4(x, self._address, out, act, cap)
