@@ -89,6 +89,16 @@ __device__ __forceinline__ void shares_meet() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// 16 columns of a warp's 32 lanes of tensor memory.
+__device__ __forceinline__ void tc_ld16(uint32_t at, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(at)
+        : "memory");
+}
+
 __device__ __forceinline__ float gated_value(int act, float gate, float up, float limit) {
     return act == 2 ? clamped_swish_fast(gate, up, limit) : (act == 0 ? gelu_tanh_fast(gate) : silu_fast(gate)) * up;
 }
@@ -130,69 +140,65 @@ __global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(const __grid
 
     if (warp < kTcMakers) {
         const int group = warp / kTcGroup, mine = warp % kTcGroup;
-        struct Codes { uint4 w[kAcc]; uint32_t scale[kAcc][SUB], zero[kAcc][SUB]; };
-        const uint8_t *code_at[kAcc], *record_at[kAcc];
+        // where the codes of gate's, or of up's, block kb are: a tile beyond the last reads the last one, and its sums are dropped
+        uint32_t code_at[kAcc], record_at[kAcc];
 #pragma unroll
-        for (int a = 0; a < kAcc; ++a) {                    // a tile beyond the last reads the last one: its sums are dropped
-            const size_t t = (size_t)a * tiles + min(f0 / 16 + mine, tiles - 1);
-            code_at[a] = p.codes + (t * k_blocks + kb0) * kBlockBytes + lane * 16;
-            record_at[a] = p.records + t * groups * kRecord + g * (kRecord / 8);
+        for (int a = 0; a < kAcc; ++a) {
+            const uint32_t t = a * tiles + min(f0 / 16 + mine, tiles - 1);
+            code_at[a] = (t * k_blocks + kb0) * kBlockBytes + lane * 16;
+            record_at[a] = t * groups * kRecord + g * (kRecord / 8);
         }
-        auto ask = [&](int i, Codes& c) {                   // the codes of block i of this share
+        uint4 codes[kAcc];
+        uint32_t scale[kAcc][SUB], zero[kAcc][SUB];
+        auto ask = [&](int a, int i) {                      // the codes of block i of this share
             if (i >= n_k) return;
-            const uint32_t record = (SUB == 2 ? 2u * (kb0 + i) : (p.group_blocks == 1 ? (uint32_t)(kb0 + i) : __umulhi((uint32_t)(kb0 + i), p.group_magic))) * kRecord;
+            const uint32_t kb = kb0 + i, record = (SUB == 2 ? 2u * kb : (p.group_blocks == 1 ? kb : __umulhi(kb, p.group_magic))) * kRecord;
+            codes[a] = load_now16(p.codes + (code_at[a] + i * kBlockBytes));
 #pragma unroll
-            for (int a = 0; a < kAcc; ++a) {
-                c.w[a] = load_now16(code_at[a] + (uint32_t)(i * kBlockBytes));
-#pragma unroll
-                for (int u = 0; u < SUB; ++u) {
-                    const uint8_t* r = record_at[a] + record + u * kRecord;
-                    if (ZEROS) {
-                        const uint2 v = load_now8(r);
-                        c.scale[a][u] = v.x;
-                        c.zero[a][u] = v.y;
-                    } else {
-                        c.scale[a][u] = load_now4(r);
-                    }
+            for (int u = 0; u < SUB; ++u) {
+                const uint8_t* r = p.records + (record_at[a] + record + u * kRecord);
+                if (ZEROS) {
+                    const uint2 v = load_now8(r);
+                    scale[a][u] = v.x;
+                    zero[a][u] = v.y;
+                } else {
+                    scale[a][u] = load_now4(r);
                 }
             }
         };
-        auto form = [&](int s, const Codes& c) {            // a block's weights into place s
+        auto form = [&](int a, int s) {                     // a block's weights into place s
+            unsigned char* to = stages + s * stage + a * kTcWeights + mine * 2048 + g * 128;
+            // the k below and from 32 on, in the other order for odd rows: eight lanes then fill all banks
 #pragma unroll
-            for (int a = 0; a < kAcc; ++a) {
-                unsigned char* to = stages + s * stage + a * kTcWeights + mine * 2048 + g * 128;
-                // the k below and from 32 on, in the other order for odd rows: eight lanes then fill all banks
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const bool upper = h != (g & 1);
-                    const uint32_t lo = upper ? c.w[a].y : c.w[a].x, hi = upper ? c.w[a].w : c.w[a].z;
-                    const uint32_t two = SUB == 2 && upper ? c.scale[a][SUB - 1] : c.scale[a][0];
-                    uint32_t z0 = kZero8, z1 = kZero8;
-                    if (ZEROS) {
-                        const uint32_t zz = SUB == 2 && upper ? c.zero[a][SUB - 1] : c.zero[a][0];
-                        z0 = __byte_perm(zz, 0, 0x1010);
-                        z1 = __byte_perm(zz, 0, 0x3232);
-                    }
-                    const uint32_t s0 = __byte_perm(two, 0, 0x1010), s1 = __byte_perm(two, 0, 0x3232);
-                    const __nv_bfloat162 sc0 = *reinterpret_cast<const __nv_bfloat162*>(&s0), sc1 = *reinterpret_cast<const __nv_bfloat162*>(&s1);
-                    uint32_t v0[4], v1[4];
-                    codes_to_bf16<true>(lo, z0, v0);
-                    codes_to_bf16<true>(hi, z1, v1);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const __nv_bfloat162 y0 = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&v0[j]), sc0);
-                        const __nv_bfloat162 y1 = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&v1[j]), sc1);
-                        v0[j] = *reinterpret_cast<const uint32_t*>(&y0);
-                        v1[j] = *reinterpret_cast<const uint32_t*>(&y1);
-                    }
-                    const int chunk = (((upper ? 4 : 0) + t4) ^ g) << 4;
-                    *reinterpret_cast<uint4*>(to + chunk) = make_uint4(v0[0], v0[1], v0[2], v0[3]);
-                    *reinterpret_cast<uint4*>(to + 1024 + chunk) = make_uint4(v1[0], v1[1], v1[2], v1[3]);
+            for (int h = 0; h < 2; ++h) {
+                const bool upper = h != (g & 1);
+                const uint32_t lo = upper ? codes[a].y : codes[a].x, hi = upper ? codes[a].w : codes[a].z;
+                const uint32_t two = SUB == 2 && upper ? scale[a][SUB - 1] : scale[a][0];
+                uint32_t z0 = kZero8, z1 = kZero8;
+                if (ZEROS) {
+                    const uint32_t zz = SUB == 2 && upper ? zero[a][SUB - 1] : zero[a][0];
+                    z0 = __byte_perm(zz, 0, 0x1010);
+                    z1 = __byte_perm(zz, 0, 0x3232);
                 }
+                const uint32_t s0 = __byte_perm(two, 0, 0x1010), s1 = __byte_perm(two, 0, 0x3232);
+                const __nv_bfloat162 sc0 = *reinterpret_cast<const __nv_bfloat162*>(&s0), sc1 = *reinterpret_cast<const __nv_bfloat162*>(&s1);
+                uint32_t v0[4], v1[4];
+                codes_to_bf16<true>(lo, z0, v0);
+                codes_to_bf16<true>(hi, z1, v1);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const __nv_bfloat162 y0 = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&v0[j]), sc0);
+                    const __nv_bfloat162 y1 = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&v1[j]), sc1);
+                    v0[j] = *reinterpret_cast<const uint32_t*>(&y0);
+                    v1[j] = *reinterpret_cast<const uint32_t*>(&y1);
+                }
+                const int chunk = (((upper ? 4 : 0) + t4) ^ g) << 4;
+                *reinterpret_cast<uint4*>(to + chunk) = make_uint4(v0[0], v0[1], v0[2], v0[3]);
+                *reinterpret_cast<uint4*>(to + 1024 + chunk) = make_uint4(v1[0], v1[1], v1[2], v1[3]);
             }
         };
-        Codes codes;
-        ask(group, codes);
+#pragma unroll
+        for (int a = 0; a < kAcc; ++a) ask(a, group);
         int s = group % S, round = group / S - 1;           // the block's place, and how often it was used before
         for (int i = group; i < n_k; i += kTcGroups) {
             if (i >= S) {
@@ -200,8 +206,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(const __grid
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
             }
-            form(s, codes);
-            ask(i + kTcGroups, codes);
+#pragma unroll
+            for (int a = 0; a < kAcc; ++a) {
+                form(a, s);
+                ask(a, i + kTcGroups);
+            }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(&full[s]);
@@ -248,20 +257,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(const __grid
         const int quarter = warp & 3, feature = quarter * 32 + lane, n = f0 + feature;
         const uint32_t from = tmem_base + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll 1
-        for (int c0 = (warp >> 2) * 32; c0 < p.tile_rows; c0 += kTcMakers * 8) {
-            uint32_t v[32], u[32];
-            tc_ld32(from + c0, v);
-            if (GATED) tc_ld32(from + columns + c0, u);
+        for (int c0 = (warp >> 2) * 16; c0 < p.tile_rows; c0 += kTcMakers * 4) {      // tile_rows is a multiple of 16
+            uint32_t v[16], u[16];
+            tc_ld16(from + c0, v);
+            if (GATED) tc_ld16(from + columns + c0, u);
             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
+            for (int j = 0; j < 16; ++j) {
                 const int c = c0 + j, m = m0 + c;
                 if (p.shares > 1) {
-                    if (c < p.tile_rows) {
-                        sums[c * 128 + feature] = __uint_as_float(v[j]);
-                        if (GATED) sums[(p.tile_rows + c) * 128 + feature] = __uint_as_float(u[j]);
-                    }
-                } else if (c < p.tile_rows && m < p.M && n < p.N) {
+                    sums[c * 128 + feature] = __uint_as_float(v[j]);
+                    if (GATED) sums[(p.tile_rows + c) * 128 + feature] = __uint_as_float(u[j]);
+                } else if (m < p.M && n < p.N) {
                     const float y = GATED ? gated_value(p.act, __uint_as_float(v[j]), __uint_as_float(u[j]), p.limit) : __uint_as_float(v[j]);
                     if (p.out_f32) ((float*)p.out)[(size_t)m * p.ldo + n] = y;
                     else ((bf16*)p.out)[(size_t)m * p.ldo + n] = __float2bfloat16_rn(y);
@@ -384,7 +391,8 @@ extern "C" int hos_product4_tc(const void* x, long long ldx, const void* matrix,
     if (M <= 0 || w.n <= 0) return 0;
     if (w.k < 64 || w.k % 8 || ldx % 8 || (uintptr_t)x % 16) HOS_REFUSE("product4_tc: rows must be 16-byte pieces (K %d, %lld apart)", w.k, ldx);
     if (w.group < 32 || (w.group != 32 && w.group % 64)) HOS_REFUSE("product4_tc: groups of %d weights (32, or a multiple of 64)", w.group);
-    if (w.k > (1 << 21)) HOS_REFUSE("product4_tc: K %d", w.k);
+    if (w.k > (1 << 21) || (long long)(w.gated ? 2 : 1) * ((w.n + 15) / 16) * ((w.k + 63) / 64) * kBlockBytes >= (1ll << 32))
+        HOS_REFUSE("product4_tc: %d x %d weights are more than 4 GB of codes, or k more than %d", w.n, w.k, 1 << 21);
     if (out_dtype != kF32 && out_dtype != kBF16) HOS_REFUSE("product4_tc: no product into type %d", out_dtype);
     if (tile_rows == 0) plan_tiles(M, w.n, w.k, w.gated != 0, tile_rows, shares);
     const int k_blocks = (w.k + 63) / 64, sub = w.group == 32 ? 2 : 1;
