@@ -45,20 +45,23 @@ struct Product4Args {
 __host__ __device__ inline int stage_bytes(bool gated, int tile_rows) { return (gated ? 2 : 1) * kTcWeights + tile_rows * 128; }
 
 // As mbar_wait_cycles, asleep for up to two microseconds at a time: a warp that polls takes issue slots from those that form weights.
+__device__ __forceinline__ bool try_wait_asleep(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(2000u)
+        : "memory");
+    return ok != 0;
+}
 __device__ __forceinline__ bool wait_asleep(uint64_t* bar, uint32_t parity, long long limit) {
+    if (try_wait_asleep(bar, parity)) return true;
     const long long t0 = clock64();
-    do {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok)
-            : "r"(smem_u32(bar)), "r"(parity), "r"(2000u)
-            : "memory");
-        if (ok != 0) return true;
-    } while (clock64() - t0 <= limit);
-    return false;
+    while (!try_wait_asleep(bar, parity))
+        if (clock64() - t0 > limit) return false;
+    return true;
 }
 
 // Loads that stay where they are written, ahead of their use.
@@ -227,24 +230,30 @@ __global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(const __grid
                 if (++s == S) { s = 0; ++round; }
             }
         }
-    } else if (lane == 0) {
-        const uint32_t idesc = tc_idesc(kTcFeatures, p.tile_rows, 0);
+    } else {
+        // the warp walks together and one lane issues: what the products take is then in uniform registers
+        const uint32_t idesc = tc_idesc(kTcFeatures, p.tile_rows, 0), step = (uint32_t)stage >> 4;
         const uint64_t weights0 = desc_kmajor(smem_u32(stages)), rows0 = desc_kmajor(smem_u32(stages) + kAcc * kTcWeights);
+        uint32_t leader;
+        asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(leader));
+        uint32_t off = 0;
         for (int i = 0, s = 0, round = 0; i < n_k; ++i) {
-            ok = wait(&full[s], round & 1) && i != p.stop_stage;
+            ok = __all_sync(0xffffffffu, mbar_wait_cycles(&full[s], round & 1, p.wait_cycles)) && i != p.stop_stage;
             if (!ok) break;
             tc_fence_after_sync();
-            const uint64_t off = (uint32_t)(s * stage) >> 4, b_desc = rows0 + off;
+            if (leader) {
 #pragma unroll
-            for (int a = 0; a < kAcc; ++a) {
-                const uint64_t a_desc = weights0 + off + a * (kTcWeights >> 4);
+                for (int a = 0; a < kAcc; ++a)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) tc_mma(tmem_base + a * columns, a_desc + 2 * k, b_desc + 2 * k, idesc, (i > 0 || k > 0) ? 1u : 0u);
+                    for (int k = 0; k < 4; ++k)
+                        tc_mma(tmem_base + a * columns, weights0 + off + a * (kTcWeights >> 4) + 2 * k, rows0 + off + 2 * k, idesc, (i > 0 || k > 0) ? 1u : 0u);
+                tc_commit(&empty[s]);
             }
-            tc_commit(&empty[s]);
-            if (++s == S) { s = 0; ++round; }
+            __syncwarp();
+            off += step;
+            if (++s == S) { s = 0; off = 0; ++round; }
         }
-        if (ok) tc_commit(&done);
+        if (ok && leader) tc_commit(&done);
     }
     __syncwarp();
     if (warp < kTcMakers && ok) {
