@@ -5,25 +5,9 @@
 // All numbers alike (s 0 or below the smallest normal number): codes 0, the value m.  A NaN, an infinity or a range that
 // overflows makes the 64 numbers NaN.  Divisions and roundings are IEEE's, so that a value is a function of its row alone.
 // A page's tile of a kv head is laid out in fourbit.cuh: keys "by row", values "by column".
-#include "common.cuh"
-#include "fourbit.cuh"
-#include "kv_layout.cuh"
-#include "mma_utils.cuh"
+#include "attention4.cuh"
 
 namespace hos {
-
-// One call's view of the pages, as the host hands it over (ops.Paged4).
-struct Paged4 {
-    uint8_t* k_pages;
-    uint8_t* v_pages;
-    const int* page_table;
-    int table_stride, ring_pages, n_kv_heads, head_dim;
-};
-
-__device__ __forceinline__ int page4_of(const Paged4& c, int slot, int pos) {
-    const int lp = pos / kPageTokens;
-    return c.page_table[(size_t)slot * c.table_stride + (c.ring_pages > 0 ? lp % c.ring_pages : lp)];
-}
 
 // ---- rows into pages ---------------------------------------------------------------------------------------------------
 // Four lanes hold 64 numbers of a row, 16 each.  Many rows are bound by reading them and writing what is held, and near that by the
@@ -166,43 +150,6 @@ store4_few_kernel(const T* rows, long long stride, T* held, long long held_strid
     if (l == 0) *(uint32_t*)(tile + tile4_codes(dim) + (row * groups + g) * 4) = sm;
 }
 
-// Block `left` of the step's rows, cut into blocks of up to `size` rows of one sequence (begun anew where a position is a multiple of
-// size if `align` is size - 1, else, 0, at a sequence's first row), in order; after them come the padding rows, `size` at a time (seq
-// -1).  Every lane of a warp looks at a sequence, their numbers of blocks are added up.  count <= 0: there is no such block.
-struct RowBlock { int seq, row0, pos0, count; };
-__device__ __forceinline__ RowBlock find_rows(const int* __restrict__ cu_seqlens, int row_base, int n_seqs, const int* __restrict__ token_pos, int n_tokens,
-                                              int left, int size, int align) {
-    const int lane = threadIdx.x & 31;
-    for (int s0 = 0; s0 < n_seqs; s0 += 32) {
-        const int s = s0 + lane;
-        int first = 0, n = 0, pos = 0, nb = 0;
-        if (s < n_seqs) {
-            first = cu_seqlens[s] - row_base;
-            n = cu_seqlens[s + 1] - row_base - first;
-            pos = n > 0 ? token_pos[first] : 0;
-            nb = n > 0 ? ((pos & align) + n + size - 1) / size : 0;
-        }
-        int upto = nb;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += v;
-        }
-        const uint32_t found = __ballot_sync(0xffffffffu, left < upto);
-        if (found != 0) {
-            const int who = __ffs(found) - 1, in = left - (__shfl_sync(0xffffffffu, upto, who) - __shfl_sync(0xffffffffu, nb, who));
-            first = __shfl_sync(0xffffffffu, first, who);
-            n = __shfl_sync(0xffffffffu, n, who);
-            pos = __shfl_sync(0xffffffffu, pos, who);
-            const int skip = in == 0 ? 0 : size * in - (pos & align);  // rows of the sequence before the block
-            return RowBlock{s0 + who, first + skip, pos + skip, min(size - ((pos + skip) & align), n - skip)};
-        }
-        left -= __shfl_sync(0xffffffffu, upto, 31);
-    }
-    const int row0 = cu_seqlens[n_seqs] - row_base + size * left;
-    return RowBlock{-1, row0, 0, min(size, n_tokens - row0)};
-}
-
 // Many rows: a warp takes 64 numbers of the up to 16 rows whose positions make a block of the pages, forms the block's 512 bytes in shared
 // memory and writes them at once (with positions missing, or written over by the same step, what is there only).  Blocks are the
 // sequences' in order, and after them the padding rows, 16 at a time, which store nothing but are handed back.
@@ -266,13 +213,6 @@ store4_many_kernel(const T* rows, long long stride, T* held, long long held_stri
     }
 }
 
-// d += a . b, free to be woven into its neighbours.
-__device__ __forceinline__ void mma_plain(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
 // ---- attention of single rows --------------------------------------------------------------------------------------
 // Bound by reading the held keys and values once, and close behind by the instructions that make operands of codes.
 //
@@ -289,7 +229,7 @@ __device__ __forceinline__ void mma_plain(float (&d)[4], const uint32_t (&a)[4],
 // cp.async fills, so that no barrier stands in the walk.  Running maxima are a warp's own and are raised when a score passes them by
 // 2^8.  The warps merge through shared memory; up to 8 shares are a cluster and merge through its shared memory, more through a
 // workspace and attend4_merge_kernel.
-constexpr int kAttendWarps = 8, kMaxSharePages = 256, kMaxShares = 1024, kClusterShares = 8;
+constexpr int kAttendWarps = 8, kMaxSharePages = 256, kClusterShares = 8;
 
 template <int DIM> struct Attend4 {
     static constexpr int kGroups = DIM / 64;
@@ -704,12 +644,6 @@ int launch_attend4(const void* q, long long q_stride, void* out, long long out_s
 
 using namespace hos;
 
-#define HOS_CHECK_PAGED4(what)                                                                                            \
-    const Paged4 c = *(const Paged4*)cache;                                                                                \
-    const int head_dim = c.head_dim, n_kv_heads = c.n_kv_heads;                                                            \
-    if (head_dim % 64 || head_dim < 64 || head_dim > 256) HOS_REFUSE(what ": head size %d (64, 128, 192 or 256)", head_dim);     \
-    if (n_kv_heads <= 0) HOS_REFUSE(what ": %d kv heads", n_kv_heads)
-
 // Rows and `held` (or null) have their numbers side by side; sequences' rows are cu_seqlens[s] - row_base .. in order (their entries of
 // seq_slot and seq_len_after begin at seq_base), then padding rows.  single: the sequences bring a row each.
 extern "C" int hos_store4(const void* rows, int dtype, long long stride, void* held, long long held_stride, const int* token_pos, const int* token_seq,
@@ -758,4 +692,18 @@ extern "C" int hos_attend4(const void* q, int dtype, long long q_stride, void* o
 #define HOS_A4_D(T) do { if (head_dim == 64) HOS_A4(T, 64); else if (head_dim == 128) HOS_A4(T, 128); else if (head_dim == 192) HOS_A4(T, 192); else HOS_A4(T, 256); } while (0)
     if (dtype == kF32) HOS_A4_D(float);
     else HOS_A4_D(bf16);
+}
+
+// The shares' sums in `parts` (hos_attend4, hos_attend4_tiles) added up into out.
+extern "C" int hos_attend4_merge(void* out, int dtype, long long out_stride, int head_dim, int n_tokens, int n_heads, int splits, float* parts, cudaStream_t stream) {
+    if (n_tokens <= 0) return 0;
+    if (parts == nullptr || splits < 1 || splits > kMaxShares || n_heads <= 0 || (long long)n_tokens * n_heads > 0x7fffffffll)
+        HOS_REFUSE("attend4_merge: %d rows of %d heads in %d shares", n_tokens, n_heads, splits);
+    const float2* part_ml = (const float2*)parts;
+    const float* part_o = parts + 2 * (size_t)n_tokens * n_heads * splits;
+#define HOS_AM(T, D) launch_pdl(attend4_merge_kernel<T, D>, dim3((unsigned)((long long)n_tokens * n_heads)), dim3(D), 0, stream, (T*)out, out_stride, n_heads, splits, part_o, part_ml)
+#define HOS_AM_D(T) do { if (head_dim == 64) HOS_AM(T, 64); else if (head_dim == 128) HOS_AM(T, 128); else if (head_dim == 192) HOS_AM(T, 192); else if (head_dim == 256) HOS_AM(T, 256); else HOS_REFUSE("attend4_merge: head size %d", head_dim); } while (0)
+    if (dtype == kF32) HOS_AM_D(float);
+    else HOS_AM_D(bf16);
+    return check_launch("attend4_merge");
 }

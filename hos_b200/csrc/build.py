@@ -60,7 +60,7 @@ _STATIC_LIBS: Dict[str, Tuple[List[str], List[str]]] = {
     "blocks": (["latent_attention.cu", "latent_prompt.cu", "wkv.cu"], []),
     "gated_attn": (["gated_attention.cu", "gated_attention_mma.cu"], []),
     "mixers": (["postnorm.cu", "state_scan.cu", "hyper.cu"], []),
-    "fourbit": (["weights4.cu", "weights4_tc.cu", "attention4.cu", "pages.cu"], []),
+    "fourbit": (["weights4.cu", "weights4_tc.cu", "attention4.cu", "attention4_tiles.cu", "pages.cu"], []),
 }
 
 _loaded: Dict[str, ctypes.CDLL] = {}

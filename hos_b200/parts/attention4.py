@@ -88,6 +88,8 @@ def attend(q: torch.Tensor, out: torch.Tensor, step, cache: ops.PagedKVArgs, n_h
     _check_step(n, step, "attend")
     kv = cache.n_kv_heads
     items = kv * -(-(n_heads // kv) // 8)
+    if _tiles_take(q, out, step, n_heads // kv):
+        return _attend_tiles(q, out, step, cache, n_heads, scale, softcap, window)
     together = 1 if step.single_token else max(1, 8 // (n_heads // kv))      # rows of a sequence that share a walk
     key = ("shares of 4-bit pages", n, items, together, window, step.row_offset)
     plan = step.shared.get(key)                      # once per step and kind of layer
@@ -102,3 +104,45 @@ def attend(q: torch.Tensor, out: torch.Tensor, step, cache: ops.PagedKVArgs, n_h
                        step.token_seq.data_ptr(), step.seq_slot.data_ptr(), step.token_slot.data_ptr() if step.token_slot is not None else None,
                        step.cu_seqlens.data_ptr() if together > 1 else None, step.row_offset, step.n_seqs, ops.paged4(cache), n, n_heads,
                        scale, softcap, window or 0, share, splits, parts.data_ptr() if parts is not None else None, ops._stream())
+
+
+TILE_ROWS = 128                # (row, head) pairs of a kv head that a block of the kernel for pieces takes
+TILE_MIN_PAIRS = 48
+
+
+def _tiles_take(q, out, step, per: int) -> bool:
+    """Whether the rows go to the kernel for pieces: bfloat16 rows on 16 bytes, and sequences that bring enough (row, head) pairs."""
+    return (not step.single_token and q.dtype == torch.bfloat16 and step.max_new * per >= TILE_MIN_PAIRS and per <= TILE_ROWS and q.stride(0) % 8 == 0
+            and out.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0)
+
+
+def _attend_tiles(q, out, step, cache: ops.PagedKVArgs, n_heads: int, scale: float, softcap: float, window: Optional[int]) -> None:
+    n, kv = q.shape[0], cache.n_kv_heads
+    size = TILE_ROWS // (n_heads // kv)
+    key = ("tiles over 4-bit pages", n, size, kv, window, step.row_offset)
+    plan = step.shared.get(key)                      # once per step and kind of layer
+    if plan is None:
+        plan = step.shared[key] = tile_shares(-(-n // size) if not step.cu_host else
+                                              sum(-(-(b - a) // size) for a, b in zip(step.cu_host, step.cu_host[1:])), kv,
+                                              step.max_len_after, step.max_new, window)
+    share, splits = plan
+    parts = None
+    if splits > 1:
+        parts = torch.empty(n * n_heads * splits * (cache.head_dim + 2), dtype=torch.float32, device=q.device)
+    lib = ops.fourbit()
+    lib.call("hos_attend4_tiles", q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), step.token_pos.data_ptr(), step.seq_slot.data_ptr(),
+             step.seq_offset, step.cu_seqlens.data_ptr(), step.row_offset, step.n_seqs, ops.paged4(cache), n, n_heads, scale, softcap, window or 0, share,
+             splits, parts.data_ptr() if parts is not None else None, ops._stream())
+    if splits > 1:
+        lib.call("hos_attend4_merge", out.data_ptr(), ops.dtype_code(out.dtype), out.stride(0), cache.head_dim, n, n_heads, splits, parts.data_ptr(),
+                 ops._stream())
+
+
+def tile_shares(blocks: int, kv: int, longest: int, new: int, window: Optional[int]):
+    """(pages of a share, shares) for `blocks` blocks of rows and kv heads of which an SM takes one at a time: as many shares as fill
+    the SMs, each of at least 8 pages (a share costs about 2 besides, and its sums are written, read and merged)."""
+    span = min(longest, window + new) if window else longest
+    pages = max(1, -(-span // ops.PAGE_TOKENS) + (1 if window else 0))
+    splits = max(1, min(pages // 8, ops.sm_count() // max(1, blocks * kv)))
+    share = -(-pages // splits)
+    return share, -(-pages // share)
