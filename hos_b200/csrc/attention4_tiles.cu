@@ -135,16 +135,22 @@ attend4_tiles_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __res
         mid[i][0] = mid[i][1] = 0.f;
     }
     const float scale2 = scale * 1.44269504f, cap2 = cap * 1.44269504f, in_cap = cap > 0.f ? 2.f * scale2 / cap : 0.f;
-    const uint32_t q_at = smem_u32(smem + A::kQ) + (warp * 16 + (lane & 15)) * A::kRowBytes, q_half = lane >> 4, q_swap = lane & 7;
-    const int frag_row = lane & 7, frag_chunk = lane >> 3;     // of an ldmatrix of four: row, and which 16 bytes
+    // where a lane's row of an ldmatrix of four begins in a group's 128 bytes, swapped as the rows are
+    uint32_t q_at[4], k_at[2];
+#pragma unroll
+    for (int st = 0; st < 4; ++st)
+        q_at[st] = smem_u32(smem + A::kQ) + (warp * 16 + (lane & 15)) * A::kRowBytes + (((2 * st + (lane >> 4)) ^ (lane & 7)) << 4);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) k_at[h] = ((4 * h + (lane >> 3)) ^ (lane & 7)) << 4;
+    const uint32_t k_rows = smem_u32(smem + A::kK) + (lane & 7) * A::kRowBytes, v_rows = smem_u32(smem + A::kV) + (lane & 7) * 128;
 
     for (int p = p0; p < p1; ++p) {
         const int buffer = (p - p0) & 1;
         if (p + 1 < p1) ask(p + 1);
         // what lies wholly behind a warp's rows, or before their windows, is not walked over
         if (busy && p * kPageTokens <= warp_last && !(window > 0 && p * kPageTokens + 63 <= warp_first - window)) {
-            const uint32_t k_at = smem_u32(smem + A::kK) + buffer * 64 * A::kRowBytes + frag_row * A::kRowBytes;
-            const uint32_t v_at = smem_u32(smem + A::kV) + buffer * 64 * A::kRowBytes + frag_row * 128;
+            const uint32_t page_at = buffer * 64 * A::kRowBytes, k0 = k_rows + page_at + k_at[0], k1 = k_rows + page_at + k_at[1];
+            const uint32_t v0 = v_rows + page_at + k_at[0], v1 = v_rows + page_at + k_at[1];
             const uint32_t* km = (const uint32_t*)(smem + A::kMeta) + buffer * 2 * G * 64;
             const uint32_t* vm = km + G * 64;
             float s[8][4];
@@ -155,20 +161,30 @@ attend4_tiles_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __res
                 uint32_t a[4][4];
                 const float q_sum[2] = {((const float*)(smem + A::kQSum))[row_a * G + grp], ((const float*)(smem + A::kQSum))[row_b * G + grp]};
 #pragma unroll
-                for (int st = 0; st < 4; ++st) ldmatrix_x4(a[st], q_at + (((8 * grp + 2 * st + q_half) ^ q_swap) << 4));
+                for (int st = 0; st < 4; ++st) ldmatrix_x4(a[st], q_at[st] + grp * 128);
 #pragma unroll
-                for (int n = 0; n < 8; ++n) {
-                    uint32_t b[2][4];
+                for (int n0 = 0; n0 < 8; n0 += 4) {            // four products side by side: one alone would wait for its own sums
+                    float part[4][4];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) ldmatrix_x4(b[h], k_at + n * 8 * A::kRowBytes + (((8 * grp + 4 * h + frag_chunk) ^ frag_row) << 4));
-                    float part[4] = {0.f, 0.f, 0.f, 0.f};
+                    for (int i = 0; i < 4; ++i) part[i][0] = part[i][1] = part[i][2] = part[i][3] = 0.f;
 #pragma unroll
-                    for (int st = 0; st < 4; ++st) mma_bf16(part, a[st], b[st >> 1][2 * (st & 1)], b[st >> 1][2 * (st & 1) + 1]);
-                    const uint2 sm = *(const uint2*)&km[grp * 64 + n * 8 + 2 * t4];
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t b[4][4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint32_t w = (e & 1) ? sm.y : sm.x;
-                        s[n][e] = fmaf(bf16_lo(w), part[e], fmaf(bf16_hi(w), q_sum[e >> 1], s[n][e]));
+                        for (int i = 0; i < 4; ++i) ldmatrix_x4(b[i], (h ? k1 : k0) + (n0 + i) * 8 * A::kRowBytes + grp * 128);
+#pragma unroll
+                        for (int st = 0; st < 2; ++st)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) mma_bf16(part[i], a[2 * h + st], b[i][2 * st], b[i][2 * st + 1]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint2 sm = *(const uint2*)&km[grp * 64 + (n0 + i) * 8 + 2 * t4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t w = (e & 1) ? sm.y : sm.x;
+                            s[n0 + i][e] = fmaf(bf16_lo(w), part[i][e], fmaf(bf16_hi(w), q_sum[e >> 1], s[n0 + i][e]));
+                        }
                     }
                 }
             }
@@ -177,22 +193,33 @@ attend4_tiles_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __res
             const bool edge = base + 63 > rows.pos0 || (window > 0 && base <= last - window);
             uint32_t hidden = 0u;
             float top[2] = {-INFINITY, -INFINITY};
+            if (cap > 0.f) {
 #pragma unroll
-            for (int n = 0; n < 8; ++n)
+                for (int n = 0; n < 8; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float v = s[n][e];
-                    v = cap > 0.f ? cap2 * (1.f - 2.f * rcp_approx(1.f + ex2_approx(v * in_cap))) : v * scale2;
-                    if (edge) {
+                    for (int e = 0; e < 4; ++e) s[n][e] = fmaf(-2.f * cap2, rcp_approx(1.f + ex2_approx(s[n][e] * in_cap)), cap2);
+            } else {
+#pragma unroll
+                for (int n = 0; n < 8; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[n][e] *= scale2;
+            }
+            if (edge) {
+#pragma unroll
+                for (int n = 0; n < 8; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
                         const int key = base + n * 8 + 2 * t4 + (e & 1), mine = pos[e >> 1];
                         if (key > mine || (window > 0 && key <= mine - window)) {
-                            v = -INFINITY;
+                            s[n][e] = -INFINITY;
                             hidden |= 1u << (n * 4 + e);
                         }
                     }
-                    s[n][e] = v;
-                    top[e >> 1] = fmaxf(top[e >> 1], v);
-                }
+            }
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
             if (__any_sync(0xffffffffu, top[0] > best[0] + 8.f || top[1] > best[1] + 8.f)) {
                 float f[2];
 #pragma unroll
@@ -211,42 +238,55 @@ attend4_tiles_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __res
                     o[i][0] *= f[0]; o[i][1] *= f[0]; o[i][2] *= f[1]; o[i][3] *= f[1];
                 }
             }
+            const float from[2] = {best[0] == -INFINITY ? 0.f : best[0], best[1] == -INFINITY ? 0.f : best[1]};      // no key seen yet: all weights 0
 #pragma unroll
             for (int n = 0; n < 8; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    s[n][e] = (hidden >> (n * 4 + e)) & 1u ? 0.f : ex2_approx(s[n][e] - best[e >> 1]);
+                    s[n][e] = ex2_approx(s[n][e] - from[e >> 1]);
                     sum[e >> 1] += s[n][e];
                 }
 #pragma unroll
             for (int grp = 0; grp < G; ++grp) {
                 uint32_t a[4][4];
+                if (!edge) {
 #pragma unroll
-                for (int n = 0; n < 8; ++n) {
-                    const uint2 sm = *(const uint2*)&vm[grp * 64 + n * 8 + 2 * t4];
-                    float w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint32_t m = (e & 1) ? sm.y : sm.x;
-                        w[e] = s[n][e] * bf16_lo(m);
-                        float with = fmaf(s[n][e], bf16_hi(m), mid[grp][e >> 1]);
-                        if (edge && ((hidden >> (n * 4 + e)) & 1u)) {
-                            w[e] = 0.f;
-                            with = mid[grp][e >> 1];
-                        }
-                        mid[grp][e >> 1] = with;
+                    for (int n = 0; n < 8; ++n) {
+                        const uint2 sm = *(const uint2*)&vm[grp * 64 + n * 8 + 2 * t4];
+                        const float sv[2] = {bf16_lo(sm.x), bf16_lo(sm.y)}, mv[2] = {bf16_hi(sm.x), bf16_hi(sm.y)};
+                        a[n >> 1][2 * (n & 1)] = pack_bf16(s[n][0] * sv[0], s[n][1] * sv[1]);
+                        a[n >> 1][2 * (n & 1) + 1] = pack_bf16(s[n][2] * sv[0], s[n][3] * sv[1]);
+                        mid[grp][0] = fmaf(s[n][1], mv[1], fmaf(s[n][0], mv[0], mid[grp][0]));
+                        mid[grp][1] = fmaf(s[n][3], mv[1], fmaf(s[n][2], mv[0], mid[grp][1]));
                     }
-                    a[n >> 1][2 * (n & 1)] = pack_bf16(w[0], w[1]);
-                    a[n >> 1][2 * (n & 1) + 1] = pack_bf16(w[2], w[3]);
+                } else {
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) {
+                        const uint2 sm = *(const uint2*)&vm[grp * 64 + n * 8 + 2 * t4];
+                        float w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t m = (e & 1) ? sm.y : sm.x;
+                            const bool seen = !((hidden >> (n * 4 + e)) & 1u);
+                            w[e] = seen ? s[n][e] * bf16_lo(m) : 0.f;
+                            if (seen) mid[grp][e >> 1] = fmaf(s[n][e], bf16_hi(m), mid[grp][e >> 1]);
+                        }
+                        a[n >> 1][2 * (n & 1)] = pack_bf16(w[0], w[1]);
+                        a[n >> 1][2 * (n & 1) + 1] = pack_bf16(w[2], w[3]);
+                    }
                 }
 #pragma unroll
-                for (int d = 0; d < 8; ++d) {
-                    uint32_t b[2][4];
+                for (int d0 = 0; d0 < 8; d0 += 4)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) ldmatrix_x4(b[h], v_at + (grp * 64 + d * 8) * 128 + (((4 * h + frag_chunk) ^ frag_row) << 4));
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t b[4][4];
 #pragma unroll
-                    for (int st = 0; st < 4; ++st) mma_bf16(o[grp * 8 + d], a[st], b[st >> 1][2 * (st & 1)], b[st >> 1][2 * (st & 1) + 1]);
-                }
+                        for (int i = 0; i < 4; ++i) ldmatrix_x4(b[i], (h ? v1 : v0) + (grp * 64 + (d0 + i) * 8) * 128);
+#pragma unroll
+                        for (int st = 0; st < 2; ++st)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) mma_bf16(o[grp * 8 + d0 + i], a[2 * h + st], b[i][2 * st], b[i][2 * st + 1]);
+                    }
             }
         }
         if (p + 1 < p1) {
