@@ -220,9 +220,10 @@ store4_many_kernel(const T* rows, long long stride, T* held, long long held_stri
 // neighbouring rows of a sequence, each with its own mask).  The score of a key is
 // sum_g (s_g (sum_{d in g} q c') - 136 s_g sum q + m_g sum q) over its groups of 64, c' = 128 + c + 8 the operand as codes_to_bf16 makes
 // it without subtracting: a group's product starts at -136 sum q and is multiplied by the key's scale, in 32 bits; neither scale nor
-// middle is rounded into an operand.  Values: O^T = V^T P^T with 16 numbers of a head as rows, P times the value's scale rounded to
-// bfloat16 (the one rounding, 2^-9 of a weight, beside the 2^-9 of the result), the codes exact, and the middles' sum, one number a
-// group and head, in 32 bits beside it.  The scores' registers, transposed eight by eight, are P's operand.
+// middle is rounded into an operand.  Values: O^T = V^T P^T with 16 numbers of a head as rows, P times the value's scale as two bfloat16
+// numbers (2^-17 of a weight; with one, 2^-9, long rows whose output is a small mean lost as much as the result's own rounding), the
+// codes exact, and the middles' sum, one number a group and head, in 32 bits beside it.  The scores' registers, transposed eight by
+// eight, are P's operand.
 // Rows in 32 bits: q, and p times the scale, are three bfloat16 numbers each, exactly, and the codes are subtracted first.
 //
 // A CTA takes a share of the pages of one (row or neighbouring rows, kv head, 8 heads); its warps take 16 keys in turn, each through a ring of its own that
@@ -275,7 +276,7 @@ attend4_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out,
                const int* __restrict__ token_seq, const int* __restrict__ seq_slot, const int* __restrict__ token_slot, const int* __restrict__ cu_seqlens, int row_base,
                int n_seqs, int n_tokens, Paged4 c, int n_heads, float scale, float cap, int window, int share, int splits, float* __restrict__ part_o, float2* __restrict__ part_ml) {
     using A = Attend4<DIM>;
-    constexpr int G = A::kGroups, kTerms = sizeof(T) == 4 ? 3 : 1, kTiles = DIM / 16;
+    constexpr int G = A::kGroups, kTerms = sizeof(T) == 4 ? 3 : 1, kWeightTerms = kTerms == 3 ? 3 : 2, kTiles = DIM / 16;
     constexpr bool kExact = kTerms == 3;
     extern __shared__ __align__(16) uint8_t ring_bytes[];
     __shared__ __align__(16) uint4 q_frag[kTerms][G][2][32];
@@ -478,9 +479,9 @@ attend4_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out,
                 w[e] = hidden[e] ? 0.f : p[e] * bf16_lo(sm);
                 mid[i][e & 1] = hidden[e] ? mid[i][e & 1] : fmaf(p[e], bf16_hi(sm), mid[i][e & 1]);
             }
-            uint32_t pb[kTerms][2];
+            uint32_t pb[kWeightTerms][2];
 #pragma unroll
-            for (int term = 0; term < kTerms; ++term) {
+            for (int term = 0; term < kWeightTerms; ++term) {
                 const uint32_t a = pack_bf16(w[0], w[1]), b8 = pack_bf16(w[2], w[3]);
                 pb[term][0] = transposed_8x8(a);
                 pb[term][1] = transposed_8x8(b8);
@@ -493,7 +494,7 @@ attend4_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out,
                 uint32_t a[4];
                 codes_to_bf16<true>(words[mt], kZero8, a);
 #pragma unroll
-                for (int term = kTerms - 1; term >= 0; --term) mma_plain(o[4 * i + mt], a, pb[term][0], pb[term][1]);
+                for (int term = kWeightTerms - 1; term >= 0; --term) mma_plain(o[4 * i + mt], a, pb[term][0], pb[term][1]);
             }
         }
         before = slot;

@@ -2,8 +2,8 @@
 //
 // 128 (row, head) pairs of a kv head to a CTA, 16 to a warp; a page's keys and values are formed once for all of them, as bare codes -8..7,
 // exact in bfloat16, in shared memory.  Scales and middles stay out of the operands, as in attention4.cu: a group's part of a score is
-// s (q . c) + m sum q in 32 bits; a weight times its value's scale is rounded to bfloat16, for each group of 64 numbers anew, and
-// the middles' sum goes beside.  Bound by mma.sync (526 TFLOP/s at most): the next page is asked for while one is multiplied and
+// s (q . c) + m sum q in 32 bits; a weight times its value's scale is two bfloat16 numbers, for each group of 64 numbers anew, and the
+// middles' sum goes beside.  Bound by mma.sync (526 TFLOP/s at most): the next page is asked for while one is multiplied and
 // formed behind it.  Shares of the pages, if rows are few, merge in attention4.cu.
 // Measured (B200): a turn of 739 tokens on 7,453, 8 heads over 4 of 256: the kernel of few rows 412 us.
 #include "attention4.cuh"
@@ -248,45 +248,55 @@ attend4_tiles_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __res
                 }
 #pragma unroll
             for (int grp = 0; grp < G; ++grp) {
-                uint32_t a[4][4];
-                if (!edge) {
+                // the weights times the scales as two bfloat16 numbers: the first, its products, then the rest of them
 #pragma unroll
-                    for (int n = 0; n < 8; ++n) {
-                        const uint2 sm = *(const uint2*)&vm[grp * 64 + n * 8 + 2 * t4];
-                        const float sv[2] = {bf16_lo(sm.x), bf16_lo(sm.y)}, mv[2] = {bf16_hi(sm.x), bf16_hi(sm.y)};
-                        a[n >> 1][2 * (n & 1)] = pack_bf16(s[n][0] * sv[0], s[n][1] * sv[1]);
-                        a[n >> 1][2 * (n & 1) + 1] = pack_bf16(s[n][2] * sv[0], s[n][3] * sv[1]);
-                        mid[grp][0] = fmaf(s[n][1], mv[1], fmaf(s[n][0], mv[0], mid[grp][0]));
-                        mid[grp][1] = fmaf(s[n][3], mv[1], fmaf(s[n][2], mv[0], mid[grp][1]));
-                    }
-                } else {
+                for (int term = 0; term < 2; ++term) {
+                    uint32_t a[4][4];
+                    auto operand = [&](int n, const float (&w)[4]) {
+                        const uint32_t first = pack_bf16(w[0], w[1]), second = pack_bf16(w[2], w[3]);
+                        a[n >> 1][2 * (n & 1)] = term == 0 ? first : pack_bf16(w[0] - bf16_lo(first), w[1] - bf16_hi(first));
+                        a[n >> 1][2 * (n & 1) + 1] = term == 0 ? second : pack_bf16(w[2] - bf16_lo(second), w[3] - bf16_hi(second));
+                    };
+                    if (!edge) {
 #pragma unroll
-                    for (int n = 0; n < 8; ++n) {
-                        const uint2 sm = *(const uint2*)&vm[grp * 64 + n * 8 + 2 * t4];
-                        float w[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint32_t m = (e & 1) ? sm.y : sm.x;
-                            const bool seen = !((hidden >> (n * 4 + e)) & 1u);
-                            w[e] = seen ? s[n][e] * bf16_lo(m) : 0.f;
-                            if (seen) mid[grp][e >> 1] = fmaf(s[n][e], bf16_hi(m), mid[grp][e >> 1]);
+                        for (int n = 0; n < 8; ++n) {
+                            const uint2 sm = *(const uint2*)&vm[grp * 64 + n * 8 + 2 * t4];
+                            const float sv[2] = {bf16_lo(sm.x), bf16_lo(sm.y)}, mv[2] = {bf16_hi(sm.x), bf16_hi(sm.y)};
+                            const float w[4] = {s[n][0] * sv[0], s[n][1] * sv[1], s[n][2] * sv[0], s[n][3] * sv[1]};
+                            operand(n, w);
+                            if (term == 0) {
+                                mid[grp][0] = fmaf(s[n][1], mv[1], fmaf(s[n][0], mv[0], mid[grp][0]));
+                                mid[grp][1] = fmaf(s[n][3], mv[1], fmaf(s[n][2], mv[0], mid[grp][1]));
+                            }
                         }
-                        a[n >> 1][2 * (n & 1)] = pack_bf16(w[0], w[1]);
-                        a[n >> 1][2 * (n & 1) + 1] = pack_bf16(w[2], w[3]);
+                    } else {
+#pragma unroll
+                        for (int n = 0; n < 8; ++n) {
+                            const uint2 sm = *(const uint2*)&vm[grp * 64 + n * 8 + 2 * t4];
+                            float w[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const uint32_t m = (e & 1) ? sm.y : sm.x;
+                                const bool seen = !((hidden >> (n * 4 + e)) & 1u);
+                                w[e] = seen ? s[n][e] * bf16_lo(m) : 0.f;
+                                if (seen && term == 0) mid[grp][e >> 1] = fmaf(s[n][e], bf16_hi(m), mid[grp][e >> 1]);
+                            }
+                            operand(n, w);
+                        }
                     }
+#pragma unroll
+                    for (int d0 = 0; d0 < 8; d0 += 4)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            uint32_t b[4][4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) ldmatrix_x4(b[i], (h ? v1 : v0) + (grp * 64 + (d0 + i) * 8) * 128);
+#pragma unroll
+                            for (int st = 0; st < 2; ++st)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) mma_bf16(o[grp * 8 + d0 + i], a[2 * h + st], b[i][2 * st], b[i][2 * st + 1]);
+                        }
                 }
-#pragma unroll
-                for (int d0 = 0; d0 < 8; d0 += 4)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        uint32_t b[4][4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) ldmatrix_x4(b[i], (h ? v1 : v0) + (grp * 64 + (d0 + i) * 8) * 128);
-#pragma unroll
-                        for (int st = 0; st < 2; ++st)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) mma_bf16(o[grp * 8 + d0 + i], a[2 * h + st], b[i][2 * st], b[i][2 * st + 1]);
-                    }
             }
         }
         if (p + 1 < p1) {

@@ -1,8 +1,10 @@
 // Products of many rows with weights in 4 bits on the 5th-generation tensor cores: out[M, N] = x[M, K] . W[N, K]^T in bfloat16.
 //
-// The weights are formed in bfloat16 on their way: (c - z) s, c - z exact and the product rounded once (2^-9 of a weight, as a matrix
-// kept in bfloat16 would be), straight into the operand's place in shared memory, so that they cross memory in 4 bits however many
-// rows there are.  A CTA takes 128 features (gated: 128 of gate and the same 128 of up) and up to 256 rows, tcgen05.mma with M = 128
+// The weights are formed in half precision on their way: (c - z) s, c - z exact and the product, of 12 bits, rounded once (2^-12 of a
+// weight; in bfloat16 it would be 2^-9, as much as the result's own rounding), straight into the operand's place in shared memory, so
+// that they cross memory in 4 bits however many rows there are.  Half precision has few exponents: a feature's scales are held times a
+// power of two that brings the largest between 1 and 2 (parts/weights4.py), a row of x is brought to 2^10 at most by one of its own
+// (rows_to_half_kernel; numbers below 2^-34 of the row's largest are lost), and the powers come back in the epilogue, exactly.  A CTA takes 128 features (gated: 128 of gate and the same 128 of up) and up to 256 rows, tcgen05.mma with M = 128
 // features and N = rows.  Three groups of eight warps take the stages of 64 k in turn: each warp forms 16 features (its codes wait in
 // registers, asked for a turn ahead); one more warp brings the rows of x by TMA, and one issues the products.  (With the rows
 // brought by the makers' cp.async the fence behind what they form waited for those copies too: 2304 x 9216, 64 rows on one SM a tile 64 us.)
@@ -13,6 +15,7 @@
 #include "fourbit.cuh"
 #include "mma_utils.cuh"
 #include "tcgen05_one.cuh"
+#include <cuda_fp16.h>
 
 namespace hos {
 
@@ -33,7 +36,8 @@ __device__ __forceinline__ void product4_give_up() {
 }
 
 struct Product4Args {
-    const uint8_t *codes, *records;
+    const uint8_t *codes, *records;      // scales, and 1024 + zero codes, in half precision
+    const float *powers, *row_powers;    // of a feature (gate's, then up's), of a row
     void* out;
     long long ldo, wait_cycles;     // wait_cycles: the limit of every wait
     uint32_t group_magic;                // ceil(2^32 / blocks of 64 a group): the group of a block is a product's high half
@@ -107,6 +111,95 @@ __device__ __forceinline__ float gated_value(int act, float gate, float up, floa
 }
 
 // S: stages of operands; SUB: scales a block of 64 (2: groups of 32).
+// A row of x in half precision, its numbers times a power of two, padded to `width` with zeros; a block a row.
+__global__ void __launch_bounds__(256) rows_to_half_kernel(const bf16* __restrict__ x, long long ldx, int K, int width, __half* __restrict__ y,
+                                                           float* __restrict__ row_powers, int whole) {
+    __shared__ float scratch[32];
+    pdl_enter();
+    const bf16* row = x + (size_t)blockIdx.x * ldx;
+    __half* to = y + (size_t)blockIdx.x * width;
+    constexpr int kHeld = 4;                                 // pieces of eight numbers that a thread holds between the two walks
+    uint4 held[kHeld];
+    float most = 0.f;
+    auto load = [&](int i) {
+        if (whole) return __ldg(reinterpret_cast<const uint4*>(row) + i);
+        uint32_t w[4];
+        const unsigned short* u = reinterpret_cast<const unsigned short*>(row);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            w[j] = (8 * i + 2 * j < K ? (uint32_t)u[8 * i + 2 * j] : 0u) | (8 * i + 2 * j + 1 < K ? (uint32_t)u[8 * i + 2 * j + 1] << 16 : 0u);
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    };
+    auto look = [&](const uint4& v) {                        // infinities and NaN keep out of it
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float a = fabsf(bf16_lo(w[j])), b = fabsf(bf16_hi(w[j]));
+            if (a < INFINITY) most = fmaxf(most, a);
+            if (b < INFINITY) most = fmaxf(most, b);
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+        const int i = threadIdx.x + 256 * j;
+        held[j] = 8 * i < width ? load(i) : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) look(held[j]);
+    for (int i = threadIdx.x + 256 * kHeld; 8 * i < width; i += 256) look(load(i));
+    most = block_max(most, scratch);
+    // 2^e <= most < 2^(e+1): times 2^(10 - e), in two factors of which each is a normal number
+    const int e = most > 0.f ? max(-126, min(127, (int)((__float_as_uint(most) >> 23) & 255u) - 127)) : 10;
+    const float a = __uint_as_float((uint32_t)(127 + (10 - e) / 2) << 23), b = __uint_as_float((uint32_t)(127 + (10 - e) - (10 - e) / 2) << 23);
+    if (threadIdx.x == 0) row_powers[blockIdx.x] = (1.f / a) * (1.f / b);
+    auto put = [&](int i, const uint4& v) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        uint32_t h[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const __half2 t = __floats2half2_rn(bf16_lo(w[j]) * a * b, bf16_hi(w[j]) * a * b);
+            h[j] = *reinterpret_cast<const uint32_t*>(&t);
+        }
+        *reinterpret_cast<uint4*>(to + 8 * i) = make_uint4(h[0], h[1], h[2], h[3]);
+    };
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+        const int i = threadIdx.x + 256 * j;
+        if (8 * i < width) put(i, held[j]);
+    }
+    for (int i = threadIdx.x + 256 * kHeld; 8 * i < width; i += 256) put(i, load(i));
+}
+
+// The operand's registers of a word of codes: 1024 + c where a code's bits are the lowest of a half, 1024 + 16 c where they are the next;
+// minus 1024 + z or 1024 + 16 z, exact, times s or s / 16.
+struct Scale16 { uint32_t s, s16, z, z16; };
+__device__ __forceinline__ uint32_t half_weight(uint32_t w, uint32_t mask, uint32_t z, uint32_t s) {
+    uint32_t v;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(w), "r"(mask), "r"(0x64006400u));
+    const __half2 c = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&z)), *reinterpret_cast<const __half2*>(&s));
+    return *reinterpret_cast<const uint32_t*>(&c);
+}
+__device__ __forceinline__ uint4 half_weights(uint32_t w, const Scale16& k) {
+    const uint32_t up = w >> 8;
+    return make_uint4(half_weight(w, 0x000f000fu, k.z, k.s), half_weight(w, 0x00f000f0u, k.z16, k.s16), half_weight(up, 0x000f000fu, k.z, k.s),
+                      half_weight(up, 0x00f000f0u, k.z16, k.s16));
+}
+template <bool ZEROS>
+__device__ __forceinline__ Scale16 scale_of(uint32_t two, uint32_t zeros, uint32_t pick) {
+    Scale16 k;
+    k.s = __byte_perm(two, 0, pick);
+    const __half2 s16 = __hmul2(*reinterpret_cast<const __half2*>(&k.s), __float2half2_rn(0.0625f));
+    k.s16 = *reinterpret_cast<const uint32_t*>(&s16);
+    k.z = 0x64086408u;                                       // 1024 + 8
+    k.z16 = 0x64806480u;                                     // 1024 + 128
+    if (ZEROS) {
+        k.z = __byte_perm(zeros, 0, pick);
+        const __half2 z16 = __hfma2(*reinterpret_cast<const __half2*>(&k.z), __float2half2_rn(16.f), __float2half2_rn(-15360.f));
+        k.z16 = *reinterpret_cast<const uint32_t*>(&z16);
+    }
+    return k;
+}
+
 template <int S, bool GATED, int SUB, bool ZEROS>
 __global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(const __grid_constant__ CUtensorMap rows_map, Product4Args p) {
     constexpr int kAcc = GATED ? 2 : 1, kRecord = ZEROS ? 64 : 32;
@@ -177,27 +270,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(const __grid
                 const bool upper = h != (g & 1);
                 const uint32_t lo = upper ? codes[a].y : codes[a].x, hi = upper ? codes[a].w : codes[a].z;
                 const uint32_t two = SUB == 2 && upper ? scale[a][SUB - 1] : scale[a][0];
-                uint32_t z0 = kZero8, z1 = kZero8;
-                if (ZEROS) {
-                    const uint32_t zz = SUB == 2 && upper ? zero[a][SUB - 1] : zero[a][0];
-                    z0 = __byte_perm(zz, 0, 0x1010);
-                    z1 = __byte_perm(zz, 0, 0x3232);
-                }
-                const uint32_t s0 = __byte_perm(two, 0, 0x1010), s1 = __byte_perm(two, 0, 0x3232);
-                const __nv_bfloat162 sc0 = *reinterpret_cast<const __nv_bfloat162*>(&s0), sc1 = *reinterpret_cast<const __nv_bfloat162*>(&s1);
-                uint32_t v0[4], v1[4];
-                codes_to_bf16<true>(lo, z0, v0);
-                codes_to_bf16<true>(hi, z1, v1);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const __nv_bfloat162 y0 = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&v0[j]), sc0);
-                    const __nv_bfloat162 y1 = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&v1[j]), sc1);
-                    v0[j] = *reinterpret_cast<const uint32_t*>(&y0);
-                    v1[j] = *reinterpret_cast<const uint32_t*>(&y1);
-                }
+                const uint32_t zz = !ZEROS ? 0u : (SUB == 2 && upper ? zero[a][SUB - 1] : zero[a][0]);
                 const int chunk = (((upper ? 4 : 0) + t4) ^ g) << 4;
-                *reinterpret_cast<uint4*>(to + chunk) = make_uint4(v0[0], v0[1], v0[2], v0[3]);
-                *reinterpret_cast<uint4*>(to + 1024 + chunk) = make_uint4(v1[0], v1[1], v1[2], v1[3]);
+                *reinterpret_cast<uint4*>(to + chunk) = half_weights(lo, scale_of<ZEROS>(two, zz, 0x1010));
+                *reinterpret_cast<uint4*>(to + 1024 + chunk) = half_weights(hi, scale_of<ZEROS>(two, zz, 0x3232));
             }
         };
 #pragma unroll
@@ -231,8 +307,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(const __grid
             }
         }
     } else {
-        // the warp walks together and one lane issues: what the products take is then in uniform registers
-        const uint32_t idesc = tc_idesc(kTcFeatures, p.tile_rows, 0), step = (uint32_t)stage >> 4;
+        // the warp walks together and one lane issues: what the products take is then in uniform registers; both operands in half precision
+        const uint32_t idesc = tc_idesc(kTcFeatures, p.tile_rows, 0) & ~((1u << 7) | (1u << 10)), step = (uint32_t)stage >> 4;
         const uint64_t weights0 = desc_kmajor(smem_u32(stages)), rows0 = desc_kmajor(smem_u32(stages) + kAcc * kTcWeights);
         uint32_t leader;
         asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(leader));
@@ -264,6 +340,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(const __grid
     float* sums = reinterpret_cast<float*>(stages);          // [kAcc][tile_rows][128] of a share, over operands that are done with
     if (warp < kTcMakers && ok) {
         const int quarter = warp & 3, feature = quarter * 32 + lane, n = f0 + feature;
+        const float power = n < p.N ? p.powers[n] : 0.f, up_power = GATED && n < p.N ? p.powers[p.N + n] : 0.f;
         const uint32_t from = tmem_base + ((uint32_t)(quarter * 32) << 16);
 #pragma unroll 1
         for (int c0 = (warp >> 2) * 16; c0 < p.tile_rows; c0 += kTcMakers * 4) {      // tile_rows is a multiple of 16
@@ -275,10 +352,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(const __grid
             for (int j = 0; j < 16; ++j) {
                 const int c = c0 + j, m = m0 + c;
                 if (p.shares > 1) {
-                    sums[c * 128 + feature] = __uint_as_float(v[j]);
-                    if (GATED) sums[(p.tile_rows + c) * 128 + feature] = __uint_as_float(u[j]);
+                    sums[c * 128 + feature] = __uint_as_float(v[j]) * power;
+                    if (GATED) sums[(p.tile_rows + c) * 128 + feature] = __uint_as_float(u[j]) * up_power;
                 } else if (m < p.M && n < p.N) {
-                    const float y = GATED ? gated_value(p.act, __uint_as_float(v[j]), __uint_as_float(u[j]), p.limit) : __uint_as_float(v[j]);
+                    const float back = p.row_powers[m], gate = __uint_as_float(v[j]) * power * back;
+                    const float y = GATED ? gated_value(p.act, gate, __uint_as_float(u[j]) * up_power * back, p.limit) : gate;
                     if (p.out_f32) ((float*)p.out)[(size_t)m * p.ldo + n] = y;
                     else ((bf16*)p.out)[(size_t)m * p.ldo + n] = __float2bfloat16_rn(y);
                 }
@@ -301,7 +379,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(const __grid
                 }
                 const int m = m0 + c;
                 if (m < p.M && n < p.N) {
-                    const float y = GATED ? gated_value(p.act, v, u, p.limit) : v;
+                    const float back = p.row_powers[m], y = GATED ? gated_value(p.act, v * back, u * back, p.limit) : v * back;
                     if (p.out_f32) ((float*)p.out)[(size_t)m * p.ldo + n] = y;
                     else ((bf16*)p.out)[(size_t)m * p.ldo + n] = __float2bfloat16_rn(y);
                 }
@@ -392,16 +470,18 @@ extern "C" int hos_product4_tc_set_error_word(void* word) {
     return cudaMemcpyToSymbol(g_product4_error_host, &word, sizeof(word)) == cudaSuccess ? 0 : -1;
 }
 
-// As hos_product4 for bfloat16 rows that begin on 16 bytes, K and ldx multiples of 8.  tile_rows 0: chosen here, with shares.
+// As hos_product4 for bfloat16 rows.  half_rows: M * (K rounded up to 8) numbers of 16 bits on 16 bytes, and row_powers: M of 32, for the rows
+// on their way.  tile_rows 0: chosen here, with shares.
 extern "C" int hos_product4_tc(const void* x, long long ldx, const void* matrix, void* out, int out_dtype, long long ldo, int M, int act, float limit,
-                               int tile_rows, int shares, long long wait_cycles, int stop_stage, cudaStream_t stream) {
-    struct Matrix4 { const uint8_t *codes, *records; int n, k, group, zeros, gated; };
+                               void* half_rows, float* row_powers, int tile_rows, int shares, long long wait_cycles, int stop_stage, cudaStream_t stream) {
+    struct Matrix4 { const uint8_t *codes, *records, *records16; const float* powers; int n, k, group, zeros, gated; };
     const Matrix4 w = *(const Matrix4*)matrix;
     if (M <= 0 || w.n <= 0) return 0;
-    if (w.k < 64 || w.k % 8 || ldx % 8 || (uintptr_t)x % 16) HOS_REFUSE("product4_tc: rows must be 16-byte pieces (K %d, %lld apart)", w.k, ldx);
+    if (w.k < 64 || half_rows == nullptr || row_powers == nullptr || (uintptr_t)half_rows % 16) HOS_REFUSE("product4_tc: K %d (64 at least), or no place for the rows", w.k);
     if (w.group < 32 || (w.group != 32 && w.group % 64)) HOS_REFUSE("product4_tc: groups of %d weights (32, or a multiple of 64)", w.group);
     if (w.k > (1 << 21) || (long long)(w.gated ? 2 : 1) * ((w.n + 15) / 16) * ((w.k + 63) / 64) * kBlockBytes >= (1ll << 32))
         HOS_REFUSE("product4_tc: %d x %d weights are more than 4 GB of codes, or k more than %d", w.n, w.k, 1 << 21);
+    const int width = (w.k + 7) / 8 * 8;
     if (out_dtype != kF32 && out_dtype != kBF16) HOS_REFUSE("product4_tc: no product into type %d", out_dtype);
     if (tile_rows == 0) plan_tiles(M, w.n, w.k, w.gated != 0, tile_rows, shares);
     const int k_blocks = (w.k + 63) / 64, sub = w.group == 32 ? 2 : 1;
@@ -409,8 +489,8 @@ extern "C" int hos_product4_tc(const void* x, long long ldx, const void* matrix,
         HOS_REFUSE("product4_tc: tiles of %d rows in %d shares", tile_rows, shares);
     Product4Args p = {};
     CUtensorMap rows_map;                                    // boxes of 64 numbers of tile_rows rows; what is beyond them reads as zeros
-    if (int rc = tc_make_map(&rows_map, x, M, w.k, (int)ldx, tile_rows)) return rc;
-    p.codes = w.codes; p.records = w.records; p.out = out; p.ldo = ldo;
+    if (int rc = tc_make_map(&rows_map, half_rows, M, width, width, tile_rows)) return rc;
+    p.codes = w.codes; p.records = w.records16; p.powers = w.powers; p.row_powers = row_powers; p.out = out; p.ldo = ldo;
     p.wait_cycles = wait_cycles > 0 ? wait_cycles : kProductWaitCycles;
     p.out_f32 = out_dtype == kF32; p.M = M; p.N = w.n; p.K = w.k; p.group_blocks = w.group / 64;
     p.group_magic = p.group_blocks > 1 ? (uint32_t)(((1ull << 32) + p.group_blocks - 1) / p.group_blocks) : 0u; p.act = act; p.limit = limit;
@@ -419,6 +499,9 @@ extern "C" int hos_product4_tc(const void* x, long long ldx, const void* matrix,
     if (ctas > 0x7fffffffll) HOS_REFUSE("product4_tc: %d rows", M);
     const int a_stage = stage_bytes(w.gated, tile_rows);
     const int S = 6 * a_stage + 1024 <= kTcShared ? 6 : (4 * a_stage + 1024 <= kTcShared ? 4 : 3), smem = S * a_stage + 1024;
+    launch_pdl(rows_to_half_kernel, dim3((unsigned)M), dim3(256), 0, stream, (const bf16*)x, ldx, w.k, width, (__half*)half_rows, row_powers,
+               w.k % 8 == 0 && ldx % 8 == 0 && (uintptr_t)x % 16 == 0 ? 1 : 0);
+    if (int rc = check_launch("product4_tc: rows")) return rc;
 #define HOS_PT(SS, G, U, Z) return launch_product4_tc<SS, G, U, Z>(rows_map, p, (int)ctas, smem, stream)
 #define HOS_PT_S(G, U, Z) do { if (S == 6) HOS_PT(6, G, U, Z); else if (S == 4) HOS_PT(4, G, U, Z); else HOS_PT(3, G, U, Z); } while (0)
 #define HOS_PT_U(G, Z) do { if (sub == 2) HOS_PT_S(G, 2, Z); else HOS_PT_S(G, 1, Z); } while (0)

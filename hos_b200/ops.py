@@ -1421,7 +1421,7 @@ def _check_rows(t: torch.Tensor, what: str, dtype=None) -> None:
 
 class Matrix4(ctypes.Structure):
     """A matrix in 4 bits as csrc/weights4.cu takes it."""
-    _fields_ = [("codes", _p), ("records", _p), ("n", _i), ("k", _i), ("group", _i), ("zeros", _i), ("gated", _i)]
+    _fields_ = [("codes", _p), ("records", _p), ("records16", _p), ("powers", _p), ("n", _i), ("k", _i), ("group", _i), ("zeros", _i), ("gated", _i)]
 
 
 class Paged4(ctypes.Structure):
@@ -1445,12 +1445,15 @@ def product4(x: torch.Tensor, matrix: int, out: torch.Tensor, act: int = 0, limi
                    act, limit, _stream())
 
 
-def product4_tc(x: torch.Tensor, matrix: int, out: torch.Tensor, act: int = 0, limit: float = 0.0, tile_rows: int = 0, shares: int = 1,
+def product4_tc(x: torch.Tensor, matrix: int, k: int, out: torch.Tensor, act: int = 0, limit: float = 0.0, tile_rows: int = 0, shares: int = 1,
                 wait_cycles: int = 0, stop_stage: int = -1) -> None:
-    """As product4 for many bfloat16 rows, on the tcgen05 tensor cores; the weights are rounded to bfloat16.  tile_rows, shares: rows of a
+    """As product4 for many bfloat16 rows of k numbers, on the tcgen05 tensor cores; the weights are formed in half precision.  tile_rows, shares: rows of a
     tile (0: chosen by the kernel's library) and CTAs that share its k.  wait_cycles, stop_stage: for tests of a wait that runs out."""
-    fourbit().call("hos_product4_tc", x.data_ptr(), x.stride(0), matrix, out.data_ptr(), dtype_code(out.dtype), out.stride(0), x.shape[0], act, limit,
-                   tile_rows, shares, wait_cycles, stop_stage, _stream())
+    m, width = x.shape[0], -(-k // 8) * 8
+    rows = torch.empty(m * width + 2 * m, dtype=torch.float16, device=x.device)      # and a 32-bit power of two a row behind them
+    at = rows.data_ptr()
+    fourbit().call("hos_product4_tc", x.data_ptr(), x.stride(0), matrix, out.data_ptr(), dtype_code(out.dtype), out.stride(0), m, act, limit,
+                   at, at + 2 * m * width, tile_rows, shares, wait_cycles, stop_stage, _stream())
 
 
 def copy_pages(table: torch.Tensor, most_bytes: int, src: torch.Tensor, dst: torch.Tensor, n_pages: int) -> None:

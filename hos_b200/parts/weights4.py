@@ -15,14 +15,31 @@ from .. import ops
 from ..errors import KernelError, SpecError
 
 ROWS, COLS = 16, 64             # of a block of codes
-FEW_ROWS = 32                   # up to so many rows the codes are multiplied as they are, above the weights are rounded to bfloat16
+FEW_ROWS = 32                   # up to so many rows the codes are multiplied as they are, above the weights are formed in half precision
+MOST_TC_K = 1 << 21
+
+
+def _in_half(records: torch.Tensor, n: int, blocks: int, zeros: bool):
+    """What the products of many rows take: the records with scales in half precision, a feature's times the power of two that brings its
+    largest between 1 and 2, and 1024 + zero codes; and the powers that undo it, float32 [blocks * n]."""
+    r = records.float()                                          # [blocks * tiles, groups, 8, 1 or 2, 2]
+    tiles = r.shape[0] // blocks
+    scale = r[:, :, :, 0].nan_to_num(0.0, 0.0, 0.0).abs().amax(1)   # [blocks * tiles, 8, 2]: of the rows g and g + 8
+    power = torch.exp2(torch.floor(torch.log2(scale.double().clamp(min=2.0 ** -126))).clamp(-126, 127)).float()
+    power = torch.where(scale > 0, power, 1.0)
+    r[:, :, :, 0] /= power[:, None]
+    if zeros:
+        r[:, :, :, 1] += 1024.0 - 128.0
+    powers = power.permute(0, 2, 1).reshape(blocks, tiles * ROWS)[:, :n].contiguous()
+    return r.to(torch.float16).contiguous(), powers.view(-1)
 
 
 class Weight4:
     def __init__(self, codes: torch.Tensor, records: torch.Tensor, n: int, k: int, group: int, blocks: int, zeros: bool):
         self.codes, self.records = codes, records
+        self.records16, self.powers = _in_half(records, n, blocks, zeros)
         self.n, self.k, self.group, self.blocks, self.zeros = n, k, group, blocks, zeros
-        self._matrix = ops.Matrix4(codes.data_ptr(), records.data_ptr(), n, k, group, int(zeros), int(blocks == 2))
+        self._matrix = ops.Matrix4(codes.data_ptr(), records.data_ptr(), self.records16.data_ptr(), self.powers.data_ptr(), n, k, group, int(zeros), int(blocks == 2))
         self._address = ctypes.addressof(self._matrix)
 
     @property
@@ -30,7 +47,7 @@ class Weight4:
         return torch.Size((self.blocks * self.n, self.k))
 
     def nbytes(self) -> int:
-        return self.codes.numel() + 2 * self.records.numel()
+        return self.codes.numel() + 2 * (self.records.numel() + self.records16.numel()) + 4 * self.powers.numel()
 
     @classmethod
     def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor], group: int, blocks: int = 1) -> "Weight4":
@@ -112,8 +129,8 @@ class Weight4:
             ops._check_rows(out, "product")
             if tuple(out.shape) != (x.shape[0], self.n):
                 raise KernelError(f"product with 4-bit weights: the output is {tuple(out.shape)}, not {(x.shape[0], self.n)}")
-        if x.shape[0] > FEW_ROWS and x.dtype == torch.bfloat16 and self.k >= COLS and self.k % 8 == 0 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0:
-            ops.product4_tc(x, self._address, out, act, cap)
+        if x.shape[0] > FEW_ROWS and x.dtype == torch.bfloat16 and COLS <= self.k <= MOST_TC_K and self.codes.numel() < 1 << 32:
+            ops.product4_tc(x, self._address, self.k, out, act, cap)
         else:
             ops.product4(x, self._address, out, act, cap)
         return out
