@@ -220,10 +220,10 @@ store4_many_kernel(const T* rows, long long stride, T* held, long long held_stri
 // neighbouring rows of a sequence, each with its own mask).  The score of a key is
 // sum_g (s_g (sum_{d in g} q c') - 136 s_g sum q + m_g sum q) over its groups of 64, c' = 128 + c + 8 the operand as codes_to_bf16 makes
 // it without subtracting: a group's product starts at -136 sum q and is multiplied by the key's scale, in 32 bits; neither scale nor
-// middle is rounded into an operand.  Values: O^T = V^T P^T with 16 numbers of a head as rows, P times the value's scale as two bfloat16
-// numbers (2^-17 of a weight; with one, 2^-9, long rows whose output is a small mean lost as much as the result's own rounding), the
-// codes exact, and the middles' sum, one number a group and head, in 32 bits beside it.  The scores' registers, transposed eight by
-// eight, are P's operand.
+// middle is rounded into an operand.  Values: O^T = V^T P^T with 16 numbers of a head as rows, P times the value's scale in half
+// precision (attention4.cuh; in bfloat16, 2^-9 of a weight, long rows whose output is a small mean lost as much as the result's own
+// rounding), the codes exact, and the middles' sum, one number a group and head, in 32 bits beside it.  The scores' registers,
+// transposed eight by eight, are P's operand.
 // Rows in 32 bits: q, and p times the scale, are three bfloat16 numbers each, exactly, and the codes are subtracted first.
 //
 // A CTA takes a share of the pages of one (row or neighbouring rows, kv head, 8 heads); its warps take 16 keys in turn, each through a ring of its own that
@@ -276,7 +276,7 @@ attend4_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out,
                const int* __restrict__ token_seq, const int* __restrict__ seq_slot, const int* __restrict__ token_slot, const int* __restrict__ cu_seqlens, int row_base,
                int n_seqs, int n_tokens, Paged4 c, int n_heads, float scale, float cap, int window, int share, int splits, float* __restrict__ part_o, float2* __restrict__ part_ml) {
     using A = Attend4<DIM>;
-    constexpr int G = A::kGroups, kTerms = sizeof(T) == 4 ? 3 : 1, kWeightTerms = kTerms == 3 ? 3 : 2, kTiles = DIM / 16;
+    constexpr int G = A::kGroups, kTerms = sizeof(T) == 4 ? 3 : 1, kTiles = DIM / 16;
     constexpr bool kExact = kTerms == 3;
     extern __shared__ __align__(16) uint8_t ring_bytes[];
     __shared__ __align__(16) uint4 q_frag[kTerms][G][2][32];
@@ -373,6 +373,9 @@ attend4_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out,
     __syncthreads();
 
     float o[kTiles][4], mid[G][2], best[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+    float into[G];                                              // of the weights in half precision
+#pragma unroll
+    for (int i = 0; i < G; ++i) into[i] = kIntoFirst;
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 #pragma unroll
@@ -444,7 +447,30 @@ attend4_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out,
             if (hidden[e]) s[e] = -INFINITY;
         }
         float top[2] = {fmaxf(s[0], s[2]), fmaxf(s[1], s[3])};
-        if (__any_sync(0xffffffffu, top[0] > best[0] + 8.f || top[1] > best[1] + 8.f)) {
+        float scale_of[G], most = 0.f;                         // the larger of a lane's two values' scales, where a column sees them
+        if (!kExact) {
+            const bool seen[2] = {!edge || (key <= last && (window == 0 || key > pos0 - window)), !edge || (key + 8 <= last && (window == 0 || key + 8 > pos0 - window))};
+#pragma unroll
+            for (int i = 0; i < G; ++i) {
+                scale_of[i] = fmaxf(seen[0] ? bf16_lo(vm[0][i]) : 0.f, seen[1] ? bf16_lo(vm[1][i]) : 0.f);
+                most = fmaxf(most, scale_of[i] * into[i]);
+            }
+        }
+        if (__any_sync(0xffffffffu, top[0] > best[0] + 8.f || top[1] > best[1] + 8.f || most > kIntoMost)) {
+            if (!kExact) {
+#pragma unroll
+                for (int i = 0; i < G; ++i) {
+                    const float largest = warp_max(scale_of[i]);
+                    if (largest * into[i] > kIntoMost && largest < INFINITY) {
+                        const float now = into_of(largest), f = now * back_of(into[i]);
+                        into[i] = now;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            o[4 * i + j][0] *= f; o[4 * i + j][1] *= f; o[4 * i + j][2] *= f; o[4 * i + j][3] *= f;
+                        }
+                    }
+                }
+            }
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) {
                 top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], off));
@@ -472,29 +498,39 @@ attend4_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out,
         sum[1] += p[1] + p[3];
 #pragma unroll
         for (int i = 0; i < G; ++i) {
+            const float sv[2] = {kExact ? bf16_lo(vm[0][i]) : bf16_lo(vm[0][i]) * into[i], kExact ? bf16_lo(vm[1][i]) : bf16_lo(vm[1][i]) * into[i]};
             float w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const uint32_t sm = vm[e >> 1][i];
-                w[e] = hidden[e] ? 0.f : p[e] * bf16_lo(sm);
-                mid[i][e & 1] = hidden[e] ? mid[i][e & 1] : fmaf(p[e], bf16_hi(sm), mid[i][e & 1]);
-            }
-            uint32_t pb[kWeightTerms][2];
-#pragma unroll
-            for (int term = 0; term < kWeightTerms; ++term) {
-                const uint32_t a = pack_bf16(w[0], w[1]), b8 = pack_bf16(w[2], w[3]);
-                pb[term][0] = transposed_8x8(a);
-                pb[term][1] = transposed_8x8(b8);
-                w[0] -= bf16_lo(a); w[1] -= bf16_hi(a); w[2] -= bf16_lo(b8); w[3] -= bf16_hi(b8);
+                w[e] = hidden[e] ? 0.f : p[e] * sv[e >> 1];
+                mid[i][e & 1] = hidden[e] ? mid[i][e & 1] : fmaf(p[e], bf16_hi(vm[e >> 1][i]), mid[i][e & 1]);
             }
             const uint4 v = lds16(slot + A::kCodes + A::kMeta + i * kBlockBytes + lane * 16);
             const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+            if (kExact) {
+                uint32_t pb[kTerms][2];
 #pragma unroll
-            for (int mt = 0; mt < 4; ++mt) {
-                uint32_t a[4];
-                codes_to_bf16<true>(words[mt], kZero8, a);
+                for (int term = 0; term < kTerms; ++term) {
+                    const uint32_t a = pack_bf16(w[0], w[1]), b8 = pack_bf16(w[2], w[3]);
+                    pb[term][0] = transposed_8x8(a);
+                    pb[term][1] = transposed_8x8(b8);
+                    w[0] -= bf16_lo(a); w[1] -= bf16_hi(a); w[2] -= bf16_lo(b8); w[3] -= bf16_hi(b8);
+                }
 #pragma unroll
-                for (int term = kWeightTerms - 1; term >= 0; --term) mma_plain(o[4 * i + mt], a, pb[term][0], pb[term][1]);
+                for (int mt = 0; mt < 4; ++mt) {
+                    uint32_t a[4];
+                    codes_to_bf16<true>(words[mt], kZero8, a);
+#pragma unroll
+                    for (int term = kTerms - 1; term >= 0; --term) mma_plain(o[4 * i + mt], a, pb[term][0], pb[term][1]);
+                }
+            } else {
+                const uint32_t p0 = transposed_8x8(pack_half(w[0], w[1])), p8 = transposed_8x8(pack_half(w[2], w[3]));
+#pragma unroll
+                for (int mt = 0; mt < 4; ++mt) {
+                    uint32_t a[4];
+                    codes_to_half(words[mt], a);
+                    mma_half(o[4 * i + mt], a, p0, p8);
+                }
             }
         }
         before = slot;
@@ -522,8 +558,9 @@ attend4_kernel(const T* __restrict__ q, long long q_stride, T* __restrict__ out,
             float* to = sums + (warp * 8 + 2 * t4 + h) * A::kPitch;
 #pragma unroll
             for (int i = 0; i < kTiles; ++i) {
-                to[i * 16 + g] = o[i][h] + mid[i / 4][h];
-                to[i * 16 + g + 8] = o[i][2 + h] + mid[i / 4][h];
+                const float back = kExact ? 1.f : back_of(into[i / 4]);       // a power of two
+                to[i * 16 + g] = fmaf(o[i][h], back, mid[i / 4][h]);
+                to[i * 16 + g + 8] = fmaf(o[i][2 + h], back, mid[i / 4][h]);
             }
         }
     }

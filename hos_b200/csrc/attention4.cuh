@@ -4,6 +4,7 @@
 #include "fourbit.cuh"
 #include "kv_layout.cuh"
 #include "mma_utils.cuh"
+#include <cuda_fp16.h>
 
 namespace hos {
 
@@ -64,6 +65,37 @@ __device__ __forceinline__ void mma_plain(float (&d)[4], const uint32_t (&a)[4],
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The same of half precision, and what the products of weights and values take: codes -8..7 (a register's bits lie where 1024 + c or 1024 + 16 c
+// is made of them at once) and weights, which are at most 2^8, times the values' scales, brought below 2^7 by a power of two of a
+// group's and walk's own (`into`, raised when a scale passes it): rounded to 2^-12 of themselves down to 2^-20 of the largest.
+__device__ __forceinline__ void mma_half(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t (&r)[4]) {
+    const uint32_t up = w >> 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t v;
+        asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(i < 2 ? w : up), "r"((i & 1) ? 0x00f000f0u : 0x000f000fu), "r"(0x64006400u));
+        const __half2 c = *reinterpret_cast<const __half2*>(&v);
+        const __half2 d = (i & 1) ? __hfma2(c, __float2half2_rn(0.0625f), __float2half2_rn(-72.f)) : __hsub2(c, __float2half2_rn(1032.f));
+        r[i] = *reinterpret_cast<const uint32_t*>(&d);
+    }
+}
+constexpr float kIntoFirst = 8.5070592e37f, kIntoMost = 128.f;        // 2^126: before the first scale
+// 1 / into
+__device__ __forceinline__ float back_of(float into) { return __uint_as_float((254u << 23) - __float_as_uint(into)); }
+__device__ __forceinline__ float into_of(float scale) {                // 2^6 <= scale * into < 2^7
+    const int e = (int)((__float_as_uint(scale) >> 23) & 255u) - 127;
+    return __uint_as_float((uint32_t)(127 + max(-126, min(126, 6 - e))) << 23);
 }
 
 }  // namespace hos

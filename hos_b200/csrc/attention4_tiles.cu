@@ -2,8 +2,8 @@
 //
 // 128 (row, head) pairs of a kv head to a CTA, 16 to a warp; a page's keys and values are formed once for all of them, as bare codes -8..7,
 // exact in bfloat16, in shared memory.  Scales and middles stay out of the operands, as in attention4.cu: a group's part of a score is
-// s (q . c) + m sum q in 32 bits; a weight times its value's scale is two bfloat16 numbers, for each group of 64 numbers anew, and the
-// middles' sum goes beside.  Bound by mma.sync (526 TFLOP/s at most): the next page is asked for while one is multiplied and
+// s (q . c) + m sum q in 32 bits; a weight times its value's scale is rounded to half precision (attention4.cuh), for each group of 64
+// numbers anew, and the middles' sum goes beside.  Bound by mma.sync (526 TFLOP/s at most): the next page is asked for while one is multiplied and
 // formed behind it.  Shares of the pages, if rows are few, merge in attention4.cu.
 // Measured (B200): a turn of 739 tokens on 7,453, 8 heads over 4 of 256: the kernel of few rows 412 us.
 #include "attention4.cuh"
@@ -16,7 +16,7 @@ template <int DIM> struct Tiles4 {
     static constexpr int kGroups = DIM / 64, kRowBytes = DIM * 2;
     static constexpr int kQ = 0, kK = kTileRows * kRowBytes, kV = kK + 2 * 64 * kRowBytes;          // bytes: two pages each
     static constexpr int kMeta = kV + 2 * 64 * kRowBytes, kQSum = kMeta + 2 * 2 * kGroups * 64 * 4, kRaw = kQSum + kTileRows * kGroups * 4;
-    static constexpr int kShared = kRaw + 2 * 36 * DIM;                                             // and a page's codes as they came
+    static constexpr int kMost = kRaw + 2 * 36 * DIM, kShared = kMost + 3 * 4 * 4;                                             // and a page's codes as they came
     static constexpr int kItems = 128 * kGroups;                                                    // 16-byte pieces of a page's codes
     static constexpr int kEach = (kItems + 255) / 256;
 };
@@ -68,7 +68,8 @@ attend4_tiles_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __res
         }
         copies_commit();
     };
-    auto form = [&](int buffer) {
+    int* most = (int*)(smem + A::kMost);                       // [3][4]: a group's largest scale of the values of page p, at p % 3
+    auto form = [&](int p, int buffer) {
         copies_wait<0>();
 #pragma unroll
         for (int i = 0; i < A::kEach; ++i) {
@@ -87,7 +88,7 @@ attend4_tiles_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __res
 #pragma unroll
             for (int w = 0; w < 4; ++w) {                      // values [number][position]: two neighbouring positions to a register
                 uint32_t r[4];
-                codes_to_bf16<true>(vw[w], kZero8, r);
+                codes_to_half(vw[w], r);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int d = grp * 64 + w * 16 + lg + 8 * (e & 1), chunk = (row16 >> 3) + (e >> 1);
@@ -101,9 +102,17 @@ attend4_tiles_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __res
             const uint4 m = lds16(raw + v * 36 * DIM + tile4_codes(DIM) + piece * 16);
             const uint32_t w[4] = {m.x, m.y, m.z, m.w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) meta[(v * G + (4 * piece + e) % G) * 64 + (4 * piece + e) / G] = w[e];
+            for (int e = 0; e < 4; ++e) {
+                const int grp = (4 * piece + e) % G, row = (4 * piece + e) / G, key = p * kPageTokens + row;
+                // a key that no row here sees may be anything: it becomes zeros
+                const uint32_t m = key <= last && (window == 0 || key > rows.pos0 - window) ? w[e] : 0u;
+                meta[(v * G + grp) * 64 + row] = m;
+                if (v == 1 && bf16_lo(m) < INFINITY) atomicMax(&most[p % 3 * 4 + grp], __float_as_int(bf16_lo(m)));      // scales are not negative
+            }
         }
     };
+    if (threadIdx.x < 12) most[threadIdx.x] = 0;
+    __syncthreads();
     ask(p0);
     // the pairs' numbers, and their sums over 64
     for (int i = threadIdx.x; i < kTileRows * DIM / 8; i += 256) {
@@ -120,14 +129,16 @@ attend4_tiles_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __res
         s += __shfl_xor_sync(0xffffffffu, s, 4);
         if ((i & 7) == 0) ((float*)(smem + A::kQSum))[j * G + chunk / 8] = s;
     }
-    form(0);
+    form(p0, 0);
     __syncthreads();
 
     const int row_a = warp * 16 + g, row_b = row_a + 8;        // a lane's two pairs
     const int pos[2] = {rows.pos0 + min(row_a, pairs - 1) / per, rows.pos0 + min(row_b, pairs - 1) / per};
     const int warp_first = rows.pos0 + min(warp * 16, pairs - 1) / per, warp_last = rows.pos0 + min(warp * 16 + 15, pairs - 1) / per;
     const bool busy = warp * 16 < pairs;
-    float o[DIM / 8][4], mid[G][2], best[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+    float o[DIM / 8][4], mid[G][2], best[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, into[G];
+#pragma unroll
+    for (int i = 0; i < G; ++i) into[i] = kIntoFirst;
 #pragma unroll
     for (int i = 0; i < DIM / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 #pragma unroll
@@ -147,6 +158,7 @@ attend4_tiles_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __res
     for (int p = p0; p < p1; ++p) {
         const int buffer = (p - p0) & 1;
         if (p + 1 < p1) ask(p + 1);
+        if (threadIdx.x < G) most[(p + 2) % 3 * 4 + threadIdx.x] = 0;          // read before the last barrier, raised behind the next
         // what lies wholly behind a warp's rows, or before their windows, is not walked over
         if (busy && p * kPageTokens <= warp_last && !(window > 0 && p * kPageTokens + 63 <= warp_first - window)) {
             const uint32_t page_at = buffer * 64 * A::kRowBytes, k0 = k_rows + page_at + k_at[0], k1 = k_rows + page_at + k_at[1];
@@ -248,61 +260,65 @@ attend4_tiles_kernel(const bf16* __restrict__ q, long long q_stride, bf16* __res
                 }
 #pragma unroll
             for (int grp = 0; grp < G; ++grp) {
-                // the weights times the scales as two bfloat16 numbers: the first, its products, then the rest of them
+                const float largest = __int_as_float(most[p % 3 * 4 + grp]);
+                if (largest * into[grp] > kIntoMost) {
+                    const float now = into_of(largest), f = now * back_of(into[grp]);
+                    into[grp] = now;
 #pragma unroll
-                for (int term = 0; term < 2; ++term) {
-                    uint32_t a[4][4];
-                    auto operand = [&](int n, const float (&w)[4]) {
-                        const uint32_t first = pack_bf16(w[0], w[1]), second = pack_bf16(w[2], w[3]);
-                        a[n >> 1][2 * (n & 1)] = term == 0 ? first : pack_bf16(w[0] - bf16_lo(first), w[1] - bf16_hi(first));
-                        a[n >> 1][2 * (n & 1) + 1] = term == 0 ? second : pack_bf16(w[2] - bf16_lo(second), w[3] - bf16_hi(second));
-                    };
-                    if (!edge) {
-#pragma unroll
-                        for (int n = 0; n < 8; ++n) {
-                            const uint2 sm = *(const uint2*)&vm[grp * 64 + n * 8 + 2 * t4];
-                            const float sv[2] = {bf16_lo(sm.x), bf16_lo(sm.y)}, mv[2] = {bf16_hi(sm.x), bf16_hi(sm.y)};
-                            const float w[4] = {s[n][0] * sv[0], s[n][1] * sv[1], s[n][2] * sv[0], s[n][3] * sv[1]};
-                            operand(n, w);
-                            if (term == 0) {
-                                mid[grp][0] = fmaf(s[n][1], mv[1], fmaf(s[n][0], mv[0], mid[grp][0]));
-                                mid[grp][1] = fmaf(s[n][3], mv[1], fmaf(s[n][2], mv[0], mid[grp][1]));
-                            }
-                        }
-                    } else {
-#pragma unroll
-                        for (int n = 0; n < 8; ++n) {
-                            const uint2 sm = *(const uint2*)&vm[grp * 64 + n * 8 + 2 * t4];
-                            float w[4];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const uint32_t m = (e & 1) ? sm.y : sm.x;
-                                const bool seen = !((hidden >> (n * 4 + e)) & 1u);
-                                w[e] = seen ? s[n][e] * bf16_lo(m) : 0.f;
-                                if (seen && term == 0) mid[grp][e >> 1] = fmaf(s[n][e], bf16_hi(m), mid[grp][e >> 1]);
-                            }
-                            operand(n, w);
-                        }
+                    for (int d = 0; d < 8; ++d) {
+                        o[grp * 8 + d][0] *= f; o[grp * 8 + d][1] *= f; o[grp * 8 + d][2] *= f; o[grp * 8 + d][3] *= f;
                     }
-#pragma unroll
-                    for (int d0 = 0; d0 < 8; d0 += 4)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            uint32_t b[4][4];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) ldmatrix_x4(b[i], (h ? v1 : v0) + (grp * 64 + (d0 + i) * 8) * 128);
-#pragma unroll
-                            for (int st = 0; st < 2; ++st)
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) mma_bf16(o[grp * 8 + d0 + i], a[2 * h + st], b[i][2 * st], b[i][2 * st + 1]);
-                        }
                 }
+                uint32_t a[4][4];
+                if (!edge) {
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) {
+                        const uint2 sm = *(const uint2*)&vm[grp * 64 + n * 8 + 2 * t4];
+                        const float sv[2] = {bf16_lo(sm.x) * into[grp], bf16_lo(sm.y) * into[grp]}, mv[2] = {bf16_hi(sm.x), bf16_hi(sm.y)};
+                        a[n >> 1][2 * (n & 1)] = pack_half(s[n][0] * sv[0], s[n][1] * sv[1]);
+                        a[n >> 1][2 * (n & 1) + 1] = pack_half(s[n][2] * sv[0], s[n][3] * sv[1]);
+                        mid[grp][0] = fmaf(s[n][1], mv[1], fmaf(s[n][0], mv[0], mid[grp][0]));
+                        mid[grp][1] = fmaf(s[n][3], mv[1], fmaf(s[n][2], mv[0], mid[grp][1]));
+                    }
+                } else {
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) {
+                        const uint2 sm = *(const uint2*)&vm[grp * 64 + n * 8 + 2 * t4];
+                        float w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t m = (e & 1) ? sm.y : sm.x;
+                            const bool seen = !((hidden >> (n * 4 + e)) & 1u);
+                            w[e] = seen ? s[n][e] * (bf16_lo(m) * into[grp]) : 0.f;
+                            if (seen) mid[grp][e >> 1] = fmaf(s[n][e], bf16_hi(m), mid[grp][e >> 1]);
+                        }
+                        a[n >> 1][2 * (n & 1)] = pack_half(w[0], w[1]);
+                        a[n >> 1][2 * (n & 1) + 1] = pack_half(w[2], w[3]);
+                    }
+                }
+#pragma unroll
+                for (int d0 = 0; d0 < 8; d0 += 4)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t b[4][4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) ldmatrix_x4(b[i], (h ? v1 : v0) + (grp * 64 + (d0 + i) * 8) * 128);
+#pragma unroll
+                        for (int st = 0; st < 2; ++st)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) mma_half(o[grp * 8 + d0 + i], a[2 * h + st], b[i][2 * st], b[i][2 * st + 1]);
+                    }
             }
         }
         if (p + 1 < p1) {
-            form(buffer ^ 1);                                  // nobody reads that one: the walk over it ended before the last barrier
+            form(p + 1, buffer ^ 1);                            // nobody reads that one: the walk over it ended before the last barrier
             __syncthreads();
         }
+    }
+#pragma unroll
+    for (int i = 0; i < DIM / 8; ++i) {
+        const float back = back_of(into[i / 8]);                  // a power of two
+        o[i][0] *= back; o[i][1] *= back; o[i][2] *= back; o[i][3] *= back;
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
