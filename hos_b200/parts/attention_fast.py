@@ -532,8 +532,9 @@ def attend_chunks(mixer, qkv, att, part, cache) -> bool:
 
 
 def attend(mixer, qkv, att, step, cache, packed: bool) -> bool:
-    """Runs the tensor-core kernel if it takes the case; False hands it to the plain kernel."""
-    if cache.k_pages.dtype != torch.bfloat16 or not supports(mixer.head_dim):
+    """Runs the tensor-core kernel if it takes the case; False hands it to the plain kernel.  `packed`: over the step's own rows, whatever
+    the cache holds its keys and values in."""
+    if (qkv if packed else cache.k_pages).dtype != torch.bfloat16 or not supports(mixer.head_dim):
         return False
     if packed:
         if not enabled["prefill"]:

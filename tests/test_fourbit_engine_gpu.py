@@ -122,3 +122,16 @@ def test_the_example_runs(tmp_path, capsys):
     assert mod.main(["--random", str(cfg), "-p", "2,5,9,11", "--answers", "3", "-n", "6", "--max-seq-len", "256"]) == 0
     lines = capsys.readouterr().out.strip().splitlines()
     assert len(lines) == 3 and len(set(lines)) > 1
+
+
+def test_prompts_over_their_own_rows_take_the_kernel_for_them(monkeypatch):
+    """A prompt attends over its own rows, which are bfloat16 whatever the pages hold: not the plain kernel's business."""
+    from hos_b200 import ops
+
+    def plain(*a, **kw):
+        raise AssertionError("the plain attention kernel ran")
+    monkeypatch.setattr(ops, "attn_plain", plain)
+    eng = engine("bfloat16", cache_bits=4)
+    eng.runner.step(eng.runner.admit(2), [ids(40, 1), ids(300, 2)])
+    eng.runner.step(eng.runner.admit(1), [ids(400, 3)], [[0, 399]])
+    torch.cuda.synchronize()
