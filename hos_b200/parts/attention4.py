@@ -49,7 +49,7 @@ def store(rows: torch.Tensor, step, cache: ops.PagedKVArgs, held: Optional[torch
                        ops.paged4(cache), n, ops._stream())
 
 
-MAX_SHARES, CLUSTER_SHARES = 1024, 8
+MAX_SHARES, CLUSTER_SHARES, MANY_SHARES = 1024, 8, 32
 
 
 def shares(rows: int, kv_items: int, longest: int, window: Optional[int], fill: float = 1.0):
@@ -58,13 +58,17 @@ def shares(rows: int, kv_items: int, longest: int, window: Optional[int], fill: 
     as fill them; many rows of unequal lengths (`fill`: the sum of the keys over rows * the longest) into shares of up to 32 pages,
     which CTAs take as they come free.  Up to 8 shares of few rows of like lengths merge as a cluster (of unlike lengths the CTAs
     without keys would wait for the others: 32 rows of up to 4,000 keys 19 us, through the workspace 15); more cost a second kernel,
-    about the time of 4 pages, and have to save that."""
+    about the time of 4 pages, and have to save that.  Beyond 32 shares one CTA an SM is enough, as the sums that are merged cost more
+    than the second brings (8 heads of 256 over 4, 8,192 keys: 64 shares 16.5 us, 32 shares 14.0; 32,000 keys: 63 shares 26.2, 32
+    shares 24.8)."""
     span = min(longest, window) if window else longest
     pages = max(1, -(-span // ops.PAGE_TOKENS) + (1 if window and longest > window else 0))
     places, items = 2 * ops.sm_count(), max(1, rows * kv_items)
     few = items * fill < places
     if few:
         share = -(-pages // max(1, int(places // max(1.0, items * fill))))
+        if -(-pages // share) > MANY_SHARES:
+            share = -(-pages // max(MANY_SHARES, int(places // 2 // max(1.0, items * fill))))
     else:
         share = pages if fill > 0.9 and items % places == 0 else 32
     share = max(1, min(share, pages), -(-pages // MAX_SHARES))
