@@ -700,8 +700,10 @@ extern "C" int hos_store4(const void* rows, int dtype, long long stride, void* h
     HOS_CHECK_PAGED4("store4");
     const int per_row = 2 * n_kv_heads * (head_dim / 64), piece = dtype == kF32 ? 4 : 8;
     const int vec = (stride % piece == 0 && (uintptr_t)rows % 16 == 0 ? 1 : 0) | (held_stride % piece == 0 && (uintptr_t)held % 16 == 0 ? 2 : 0);
-    const bool many = n_tokens >= 32 && !single;
     const long long items = (long long)n_tokens * per_row;
+    // Pieces of 64 numbers from which blocks of 16 positions written whole pay (us, a piece's lanes for themselves / blocks of positions;
+    // 4 kv heads of 256: 128 rows, 4,096 pieces, 3.3 / 5.0, 512 rows, 16,384, 4.5 / 5.2; 16 of 128: 512 rows, 32,768, 6.6 / 5.9).
+    const bool many = items >= 24576 && !single;
     // every sequence may begin and end inside a block
     const dim3 few_grid((unsigned)((items + 31) / 32)), many_grid((unsigned)((n_tokens + 15) / 16 + 2 * n_seqs), (unsigned)((per_row + 7) / 8));
     if (many && many_grid.y > 65535) HOS_REFUSE("store4: %d kv heads", n_kv_heads);

@@ -52,17 +52,24 @@ def store(rows: torch.Tensor, step, cache: ops.PagedKVArgs, held: Optional[torch
 MAX_SHARES, CLUSTER_SHARES, MANY_SHARES = 1024, 8, 32
 
 
+def _pages(longest: int, window: Optional[int], new: int = 0) -> int:
+    """Pages that a walk for `new` more rows than one sees at most."""
+    span = min(longest, window + new) if window else longest
+    return max(1, -(-span // ops.PAGE_TOKENS) + (1 if window and longest > window else 0))
+
+
 def shares(rows: int, kv_items: int, longest: int, window: Optional[int], fill: float = 1.0):
     """(pages of a share, shares of a row, whether the shares are a cluster): `rows` rows times `kv_items` (kv heads, times the eights of
     query heads that share one) over up to `longest` keys.  Two CTAs fit an SM: rows that leave CTAs free are cut into as many shares
     as fill them; many rows of unequal lengths (`fill`: the sum of the keys over rows * the longest) into shares of up to 32 pages,
-    which CTAs take as they come free.  Up to 8 shares of few rows of like lengths merge as a cluster (of unlike lengths the CTAs
-    without keys would wait for the others: 32 rows of up to 4,000 keys 19 us, through the workspace 15); more cost a second kernel,
-    about the time of 4 pages, and have to save that.  Beyond 32 shares one CTA an SM is enough, as the sums that are merged cost more
-    than the second brings (8 heads of 256 over 4, 8,192 keys: 64 shares 16.5 us, 32 shares 14.0; 32,000 keys: 63 shares 26.2, 32
-    shares 24.8)."""
-    span = min(longest, window) if window else longest
-    pages = max(1, -(-span // ops.PAGE_TOKENS) + (1 if window and longest > window else 0))
+    which CTAs take as they come free.  2, 4 or 8 shares of few rows of like lengths merge as a cluster (16 rows, 8 heads of 256 over 4,
+    2,000 keys, 4 shares: 20.0 us, through the workspace 22.5), not 3 or 6, whose clusters leave places of their neighbourhood of SMs
+    empty and run in two rounds (12 rows, 6 shares 28.9 us, through the workspace 20.4), nor, for the same reason, 4 or 8 in more than
+    256 CTAs (36 rows, 16 heads of 64 over 2, 4 shares 35.4 and 25.0), nor of unlike lengths, where CTAs without keys would wait for the
+    others (32 rows of up to 4,000 keys 19 us, 15).  More cost a second kernel, about the time of 4 pages, and have to save that.
+    Beyond 32 shares one CTA an SM is enough, as the sums that are merged cost more than the second brings (8 heads of 256 over 4,
+    8,192 keys: 64 shares 16.5 us, 32 shares 14.0; 32,000 keys: 63 shares 26.2, 32 shares 24.8)."""
+    pages = _pages(longest, window)
     places, items = 2 * ops.sm_count(), max(1, rows * kv_items)
     few = items * fill < places
     if few:
@@ -76,7 +83,7 @@ def shares(rows: int, kv_items: int, longest: int, window: Optional[int], fill: 
     if few and share < least <= share + 4:
         share = least
     splits = -(-pages // share)
-    return share, splits, few and fill > 0.8 and 1 < splits <= CLUSTER_SHARES
+    return share, splits, few and fill > 0.8 and (splits == 2 or splits in (4, 8) and items * splits <= 256)
 
 
 def attend(q: torch.Tensor, out: torch.Tensor, step, cache: ops.PagedKVArgs, n_heads: int, scale: float, softcap: float = 0.0,
@@ -93,7 +100,9 @@ def attend(q: torch.Tensor, out: torch.Tensor, step, cache: ops.PagedKVArgs, n_h
     kv = cache.n_kv_heads
     items = kv * -(-(n_heads // kv) // 8)
     if _tiles_take(q, out, step, n_heads // kv):
-        return _attend_tiles(q, out, step, cache, n_heads, scale, softcap, window)
+        plan = _tile_plan(n, step, cache, n_heads // kv, items, window)
+        if plan is not None:
+            return _attend_tiles(q, out, step, cache, n_heads, scale, softcap, window, plan)
     together = 1 if step.single_token else max(1, 8 // (n_heads // kv))      # rows of a sequence that share a walk
     key = ("shares of 4-bit pages", n, items, together, window, step.row_offset)
     plan = step.shared.get(key)                      # once per step and kind of layer
@@ -111,24 +120,43 @@ def attend(q: torch.Tensor, out: torch.Tensor, step, cache: ops.PagedKVArgs, n_h
 
 
 TILE_ROWS = 128                # (row, head) pairs of a kv head that a block of the kernel for pieces takes
-TILE_MIN_PAIRS = 48
+TILE_LEAST = 2                 # pages of a share at least
 
 
 def _tiles_take(q, out, step, per: int) -> bool:
-    """Whether the rows go to the kernel for pieces: bfloat16 rows on 16 bytes, and sequences that bring enough (row, head) pairs."""
-    return (not step.single_token and q.dtype == torch.bfloat16 and step.max_new * per >= TILE_MIN_PAIRS and per <= TILE_ROWS and q.stride(0) % 8 == 0
-            and out.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0)
+    """Whether the kernel for pieces could take the rows: bfloat16 rows on 16 bytes of sequences that go on by several tokens."""
+    return (not step.single_token and q.dtype == torch.bfloat16 and per <= TILE_ROWS and q.stride(0) % 8 == 0 and out.stride(0) % 8 == 0
+            and q.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0)
 
 
-def _attend_tiles(q, out, step, cache: ops.PagedKVArgs, n_heads: int, scale: float, softcap: float, window: Optional[int]) -> None:
-    n, kv = q.shape[0], cache.n_kv_heads
-    size = TILE_ROWS // (n_heads // kv)
-    key = ("tiles over 4-bit pages", n, size, kv, window, step.row_offset)
-    plan = step.shared.get(key)                      # once per step and kind of layer
-    if plan is None:
-        plan = step.shared[key] = tile_shares(-(-n // size) if not step.cu_host else
-                                              sum(-(-(b - a) // size) for a, b in zip(step.cu_host, step.cu_host[1:])), kv,
-                                              step.max_len_after, step.max_new, window)
+def _tile_plan(n: int, step, cache: ops.PagedKVArgs, per: int, items: int, window: Optional[int]):
+    """(pages of a share, shares) of the kernel for pieces, or None where the kernel of few rows is the faster by both's estimates."""
+    size, kv = TILE_ROWS // per, cache.n_kv_heads
+    key = ("tiles over 4-bit pages", n, size, kv, cache.head_dim, window, step.row_offset)
+    if key not in step.shared:                       # once per step and kind of layer
+        blocks = -(-n // size) if not step.cu_host else sum(-(-(b - a) // size) for a, b in zip(step.cu_host, step.cu_host[1:]))
+        blocks = max(1, blocks)
+        plan = tile_shares(blocks, kv, step.max_len_after, step.max_new, window)
+        walks = -(-n // max(1, 8 // per))
+        take = tiles_are_faster(blocks * kv, plan, n / (blocks * size), walks * items * _pages(step.max_len_after, window),
+                                step.fill_for(window), cache.head_dim)
+        step.shared[key] = plan if take else None
+    return step.shared[key]
+
+
+def tiles_are_faster(blocks: int, plan, filled: float, row_pages: float, fill: float, dim: int) -> bool:
+    """Microseconds of both kernels, fitted to batches of pieces (B200; heads of 64, 128 and 256, 16 to 1,000 rows on up to 16,000 keys):
+    an SM's page with 128 pairs, or with some of a block's eight warps at work (`filled`), no less than 0.6 of it; and a page for eight
+    pairs in one of two CTAs an SM.  Of 114 batches 107 run within 4% of the faster kernel's time, the worst 1.23 times it.  8 heads of 256
+    over 4, tiles / few rows: 739 on 7,453 312 us / 412, 400 on 2,600 93 / 125, 128 on 872 38 / 27, 16 on 7,984 36 / 26."""
+    share, splits = plan
+    tiles = max(1.0, blocks * splits * fill / ops.sm_count()) * share * max(0.6, min(1.0, filled)) * (0.65 + 0.03 * dim) + 10 + dim / 25
+    rows = row_pages * fill / (2 * ops.sm_count()) * (0.2 + 0.0055 * dim) + 7 + dim / 50
+    return tiles < rows
+
+
+def _attend_tiles(q, out, step, cache: ops.PagedKVArgs, n_heads: int, scale: float, softcap: float, window: Optional[int], plan) -> None:
+    n = q.shape[0]
     share, splits = plan
     parts = None
     if splits > 1:
@@ -144,9 +172,8 @@ def _attend_tiles(q, out, step, cache: ops.PagedKVArgs, n_heads: int, scale: flo
 
 def tile_shares(blocks: int, kv: int, longest: int, new: int, window: Optional[int]):
     """(pages of a share, shares) for `blocks` blocks of rows and kv heads of which an SM takes one at a time: as many shares as fill
-    the SMs, each of at least 8 pages (a share costs about 2 besides, and its sums are written, read and merged)."""
-    span = min(longest, window + new) if window else longest
-    pages = max(1, -(-span // ops.PAGE_TOKENS) + (1 if window else 0))
-    splits = max(1, min(pages // 8, ops.sm_count() // max(1, blocks * kv)))
+    the SMs, each of at least 2 pages (48 rows on 952 keys, 8 heads of 256 over 4: 30 us, of 4 pages 40, of 8 62)."""
+    pages = _pages(longest, window, new)
+    splits = max(1, min(pages // TILE_LEAST, ops.sm_count() // max(1, blocks * kv)))
     share = -(-pages // splits)
     return share, -(-pages // share)

@@ -15,7 +15,11 @@ from .. import ops
 from ..errors import KernelError, SpecError
 
 ROWS, COLS = 16, 64             # of a block of codes
-FEW_ROWS = 32                   # up to so many rows the codes are multiplied as they are, above the weights are formed in half precision
+# Up to so many rows the codes are multiplied as they are, above the weights are formed in half precision (us a product, that kernel's / the
+# tcgen05 one's: 2304 x 9216, 32 rows 12.8 / 19.3, 33 rows, one more tile of 32, 22.1 / 19.6; 9216 x 2304 gated, 16 rows 13.6 / 17.5, 32 rows
+# 20.9 / 18.5, 33 rows 35.9 / 19.1).  Gated products of many weights would gain from 17 rows on (14336 x 3584, 24 rows 42.2 / 32.2), but
+# up to 32 rows, where most steps of a few sequences lie, no weight is rounded.
+FEW_ROWS = 32
 MOST_TC_K = 1 << 21
 
 
@@ -41,6 +45,7 @@ class Weight4:
         self.n, self.k, self.group, self.blocks, self.zeros = n, k, group, blocks, zeros
         self._matrix = ops.Matrix4(codes.data_ptr(), records.data_ptr(), self.records16.data_ptr(), self.powers.data_ptr(), n, k, group, int(zeros), int(blocks == 2))
         self._address = ctypes.addressof(self._matrix)
+        self._forms = COLS <= k <= MOST_TC_K and codes.numel() < 1 << 32      # what the kernel that forms weights takes
 
     @property
     def shape(self):
@@ -129,7 +134,7 @@ class Weight4:
             ops._check_rows(out, "product")
             if tuple(out.shape) != (x.shape[0], self.n):
                 raise KernelError(f"product with 4-bit weights: the output is {tuple(out.shape)}, not {(x.shape[0], self.n)}")
-        if x.shape[0] > FEW_ROWS and x.dtype == torch.bfloat16 and COLS <= self.k <= MOST_TC_K and self.codes.numel() < 1 << 32:
+        if x.shape[0] > FEW_ROWS and self._forms and x.dtype == torch.bfloat16:
             ops.product4_tc(x, self._address, self.k, out, act, cap)
         else:
             ops.product4(x, self._address, out, act, cap)
