@@ -136,7 +136,7 @@ def _tile_plan(n: int, step, cache: ops.PagedKVArgs, per: int, items: int, windo
     if key not in step.shared:                       # once per step and kind of layer
         blocks = -(-n // size) if not step.cu_host else sum(-(-(b - a) // size) for a, b in zip(step.cu_host, step.cu_host[1:]))
         blocks = max(1, blocks)
-        plan = tile_shares(blocks, kv, step.max_len_after, step.max_new, window)
+        plan = tile_shares(blocks, kv, step.max_len_after, step.max_new, window, cache.head_dim)
         walks = -(-n // max(1, 8 // per))
         take = tiles_are_faster(blocks * kv, plan, n / (blocks * size), walks * items * _pages(step.max_len_after, window),
                                 step.fill_for(window), cache.head_dim)
@@ -150,7 +150,8 @@ def tiles_are_faster(blocks: int, plan, filled: float, row_pages: float, fill: f
     pairs in one of two CTAs an SM.  Of 114 batches 107 run within 4% of the faster kernel's time, the worst 1.23 times it.  8 heads of 256
     over 4, tiles / few rows: 739 on 7,453 312 us / 412, 400 on 2,600 93 / 125, 128 on 872 38 / 27, 16 on 7,984 36 / 26."""
     share, splits = plan
-    tiles = max(1.0, blocks * splits * fill / ops.sm_count()) * share * max(0.6, min(1.0, filled)) * (0.65 + 0.03 * dim) + 10 + dim / 25
+    two = dim == 64 and blocks * splits > ops.sm_count()      # on an SM, which slows each
+    tiles = (1.6 if two else 1.0) * max(1.0, blocks * splits * fill / ((2 if two else 1) * ops.sm_count())) * share * max(0.6, min(1.0, filled)) * (0.65 + 0.03 * dim) + 10 + dim / 25
     rows = row_pages * fill / (2 * ops.sm_count()) * (0.2 + 0.0055 * dim) + 7 + dim / 50
     return tiles < rows
 
@@ -170,10 +171,11 @@ def _attend_tiles(q, out, step, cache: ops.PagedKVArgs, n_heads: int, scale: flo
                  ops._stream())
 
 
-def tile_shares(blocks: int, kv: int, longest: int, new: int, window: Optional[int]):
-    """(pages of a share, shares) for `blocks` blocks of rows and kv heads of which an SM takes one at a time: as many shares as fill
+def tile_shares(blocks: int, kv: int, longest: int, new: int, window: Optional[int], head_dim: int = 128):
+    """(pages of a share, shares) for `blocks` blocks of rows and kv heads of which an SM takes one at a time (of heads of 64 two: 400 rows
+    on 7,600 keys, 16 heads over 2, shares for one 180 us, for two 110; of 128 two gain 3% at most and few rows lose): as many shares as fill
     the SMs, each of at least 2 pages (48 rows on 952 keys, 8 heads of 256 over 4: 30 us, of 4 pages 40, of 8 62)."""
     pages = _pages(longest, window, new)
-    splits = max(1, min(pages // TILE_LEAST, ops.sm_count() // max(1, blocks * kv)))
+    splits = max(1, min(pages // TILE_LEAST, (2 if head_dim == 64 else 1) * ops.sm_count() // max(1, blocks * kv)))
     share = -(-pages // splits)
     return share, -(-pages // share)
