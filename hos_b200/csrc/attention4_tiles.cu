@@ -3,9 +3,11 @@
 // 128 (row, head) pairs of a kv head to a CTA, 16 to a warp; a page's keys and values are formed once for all of them, as bare codes -8..7,
 // exact in bfloat16, in shared memory.  Scales and middles stay out of the operands, as in attention4.cu: a group's part of a score is
 // s (q . c) + m sum q in 32 bits; a weight times its value's scale is rounded to half precision (attention4.cuh), for each group of 64
-// numbers anew, and the middles' sum goes beside.  Bound by mma.sync (526 TFLOP/s at most): the next page is asked for while one is multiplied and
-// formed behind it.  Shares of the pages, if rows are few, merge in attention4.cu.
-// Measured (B200): a turn of 739 tokens on 7,453, 8 heads over 4 of 256: the kernel of few rows 412 us.
+// numbers anew, and the middles' sum goes beside.  The next page is asked for while one is multiplied and formed behind it.  Shares of the
+// pages, if rows are few, merge in attention4.cu.
+// Measured (B200): a turn of 739 tokens on 7,453, 8 heads over 4 of 256, 312 us, 152 TFLOP/s of the 526 that mma.sync gives at most; the
+// kernel of few rows 412.  Bound by latency: the sums of 128 pairs leave registers for 8 warps an SM, which issue in 36% of the clocks; the
+// tensor pipe is busy in 33%, shared memory in 19%.  (16 warps, heads of 128, with sums in local memory: 3% faster at most.)
 #include "attention4.cuh"
 
 namespace hos {

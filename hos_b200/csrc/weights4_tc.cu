@@ -11,6 +11,7 @@
 // Few tiles share K as a cluster, whose sums meet in shared memory.
 // Bound by the products where rows fill the tile (2 clocks a row and stage), else by forming the weights: plan_tiles below chooses rows
 // a tile and CTAs a cluster by these.
+// Measured (B200, 14336 x 3584 gated, groups of 128 with zero codes): 64 rows 34 us, 512 rows 100 us (1.05 PFLOP/s), 2,048 rows 355 us (1.19).
 #include "common.cuh"
 #include "fourbit.cuh"
 #include "mma_utils.cuh"
@@ -442,7 +443,8 @@ static int clusters_at_once(int shares) {
 }
 
 // Rows of a tile and CTAs that share a tile's K: the least of waves x (stages x clocks a stage + what a tile costs besides), in clocks.
-// Sums of shares have to fit where the operands were.
+// Sums of shares have to fit where the operands were.  Of 40 products of 33 to 2,048 rows and four shapes the plan chosen took the least time
+// of those tried or up to 2% more, but for 200 and 256 rows of 4096 x 2048 (18.8 and 19.5 us, 17.8 with tiles of 64).
 static void plan_tiles(int M, int N, int K, bool gated, int& tile_rows, int& shares) {
     const int sm = sm_count_cached(), acc = gated ? 2 : 1, feature_tiles = (N + kTcFeatures - 1) / kTcFeatures, k_blocks = (K + 63) / 64;
     double best = 0.;
