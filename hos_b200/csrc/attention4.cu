@@ -723,9 +723,10 @@ extern "C" int hos_store4(const void* rows, int dtype, long long stride, void* h
     return check_launch("store4");
 }
 
-// token_slot: seq_slot[token_seq] of every row, or null.  cu_seqlens: the sequences' rows (less row_base), n_seqs + 1 of
-// them, padding rows behind: neighbouring rows of a sequence share a walk if the kv heads have few heads; null: every row alone.  A walk over its pages, `share` of them to a CTA: `splits` shares cover the longest row's.  2 to 8 without
-// `parts` are a cluster; else more than one need `parts`, n_tokens * n_heads * splits * (head_dim + 2) 32-bit numbers.
+// token_slot: seq_slot[token_seq] of every row, or null.  cu_seqlens: the sequences' rows (less row_base), n_seqs + 1 of them, padding rows
+// behind: neighbouring rows of a sequence share a walk if the kv heads have few heads; null: every row alone.  A walk is cut into shares
+// of `share` pages, a CTA each: `splits` of them cover the longest row's.  2 to 8 without `parts` are a cluster; else more than one need
+// `parts`, n_tokens * n_heads * splits * (head_dim + 2) 32-bit numbers.
 extern "C" int hos_attend4(const void* q, int dtype, long long q_stride, void* out, long long out_stride, const int* token_pos, const int* token_seq,
                            const int* seq_slot, const int* token_slot, const int* cu_seqlens, int row_base, int n_seqs, const void* cache, int n_tokens, int n_heads, float scale, float cap, int window,
                            int share, int splits, float* parts, cudaStream_t stream) {
