@@ -1,11 +1,13 @@
 // Products of many rows with weights in 4 bits on the 5th-generation tensor cores: out[M, N] = x[M, K] . W[N, K]^T in bfloat16.
 //
-// The weights are formed in half precision on their way: (c - z) s, c - z exact and the product, of 12 bits, rounded once (2^-12 of a
-// weight; in bfloat16 it would be 2^-9, as much as the result's own rounding), straight into the operand's place in shared memory, so
+// The weights are formed in half precision on their way: (c - z) s, c - z exact and the product, of 12 bits, rounded once (2^-11 of a
+// weight; in bfloat16 it would be 2^-8, as much as the result's own rounding), straight into the operand's place in shared memory, so
 // that they cross memory in 4 bits however many rows there are.  Half precision has few exponents: a feature's scales are held times a
-// power of two that brings the largest between 1 and 2 (parts/weights4.py), a row of x is brought to 2^10 at most by one of its own
-// (rows_to_half_kernel; numbers below 2^-34 of the row's largest are lost), and the powers come back in the epilogue, exactly.  A CTA takes 128 features (gated: 128 of gate and the same 128 of up) and up to 256 rows, tcgen05.mma with M = 128
-// features and N = rows.  Three groups of eight warps take the stages of 64 k in turn: each warp forms 16 features (its codes wait in
+// power of two that brings the largest between 2^11 and 2^12 (parts/weights4.py; 15 of it are still a number, and scales down to 2^-25 of the
+// largest keep all their bits, the last of them is lost below 2^-36), a row of x by one of its own to between 2^10 and 2^11 at its largest
+// (rows_to_half_kernel; numbers below 2^-36 of that are lost), and the powers come back in the epilogue, exactly.
+// A CTA takes 128 features (gated: 128 of gate and the same 128 of up) and up to 256 rows, tcgen05.mma with M = 128 features and N =
+// rows.  Three groups of eight warps take the stages of 64 k in turn: each warp forms 16 features (its codes wait in
 // registers, asked for a turn ahead); one more warp brings the rows of x by TMA, and one issues the products.  (With the rows
 // brought by the makers' cp.async the fence behind what they form waited for those copies too: 2304 x 9216, 64 rows on one SM a tile 64 us.)
 // Few tiles share K as a cluster, whose sums meet in shared memory.
@@ -171,32 +173,31 @@ __global__ void __launch_bounds__(256) rows_to_half_kernel(const bf16* __restric
     for (int i = threadIdx.x + 256 * kHeld; 8 * i < width; i += 256) put(i, load(i));
 }
 
-// The operand's registers of a word of codes: 1024 + c where a code's bits are the lowest of a half, 1024 + 16 c where they are the next;
-// minus 1024 + z or 1024 + 16 z, exact, times s or s / 16.
-struct Scale16 { uint32_t s, s16, z, z16; };
-__device__ __forceinline__ uint32_t half_weight(uint32_t w, uint32_t mask, uint32_t z, uint32_t s) {
+// The operand's registers of a word of codes: 1024 + c where a code's bits are the lowest of a half, 1024 + 16 c where they are the next,
+// a sixteenth of which is 64 + c; minus 1024 + z or 64 + z, both exact, times s: the only rounding.
+struct Scale16 { uint32_t s, z, z64; };                      // s, 1024 + z, -(64 + z)
+__device__ __forceinline__ uint32_t half_weight(uint32_t w, bool upper, const Scale16& k) {
     uint32_t v;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(w), "r"(mask), "r"(0x64006400u));
-    const __half2 c = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&z)), *reinterpret_cast<const __half2*>(&s));
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(w), "r"(upper ? 0x00f000f0u : 0x000f000fu), "r"(0x64006400u));
+    const __half2 h = *reinterpret_cast<const __half2*>(&v);
+    const __half2 code = upper ? __hfma2(h, __float2half2_rn(0.0625f), *reinterpret_cast<const __half2*>(&k.z64)) : __hsub2(h, *reinterpret_cast<const __half2*>(&k.z));
+    const __half2 c = __hmul2(code, *reinterpret_cast<const __half2*>(&k.s));
     return *reinterpret_cast<const uint32_t*>(&c);
 }
 __device__ __forceinline__ uint4 half_weights(uint32_t w, const Scale16& k) {
     const uint32_t up = w >> 8;
-    return make_uint4(half_weight(w, 0x000f000fu, k.z, k.s), half_weight(w, 0x00f000f0u, k.z16, k.s16), half_weight(up, 0x000f000fu, k.z, k.s),
-                      half_weight(up, 0x00f000f0u, k.z16, k.s16));
+    return make_uint4(half_weight(w, false, k), half_weight(w, true, k), half_weight(up, false, k), half_weight(up, true, k));
 }
 template <bool ZEROS>
 __device__ __forceinline__ Scale16 scale_of(uint32_t two, uint32_t zeros, uint32_t pick) {
     Scale16 k;
     k.s = __byte_perm(two, 0, pick);
-    const __half2 s16 = __hmul2(*reinterpret_cast<const __half2*>(&k.s), __float2half2_rn(0.0625f));
-    k.s16 = *reinterpret_cast<const uint32_t*>(&s16);
     k.z = 0x64086408u;                                       // 1024 + 8
-    k.z16 = 0x64806480u;                                     // 1024 + 128
+    k.z64 = 0xd480d480u;                                     // -(64 + 8)
     if (ZEROS) {
         k.z = __byte_perm(zeros, 0, pick);
-        const __half2 z16 = __hfma2(*reinterpret_cast<const __half2*>(&k.z), __float2half2_rn(16.f), __float2half2_rn(-15360.f));
-        k.z16 = *reinterpret_cast<const uint32_t*>(&z16);
+        const __half2 z64 = __hsub2(__float2half2_rn(960.f), *reinterpret_cast<const __half2*>(&k.z));
+        k.z64 = *reinterpret_cast<const uint32_t*>(&z64);
     }
     return k;
 }

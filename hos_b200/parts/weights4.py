@@ -21,16 +21,18 @@ ROWS, COLS = 16, 64             # of a block of codes
 # up to 32 rows, where most steps of a few sequences lie, no weight is rounded.
 FEW_ROWS = 32
 MOST_TC_K = 1 << 21
+LARGEST_SCALE = 2048.0          # a feature's largest scale in half precision lies between it and twice it
 
 
 def _in_half(records: torch.Tensor, n: int, blocks: int, zeros: bool):
     """What the products of many rows take: the records with scales in half precision, a feature's times the power of two that brings its
-    largest between 1 and 2, and 1024 + zero codes; and the powers that undo it, float32 [blocks * n]."""
+    largest between 2^11 and 2^12 (a weight is at most 15 of it, 61,440), and 1024 + zero codes; and the powers that undo it, float32
+    [blocks * n]."""
     r = records.float()                                          # [blocks * tiles, groups, 8, 1 or 2, 2]
     tiles = r.shape[0] // blocks
     scale = r[:, :, :, 0].nan_to_num(0.0, 0.0, 0.0).abs().amax(1)   # [blocks * tiles, 8, 2]: of the rows g and g + 8
     power = torch.exp2(torch.floor(torch.log2(scale.double().clamp(min=2.0 ** -126))).clamp(-126, 127)).float()
-    power = torch.where(scale > 0, power, 1.0)
+    power = torch.where(scale > 0, power, 1.0) / LARGEST_SCALE
     r[:, :, :, 0] /= power[:, None]
     if zeros:
         r[:, :, :, 1] += 1024.0 - 128.0
