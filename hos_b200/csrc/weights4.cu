@@ -9,7 +9,7 @@
 // rows of x) and a share of K; its blocks come through a ring of its own in shared memory by cp.async, kRing blocks ahead, so that
 // nothing but its own copies is ever waited for.  The warps of a CTA share K; their sums are added in a fixed order, and how K is cut
 // hangs on N and K alone, so that a row's bits hang on no other row.  Rows in 32 bits are three bfloat16 numbers each,
-// x = x1 + x2 + x3 exactly (8 + 8 + 8 bits), and three products a block.
+// x = x1 + x2 + x3 exactly (8 + 8 + 8 bits), and three products a block.  A sum that is not finite is formed again number by number.
 // Measured (B200): 8 rows of 36864 x 4608 gated 41 us (4.4 TB/s of codes and scales: a block's operands take about as many instructions as
 // its bytes take time); 1 row of 2304 x 9216 7.2 us, 5 rows in 32 bits of 2051 x 1999 4.7 us (11 and 2 MB: launch, first bytes, sums).
 #include "common.cuh"
@@ -82,9 +82,79 @@ __device__ __forceinline__ void load_row(Row16 (&r)[3], const float* p, int left
     }
 }
 
+// One number of the product by the definition, for sums that are not finite: an infinity of x, or numbers near the largest, meet 128 + c,
+// an infinity's rest or a group's sum of bare codes on their way above, and give NaN where the result is an infinity or a number.  (c - z) s
+// is exact in 32 bits, so nothing is larger here than the products themselves.  tile, records: of the feature's 16 rows, of which it is row r.
+template <typename XT, int SUB, bool ZEROS>
+__device__ float sum_by_definition(const XT* __restrict__ x, const uint8_t* __restrict__ tile, const uint8_t* __restrict__ records, int r, int K,
+                                   int group_blocks) {
+    constexpr int kRecord = ZEROS ? 64 : 32;
+    float total = 0.f;
+#pragma unroll 1
+    for (int kb = 0; kb * 64 < K; ++kb) {
+        float block = 0.f;
+#pragma unroll 1
+        for (int e = 0; e < 8; ++e) {                              // eight numbers to a word
+            const uint8_t* rec = records + (size_t)(SUB == 2 ? 2 * kb + (e >> 2) : kb / group_blocks) * kRecord + (r & 7) * (kRecord / 8) + (r >> 3) * 2;
+            const uint32_t w = *(const uint32_t*)(tile + (size_t)kb * kBlockBytes + ((r & 7) * 4 + (e & 3)) * 16 + ((r >> 3) * 2 + (e >> 2)) * 4);
+            const float s = to_float(*(const bf16*)rec), z = ZEROS ? to_float(*(const bf16*)(rec + 4)) - 128.f : 8.f;
+            const int k = kb * 64 + e * 8;
+            float part = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (k + j < K) part = fmaf(((float)((w >> code_shift(j)) & 15u) - z) * s, to_float(x[k + j]), part);
+            block += part;
+        }
+        total += block;
+    }
+    return total;
+}
+
 // MT: tiles of 8 rows of x; T: tiles of 16 features a warp (the first half of them gate's, the other up's, if GATED); SUB: scales a
 // block of 64 (2: groups of 32); ring_of: blocks of T tiles that a warp's ring holds.
 template <int T> struct ring_of { static constexpr int value = T == 1 ? 8 : (T == 2 ? 6 : 4); };
+// The warps' sums (fixed order) and the epilogue.  AGAIN: sums that are not finite are formed by the definition.  That is a function of its
+// own, so that what only it needs takes no registers from the walk; up to 16 rows it is called for such sums alone (a call costs 0.2 us of
+// 4.5), above always, as the walk's registers are full and even the look at the sums beside it would spill more of them (24 rows of 14336 x
+// 3584 gated, 41 us, 51).
+template <typename XT, int MT, int T, bool GATED, int SUB, bool ZEROS, int WARPS, bool AGAIN>
+__device__ __forceinline__ bool write_sums(const float* sums, const XT* __restrict__ x, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ records,
+                                           void* __restrict__ out, int out_f32, int M, int N, int K, long long ldx, long long ldo, int group_blocks, int act,
+                                           float limit) {
+    constexpr int kWide = GATED ? T / 2 : T, kSums = T * MT * 16 * 9, kTerms = sizeof(XT) == 4 ? 3 : 1, kRecord = ZEROS ? 64 : 32;
+    const int m0 = blockIdx.y * 8 * MT;
+    bool finite = true;
+    for (int i = threadIdx.x; i < MT * 8 * 16 * kWide; i += WARPS * 32) {
+        const int tok = i / (16 * kWide), r = i % (16 * kWide), n = blockIdx.x * 16 * kWide + r;      // consecutive threads: consecutive features
+        if (m0 + tok >= M || n >= N) continue;
+        float v[GATED ? 2 : 1];
+#pragma unroll
+        for (int h = 0; h < (GATED ? 2 : 1); ++h) {
+            v[h] = 0.f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) v[h] += sums[w * kSums + ((h * kWide + r / 16) * MT + tok / 8) * 144 + (r & 15) * 9 + tok % 8];
+            if (!AGAIN) finite &= isfinite(v[h]);
+            if (AGAIN && !isfinite(v[h])) {
+                const int tiles = (N + 15) / 16, k_blocks = (K + 63) / 64, groups = SUB == 2 ? 2 * k_blocks : (k_blocks + group_blocks - 1) / group_blocks;
+                const size_t tile = (size_t)h * tiles + blockIdx.x * kWide + r / 16;
+                v[h] = sum_by_definition<XT, SUB, ZEROS>(x + (size_t)(m0 + tok) * ldx, codes + tile * k_blocks * kBlockBytes,
+                                                         records + tile * groups * kRecord, r & 15, K, group_blocks);
+            }
+        }
+        const float y = GATED ? gate_times(act, v[0], v[GATED ? 1 : 0], limit, kTerms == 1) : v[0];
+        const size_t at = (size_t)(m0 + tok) * ldo + n;
+        if (kTerms == 3 || out_f32) ((float*)out)[at] = y;
+        else ((bf16*)out)[at] = __float2bfloat16_rn(y);
+    }
+    return finite;
+}
+template <typename XT, int MT, int T, bool GATED, int SUB, bool ZEROS, int WARPS>
+__device__ __noinline__ void write_sums_again(const float* sums, const XT* __restrict__ x, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ records,
+                                              void* __restrict__ out, int out_f32, int M, int N, int K, long long ldx, long long ldo, int group_blocks, int act,
+                                              float limit) {
+    write_sums<XT, MT, T, GATED, SUB, ZEROS, WARPS, true>(sums, x, codes, records, out, out_f32, M, N, K, ldx, ldo, group_blocks, act, limit);
+}
+
 template <typename XT, int MT, int T, bool GATED, int SUB, bool ZEROS, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32, 16 / WARPS)
 product4_kernel(const XT* __restrict__ x, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ records, void* __restrict__ out, int out_f32,
@@ -290,21 +360,8 @@ product4_kernel(const XT* __restrict__ x, const uint8_t* __restrict__ codes, con
             p[(g + 8) * 9 + 2 * t4 + 1] = acc[t][m][3];
         }
     __syncthreads();
-    for (int i = threadIdx.x; i < MT * 8 * 16 * kWide; i += WARPS * 32) {
-        const int tok = i / (16 * kWide), r = i % (16 * kWide), n = blockIdx.x * 16 * kWide + r;      // consecutive threads: consecutive features
-        if (m0 + tok >= M || n >= N) continue;
-        float v[GATED ? 2 : 1];
-#pragma unroll
-        for (int h = 0; h < (GATED ? 2 : 1); ++h) {
-            v[h] = 0.f;
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w) v[h] += sums[w * kSums + ((h * kWide + r / 16) * MT + tok / 8) * 144 + (r & 15) * 9 + tok % 8];
-        }
-        const float y = GATED ? gate_times(act, v[0], v[GATED ? 1 : 0], limit, kTerms == 1) : v[0];
-        const size_t at = (size_t)(m0 + tok) * ldo + n;
-        if (kTerms == 3 || out_f32) ((float*)out)[at] = y;
-        else ((bf16*)out)[at] = __float2bfloat16_rn(y);
-    }
+    if (MT == 4 || !write_sums<XT, MT, T, GATED, SUB, ZEROS, WARPS, false>(sums, x, codes, records, out, out_f32, M, N, K, ldx, ldo, group_blocks, act, limit))
+        write_sums_again<XT, MT, T, GATED, SUB, ZEROS, WARPS>(sums, x, codes, records, out, out_f32, M, N, K, ldx, ldo, group_blocks, act, limit);
 }
 
 template <typename XT, int MT, int T, bool GATED, int SUB, bool ZEROS, int WARPS>

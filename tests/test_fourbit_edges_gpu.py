@@ -29,3 +29,64 @@ def test_weights_of_many_rows_are_rounded_once_however_small_their_scale_is(grou
     w = (codes.double() - (z.double()[:, at] if zeros else 8.0)) * scales.double()[:, at]
     got = Weight4.from_codes(codes, scales, z, group).product(torch.eye(k, device=DEV, dtype=BF), F32)
     assert bool(((got.double() - w.T).abs() <= 2.0 ** -11 * w.T.abs()).all())
+
+
+def check_odd_rows(x, w4, w, eps):
+    """A product's row is infinite, or not a number, where the definition's is; elsewhere as near as ever."""
+    got = w4.product(x, F32).double()
+    xd = x.double()
+    y, size = xd @ w.T, xd.abs() @ w.abs().T
+    assert torch.equal(torch.isnan(got), torch.isnan(y))
+    inf = torch.isinf(y)
+    assert torch.equal(torch.isinf(got), inf) and torch.equal(got[inf], y[inf])
+    fine = torch.isfinite(y)
+    assert bool(((got - y).abs() <= size * eps)[fine].all())
+
+
+@pytest.mark.parametrize("dtype,eps", [(BF, 2.0 ** -18), (F32, 2.0 ** -20)])
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True)])
+@pytest.mark.parametrize("m", [1, 7, 12, 32])
+def test_infinities_in_rows_give_infinities(m, group, zeros, dtype, eps):
+    from hos_b200.parts.weights4 import Weight4
+    codes, scales, z, w = made_weights(100, 333, group, zeros, 13)
+    w4 = Weight4.from_codes(codes, scales, z, group)
+    x = torch.randn(m, 333, generator=gen(14)).to(dtype).to(DEV)
+    x[m // 2, 5] = math.inf
+    check_odd_rows(x, w4, w, eps)
+    x[m - 1, 332] = -math.inf
+    check_odd_rows(x, w4, w, eps)
+    x[0, 100] = math.nan
+    check_odd_rows(x, w4, w, eps)
+
+
+@pytest.mark.parametrize("dtype,eps", [(BF, 2.0 ** -18), (F32, 2.0 ** -20)])
+@pytest.mark.parametrize("m", [1, 7, 12, 32])
+def test_rows_of_numbers_near_the_largest(m, dtype, eps):
+    """Sums of codes times numbers pass the largest that 32 bits hold, sums of weights times numbers do not."""
+    from hos_b200.parts.weights4 import Weight4
+    for zeros in (False, True):
+        codes, scales, z, w = made_weights(100, 512, 64, zeros, 15)
+        w4 = Weight4.from_codes(codes, scales, z, 64)
+        x = torch.randn(m, 512, generator=gen(16)).to(DEV)
+        x[m // 2] = 2.0 ** 121 * (1 + torch.rand(512, generator=gen(17)).to(DEV))
+        check_odd_rows(x.to(dtype), w4, w, eps)
+
+
+@pytest.mark.parametrize("m", [1, 20])
+def test_gated_products_of_infinities(m):
+    from hos_b200 import ops
+    from hos_b200.parts import linear
+    from hos_b200.parts.weights4 import Weight4
+    codes, scales, z, w = made_weights(2 * 50, 256, 64, False, 18)
+    scales = scales.abs() + 0.001
+    codes = torch.where(codes == 8, 9, codes).to(torch.uint8)      # no weight is 0: an infinity times it is one
+    w4 = Weight4.from_codes(codes, scales, None, 64, blocks=2)
+    w = (codes.double() - 8) * scales.double().repeat_interleave(64, 1)
+    x = torch.randn(m, 256, generator=gen(19)).to(BF).to(DEV)
+    x[m - 1, 77] = -math.inf
+    got = linear.matmul(x, w4, F32, epilogue=ops.EPI_GATED, act=ops.ACT_GELU_TANH).double()
+    gate, up = (x.double() @ w.T).split(50, dim=1)
+    row = torch.where(gate[m - 1] > 0, gate[m - 1] * up[m - 1], math.nan)      # gelu of -infinity is 0, or, as formed, not a number
+    pos = gate[m - 1] > 0
+    assert bool(pos.any()) and torch.equal(got[m - 1][pos], row[pos])
+    assert bool(torch.isfinite(got[:m - 1]).all())
