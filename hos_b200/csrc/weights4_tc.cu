@@ -113,7 +113,12 @@ __device__ __forceinline__ float gated_value(int act, float gate, float up, floa
     return act == 2 ? clamped_swish_fast(gate, up, limit) : (act == 0 ? gelu_tanh_fast(gate) : silu_fast(gate)) * up;
 }
 
-// S: stages of operands; SUB: scales a block of 64 (2: groups of 32).
+// A sum times its feature's and its row's power of two.  Where one is as large as the other is small, the two first: the sum times one of
+// them may pass the largest number.  Else one after the other, as the two together might, beside a sum of 0.
+__device__ __forceinline__ float times_powers(float v, float feature, float row) {
+    return (feature < 1.f) == (row < 1.f) ? v * feature * row : v * (feature * row);
+}
+
 // A row of x in half precision, its numbers times a power of two, padded to `width` with zeros; a block a row.
 __global__ void __launch_bounds__(256) rows_to_half_kernel(const bf16* __restrict__ x, long long ldx, int K, int width, __half* __restrict__ y,
                                                            float* __restrict__ row_powers, int whole) {
@@ -202,6 +207,7 @@ __device__ __forceinline__ Scale16 scale_of(uint32_t two, uint32_t zeros, uint32
     return k;
 }
 
+// S: stages of operands; SUB: scales a block of 64 (2: groups of 32).
 template <int S, bool GATED, int SUB, bool ZEROS>
 __global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(const __grid_constant__ CUtensorMap rows_map, Product4Args p) {
     constexpr int kAcc = GATED ? 2 : 1, kRecord = ZEROS ? 64 : 32;
@@ -354,11 +360,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(const __grid
             for (int j = 0; j < 16; ++j) {
                 const int c = c0 + j, m = m0 + c;
                 if (p.shares > 1) {
-                    sums[c * 128 + feature] = __uint_as_float(v[j]) * power;
-                    if (GATED) sums[(p.tile_rows + c) * 128 + feature] = __uint_as_float(u[j]) * up_power;
+                    sums[c * 128 + feature] = __uint_as_float(v[j]);
+                    if (GATED) sums[(p.tile_rows + c) * 128 + feature] = __uint_as_float(u[j]);
                 } else if (m < p.M && n < p.N) {
-                    const float back = p.row_powers[m], gate = __uint_as_float(v[j]) * power * back;
-                    const float y = GATED ? gated_value(p.act, gate, __uint_as_float(u[j]) * up_power * back, p.limit) : gate;
+                    const float back = p.row_powers[m], gate = times_powers(__uint_as_float(v[j]), power, back);
+                    const float y = GATED ? gated_value(p.act, gate, times_powers(__uint_as_float(u[j]), up_power, back), p.limit) : gate;
                     if (p.out_f32) ((float*)p.out)[(size_t)m * p.ldo + n] = y;
                     else ((bf16*)p.out)[(size_t)m * p.ldo + n] = __float2bfloat16_rn(y);
                 }
@@ -372,6 +378,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(const __grid
         shares_meet();
         if (warp < kTcMakers && !gave_up) {
             const int feature = threadIdx.x & 127, n = f0 + feature;
+            const float power = n < p.N ? p.powers[n] : 0.f, up_power = GATED && n < p.N ? p.powers[p.N + n] : 0.f;
             const uint32_t at = smem_u32(sums);
             for (int c = kTcMakers / 4 * share + (threadIdx.x >> 7); c < p.tile_rows; c += kTcMakers / 4 * p.shares) {
                 float v = 0.f, u = 0.f;
@@ -381,7 +388,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) product4_tc_kernel(const __grid
                 }
                 const int m = m0 + c;
                 if (m < p.M && n < p.N) {
-                    const float back = p.row_powers[m], y = GATED ? gated_value(p.act, v * back, u * back, p.limit) : v * back;
+                    const float back = p.row_powers[m], gate = times_powers(v, power, back);
+                    const float y = GATED ? gated_value(p.act, gate, times_powers(u, up_power, back), p.limit) : gate;
                     if (p.out_f32) ((float*)p.out)[(size_t)m * p.ldo + n] = y;
                     else ((bf16*)p.out)[(size_t)m * p.ldo + n] = __float2bfloat16_rn(y);
                 }

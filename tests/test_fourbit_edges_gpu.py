@@ -90,3 +90,35 @@ def test_gated_products_of_infinities(m):
     pos = gate[m - 1] > 0
     assert bool(pos.any()) and torch.equal(got[m - 1][pos], row[pos])
     assert bool(torch.isfinite(got[:m - 1]).all())
+
+
+@pytest.mark.parametrize("shares", [1, 4])
+@pytest.mark.parametrize("scale,row", [(112, -112), (-112, 112), (120, -100), (-120, 100)])
+def test_a_features_scale_and_a_rows_size_far_from_one_undo_each_other(scale, row, shares):
+    from hos_b200 import ops
+    from hos_b200.parts.weights4 import Weight4
+    codes, scales, z, w = made_weights(150, 512, 64, True, 20)
+    scales = (scales.float() * 2.0 ** scale).to(BF)                # some of the smallest are subnormal: rounded here
+    w4 = Weight4.from_codes(codes, scales, z, 64)
+    at = torch.arange(512, device=DEV) // 64
+    w = (codes.double() - z.double()[:, at]) * scales.double()[:, at]
+    x = (torch.randn(48, 512, generator=gen(21)) * 2.0 ** row).to(BF).to(DEV)
+    got = torch.empty(48, 150, device=DEV)
+    ops.product4_tc(x, w4._address, 512, got, 0, 0.0, 48, shares)
+    y, size = x.double() @ w.T, x.double().abs() @ w.abs().T
+    assert bool(((got.double() - y).abs() <= size * 2.0 ** -10.9).all())
+
+
+@pytest.mark.parametrize("shares", [1, 4])
+def test_nothing_times_the_largest_powers_is_nothing(shares):
+    from hos_b200 import ops
+    from hos_b200.parts.weights4 import Weight4
+    codes = torch.full((128, 256), 8, dtype=torch.uint8, device=DEV)
+    codes[1] = 9                                                   # one feature whose products pass the largest number
+    w4 = Weight4.from_codes(codes, torch.full((128, 4), 2.0 ** 120, device=DEV, dtype=BF), None, 64)
+    x = torch.full((48, 256), 2.0 ** 100, device=DEV, dtype=BF)
+    got = torch.empty(48, 128, device=DEV)
+    ops.product4_tc(x, w4._address, 256, got, 0, 0.0, 48, shares)
+    assert bool(torch.isinf(got[:, 1]).all())
+    got[:, 1] = 0
+    assert float(got.abs().max()) == 0
