@@ -40,8 +40,16 @@ def _in_half(records: torch.Tensor, n: int, blocks: int, zeros: bool):
     return r.to(torch.float16).contiguous(), powers.view(-1)
 
 
+def _check_on_gpu(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """The kernels keep the tensors' addresses: all of them have to be one GPU's."""
+    there = {t.device for t in tensors if t is not None}
+    if len(there) != 1 or next(iter(there)).type != "cuda":
+        raise SpecError(f"{what} must be on the GPU, all on the same, found {sorted(map(str, there))}")
+
+
 class Weight4:
     def __init__(self, codes: torch.Tensor, records: torch.Tensor, n: int, k: int, group: int, blocks: int, zeros: bool):
+        _check_on_gpu("a matrix in 4 bits", codes, records)
         self.codes, self.records = codes, records
         self.records16, self.powers = _in_half(records, n, blocks, zeros)
         self.n, self.k, self.group, self.blocks, self.zeros = n, k, group, blocks, zeros
@@ -58,12 +66,13 @@ class Weight4:
 
     @classmethod
     def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor], group: int, blocks: int = 1) -> "Weight4":
-        """codes: uint8 [rows, k], 0..15; scales: [rows, ceil(k / group)], kept in bfloat16; zeros: uint8 like the scales, or None.
+        """On the GPU, codes: uint8 [rows, k], 0..15; scales: [rows, ceil(k / group)], kept in bfloat16; zeros: uint8 like the scales, or None.
         `blocks`: the rows are that many matrices one after another (2: gate and up of a gated feed-forward)."""
         if group != 32 and (group < 64 or group % 64):
             raise SpecError(f"groups of {group} weights: 32 or a multiple of 64 is wanted")
         if codes.dim() != 2 or codes.dtype != torch.uint8:
             raise SpecError(f"codes must be uint8 [rows, k], found {codes.dtype} {tuple(codes.shape)}")
+        _check_on_gpu("codes, scales and zero codes", codes, scales, zeros)
         rows, k = codes.shape
         want = (rows, -(-k // group))
         if k == 0 or rows == 0 or blocks < 1 or rows % blocks:
@@ -98,6 +107,7 @@ class Weight4:
         magnitude / 7, per group; the scale is rounded to bfloat16 before the codes are taken."""
         if w.dim() != 2 or not w.is_floating_point():
             raise SpecError(f"a matrix is wanted, found {w.dtype} {tuple(w.shape)}")
+        _check_on_gpu("a matrix to be held in 4 bits", w)
         rows, k = w.shape
         g = torch.nn.functional.pad(w.float(), (0, -k % group)).view(rows, -1, group)
         if not bool(torch.isfinite(g).all()):

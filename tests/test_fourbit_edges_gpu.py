@@ -122,3 +122,13 @@ def test_nothing_times_the_largest_powers_is_nothing(shares):
     assert bool(torch.isinf(got[:, 1]).all())
     got[:, 1] = 0
     assert float(got.abs().max()) == 0
+
+
+def test_scales_and_zero_codes_that_lie_elsewhere_than_the_codes_are_refused():
+    from hos_b200.errors import SpecError
+    from hos_b200.parts.weights4 import Weight4
+    codes, scales, z, _ = made_weights(32, 128, 64, True, 22)
+    for bad in (dict(codes=codes.cpu()), dict(scales=scales.cpu()), dict(scales=scales.cpu(), zeros=None), dict(zeros=z.cpu()),
+                dict(codes=codes.cpu(), scales=scales.cpu(), zeros=None)):
+        with pytest.raises(SpecError, match="GPU"):
+            Weight4.from_codes(**{**dict(codes=codes, scales=scales, zeros=z, group=64), **bad})

@@ -1,0 +1,19 @@
+"""What the 4-bit operators refuse on the host, before any kernel has an address (no GPU)."""
+import pytest
+import torch
+
+from hos_b200.errors import SpecError
+from hos_b200.parts.weights4 import Weight4
+
+
+def test_weights_that_are_not_on_the_gpu_are_refused():
+    """Codes of a checkpoint lie on the host at first; a kernel would read the host's addresses."""
+    codes, scales = torch.zeros(32, 128, dtype=torch.uint8), torch.ones(32, 2)
+    with pytest.raises(SpecError, match="GPU"):
+        Weight4.from_codes(codes, scales, None, 64)
+    with pytest.raises(SpecError, match="GPU"):
+        Weight4.from_codes(codes, scales, torch.zeros(32, 2, dtype=torch.uint8), 64)
+    with pytest.raises(SpecError, match="GPU"):
+        Weight4.from_matrix(torch.ones(32, 128))
+    with pytest.raises(SpecError, match="GPU"):
+        Weight4(torch.zeros(2, 2, 512, dtype=torch.uint8), torch.zeros(2, 2, 8, 1, 2, dtype=torch.bfloat16), 32, 128, 64, 1, False)
