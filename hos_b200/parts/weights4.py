@@ -47,6 +47,11 @@ def _check_on_gpu(what: str, *tensors: Optional[torch.Tensor]) -> None:
         raise SpecError(f"{what} must be on the GPU, all on the same, found {sorted(map(str, there))}")
 
 
+def _check_group(group: int) -> None:
+    if group != 32 and (group < 64 or group % 64):
+        raise SpecError(f"groups of {group} weights: 32 or a multiple of 64 is wanted")
+
+
 class Weight4:
     def __init__(self, codes: torch.Tensor, records: torch.Tensor, n: int, k: int, group: int, blocks: int, zeros: bool):
         _check_on_gpu("a matrix in 4 bits", codes, records)
@@ -68,8 +73,7 @@ class Weight4:
     def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor], group: int, blocks: int = 1) -> "Weight4":
         """On the GPU, codes: uint8 [rows, k], 0..15; scales: [rows, ceil(k / group)], kept in bfloat16; zeros: uint8 like the scales, or None.
         `blocks`: the rows are that many matrices one after another (2: gate and up of a gated feed-forward)."""
-        if group != 32 and (group < 64 or group % 64):
-            raise SpecError(f"groups of {group} weights: 32 or a multiple of 64 is wanted")
+        _check_group(group)
         if codes.dim() != 2 or codes.dtype != torch.uint8:
             raise SpecError(f"codes must be uint8 [rows, k], found {codes.dtype} {tuple(codes.shape)}")
         _check_on_gpu("codes, scales and zero codes", codes, scales, zeros)
@@ -87,14 +91,14 @@ class Weight4:
         tiles, k_blocks = -(-n // ROWS), -(-k // COLS)
         groups = -(-k_blocks * COLS // group)
         padded = codes.new_zeros((blocks, tiles * ROWS, k_blocks * COLS))
-        padded[:, :n, :k] = codes.view(blocks, n, k)
+        padded[:, :n, :k] = codes.reshape(blocks, n, k)
         # a row 8 hi + g, a number 32 w + 8 t + 2 r + h of a block: byte (g, t, hi, w, h, r / 2), nibble r % 2
         p = padded.view(blocks * tiles, 2, 8, k_blocks, 2, 4, 4, 2).permute(0, 3, 2, 5, 1, 4, 7, 6)
         packed = (p[..., 0::2] | (p[..., 1::2] << 4)).contiguous().view(blocks * tiles, k_blocks, 512)
 
         def records(t):                                      # [blocks * tiles, groups, 8, 2]: rows g and g + 8 side by side
             r = t.new_zeros((blocks, tiles * ROWS, groups), dtype=torch.bfloat16)
-            r[:, :n, :want[1]] = t.view(blocks, n, want[1]).to(torch.bfloat16)
+            r[:, :n, :want[1]] = t.reshape(blocks, n, want[1]).to(torch.bfloat16)
             return r.view(blocks * tiles, 2, 8, groups).permute(0, 3, 2, 1)
         parts = [records(scales)]
         if zeros is not None:
@@ -105,11 +109,12 @@ class Weight4:
     def from_matrix(cls, w: torch.Tensor, group: int = 64, zeros: bool = False, blocks: int = 1) -> "Weight4":
         """The matrix [rows, k] rounded: scale (max - min) / 15 and the zero code nearest to 0's place (`zeros`), or largest
         magnitude / 7, per group; the scale is rounded to bfloat16 before the codes are taken."""
+        _check_group(group)
         if w.dim() != 2 or not w.is_floating_point():
             raise SpecError(f"a matrix is wanted, found {w.dtype} {tuple(w.shape)}")
         _check_on_gpu("a matrix to be held in 4 bits", w)
         rows, k = w.shape
-        g = torch.nn.functional.pad(w.float(), (0, -k % group)).view(rows, -1, group)
+        g = torch.nn.functional.pad(w.float(), (0, -k % group)).reshape(rows, -1, group)
         if not bool(torch.isfinite(g).all()):
             raise SpecError("a matrix with infinities or NaN cannot be held in 4 bits")
         if zeros:

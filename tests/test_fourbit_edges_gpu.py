@@ -132,3 +132,15 @@ def test_scales_and_zero_codes_that_lie_elsewhere_than_the_codes_are_refused():
                 dict(codes=codes.cpu(), scales=scales.cpu(), zeros=None)):
         with pytest.raises(SpecError, match="GPU"):
             Weight4.from_codes(**{**dict(codes=codes, scales=scales, zeros=z, group=64), **bad})
+
+
+def test_matrices_and_codes_whose_numbers_do_not_lie_side_by_side():
+    from hos_b200.parts.weights4 import Weight4
+    codes, scales, z, _ = made_weights(48, 128, 64, True, 23)
+    x = torch.randn(3, 128, device=DEV)
+    want = Weight4.from_codes(codes, scales, z, 64, blocks=1).product(x)
+    apart = Weight4.from_codes(codes.t().contiguous().t(), scales.t().contiguous().t(), z.repeat_interleave(2, 1)[:, ::2], 64)
+    assert torch.equal(apart.product(x), want)
+    w = torch.randn(128, 48, device=DEV).t()
+    for zeros in (False, True):
+        assert torch.equal(Weight4.from_matrix(w, 64, zeros).product(x), Weight4.from_matrix(w.contiguous(), 64, zeros).product(x))

@@ -17,3 +17,11 @@ def test_weights_that_are_not_on_the_gpu_are_refused():
         Weight4.from_matrix(torch.ones(32, 128))
     with pytest.raises(SpecError, match="GPU"):
         Weight4(torch.zeros(2, 2, 512, dtype=torch.uint8), torch.zeros(2, 2, 8, 1, 2, dtype=torch.bfloat16), 32, 128, 64, 1, False)
+
+
+@pytest.mark.parametrize("group", [0, -64, 48, 33])
+def test_groups_that_no_kernel_takes_are_refused(group):
+    with pytest.raises(SpecError, match="groups"):
+        Weight4.from_matrix(torch.ones(32, 128), group)
+    with pytest.raises(SpecError, match="groups"):
+        Weight4.from_codes(torch.zeros(32, 128, dtype=torch.uint8), torch.ones(32, 2), None, group)
