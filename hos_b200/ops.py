@@ -1430,9 +1430,15 @@ class Paged4(ctypes.Structure):
 
 
 def paged4(cache: PagedKVArgs) -> int:
-    """Address of the view's description, made once for as long as the view's arrays stay."""
+    """Address of the view's description, made (and the view looked at) once for as long as the view's arrays stay."""
     d = cache.four
     if d is None:
+        tile = (cache.n_kv_heads, tile4_bytes(cache.head_dim))
+        for t, what in ((cache.k_pages, "pages of keys"), (cache.v_pages, "pages of values")):
+            _check(t, what, torch.uint8, 3)
+            if tuple(t.shape[1:]) != tile or t.shape[0] != cache.k_pages.shape[0]:
+                raise KernelError(f"{what} in 4 bits must be [{cache.k_pages.shape[0]}, {tile[0]}, {tile[1]}], found {tuple(t.shape)}")
+        _check(cache.page_table, "page table", torch.int32, 2)
         d = Paged4(cache.k_pages.data_ptr(), cache.v_pages.data_ptr(), cache.page_table.data_ptr(), cache.table_stride, cache.ring_pages,
                    cache.n_kv_heads, cache.head_dim)
         cache.four = d = (d, ctypes.addressof(d))

@@ -27,6 +27,8 @@ def _check_cache(cache: ops.PagedKVArgs) -> None:
 def _check_step(n: int, step, what: str) -> None:
     if step.n_tokens != n:
         raise KernelError(f"{what}: {n} rows for a step of {step.n_tokens} tokens")
+    if not step.token_pos.is_cuda:               # a step's arrays are made together
+        raise KernelError(f"{what}: the step must be on the GPU")
 
 
 def store(rows: torch.Tensor, step, cache: ops.PagedKVArgs, held: Optional[torch.Tensor] = None) -> None:

@@ -8,7 +8,7 @@ import math
 import pytest
 import torch
 
-from test_fourbit_gpu import gen, made_weights
+from test_fourbit_gpu import Paged, gen, made_weights
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -144,3 +144,22 @@ def test_matrices_and_codes_whose_numbers_do_not_lie_side_by_side():
     w = torch.randn(128, 48, device=DEV).t()
     for zeros in (False, True):
         assert torch.equal(Weight4.from_matrix(w, 64, zeros).product(x), Weight4.from_matrix(w.contiguous(), 64, zeros).product(x))
+
+
+def test_views_and_steps_of_another_kind_are_refused():
+    import dataclasses
+    from hos_b200.engine.batch import build_step
+    from hos_b200.errors import KernelError
+    from hos_b200.parts import attention4
+    p = Paged([10, 20], 2, 64)
+    rows, q, step = torch.zeros(2, 256, device=DEV, dtype=BF), torch.zeros(2, 256, device=DEV, dtype=BF), p.step([1, 1])
+    attention4.store(rows, step, p.view)
+    on_host = build_step([[0], [0]], [9, 19], p.slots, torch.device("cpu"), 1)
+    for call in (lambda s, v: attention4.store(rows, s, v), lambda s, v: attention4.attend(q, torch.empty_like(q), s, v, 4, 1.0)):
+        with pytest.raises(KernelError, match="GPU"):
+            call(on_host, p.view)
+        for other in (dict(k_pages=p.view.k_pages.cpu()), dict(v_pages=p.view.v_pages.cpu()), dict(page_table=p.view.page_table.cpu()),
+                      dict(k_pages=p.view.k_pages.float()), dict(v_pages=p.view.v_pages[:, :1].contiguous()), dict(head_dim=128),
+                      dict(page_table=p.view.page_table.long()), dict(k_pages=p.view.k_pages[:, :, ::2]), dict(v_pages=p.view.v_pages[:1])):
+            with pytest.raises(KernelError):
+                call(step, dataclasses.replace(p.view, four=None, **other))

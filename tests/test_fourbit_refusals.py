@@ -2,7 +2,12 @@
 import pytest
 import torch
 
-from hos_b200.errors import SpecError
+from hos_b200 import ops
+from hos_b200.cache import CacheManager
+from hos_b200.engine.batch import build_step
+from hos_b200.errors import KernelError, SpecError
+from hos_b200.parts import attention4
+from hos_b200.parts.base import KVNeed
 from hos_b200.parts.weights4 import Weight4
 
 
@@ -25,3 +30,12 @@ def test_groups_that_no_kernel_takes_are_refused(group):
         Weight4.from_matrix(torch.ones(32, 128), group)
     with pytest.raises(SpecError, match="groups"):
         Weight4.from_codes(torch.zeros(32, 128, dtype=torch.uint8), torch.ones(32, 2), None, group)
+
+
+def test_pages_and_steps_that_are_not_on_the_gpu_are_refused():
+    cpu = torch.device("cpu")
+    cache = CacheManager([KVNeed(2, 64, None, bits=4)], [None], [[]], 256, 256, torch.float32, cpu)
+    with pytest.raises(KernelError, match="GPU"):
+        ops.paged4(cache.stores[0].kv)
+    with pytest.raises(KernelError, match="GPU"):
+        attention4._check_step(1, build_step([[0]], [1], [0], cpu, 1), "attend")
