@@ -66,6 +66,7 @@ class KVGroup:
         self._slot_pages: Dict[int, List[int]] = {}
         self._holders: Dict[int, int] = {}             # pages that several slots hold -> how many
         self._dirty: set = set()
+        self._views: Dict[int, ops.PagedKVArgs] = {}
         self._arrays: Optional[torch.Tensor] = None    # what ops.copy_pages wants of the arrays, made at the first copy
 
     def chunk_room(self):
@@ -154,9 +155,10 @@ class KVGroup:
         """Move the held pages to the front of the arrays; the number of them."""
         n = self.pages.n_held
         olds = sorted(p for p in self.pages.held() if p >= n)
-        news = self.pages.move_down(olds)
         if olds:
+            news = self.pages.lowest_free(len(olds))
             self._copy_listed(olds, news)
+            self.pages.exchange(olds, news)
             to = dict(zip(olds, news))
             self._holders = {to.get(p, p): k for p, k in self._holders.items()}
             for slot, held in self._slot_pages.items():
@@ -166,18 +168,22 @@ class KVGroup:
                     self._dirty.add(slot)
         return n
 
-    def resize(self, n_pages: int) -> None:
-        """Arrays of n_pages pages with what the held pages hold (they must fit); the old arrays' memory goes back."""
-        if self.compact() > n_pages:
-            raise CacheError(f"{self.pages.n_held} pages are held: they do not fit into {n_pages}")
-        keep = min(n_pages, self.pages.n)
-        for arrays in (self.k, self.v):
-            for i, old in enumerate(arrays):
-                if old is not None:
-                    arrays[i] = new = torch.zeros((n_pages,) + tuple(old.shape[1:]), dtype=old.dtype, device=old.device)
-                    new[:keep].copy_(old[:keep])
-        self.pages.resize(n_pages)
+    def new_arrays(self, n_pages: int) -> None:
+        """Arrays of n_pages pages in the place of the old ones, one after another, with what the pages of both sizes hold; the held pages
+        must be among those, and no other may be taken while this runs.  Each old array's memory goes back before the next is made.  If there is
+        no room for one of them, the arrays made so far stay: each of them holds the pages that both sizes have."""
         self._arrays = None
+        for arrays, name in ((self.k, "k_pages"), (self.v, "v_pages")):
+            for i in range(self.n_entries):
+                if arrays[i] is None:
+                    continue
+                new = torch.zeros((n_pages,) + tuple(arrays[i].shape[1:]), dtype=arrays[i].dtype, device=arrays[i].device)
+                keep = min(n_pages, arrays[i].shape[0])
+                new[:keep].copy_(arrays[i][:keep])
+                arrays[i] = new
+                if i in self._views:
+                    setattr(self._views[i], name, new)
+                    self._views[i].four = None
 
     def copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Page src[i] to page dst[i] (int32, on the cache's device) in the arrays of all entries, in one launch; pairs with a page
@@ -215,8 +221,11 @@ class KVGroup:
             at = end
 
     def view(self, entry: int) -> ops.PagedKVArgs:
-        return ops.PagedKVArgs(self.k[entry], self.v[entry], self.table_dev, self.ring_pages,
-                               self.need.n_kv_heads, self.need.head_dim, self.need.v_head_dim or 0, self.need.bits)
+        """What the kernels take of an entry: one object an entry, which always names the arrays that there are."""
+        if entry not in self._views:
+            self._views[entry] = ops.PagedKVArgs(self.k[entry], self.v[entry], self.table_dev, self.ring_pages,
+                                                 self.need.n_kv_heads, self.need.head_dim, self.need.v_head_dim or 0, self.need.bits)
+        return self._views[entry]
 
     def bytes_per_token(self) -> int:
         if self.need.bits is not None:

@@ -75,11 +75,9 @@ class CacheManager:
                 placed[e] = (len(self.groups), j)
             self.groups.append(g)
         self.stores: List[CallStore] = []
-        self._placed: List[Optional[Tuple[int, int]]] = []      # entry -> (group, index in group) of what it reads
         for i, need in enumerate(kv_needs):
             src = cache_from[i]
             kv, owns = None, True
-            self._placed.append(None)
             if need is not None:
                 owner = i if src is None else src
                 if owner not in placed:
@@ -89,7 +87,6 @@ class CacheManager:
                     raise CacheError(f"entry {i} reads the cache of entry {src}, whose keys have "
                                      f"another shape or window")
                 kv, owns = self.groups[gi].view(j), src is None
-                self._placed[-1] = (gi, j)
             state = {s.name: torch.zeros((self.n_slots,) + tuple(s.shape), dtype=s.dtype,
                                          device=self.device) for s in state_needs[i]}
             self.stores.append(CallStore(kv, owns, state))
@@ -219,20 +216,24 @@ class CacheManager:
     def resize(self, max_tokens: int) -> None:
         """Pages for max_tokens tokens from now on (see the class): a smaller cache gives memory back, a larger one takes more.  The
         sequences held must fit; slots, and the longest sequence that the page tables have room for, stay as they were made.  The
-        arrays are new ones: graphs captured before must not be replayed."""
+        arrays are new ones: graphs captured before must not be replayed.  Besides the arrays one of them is held twice at a time.  If there is no
+        memory for one, the error comes with the sequences as they were, in a cache of the smaller of both sizes."""
         if max_tokens <= 0:
             raise CacheError("the cache must hold at least one token")
         n_pages = (max_tokens + PAGE - 1) // PAGE
         for g in self.groups:
             if g.pages.n_held > n_pages:
                 raise CacheError(f"{g.pages.n_held} pages are held: they do not fit into {n_pages}")
-        self.n_pages = n_pages
+        both = min(n_pages, self.n_pages)
+        for g in self.groups:                # while arrays of both sizes may stand side by side: the pages that all of them have
+            g.compact()
+            g.pages.resize(both)
+        self.n_pages = both
         for g in self.groups:
-            g.resize(n_pages)
-        for store, place in zip(self.stores, self._placed):
-            if place is not None:
-                view = self.groups[place[0]].view(place[1])
-                store.kv.k_pages, store.kv.v_pages, store.kv.four = view.k_pages, view.v_pages, None
+            g.new_arrays(n_pages)
+        for g in self.groups:
+            g.pages.resize(n_pages)
+        self.n_pages = n_pages
 
     def release(self, slot: int) -> None:
         if slot not in self.lengths:

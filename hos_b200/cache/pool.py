@@ -52,14 +52,15 @@ class IdPool:
                 hi = mid
         self._free.insert(lo, i)
 
-    def move_down(self, ids: List[int]) -> List[int]:
-        """Hold the lowest free ids in the place of these held ones; the new ids, in the same order."""
-        new = [self._free.pop() for _ in ids]
-        for i in ids:
-            self._held.remove(i)
+    def lowest_free(self, n: int) -> List[int]:
+        """The n lowest free ids, which stay free."""
+        return self._free[len(self._free) - n:][::-1]
+
+    def exchange(self, ids: List[int], new: List[int]) -> None:
+        """Hold these free ids in the place of these held ones."""
+        self._held.difference_update(ids)
         self._held.update(new)
         self._free = sorted(set(range(self.n)) - self._held, reverse=True)
-        return new
 
     def resize(self, n: int) -> None:
         """Ids 0..n-1 from now on; none of the held ones may be n or above."""
