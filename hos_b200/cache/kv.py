@@ -67,7 +67,11 @@ class KVGroup:
         self._holders: Dict[int, int] = {}             # pages that several slots hold -> how many
         self._dirty: set = set()
         self._views: Dict[int, ops.PagedKVArgs] = {}
-        self._arrays: Optional[torch.Tensor] = None    # what ops.copy_pages wants of the arrays, made at the first copy
+        # what ops.copy_pages wants of the arrays (the keys', then the values'): address and bytes of a page
+        arrays = self.k + [v for v in self.v if v is not None]
+        page = [a[0].numel() * a.element_size() for a in arrays]
+        self._most_bytes = max(page)
+        self._arrays = torch.tensor([[a.data_ptr(), b] for a, b in zip(arrays, page)], dtype=torch.int64).to(device)
 
     def chunk_room(self):
         """The most tokens a sequence may bring in one step that attends over this group's
@@ -172,8 +176,7 @@ class KVGroup:
         """Arrays of n_pages pages in the place of the old ones, one after another, with what the pages of both sizes hold; the held pages
         must be among those, and no other may be taken while this runs.  Each old array's memory goes back before the next is made.  If there is
         no room for one of them, the arrays made so far stay: each of them holds the pages that both sizes have."""
-        self._arrays = None
-        for arrays, name in ((self.k, "k_pages"), (self.v, "v_pages")):
+        for arrays, name, first in ((self.k, "k_pages", 0), (self.v, "v_pages", self.n_entries)):
             for i in range(self.n_entries):
                 if arrays[i] is None:
                     continue
@@ -181,6 +184,7 @@ class KVGroup:
                 keep = min(n_pages, arrays[i].shape[0])
                 new[:keep].copy_(arrays[i][:keep])
                 arrays[i] = new
+                self._arrays[first + i, 0].fill_(new.data_ptr())
                 if i in self._views:
                     setattr(self._views[i], name, new)
                     self._views[i].four = None
@@ -188,11 +192,7 @@ class KVGroup:
     def copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Page src[i] to page dst[i] (int32, on the cache's device) in the arrays of all entries, in one launch; pairs with a page
         outside the arrays copy nothing.  No page may be written twice, or read and written, in one call."""
-        arrays = self.k + [v for v in self.v if v is not None]
-        if self._arrays is None:
-            page = [a[0].numel() * a.element_size() for a in arrays]
-            self._arrays = torch.tensor([[a.data_ptr(), b] for a, b in zip(arrays, page)], dtype=torch.int64).to(arrays[0].device), max(page)
-        ops.copy_pages(self._arrays[0], self._arrays[1], src, dst, self.pages.n)
+        ops.copy_pages(self._arrays, self._most_bytes, src, dst, self.pages.n)
 
     def _copy_listed(self, src: Sequence[int], dst: Sequence[int]) -> None:
         if self.table_dev.device.type != "cuda":            # the bookkeeping without a GPU

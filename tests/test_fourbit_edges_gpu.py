@@ -163,3 +163,28 @@ def test_views_and_steps_of_another_kind_are_refused():
                       dict(page_table=p.view.page_table.long()), dict(k_pages=p.view.k_pages[:, :, ::2]), dict(v_pages=p.view.v_pages[:1])):
             with pytest.raises(KernelError):
                 call(step, dataclasses.replace(p.view, four=None, **other))
+
+
+@pytest.mark.parametrize("keys_only", [False, True])
+def test_the_first_copy_of_a_cache_and_the_first_after_a_resize_upload_nothing(monkeypatch, keys_only):
+    from hos_b200.cache import CacheManager, kv
+    from hos_b200.parts.base import KVNeed
+    c = CacheManager([KVNeed(2, 64, None, keys_only)] * 3, [None] * 3, [[]] * 3, 20 * 64, 640, BF, torch.device(DEV))
+    g, pairs = c.groups[0], torch.tensor([[0, 3], [1, 7]], dtype=torch.int32, device=DEV)
+
+    def none(*a, **kw):
+        raise AssertionError("an upload")
+    for pages in (20, 10, 30):
+        if pages != 20:
+            c.resize(pages * 64)
+        arrays = [a for a in g.k + g.v if a is not None]
+        assert len(arrays) == (3 if keys_only else 6)
+        for a in arrays:
+            a.copy_(torch.randn(a.shape))
+        want = [a.clone() for a in arrays]
+        for a in want:
+            a[[1, 7]] = a[[0, 3]]
+        with monkeypatch.context() as m:
+            m.setattr(kv.torch, "tensor", none)
+            g.copy_pages(pairs[0], pairs[1])
+        assert all(torch.equal(a, b) for a, b in zip(arrays, want))
