@@ -123,7 +123,12 @@ class KVGroup:
         if shared:
             olds = [held[e] for e in shared]
             news = [self.pages.take() for _ in shared]
-            self._copy_listed(olds, news)
+            try:
+                self._copy_listed(olds, news)
+            except Exception:
+                for page in news:
+                    self.pages.give_back(page)
+                raise
             for e, old, new in zip(shared, olds, news):
                 row[e] = held[e] = new
                 self._let_go(old)

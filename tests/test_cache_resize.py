@@ -77,3 +77,34 @@ def test_a_resize_takes_one_array_more_at_a_time():
     finally:
         kv.torch = before
     assert alive == [6, 5, 4, 3, 2, 1] and all(r() is None for r in old)
+
+
+@pytest.mark.parametrize("act", ["write", "compact"])
+def test_a_copy_that_fails_takes_no_page(monkeypatch, act):
+    c = make(max_tokens=512, window=None, max_seq_len=256)
+    g = c.groups[0]
+    gone, a = c.admit([0, 0])
+    c.extend(gone, 64)
+    c.extend(a, 100)
+    c.flush()
+    for page in g._slot_pages[a]:
+        g.k[0][page] = page + 1
+    b = c.fork(a)[0]
+    c.release(gone)
+    want = [float(g.k[0][p].max()) for p in g._slot_pages[a]]
+
+    def fails(src, dst):
+        raise RuntimeError("no pinned memory left")
+    run = (lambda: c.extend(b, 101)) if act == "write" else c.compact
+    with monkeypatch.context() as m:
+        m.setattr(g, "_copy_listed", fails)
+        with pytest.raises(RuntimeError, match="pinned"):
+            run()
+    c.check()
+    assert c.lengths[b] == 100 and g.pages.n_held == 2
+    for slot in (a, b):
+        assert [float(g.k[0][p].max()) for p in g._slot_pages[slot]] == want
+    run()
+    c.check()
+    for slot in (a, b):
+        assert [float(g.k[0][p].max()) for p in g._slot_pages[slot]] == want
