@@ -88,6 +88,21 @@ def shares(rows: int, kv_items: int, longest: int, window: Optional[int], fill: 
     return share, splits, few and fill > 0.8 and (splits == 2 or splits in (4, 8) and items * splits <= 256)
 
 
+MOST_PARTS = 64 << 20          # bytes of the shares' sums that wait for the merge
+
+
+def bounded_shares(n: int, rows: int, kv_items: int, n_heads: int, head_dim: int, longest: int, window: Optional[int], fill: float = 1.0):
+    """As `shares`, for n rows in `rows` walks, but shares that merge through the workspace are no more than MOST_PARTS holds (one, if not two):
+    rows in such numbers fill the GPU without (2,048 rows of 32 heads of 128 on 131,072 keys would be 64 shares and 2 GB)."""
+    share, splits, cluster = shares(rows, kv_items, longest, window, fill)
+    most = max(1, MOST_PARTS // (4 * n * n_heads * (head_dim + 2)))
+    if splits > most and not cluster:
+        pages = _pages(longest, window)
+        share = -(-pages // most)
+        splits = -(-pages // share)
+    return share, splits, cluster
+
+
 def attend(q: torch.Tensor, out: torch.Tensor, step, cache: ops.PagedKVArgs, n_heads: int, scale: float, softcap: float = 0.0,
            window: Optional[int] = None) -> None:
     """out[N, n_heads * head_dim] = softmax attention of the step's rows, each at its own position, over what the pages hold up to
@@ -106,11 +121,11 @@ def attend(q: torch.Tensor, out: torch.Tensor, step, cache: ops.PagedKVArgs, n_h
         if plan is not None:
             return _attend_tiles(q, out, step, cache, n_heads, scale, softcap, window, plan)
     together = 1 if step.single_token else max(1, 8 // (n_heads // kv))      # rows of a sequence that share a walk
-    key = ("shares of 4-bit pages", n, items, together, window, step.row_offset)
+    key = ("shares of 4-bit pages", n, items, together, n_heads, cache.head_dim, window, step.row_offset)
     plan = step.shared.get(key)                      # once per step and kind of layer
     if plan is None:
         walks = n if together == 1 else -(-n // together)
-        plan = step.shared[key] = shares(walks, items, step.max_len_after, window, step.fill_for(window))
+        plan = step.shared[key] = bounded_shares(n, walks, items, n_heads, cache.head_dim, step.max_len_after, window, step.fill_for(window))
     share, splits, cluster = plan
     parts = None
     if splits > 1 and not cluster:

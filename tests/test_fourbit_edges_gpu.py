@@ -8,7 +8,7 @@ import math
 import pytest
 import torch
 
-from test_fourbit_gpu import Paged, gen, made_weights
+from test_fourbit_gpu import Paged, check_attention, gen, made_weights
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -188,3 +188,11 @@ def test_the_first_copy_of_a_cache_and_the_first_after_a_resize_upload_nothing(m
             m.setattr(kv.torch, "tensor", none)
             g.copy_pages(pairs[0], pairs[1])
         assert all(torch.equal(a, b) for a, b in zip(arrays, want))
+
+
+@pytest.mark.parametrize("most", [1, 40000, 1 << 30])
+def test_shares_within_the_workspace_give_the_same(monkeypatch, most):
+    from hos_b200.parts import attention4
+    monkeypatch.setattr(attention4, "MOST_PARTS", most)
+    check_attention([3000, 2500, 100], [9, 1, 1], 8, 4, 64, dtype=F32)
+    check_attention([5000] * 3, [1] * 3, 4, 4, 128, window=3000)
