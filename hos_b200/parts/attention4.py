@@ -115,6 +115,8 @@ def attend(q: torch.Tensor, out: torch.Tensor, step, cache: ops.PagedKVArgs, n_h
         raise KernelError(f"queries {tuple(q.shape)} and output {tuple(out.shape)} for {n_heads} heads of {cache.head_dim}")
     _check_step(n, step, "attend")
     kv = cache.n_kv_heads
+    if n_heads <= 0 or n_heads % kv:
+        raise KernelError(f"attend: {n_heads} query heads over {kv} kv heads")
     items = kv * -(-(n_heads // kv) // 8)
     if _tiles_take(q, out, step, n_heads // kv):
         plan = _tile_plan(n, step, cache, n_heads // kv, items, window)

@@ -196,3 +196,14 @@ def test_shares_within_the_workspace_give_the_same(monkeypatch, most):
     monkeypatch.setattr(attention4, "MOST_PARTS", most)
     check_attention([3000, 2500, 100], [9, 1, 1], 8, 4, 64, dtype=F32)
     check_attention([5000] * 3, [1] * 3, 4, 4, 128, window=3000)
+
+
+@pytest.mark.parametrize("new", [1, 3])
+@pytest.mark.parametrize("heads", [1, 3, 0])
+def test_heads_that_are_no_multiple_of_the_kv_heads_are_refused(heads, new):
+    from hos_b200.errors import KernelError
+    from hos_b200.parts import attention4
+    p = Paged([10, 20], 2, 64)
+    q = torch.zeros(2 * new, heads * 64, device=DEV, dtype=BF)
+    with pytest.raises(KernelError, match="heads"):
+        attention4.attend(q, torch.empty_like(q), p.step([new, new]), p.view, heads, 1.0)
