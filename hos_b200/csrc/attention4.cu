@@ -10,8 +10,9 @@
 namespace hos {
 
 // ---- rows into pages ---------------------------------------------------------------------------------------------------
-// Four lanes hold 64 numbers of a row, 16 each.  Many rows are bound by reading them and writing what is held, and near that by the
-// dozen instructions a number costs (B200: 8,192 rows of 16 kv heads of 128, 67 MB read and as many handed back, 49 us; 8 rows 3.2).
+// Four lanes hold 64 numbers of a row, 16 each.  Many rows are bound by instructions, 35 a number (the row's two sums with NaN kept in sight, a
+// quotient that is IEEE's, two codes to a byte by column): they are issued in 73% of the clocks, memory runs at a quarter of its rate (B200:
+// 8,192 rows of 16 kv heads of 128, 67 MB read and as many handed back, 49 us; 8 rows 3.2).
 struct Numbers { float v[16]; };
 __device__ __forceinline__ Numbers load16(const float* p, bool vec) {
     Numbers x;
@@ -214,14 +215,16 @@ store4_many_kernel(const T* rows, long long stride, T* held, long long held_stri
 }
 
 // ---- attention of single rows --------------------------------------------------------------------------------------
-// Bound by reading the held keys and values once, and close behind by the instructions that make operands of codes.
+// No unit is full (8 rows over 8,192 keys: reads at 29% of their rate, ALU 41%, mma.sync 14%, an instruction issued in 48% of the clocks, 850 for
+// 16 keys of a kv head of 256): 14 warps an SM, which wait for their own results and, at the merge, for one another.  An infinity in a query
+// gives NaN, as without a soft-cap the definition does.
 //
 // Scores: S^T = K Q^T with 16 keys as the MMA's rows and up to 8 query heads of a kv head as its columns (fewer heads: of several
 // neighbouring rows of a sequence, each with its own mask).  The score of a key is
 // sum_g (s_g (sum_{d in g} q c') - 136 s_g sum q + m_g sum q) over its groups of 64, c' = 128 + c + 8 the operand as codes_to_bf16 makes
 // it without subtracting: a group's product starts at -136 sum q and is multiplied by the key's scale, in 32 bits; neither scale nor
 // middle is rounded into an operand.  Values: O^T = V^T P^T with 16 numbers of a head as rows, P times the value's scale in half
-// precision (attention4.cuh; in bfloat16, 2^-9 of a weight, long rows whose output is a small mean lost as much as the result's own
+// precision (attention4.cuh; in bfloat16, 2^-8 of a weight, long rows whose output is a small mean lost as much as the result's own
 // rounding), the codes exact, and the middles' sum, one number a group and head, in 32 bits beside it.  The scores' registers,
 // transposed eight by eight, are P's operand.
 // Rows in 32 bits: q, and p times the scale, are three bfloat16 numbers each, exactly, and the codes are subtracted first.

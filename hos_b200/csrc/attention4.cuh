@@ -69,7 +69,7 @@ __device__ __forceinline__ void mma_plain(float (&d)[4], const uint32_t (&a)[4],
 
 // The same of half precision, and what the products of weights and values take: codes -8..7 (a register's bits lie where 1024 + c or 1024 + 16 c
 // is made of them at once) and weights, which are at most 2^8, times the values' scales, brought below 2^7 by a power of two of a
-// group's and walk's own (`into`, raised when a scale passes it): rounded to 2^-12 of themselves down to 2^-20 of the largest.
+// group's and walk's own (`into`, raised when a scale passes it): rounded to 2^-11 of themselves down to 2^-20 of the largest.
 __device__ __forceinline__ void mma_half(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])

@@ -13,7 +13,7 @@
 // Few tiles share K as a cluster, whose sums meet in shared memory.
 // Bound by the products where rows fill the tile (2 clocks a row and stage), else by forming the weights: plan_tiles below chooses rows
 // a tile and CTAs a cluster by these.
-// Measured (B200, 14336 x 3584 gated, groups of 128 with zero codes): 64 rows 34 us, 512 rows 100 us (1.05 PFLOP/s), 2,048 rows 355 us (1.19).
+// Measured (B200, 14336 x 3584 gated, groups of 128 with zero codes): 64 rows 34 us, 512 rows 103 us (1.02 PFLOP/s), 2,048 rows 369 us (1.14).
 #include "common.cuh"
 #include "fourbit.cuh"
 #include "mma_utils.cuh"

@@ -1,6 +1,7 @@
 """A matrix held in 4 bits: codes 0..15, a scale (bfloat16) and, if it has them, a zero code per `group` neighbouring weights of a
 row; W[n, k] = (code - zero) * scale, zero 8 where there are none.  Products with it go through `linear.matmul` like those with any
-other matrix, with rows in bfloat16 or in 32 bits.
+other matrix, with rows in bfloat16 or in 32 bits.  Up to 32 rows, and for rows in 32 bits, no weight is rounded; for more bfloat16 rows a
+weight is rounded once to 11 bits, also where the result is asked for in 32 bits (csrc/weights4_tc.cu).
 
 `from_codes` takes what a quantised checkpoint holds, `from_matrix` rounds a matrix.  Both lay the codes out once, as the
 operand registers of the tensor cores want them (csrc/fourbit.cuh)."""
@@ -17,7 +18,7 @@ from ..errors import KernelError, SpecError
 ROWS, COLS = 16, 64             # of a block of codes
 # Up to so many rows the codes are multiplied as they are, above the weights are formed in half precision (us a product, that kernel's / the
 # tcgen05 one's: 2304 x 9216, 32 rows 12.8 / 19.3, 33 rows, one more tile of 32, 22.1 / 19.6; 9216 x 2304 gated, 16 rows 13.6 / 17.5, 32 rows
-# 20.9 / 18.5, 33 rows 35.9 / 19.1).  Gated products of many weights would gain from 17 rows on (14336 x 3584, 24 rows 42.2 / 32.2), but
+# 21.1 / 18.5, 33 rows 35.9 / 19.1).  Gated products of many weights would gain from 17 rows on (14336 x 3584, 24 rows 41.4 / 32.2), but
 # up to 32 rows, where most steps of a few sequences lie, no weight is rounded.
 FEW_ROWS = 32
 MOST_TC_K = 1 << 21
@@ -71,7 +72,8 @@ class Weight4:
 
     @classmethod
     def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor], group: int, blocks: int = 1) -> "Weight4":
-        """On the GPU, codes: uint8 [rows, k], 0..15; scales: [rows, ceil(k / group)], kept in bfloat16; zeros: uint8 like the scales, or None.
+        """On the GPU, codes: uint8 [rows, k], 0..15; scales: [rows, ceil(k / group)], kept in
+        bfloat16 (scales in another type are rounded to it, by up to 2^-8 of themselves); zeros: uint8 like the scales, or None.
         `blocks`: the rows are that many matrices one after another (2: gate and up of a gated feed-forward)."""
         _check_group(group)
         if codes.dim() != 2 or codes.dtype != torch.uint8:
