@@ -660,8 +660,8 @@ attend4_merge_kernel(T* __restrict__ out, long long out_stride, int n_heads, int
 
 template <typename T, int DIM, bool GROUPS>
 int launch_attend4(const void* q, long long q_stride, void* out, long long out_stride, const int* token_pos, const int* token_seq, const int* seq_slot,
-                   const int* token_slot, const int* cu_seqlens, int row_base, int n_seqs, const Paged4& c, int n_tokens, int n_heads, float scale, float cap, int window, int share, int splits, float* part_o, float2* part_ml,
-                   cudaStream_t stream) {
+                   const int* token_slot, const int* cu_seqlens, int row_base, int n_seqs, const Paged4& c, int n_tokens, int n_heads, float scale,
+                   float cap, int window, int share, int splits, float* part_o, float2* part_ml, cudaStream_t stream) {
     constexpr int smem = Attend4<DIM>::kShared;
     auto kernel = attend4_kernel<T, DIM, GROUPS>;
     static bool set = false;                                   // once per kernel: the attribute stays
@@ -731,8 +731,8 @@ extern "C" int hos_store4(const void* rows, int dtype, long long stride, void* h
 // of `share` pages, a CTA each: `splits` of them cover the longest row's.  2 to 8 without `parts` are a cluster; else more than one need
 // `parts`, n_tokens * n_heads * splits * (head_dim + 2) 32-bit numbers.
 extern "C" int hos_attend4(const void* q, int dtype, long long q_stride, void* out, long long out_stride, const int* token_pos, const int* token_seq,
-                           const int* seq_slot, const int* token_slot, const int* cu_seqlens, int row_base, int n_seqs, const void* cache, int n_tokens, int n_heads, float scale, float cap, int window,
-                           int share, int splits, float* parts, cudaStream_t stream) {
+                           const int* seq_slot, const int* token_slot, const int* cu_seqlens, int row_base, int n_seqs, const void* cache, int n_tokens,
+                           int n_heads, float scale, float cap, int window, int share, int splits, float* parts, cudaStream_t stream) {
     if (n_tokens <= 0) return 0;
     HOS_CHECK_PAGED4("attend4");
     if (n_heads <= 0 || n_heads % n_kv_heads) HOS_REFUSE("attend4: %d query heads over %d kv heads", n_heads, n_kv_heads);
@@ -743,7 +743,10 @@ extern "C" int hos_attend4(const void* q, int dtype, long long q_stride, void* o
     float2* part_ml = (float2*)parts;                          // pairs first: they want 8 bytes' alignment
     float* part_o = parts == nullptr ? nullptr : parts + 2 * n_parts;
     const bool groups = cu_seqlens != nullptr && 2 * (n_heads / n_kv_heads) <= 8;
-#define HOS_A4(T, D) return (groups ? launch_attend4<T, D, true> : launch_attend4<T, D, false>)(q, q_stride, out, out_stride, token_pos, token_seq, seq_slot, token_slot, cu_seqlens, row_base, n_seqs, c, n_tokens, n_heads, scale, cap, window, share, splits, part_o, part_ml, stream)
+#define HOS_A4(T, D)                                                                                                                             \
+    return (groups ? launch_attend4<T, D, true> : launch_attend4<T, D, false>)(q, q_stride, out, out_stride, token_pos, token_seq, seq_slot,       \
+                                                                               token_slot, cu_seqlens, row_base, n_seqs, c, n_tokens, n_heads,     \
+                                                                               scale, cap, window, share, splits, part_o, part_ml, stream)
 #define HOS_A4_D(T) do { if (head_dim == 64) HOS_A4(T, 64); else if (head_dim == 128) HOS_A4(T, 128); else if (head_dim == 192) HOS_A4(T, 192); else HOS_A4(T, 256); } while (0)
     if (dtype == kF32) HOS_A4_D(float);
     else HOS_A4_D(bf16);
@@ -756,8 +759,17 @@ extern "C" int hos_attend4_merge(void* out, int dtype, long long out_stride, int
         HOS_REFUSE("attend4_merge: %d rows of %d heads in %d shares", n_tokens, n_heads, splits);
     const float2* part_ml = (const float2*)parts;
     const float* part_o = parts + 2 * (size_t)n_tokens * n_heads * splits;
-#define HOS_AM(T, D) launch_pdl(attend4_merge_kernel<T, D>, dim3((unsigned)((long long)n_tokens * n_heads)), dim3(merge_threads(D, splits)), 0, stream, (T*)out, out_stride, n_heads, splits, part_o, part_ml)
-#define HOS_AM_D(T) do { if (head_dim == 64) HOS_AM(T, 64); else if (head_dim == 128) HOS_AM(T, 128); else if (head_dim == 192) HOS_AM(T, 192); else if (head_dim == 256) HOS_AM(T, 256); else HOS_REFUSE("attend4_merge: head size %d", head_dim); } while (0)
+#define HOS_AM(T, D)                                                                                                                             \
+    launch_pdl(attend4_merge_kernel<T, D>, dim3((unsigned)((long long)n_tokens * n_heads)), dim3(merge_threads(D, splits)), 0, stream, (T*)out,    \
+               out_stride, n_heads, splits, part_o, part_ml)
+#define HOS_AM_D(T)                                                                                                                              \
+    do {                                                                                                                                         \
+        if (head_dim == 64) HOS_AM(T, 64);                                                                                                       \
+        else if (head_dim == 128) HOS_AM(T, 128);                                                                                                \
+        else if (head_dim == 192) HOS_AM(T, 192);                                                                                                \
+        else if (head_dim == 256) HOS_AM(T, 256);                                                                                                \
+        else HOS_REFUSE("attend4_merge: head size %d", head_dim);                                                                                \
+    } while (0)
     if (dtype == kF32) HOS_AM_D(float);
     else HOS_AM_D(bf16);
     return check_launch("attend4_merge");

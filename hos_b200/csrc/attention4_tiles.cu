@@ -383,7 +383,9 @@ extern "C" int hos_attend4_tiles(const void* q, long long q_stride, void* out, l
     const size_t n_parts = (size_t)n_tokens * n_heads * splits;
     float2* part_ml = (float2*)parts;
     float* part_o = parts == nullptr ? nullptr : parts + 2 * n_parts;
-#define HOS_AT(D) return launch_attend4_tiles<D>(q, q_stride, out, out_stride, token_pos, seq_slot, seq_base, cu_seqlens, row_base, n_seqs, c, n_tokens, n_heads, scale, cap, window, share, splits, part_o, part_ml, stream)
+#define HOS_AT(D)                                                                                                                                \
+    return launch_attend4_tiles<D>(q, q_stride, out, out_stride, token_pos, seq_slot, seq_base, cu_seqlens, row_base, n_seqs, c, n_tokens, n_heads, \
+                                   scale, cap, window, share, splits, part_o, part_ml, stream)
     if (head_dim == 64) HOS_AT(64);
     if (head_dim == 128) HOS_AT(128);
     if (head_dim == 192) HOS_AT(192);

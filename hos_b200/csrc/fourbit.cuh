@@ -59,6 +59,13 @@ constexpr uint32_t kZero8 = 0x43084308u;       // 128 + 8 twice
 __device__ __forceinline__ float bf16_lo(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
+// A matrix as the host hands it over (ops.Matrix4): N features (gated: of gate, and as many of up, gate's 16-row tiles first).
+struct Matrix4 {
+    const uint8_t *codes, *records, *records16;
+    const float* powers;                 // records16 and powers: for the products of many rows (weights4_tc.cu)
+    int n, k, group, zeros, gated;
+};
+
 // 16 bytes from global to shared memory without registers, `bytes` of them read and the rest zeros; groups of a thread's copies
 // end in order, and a warp that waits for its own and meets at __syncwarp() sees all of its lanes' copies.
 __device__ __forceinline__ void copy16_async(uint32_t smem, const void* gmem, int bytes = 16) {

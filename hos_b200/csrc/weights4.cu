@@ -389,13 +389,6 @@ using namespace hos;
 
 extern "C" const char* hos_last_error() { return error_buffer(); }
 
-// A matrix as the host hands it over (ops.Matrix4): N features (gated: of gate, and as many of up, gate's 16-row tiles first).
-struct Matrix4 {
-    const uint8_t *codes, *records, *records16;
-    const float* powers;                 // records16 and powers: for the products of many rows (weights4_tc.cu)
-    int n, k, group, zeros, gated;
-};
-
 // Rows of x are ldx numbers apart, rows of out ldo.
 extern "C" int hos_product4(const void* x, int x_dtype, long long ldx, const void* matrix, void* out, int out_dtype, long long ldo, int M, int act, float limit,
                             cudaStream_t stream) {

@@ -485,7 +485,6 @@ extern "C" int hos_product4_tc_set_error_word(void* word) {
 // on their way.  tile_rows 0: chosen here, with shares.
 extern "C" int hos_product4_tc(const void* x, long long ldx, const void* matrix, void* out, int out_dtype, long long ldo, int M, int act, float limit,
                                void* half_rows, float* row_powers, int tile_rows, int shares, long long wait_cycles, int stop_stage, cudaStream_t stream) {
-    struct Matrix4 { const uint8_t *codes, *records, *records16; const float* powers; int n, k, group, zeros, gated; };
     const Matrix4 w = *(const Matrix4*)matrix;
     if (M <= 0 || w.n <= 0) return 0;
     if (w.k < 64 || half_rows == nullptr || row_powers == nullptr || (uintptr_t)half_rows % 16) HOS_REFUSE("product4_tc: K %d (64 at least), or no place for the rows", w.k);

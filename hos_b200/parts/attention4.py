@@ -63,8 +63,8 @@ def _pages(longest: int, window: Optional[int], new: int = 0) -> int:
 def shares(rows: int, kv_items: int, longest: int, window: Optional[int], fill: float = 1.0):
     """(pages of a share, shares of a row, whether the shares are a cluster): `rows` rows times `kv_items` (kv heads, times the eights of
     query heads that share one) over up to `longest` keys.  Two CTAs fit an SM: rows that leave CTAs free are cut into as many shares
-    as fill them, of 2 pages at least (8 rows, 8 heads of 256 over 4, 500 keys: 8 shares of a page 10.6 us, 4 of two 9.0); many rows of unequal lengths (`fill`: the sum of the keys over rows * the longest) into shares of up to 32 pages,
-    which CTAs take as they come free.  2, 4 or 8 shares of few rows of like lengths merge as a cluster (16 rows, 8 heads of 256 over 4,
+    as fill them, of 2 pages at least (8 rows, 8 heads of 256 over 4, 500 keys: 8 shares of a page 10.6 us, 4 of two 9.0); many rows of
+    unequal lengths (`fill`: the sum of the keys over rows * the longest) into shares of up to 32 pages, which CTAs take as they come free.  2, 4 or 8 shares of few rows of like lengths merge as a cluster (16 rows, 8 heads of 256 over 4,
     2,000 keys, 4 shares: 20.0 us, through the workspace 22.5), not 3 or 6, whose clusters leave places of their neighbourhood of SMs
     empty and run in two rounds (12 rows, 6 shares 28.9 us, through the workspace 20.4), nor, for the same reason, 4 or 8 in more than
     256 CTAs (36 rows, 16 heads of 64 over 2, 4 shares 35.4 and 25.0), nor of unlike lengths, where CTAs without keys would wait for the
