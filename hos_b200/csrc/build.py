@@ -15,6 +15,8 @@ Libraries and what needs them:
               per-slot record
   attn_hdN    bfloat16 models with head_dim N: tensor-core attention for prompts
               and for decoding over the paged cache
+  shared_hdN  bfloat16 models with head_dim N whose sequences share pages: attention over a
+              shared prefix
   gemm_tc     bfloat16 models: the tcgen05/TMA matrix product
   gemm_skinny bfloat16 models: the matrix product for up to 16 rows (decoding)
   rows        the hashed token-pair embedding, the parallel block's add-and-norms, the norm
@@ -28,6 +30,7 @@ Libraries and what needs them:
               delta rule and short convolutions) or per key channel, hyper-connections
   fourbit     products with 4-bit weights, keys and values in 4-bit pages and attention over them,
               copies of pages (a forked sequence, a compacted cache)
+  scores      log probabilities of tokens, the entropy and the likeliest tokens, from logits
 A model builds only the libraries whose parts it has.
 """
 from __future__ import annotations
@@ -60,6 +63,7 @@ _STATIC_LIBS: Dict[str, Tuple[List[str], List[str]]] = {
     "blocks": (["latent_attention.cu", "latent_prompt.cu", "wkv.cu"], []),
     "gated_attn": (["gated_attention.cu", "gated_attention_mma.cu"], []),
     "mixers": (["postnorm.cu", "state_scan.cu", "hyper.cu"], []),
+    "scores": (["log_probs.cu"], []),
     "fourbit": (["weights4.cu", "weights4_tc.cu", "attention4.cu", "attention4_tiles.cu", "pages.cu"], []),
 }
 
@@ -73,6 +77,8 @@ def library_spec(name: str) -> Tuple[List[str], List[str]]:
     if name.startswith("attn_hd"):
         hd = int(name[len("attn_hd"):])
         return ["attention_decode.cu", "attention_prefill.cu", "attention_prefill_tc.cu"], [f"-DHOS_HEAD_DIM={hd}"]
+    if name.startswith("shared_hd"):
+        return ["attention_shared.cu"], [f"-DHOS_HEAD_DIM={int(name[len('shared_hd'):])}"]
     raise ExtensionMissingError(f"no CUDA library named {name!r}")
 
 
@@ -195,8 +201,8 @@ def load(name: str) -> ctypes.CDLL:
 
 
 def build_all(head_dims: Sequence[int] = (16, 32, 48, 64, 80, 128, 256)) -> List[str]:
-    """Build every library (the attention library once per head size: the sizes of the Gemma-2 checkpoints, 128
+    """Build every library (the attention libraries once per head size: the sizes of the Gemma-2 checkpoints, 128
     and 256, and the ones that the tests' small configurations have; any other multiple of 16 is built when a
     model with it is first loaded)."""
-    names = list(_STATIC_LIBS) + [f"attn_hd{h}" for h in head_dims]
+    names = list(_STATIC_LIBS) + [f"{lib}{h}" for lib in ("attn_hd", "shared_hd") for h in head_dims]
     return [library_path(n) for n in names]

@@ -169,10 +169,10 @@ _launch_ahead = False
 
 _ERROR_WORD_SETTERS = ("hos_gemm_tc_set_error_word", "hos_attn_decode_set_error_word",
                        "hos_attn_prefill_tc_set_error_word", "hos_latent_prompt_set_error_word", "hos_moe_grouped_set_error_word",
-                       "hos_product4_tc_set_error_word")
+                       "hos_product4_tc_set_error_word", "hos_attn_shared_set_error_word")
 GIVE_UP_CODES = {1: "the tcgen05 matrix product", 2: "the decode attention", 3: "the tcgen05 prompt attention",
                  4: "the tcgen05 prompt attention over latent rows", 5: "the tcgen05 products of the routed experts",
-                 6: "the tcgen05 product with 4-bit weights"}
+                 6: "the tcgen05 product with 4-bit weights", 7: "the attention over shared pages"}
 _error_word_tensor: Optional[torch.Tensor] = None
 _after_give_up = []        # callables that put shared scratch state right after a kernel gave up
 
@@ -513,6 +513,69 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, out: torch.Tensor, temp
     core().call("hos_sample", _ptr(logits), v, b, v, _ptr(uniforms), _ptr(recent),
                 recent.shape[1] if recent is not None else 0, _ptr(recent_len), float(temp),
                 int(top_k), float(top_p), float(rep_penalty), _ptr(out), _stream())
+
+
+# ---- log probabilities (csrc/log_probs.cu) -------------------------------------------------
+LOG_PROBS_MAX_TOP = 32
+_scores: Optional[Library] = None
+
+
+def scores() -> Library:
+    """Log probabilities, entropy and alternatives from logits."""
+    global _scores
+    if _scores is None:
+        _scores = Library("scores")
+    return _scores
+
+
+def _check_here(t: torch.Tensor, what: str) -> None:
+    """On the device that kernels are launched on (the current one, which stays the same one: see _stream)."""
+    if not t.is_cuda:
+        raise KernelError(f"{what} must be on the GPU")
+    here = torch.cuda.current_device() if _device_index is None else _device_index
+    if t.device.index != here or torch.cuda.current_device() != here:
+        raise KernelError(f"{what} must be on the current device, which is the one of the first launch (cuda:{here}), found {t.device}")
+
+
+def log_probs_blocks(rows: int, vocab: int) -> tuple:
+    """(threads of a block, blocks that share a row)."""
+    if rows * 8 <= sm_count() and vocab > 8192:
+        return 1024, 8
+    blocks = 1
+    while blocks < 8 and rows * blocks < 4 * sm_count() and vocab > 8192 * blocks:
+        blocks *= 2
+    return 256, blocks
+
+
+def log_probs(logits: torch.Tensor, tokens: torch.Tensor, logprob: torch.Tensor, entropy: torch.Tensor,
+              top_ids: Optional[torch.Tensor] = None, top_logprobs: Optional[torch.Tensor] = None) -> None:
+    """Of row b: logprob[b] = logits[b, tokens[b]] - log sum exp, entropy[b], and the likeliest top_ids.shape[1] tokens with their log
+    probabilities (see sampling.log_probs)."""
+    _check_here(logits, "logits")
+    _check_rows(logits, "logits", torch.float32)
+    b, v = logits.shape
+    _check(tokens, "tokens", torch.int32, 1)
+    _check(logprob, "log probabilities", torch.float32, 1)
+    _check(entropy, "entropies", torch.float32, 1)
+    if tokens.shape[0] != b or logprob.shape[0] != b or entropy.shape[0] != b:
+        raise KernelError(f"log_probs: {b} rows of logits for {tokens.shape[0]} tokens, {logprob.shape[0]} and {entropy.shape[0]} scores")
+    top = 0
+    if top_ids is not None:
+        _check(top_ids, "likeliest tokens", torch.int32, 2)
+        _check(top_logprobs, "their log probabilities", torch.float32, 2)
+        top = top_ids.shape[1]
+        if top_ids.shape != top_logprobs.shape or top_ids.shape[0] != b:
+            raise KernelError(f"log_probs: {b} rows with likeliest tokens {tuple(top_ids.shape)} and log probabilities {tuple(top_logprobs.shape)}")
+        if top > min(LOG_PROBS_MAX_TOP, v):
+            raise KernelError(f"log_probs: {top} alternatives of {v} tokens (at most {LOG_PROBS_MAX_TOP})")
+    if b == 0:
+        return
+    if v == 0:
+        raise KernelError("log_probs: a vocabulary without tokens")
+    threads, blocks = log_probs_blocks(b, v)
+    scores().call("hos_log_probs", logits.data_ptr(), logits.stride(0) if b > 1 else v, b, v, tokens.data_ptr(), logprob.data_ptr(),
+                  entropy.data_ptr(), top, top_ids.data_ptr() if top else None, top_logprobs.data_ptr() if top else None, threads, blocks,
+                  _stream())
 
 
 # ---- the per-slot record (csrc/slot_state.cu) ----------------------------------------------

@@ -1,0 +1,42 @@
+"""How likely tokens are: log probabilities of given tokens, the entropy of the distribution they come from, and the likeliest
+tokens beside them (csrc/log_probs.cu).
+
+The distribution is the softmax of the logits as they are: temperature, top-k, top-p and the repetition penalty are the sampler's
+business.  All of it is float32."""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+
+from .. import ops
+
+MAX_TOP = ops.LOG_PROBS_MAX_TOP
+
+
+class TokenScores(NamedTuple):
+    """Per row: the log probability of the row's token (natural logarithm), the entropy (nats) and, if asked for, the likeliest
+    tokens, the most likely first and of equal ones the lower token first, with their log probabilities."""
+    logprob: torch.Tensor                            # float32 [rows]
+    entropy: torch.Tensor                            # float32 [rows]
+    top_ids: Optional[torch.Tensor] = None           # int32 [rows, top]
+    top_logprobs: Optional[torch.Tensor] = None      # float32 [rows, top]
+
+    @staticmethod
+    def empty(rows: int, top: int, device) -> "TokenScores":
+        both = torch.empty((2, rows), dtype=torch.float32, device=device)
+        if not top:
+            return TokenScores(both[0], both[1])
+        return TokenScores(both[0], both[1], torch.empty((rows, top), dtype=torch.int32, device=device),
+                           torch.empty((rows, top), dtype=torch.float32, device=device))
+
+
+def log_probs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, out: Optional[TokenScores] = None) -> TokenScores:
+    """Scores of tokens[i] under row i of the logits (float32 [rows, vocab], rows any number of numbers apart; int32 [rows]), with
+    the `top` likeliest tokens beside it (0 to 32).  A token outside the vocabulary marks a padding row: zeros, ids -1.
+    -inf rules a token out; a row that holds nothing else, +inf or a number that is none has no distribution, and its scores are no
+    numbers.  Among the likeliest a number that is none counts as -inf.  `out`: scores of the same sizes to write into."""
+    if out is None:
+        out = TokenScores.empty(logits.shape[0] if logits.dim() else 0, top, logits.device)
+    ops.log_probs(logits, tokens, out.logprob, out.entropy, out.top_ids if top else None, out.top_logprobs if top else None)
+    return out
