@@ -23,6 +23,7 @@ from __future__ import annotations
 
 from typing import Dict, List, Optional, Sequence
 
+import numpy as np
 import torch
 
 from .. import ops
@@ -31,6 +32,25 @@ from ..parts.base import KVNeed
 from .pool import IdPool
 
 PAGE = ops.PAGE_TOKENS
+
+
+def _best_runs(table: np.ndarray, members: List[int]) -> tuple:
+    """(pages saved, [(members, pages)]): rows of page numbers as a tree of common beginnings; a branch is one run as far as all of
+    it agrees, or what its branches save by themselves if that is more."""
+    m, n = table.shape
+    agree = (table == table[0]).all(axis=0)
+    common = n if agree.all() else int(np.argmin(agree))
+    whole = ((m - 1) * common, [(members, common)] if common else [])
+    if m <= 2 or common == n:
+        return whole
+    saved, runs = 0, []
+    pages, which = np.unique(table[:, common], return_inverse=True)
+    for b in range(len(pages)):
+        rows = np.flatnonzero(which == b)
+        if len(rows) > 1:
+            s, r = _best_runs(table[rows], [members[i] for i in rows])
+            saved, runs = saved + s, runs + r
+    return whole if whole[0] >= saved else (saved, runs)
 
 
 class KVGroup:
@@ -65,6 +85,7 @@ class KVGroup:
         self.table_dev = torch.zeros((n_slots, self.table_stride), dtype=torch.int32, device=device)
         self._slot_pages: Dict[int, List[int]] = {}
         self._holders: Dict[int, int] = {}             # pages that several slots hold -> how many
+        self.version = 0                               # moves on whenever a slot's pages change
         self._dirty: set = set()
         self._views: Dict[int, ops.PagedKVArgs] = {}
         # what ops.copy_pages wants of the arrays (the keys', then the values'): address and bytes of a page
@@ -88,6 +109,7 @@ class KVGroup:
         if slot in self._slot_pages:
             raise CacheError(f"slot {slot} is opened twice")
         self._slot_pages[slot] = []
+        self.version += 1
 
     def shared_before(self, slot: int, old_len: int, new_len: int) -> List[int]:
         """Table entries of the slot that positions old_len..new_len-1 are written to and whose pages others hold too."""
@@ -133,13 +155,16 @@ class KVGroup:
                 row[e] = held[e] = new
                 self._let_go(old)
             self._dirty.add(slot)
+            self.version += 1
         while len(held) < want:
             page = self.pages.take()
+            self.version += 1
             row[len(held)] = page
             held.append(page)
             self._dirty.add(slot)
 
     def close_slot(self, slot: int) -> None:
+        self.version += 1
         for page in self._slot_pages.pop(slot):
             self._let_go(page)
 
@@ -159,6 +184,52 @@ class KVGroup:
         self._slot_pages[new_slot] = list(pages)
         self._table_np[new_slot, :len(pages)] = pages
         self._dirty.add(new_slot)
+        self.version += 1
+
+    def shared_runs(self, slots: Sequence[int], lengths: Sequence[int]) -> List[tuple]:
+        """Where sequences of these lengths share pages: [(places in `slots`, first logical page, the page behind the last)], each
+        place in one run at most, the runs chosen so that the fewest pages are read when a run's are read once.  In a ring only what
+        all of a run's sequences still hold counts.  A run stays true until one of the slots' pages changes (`version`)."""
+        if not self._holders:
+            return []
+        held = [self._slot_pages[s] for s in slots]
+        several = np.fromiter(self._holders, dtype=np.int64, count=len(self._holders))
+        # sequences that hold a shared page in common, directly or by way of others, are looked at together
+        counts = [len(h) for h in held]
+        flat = np.fromiter((p for h in held for p in h), dtype=np.int64, count=sum(counts))
+        owner = np.repeat(np.arange(len(slots)), counts)
+        mine = np.isin(flat, several)
+        kin = list(range(len(slots)))
+
+        def root(i: int) -> int:
+            while kin[i] != i:
+                kin[i] = kin[kin[i]]
+                i = kin[i]
+            return i
+
+        first: Dict[int, int] = {}
+        for page, i in zip(flat[mine].tolist(), owner[mine].tolist()):
+            j = first.setdefault(page, i)
+            if j != i:
+                kin[root(i)] = root(j)
+        families: Dict[int, List[int]] = {}
+        for i in sorted(set(owner[mine].tolist())):
+            families.setdefault(root(i), []).append(i)
+        out: List[tuple] = []
+        for members in families.values():
+            if len(members) < 2:
+                continue
+            last = [(lengths[i] - 1) // PAGE for i in members]
+            lo, hi = 0, min(last) + 1
+            if self.ring_pages:
+                lo = max(0, max(last) - self.ring_pages + 1)             # what the longest has not written over
+            if hi <= lo:
+                continue
+            entries = np.arange(lo, hi)
+            if self.ring_pages:
+                entries %= self.ring_pages
+            out += [(m, lo, lo + n) for m, n in _best_runs(self._table_np[np.asarray([slots[i] for i in members])][:, entries], members)[1]]
+        return out
 
     def compact(self) -> int:
         """Move the held pages to the front of the arrays; the number of them."""
@@ -168,6 +239,7 @@ class KVGroup:
             news = self.pages.lowest_free(len(olds))
             self._copy_listed(olds, news)
             self.pages.exchange(olds, news)
+            self.version += 1
             to = dict(zip(olds, news))
             self._holders = {to.get(p, p): k for p, k in self._holders.items()}
             for slot, held in self._slot_pages.items():

@@ -1,0 +1,153 @@
+"""Attention over pages that sequences share, against the formula in 64 bits on what each sequence holds (bound: shared_cases.share_bound)."""
+import random
+
+import pytest
+import torch
+from shared_cases import Tree, share_bound
+
+from hos_b200.errors import KernelError
+from hos_b200.parts import shared_attention as sa
+
+pytestmark = pytest.mark.gpu
+
+
+def compare(t, which, news, heads, cap=0.0, scale=None, plan=None, q=None, out=None):
+    step = t.step(which, news)
+    plan = plan or sa.plan(t.group, step)
+    scale = scale if scale is not None else t.dim ** -0.5
+    if q is None:
+        q = torch.randn(sum(news), heads * t.dim, generator=t.gen).to(torch.bfloat16).to(t.dev)
+    out = out if out is not None else torch.full(q.shape, 7.0, dtype=q.dtype, device=t.dev)
+    sa.attend(q, out, step, t.view, plan, heads, scale, cap, t.window)
+    got = out.double().cpu()
+    want = t.exact(q, which, news, heads, scale, cap, t.window)
+    keep = t.v
+    t.v = [v.abs() for v in keep]                            # the weighted means of |v|
+    bound = share_bound(t.exact(q, which, news, heads, scale, cap, t.window), want)
+    t.v = keep
+    worst = ((got - want).abs() / bound).max()
+    assert worst <= 1, float(worst)
+    return plan
+
+
+@pytest.mark.parametrize("dim,kv,per", [(64, 2, 2), (128, 2, 4), (256, 2, 2), (256, 1, 1), (16, 2, 3), (80, 1, 5), (48, 3, 1), (32, 2, 8), (128, 1, 16), (64, 1, 20),
+                                        (192, 1, 2)])
+@pytest.mark.parametrize("prefix,forks", [(1, 1), (64, 2), (130, 7), (700, 20)])
+def test_forks_of_a_prompt(dim, kv, per, prefix, forks):
+    t = Tree(kv, dim, seed=dim + prefix)
+    a = t.new(prefix)
+    all_ = [a] + t.fork(a, forks)
+    for j, i in enumerate(all_):
+        t.bring([i], [1 + (17 * j) % 90])
+    compare(t, all_, [1] * len(all_), per * kv, cap=50.0 if kv > 1 else 0.0)
+
+
+@pytest.mark.parametrize("window,chunk", [(70, 1), (200, 1), (200, 64), (1000, 64)])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_windows_and_rings(window, chunk, dim):
+    t = Tree(2, dim, window=window, chunk=chunk, seed=window + chunk)
+    a, b = t.new(500), t.new(90)
+    fa, fb = t.fork(a, 4), t.fork(b, 2)
+    order = fb + [a] + fa + [b]
+    for j, i in enumerate(order):
+        for _ in range(1 + j % 3):
+            t.bring([i], [min(chunk, 1 + 31 * j)])
+    compare(t, order, [1] * len(order), 4, cap=30.0)
+
+
+@pytest.mark.parametrize("dim,per", [(64, 2), (128, 4), (256, 2), (80, 3)])
+@pytest.mark.parametrize("window", [None, 150])
+@pytest.mark.parametrize("news", [(2, 2, 2, 2), (37, 37, 37, 37), (1, 64, 3, 20)])
+def test_pieces_of_several_rows(dim, per, window, news):
+    t = Tree(2, dim, window=window, chunk=64, seed=dim)
+    a = t.new(333)
+    all_ = [a] + t.fork(a, 3)
+    t.bring(all_, list(news))
+    compare(t, all_, list(news), 2 * per, cap=50.0)
+
+
+def test_a_tree_of_forks_in_no_order_with_strangers():
+    t = Tree(2, 128, seed=9)
+    a, x = t.new(300), t.new(77)
+    b, = t.fork(a)
+    t.bring([a], [200]), t.bring([b], [130])
+    fa, fb = t.fork(a, 3), t.fork(b, 5)
+    order = [x, a, b] + fa + fb
+    random.Random(3).shuffle(order)
+    for i in order:
+        t.bring([i], [5])
+    compare(t, order, [1] * len(order), 8)
+
+
+def test_sequences_that_share_nothing():
+    t = Tree(2, 64, seed=4)
+    order = [t.new(n) for n in (1, 64, 200, 1000)]
+    plan = compare(t, order, [1] * 4, 4)
+    assert plan.runs == []
+
+
+def test_long_sequences_are_cut():
+    t = Tree(1, 64, seed=5, max_seq_len=20000, pages=800)
+    a = t.new(16000)
+    all_ = [a] + t.fork(a, 2)
+    t.bring(all_, [900, 1, 64])
+    plan = compare(t, all_, [1, 1, 1], 2)
+    assert plan.work(2).parts > 40
+
+
+def test_scores_far_apart_and_a_steep_scale():
+    t = Tree(2, 128, seed=6)
+    a = t.new(400)
+    all_ = [a] + t.fork(a, 5)
+    t.bring(all_, [3] * 6)
+    compare(t, all_, [1] * 6, 4, cap=8.0, scale=1.0)
+    # one key far above the others
+    q = torch.zeros(6, 4 * 128)
+    q[:, ::128] = 8.0
+    compare(t, all_, [1] * 6, 4, scale=0.125, q=q.to(torch.bfloat16).cuda())
+
+
+def test_rows_apart_another_stream_and_a_replayed_graph():
+    t = Tree(2, 64, seed=7)
+    a = t.new(500)
+    all_ = [a] + t.fork(a, 9)
+    t.bring(all_, [20 + 7 * i for i in range(10)])
+    big = torch.randn(10, 3 * 256, generator=t.gen).to(torch.bfloat16).cuda()
+    q, out = big[:, 256:512], torch.zeros(10, 600, dtype=torch.bfloat16, device="cuda")
+    plan = compare(t, all_, [1] * 10, 4, q=q, out=out[:, 8:264])
+    assert not out[:, :8].any() and not out[:, 264:].any()
+    step = t.step(all_, [1] * 10)
+    first = out[:, 8:264].clone()
+    side = torch.cuda.Stream()
+    other = torch.zeros_like(first)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        sa.attend(q, other, step, t.view, plan, 4, 0.125)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(other, first)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        sa.attend(q, other, step, t.view, plan, 4, 0.125)
+    q.copy_(torch.randn(10, 256, generator=t.gen))
+    graph.replay()
+    second = other.clone()
+    compare(t, all_, [1] * 10, 4, q=q.contiguous(), out=other)
+    assert torch.equal(second, other) and not torch.equal(second, first)
+
+
+def test_refusals():
+    t = Tree(2, 64)
+    a = t.new(70)
+    f, = t.fork(a)
+    t.bring([a, f], [1, 1])
+    step, q = t.step([a, f], [1, 1]), torch.zeros(2, 256, dtype=torch.bfloat16, device="cuda")
+    plan = sa.plan(t.group, step)
+    for bad in (dict(q=q.float()), dict(q=q[:1]), dict(n_heads=3), dict(n_heads=2), dict(out=q[:, :128]), dict(window=64), dict(out=q.float()), dict(n_heads=0)):
+        k = dict(dict(q=q, out=q.clone(), n_heads=4, window=None), **bad)
+        with pytest.raises(KernelError):
+            sa.attend(k["q"], k["out"], step, t.view, plan, k["n_heads"], 1.0, 0.0, k["window"])
+    with pytest.raises(KernelError, match="16 bytes"):
+        sa.attend(torch.zeros(2, 257, dtype=torch.bfloat16, device="cuda")[:, 1:], q.clone(), step, t.view, plan, 4, 1.0)
+    t.bring([f], [64])
+    with pytest.raises(KernelError, match="changed"):
+        sa.attend(q, q.clone(), step, t.view, plan, 4, 1.0)
