@@ -119,6 +119,10 @@ class LinearHead(Part):
         epi = ops.EPI_SOFTCAP if self.softcap > 0.0 else ops.EPI_NONE
         return linear.matmul(h, self.table, out_dtype=torch.float32, epilogue=epi, cap=self.softcap)
 
+    def log_probs(self, h: torch.Tensor, tokens: torch.Tensor, top: int = 0):
+        """Scores (sampling.TokenScores) of tokens[i] under the logits of row i, without holding all of the logits."""
+        return linear.log_probs(h, self.table, tokens, cap=self.softcap, top=top)
+
 
 register_part("embedding", "scaled_embedding", ScaledEmbedding)
 register_part("embedding", "pair_hash_embedding", PairHashEmbedding)
