@@ -20,7 +20,7 @@
 //
 // Epilogues: none; soft-cap c*tanh(x/c) with 32-bit output (logits); gated act(gate)*up,
 // where W holds the gate rows followed by the up rows and a tile loads matching rows of both; act(x + bias[n]) or,
-// without a bias, act(x), act none, the erf-form or the tanh-form GELU.
+// without a bias, act(x), act none, the erf-form or the tanh-form GELU; the moments of rows of logits, for log probabilities (below).
 //
 // Every wait on an mbarrier is bounded in time: a wait that runs out sets an error flag,
 // the roles leave their loops, tensor memory is freed and the kernel returns.
@@ -28,6 +28,7 @@
 #include "common.cuh"
 #include "kv_layout.cuh"
 #include "mma_utils.cuh"
+#include "moments.cuh"
 #include "tcgen05_pair.cuh"
 
 namespace hos {
@@ -38,7 +39,7 @@ constexpr int kGemmThreads = 192;
 constexpr int kPairThreads = 320;         // the kernel on pairs of SMs: TMA warp, MMA warp, 8 epilogue warps
 constexpr long long kWaitCycles = 1ll << 31;     // about a second
 
-enum { kGEpiNone = 0, kGEpiSoftcap = 1, kGEpiGated = 2, kGEpiBias = 3, kGEpiRope = 4 };
+enum { kGEpiNone = 0, kGEpiSoftcap = 1, kGEpiGated = 2, kGEpiBias = 3, kGEpiRope = 4, kGEpiScores = 5 };
 
 __device__ int g_gemm_error = 0;
 __device__ int* g_gemm_error_host = nullptr;     // a word in pinned host memory, if the host gave one
@@ -150,6 +151,16 @@ struct RopeEpi {
     int n_heads, n_kv_heads, write_cache;
 };
 
+// What the epilogue of a head's product leaves instead of the logits (kGEpiScores): an epilogue thread has 128 columns of a row of a tile,
+// and joins their moments (moments.cuh) to those of the tiles of this row that its CTA took before; parts[part][row] are written when
+// the rows change, and `wanted` gets the logit of the row's token from the thread that meets it.
+struct ScoreEpi {
+    const int* tokens;         // [M]
+    float4* parts;             // [parts][rows of m_tiles x 256]: (maximum, sum, weighted sum, unused)
+    float* wanted;             // [M]
+    int same_rows;             // 1: a pair's tiles are all of the same rows (it leaves one part), 0: one part a tile
+};
+
 struct GemmParams {
     void* out;            // [M, N] row-major (bf16 or f32); with K splits: f32 partials [splits][M][N]
     int M, N, K;          // the product's logical sizes: rows of A, rows of W (per half if gated), K
@@ -160,6 +171,7 @@ struct GemmParams {
     int act;              // gated: 0 tanh-form GELU, 1 x logistic(x), 2 the clamped form (common.cuh); bias: 0 none, 1 erf-form GELU, 2 tanh form
     const float* bias;    // kGEpiBias: [N], or null
     RopeEpi rope;         // kGEpiRope only
+    ScoreEpi score;       // kGEpiScores only
 };
 
 // Thirty-two columns n0.. of one row, with their bias and activation (all lanes of a warp read the same bias: one line).
@@ -603,6 +615,7 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a,     // A: boxes o
         const int col_half = (warp - 2) >> 2;
         int local_tile = 0;
         bool ok = true;
+        Moments row_sums{-INFINITY, 0.f, 0.f};                 // kGEpiScores
         for (int tile = pair; tile < total_tiles && ok; tile += n_pairs, ++local_tile) {
             int mt, nt, ks;
             tile_coords(tile, mt, nt, ks);
@@ -743,6 +756,48 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a,     // A: boxes o
                         advance(col0_n, c0_n);
                     }
                 }
+            } else if constexpr (EPI == kGEpiScores) {
+                const int m = mt * 2 * GM + (int)rank * GM + quarter * 32 + lane;
+                const int token = m < p.M ? p.score.tokens[m] : -1;
+                if (!mbar_wait_timed(&acc_full[acc], (local_tile >> 1) & 1)) { ok = false; break; }
+                tc_fence_after();
+                const float twice = p.cap > 0.f ? 2.f * 1.44269504f / p.cap : 0.f;
+#pragma unroll 1
+                for (int c0 = col_half * (BN / 2); c0 < (col_half + 1) * (BN / 2); c0 += 32) {
+                    const int n0 = nt * BN + c0;
+                    if (n0 >= p.N) break;
+                    uint32_t v[32];
+                    tmem_ld_32x32(t_lane + c0, v);
+                    tmem_ld_wait();
+                    float f[32];
+                    if (p.cap > 0.f) {                         // c tanh(x / c) = c - 2 c / (1 + e^(2 x / c)): off by 2^-22 c at most
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            f[j] = fmaf(-2.f * p.cap, rcp_approx(1.f + ex2_approx(twice * __uint_as_float(v[j]))), p.cap);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
+                    }
+                    if (n0 + 32 > p.N) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) f[j] = n0 + j < p.N ? f[j] : -INFINITY;
+                    }
+                    if ((unsigned)(token - n0) < 32u) {
+                        float x = f[0];
+#pragma unroll
+                        for (int j = 1; j < 32; ++j) x = token - n0 == j ? f[j] : x;
+                        p.score.wanted[m] = x;
+                    }
+                    float most = f[0];
+#pragma unroll
+                    for (int j = 1; j < 32; ++j) most = fmaxf(most, f[j]);
+                    add_to(row_sums, f, most);
+                }
+                if (!p.score.same_rows || tile + n_pairs >= total_tiles) {
+                    const int part = 2 * (p.score.same_rows ? pair / m_tiles : nt) + col_half;
+                    p.score.parts[(size_t)part * (m_tiles * 2 * GM) + m] = make_float4(row_sums.m, row_sums.s, row_sums.u, 0.f);
+                    row_sums = Moments{-INFINITY, 0.f, 0.f};
+                }
             } else {
             if (!mbar_wait_timed(&acc_full[acc], (local_tile >> 1) & 1)) { ok = false; break; }
             tc_fence_after();
@@ -845,6 +900,30 @@ __global__ void splitk_reduce_kernel(const float* __restrict__ part, OutT* __res
     float s = 0.f;
     for (int k = 0; k < splits; ++k) s += part[(size_t)k * M * N + i];
     out[(i / N) * ldo + (i % N)] = from_float<OutT>(s);
+}
+
+// The parts of kGEpiScores joined: 8 rows a block, 32 threads a row.  A row whose token is outside the vocabulary is padding: zeros.
+__global__ void __launch_bounds__(256) score_merge_kernel(ScoreEpi s, int parts, int stride, int M, int N, float* __restrict__ logprob,
+                                                          float* __restrict__ entropy) {
+    __shared__ Moments held[32][8];
+    pdl_enter();
+    const int r = threadIdx.x & 7, deep = threadIdx.x >> 3, m = blockIdx.x * 8 + r;
+    Moments mine{-INFINITY, 0.f, 0.f};
+#pragma unroll 4
+    for (int p = deep; p < parts; p += 32) {
+        const float4 v = s.parts[(size_t)p * stride + m];      // (rows behind the last are there too)
+        mine = joined(mine, Moments{v.x, v.y, v.z});
+    }
+    held[deep][r] = mine;
+    __syncthreads();
+    if (deep == 0 && m < M) {
+        for (int d = 1; d < 32; ++d) mine = joined(mine, held[d][r]);
+        const int token = s.tokens[m];
+        const bool padding = token < 0 || token >= N;
+        const float log_s = logf(mine.s);
+        logprob[m] = padding ? 0.f : (s.wanted[m] - mine.m) - log_s;
+        entropy[m] = padding ? 0.f : log_s - mine.u / mine.s;
+    }
 }
 
 // ---- host side -----------------------------------------------------------------------------
@@ -1170,4 +1249,45 @@ extern "C" int hos_gemm_tc_qkv_rope(const void* A, const void* W, void* out, int
     if ((rc = make_map(&mn, W, N, K, ldw, 128))) return rc;
     const int m_tiles = (M + 2 * GM - 1) / (2 * GM);
     return launch_pair<kGEpiRope, bf16>(mm, mn, p, m_tiles * ((N + 255) / 256), stream);
+}
+
+// How many pairs of SMs a product of `tiles` tiles runs on, and whether each pair then has tiles of the same rows only.
+static int score_pairs(int m_tiles, int n_tiles) {
+    const long long tiles = (long long)m_tiles * n_tiles;
+    const int most = sm_count() / 2;
+    return tiles < most ? (int)tiles : most;
+}
+static bool score_same_rows(int m_tiles, int n_tiles) { return score_pairs(m_tiles, n_tiles) % m_tiles == 0; }
+
+// Floats of workspace of hos_gemm_tc_scores: the parts, and a wanted logit a row.
+extern "C" long long hos_gemm_tc_scores_workspace(int M, int N) {
+    const int m_tiles = (M + 2 * GM - 1) / (2 * GM), n_tiles = (N + 255) / 256;
+    const long long parts = 2ll * (score_same_rows(m_tiles, n_tiles) ? score_pairs(m_tiles, n_tiles) / m_tiles : n_tiles);
+    return (parts * 4 + 1) * m_tiles * 2 * GM;
+}
+
+// logprob[m] = l_t - log sum e^l and entropy[m] of the rows l = c tanh(A . W^T / c) (cap c > 0) or A . W^T, t = tokens[m] (outside 0..N-1:
+// zeros), on pairs of SMs, without the logits in memory.  workspace: 16-byte aligned.
+extern "C" int hos_gemm_tc_scores(const void* A, const void* W, const int* tokens, float* logprob, float* entropy, int M, int N, int K,
+                                  int lda, int ldw, float cap, float* workspace, cudaStream_t stream) {
+    if (M <= 0) return 0;
+    if (N <= 0 || K <= 0) HOS_REFUSE("gemm_tc_scores: a head of %d tokens by %d", N, K);
+    if ((K % 8) || (lda % 8) || (ldw % 8) || ((uintptr_t)A % 16) || ((uintptr_t)W % 16))
+        HOS_REFUSE("gemm_tc_scores: K and the leading dimensions must be multiples of 8 elements and the operands "
+                   "16-byte aligned (K %d lda %d ldw %d)", K, lda, ldw);
+    if (workspace == nullptr || ((uintptr_t)workspace % 16)) HOS_REFUSE("gemm_tc_scores: a workspace on 16 bytes is needed");
+    const int m_tiles = (M + 2 * GM - 1) / (2 * GM), n_tiles = (N + 255) / 256;
+    if ((long long)m_tiles * n_tiles > (1 << 30)) HOS_REFUSE("gemm_tc_scores: %d rows by %d tokens", M, N);
+    const bool same = score_same_rows(m_tiles, n_tiles);
+    const int parts = 2 * (same ? score_pairs(m_tiles, n_tiles) / m_tiles : n_tiles), stride = m_tiles * 2 * GM;
+    GemmParams p = {};
+    p.M = M; p.N = N; p.K = K; p.k_splits = 1; p.gate_rows = N; p.cap = cap;
+    p.score = ScoreEpi{tokens, reinterpret_cast<float4*>(workspace), workspace + (size_t)parts * 4 * stride, same ? 1 : 0};
+    CUtensorMap mm, mn;
+    int rc;
+    if ((rc = make_map(&mm, A, M, K, lda, GM))) return rc;
+    if ((rc = make_map(&mn, W, N, K, ldw, 128))) return rc;
+    if ((rc = launch_pair<kGEpiScores, float>(mm, mn, p, m_tiles * n_tiles, stream))) return rc;
+    launch_pdl(score_merge_kernel, dim3((M + 7) / 8), dim3(256), 0, stream, p.score, parts, stride, M, N, logprob, entropy);
+    return check_launch("gemm_tc_scores");
 }

@@ -1,8 +1,8 @@
 // Log probabilities of given tokens, the entropy, and the likeliest tokens, from rows of logits.
 //
-// Of a row l: M = max l, S = sum e^(l - M), U = sum e^(l - M) (l - M).  Then log p(t) = (l_t - M) - log S and the entropy
-// -sum p log p = log S - U / S.  A thread keeps (M, S, U) of what it has seen and, when its maximum grows by d, takes S to S e^-d and
-// U to (U - S d) e^-d, so the logits are read once.  All of it is held in 32 bits; a thread adds some hundred terms, trees the rest.
+// Of a row l: M = max l, S = sum e^(l - M), U = sum e^(l - M) (l - M) (moments.cuh).  A thread keeps them of what it has seen and, when
+// its maximum grows by d, takes S to S e^-d and U to (U - S d) e^-d, so the logits are read once.  All of it is held in 32 bits; a
+// thread adds some hundred terms, trees the rest.
 //
 // The likeliest k tokens in the same pass.  A number and its token make a key of 64 bits, larger for larger numbers and, of equal
 // ones, for lower tokens: keys are all different, so ties, rows ruled out (-inf) and rows that hold one number only need no path of
@@ -14,6 +14,7 @@
 // A row is one block's, or is cut over a cluster of 2 to 8 blocks whose first merges what they leave in shared memory: nothing is
 // kept in device memory, and every sum has a fixed order.
 #include "common.cuh"
+#include "moments.cuh"
 
 namespace hos {
 
@@ -41,22 +42,6 @@ __device__ __forceinline__ float least_of(Key k) {
     return v == v ? v : -INFINITY;                     // (below every number's keys)
 }
 __device__ __forceinline__ int key_token(Key k) { return (int)~(uint32_t)k; }
-
-struct Moments { float m, s, u; };                     // maximum, sum of e^(l - m), sum of e^(l - m) (l - m)
-
-__device__ __forceinline__ float exp_of(float d) { return ex2_approx(d * 1.44269504f); }
-
-// Both with the larger maximum.
-__device__ __forceinline__ Moments joined(const Moments& a, const Moments& b) {
-    Moments r;
-    r.m = fmaxf(a.m, b.m);
-    const float da = a.m == r.m ? 0.f : a.m - r.m, db = b.m == r.m ? 0.f : b.m - r.m;
-    const float ea = exp_of(da), eb = exp_of(db);
-    // a part without a number (s = 0, m = -inf) adds nothing; a not-a-number stays one
-    r.s = a.s * ea + b.s * eb;
-    r.u = (a.s == 0.f ? 0.f : (a.u + a.s * da) * ea) + (b.s == 0.f ? 0.f : (b.u + b.s * db) * eb);
-    return r;
-}
 
 struct LogProbArgs {
     const float* logits;
@@ -166,22 +151,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(LogP
         float most = x[0];
 #pragma unroll
         for (int j = 1; j < kEach; ++j) most = fmaxf(most, x[j]);
-        if (most > mine.m) {
-            const float d = mine.m - most, e = mine.s == 0.f ? 0.f : exp_of(d);
-            mine.u = mine.s == 0.f ? 0.f : (mine.u + mine.s * d) * e;
-            mine.s *= e;
-            mine.m = most;
-        }
-        const float m = mine.m == -INFINITY ? 0.f : mine.m;
-        float s[2] = {}, u[2] = {};
-#pragma unroll
-        for (int j = 0; j < kEach; ++j) {
-            const float d = x[j] - m, e = exp_of(d);
-            s[j & 1] += e;
-            u[j & 1] = fmaf(e, fmaxf(d, -1000.f), u[j & 1]);     // (0 times -inf would be no number)
-        }
-        mine.s += s[0] + s[1];
-        mine.u += u[0] + u[1];
+        add_to(mine, x, most);
         if (!TOP) continue;
 
         // ---- candidates of this tile ----

@@ -100,6 +100,27 @@ def matmul_partials(x, w, k_splits: Optional[int] = None) -> Optional[torch.Tens
     return ws[: used.value]
 
 
+SCORE_MIN_ROWS = PAIR_MIN_ROWS
+
+
+def can_score(x: torch.Tensor, w: torch.Tensor) -> bool:
+    """Whether log probabilities come out of the head's product itself: the product's rules, and rows enough."""
+    return (enabled and x.dtype == torch.bfloat16 and w.dtype == torch.bfloat16 and x.shape[0] >= SCORE_MIN_ROWS and x.shape[1] == w.shape[1]
+            and x.shape[1] % 8 == 0 and x.stride(1) == 1 and w.stride(1) == 1 and x.stride(0) % 8 == 0 and w.stride(0) % 8 == 0
+            and x.data_ptr() % 16 == 0 and w.data_ptr() % 16 == 0)
+
+
+def log_probs(x: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, logprob: torch.Tensor, entropy: torch.Tensor, cap: float) -> None:
+    """logprob[m], entropy[m] of tokens[m] under the logits x[m] . w^T (soft-capped if cap > 0), which are never in memory."""
+    m, k = x.shape
+    n = w.shape[0]
+    f = lib().lib.hos_gemm_tc_scores_workspace
+    f.restype, f.argtypes = ctypes.c_longlong, [ctypes.c_int, ctypes.c_int]
+    ws = torch.empty(f(m, n), dtype=torch.float32, device=x.device)
+    lib().call("hos_gemm_tc_scores", x.data_ptr(), w.data_ptr(), tokens.data_ptr(), logprob.data_ptr(), entropy.data_ptr(), m, n, k, x.stride(0),
+               w.stride(0), float(cap), ws.data_ptr(), ops._stream())
+
+
 def wait_probe(limit_cycles: int = 1 << 20) -> None:
     """A tiny kernel that waits on a barrier nothing arrives at, gives up after `limit_cycles` (well
     under a millisecond by default) and records it as the product kernels do: for tests of what

@@ -87,13 +87,21 @@ LOGITS_BYTES = 256 << 20        # of logits that `log_probs` holds at a time
 def log_probs(x: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, cap: float = 0.0, top: int = 0):
     """Scores (sampling.TokenScores) of tokens[i] (int32 [rows]) under the logits x[i] . w^T of a head w [vocab, width], soft-capped
     cap * tanh(l / cap) if cap > 0, with the `top` likeliest tokens if asked for; a token outside the vocabulary marks a padding row
-    (zeros).  At most LOGITS_BYTES of logits are held at a time."""
+    (zeros).  Many bfloat16 rows without alternatives: the scores come out of the product, and no logits are held; else at most LOGITS_BYTES of
+    them at a time."""
     from ..sampling.scores import TokenScores, log_probs as from_logits
     ops._check_here(x, "hidden rows")
     if x.dim() != 2 or x.dtype not in (torch.float32, torch.bfloat16) or tokens.shape != x.shape[:1]:
         raise KernelError(f"log_probs: one token for each hidden row is needed, found rows {tuple(x.shape)} ({x.dtype}) and tokens {tuple(tokens.shape)}")
     m, vocab = x.shape[0], w.n if isinstance(w, Weight4) else w.shape[0]
     out = TokenScores.empty(m, top, x.device)
+    if not top and not _force_plain and not isinstance(w, Weight4) and x.dtype == torch.bfloat16:
+        from . import gemm_tc
+        if gemm_tc.can_score(x, w):
+            ops._check(tokens, "tokens", torch.int32, 1)
+            ops._check_here(w, "head")
+            gemm_tc.log_probs(x, w, tokens, out.logprob, out.entropy, cap)
+            return out
     epilogue = ops.EPI_SOFTCAP if cap > 0.0 else ops.EPI_NONE
     each = max(1, LOGITS_BYTES // (4 * vocab))
     for lo in range(0, m, each):
