@@ -4,12 +4,13 @@
 // its maximum grows by d, takes S to S e^-d and U to (U - S d) e^-d, so the logits are read once.  All of it is held in 32 bits; a
 // thread adds some hundred terms, trees the rest.
 //
-// The likeliest k tokens in the same pass.  A number and its token make a key of 64 bits, larger for larger numbers and, of equal
-// ones, for lower tokens: keys are all different, so ties, rows ruled out (-inf) and rows that hold one number only need no path of
-// their own.  The block keeps a threshold that at least k of its keys so far reach, and a list of those that do.  The first threshold
-// is found by halving an interval of keys until between k and 2k of the THREADS' largest keys reach it; after that few numbers are
-// anywhere near, and a tile costs a comparison a thread.  A list that grows is cut back by halving again; a tile that brings more
-// keys than the list holds (numbers in rising order) gets a threshold of its own first.
+// The likeliest k tokens in the same pass.  A number and its token make a key of 64 bits, larger for larger numbers and, of equal ones,
+// for lower tokens: keys are all different.  32 groups of threads say what the largest number is that they have had; at least k numbers
+// reach the k'th largest of these, and it rises as the row goes by.  What reaches it goes into a list, some 2 k ln(tiles) of a row in no
+// order; a warp without a candidate does a comparison a tile, and no warp waits for another after the first tile.  The largest keys of
+// the list are the answer.  If the list cannot hold the candidates (numbers in rising order), they are collected once more with the
+// last border; if it still cannot (equal numbers), the border between the k'th key and the next is found by halving an interval of
+// keys and counting.
 //
 // A row is one block's, or is cut over a cluster of 2 to 8 blocks whose first merges what they leave in shared memory: nothing is
 // kept in device memory, and every sum has a fixed order.
@@ -20,8 +21,7 @@ namespace hos {
 
 constexpr int kMostTop = 32;                           // alternatives a row
 constexpr int kEach = 32;                              // numbers that a thread holds of a tile
-constexpr int kCompactAbove = 128;                     // keys in the list after which it is cut back
-constexpr int kListRoom = kCompactAbove + 2 * kMostTop * kEach;
+constexpr int kListRoom = 1024;                        // candidates of a block
 
 typedef unsigned long long Key;
 
@@ -32,14 +32,8 @@ __device__ __forceinline__ Key key_of(float v, int token) {
     const uint32_t up = b & 0x80000000u ? ~b : b | 0x80000000u;
     return (Key)up << 32 | (uint32_t)~token;
 }
-__device__ __forceinline__ float key_number(Key k) {
-    const uint32_t up = (uint32_t)(k >> 32);
+__device__ __forceinline__ float number_of(uint32_t up) {        // of a key's upper half
     return __uint_as_float(up & 0x80000000u ? up & 0x7fffffffu : ~up);
-}
-// What a thread's largest number is compared with: no number that is less has a key that reaches k.
-__device__ __forceinline__ float least_of(Key k) {
-    const float v = key_number(k);
-    return v == v ? v : -INFINITY;                     // (below every number's keys)
 }
 __device__ __forceinline__ int key_token(Key k) { return (int)~(uint32_t)k; }
 
@@ -58,10 +52,10 @@ struct LogProbArgs {
 struct LogProbShared {
     Key list[kListRoom];
     Key best[kMostTop];              // a block's likeliest, sorted; in the end the first block's: all blocks'
-    Key warp_key[32];
     Moments part[32];
     Moments all;
-    Key threshold;
+    uint32_t group_most[32];
+    int warp_count[32];
     int count;
 };
 
@@ -105,6 +99,7 @@ __device__ __forceinline__ Key halved(Key lo, Key hi, int top, Count count_at) {
 template <int THREADS, bool TOP>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(LogProbArgs a, int blocks) {
     __shared__ LogProbShared sh;
+    constexpr int GROUP = THREADS / 32;                          // threads that share a number of group_most
     pdl_enter();
     const int row = blockIdx.x / blocks, rank = blockIdx.x % blocks;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -127,110 +122,131 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(LogP
     const int vectors = (a.vocab + before + 3) / 4;
     const int per_block = (vectors + blocks - 1) / blocks;
     const int v0 = rank * per_block, v1 = min(vectors, v0 + per_block);
-    if (TOP && tid == 0) { sh.count = 0; sh.threshold = 0; }
     Moments mine{-INFINITY, 0.f, 0.f};
-    if (TOP) __syncthreads();
-    Key threshold = 0;
-    float least = -INFINITY;                                     // the threshold's number: less than that is no candidate
-    bool first = true;
-
-    // the tiles are a block's in rising order of tokens; every thread of the block walks over all of them
-    for (int base = v0; base < v1; base += THREADS * (kEach / 4)) {
-        float x[kEach];
+    // numbers i to i + 3 of the row, i = 4 v - before; -inf outside the row
+    auto four = [&](int v) {
+        const int i = 4 * v - before;
+        if (i >= 0 && i + 4 <= a.vocab) return *reinterpret_cast<const float4*>(l + i);
+        auto one = [&](int c) { return i + c >= 0 && i + c < a.vocab ? l[i + c] : -INFINITY; };
+        return make_float4(one(0), one(1), one(2), one(3));
+    };
+    const uint32_t nothing = (uint32_t)(key_of(-INFINITY, 0) >> 32);
+    float least = -INFINITY;                                     // TOP: at least `top` numbers reach it
+    // the k'th largest of what the groups of threads have had; groups may be read while they rise: what they have had stays true
+    auto raise_least = [&]() {
+        const uint32_t up = *reinterpret_cast<volatile uint32_t*>(&sh.group_most[lane]);
+        uint32_t lo = __reduce_min_sync(0xffffffffu, up), hi = __reduce_max_sync(0xffffffffu, up) + 1;
+        while (hi - lo > 1) {                                    // at least `top` groups reach lo, fewer hi
+            const uint32_t mid = lo + (hi - lo) / 2;
+            const int n = __popc(__ballot_sync(0xffffffffu, up >= mid));
+            if (n >= a.top) lo = mid; else hi = mid;
+            if (n == a.top) break;
+        }
+        const float v = number_of(max(lo, nothing + 1));         // a number that is ruled out is no candidate here
+        least = fmaxf(least, v);
+    };
+    auto put = [&](Key k) {
+        const int at = atomicAdd(&sh.count, 1);
+        if (at < kListRoom) sh.list[at] = k;
+    };
+    // tiles of the block, the same number for each of its threads
+    auto walk = [&](auto take) {
+        for (int base = v0; base < v1; base += THREADS * (kEach / 4)) {
+            float x[kEach];
 #pragma unroll
-        for (int j = 0; j < kEach / 4; ++j) {
-            const int v = base + j * THREADS + tid, i = 4 * v - before;
-            if (v < v1 && i >= 0 && i + 4 <= a.vocab) {
-                const float4 f = *reinterpret_cast<const float4*>(l + i);
+            for (int j = 0; j < kEach / 4; ++j) {
+                const int v = base + j * THREADS + tid;
+                const float4 f = v < v1 ? four(v) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
                 x[4 * j] = f.x; x[4 * j + 1] = f.y; x[4 * j + 2] = f.z; x[4 * j + 3] = f.w;
-            } else {
-#pragma unroll
-                for (int c = 0; c < 4; ++c) x[4 * j + c] = v < v1 && i + c >= 0 && i + c < a.vocab ? l[i + c] : -INFINITY;
             }
+            float most = x[0];
+#pragma unroll
+            for (int j = 1; j < kEach; ++j) most = fmaxf(most, x[j]);
+            take(base, x, most);
         }
-        float most = x[0];
+    };
+    // the numbers of a tile that reach `least`, into the list: read again, so that this stays out of the registers
+    auto collect = [&](int base, const float (&x)[kEach]) {
+        uint32_t hits = 0;
 #pragma unroll
-        for (int j = 1; j < kEach; ++j) most = fmaxf(most, x[j]);
-        add_to(mine, x, most);
-        if (!TOP) continue;
-
-        // ---- candidates of this tile ----
-        if (!__syncthreads_or(first || !(most < least))) continue;
-        auto token_at = [&](int j) { return 4 * (base + (j >> 2) * THREADS + tid) - before + (j & 3); };
-        auto inside = [&](int j) { return base + (j >> 2) * THREADS + tid < v1 && token_at(j) >= 0 && token_at(j) < a.vocab; };
-        auto largest = [&]() {                                   // this thread's largest key of the tile
-            Key k = 0;
-#pragma unroll
-            for (int j = 0; j < kEach; ++j)
-                if (inside(j)) k = max(k, key_of(x[j], token_at(j)));
-            return k;
-        };
-        auto from_maxima = [&]() {                               // a threshold by the threads' largest keys of this tile
-            const Key k = largest();
-            Key hi = k;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-            if (lane == 0) sh.warp_key[warp] = hi;
-            __syncthreads();
-            hi = lane < WARPS ? sh.warp_key[lane] : 0;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-            return halved(0, hi + 1, a.top, [&](Key at) { return __syncthreads_count(k >= at); });
-        };
-        auto push = [&]() {
-            if (!(most < least)) {
-#pragma unroll
-                for (int j = 0; j < kEach; ++j)
-                    if (inside(j)) {
-                        const Key k = key_of(x[j], token_at(j));
-                        if (k >= threshold) {
-                            const int at = atomicAdd(&sh.count, 1);
-                            if (at < kListRoom) sh.list[at] = k;
-                        }
-                    }
-            }
-            __syncthreads();
-        };
-        if (first) {
-            threshold = from_maxima();
-            first = false;
-            least = least_of(threshold);
+        for (int j = 0; j < kEach; ++j) hits |= x[j] >= least ? 1u << j : 0u;
+        while (hits != 0) {
+            const int j = __ffs(hits) - 1, i = 4 * (base + (j >> 2) * THREADS + tid) - before + (j & 3);
+            hits &= hits - 1;
+            put(key_of(l[i], i));                                // (what lies outside the row is -inf and reaches nothing)
         }
-        const int held = sh.count;                               // (nobody adds to it before the barrier that is next)
+    };
+    if (TOP) {
+        if (tid < 32) sh.group_most[tid] = nothing;
+        if (tid == 0) sh.count = 0;
         __syncthreads();
-        push();
-        if (sh.count > kListRoom) {                              // too many: no more than 2 top threads' numbers with this tile's own threshold
-            __syncthreads();
-            if (tid == 0) sh.count = held;
-            threshold = max(threshold, from_maxima());
-            least = least_of(threshold);
-            __syncthreads();
-            push();
-        }
-        if (sh.count > kCompactAbove) {
-            const int n = sh.count;
-            auto count_at = [&](Key at) {
-                int c = 0;
-                for (int i = tid; i < n; i += THREADS) c += sh.list[i] >= at;
+    }
+    walk([&](int base, const float (&x)[kEach], float most) {
+        add_to(mine, x, most);
+        if (!TOP) return;
+        const bool first = base == v0;
+        if (!first && !__any_sync(0xffffffffu, most >= least)) return;
+        uint32_t up = (uint32_t)(key_of(mine.m, 0) >> 32);
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
-                __syncthreads();
-                if (lane == 0) sh.warp_key[warp] = c;
-                __syncthreads();
-                c = 0;
-                for (int w = 0; w < WARPS; ++w) c += (int)sh.warp_key[w];
-                return c;
-            };
-            threshold = max(threshold, halved(threshold, ~0ull, a.top, count_at));
-            least = least_of(threshold);
-            // the keys that reach it, moved to the front: a round of threads at a time, read before any is written
-            if (tid == 0) sh.count = 0;
-            for (int i0 = 0; i0 < n; i0 += THREADS) {
-                const Key k = i0 + tid < n ? sh.list[i0 + tid] : 0;
-                __syncthreads();
-                if (i0 + tid < n && k >= threshold) sh.list[atomicAdd(&sh.count, 1)] = k;
-            }
+        for (int o = GROUP < 32 ? GROUP / 2 : 16; o > 0; o >>= 1) up = max(up, __shfl_xor_sync(0xffffffffu, up, o));
+        if (tid % GROUP == 0) *reinterpret_cast<volatile uint32_t*>(&sh.group_most[tid / GROUP]) = up;
+        if (first) __syncthreads(); else __syncwarp();
+        raise_least();
+        if (most >= least) collect(base, x);
+        __syncwarp();
+    });
+
+    if (TOP) {
+        __syncthreads();
+        if (sh.count > kListRoom) {
+            // more than the list holds (numbers in rising order): once more with what is known now
             __syncthreads();
+            if (tid == 0) sh.count = 0;
+            raise_least();
+            __syncthreads();
+            walk([&](int base, const float (&x)[kEach], float most) { if (most >= least) collect(base, x); });
+            __syncthreads();
+        }
+        if (sh.count > kListRoom) {
+            // still more (many equal numbers, or a few threads' large ones): the border between the top'th key and the next, by counting
+            __syncthreads();
+            auto each_key = [&](auto take) {
+                for (int v = v0 + tid; v < v1; v += THREADS)
+                    for (int c = 0; c < 4; ++c) {
+                        const int i = 4 * v - before + c;
+                        if (i >= 0 && i < a.vocab) take(key_of(l[i], i));
+                    }
+            };
+            const Key border = halved(key_of(least, (1 << 30) + 1), ~0ull, a.top, [&](Key at) {
+                int n = 0;
+                each_key([&](Key k) { n += k >= at ? 1 : 0; });
+                n = __reduce_add_sync(0xffffffffu, n);
+                __syncthreads();
+                if (lane == 0) sh.warp_count[warp] = n;
+                __syncthreads();
+                n = 0;
+                for (int w = 0; w < WARPS; ++w) n += sh.warp_count[w];
+                return n;
+            });
+            if (tid == 0) sh.count = 0;
+            __syncthreads();
+            each_key([&](Key k) { if (k >= border) put(k); });
+            __syncthreads();
+        }
+        if (sh.count < a.top && warp == 0) {                     // a block of few numbers: the first of those ruled out make it up
+            int n = sh.count;
+            const int end = min(a.vocab, 4 * v1 - before);
+            for (int i0 = max(0, 4 * v0 - before); i0 < end && n < a.top; i0 += 32) {
+                const int i = i0 + lane;
+                const Key k = i < end ? key_of(l[i], i) : 0;
+                const bool out = i < end && (uint32_t)(k >> 32) == nothing;
+                const uint32_t who = __ballot_sync(0xffffffffu, out);
+                const int at = n + __popc(who & ((1u << lane) - 1));
+                if (out && at < kListRoom) sh.list[at] = k;
+                n += __popc(who);
+            }
+            __syncwarp();
+            if (lane == 0) sh.count = min(n, kListRoom);
         }
     }
 
@@ -255,6 +271,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(LogP
         for (int i = tid; i < n; i += THREADS) {
             const Key k = from[i];
             int larger = 0;
+#pragma unroll 8
             for (int j = 0; j < n; ++j) larger += from[j] > k;
             if (larger < a.top && k != 0) to[larger] = k;
         }
@@ -271,11 +288,11 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(LogP
                 sh.all = r;
             }
             if (TOP) {
-                for (int i = tid; i < blocks * kMostTop; i += THREADS) sh.list[i] = cluster_key(cluster_address(&sh.best[i % kMostTop], i / kMostTop));
+                for (int i = tid; i < blocks * a.top; i += THREADS) sh.list[i] = cluster_key(cluster_address(&sh.best[i % a.top], i / a.top));
                 __syncthreads();
                 if (tid < kMostTop) sh.best[tid] = 0;
                 __syncthreads();
-                sort_list(sh.list, blocks * kMostTop, sh.best);
+                sort_list(sh.list, blocks * a.top, sh.best);
             }
         }
         cluster_meet();                                          // nobody leaves while its memory is read
@@ -321,7 +338,7 @@ extern "C" const char* hos_last_error() { return error_buffer(); }
 
 // Per row of float32 logits (`stride` numbers from row to row): the log probability of tokens[row] and the entropy; with `top`,
 // the likeliest `top` tokens (of equal ones the lower first) and their log probabilities.  A row whose token is outside the vocabulary
-// is padding: zeros, tokens -1.  `blocks` (1, 2, 4 or 8) of `threads` (256 or 1024) threads share a row.
+// is padding: zeros, tokens -1.  `blocks` (1, 2, 4 or 8) of `threads` (128, 256 or 1024) threads share a row.
 extern "C" int hos_log_probs(const float* logits, long long stride, int rows, int vocab, const int* tokens, float* logprob,
                              float* entropy, int top, int* top_ids, float* top_logprobs, int threads, int blocks,
                              cudaStream_t stream) {
@@ -333,6 +350,7 @@ extern "C" int hos_log_probs(const float* logits, long long stride, int rows, in
     if (blocks != 1 && blocks != 2 && blocks != 4 && blocks != 8) HOS_REFUSE("log_probs: %d blocks a row", blocks);
     const LogProbArgs a{logits, stride, vocab, tokens, logprob, entropy, top, top_ids, top_logprobs};
     if (threads == 1024) return top ? launch_log_probs<1024, true>(a, rows, blocks, stream) : launch_log_probs<1024, false>(a, rows, blocks, stream);
+    if (threads == 128) return top ? launch_log_probs<128, true>(a, rows, blocks, stream) : launch_log_probs<128, false>(a, rows, blocks, stream);
     if (threads == 256) return top ? launch_log_probs<256, true>(a, rows, blocks, stream) : launch_log_probs<256, false>(a, rows, blocks, stream);
     HOS_REFUSE("log_probs: blocks of %d threads", threads);
 }

@@ -5,7 +5,8 @@ common are read once for all of their rows, the others sequence by sequence, and
 bfloat16 keys and values; heads of a multiple of 16 numbers up to 256; any number of rows a sequence."""
 from __future__ import annotations
 
-from typing import Dict, List, Optional, Sequence
+import ctypes
+from typing import Dict, Optional, Sequence
 
 import numpy as np
 import torch
@@ -16,7 +17,7 @@ from ..errors import KernelError
 MAX_HEAD_DIM = 256
 OPEN = 1 << 30                 # a page behind every sequence's last
 ITEM_INTS = 12
-PAIRS = 16                     # (row, head) pairs of an item
+PAIRS, BLOCK = 16, 128         # (row, head) pairs of an item, of a big one
 MOST_PARTS = 64 << 20          # bytes of the parts that wait for the merge
 
 _libs: Dict[int, ops.Library] = {}
@@ -40,45 +41,58 @@ class SharedPlan:
     def __init__(self, group, runs, rows: Sequence[range], slots: Sequence[int], lengths: Sequence[int], n_rows: int):
         self.group, self.version = group, group.version
         self.runs, self.rows, self.slots, self.lengths, self.n_rows = runs, rows, slots, lengths, n_rows
-        self._work: Dict[tuple, "Work"] = {}
+        self._work: Dict[int, "Work"] = {}
 
     def work(self, n_heads: int) -> "Work":
         w = self._work.get(n_heads)
         if w is None:
             need = self.group.need
             made = lists(self.runs, self.rows, self.slots, self.lengths, self.n_rows, n_heads // need.n_kv_heads, need.n_kv_heads,
-                         need.head_dim, need.window)
-            w = self._work[n_heads] = Work(made, self.group.table_dev.device)
+                         need.head_dim, need.window, has_big(need.head_dim))
+            w = self._work[n_heads] = Work(made, self.group, n_heads)
         return w
 
 
 class Lists:
-    """Items, their rows, and each row's number of parts, on the host."""
+    """Items (of up to 16 pairs, then of up to 128), their rows, and each row's number of parts, on the host."""
 
-    def __init__(self, items: np.ndarray, rows: np.ndarray, n_parts: np.ndarray):
-        self.items, self.rows, self.n_parts = items, rows, n_parts
+    def __init__(self, items: np.ndarray, big: np.ndarray, rows: np.ndarray, n_parts: np.ndarray):
+        self.items, self.big, self.rows, self.n_parts = items, big, rows, n_parts
         self.parts = int(n_parts.max()) if n_parts.size else 0
 
 
-class Work:
-    """The lists on the device, in one array: the number of items, the rows' parts, the items, their rows."""
+class SharedWork(ctypes.Structure):
+    """A list of work as csrc/attention_shared.cu takes it."""
+    _fields_ = [(name, ctypes.c_void_p) for name in ("counts", "n_parts", "items", "big_items", "rows", "page_table")] + \
+               [(name, ctypes.c_int) for name in ("most", "big_most", "parts", "table_stride", "ring_pages", "n_heads", "n_kv_heads", "window")]
 
-    def __init__(self, made: Lists, device):
-        n_items, n = len(made.items), len(made.n_parts)
-        self.most, self.parts = n_items, made.parts
+
+class Work:
+    """The lists on the device, in one array: the numbers of items, the rows' parts, the items, their rows."""
+
+    def __init__(self, made: Lists, group, n_heads: int):
+        table, need = group.table_dev, group.need
+        n = len(made.n_parts)
         at = -(-(4 + n) // 4) * 4
-        flat = np.zeros(at + ITEM_INTS * n_items + len(made.rows), dtype=np.int32)
-        flat[0] = n_items
-        flat[4:4 + n] = made.n_parts
-        flat[at:at + ITEM_INTS * n_items] = made.items.reshape(-1)
-        flat[at + ITEM_INTS * n_items:] = made.rows
+        flat = np.concatenate([np.asarray([len(made.items), len(made.big), 0, 0], dtype=np.int32), made.n_parts, np.zeros(at - 4 - n, dtype=np.int32),
+                               made.items.reshape(-1), made.big.reshape(-1), made.rows])
         host = torch.from_numpy(flat)
-        if torch.device(device).type == "cuda":
+        if table.device.type == "cuda":
             host = host.pin_memory()
-        self.array = host.to(device, non_blocking=True)
+        self.array = host.to(table.device, non_blocking=True)
         self._host = host                                   # the copy reads it
         base = self.array.data_ptr()
-        self.count, self.n_parts, self.items, self.rows = base, base + 16, base + 4 * at, base + 4 * (at + ITEM_INTS * n_items)
+        items, big = base + 4 * at, base + 4 * (at + made.items.size)
+        self.parts = made.parts
+        self.fields = SharedWork(base, base + 16, items, big, big + 4 * made.big.size, table.data_ptr(), len(made.items), len(made.big), made.parts,
+                                 table.shape[1], group.ring_pages, n_heads, need.n_kv_heads, need.window or 0)
+        self.address = ctypes.addressof(self.fields)
+        self.floats = n * n_heads * made.parts * (need.head_dim + 2)
+
+
+def has_big(head_dim: int) -> bool:
+    """Whether blocks of up to 128 pairs have a kernel (tcgen05)."""
+    return head_dim in (64, 128, 256)
 
 
 def _pages(length: int, new: int, window: Optional[int]) -> tuple:
@@ -94,42 +108,47 @@ def share_pages(pages: Sequence[int], per_item: int) -> int:
 
 
 def lists(runs, rows: Sequence[range], slots: Sequence[int], lengths: Sequence[int], n_rows: int, per: int, kv: int, head_dim: int,
-          window: Optional[int]) -> Lists:
-    """The work: a run's rows in blocks of up to 16 pairs over the run's pages, each sequence's over the rest of its own."""
-    block = max(1, PAIRS // per)
+          window: Optional[int], big: bool) -> Lists:
+    """The work: a run's rows in blocks of up to 16 pairs, or of up to 128 where they are more and a kernel has such blocks (`big`), over
+    the run's pages, each sequence's over the rest of its own."""
+    big = big and per <= BLOCK
     chunks = -(-per // PAIRS)
     skip = [(0, 0)] * len(slots)
-    blocks = []                                              # (rows, slot, lp0, lp1, skip0, skip1, pages)
+    blocks = []                                              # (big, rows, slot, lp0, lp1, skip0, skip1, pages)
+
+    def cut(of: Sequence[int], *rest) -> None:
+        large = big and len(of) * per > PAIRS
+        size = max(1, (BLOCK if large else PAIRS) // per)
+        n = -(-len(of) // size)                              # blocks of like sizes
+        for i in range(n):
+            blocks.append((large, of[len(of) * i // n:len(of) * (i + 1) // n], *rest))
+
     for members, lo, hi in runs:
         seen = [_pages(lengths[i], len(rows[i]), window) for i in members]
         n = min(hi, max(b for _, b in seen)) - max(lo, min(a for a, _ in seen))
         if n <= 0:
             continue
-        of_run = [r for i in members for r in rows[i]]
         for i in members:
             skip[i] = (lo, hi)
-        for at in range(0, len(of_run), block):
-            blocks.append((of_run[at:at + block], slots[members[0]], lo, hi, OPEN, OPEN, n))
+        cut([r for i in members for r in rows[i]], slots[members[0]], lo, hi, OPEN, OPEN, n)
     for i, slot in enumerate(slots):
         a, b = _pages(lengths[i], len(rows[i]), window)
         lo, hi = skip[i]
-        n = b - a - max(0, min(b, hi) - max(a, lo))
-        for at in range(0, len(rows[i]), block):
-            blocks.append((rows[i][at:at + block], slot, 0, OPEN, lo, hi, max(1, n)))
-    share = share_pages([b[6] for b in blocks], kv * chunks)
+        cut(rows[i], slot, 0, OPEN, lo, hi, max(1, b - a - max(0, min(b, hi) - max(a, lo))))
+    share = share_pages([b[7] for b in blocks], kv * chunks)
     most = max(2, MOST_PARTS // max(1, 4 * n_rows * per * kv * (head_dim + 2)))
     n_parts = np.zeros(n_rows, dtype=np.int32)
-    items, listed = [], []
-    for of_block, slot, lp0, lp1, skip0, skip1, n in blocks:
+    made, listed = ([], []), []
+    for large, of_block, slot, lp0, lp1, skip0, skip1, n in blocks:
         splits = max(1, min(-(-n // share), most // 2))
         part = int(n_parts[of_block[0]])
         for s in range(splits):
-            items.append((len(listed), len(of_block), slot, lp0, lp1, skip0, skip1, s, splits, part + s, -(-n // splits), 0))
+            made[large].append((len(listed), len(of_block), slot, lp0, lp1, skip0, skip1, s, splits, part + s, -(-n // splits), 0))
         listed.extend(of_block)
         for r in of_block:
             n_parts[r] += splits
-    items.sort(key=lambda it: -it[10])                       # the longest first
-    return Lists(np.asarray(items, dtype=np.int32).reshape(-1, ITEM_INTS), np.asarray(listed, dtype=np.int32), n_parts)
+    items = [np.asarray(sorted(m, key=lambda it: -it[10]), dtype=np.int32).reshape(-1, ITEM_INTS) for m in made]      # the longest first
+    return Lists(items[0], items[1], np.asarray(listed, dtype=np.int32), n_parts)
 
 
 def plan(group, step) -> SharedPlan:
@@ -163,6 +182,8 @@ def attend(q: torch.Tensor, out: torch.Tensor, step, cache: ops.PagedKVArgs, pla
         raise KernelError("attention over shared pages takes a cache in bfloat16")
     if n_heads <= 0 or n_heads % kv:
         raise KernelError(f"attend: {n_heads} query heads over {kv} kv heads")
+    if not scale > 0.0:
+        raise KernelError(f"attend: a scale of {scale}")
     if q.shape[1] != n_heads * dim or out.shape != q.shape:
         raise KernelError(f"queries {tuple(q.shape)} and output {tuple(out.shape)} for {n_heads} heads of {dim}")
     if step.n_tokens != n or plan.n_rows != n:
@@ -174,16 +195,7 @@ def attend(q: torch.Tensor, out: torch.Tensor, step, cache: ops.PagedKVArgs, pla
         raise KernelError("attend: pages have changed since the plan was made")
     if n == 0:
         return
-    run(q, out, step.token_pos, cache, plan.work(n_heads), n_heads, scale, softcap, window)
-
-
-def run(q, out, token_pos, cache: ops.PagedKVArgs, work: Work, n_heads: int, scale: float, softcap: float, window: Optional[int]) -> None:
-    n, dim, parts = q.shape[0], cache.head_dim, work.parts
-    lib = lib_for(dim)
-    places = n * n_heads * parts
-    ws = torch.empty(places * (dim + 2), dtype=torch.float32, device=q.device)
-    part_o, part_ml, stream = ws.data_ptr(), ws.data_ptr() + 4 * places * dim, ops._stream()
-    lib.call("hos_attn_shared", q.data_ptr(), q.stride(0), token_pos.data_ptr(), work.items, work.count, work.most, work.rows,
-             cache.k_pages.data_ptr(), cache.v_pages.data_ptr(), cache.page_table.data_ptr(), cache.table_stride, cache.ring_pages, n_heads,
-             cache.n_kv_heads, dim, scale, softcap, window or 0, parts, part_o, part_ml, stream)
-    lib.call("hos_attn_shared_merge", part_o, part_ml, work.n_parts, parts, n, n_heads, out.data_ptr(), out.stride(0), stream)
+    work = plan.work(n_heads)
+    ws = torch.empty(work.floats, dtype=torch.float32, device=q.device)
+    lib_for(dim).call("hos_attn_shared", q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), n, step.token_pos.data_ptr(), cache.k_pages.data_ptr(),
+                      cache.v_pages.data_ptr(), cache.k_pages.shape[0], work.address, scale, softcap, ws.data_ptr(), ops._stream())

@@ -76,8 +76,11 @@ class Tree:
 
 def share_bound(v_abs, exact):
     """Bound on the difference of attention whose weights are rounded to bfloat16 and whose sums are 32-bit, rounded to bfloat16 at
-    the end.  A weight is off by 2^-9 of itself at most from its rounding and by e from its score's: a score of 256 products rounded
-    at 32 bits, its soft-cap through an exponential, together under 2^-13 of what a score may be (8 here): e < 2^-10.  Both act on the
-    weighted mean of |v| over the keys, which `v_abs` gives, numerator and denominator: (2^-9 + 2 * 2^-10) v_abs = 2^-8 v_abs; the result's
-    own rounding: 2^-9 of it, and sums of 32 bits 2^-15 of v_abs."""
-    return (2.0 ** -8 + 2.0 ** -15) * v_abs + 2.0 ** -9 * exact.abs()
+    the end.  bfloat16 keeps 8 bits: a rounding is off by half a step, torch.finfo(torch.bfloat16).eps / 2 = 2^-8 of the number (1 + 2^-8 lies
+    in the middle between 1 and its neighbour 1 + 2^-7).  A weight is off by 2^-8 of itself from its rounding and by e from its score's: a
+    score of 256 products rounded at 32 bits, its soft-cap through an exponential, together under 2^-13 of what a score may be (8 here):
+    e < 2^-10.  The rounding acts on the numerator alone (the sum of weights is of the unrounded), e on both, each on the weighted mean of
+    |v| over the keys, which `v_abs` gives: (2^-8 + 2 * 2^-10) v_abs; the result's own rounding: 2^-8 of it, and sums of 32 bits 2^-15 of
+    v_abs."""
+    half_step = torch.finfo(torch.bfloat16).eps / 2
+    return (half_step + 2 * 2.0 ** -10 + 2.0 ** -15) * v_abs + half_step * exact.abs()

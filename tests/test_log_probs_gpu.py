@@ -60,7 +60,7 @@ def test_scores(rows, vocab, top, kind):
     check(log_probs(x, t, top), plain(x, t, top))
 
 
-@pytest.mark.parametrize("blocks,threads", [(1, 256), (2, 256), (8, 256), (1, 1024), (4, 1024)])
+@pytest.mark.parametrize("blocks,threads", [(1, 128), (8, 128), (1, 256), (2, 256), (8, 256), (1, 1024), (4, 1024)])
 def test_every_cut_of_a_row_gives_the_same_tokens(blocks, threads, monkeypatch):
     monkeypatch.setattr(ops, "log_probs_blocks", lambda r, v: (threads, blocks))
     g = torch.Generator().manual_seed(5)

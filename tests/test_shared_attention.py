@@ -110,13 +110,13 @@ def test_every_key_that_a_row_sees_is_in_one_of_its_items(seed):
     step = t.step(which, news)
     plan = sa.plan(t.group, step)
     per = rng.choice([1, 2, 3, 5, 16, 20])
-    made = sa.lists(plan.runs, plan.rows, plan.slots, plan.lengths, plan.n_rows, per, 2, 64, window)
+    made = sa.lists(plan.runs, plan.rows, plan.slots, plan.lengths, plan.n_rows, per, 2, 64, window, rng.random() < 0.5)
     pos, seq = step.token_pos.tolist(), step.token_seq.tolist()
     seen = [dict() for _ in pos]
     parts = [set() for _ in pos]
-    for row0, n_rows, slot, lp0, lp1, skip0, skip1, share, n_shares, part, _, _ in made.items.tolist():
+    for j, (row0, n_rows, slot, lp0, lp1, skip0, skip1, share, n_shares, part, _, _) in enumerate(made.items.tolist() + made.big.tolist()):
         rows = made.rows[row0:row0 + n_rows].tolist()
-        assert n_rows * min(per, 16) <= 16 or n_rows == 1
+        assert n_rows * per <= 128 if j >= len(made.items) else n_rows * min(per, 16) <= 16 or n_rows == 1
         lo = min(max(0, pos[r] + 1 - window) // PAGE if window else 0 for r in rows)
         hi = max(pos[r] // PAGE for r in rows)
         pages = [p for p in range(max(lp0, lo), min(lp1, hi + 1)) if not skip0 <= p < skip1]

@@ -66,6 +66,29 @@ def test_pieces_of_several_rows(dim, per, window, news):
     compare(t, all_, list(news), 2 * per, cap=50.0)
 
 
+@pytest.mark.parametrize("dim,kv,per,forks", [(64, 2, 1, 63), (64, 1, 8, 40), (128, 2, 2, 63), (128, 1, 5, 30), (256, 2, 2, 63), (256, 1, 16, 20), (64, 1, 100, 3), (128, 1, 128, 2)])
+@pytest.mark.parametrize("prefix,cap", [(1, 0.0), (700, 50.0), (1500, 0.0)])
+def test_many_forks(dim, kv, per, forks, prefix, cap):
+    t = Tree(kv, dim, seed=forks + prefix)
+    a = t.new(prefix)
+    all_ = [a] + t.fork(a, forks)
+    for j, i in enumerate(all_):
+        t.bring([i], [1 + (37 * j) % 130])
+    plan = compare(t, all_, [1] * len(all_), per * kv, cap=cap)
+    assert prefix < 64 or plan.work(per * kv).fields.big_most > 0
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_windows_of_many_rows_cut_pages_at_both_ends(dim):
+    t = Tree(2, dim, window=150, chunk=64, seed=dim)
+    a = t.new(310)
+    all_ = [a] + t.fork(a, 39)
+    for j, i in enumerate(all_):
+        for _ in range(1 + j % 4):
+            t.bring([i], [1 + (13 * j) % 50])
+    compare(t, all_, [1] * 40, 8, cap=50.0)
+
+
 def test_a_tree_of_forks_in_no_order_with_strangers():
     t = Tree(2, 128, seed=9)
     a, x = t.new(300), t.new(77)
@@ -142,10 +165,10 @@ def test_refusals():
     t.bring([a, f], [1, 1])
     step, q = t.step([a, f], [1, 1]), torch.zeros(2, 256, dtype=torch.bfloat16, device="cuda")
     plan = sa.plan(t.group, step)
-    for bad in (dict(q=q.float()), dict(q=q[:1]), dict(n_heads=3), dict(n_heads=2), dict(out=q[:, :128]), dict(window=64), dict(out=q.float()), dict(n_heads=0)):
-        k = dict(dict(q=q, out=q.clone(), n_heads=4, window=None), **bad)
+    for bad in (dict(q=q.float()), dict(q=q[:1]), dict(n_heads=3), dict(n_heads=2), dict(out=q[:, :128]), dict(window=64), dict(out=q.float()), dict(n_heads=0), dict(scale=0.0), dict(scale=-1.0)):
+        k = dict(dict(q=q, out=q.clone(), n_heads=4, window=None, scale=1.0), **bad)
         with pytest.raises(KernelError):
-            sa.attend(k["q"], k["out"], step, t.view, plan, k["n_heads"], 1.0, 0.0, k["window"])
+            sa.attend(k["q"], k["out"], step, t.view, plan, k["n_heads"], k["scale"], 0.0, k["window"])
     with pytest.raises(KernelError, match="16 bytes"):
         sa.attend(torch.zeros(2, 257, dtype=torch.bfloat16, device="cuda")[:, 1:], q.clone(), step, t.view, plan, 4, 1.0)
     t.bring([f], [64])
