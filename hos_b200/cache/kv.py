@@ -190,15 +190,35 @@ class KVGroup:
         """Where sequences of these lengths share pages: [(places in `slots`, first logical page, the page behind the last)], each
         place in one run at most, the runs chosen so that the fewest pages are read when a run's are read once.  In a ring only what
         all of a run's sequences still hold counts.  A run stays true until one of the slots' pages changes (`version`)."""
-        if not self._holders:
+        if not self._holders or len(slots) < 2:
             return []
-        held = [self._slot_pages[s] for s in slots]
-        several = np.fromiter(self._holders, dtype=np.int64, count=len(self._holders))
-        # sequences that hold a shared page in common, directly or by way of others, are looked at together
-        counts = [len(h) for h in held]
-        flat = np.fromiter((p for h in held for p in h), dtype=np.int64, count=sum(counts))
-        owner = np.repeat(np.arange(len(slots)), counts)
-        mine = np.isin(flat, several)
+        last = (np.asarray(lengths, dtype=np.int64) - 1) // PAGE
+        out: List[tuple] = []
+        for members in self._families(slots, last):
+            lo, hi = 0, int(last[members].min()) + 1
+            if self.ring_pages:
+                lo = max(0, int(last[members].max()) - self.ring_pages + 1)             # what the longest has not written over
+            if hi <= lo:
+                continue
+            entries = np.arange(lo, hi)
+            if self.ring_pages:
+                entries %= self.ring_pages
+            table = self._table_np[np.asarray([slots[i] for i in members])][:, entries]
+            out += [(m, lo, lo + n) for m, n in _best_runs(table, members)[1]]
+        return out
+
+    def _families(self, slots: Sequence[int], last: np.ndarray) -> List[List[int]]:
+        """Places of sequences that may share pages.  Sequences that share one share all before it: its first page, or, in a ring, the
+        first that all of them still hold.  Where there is none (lengths too unlike), those that hold a page in common, directly or by way
+        of others, are a family."""
+        at = max(0, int(last.max()) - self.ring_pages + 1) if self.ring_pages else 0
+        if at <= int(last.min()):
+            first = self._table_np[np.asarray(slots), at % self.ring_pages if self.ring_pages else 0].tolist()
+            by_page: Dict[int, List[int]] = {}
+            for i, page in enumerate(first):
+                if page in self._holders:
+                    by_page.setdefault(page, []).append(i)
+            return [m for m in by_page.values() if len(m) > 1]
         kin = list(range(len(slots)))
 
         def root(i: int) -> int:
@@ -207,29 +227,15 @@ class KVGroup:
                 i = kin[i]
             return i
 
-        first: Dict[int, int] = {}
-        for page, i in zip(flat[mine].tolist(), owner[mine].tolist()):
-            j = first.setdefault(page, i)
-            if j != i:
-                kin[root(i)] = root(j)
+        seen: Dict[int, int] = {}
+        for i, s in enumerate(slots):
+            for page in self._slot_pages[s]:
+                if page in self._holders:
+                    kin[root(i)] = root(seen.setdefault(page, i))
         families: Dict[int, List[int]] = {}
-        for i in sorted(set(owner[mine].tolist())):
+        for i in range(len(slots)):
             families.setdefault(root(i), []).append(i)
-        out: List[tuple] = []
-        for members in families.values():
-            if len(members) < 2:
-                continue
-            last = [(lengths[i] - 1) // PAGE for i in members]
-            lo, hi = 0, min(last) + 1
-            if self.ring_pages:
-                lo = max(0, max(last) - self.ring_pages + 1)             # what the longest has not written over
-            if hi <= lo:
-                continue
-            entries = np.arange(lo, hi)
-            if self.ring_pages:
-                entries %= self.ring_pages
-            out += [(m, lo, lo + n) for m, n in _best_runs(self._table_np[np.asarray([slots[i] for i in members])][:, entries], members)[1]]
-        return out
+        return [m for m in families.values() if len(m) > 1]
 
     def compact(self) -> int:
         """Move the held pages to the front of the arrays; the number of them."""

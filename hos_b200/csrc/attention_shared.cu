@@ -2,16 +2,16 @@
 //
 // The work is a list of items made on the host (parts/shared_attention.py).  An item is a block of rows of the step, a row of the page
 // table through which all of them read, and a range of that table's logical pages: the pages that the block's sequences share, or
-// the pages that a sequence has for itself (its range without the shared part).  A block's (row, query head) pairs of one kv head, up
-// to 16, are the columns of the products S^T = K Q^T and O^T = V^T P^T (m16n8k16, bfloat16, sums in 32 bits), so a page's keys and
-// values are read from shared memory once for all pairs.  Masks are a pair's own: keys up to its row's position, the last `window` of
-// them; pages outside what any of the rows sees are left out, by the positions on the device, so a list stays right while rows move on.
-// Every item leaves unnormalised sums with their maximum and sum of weights, a part of each of its rows; attn_shared_merge_kernel joins a
-// row's parts:  m = max m_i,  out = sum e^(m_i - m) o_i / sum e^(m_i - m) l_i.
+// the pages that a sequence has for itself (its range without the shared part).  Masks are a (row, query head) pair's own: keys up to
+// its row's position, the last `window` of them; pages outside what any of the rows sees are left out, by the positions on the device,
+// so a list stays right while rows move on.  Every item leaves unnormalised sums with their maximum and sum of weights, a part of each of
+// its rows; attn_shared_merge_kernel joins a row's parts:  m = max m_i,  out = sum e^(m_i - m) o_i / sum e^(m_i - m) l_i.
 //
-// The walk is persistent, a CTA an SM: a producer warp brings pages by bulk copies through a ring, over the borders of items, four
-// consumer warps take 16 keys of a page each.  Weights are rounded to bfloat16 for the product with the values (2^-8 of each at most), their sum
-// is of the weights before that rounding.
+// Items of up to 8 pairs: the pairs are the columns of the products S^T = K Q^T and O^T = V^T P^T (m16n8k16, bfloat16, sums in 32 bits).
+// The walk is persistent: a producer warp brings pages by bulk copies through a ring, over the borders of items, two groups of four
+// consumer warps take the items in turn, 16 keys of a page a warp, so that what an item costs besides its pages passes under the
+// other group's pages.  Items of up to 128 pairs: tcgen05, further down.  Weights are rounded to bfloat16 for the product with the
+// values (2^-8 of each at most), their sum is of the weights before that rounding.
 //
 // Compiled per head size: -DHOS_HEAD_DIM=N, a multiple of 16 up to 256.
 #include "common.cuh"
@@ -28,24 +28,30 @@ namespace hos {
 constexpr int HD = HOS_HEAD_DIM;
 static_assert(HD % 16 == 0 && HD >= 16 && HD <= 256, "head_dim must be a multiple of 16, at most 256");
 constexpr int kGiveUpAttnShared = 7;
-constexpr int kPairs = 16;                                   // pairs of an item
+constexpr int kPairs = 8;                                    // pairs of a small item
 constexpr int kTileBytes = kPageTokens * HD * 2;             // a page's keys of a kv head, or its values
-constexpr int kConsumers = 128;
-constexpr int kThreads = kConsumers + 32;
+constexpr int kGroups = 2, kConsumers = 128;                 // groups of consumers, threads of one
+constexpr int kThreads = kGroups * kConsumers + 32;
+constexpr int kCtasPerSm = HD <= 128 ? 2 : 1;                // as registers and shared memory allow
 constexpr long long kWaitCycles = 1ll << 31;                 // about a second
-constexpr int kSumsBytes = 4 * kPairs * (HD + 4) * 4;       // the four warps' sums (rows of HD + 4 numbers: no conflicts)
-constexpr int kStagesFit = (225 * 1024 - kPairs * HD * 2 - kSumsBytes) / (2 * kTileBytes);
+constexpr int kGroupBytes = kPairs * HD * 2 + 4 * kPairs * (HD + 4) * 4 + 4 * kPairs * 8 + kPairs * 16;      // queries, the warps' sums (rows of
+                                                             // HD + 4 numbers: no conflicts), their maxima and sums of weights, the pairs
+constexpr int kStagesFit = (225 * 1024 / kCtasPerSm - 1024 - kGroups * kGroupBytes - 1024) / (2 * kTileBytes);
 constexpr int kStages = kStagesFit < 6 ? kStagesFit : 6;
+constexpr int kShared = kStages * 2 * kTileBytes + kGroups * kGroupBytes + (2 * kGroups + 2) * kStages * 8;
+static_assert(kStages >= 2, "shared memory of the small items' ring");
 
-struct SharedItem {                                          // as parts/shared_attention.py writes it
-    int row0, n_rows;          // places in the list of rows
+struct __align__(16) SharedItem {                            // as parts/shared_attention.py writes it
+    int row0, n_rows;          // places in the list of rows (big items)
     int slot;                  // row of the page table
     int lp0, lp1;              // logical pages, lp1 exclusive ...
     int skip0, skip1;          // ... without these
     int share, n_shares;       // which of so many shares of what is left of them
     int part;                  // which part of its rows the item leaves
     int pad0, pad1;
+    int rows[kPairs];          // a small item's rows
 };
+constexpr int kOpen = 1 << 30;                               // lp1 of an item that goes up to its rows' positions
 
 struct SharedArgs {
     const bf16* q;
@@ -60,6 +66,7 @@ struct SharedArgs {
     float2* part_ml;           // [rows][heads][parts] (maximum, sum of weights)
     float scale, cap;
     int window;
+    int beside_big;            // the small items run beside the big ones' kernel, which was launched just before
 };
 
 __device__ int* g_shared_error_host = nullptr;
@@ -72,25 +79,14 @@ __device__ __forceinline__ void record_give_up() {
     }
 }
 
-// The pages of an item, by the positions of its rows: every warp for itself.
+// The pages of an item, by the lowest and the highest position of its rows.
 struct Walk {
     int first, count1, second, n;          // logical pages first .. first + count1 - 1, then second ..
     int begin, end;                        // the share's part of them
-    int all_from, all_to;                  // the keys that every row sees
 };
-__device__ __forceinline__ Walk walk_of(const SharedArgs& a, const SharedItem& it, int lane) {
-    int low = 0x7fffffff, high = -1;       // the lowest and the highest position of a row
-    for (int r = lane; r < it.n_rows; r += 32) {
-        const int pos = a.token_pos[a.rows[it.row0 + r]];
-        low = min(low, pos);
-        high = max(high, pos);
-    }
-    low = __reduce_min_sync(0xffffffffu, low);
-    high = __reduce_max_sync(0xffffffffu, high);
+__device__ __forceinline__ Walk walk_of(const SharedArgs& a, const SharedItem& it, int low, int high) {
     const int from = max(it.lp0, a.window > 0 ? max(0, low + 1 - a.window) / kPageTokens : 0), to = min(it.lp1, high / kPageTokens + 1);
     Walk w;
-    w.all_from = a.window > 0 ? max(0, high + 1 - a.window) : 0;
-    w.all_to = low;
     w.first = from;
     w.count1 = max(0, min(to, it.skip0) - from);
     w.second = max(from, it.skip1);
@@ -101,72 +97,77 @@ __device__ __forceinline__ Walk walk_of(const SharedArgs& a, const SharedItem& i
     return w;
 }
 __device__ __forceinline__ int walk_page(const Walk& w, int i) { return i < w.count1 ? w.first + i : w.second + (i - w.count1); }
+// A small item's walk.  A closed range without a window needs no position: its pages lie below every row's.
+__device__ __forceinline__ Walk small_walk(const SharedArgs& a, const SharedItem& it, int lane) {
+    int low = 0, high = kOpen;
+    if (a.window > 0 || it.lp1 >= kOpen) {
+        const int pos = lane < it.n_rows ? a.token_pos[it.rows[lane & 7]] : -1;
+        low = __reduce_min_sync(0xffffffffu, lane < it.n_rows ? pos : kOpen);
+        high = __reduce_max_sync(0xffffffffu, pos);
+    }
+    return walk_of(a, it, low, high);
+}
 
-struct SharedSmem {
-    static constexpr int kRing = kStages * 2 * kTileBytes;
-    static constexpr int kQ = kPairs * HD * 2;
-    static constexpr int kTotal = kRing + kQ + kSumsBytes + 4 * kPairs * 8 + kPairs * 16 + 4 * kStages * 8;
-};
-
-__global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(SharedArgs a) {
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) attn_shared_kernel(SharedArgs a) {
     extern __shared__ __align__(128) unsigned char smem[];
     unsigned char* ring = smem;                                                 // stage: keys, values
-    bf16* q_s = reinterpret_cast<bf16*>(smem + SharedSmem::kRing);              // [16][HD], permuted like the pages
-    float* sums = reinterpret_cast<float*>(smem + SharedSmem::kRing + SharedSmem::kQ);        // [4][16][HD + 4]
-    float2* ml = reinterpret_cast<float2*>(reinterpret_cast<unsigned char*>(sums) + kSumsBytes);      // [4][16]
-    int4* pair_of = reinterpret_cast<int4*>(ml + 4 * kPairs);                   // [16]: row, head, lowest key, position
-    uint64_t* k_full = reinterpret_cast<uint64_t*>(pair_of + kPairs);
-    uint64_t* v_full = k_full + kStages;
-    uint64_t* k_empty = v_full + kStages;
+    uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + kStages * 2 * kTileBytes + kGroups * kGroupBytes);      // [groups][stages]: a group
+    uint64_t* v_full = k_full + kGroups * kStages;                              // knows its phases by its own tiles
+    uint64_t* k_empty = v_full + kGroups * kStages;
     uint64_t* v_empty = k_empty + kStages;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
+    const int warp = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31, tid = threadIdx.x & (kConsumers - 1), who = threadIdx.x / kConsumers;
     const int group = a.n_heads / a.cache.n_kv_heads;
-    const int chunks = (group + kPairs - 1) / kPairs;        // sixteens of query heads that share a kv head
-    if (tid == 0) {
-        for (int s = 0; s < kStages; ++s) {
-            mbar_init(&k_full[s], 1); mbar_init(&v_full[s], 1);
-            mbar_init(&k_empty[s], 4); mbar_init(&v_empty[s], 4);
-        }
+    const int chunks = (group + kPairs - 1) / kPairs;        // eights of query heads that share a kv head
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kGroups * kStages; ++s) { mbar_init(&k_full[s], 1); mbar_init(&v_full[s], 1); }
+        for (int s = 0; s < kStages; ++s) { mbar_init(&k_empty[s], 4); mbar_init(&v_empty[s], 4); }
         mbar_fence_init();
     }
     __syncthreads();
-    pdl_enter();
+    // The big items' kernel lets this one start when all of its blocks have, which is after everything before them is complete; the two write
+    // other parts.  This one ends after it, so that what waits for this one waits for both.
+    if (!a.beside_big) pdl_wait();
+    pdl_launch_dependents();
     const int per_item = a.cache.n_kv_heads * chunks;
     const int n_work = *a.n_items * per_item;
+    // the work of a CTA: a round forwards, the next backwards, as the longest items come first
+    auto work_at = [&](int round) { return round & 1 ? (round + 1) * (int)gridDim.x - 1 - (int)blockIdx.x : round * (int)gridDim.x + (int)blockIdx.x; };
 
-    if (warp == 4) {
+    if (who == kGroups) {
         // ---------------- producer ----------------
         const bf16* k_pages = reinterpret_cast<const bf16*>(a.cache.k_pages);
         const bf16* v_pages = reinterpret_cast<const bf16*>(a.cache.v_pages);
         int t = 0;
         bool ok = true;
-        for (int work = blockIdx.x; work < n_work && ok; work += gridDim.x) {
-            const SharedItem it = a.items[work / per_item];
-            const int kvh = work % per_item / chunks;
-            const Walk w = walk_of(a, it, lane);
+        for (int round = 0; round * (int)gridDim.x < n_work && ok; ++round) {
+            const int work = work_at(round);
+            if (work >= n_work) continue;
+            const SharedItem& it = a.items[work / per_item];
+            const int kvh = work % per_item / chunks, to = round % kGroups * kStages;
+            const Walk w = small_walk(a, it, lane);
             const int* table = a.cache.page_table + (size_t)it.slot * a.cache.table_stride;
             for (int i0 = w.begin; i0 < w.end && ok; i0 += 32) {             // 32 pages looked up at a time
                 const int page_l = i0 + lane < w.end ? table[kv_table_entry(a.cache, walk_page(w, i0 + lane))] : 0;
                 const int n = min(32, w.end - i0);
-                for (int i = 0; i < n; ++i, ++t) {
+                for (int i = 0; i < n && ok; ++i, ++t) {
                     const int page = __shfl_sync(0xffffffffu, page_l, i);
                     if (lane == 0) {
                         const int s = t % kStages;
+                        const uint32_t parity = ((t / kStages) - 1) & 1;
                         const size_t off = kv_tile_offset(a.cache, page, kvh);
                         unsigned char* dst = ring + (size_t)s * 2 * kTileBytes;
-                        if (t >= kStages) ok = mbar_wait_cycles(&k_empty[s], ((t / kStages) - 1) & 1, kWaitCycles);
+                        if (t >= kStages) ok = mbar_wait_cycles(&k_empty[s], parity, kWaitCycles);
                         if (ok) {
-                            mbar_expect_tx(&k_full[s], kTileBytes);
-                            bulk_g2s(dst, k_pages + off, kTileBytes, &k_full[s]);
-                            if (t >= kStages) ok = mbar_wait_cycles(&v_empty[s], ((t / kStages) - 1) & 1, kWaitCycles);
+                            mbar_expect_tx(&k_full[to + s], kTileBytes);
+                            bulk_g2s(dst, k_pages + off, kTileBytes, &k_full[to + s]);
+                            if (t >= kStages) ok = mbar_wait_cycles(&v_empty[s], parity, kWaitCycles);
                         }
                         if (ok) {
-                            mbar_expect_tx(&v_full[s], kTileBytes);
-                            bulk_g2s(dst + kTileBytes, v_pages + off, kTileBytes, &v_full[s]);
+                            mbar_expect_tx(&v_full[to + s], kTileBytes);
+                            bulk_g2s(dst + kTileBytes, v_pages + off, kTileBytes, &v_full[to + s]);
                         }
                     }
                     ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-                    if (!ok) break;
                 }
             }
         }
@@ -174,103 +175,107 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(SharedArgs a) 
             if (lane == 0) record_give_up();
             let_work_under_way_end();
         }
+        if (a.beside_big) pdl_wait();
         return;
     }
 
     // ---------------- consumers ----------------
+    unsigned char* own = smem + kStages * 2 * kTileBytes + who * kGroupBytes;
+    bf16* q_s = reinterpret_cast<bf16*>(own);                                   // [8][HD], permuted like the pages
+    float* sums = reinterpret_cast<float*>(own + kPairs * HD * 2);              // [4][8][HD + 4]
+    float2* ml = reinterpret_cast<float2*>(sums + 4 * kPairs * (HD + 4));       // [4][8]
+    int4* pair_of = reinterpret_cast<int4*>(ml + 4 * kPairs);                   // [8]: row, head, lowest key, position
+    k_full += who * kStages;
+    v_full += who * kStages;
     const int g = lane >> 2, t4 = lane & 3;
     const float inv_cap = a.cap > 0.f ? 1.f / a.cap : 0.f;
     const uint32_t q_base = smem_u32(q_s);
     const int upper = (lane >> 3) & 1, right = lane >> 4;
     const int k_row = warp * 16 + (lane & 7) + upper * 8, v_row = warp * 16 + (lane & 7) + right * 8;
-    const int q_row = (lane & 7) + right * 8;
-    int t = 0;
+    int t = 0;                               // tiles of the items so far, this group's and the other's
+    uint32_t phases = 0;                     // bit s: the parity of this group's next tile in stage s
     bool ok = true;
-    auto meet = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
-    for (int work = blockIdx.x; work < n_work; work += gridDim.x) {
-        const SharedItem it = a.items[work / per_item];
+    auto meet = [&] { asm volatile("bar.sync %0, 128;" ::"r"(1 + who) : "memory"); };
+    for (int round = 0; round * (int)gridDim.x < n_work; ++round) {
+        const int work = work_at(round);
+        if (work >= n_work) continue;
+        const SharedItem& it = a.items[work / per_item];
         const int kvh = work % per_item / chunks, chunk = work % per_item % chunks;
-        const int heads = min(kPairs, group - chunk * kPairs);           // of a row
-        const int pairs = min(kPairs, it.n_rows * heads);
-        const Walk w = walk_of(a, it, lane);
-        meet();                                              // the last item's readers are done
+        const Walk w = small_walk(a, it, lane);
+        if (round % kGroups != who) {        // the other group's
+            t += w.end - w.begin;
+            continue;
+        }
+        const int heads = min(kPairs, group - chunk * kPairs), pairs = min(kPairs, it.n_rows * heads), part = it.part;
+        meet();                              // the last item's readers are done
         if (tid < kPairs) {
-            const int row = a.rows[it.row0 + min(tid / heads, it.n_rows - 1)];
+            const int row = it.rows[min(tid / heads, it.n_rows - 1)];
             const int pos = tid < pairs ? a.token_pos[row] : -1;
             pair_of[tid] = make_int4(row, kvh * group + chunk * kPairs + tid % heads, a.window > 0 ? max(0, pos + 1 - a.window) : 0, pos);
         }
-        meet();
         for (int i = tid; i < kPairs * (HD / 8); i += kConsumers) {
             const int p = i / (HD / 8), c = i % (HD / 8);
             uint4 v = make_uint4(0, 0, 0, 0);
-            if (p < pairs) v = *reinterpret_cast<const uint4*>(a.q + (size_t)pair_of[p].x * a.q_stride + (size_t)pair_of[p].y * HD + c * 8);
+            if (p < pairs)
+                v = *reinterpret_cast<const uint4*>(a.q + (size_t)it.rows[p / heads] * a.q_stride + (size_t)(kvh * group + chunk * kPairs + p % heads) * HD + c * 8);
             *reinterpret_cast<uint4*>(q_s + tile_chunk_offset<HD>(p, c)) = v;
         }
         meet();
-        const bool two = pairs > 8;                          // columns 8 to 15 are in use
-        int lo[2][2], hi[2][2];
+        uint32_t qf[HD / 16][2];
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+        for (int kk = 0; kk < HD / 16; ++kk) ldmatrix_x2(qf[kk], q_base + 2 * tile_chunk_offset<HD>(lane & 7, kk * 2 + upper));
+        int lo[2], hi[2];
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int4 p = pair_of[8 * x + 2 * t4 + r];
-                lo[x][r] = p.z;
-                hi[x][r] = p.w;
-            }
-        float m_run[2][2] = {{-INFINITY, -INFINITY}, {-INFINITY, -INFINITY}}, l_run[2][2] = {};
-        float o[HD / 16][2][4] = {};
+        for (int r = 0; r < 2; ++r) {
+            const int4 p = pair_of[2 * t4 + r];
+            lo[r] = p.z;
+            hi[r] = p.w;
+        }
+        float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+        float o[HD / 16][4] = {};
 
         for (int i = w.begin; i < w.end; ++i, ++t) {
             const int s = t % kStages;
-            const uint32_t parity = (t / kStages) & 1;
+            const uint32_t parity = (phases >> s) & 1;
+            phases ^= 1u << s;
             const uint32_t k_base = smem_u32(ring + (size_t)s * 2 * kTileBytes), v_base = k_base + kTileBytes;
             if (ok) ok = mbar_wait_cycles(&k_full[s], parity, kWaitCycles);
             ok = __all_sync(0xffffffffu, ok) != 0;
             if (!ok) continue;
-            float sc[2][4] = {}, sd[2][4] = {};              // two sums of every score, so that a chain is half as long
+            float sc[4] = {}, sd[4] = {};                    // two sums of every score, so that a chain is half as long
 #pragma unroll
             for (int kk = 0; kk < HD / 16; ++kk) {
-                uint32_t kb[4], qb[4];
+                uint32_t kb[4];
                 ldmatrix_x4(kb, k_base + 2 * tile_chunk_offset<HD>(k_row, kk * 2 + right));
-                ldmatrix_x4(qb, q_base + 2 * tile_chunk_offset<HD>(q_row, kk * 2 + upper));
-                auto& to = kk & 1 ? sd : sc;
-                mma_bf16(to[0], kb, qb[0], qb[1]);
-                if (two) mma_bf16(to[1], kb, qb[2], qb[3]);
+                mma_bf16(kk & 1 ? sd : sc, kb, qf[kk][0], qf[kk][1]);
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&k_empty[s]);
             const int key0 = walk_page(w, i) * kPageTokens + warp * 16;
-            uint32_t pb[2][2];
-            float corr[2][2];
+            float m_new[2] = {m_run[0], m_run[1]}, corr[2];
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                if (x == 1 && !two) break;
-                float m_new[2] = {m_run[x][0], m_run[x][1]};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int key = key0 + g + 8 * (j >> 1), r = j & 1;
-                    float v = softcap_fast((sc[x][j] + sd[x][j]) * a.scale, a.cap, inv_cap);
-                    v = key >= lo[x][r] && key <= hi[x][r] ? v : -INFINITY;
-                    sc[x][j] = v;
-                    m_new[r] = fmaxf(m_new[r], v);
-                }
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-#pragma unroll
-                    for (int y = 4; y < 32; y <<= 1) m_new[r] = fmaxf(m_new[r], __shfl_xor_sync(0xffffffffu, m_new[r], y));
-                    const float use = m_new[r] == -INFINITY ? 0.f : m_new[r];
-                    corr[x][r] = __expf(m_run[x][r] - use);
-                    m_run[x][r] = m_new[r];
-                    l_run[x][r] *= corr[x][r];
-#pragma unroll
-                    for (int j = r; j < 4; j += 2) {
-                        sc[x][j] = __expf(sc[x][j] - use);
-                        l_run[x][r] += sc[x][j];
-                    }
-                }
-                pb[x][0] = transposed_8x8(pack_bf16(sc[x][0], sc[x][1]));
-                pb[x][1] = transposed_8x8(pack_bf16(sc[x][2], sc[x][3]));
+            for (int j = 0; j < 4; ++j) {
+                const int key = key0 + g + 8 * (j >> 1), r = j & 1;
+                float v = softcap_fast((sc[j] + sd[j]) * a.scale, a.cap, inv_cap);
+                v = key >= lo[r] && key <= hi[r] ? v : -INFINITY;
+                sc[j] = v;
+                m_new[r] = fmaxf(m_new[r], v);
             }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+#pragma unroll
+                for (int y = 4; y < 32; y <<= 1) m_new[r] = fmaxf(m_new[r], __shfl_xor_sync(0xffffffffu, m_new[r], y));
+                const float use = m_new[r] == -INFINITY ? 0.f : m_new[r];
+                corr[r] = __expf(m_run[r] - use);
+                m_run[r] = m_new[r];
+                l_run[r] *= corr[r];
+#pragma unroll
+                for (int j = r; j < 4; j += 2) {
+                    sc[j] = __expf(sc[j] - use);
+                    l_run[r] += sc[j];
+                }
+            }
+            const uint32_t pb[2] = {transposed_8x8(pack_bf16(sc[0], sc[1])), transposed_8x8(pack_bf16(sc[2], sc[3]))};
             if (ok) ok = mbar_wait_cycles(&v_full[s], parity, kWaitCycles);
             ok = __all_sync(0xffffffffu, ok) != 0;
             if (!ok) continue;
@@ -279,13 +284,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(SharedArgs a) 
                 uint32_t va[4];
                 ldmatrix_x4_trans(va, v_base + 2 * tile_chunk_offset<HD>(v_row, dd * 2 + upper));
 #pragma unroll
-                for (int j = 0; j < 4; ++j) o[dd][0][j] *= corr[0][j & 1];
-                mma_bf16(o[dd][0], va, pb[0][0], pb[0][1]);
-                if (two) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) o[dd][1][j] *= corr[1][j & 1];
-                    mma_bf16(o[dd][1], va, pb[1][0], pb[1][1]);
-                }
+                for (int j = 0; j < 4; ++j) o[dd][j] *= corr[j & 1];
+                mma_bf16(o[dd], va, pb[0], pb[1]);
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&v_empty[s]);
@@ -293,22 +293,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(SharedArgs a) 
 
         // ---- the four warps' sums, each of other keys, are added and leave ----
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+        for (int r = 0; r < 2; ++r) {
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
+            for (int y = 4; y < 32; y <<= 1) l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], y);
+            const int p = 2 * t4 + r;
+            if (p < pairs) {
+                float* b = sums + (size_t)(warp * kPairs + p) * (HD + 4);
 #pragma unroll
-                for (int y = 4; y < 32; y <<= 1) l_run[x][r] += __shfl_xor_sync(0xffffffffu, l_run[x][r], y);
-                const int p = 8 * x + 2 * t4 + r;
-                if (p < pairs) {
-                    float* b = sums + (size_t)(warp * kPairs + p) * (HD + 4);
-#pragma unroll
-                    for (int dd = 0; dd < HD / 16; ++dd) {
-                        b[dd * 16 + g] = o[dd][x][r];
-                        b[dd * 16 + g + 8] = o[dd][x][2 + r];
-                    }
-                    if (g == 0) ml[warp * kPairs + p] = make_float2(m_run[x][r], l_run[x][r]);
+                for (int dd = 0; dd < HD / 16; ++dd) {
+                    b[dd * 16 + g] = o[dd][r];
+                    b[dd * 16 + g + 8] = o[dd][2 + r];
                 }
+                if (g == 0) ml[warp * kPairs + p] = make_float2(m_run[r], l_run[r]);
             }
+        }
         meet();
         for (int i = tid; i < pairs * (HD / 4); i += kConsumers) {
             const int p = i / (HD / 4), d = i % (HD / 4) * 4;
@@ -325,74 +323,146 @@ __global__ void __launch_bounds__(kThreads, 1) attn_shared_kernel(SharedArgs a) 
                 l += v.y * f;
                 acc.x += b.x * f; acc.y += b.y * f; acc.z += b.z * f; acc.w += b.w * f;
             }
-            const size_t at = ((size_t)pair_of[p].x * a.n_heads + pair_of[p].y) * a.parts + it.part;
+            const size_t at = ((size_t)pair_of[p].x * a.n_heads + pair_of[p].y) * a.parts + part;
             *reinterpret_cast<float4*>(a.part_o + at * HD + d) = acc;
             if (d == 0) a.part_ml[at] = make_float2(m, l);
         }
     }
     if (!ok && lane == 0) record_give_up();
+    if (a.beside_big) pdl_wait();
 }
 
 #if (HOS_HEAD_DIM == 64) || (HOS_HEAD_DIM == 128) || (HOS_HEAD_DIM == 256)
 // ---- blocks of up to 128 pairs, on tcgen05 -------------------------------------------------------------
-// With more than 16 pairs the products above cost more than a page's bytes.  Here the pairs are the 128 rows of the tensor core's
-// operand: S = Q K^T (M 128, N 64, two buffers in tensor memory), the softmax by two threads a row, O += P V with O in tensor memory.  A
-// page's 16-byte pieces lie in the cache where the 128-byte swizzle wants them, so TMA boxes of [64 rows x 64 columns] are operands
-// as they land.  A CTA takes one item and kv head.  Warps: 0 pages, 1 products, 2 to 9 queries, softmax and sums.  The maximum is raised only
-// when a tile's exceeds it by 8 (weights up to e^8 do no harm in 32-bit sums and bfloat16 weights).
+// With more than 8 pairs the products above cost more than a page's bytes.  Here the pairs are the 128 rows of the tensor core's
+// operand: S = Q K^T (M 128, N 64, two buffers in tensor memory), softmax by a thread a row, O += P V.  O and, as the operand of
+// every page's product, the queries stay in tensor memory, so that a page costs shared memory its own bytes, once in and once out, and
+// the weights'.  A page's 16-byte pieces lie in the cache where the 128-byte swizzle wants them, so TMA boxes of [64 rows x 64 columns] are
+// operands as they land.  A CTA takes one item and kv head.  Warps: 0 keys, 10 values, 1 products, 2 to 9 queries, softmax and sums, in two
+// groups of four that take the tiles in turn: a tile's softmax is a chain of latencies, of which two run beside one another.  The row's
+// maximum is handed from group to group through shared memory as soon as a tile's is known; it is raised only when a tile's exceeds it by
+// 8 (weights up to e^8 do no harm in 32-bit sums and bfloat16 weights), so that O is hardly ever scaled.
 constexpr int kBlock = 128;
 constexpr int kColumns = HD / 64;                            // blocks of 64 numbers of a head
-constexpr int kQBlockBytes = kBlock * 128, kTileBlockBytes = kPageTokens * 128, kPBytes = kBlock * 128;
-constexpr int kTcStagesFit = (227 * 1024 - kColumns * kQBlockBytes - 2 * kPBytes - 2 * kBlock * 4 - 1024 - 256) / (2 * kTileBytes);
+constexpr int kTileBlockBytes = kPageTokens * 128, kPBytes = kBlock * 128;
+constexpr int kTcStagesFit = (227 * 1024 - 2 * kPBytes - 3 * kBlock * 4 - 1024 - 256) / (2 * kTileBytes);
 constexpr int kTcStages = kTcStagesFit < 6 ? kTcStagesFit : 6;
 constexpr int kTcBarriers = 1 + 4 * kTcStages + 8;
-constexpr int kTcShared = kColumns * kQBlockBytes + kTcStages * 2 * kTileBytes + 2 * kPBytes + 2 * kBlock * 4 + kTcBarriers * 8 + 16 + 1008;
+constexpr int kTcShared = kTcStages * 2 * kTileBytes + 2 * kPBytes + 3 * kBlock * 4 + kTcBarriers * 8 + 16 + 1008;
 static_assert(kTcStages >= 2 && kTcShared <= 227 * 1024, "shared memory of the kernel on tcgen05");
-constexpr int kTcThreads = 320;
-constexpr int kColS = 0, kColO = 128, kTmemCols = 128 + HD <= 256 ? 256 : 512;
+constexpr int kTcThreads = 352;
+constexpr int kColS = 0, kColO = 128, kColQ = 128 + HD, kTmemCols = kColQ + HD / 2 <= 256 ? 256 : 512;      // queries: two numbers a column
+static_assert(kColQ + HD / 2 <= kTmemCols, "tensor memory");
 constexpr float kRescaleSlack = 8.f;
 
-// tanh: for |x| <= 0.55 x + x^3 (a + x^2 (b + x^2 c)), relative error 1.3e-6; if any of a warp's scores is larger, 1 - 2 / (1 + e^2x)
-// for all of them, absolute error 2e-7.
-__device__ __forceinline__ void tanh_scores(float (&t)[32], float pre) {
-    float big = 0.f;
+// Two numbers an instruction.
+typedef unsigned long long Two;
+__device__ __forceinline__ Two two_of(float a, float b) {
+    Two d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ void split(Two v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+    Two d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+    Two d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+    Two d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+// tanh: for |x| <= 0.55 x + x^3 (a + x^2 (b + x^2 c)), relative error 1.3e-6; 1 - 2 / (1 + e^2x) else, absolute error 2e-7.
+constexpr float kTanhSmall = 0.55f;
+__device__ __forceinline__ float tanh_of(float x) {
+    const float x2 = x * x;
+    return fabsf(x) <= kTanhSmall ? fmaf(fmaf(fmaf(-0.043099623f, x2, 0.13152355f), x2, -0.33324513f) * x2, x, x)
+                                  : fmaf(-2.f, rcp_approx(1.f + ex2_approx(2.88539008f * x)), 1.f);
+}
+// of 64 scores times `pre`; `small`: none of the warp's is larger than 0.55
+__device__ __forceinline__ void tanh_scores(Two (&t)[32], float pre, bool small) {
+    if (small) {
+        const Two a = two_of(-0.043099623f, -0.043099623f), b = two_of(0.13152355f, 0.13152355f), c = two_of(-0.33324513f, -0.33324513f), f = two_of(pre, pre);
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        t[i] *= pre;
-        big = fmaxf(big, fabsf(t[i]));
-    }
-    if (__any_sync(0xffffffffu, !(big <= 0.55f))) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) t[i] = fmaf(-2.f, rcp_approx(1.f + ex2_approx(2.88539008f * t[i])), 1.f);
+        for (int i = 0; i < 32; ++i) {
+            const Two x = mul2(t[i], f), x2 = mul2(x, x);
+            t[i] = fma2(mul2(fma2(fma2(a, x2, b), x2, c), x2), x, x);
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-            const float x = t[i], x2 = x * x;
-            t[i] = fmaf(fmaf(fmaf(-0.043099623f, x2, 0.13152355f), x2, -0.33324513f) * x2, x, x);
+            float x, y;
+            split(t[i], x, y);
+            x = fmaf(-2.f, rcp_approx(1.f + ex2_approx(2.88539008f * (x * pre))), 1.f);
+            y = fmaf(-2.f, rcp_approx(1.f + ex2_approx(2.88539008f * (y * pre))), 1.f);
+            t[i] = two_of(x, y);
         }
     }
 }
-// 2^x = 2^n p(f), n = round(x), f = x - n, p of degree 3, relative error 7.5e-5 (the weights are rounded to 2^-8): on the multiply-add
-// pipe, for a quarter of the scores, as the special-function unit takes 16 a clock and an SM
-__device__ __forceinline__ float exp2_poly(float x) {
-    x = fmaxf(x, -125.f);
-    const float xr = x + 12582912.f;
-    const float f = x - (xr - 12582912.f);
-    float p = fmaf(0.055171646f, f, 0.24261113f);
-    p = fmaf(p, f, 0.69326097f);
-    p = fmaf(p, f, 0.99992806f);
-    return __int_as_float(__float_as_int(p) + (__float_as_int(xr) << 23));
+// The larger, the smaller of three.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+    float d;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// D += A B with A [128 rows][16] in tensor memory, two numbers a column; by the lanes whose `leader` is 1 (one of them).
+__device__ __forceinline__ void tc_mma_held(uint32_t leader, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(acc), "r"(leader)
+        : "memory");
+}
+// The same with A in shared memory, and the commit.
+__device__ __forceinline__ void tc_mma_by(uint32_t leader, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(acc), "r"(leader)
+        : "memory");
+}
+__device__ __forceinline__ void tc_commit_by(uint32_t leader, uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)), "r"(leader)
+        : "memory");
+}
+// Whether a phase is over, without waiting for it.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
 }
 
 __global__ void __launch_bounds__(kTcThreads, 1)
 attn_shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, SharedArgs a) {
     extern __shared__ unsigned char smem_unaligned[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_unaligned) + 1023) & ~(uintptr_t)1023);
-    unsigned char* q_s = smem;
-    unsigned char* ring = q_s + kColumns * kQBlockBytes;         // stage: keys, values
+    unsigned char* ring = smem;                                  // stage: keys, values
     unsigned char* p_s = ring + kTcStages * 2 * kTileBytes;
-    float* xchg = reinterpret_cast<float*>(p_s + 2 * kPBytes);   // [2 halves][128 rows]
-    uint64_t* bars = reinterpret_cast<uint64_t*>(xchg + 2 * kBlock);
+    float* row_max = reinterpret_cast<float*>(p_s + 2 * kPBytes);               // [128 rows]
+    float* row_sum = row_max + kBlock;                           // [2 groups][128 rows]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(row_sum + 2 * kBlock);
     uint64_t* q_full = bars;
     uint64_t* k_full = bars + 1;
     uint64_t* k_empty = k_full + kTcStages;
@@ -415,8 +485,8 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             mbar_init(&v_full[s], 1); mbar_init(&v_empty[s], 1);
         }
         for (int s = 0; s < 2; ++s) {
-            mbar_init(&s_full[s], 1); mbar_init(&s_empty[s], 8);
-            mbar_init(&p_full[s], 8); mbar_init(&pv_done[s], 1);
+            mbar_init(&s_full[s], 1); mbar_init(&s_empty[s], 4);
+            mbar_init(&p_full[s], 4); mbar_init(&pv_done[s], 1);
         }
         mbar_fence_init();
     }
@@ -426,8 +496,17 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_base_smem)), "r"(kTmemCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    const SharedItem it = a.items[blockIdx.x / kv_heads];
-    const Walk w = walk_of(a, it, lane);
+    const SharedItem& it = a.items[blockIdx.x / kv_heads];
+    int low = kOpen, high = -1;                                  // positions of the rows
+    for (int r = lane; r < it.n_rows; r += 32) {
+        const int pos = a.token_pos[a.rows[it.row0 + r]];
+        low = min(low, pos);
+        high = max(high, pos);
+    }
+    low = __reduce_min_sync(0xffffffffu, low);
+    high = __reduce_max_sync(0xffffffffu, high);
+    const int all_from = a.window > 0 ? max(0, high + 1 - a.window) : 0;      // every row sees the keys from here to `low`
+    const Walk w = walk_of(a, it, low, high);
     const int n_tiles = w.end - w.begin;
     tc_fence_before_sync();
     __syncthreads();
@@ -436,8 +515,13 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     bool ok = true;                        // false: a wait of this thread (in the softmax warps: of its warp) ran out
     auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_cycles(bar, parity, kWaitCycles); };
 
-    if (warp == 0) {
-        // ---------------- pages ----------------
+    if (warp == 0 || warp == 10) {
+        // ---------------- pages: keys (warp 0), values (warp 10) ----------------
+        const bool keys = warp == 0;
+        const CUtensorMap* map = keys ? &map_k : &map_v;
+        uint64_t* full = keys ? k_full : v_full;
+        uint64_t* empty = keys ? k_empty : v_empty;
+        unsigned char* to = ring + (keys ? 0 : kTileBytes);
         const int* table = a.cache.page_table + (size_t)it.slot * a.cache.table_stride;
         for (int i0 = 0; i0 < n_tiles && ok; i0 += 32) {         // 32 pages looked up at a time
             const int page_l = i0 + lane < n_tiles ? table[kv_table_entry(a.cache, walk_page(w, w.begin + i0 + lane))] : 0;
@@ -445,20 +529,13 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             for (int i = 0; i < n && ok; ++i) {
                 const int page = __shfl_sync(0xffffffffu, page_l, i);
                 if (lane == 0) {
-                    const int j = i0 + i, s = j % kTcStages, row = (page * kv_heads + kvh) * kPageTokens;
-                    const uint32_t parity = ((j / kTcStages) - 1) & 1;
-                    unsigned char* kd = ring + (size_t)s * 2 * kTileBytes;
-                    if (j >= kTcStages) ok = wait(&k_empty[s], parity);
+                    const int j = i0 + i, s = j % kTcStages;
+                    if (j >= kTcStages) ok = wait(&empty[s], ((j / kTcStages) - 1) & 1);
                     if (ok) {
-                        mbar_expect_tx(&k_full[s], kTileBytes);
+                        mbar_expect_tx(&full[s], kTileBytes);
 #pragma unroll
-                        for (int c = 0; c < kColumns; ++c) tc_tma_2d(kd + c * kTileBlockBytes, &map_k, 64 * c, row, &k_full[s]);
-                        if (j >= kTcStages) ok = wait(&v_empty[s], parity);
-                    }
-                    if (ok) {
-                        mbar_expect_tx(&v_full[s], kTileBytes);
-#pragma unroll
-                        for (int c = 0; c < kColumns; ++c) tc_tma_2d(kd + kTileBytes + c * kTileBlockBytes, &map_v, 64 * c, row, &v_full[s]);
+                        for (int c = 0; c < kColumns; ++c)
+                            tc_tma_2d(to + (size_t)s * 2 * kTileBytes + c * kTileBlockBytes, map, 64 * c, (page * kv_heads + kvh) * kPageTokens, &full[s]);
                     }
                 }
                 ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
@@ -467,124 +544,214 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         if (!ok && lane == 0) record_give_up();
     } else if (warp == 1) {
         // ---------------- products ----------------
-        if (lane == 0 && n_tiles > 0) {
+        // The whole warp goes through the loop, one lane issues: descriptors stay in uniform registers.  (With the loop in one lane's branch an
+        // instruction took 75 clocks to issue, of which the tensor core needs 45.)
+        const int tiles = __shfl_sync(0xffffffffu, n_tiles, 0);
+        if (tiles > 0) {
             constexpr uint32_t idesc_s = tc_idesc(kBlock, kPageTokens, 0), idesc_o = tc_idesc(kBlock, HD, 1);      // the values lie MN-major
-            ok = wait(q_full, 0);
+            const uint32_t leader = lane == 0;
+            auto all_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+            ok = all_wait(q_full, 0);
             tc_fence_after_sync();
-            auto issue_s = [&](int j) -> bool {
-                const int s = j % kTcStages, sb = j & 1;
-                if (!wait(&k_full[s], (j / kTcStages) & 1)) return false;
-                if (j >= 2 && !wait(&s_empty[sb], ((j >> 1) - 1) & 1)) return false;
-                tc_fence_after_sync();
-                const uint32_t k_addr = smem_u32(ring + (size_t)s * 2 * kTileBytes);
+            // the operands' descriptors count 16 bytes in their lowest bits: tiles and pieces are small numbers added to the first one's
+            const uint64_t k_desc = desc_kmajor(smem_u32(ring)), p_desc = desc_kmajor(smem_u32(p_s)),
+                           v_desc = desc_mnmajor(smem_u32(ring) + kTileBytes, kTileBlockBytes);
+            const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
+            // S of tile `next` (two ahead of the values at most) and O of tile j, whichever may go first: to wait for one of them in a fixed
+            // order would hold up the other
+            int next = 0, j = 0, k_stage = 0, v_stage = 0;
+            uint32_t k_phase = 0, v_phase = 0;
+            long long since = clock64();
+            while (j < tiles && ok) {
+                const bool may_s = next < tiles && next <= j + 2 && mbar_test(&k_full[k_stage], k_phase) &&
+                                   (next < 2 || mbar_test(&s_empty[next & 1], ((next >> 1) - 1) & 1));
+                if (__all_sync(0xffffffffu, may_s)) {
+                    tc_fence_after_sync();
+                    const int sb = next & 1;
+                    const uint64_t at = k_desc + (uint32_t)k_stage * (2 * kTileBytes / 16);
 #pragma unroll
-                for (int kk = 0; kk < HD / 16; ++kk)
-                    tc_mma(tmem_base + kColS + sb * kPageTokens, desc_kmajor(smem_u32(q_s) + (kk / 4) * kQBlockBytes) + 2 * (kk % 4),
-                           desc_kmajor(k_addr + (kk / 4) * kTileBlockBytes) + 2 * (kk % 4), idesc_s, kk > 0 ? 1u : 0u);
-                tc_commit(&s_full[sb]);
-                tc_commit(&k_empty[s]);
-                return true;
-            };
-            if (ok) ok = issue_s(0);
-            for (int j = 0; j < n_tiles && ok; ++j) {
-                if (j + 1 < n_tiles && !issue_s(j + 1)) { ok = false; break; }       // the next S runs under this tile's softmax
-                const int pb = j & 1, s = j % kTcStages;
-                if (!wait(&p_full[pb], (j >> 1) & 1) || !wait(&v_full[s], (j / kTcStages) & 1)) { ok = false; break; }
-                tc_fence_after_sync();
-                const uint32_t v_addr = smem_u32(ring + (size_t)s * 2 * kTileBytes + kTileBytes);
+                    for (int kk = 0; kk < HD / 16; ++kk)
+                        tc_mma_held(leader, tmem + kColS + sb * kPageTokens, tmem + kColQ + kk * 8, at + (kk / 4) * (kTileBlockBytes / 16) + 2 * (kk % 4),
+                                    idesc_s, kk > 0 ? 1u : 0u);
+                    tc_commit_by(leader, &s_full[sb]);
+                    tc_commit_by(leader, &k_empty[k_stage]);
+                    ++next;
+                    if (++k_stage == kTcStages) { k_stage = 0; k_phase ^= 1; }
+                    since = clock64();
+                }
+                const int pb = j & 1;
+                const bool may_o = next > j && mbar_test(&p_full[pb], (j >> 1) & 1) && mbar_test(&v_full[v_stage], v_phase);
+                if (__all_sync(0xffffffffu, may_o)) {
+                    tc_fence_after_sync();
+                    const uint64_t at_p = p_desc + pb * (kPBytes / 16), at_v = v_desc + (uint32_t)v_stage * (2 * kTileBytes / 16);
 #pragma unroll
-                for (int ks = 0; ks < kPageTokens / 16; ++ks)
-                    tc_mma(tmem_base + kColO, desc_kmajor(smem_u32(p_s) + pb * kPBytes) + 2 * ks,
-                           desc_mnmajor(v_addr + ks * 16 * 128, kTileBlockBytes), idesc_o, (j > 0 || ks > 0) ? 1u : 0u);
-                tc_commit(&v_empty[s]);
-                tc_commit(&pv_done[pb]);
+                    for (int ks = 0; ks < kPageTokens / 16; ++ks)
+                        tc_mma_by(leader, tmem + kColO, at_p + 2 * ks, at_v + ks * (16 * 128 / 16), idesc_o, (j > 0 || ks > 0) ? 1u : 0u);
+                    tc_commit_by(leader, &v_empty[v_stage]);
+                    tc_commit_by(leader, &pv_done[pb]);
+                    ++j;
+                    if (++v_stage == kTcStages) { v_stage = 0; v_phase ^= 1; }
+                    since = clock64();
+                }
+                ok = __all_sync(0xffffffffu, clock64() - since <= kWaitCycles) != 0;
             }
-            if (!ok) record_give_up();
+            if (!ok && lane == 0) record_give_up();
         }
-        __syncwarp();
     } else {
-        // ---------------- queries, softmax, sums: two threads a row, each 32 of a tile's keys ----------------
-        const int quarter = warp & 3, half = (warp - 2) >> 2, tid = threadIdx.x - 64;
+        // ---------------- queries, softmax, sums: group `side` takes the tiles side, side + 2, ..., a thread a row ----------------
+        const int quarter = warp & 3, side = (warp - 2) >> 2, tid = threadIdx.x - 64;
         const int r = quarter * 32 + lane;                       // row of the tile = lane of tensor memory
         const int group = a.n_heads / kv_heads, pairs = it.n_rows * group;
-        for (int i = tid; i < kBlock * (HD / 8); i += 256) {
-            const int p = i / (HD / 8), c = i % (HD / 8);
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (p < pairs)
-                v = *reinterpret_cast<const uint4*>(a.q + (size_t)a.rows[it.row0 + p / group] * a.q_stride + (size_t)(kvh * group + p % group) * HD + c * 8);
-            *reinterpret_cast<uint4*>(q_s + (c / 8) * kQBlockBytes + p * 128 + (((c % 8) ^ (p & 7)) << 4)) = v;
+        {   // 64 numbers of all rows at a time: in order through this group's buffer of weights, then a row a thread into tensor memory
+            const int in_group = tid & 127, piece = in_group & 7;
+            unsigned char* stage = p_s + (size_t)side * kPBytes;
+            int rows[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) rows[e] = a.rows[it.row0 + min((e * 16 + (in_group >> 3)) / group, it.n_rows - 1)];
+            uint4 v[(kColumns + 1) / 2][8];
+#pragma unroll
+            for (int c2 = 0; c2 < (kColumns + 1) / 2; ++c2)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int p = e * 16 + (in_group >> 3), c = min(2 * c2 + side, kColumns - 1);
+                    v[c2][e] = *reinterpret_cast<const uint4*>(a.q + (size_t)rows[e] * a.q_stride + (size_t)(kvh * group + p % group) * HD + c * 64 + piece * 8);
+                }
+#pragma unroll
+            for (int c2 = 0; c2 < (kColumns + 1) / 2; ++c2) {
+                const int c = 2 * c2 + side;
+                if (c >= kColumns) break;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int p = e * 16 + (in_group >> 3);
+                    *reinterpret_cast<uint4*>(stage + p * 128 + ((piece ^ (p & 7)) << 4)) = p < pairs ? v[c2][e] : make_uint4(0, 0, 0, 0);
+                }
+                asm volatile("bar.sync %0, 128;" ::"r"(4 + side) : "memory");
+                uint32_t q[32];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(stage + r * 128 + ((i ^ (r & 7)) << 4));
+                    q[4 * i] = x.x; q[4 * i + 1] = x.y; q[4 * i + 2] = x.z; q[4 * i + 3] = x.w;
+                }
+                tc_st32(tmem_base + ((uint32_t)(quarter * 32) << 16) + kColQ + c * 32, q);
+                asm volatile("bar.sync %0, 128;" ::"r"(4 + side) : "memory");
+            }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // generic writes -> visible to the tensor core
-        __syncwarp();
-        if (lane == 0) mbar_arrive(q_full);
-        const int row = a.rows[it.row0 + min(r / group, it.n_rows - 1)];
+        const int row = a.rows[it.row0 + min(r / group, it.n_rows - 1)], part = it.part;
         const int pos = a.token_pos[row], lowest = a.window > 0 ? max(0, pos + 1 - a.window) : 0;
         const uint32_t t_lane = tmem_base + ((uint32_t)(quarter * 32) << 16);
         // t = tanh(s scale / cap), or s: the score is c_logit t, and a weight 2^(t c2 - m c2)
         const bool capped = a.cap > 0.f;
         const float pre = capped ? a.scale / a.cap : 1.f, c_logit = capped ? a.cap : a.scale;
         const float c2 = c_logit * 1.44269504f, slack = kRescaleSlack / c_logit;
-        float m_ref = -INFINITY, l_run = 0.f;                    // l_run: of this thread's keys
+        const bool idle = quarter * 32 >= pairs;
+        float m_mine = -INFINITY, l_run = 0.f;                   // the sum of this thread's weights, by this maximum
         auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
-        for (int j = 0; j < n_tiles; ++j) {
-            const int sb = j & 1, key0 = walk_page(w, w.begin + j) * kPageTokens;
-            float m_half = -INFINITY;
-            float sc[32];
-            if (ok) ok = warp_wait(&s_full[sb], (j >> 1) & 1);
-            if (ok) {
+        for (int j = side; j < n_tiles; j += 2) {
+            const int key0 = walk_page(w, w.begin + j) * kPageTokens;
+            float m_tile = -INFINITY;
+            Two sc[32];
+            bool small = true, edge = false;
+            if (ok) ok = warp_wait(&s_full[side], (j >> 1) & 1);
+            if (ok && idle) {
+                if (lane == 0) mbar_arrive(&s_empty[side]);
+            } else if (ok) {
                 tc_fence_after_sync();
-                {
-                    uint32_t v[32];
-                    tc_ld32(t_lane + kColS + sb * kPageTokens + 32 * half, v);
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) sc[i] = __uint_as_float(v[i]);
-                }
+                uint32_t v0[32], v1[32];
+                tc_ld32(t_lane + kColS + side * kPageTokens, v0);
+                tc_ld32(t_lane + kColS + side * kPageTokens + 32, v1);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                 tc_fence_before_sync();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&s_empty[sb]);
-                if (capped) tanh_scores(sc, pre);
-                if (key0 < w.all_from || key0 + kPageTokens - 1 > w.all_to) {
+                if (lane == 0) mbar_arrive(&s_empty[side]);
+                // the largest and the smallest score: with a cap the largest's tanh is the tile's maximum
+                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, n4[4] = {INFINITY, INFINITY, INFINITY, INFINITY};
+                if (capped) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const int key = key0 + 32 * half + i;
-                        sc[i] = key >= lowest && key <= pos ? sc[i] : -INFINITY;
+                    for (int i = 0; i < 32; i += 2) {
+                        n4[i / 2 & 3] = min3(n4[i / 2 & 3], __uint_as_float(v0[i]), __uint_as_float(v0[i + 1]));
+                        n4[i / 2 & 3] = min3(n4[i / 2 & 3], __uint_as_float(v1[i]), __uint_as_float(v1[i + 1]));
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < 32; ++i) m_half = fmaxf(m_half, sc[i]);
+                for (int i = 0; i < 32; i += 2) {
+                    m4[i / 2 & 3] = max3(m4[i / 2 & 3], __uint_as_float(v0[i]), __uint_as_float(v0[i + 1]));
+                    m4[i / 2 & 3] = max3(m4[i / 2 & 3], __uint_as_float(v1[i]), __uint_as_float(v1[i + 1]));
+                    sc[i / 2] = two_of(__uint_as_float(v0[i]), __uint_as_float(v0[i + 1]));
+                    sc[16 + i / 2] = two_of(__uint_as_float(v1[i]), __uint_as_float(v1[i + 1]));
+                }
+                m_tile = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+                if (capped) {
+                    const float n_tile = fminf(fminf(n4[0], n4[1]), fminf(n4[2], n4[3]));
+                    small = __all_sync(0xffffffffu, m_tile * pre <= kTanhSmall && n_tile * pre >= -kTanhSmall) != 0;
+                }
+                edge = key0 < all_from || key0 + kPageTokens - 1 > low;
+                if (edge) {                                      // only what the row sees
+                    m_tile = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const float a0 = __uint_as_float(v0[i]), a1 = __uint_as_float(v1[i]);
+                        if (key0 + i >= lowest && key0 + i <= pos) m_tile = fmaxf(m_tile, a0);
+                        if (key0 + 32 + i >= lowest && key0 + 32 + i <= pos) m_tile = fmaxf(m_tile, a1);
+                    }
+                }
+                if (capped && m_tile != -INFINITY) m_tile = tanh_of(m_tile * pre);
             }
-            // the row's maximum over both halves; two places, so that one barrier is enough
-            xchg[half * kBlock + r] = m_half;
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-            const float m_tile = fmaxf(m_half, xchg[(half ^ 1) * kBlock + r]);
-            asm volatile("bar.sync 1, 256;" ::: "memory");
+            // the maximum from the tile before, and to the tile after (every thread comes here, whatever its waits did)
+            if (j > 0) asm volatile("bar.sync %0, 256;" ::"r"(1 + side) : "memory");
+            const float m_old = j > 0 ? row_max[r] : -INFINITY;
+            const bool raise = m_tile > m_old + slack || (m_old == -INFINITY && m_tile > -INFINITY);
+            const float m_ref = raise ? m_tile : m_old;
+            if (j + 1 < n_tiles) {
+                row_max[r] = m_ref;
+                asm volatile("bar.arrive %0, 256;" ::"r"(2 - side) : "memory");
+            }
             if (!ok) continue;
-            float factor = 1.f;
-            if (m_tile > m_ref + slack || (m_ref == -INFINITY && m_tile > -INFINITY)) {
-                factor = m_ref == -INFINITY ? 0.f : __expf((m_ref - m_tile) * c_logit);
-                m_ref = m_tile;
+            if (idle) {                                          // no pair in this warp's rows: what the products make of them goes nowhere
+                if (j >= 2) ok = warp_wait(&pv_done[side], ((j >> 1) - 1) & 1);
+                if (ok && lane == 0) mbar_arrive(&p_full[side]);
+                continue;
+            }
+            if (capped) tanh_scores(sc, pre, small);
+            if (edge) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    float a0, a1;
+                    split(sc[i], a0, a1);
+                    const int key = key0 + 2 * i;
+                    sc[i] = two_of(key >= lowest && key <= pos ? a0 : -INFINITY, key + 1 >= lowest && key + 1 <= pos ? a1 : -INFINITY);
+                }
             }
             const float m2 = (m_ref == -INFINITY ? 0.f : m_ref) * c2;
-            float sum = 0.f;
-            uint32_t packed[16];
+            const Two by = two_of(c2, c2), less = two_of(-m2, -m2);
+            Two sums[2] = {0, 0};
+            uint32_t packed[32];
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-                const float e0 = fmaf(sc[i], c2, -m2), e1 = fmaf(sc[i + 1], c2, -m2);
-                const bool poly = ((i >> 1) & 3) == 0;
-                const float p0 = poly ? exp2_poly(e0) : ex2_approx(e0), p1 = poly ? exp2_poly(e1) : ex2_approx(e1);
-                sum += p0 + p1;
-                packed[i / 2] = pack_bf16(p0, p1);
+            for (int i = 0; i < 32; ++i) {
+                float e0, e1;
+                split(fma2(sc[i], by, less), e0, e1);
+                e0 = ex2_approx(e0);
+                e1 = ex2_approx(e1);
+                sums[i & 1] = add2(sums[i & 1], two_of(e0, e1));
+                packed[i] = pack_bf16(e0, e1);
             }
-            l_run = l_run * factor + sum;
-            if (j >= 2) ok = warp_wait(&pv_done[sb], ((j >> 1) - 1) & 1);      // this buffer of weights has been read
+            float sum0, sum1;
+            split(add2(sums[0], sums[1]), sum0, sum1);
+            if (m_mine != m_ref) l_run *= m_mine == -INFINITY ? 0.f : ex2_approx((m_mine - m_ref) * c2);      // l_run is 0 where nothing was seen
+            m_mine = m_ref;
+            l_run += sum0 + sum1;
+            if (j >= 2) ok = warp_wait(&pv_done[side], ((j >> 1) - 1) & 1);      // this group's weights of two tiles ago have been read
             if (!ok) continue;
-            if (j > 0 && __any_sync(0xffffffffu, factor != 1.f)) {
-                ok = warp_wait(&pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1);      // O is touched only between products
+            if (j > 0 && __any_sync(0xffffffffu, raise)) {
+                ok = warp_wait(&pv_done[side ^ 1], ((j - 1) >> 1) & 1);          // O is touched only between products
                 if (!ok) continue;
                 tc_fence_after_sync();
+                const float factor = !raise ? 1.f : m_old == -INFINITY ? 0.f : ex2_approx((m_old - m_ref) * c2);
 #pragma unroll 1
-                for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 32) {
+                for (int c = 0; c < HD; c += 32) {
                     uint32_t o[32];
                     tc_ld32(t_lane + kColO + c, o);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -594,35 +761,46 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 }
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             }
-            unsigned char* prow = p_s + (size_t)sb * kPBytes + (size_t)r * 128;
+            unsigned char* prow = p_s + (size_t)side * kPBytes + (size_t)r * 128;
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-                *reinterpret_cast<uint4*>(prow + (((4 * half + c) ^ (r & 7)) << 4)) =
-                    make_uint4(packed[4 * c], packed[4 * c + 1], packed[4 * c + 2], packed[4 * c + 3]);
+            for (int c = 0; c < 8; ++c)
+                *reinterpret_cast<uint4*>(prow + ((c ^ (r & 7)) << 4)) = make_uint4(packed[4 * c], packed[4 * c + 1], packed[4 * c + 2], packed[4 * c + 3]);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[sb]);
+            if (lane == 0) mbar_arrive(&p_full[side]);
         }
-        // ---- the sums leave, not divided ----
-        if (ok && n_tiles > 0) ok = warp_wait(&pv_done[(n_tiles - 1) & 1], ((n_tiles - 1) >> 1) & 1);
+        // ---- the sums leave, not divided: each group half of a row's numbers ----
+        const int last = n_tiles - 1;
+        if (ok && n_tiles > 0) ok = warp_wait(&pv_done[last & 1], (last >> 1) & 1);
         tc_fence_after_sync();
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        xchg[half * kBlock + r] = l_run;
-        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (side == (last & 1)) row_max[r] = m_mine;             // the last tile's is the row's (without tiles: -inf, of group 1)
+        asm volatile("bar.sync 3, 256;" ::: "memory");
+        const float m_row = row_max[r];
+        row_sum[side * kBlock + r] = m_mine == -INFINITY ? 0.f : l_run * ex2_approx((m_mine - m_row) * c2);
+        asm volatile("bar.sync 3, 256;" ::: "memory");
         if (ok) {
-            const size_t at = ((size_t)row * a.n_heads + kvh * group + r % group) * a.parts + it.part;
-            if (half == 0 && r < pairs) a.part_ml[at] = make_float2(m_ref * c_logit, l_run + xchg[kBlock + r]);
-            if (n_tiles > 0) {
+            const size_t at = ((size_t)row * a.n_heads + kvh * group + r % group) * a.parts + part;
+            if (side == 0 && r < pairs) a.part_ml[at] = make_float2(m_row * c_logit, row_sum[r] + row_sum[kBlock + r]);
+            if (n_tiles > 0 && !idle) {
+                // 32 rows by 32 numbers of a warp at a time through shared memory, so that whole lines are written
+                unsigned char* stage = p_s + (size_t)(warp - 2) * 4096;
 #pragma unroll 1
-                for (int c = half * (HD / 2); c < (half + 1) * (HD / 2); c += 32) {
+                for (int c = side * (HD / 2); c < (side + 1) * (HD / 2); c += 32) {
                     uint32_t o[32];
                     tc_ld32(t_lane + kColO + c, o);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    if (r < pairs) {
-                        uint4* dst = reinterpret_cast<uint4*>(a.part_o + at * HD + c);
+                    __syncwarp();
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    for (int i = 0; i < 8; ++i)
+                        *reinterpret_cast<uint4*>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int x = 4 * i + (lane >> 3), p = quarter * 32 + x;       // four rows a store, eight lanes each
+                        const uint4 v = *reinterpret_cast<const uint4*>(stage + x * 128 + (((lane & 7) ^ (x & 7)) << 4));
+                        const size_t first = __shfl_sync(0xffffffffu, at, x);
+                        if (p < pairs) *reinterpret_cast<uint4*>(a.part_o + first * HD + c + (lane & 7) * 4) = v;
                     }
                 }
             }
@@ -636,43 +814,77 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
 }
 #endif
 
-// A row's parts joined; a row without parts (padding) becomes zeros, and so does one that sees no key.  A block takes a (row, head): HD / 4
-// threads a part, as many parts at a time as 256 threads are.
+// A row's parts joined; a row without parts (padding) becomes zeros, and so does one that sees no key.  WARPS warps take a (row, head), a
+// share of its parts each: lanes read the maxima of 32 parts at a time, then the sums of each part together.
+template <int WARPS>
 __global__ void __launch_bounds__(256) attn_shared_merge_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml,
-                                                                const int* __restrict__ n_parts, int parts, int n_heads, bf16* out, int out_stride) {
-    constexpr int ACROSS = HD / 4, DEEP = 256 / ACROSS;
-    __shared__ float4 sums[DEEP * ACROSS];
+                                                                const int* __restrict__ n_parts, int parts, int n_rows, int n_heads, bf16* out,
+                                                                int out_stride) {
+    constexpr int EACH = (HD / 4 + 31) / 32;                 // fours of numbers a lane
+    __shared__ float4 shared_acc[WARPS > 1 ? 8 : 1][WARPS > 1 ? EACH * 32 : 1];
+    __shared__ float2 shared_ml[8];
     pdl_enter();
-    const int n = blockIdx.x / n_heads, head = blockIdx.x % n_heads;
-    const int have = n_parts[n];
-    const size_t at = ((size_t)n * n_heads + head) * parts;
-    const int across = threadIdx.x % ACROSS, deep = threadIdx.x / ACROSS;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, pair = blockIdx.x * (8 / WARPS) + warp / WARPS;
+    if (WARPS == 1 && pair >= n_rows * n_heads) return;      // (with more warps a pair there is a barrier, and no such block)
+    const int n = pair / n_heads, head = pair % n_heads;
+    const int have = n_parts[n], each = (have + WARPS - 1) / WARPS, first = warp % WARPS * each, last = min(have, first + each);
+    const size_t at = (size_t)pair * parts;
+    float4 acc[EACH] = {};
     float m = -INFINITY, l = 0.f;
-    for (int p = 0; p < have; ++p) m = fmaxf(m, part_ml[at + p].x);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int p = deep; p < have; p += DEEP) {
-        const float2 v = part_ml[at + p];
-        if (deep >= DEEP || v.x == -INFINITY) continue;      // (a part without a key left no sums)
-        const float f = __expf(v.x - m);
-        const float4 b = *reinterpret_cast<const float4*>(part_o + (at + p) * HD + across * 4);
-        acc.x += b.x * f; acc.y += b.y * f; acc.z += b.z * f; acc.w += b.w * f;
-    }
-    if (deep < DEEP) sums[deep * ACROSS + across] = acc;
-    for (int p = 0; p < have; ++p) {
-        const float2 v = part_ml[at + p];
-        if (v.x != -INFINITY) l += v.y * __expf(v.x - m);
-    }
-    __syncthreads();
-    if (deep == 0) {
-#pragma unroll 4
-        for (int d = 1; d < DEEP; ++d) {
-            const float4 b = sums[d * ACROSS + across];
-            acc.x += b.x; acc.y += b.y; acc.z += b.z; acc.w += b.w;
+    for (int p0 = first; p0 < last; p0 += 32) {
+        const float2 v = p0 + lane < last ? part_ml[at + p0 + lane] : make_float2(-INFINITY, 0.f);
+        float most = fmaxf(v.x, m);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        if (most == -INFINITY) continue;                     // no key so far
+        const float before = m == -INFINITY ? 0.f : __expf(m - most), f = v.x == -INFINITY ? 0.f : __expf(v.x - most);
+        m = most;
+        l = l * before + warp_sum(v.y * f);
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) { acc[e].x *= before; acc[e].y *= before; acc[e].z *= before; acc[e].w *= before; }
+        const int n_here = min(32, last - p0);
+#pragma unroll 8
+        for (int p = 0; p < n_here; ++p) {
+            const float fp = __shfl_sync(0xffffffffu, f, p);
+            const float4* src = reinterpret_cast<const float4*>(part_o + (at + p0 + p) * HD);
+#pragma unroll
+            for (int e = 0; e < EACH; ++e)
+                if (fp != 0.f && e * 32 + lane < HD / 4) {       // (a part without a key left no sums)
+                    const float4 b = src[e * 32 + lane];
+                    acc[e].x += b.x * fp; acc[e].y += b.y * fp; acc[e].z += b.z * fp; acc[e].w += b.w * fp;
+                }
         }
-        const float r = l > 0.f ? 1.f / l : 0.f;
-        *reinterpret_cast<uint2*>(out + (size_t)n * out_stride + (size_t)head * HD + across * 4) =
-            make_uint2(pack_bf16(acc.x * r, acc.y * r), pack_bf16(acc.z * r, acc.w * r));
     }
+    if constexpr (WARPS > 1) {
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) shared_acc[warp][e * 32 + lane] = acc[e];
+        if (lane == 0) shared_ml[warp] = make_float2(m, l);
+        __syncthreads();
+        if (warp % WARPS != 0) return;
+        float all = -INFINITY;
+#pragma unroll
+        for (int y = 0; y < WARPS; ++y) all = fmaxf(all, shared_ml[warp + y].x);
+        l = 0.f;
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) acc[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int y = 0; y < WARPS; ++y) {
+            const float2 v = shared_ml[warp + y];
+            const float f = v.x == -INFINITY ? 0.f : __expf(v.x - all);
+            l += v.y * f;
+#pragma unroll
+            for (int e = 0; e < EACH; ++e) {
+                const float4 b = shared_acc[warp + y][e * 32 + lane];
+                acc[e].x += b.x * f; acc[e].y += b.y * f; acc[e].z += b.z * f; acc[e].w += b.w * f;
+            }
+        }
+    }
+    const float r = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e)
+        if (e * 32 + lane < HD / 4)
+            *reinterpret_cast<uint2*>(out + (size_t)n * out_stride + (size_t)head * HD + (e * 32 + lane) * 4) =
+                make_uint2(pack_bf16(acc[e].x * r, acc[e].y * r), pack_bf16(acc[e].z * r, acc[e].w * r));
 }
 
 }  // namespace hos
@@ -689,9 +901,9 @@ extern "C" int hos_attn_shared_set_error_word(int* word) {
 
 // What a list of work is (parts/shared_attention.py makes one a step and kind of layer): on the device, but for the numbers.
 struct SharedWork {
-    const int* counts;         // [0] items of up to 16 pairs, [1] of up to 128
+    const int* counts;         // [0] items of up to 8 pairs, [1] of up to 128
     const int* n_parts;        // [rows]
-    const int* items;          // of up to 16 pairs, then
+    const int* items;          // of up to 8 pairs, then
     const int* big_items;      // of up to 128
     const int* rows;
     const int* page_table;
@@ -719,7 +931,7 @@ extern "C" int hos_attn_shared(const void* q, int q_stride, void* out, int out_s
     float* part_ml = workspace + (size_t)n_rows * k.n_heads * k.parts * HD;
     SharedArgs a{(const bf16*)q, q_stride, token_pos, reinterpret_cast<const SharedItem*>(k.items), k.counts, k.rows,
                  PagedKV{const_cast<void*>(k_pages), const_cast<void*>(v_pages), k.page_table, k.table_stride, k.ring_pages, k.n_kv_heads, HD},
-                 k.n_heads, k.parts, workspace, reinterpret_cast<float2*>(part_ml), scale, cap, k.window};
+                 k.n_heads, k.parts, workspace, reinterpret_cast<float2*>(part_ml), scale, cap, k.window, k.big_most > 0 ? 1 : 0};
     int rc;
     if (k.big_most > 0) {
 #if (HOS_HEAD_DIM == 64) || (HOS_HEAD_DIM == 128) || (HOS_HEAD_DIM == 256)
@@ -747,16 +959,22 @@ extern "C" int hos_attn_shared(const void* q, int q_stride, void* out, int out_s
     if (k.most > 0) {
         static bool set = false;
         if (!set) {
-            if (cudaFuncSetAttribute(attn_shared_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SharedSmem::kTotal) != cudaSuccess)
-                HOS_REFUSE("attn_shared: cannot get %d bytes of shared memory", SharedSmem::kTotal);
+            if (cudaFuncSetAttribute(attn_shared_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kShared) != cudaSuccess)
+                HOS_REFUSE("attn_shared: cannot get %d bytes of shared memory", kShared);
             set = true;
         }
         const long long items = (long long)k.most * k.n_kv_heads * ((group + kPairs - 1) / kPairs);
-        const int grid = (int)(items < sm_count_cached() ? items : sm_count_cached());
-        launch_pdl(attn_shared_kernel, dim3(grid), dim3(kThreads), SharedSmem::kTotal, stream, a);
+        const int places = kCtasPerSm * sm_count_cached(), grid = (int)(items < places ? items : places);
+        launch_ahead(k.big_most > 0 || pdl_enabled(), attn_shared_kernel, dim3(grid), dim3(kThreads), kShared, stream, a);
         if ((rc = check_launch("attn_shared"))) return rc;
     }
-    launch_pdl(attn_shared_merge_kernel, dim3(n_rows * k.n_heads), dim3(256), 0, stream, workspace, reinterpret_cast<const float2*>(part_ml), k.n_parts,
-               k.parts, k.n_heads, (bf16*)out, out_stride);
+    // many parts of few rows: eight warps a (row, head) (8 rows of 8 heads of 256, 33 parts: 6.8 us with one, MERGE8)
+    const int merged = n_rows * k.n_heads;
+    auto merge = [&](auto kernel, int blocks) {
+        launch_ahead(true, kernel, dim3(blocks), dim3(256), 0, stream, workspace, reinterpret_cast<const float2*>(part_ml), k.n_parts, k.parts, n_rows,
+                     k.n_heads, (bf16*)out, out_stride);
+    };
+    if (k.parts >= 8 && merged <= 512) merge(attn_shared_merge_kernel<8>, merged);
+    else merge(attn_shared_merge_kernel<1>, (merged + 7) / 8);
     return check_launch("attn_shared (merge)");
 }

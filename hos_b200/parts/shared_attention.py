@@ -16,8 +16,9 @@ from ..errors import KernelError
 
 MAX_HEAD_DIM = 256
 OPEN = 1 << 30                 # a page behind every sequence's last
-ITEM_INTS = 12
-PAIRS, BLOCK = 16, 128         # (row, head) pairs of an item, of a big one
+ITEM_INTS = 20
+PAIRS, BLOCK = 8, 128          # (row, head) pairs of an item, of a big one
+FEW_PAIRS = 16                 # up to so many pairs are several small blocks
 MOST_PARTS = 64 << 20          # bytes of the parts that wait for the merge
 
 _libs: Dict[int, ops.Library] = {}
@@ -54,7 +55,7 @@ class SharedPlan:
 
 
 class Lists:
-    """Items (of up to 16 pairs, then of up to 128), their rows, and each row's number of parts, on the host."""
+    """Items (of up to 8 pairs, then of up to 128), their rows, and each row's number of parts, on the host."""
 
     def __init__(self, items: np.ndarray, big: np.ndarray, rows: np.ndarray, n_parts: np.ndarray):
         self.items, self.big, self.rows, self.n_parts = items, big, rows, n_parts
@@ -95,59 +96,116 @@ def has_big(head_dim: int) -> bool:
     return head_dim in (64, 128, 256)
 
 
-def _pages(length: int, new: int, window: Optional[int]) -> tuple:
-    """(first, behind the last) logical page that the last `new` rows of a sequence see."""
-    lowest = max(0, length - new + 1 - window) if window else 0
-    return lowest // ops.PAGE_TOKENS, (length - 1) // ops.PAGE_TOKENS + 1
+# Microseconds of an item, by head size (64, 128, 256): a small one and a page of it (a CTA takes two side by side), a big one and a page of it,
+# of a CTA by itself; and bytes of pages and of parts a microsecond, of all.  Measured (B200): 1,024 pages of 128 numbers for 32 rows of 4
+# heads in shares of 16 and 64, 25.3 and 63.9 us; 64 rows of 16 pages each, 8 heads of 256 over 4, 49.8 us of which the bytes are 41.0.
+SMALL_US, BIG_US = 2.0, 8.0
+BYTES_US, PART_BYTES_US = 6.0e6, 5.0e6
 
 
-def share_pages(pages: Sequence[int], per_item: int) -> int:
-    """Pages of a share at most, for items of so many pages that each run `per_item` times: as many shares as fill the SMs once."""
-    total = sum(pages) * per_item
-    return max(2, -(-total // ops.sm_count()))
+def _page_us(head_dim: int) -> tuple:
+    return 0.2 + head_dim / 800, 0.6 + head_dim / 550
+
+
+def _cuts(pages: np.ndarray):
+    """Lengths of a share that are looked at, and how many shares of each the blocks make."""
+    most = max(2, int(pages.max())) if pages.size else 2
+    lengths, n = [], 2
+    while n < most:
+        lengths.append(n)
+        n = max(n + 1, n * 5 // 4)
+    lengths.append(most)
+    return lengths, -(-pages[:, None] // np.asarray(lengths)) if pages.size else np.zeros((0, len(lengths)), dtype=np.int64)
+
+
+def shares(small: np.ndarray, big: np.ndarray, big_pairs: np.ndarray, per_item: int, kv: int, head_dim: int, distinct: int) -> tuple:
+    """(pages of a small share, of a big one) for small blocks and big blocks of so many pages, `distinct` of them not the same: the cut that
+    makes the step shortest by the estimate above.  An item is run per_item times (a big one kv times); big ones have an SM for
+    themselves, small ones take what is left, then all."""
+    sms, (small_page, big_page) = ops.sm_count(), _page_us(head_dim)
+    read = 256.0 * head_dim * distinct * kv / BYTES_US
+    part_us = (head_dim + 2) * 8.0 / PART_BYTES_US
+    lengths, splits = _cuts(small)
+    items = splits.sum(axis=0) * per_item
+    s_work = items * SMALL_US + float(small.sum()) * per_item * small_page
+    s_long = np.where(items > 0, SMALL_US + np.asarray(lengths) * small_page, 0.0)
+    s_parts = items * 8.0 * part_us
+    big_lengths, big_splits = _cuts(big)
+    items = big_splits.sum(axis=0) * kv
+    b_work = items * BIG_US + float(big.sum()) * kv * big_page
+    b_long = np.where(items > 0, -(-items // sms) * (BIG_US + np.asarray(big_lengths) * big_page), 0.0)
+    b_parts = (big_splits * big_pairs[:, None]).sum(axis=0) * kv * part_us
+    us = np.maximum(np.maximum(b_long[:, None], s_long), np.maximum((b_work[:, None] + s_work) / sms, read)) + b_parts[:, None] + s_parts
+    i, j = divmod(int(np.argmin(us)), len(lengths))
+    return lengths[j], big_lengths[i]
 
 
 def lists(runs, rows: Sequence[range], slots: Sequence[int], lengths: Sequence[int], n_rows: int, per: int, kv: int, head_dim: int,
           window: Optional[int], big: bool) -> Lists:
-    """The work: a run's rows in blocks of up to 16 pairs, or of up to 128 where they are more and a kernel has such blocks (`big`), over
-    the run's pages, each sequence's over the rest of its own."""
+    """The work: a run's rows in blocks of up to 8 pairs, or, where they are more than FEW_PAIRS and a kernel has such blocks (`big`), of up to
+    128, over the run's pages, each sequence's over the rest of its own."""
     big = big and per <= BLOCK
     chunks = -(-per // PAIRS)
-    skip = [(0, 0)] * len(slots)
-    blocks = []                                              # (big, rows, slot, lp0, lp1, skip0, skip1, pages)
+    n_seqs = len(slots)
+    lens = np.asarray(lengths, dtype=np.int64)
+    news = np.asarray([len(r) for r in rows], dtype=np.int64)
+    first = np.maximum(0, lens - news + 1 - window) // ops.PAGE_TOKENS if window else np.zeros(n_seqs, dtype=np.int64)
+    behind = (lens - 1) // ops.PAGE_TOKENS + 1              # the logical pages that a sequence's rows see
+    skip = np.zeros((n_seqs, 2), dtype=np.int64)
+    blocks = ([], [])                                        # small, big: (rows, slot, lp0, lp1, skip0, skip1, pages)
+    made = []                                                # which of both, one after another
 
     def cut(of: Sequence[int], *rest) -> None:
-        large = big and len(of) * per > PAIRS
+        large = big and len(of) * per > FEW_PAIRS
         size = max(1, (BLOCK if large else PAIRS) // per)
         n = -(-len(of) // size)                              # blocks of like sizes
         for i in range(n):
-            blocks.append((large, of[len(of) * i // n:len(of) * (i + 1) // n], *rest))
+            blocks[large].append((of[len(of) * i // n:len(of) * (i + 1) // n], *rest))
+            made.append(large)
 
+    distinct = 0
     for members, lo, hi in runs:
-        seen = [_pages(lengths[i], len(rows[i]), window) for i in members]
-        n = min(hi, max(b for _, b in seen)) - max(lo, min(a for a, _ in seen))
+        n = min(hi, int(behind[members].max())) - max(lo, int(first[members].min()))
         if n <= 0:
             continue
-        for i in members:
-            skip[i] = (lo, hi)
+        distinct += n
+        skip[members] = (lo, hi)
         cut([r for i in members for r in rows[i]], slots[members[0]], lo, hi, OPEN, OPEN, n)
-    for i, slot in enumerate(slots):
-        a, b = _pages(lengths[i], len(rows[i]), window)
-        lo, hi = skip[i]
-        cut(rows[i], slot, 0, OPEN, lo, hi, max(1, b - a - max(0, min(b, hi) - max(a, lo))))
-    share = share_pages([b[7] for b in blocks], kv * chunks)
+    rest = np.maximum(1, behind - first - np.maximum(0, np.minimum(behind, skip[:, 1]) - np.maximum(first, skip[:, 0])))
+    distinct += int(rest.sum())
+    for i, (slot, of, lo_hi, n) in enumerate(zip(slots, rows, skip.tolist(), rest.tolist())):
+        if len(of) == 1:
+            blocks[big and per > FEW_PAIRS].append((of, slot, 0, OPEN, *lo_hi, n))
+            made.append(big and per > FEW_PAIRS)
+        else:
+            cut(of, slot, 0, OPEN, *lo_hi, n)
+    pages = [np.asarray([b[6] for b in of], dtype=np.int64) for of in blocks]
+    share = shares(pages[0], pages[1], np.asarray([len(b[0]) * per for b in blocks[1]], dtype=np.int64), kv * chunks, kv, head_dim, distinct)
     most = max(2, MOST_PARTS // max(1, 4 * n_rows * per * kv * (head_dim + 2)))
     n_parts = np.zeros(n_rows, dtype=np.int32)
-    made, listed = ([], []), []
-    for large, of_block, slot, lp0, lp1, skip0, skip1, n in blocks:
-        splits = max(1, min(-(-n // share), most // 2))
-        part = int(n_parts[of_block[0]])
-        for s in range(splits):
-            made[large].append((len(listed), len(of_block), slot, lp0, lp1, skip0, skip1, s, splits, part + s, -(-n // splits), 0))
+    listed = []
+    splits = [np.minimum(-(-p // n), max(1, most // 2)) for p, n in zip(pages, share)]
+    table = [np.zeros((len(p), ITEM_INTS), dtype=np.int32) for p in pages]
+    at = [0, 0]
+    for large in made:                                       # as they were made: all rows of a block have had as many parts
+        i = at[large]
+        at[large] += 1
+        of_block, *places = blocks[large][i][:6]
+        table[large][i, :7] = (len(listed), len(of_block), *places)
+        table[large][i, 9] = n_parts[of_block[0]]
+        if not large:
+            table[large][i, 12:12 + len(of_block)] = of_block
         listed.extend(of_block)
-        for r in of_block:
-            n_parts[r] += splits
-    items = [np.asarray(sorted(m, key=lambda it: -it[10]), dtype=np.int32).reshape(-1, ITEM_INTS) for m in made]      # the longest first
+        n_parts[slice(of_block.start, of_block.stop) if isinstance(of_block, range) else of_block] += splits[large][i]
+    items = []
+    for rows_of, n, p in zip(table, splits, pages):
+        if len(p):
+            rows_of[:, 8], rows_of[:, 10] = n, -(-p // n)
+        rows_of = np.repeat(rows_of, n, axis=0)
+        share_of = np.arange(len(rows_of)) - np.repeat(np.cumsum(n) - n, n)
+        rows_of[:, 7] = share_of
+        rows_of[:, 9] += share_of.astype(np.int32)
+        items.append(rows_of[np.argsort(-rows_of[:, 10], kind="stable")])      # the longest first
     return Lists(items[0], items[1], np.asarray(listed, dtype=np.int32), n_parts)
 
 

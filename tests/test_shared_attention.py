@@ -89,7 +89,7 @@ def test_a_plan_ends_when_pages_change():
     assert t.group.version != before
 
 
-@pytest.mark.parametrize("seed", range(30))
+@pytest.mark.parametrize("seed", range(60))
 def test_every_key_that_a_row_sees_is_in_one_of_its_items(seed):
     rng = random.Random(seed)
     window = rng.choice([None, None, 70, 200, 300])
@@ -103,10 +103,9 @@ def test_every_key_that_a_row_sees_is_in_one_of_its_items(seed):
     which = rng.sample(range(len(t.slots)), rng.randint(1, len(t.slots)))
     for i in which:
         t.bring([i], [1])
-    news = [rng.choice([1, 1, min(len(t.k[i]), rng.randint(1, 40), 64)]) for i in which]
-    news = [n if not window else 1 for n in news]
-    which = [i for i, n in sorted(zip(which, news), key=lambda x: len(t.k[x[0]]) > x[1])]
-    news = [n if not window else 1 for n in [min(news[0], len(t.k[i])) for i in which]]
+    news = [1 if window and t.group.ring_pages * 64 < window + 64 else min(len(t.k[i]), rng.choice([1, 1, 3, 40, 64])) for i in which]
+    order = sorted(range(len(which)), key=lambda i: len(t.k[which[i]]) > news[i])
+    which, news = [which[i] for i in order], [news[i] for i in order]
     step = t.step(which, news)
     plan = sa.plan(t.group, step)
     per = rng.choice([1, 2, 3, 5, 16, 20])
@@ -114,9 +113,10 @@ def test_every_key_that_a_row_sees_is_in_one_of_its_items(seed):
     pos, seq = step.token_pos.tolist(), step.token_seq.tolist()
     seen = [dict() for _ in pos]
     parts = [set() for _ in pos]
-    for j, (row0, n_rows, slot, lp0, lp1, skip0, skip1, share, n_shares, part, _, _) in enumerate(made.items.tolist() + made.big.tolist()):
+    for j, (row0, n_rows, slot, lp0, lp1, skip0, skip1, share, n_shares, part, _, _, *inline) in enumerate(made.items.tolist() + made.big.tolist()):
         rows = made.rows[row0:row0 + n_rows].tolist()
-        assert n_rows * per <= 128 if j >= len(made.items) else n_rows * min(per, 16) <= 16 or n_rows == 1
+        assert n_rows * per <= 128 if j >= len(made.items) else n_rows * per <= 8 or n_rows == 1
+        assert j >= len(made.items) or inline[:n_rows] == rows
         lo = min(max(0, pos[r] + 1 - window) // PAGE if window else 0 for r in rows)
         hi = max(pos[r] // PAGE for r in rows)
         pages = [p for p in range(max(lp0, lo), min(lp1, hi + 1)) if not skip0 <= p < skip1]
@@ -161,7 +161,19 @@ def test_refusals():
     assert not sa.supports(24) and not sa.supports(272) and sa.supports(80)
 
 
-@pytest.mark.parametrize("pages,per_item", [([1], 1), ([125] + [2] * 8, 4), ([61] * 8 + [6] * 64, 16), ([2000] * 16, 8)])
-def test_shares_fill_the_sms(pages, per_item):
-    n = sa.share_pages(pages, per_item)
-    assert n >= 2 and sum(-(-p // n) for p in pages) * per_item <= 148 + per_item * len(pages)
+@pytest.mark.parametrize("small,big,kv", [([1], [], 1), ([125] * 2 + [2] * 8, [], 4), ([6] * 64, [61] * 8, 16), ([], [2000] * 4, 8), ([3] * 200, [], 8),
+                                          ([], [46] * 3 + [2] * 5, 4)])
+@pytest.mark.parametrize("dim", [16, 64, 128, 256])
+def test_shares_leave_no_round_of_big_items_nearly_empty(small, big, kv, dim):
+    n_small, n_big = sa.shares(np.asarray(small, dtype=np.int64), np.asarray(big, dtype=np.int64), np.asarray([128] * len(big), dtype=np.int64), kv, kv, dim, sum(small) + sum(big))
+    assert n_small >= 1 and n_big >= 1
+    items = sum(-(-p // n_big) for p in big) * kv
+    assert items <= 148 or len(big) * kv > 148 or items > 2 * 148 - 8 * kv
+
+
+def test_blocks_of_few_pairs_and_of_many():
+    rows = [range(i, i + 1) for i in range(40)]
+    made = sa.lists([(list(range(8)), 0, 50), (list(range(8, 40)), 0, 60)], rows, list(range(40)), [4000] * 40, 40, 2, 4, 128, None, True)
+    assert sorted({it[1] for it in made.items.tolist()}) == [1, 4] and {it[1] for it in made.big.tolist()} == {32}
+    plain = sa.lists([(list(range(40)), 0, 60)], rows, list(range(40)), [4000] * 40, 40, 2, 4, 128, None, False)
+    assert len(plain.big) == 0 and max(it[1] for it in plain.items.tolist()) == 4
