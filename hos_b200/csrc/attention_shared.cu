@@ -908,6 +908,7 @@ struct SharedWork {
     const int* rows;
     const int* page_table;
     int most, big_most;        // how many items there may be (what the grids are made for)
+    int sms;                   // for the small ones
     int parts;                 // places of a (row, head) in the workspace
     int table_stride, ring_pages, n_heads, n_kv_heads, window;
 };
@@ -964,11 +965,11 @@ extern "C" int hos_attn_shared(const void* q, int q_stride, void* out, int out_s
             set = true;
         }
         const long long items = (long long)k.most * k.n_kv_heads * ((group + kPairs - 1) / kPairs);
-        const int places = kCtasPerSm * sm_count_cached(), grid = (int)(items < places ? items : places);
+        const int places = kCtasPerSm * (k.sms > 0 ? k.sms : sm_count_cached()), grid = (int)(items < places ? items : places);
         launch_ahead(k.big_most > 0 || pdl_enabled(), attn_shared_kernel, dim3(grid), dim3(kThreads), kShared, stream, a);
         if ((rc = check_launch("attn_shared"))) return rc;
     }
-    // many parts of few rows: eight warps a (row, head) (8 rows of 8 heads of 256, 33 parts: 6.8 us with one, MERGE8)
+    // many parts of few rows: eight warps a (row, head) (8 rows of 8 heads of 256, 33 parts: 6.8 us with one, 3.2 with eight)
     const int merged = n_rows * k.n_heads;
     auto merge = [&](auto kernel, int blocks) {
         launch_ahead(true, kernel, dim3(blocks), dim3(256), 0, stream, workspace, reinterpret_cast<const float2*>(part_ml), k.n_parts, k.parts, n_rows,

@@ -18,7 +18,6 @@ MAX_HEAD_DIM = 256
 OPEN = 1 << 30                 # a page behind every sequence's last
 ITEM_INTS = 20
 PAIRS, BLOCK = 8, 128          # (row, head) pairs of an item, of a big one
-FEW_PAIRS = 16                 # up to so many pairs are several small blocks
 MOST_PARTS = 64 << 20          # bytes of the parts that wait for the merge
 
 _libs: Dict[int, ops.Library] = {}
@@ -55,17 +54,17 @@ class SharedPlan:
 
 
 class Lists:
-    """Items (of up to 8 pairs, then of up to 128), their rows, and each row's number of parts, on the host."""
+    """Items (of up to 8 pairs, then of up to 128), their rows, each row's number of parts, and SMs for the small ones, on the host."""
 
-    def __init__(self, items: np.ndarray, big: np.ndarray, rows: np.ndarray, n_parts: np.ndarray):
-        self.items, self.big, self.rows, self.n_parts = items, big, rows, n_parts
+    def __init__(self, items: np.ndarray, big: np.ndarray, rows: np.ndarray, n_parts: np.ndarray, sms: int):
+        self.items, self.big, self.rows, self.n_parts, self.sms = items, big, rows, n_parts, sms
         self.parts = int(n_parts.max()) if n_parts.size else 0
 
 
 class SharedWork(ctypes.Structure):
     """A list of work as csrc/attention_shared.cu takes it."""
     _fields_ = [(name, ctypes.c_void_p) for name in ("counts", "n_parts", "items", "big_items", "rows", "page_table")] + \
-               [(name, ctypes.c_int) for name in ("most", "big_most", "parts", "table_stride", "ring_pages", "n_heads", "n_kv_heads", "window")]
+               [(name, ctypes.c_int) for name in ("most", "big_most", "sms", "parts", "table_stride", "ring_pages", "n_heads", "n_kv_heads", "window")]
 
 
 class Work:
@@ -85,7 +84,7 @@ class Work:
         base = self.array.data_ptr()
         items, big = base + 4 * at, base + 4 * (at + made.items.size)
         self.parts = made.parts
-        self.fields = SharedWork(base, base + 16, items, big, big + 4 * made.big.size, table.data_ptr(), len(made.items), len(made.big), made.parts,
+        self.fields = SharedWork(base, base + 16, items, big, big + 4 * made.big.size, table.data_ptr(), len(made.items), len(made.big), made.sms, made.parts,
                                  table.shape[1], group.ring_pages, n_heads, need.n_kv_heads, need.window or 0)
         self.address = ctypes.addressof(self.fields)
         self.floats = n * n_heads * made.parts * (need.head_dim + 2)
@@ -96,15 +95,18 @@ def has_big(head_dim: int) -> bool:
     return head_dim in (64, 128, 256)
 
 
-# Microseconds of an item, by head size (64, 128, 256): a small one and a page of it (a CTA takes two side by side), a big one and a page of it,
-# of a CTA by itself; and bytes of pages and of parts a microsecond, of all.  Measured (B200): 1,024 pages of 128 numbers for 32 rows of 4
-# heads in shares of 16 and 64, 25.3 and 63.9 us; 64 rows of 16 pages each, 8 heads of 256 over 4, 49.8 us of which the bytes are 41.0.
-SMALL_US, BIG_US = 2.0, 8.0
-BYTES_US, PART_BYTES_US = 6.0e6, 5.0e6
+# The estimate, us.  A small item 3.0 and a page of it 0.35 + 0.003 head_dim; what follows on the same SM 1.0 (the other group's pages hide the
+# rest) and its pages, of heads of up to 128 in half the time (two CTAs).  A big item 9.0 and a page of it 0.5 + head_dim / 480.
+# Pages come at 5.8 TB/s (out of L2 no faster: 125 pages read by two blocks of 8 pairs take 20 us, by one of 16 pairs, 4 kv heads of 256, 17), parts
+# are written and read at 5 TB/s.  Measured (B200), 8 answers on 8,000 keys, 8 heads of 256 over 4, shares of 5 / 8 / 16 / 32 pages of a block of
+# 16 pairs 19.9 / 21.0 / 27.9 / 44.3 us; of 8 / 16 / 32 pages of two blocks of 8 pairs 19.5 / 26.5 / 45.4; 16 heads of 128 over 16, of 4 / 16 / 32 / 64
+# pages of two blocks of 8 pairs 31.3 / 26.4 / 37.4 / 62.4.
+SMALL_US, SMALL_MORE_US, BIG_US = 3.0, 1.0, 9.0
+BYTES_US, PART_BYTES_US = 5.8e6, 5.0e6
 
 
 def _page_us(head_dim: int) -> tuple:
-    return 0.2 + head_dim / 800, 0.6 + head_dim / 550
+    return 0.35 + 0.003 * head_dim, 0.5 + head_dim / 480
 
 
 def _cuts(pages: np.ndarray):
@@ -113,37 +115,51 @@ def _cuts(pages: np.ndarray):
     lengths, n = [], 2
     while n < most:
         lengths.append(n)
-        n = max(n + 1, n * 5 // 4)
+        n = max(n + 1, n * 6 // 5)
     lengths.append(most)
-    return lengths, -(-pages[:, None] // np.asarray(lengths)) if pages.size else np.zeros((0, len(lengths)), dtype=np.int64)
+    return np.asarray(lengths), -(-pages[:, None] // np.asarray(lengths)) if pages.size else np.zeros((0, len(lengths)), dtype=np.int64)
 
 
 def shares(small: np.ndarray, big: np.ndarray, big_pairs: np.ndarray, per_item: int, kv: int, head_dim: int, distinct: int) -> tuple:
-    """(pages of a small share, of a big one) for small blocks and big blocks of so many pages, `distinct` of them not the same: the cut that
-    makes the step shortest by the estimate above.  An item is run per_item times (a big one kv times); big ones have an SM for
-    themselves, small ones take what is left, then all."""
+    """(pages of a small share, of a big one, SMs for the small ones) for small blocks and big blocks of so many pages, `distinct` pages in all
+    counting shared ones once: the cut that makes the step shortest by the estimate above.  An item is run per_item times (a big one kv
+    times).  Big items have an SM each; the small ones run beside them on the SMs that are left, or after them on all."""
     sms, (small_page, big_page) = ops.sm_count(), _page_us(head_dim)
-    read = 256.0 * head_dim * distinct * kv / BYTES_US
+    at_once = 2 if head_dim <= 128 else 1
     part_us = (head_dim + 2) * 8.0 / PART_BYTES_US
+    tile_us = 256.0 * head_dim / BYTES_US
     lengths, splits = _cuts(small)
     items = splits.sum(axis=0) * per_item
-    s_work = items * SMALL_US + float(small.sum()) * per_item * small_page
-    s_long = np.where(items > 0, SMALL_US + np.asarray(lengths) * small_page, 0.0)
-    s_parts = items * 8.0 * part_us
+    work = items * SMALL_MORE_US + float(small.sum()) * per_item * small_page / at_once       # of one SM
+    alone = np.where(items > 0, SMALL_US + lengths * small_page, 0.0)
     big_lengths, big_splits = _cuts(big)
-    items = big_splits.sum(axis=0) * kv
-    b_work = items * BIG_US + float(big.sum()) * kv * big_page
-    b_long = np.where(items > 0, -(-items // sms) * (BIG_US + np.asarray(big_lengths) * big_page), 0.0)
-    b_parts = (big_splits * big_pairs[:, None]).sum(axis=0) * kv * part_us
-    us = np.maximum(np.maximum(b_long[:, None], s_long), np.maximum((b_work[:, None] + s_work) / sms, read)) + b_parts[:, None] + s_parts
+    big_items = big_splits.sum(axis=0) * kv
+    rounds = -(-big_items // sms)
+    big_us = rounds * (BIG_US + big_lengths * big_page) if big.size else np.zeros(len(big_lengths))
+    left = np.maximum(0, sms - big_items)
+    # beside the big ones, or after them
+    beside = np.where((left > 0)[:, None], np.maximum(alone, SMALL_US + work / np.maximum(1, left)[:, None]), np.inf) if small.size else np.zeros((len(big_lengths), len(lengths)))
+    after = big_us[:, None] + np.maximum(alone, np.where(items > 0, SMALL_US + work / sms, 0.0))
+    us = np.minimum(np.maximum(big_us[:, None], beside), after)
+    us = np.maximum(us, tile_us * max(distinct * kv, float(small.sum()) * per_item + float(big.sum()) * kv) + SMALL_US)
+    us = us + (big_splits * big_pairs[:, None]).sum(axis=0)[:, None] * kv * part_us + items * 8.0 * part_us
     i, j = divmod(int(np.argmin(us)), len(lengths))
-    return lengths[j], big_lengths[i]
+    spare = int(left[i])
+    return int(lengths[j]), int(big_lengths[i]), spare if spare and big.size and max(big_us[i], beside[i, j]) <= after[i, j] else sms
+
+
+def is_big(pairs: int, pages: int, head_dim: int) -> bool:
+    """Whether a block of so many pairs over so many pages is one for the kernel of blocks of 128 pairs, or several of up to 8: by what
+    either takes an SM (2 pairs of rows and heads that need 16 columns, one page of 128 numbers: 752 of them 49.9 us as big items, 23.1 as
+    small ones)."""
+    small_page, big_page = _page_us(head_dim)
+    return pairs > PAIRS and -(-pairs // PAIRS) * (SMALL_MORE_US + pages * small_page) > -(-pairs // BLOCK) * (BIG_US + pages * big_page)
 
 
 def lists(runs, rows: Sequence[range], slots: Sequence[int], lengths: Sequence[int], n_rows: int, per: int, kv: int, head_dim: int,
           window: Optional[int], big: bool) -> Lists:
-    """The work: a run's rows in blocks of up to 8 pairs, or, where they are more than FEW_PAIRS and a kernel has such blocks (`big`), of up to
-    128, over the run's pages, each sequence's over the rest of its own."""
+    """The work: a run's rows in blocks of up to 8 pairs, or of up to 128 where a kernel has such blocks (`big`) and that is faster, over the
+    run's pages, each sequence's over the rest of its own."""
     big = big and per <= BLOCK
     chunks = -(-per // PAIRS)
     n_seqs = len(slots)
@@ -156,7 +172,7 @@ def lists(runs, rows: Sequence[range], slots: Sequence[int], lengths: Sequence[i
     made = []                                                # which of both, one after another
 
     def cut(of: Sequence[int], *rest) -> None:
-        large = big and len(of) * per > FEW_PAIRS
+        large = big and is_big(len(of) * per, rest[-1], head_dim)
         size = max(1, (BLOCK if large else PAIRS) // per)
         n = -(-len(of) // size)                              # blocks of like sizes
         for i in range(n):
@@ -174,9 +190,9 @@ def lists(runs, rows: Sequence[range], slots: Sequence[int], lengths: Sequence[i
     rest = np.maximum(1, behind - first - np.maximum(0, np.minimum(behind, skip[:, 1]) - np.maximum(first, skip[:, 0])))
     distinct += int(rest.sum())
     for i, (slot, of, lo_hi, n) in enumerate(zip(slots, rows, skip.tolist(), rest.tolist())):
-        if len(of) == 1:
-            blocks[big and per > FEW_PAIRS].append((of, slot, 0, OPEN, *lo_hi, n))
-            made.append(big and per > FEW_PAIRS)
+        if len(of) == 1 and per <= PAIRS:                    # (most of a decoding step's)
+            blocks[0].append((of, slot, 0, OPEN, *lo_hi, n))
+            made.append(0)
         else:
             cut(of, slot, 0, OPEN, *lo_hi, n)
     pages = [np.asarray([b[6] for b in of], dtype=np.int64) for of in blocks]
@@ -206,7 +222,7 @@ def lists(runs, rows: Sequence[range], slots: Sequence[int], lengths: Sequence[i
         rows_of[:, 7] = share_of
         rows_of[:, 9] += share_of.astype(np.int32)
         items.append(rows_of[np.argsort(-rows_of[:, 10], kind="stable")])      # the longest first
-    return Lists(items[0], items[1], np.asarray(listed, dtype=np.int32), n_parts)
+    return Lists(items[0], items[1], np.asarray(listed, dtype=np.int32), n_parts, share[2])
 
 
 def plan(group, step) -> SharedPlan:

@@ -165,15 +165,15 @@ def test_refusals():
                                           ([], [46] * 3 + [2] * 5, 4)])
 @pytest.mark.parametrize("dim", [16, 64, 128, 256])
 def test_shares_leave_no_round_of_big_items_nearly_empty(small, big, kv, dim):
-    n_small, n_big = sa.shares(np.asarray(small, dtype=np.int64), np.asarray(big, dtype=np.int64), np.asarray([128] * len(big), dtype=np.int64), kv, kv, dim, sum(small) + sum(big))
-    assert n_small >= 1 and n_big >= 1
+    n_small, n_big, sms = sa.shares(np.asarray(small, dtype=np.int64), np.asarray(big, dtype=np.int64), np.asarray([128] * len(big), dtype=np.int64), kv, kv, dim, sum(small) + sum(big))
+    assert n_small >= 1 and n_big >= 1 and 1 <= sms <= 148
     items = sum(-(-p // n_big) for p in big) * kv
     assert items <= 148 or len(big) * kv > 148 or items > 2 * 148 - 8 * kv
 
 
 def test_blocks_of_few_pairs_and_of_many():
     rows = [range(i, i + 1) for i in range(40)]
-    made = sa.lists([(list(range(8)), 0, 50), (list(range(8, 40)), 0, 60)], rows, list(range(40)), [4000] * 40, 40, 2, 4, 128, None, True)
+    made = sa.lists([(list(range(4)), 0, 50), (list(range(8, 40)), 0, 60)], rows, list(range(40)), [4000] * 40, 40, 2, 4, 128, None, True)
     assert sorted({it[1] for it in made.items.tolist()}) == [1, 4] and {it[1] for it in made.big.tolist()} == {32}
     plain = sa.lists([(list(range(40)), 0, 60)], rows, list(range(40)), [4000] * 40, 40, 2, 4, 128, None, False)
     assert len(plain.big) == 0 and max(it[1] for it in plain.items.tolist()) == 4
