@@ -13,6 +13,10 @@
 // other group's pages.  Items of up to 128 pairs: tcgen05, further down.  Weights are rounded to bfloat16 for the product with the
 // values (2^-8 of each at most), their sum is of the weights before that rounding.
 //
+// What lies in a page where none of a block's rows looks (behind the last token, before the window: another sequence's leftovers, NaN among
+// them) is kept out of the products: such values are zeroed in shared memory, as a weight of 0 times NaN would be NaN.  A NaN that a row does
+// see, in its query, a key or a value, makes the row's output NaN: its part leaves with a maximum of +infinity, which no other part outweighs.
+//
 // Compiled per head size: -DHOS_HEAD_DIM=N, a multiple of 16 up to 256.
 #include "common.cuh"
 #include "kv_layout.cuh"
@@ -98,8 +102,9 @@ __device__ __forceinline__ Walk walk_of(const SharedArgs& a, const SharedItem& i
 }
 __device__ __forceinline__ int walk_page(const Walk& w, int i) { return i < w.count1 ? w.first + i : w.second + (i - w.count1); }
 // A small item's walk.  A closed range without a window needs no position: its pages lie below every row's.
-__device__ __forceinline__ Walk small_walk(const SharedArgs& a, const SharedItem& it, int lane) {
-    int low = 0, high = kOpen;
+__device__ __forceinline__ Walk small_walk(const SharedArgs& a, const SharedItem& it, int lane, int& low, int& high) {
+    low = 0;
+    high = kOpen;
     if (a.window > 0 || it.lp1 >= kOpen) {
         const int pos = lane < it.n_rows ? a.token_pos[it.rows[lane & 7]] : -1;
         low = __reduce_min_sync(0xffffffffu, lane < it.n_rows ? pos : kOpen);
@@ -144,7 +149,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attn_shared_kernel(Share
             if (work >= n_work) continue;
             const SharedItem& it = a.items[work / per_item];
             const int kvh = work % per_item / chunks, to = round % kGroups * kStages;
-            const Walk w = small_walk(a, it, lane);
+            int low, high;
+            const Walk w = small_walk(a, it, lane, low, high);
             const int* table = a.cache.page_table + (size_t)it.slot * a.cache.table_stride;
             for (int i0 = w.begin; i0 < w.end && ok; i0 += 32) {             // 32 pages looked up at a time
                 const int page_l = i0 + lane < w.end ? table[kv_table_entry(a.cache, walk_page(w, i0 + lane))] : 0;
@@ -201,11 +207,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attn_shared_kernel(Share
         if (work >= n_work) continue;
         const SharedItem& it = a.items[work / per_item];
         const int kvh = work % per_item / chunks, chunk = work % per_item % chunks;
-        const Walk w = small_walk(a, it, lane);
+        int low, high;
+        const Walk w = small_walk(a, it, lane, low, high);
         if (round % kGroups != who) {        // the other group's
             t += w.end - w.begin;
             continue;
         }
+        const int seen_from = a.window > 0 ? max(0, low + 1 - a.window) : 0;
+        const uint32_t whole = max(0, high - 14 - seen_from);    // 16 keys from one of so many on are seen by a row, every one
         const int heads = min(kPairs, group - chunk * kPairs), pairs = min(kPairs, it.n_rows * heads), part = it.part;
         meet();                              // the last item's readers are done
         if (tid < kPairs) {
@@ -279,6 +288,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attn_shared_kernel(Share
             if (ok) ok = mbar_wait_cycles(&v_full[s], parity, kWaitCycles);
             ok = __all_sync(0xffffffffu, ok) != 0;
             if (!ok) continue;
+            if ((uint32_t)(key0 - seen_from) >= whole) {     // values that no row sees; only this warp reads them
+                bf16* values = reinterpret_cast<bf16*>(ring + (size_t)s * 2 * kTileBytes + kTileBytes);
+                for (int c = lane; c < 16 * (HD / 8); c += 32) {
+                    const int r = c / (HD / 8);
+                    if (key0 + r > high || key0 + r < seen_from)
+                        *reinterpret_cast<uint4*>(values + tile_chunk_offset<HD>(warp * 16 + r, c % (HD / 8))) = make_uint4(0, 0, 0, 0);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // before the next page comes here
+                __syncwarp();
+            }
 #pragma unroll
             for (int dd = 0; dd < HD / 16; ++dd) {
                 uint32_t va[4];
@@ -304,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attn_shared_kernel(Share
                     b[dd * 16 + g] = o[dd][r];
                     b[dd * 16 + g + 8] = o[dd][2 + r];
                 }
-                if (g == 0) ml[warp * kPairs + p] = make_float2(m_run[r], l_run[r]);
+                if (g == 0) ml[warp * kPairs + p] = make_float2(l_run[r] != l_run[r] ? INFINITY : m_run[r], l_run[r]);
             }
         }
         meet();
@@ -378,21 +397,22 @@ __device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
     return d;
 }
-// tanh: for |x| <= 0.55 x + x^3 (a + x^2 (b + x^2 c)), relative error 1.3e-6; 1 - 2 / (1 + e^2x) else, absolute error 2e-7.
-constexpr float kTanhSmall = 0.55f;
+// tanh: for |x| <= 1/2  x + x^3 (a + x^2 (b + x^2 c)) with the a, b, c whose largest relative error there is least (fitted by repeatedly
+// weighted least squares; 6.9e-7 in 32 bits); 1 - 2 / (1 + e^2x) else, absolute error 2e-7.
+constexpr float kTanhSmall = 0.5f, kTanhA = -0.333281606f, kTanhB = 0.132053599f, kTanhC = -0.0447506383f;
 __device__ __forceinline__ float tanh_of(float x) {
     const float x2 = x * x;
-    return fabsf(x) <= kTanhSmall ? fmaf(fmaf(fmaf(-0.043099623f, x2, 0.13152355f), x2, -0.33324513f) * x2, x, x)
+    return fabsf(x) <= kTanhSmall ? fmaf(fmaf(fmaf(kTanhC, x2, kTanhB), x2, kTanhA) * x2, x, x)
                                   : fmaf(-2.f, rcp_approx(1.f + ex2_approx(2.88539008f * x)), 1.f);
 }
-// of 64 scores times `pre`; `small`: none of the warp's is larger than 0.55
+// of 64 scores times `pre`; `small`: none of the warp's is larger than 1/2
 __device__ __forceinline__ void tanh_scores(Two (&t)[32], float pre, bool small) {
     if (small) {
-        const Two a = two_of(-0.043099623f, -0.043099623f), b = two_of(0.13152355f, 0.13152355f), c = two_of(-0.33324513f, -0.33324513f), f = two_of(pre, pre);
+        const Two c = two_of(kTanhC, kTanhC), b = two_of(kTanhB, kTanhB), a = two_of(kTanhA, kTanhA), f = two_of(pre, pre);
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
             const Two x = mul2(t[i], f), x2 = mul2(x, x);
-            t[i] = fma2(mul2(fma2(fma2(a, x2, b), x2, c), x2), x, x);
+            t[i] = fma2(mul2(fma2(fma2(c, x2, b), x2, a), x2), x, x);
         }
     } else {
 #pragma unroll
@@ -557,6 +577,7 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             const uint64_t k_desc = desc_kmajor(smem_u32(ring)), p_desc = desc_kmajor(smem_u32(p_s)),
                            v_desc = desc_mnmajor(smem_u32(ring) + kTileBytes, kTileBlockBytes);
             const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
+            const int seen_from = a.window > 0 ? max(0, low + 1 - a.window) : 0;
             // S of tile `next` (two ahead of the values at most) and O of tile j, whichever may go first: to wait for one of them in a fixed
             // order would hold up the other
             int next = 0, j = 0, k_stage = 0, v_stage = 0;
@@ -583,6 +604,18 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 const bool may_o = next > j && mbar_test(&p_full[pb], (j >> 1) & 1) && mbar_test(&v_full[v_stage], v_phase);
                 if (__all_sync(0xffffffffu, may_o)) {
                     tc_fence_after_sync();
+                    const int key0 = walk_page(w, w.begin + j) * kPageTokens;
+                    if (key0 + kPageTokens - 1 > high || key0 < seen_from) {     // values that no row sees
+                        unsigned char* values = ring + (size_t)v_stage * 2 * kTileBytes + kTileBytes;
+#pragma unroll 1
+                        for (int i = lane; i < kPageTokens * (HD / 8); i += 32) {
+                            const int key = i / (HD / 8), c = i % (HD / 8);
+                            if (key0 + key > high || key0 + key < seen_from)
+                                *reinterpret_cast<uint4*>(values + (c >> 3) * kTileBlockBytes + key * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                    }
                     const uint64_t at_p = p_desc + pb * (kPBytes / 16), at_v = v_desc + (uint32_t)v_stage * (2 * kTileBytes / 16);
 #pragma unroll
                     for (int ks = 0; ks < kPageTokens / 16; ++ks)
@@ -777,11 +810,14 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         if (side == (last & 1)) row_max[r] = m_mine;             // the last tile's is the row's (without tiles: -inf, of group 1)
         asm volatile("bar.sync 3, 256;" ::: "memory");
         const float m_row = row_max[r];
-        row_sum[side * kBlock + r] = m_mine == -INFINITY ? 0.f : l_run * ex2_approx((m_mine - m_row) * c2);
+        row_sum[side * kBlock + r] = m_mine == -INFINITY ? l_run : l_run * ex2_approx((m_mine - m_row) * c2);      // (no key: 0, or NaN)
         asm volatile("bar.sync 3, 256;" ::: "memory");
         if (ok) {
             const size_t at = ((size_t)row * a.n_heads + kvh * group + r % group) * a.parts + part;
-            if (side == 0 && r < pairs) a.part_ml[at] = make_float2(m_row * c_logit, row_sum[r] + row_sum[kBlock + r]);
+            if (side == 0 && r < pairs) {
+                const float l = row_sum[r] + row_sum[kBlock + r];
+                a.part_ml[at] = make_float2(l != l ? INFINITY : m_row * c_logit, l);
+            }
             if (n_tiles > 0 && !idle) {
                 // 32 rows by 32 numbers of a warp at a time through shared memory, so that whole lines are written
                 unsigned char* stage = p_s + (size_t)(warp - 2) * 4096;
@@ -912,9 +948,6 @@ struct SharedWork {
     int parts;                 // places of a (row, head) in the workspace
     int table_stride, ring_pages, n_heads, n_kv_heads, window;
 };
-
-// 1: blocks of up to 128 pairs have a kernel for this head size.
-extern "C" int hos_attn_shared_big() { return HD == 64 || HD == 128 || HD == 256; }
 
 // out[n_rows, n_heads * head_dim] = softmax(c tanh(scale q . k / c)) v by the items of the work; see the head of this file.  workspace:
 // n_rows * n_heads * parts * (head_dim + 2) floats.

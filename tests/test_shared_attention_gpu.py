@@ -174,3 +174,60 @@ def test_refusals():
     t.bring([f], [64])
     with pytest.raises(KernelError, match="changed"):
         sa.attend(q, q.clone(), step, t.view, plan, 4, 1.0)
+
+
+@pytest.mark.parametrize("dim,per,forks,news,window", [(64, 2, 3, 1, None), (64, 2, 3, 1, 100), (128, 2, 40, 1, None), (256, 2, 40, 1, 70), (128, 4, 2, 37, 90), (80, 3, 6, 5, 100),
+                                                       (64, 2, 70, 1, 130), (64, 2, 3, 1, 5), (128, 2, 40, 1, 3)])
+def test_what_no_row_sees_may_be_anything(dim, per, forks, news, window):
+    """NaN and infinities in the pages behind every sequence's last token, before its window, and in the pages that nothing holds: the
+    outputs are the same to the bit."""
+    t = Tree(2, dim, window=window, seed=dim, chunk=64, slots=80)
+    a = t.new(300)
+    all_ = [a] + t.fork(a, forks)
+    for j, i in enumerate(all_):
+        t.bring([i], [news + j % 5])
+    step = t.step(all_, [news] * len(all_))
+    q = torch.randn(news * len(all_), 2 * per * dim, generator=t.gen).to(torch.bfloat16).cuda()
+    outs = []                                                # (a window of 3 or 5: less than the 16 keys of a warp)
+    for poison in (None, float("nan"), float("inf"), float("-inf")):
+        if poison is not None:
+            seen = torch.zeros(t.group.k[0].shape[0], 64, dtype=torch.bool)         # (page, place)
+            for i in all_:
+                n = len(t.k[i])
+                for pos in range(max(0, n - news + 1 - window) if window else 0, n):
+                    entry = pos // 64 % t.group.ring_pages if t.group.ring_pages else pos // 64
+                    seen[int(t.group.table_host[t.slots[i], entry]), pos % 64] = True
+            for pages in (t.group.k[0], t.group.v[0]):
+                rows = pages.view(pages.shape[0], 2, 64, dim)                       # (a token's numbers stay in its row)
+                rows.masked_fill_(~seen.cuda()[:, None, :, None], poison)
+        out = torch.empty_like(q)
+        sa.attend(q, out, step, t.view, sa.plan(t.group, step), 2 * per, dim ** -0.5, 20.0, window)
+        outs.append(out)
+    assert outs[0].isfinite().all()
+    for out in outs[1:]:
+        assert torch.equal(out, outs[0])
+
+
+@pytest.mark.parametrize("dim,forks,cap", [(64, 3, 0.0), (64, 70, 30.0), (128, 70, 0.0), (256, 70, 30.0), (80, 5, 0.0)])
+def test_a_nan_that_a_row_sees_is_its_own(dim, forks, cap):
+    t = Tree(2, dim, seed=3, slots=80)
+    a = t.new(1500)
+    all_ = [a] + t.fork(a, forks)
+    t.bring(all_, [3] * len(all_))
+    step = t.step(all_, [1] * len(all_))
+    plan = sa.plan(t.group, step)
+    q = torch.randn(len(all_), 4 * dim, generator=t.gen).to(torch.bfloat16).cuda()
+    out, bad = torch.empty_like(q), torch.empty_like(q)
+    sa.attend(q, out, step, t.view, plan, 4, dim ** -0.5, cap, None)
+    q[1, dim + 3] = float("nan")
+    q[2] = float("nan")
+    sa.attend(q, bad, step, t.view, plan, 4, dim ** -0.5, cap, None)
+    hit = torch.zeros_like(q, dtype=torch.bool)
+    hit[1, dim:2 * dim] = True
+    hit[2] = True
+    assert bad[hit].isnan().all() and torch.equal(bad[~hit], out[~hit])
+    place = int(t.group.table_host[t.slots[all_[3]], 1502 // 64])                   # the last sequence's own page but one
+    t.group.v[0].view(-1, 2, 64, dim)[place, 1, 1502 % 64] = float("nan")           # a value of kv head 1 of one sequence alone
+    sa.attend(q, bad, step, t.view, plan, 4, dim ** -0.5, cap, None)
+    hit[3, 2 * dim:] = True
+    assert bad[hit].isnan().all() and torch.equal(bad[~hit], out[~hit])
