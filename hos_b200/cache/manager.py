@@ -77,7 +77,7 @@ class CacheManager:
         self.stores: List[CallStore] = []
         for i, need in enumerate(kv_needs):
             src = cache_from[i]
-            kv, owns = None, True
+            kv, owns, group = None, True, None
             if need is not None:
                 owner = i if src is None else src
                 if owner not in placed:
@@ -86,10 +86,11 @@ class CacheManager:
                 if src is not None and kv_needs[src] != need:
                     raise CacheError(f"entry {i} reads the cache of entry {src}, whose keys have "
                                      f"another shape or window")
-                kv, owns = self.groups[gi].view(j), src is None
+                group = self.groups[gi]
+                kv, owns = group.view(j), src is None
             state = {s.name: torch.zeros((self.n_slots,) + tuple(s.shape), dtype=s.dtype,
                                          device=self.device) for s in state_needs[i]}
-            self.stores.append(CallStore(kv, owns, state))
+            self.stores.append(CallStore(kv, owns, state, group))
         # what the embedding keeps per sequence (e.g. the previous token, for a table of token pairs)
         self.embedding_store = CallStore(None, True, {
             s.name: torch.zeros((self.n_slots,) + tuple(s.shape), dtype=s.dtype, device=self.device)

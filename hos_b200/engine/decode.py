@@ -29,8 +29,10 @@ import numpy as np
 import torch
 
 from .. import ops
+from ..parts import shared_attention
 from ..parts.base import StepInfo
 from ..sampling.sampler import SamplingParams
+from ..sampling.scores import TokenScores, log_probs, scored_tokens
 
 BUCKETS = (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256)
 META = 2 + ops.MAX_STOPS        # live rows, number of stop ids, the stop ids
@@ -124,6 +126,8 @@ class DecodeSession:
         # sampled tokens on their way to the host: pinned buffers used in turn
         self._fetch_hosts = [torch.zeros(b, dtype=torch.int32).pin_memory() for _ in range(3)]
         self._fetch_turn = 0
+        self._scores = {}                       # number of alternatives -> static TokenScores [b]; and their pinned buffers
+        self._score_hosts = {}
         self.logits: Optional[torch.Tensor] = None
         self._programs = {}                     # key -> (graph or None, logits buffer)
         self._pool = None                       # the programs' buffers share one pool: only one of them runs at a time
@@ -134,6 +138,9 @@ class DecodeSession:
         self._planned_fill = ()                 # and how full of keys the sequences are, per window (see fill_class)
         self._seen_len, self._seen_fill = self._max_len, ()     # what the step at hand really holds: a new capture plans with it
         self._windows = sorted({g.need.window or 0 for g in runner.cache.groups})
+        # attention over pages that sequences share: the lists of work by (cache group, query heads), which of them the step at hand uses, and
+        # for which slots and pages they were made
+        self._page_works, self.page_work, self._page_key, self._paged_for = {}, {}, (), None
         self.n_live = 0
 
     @property
@@ -147,7 +154,7 @@ class DecodeSession:
                         max_len_after=self._seen_len, slots_host=(), cu_host=tuple(range(self.b + 1)),
                         starts_host=(), token_slot=self.slot,      # row n is sequence n here
                         min_live=self._planned_live[0], max_live=self._planned_live[1], fills=self._seen_fill,
-                        replayed=True)
+                        replayed=True, share_pages=bool(self.page_work), page_work=dict(self.page_work))
 
     def upload(self, slots: Sequence[int], tokens: Optional[Sequence[int]] = None,
                stop_ids: Sequence[int] = (), longest: Optional[int] = None,
@@ -174,6 +181,7 @@ class DecodeSession:
                     for w in self._windows]
             self._seen_fill = tuple((w, min(1.0, total / float(n * most))) for w, total, most in held)
             self._planned_fill = tuple((w, fill_class(total, n, most)) for w, total, most in held)
+        self._share(slots, lengths)
         turn = self._turn
         self._turn ^= 1
         if self._copied[turn] is not None:
@@ -194,6 +202,31 @@ class DecodeSession:
         ev.record()
         self._copied[turn] = ev
 
+    def _share(self, slots: Sequence[int], lengths: Optional[Sequence[int]]) -> None:
+        """The lists of work for attention over pages that these sequences share, on the device (where the runner shares pages, the lengths are
+        known and it pays); made anew when the slots or their pages have changed."""
+        sharers = self.runner.sharers
+        if not sharers or lengths is None:
+            self.page_work, self._page_key, self._paged_for = {}, (), None
+            return
+        made_for = (tuple(slots), tuple(g.version for g, _ in sharers))
+        if made_for == self._paged_for:
+            return
+        self.page_work, key, plans = {}, [], {}
+        for i, (group, n_heads) in enumerate(sharers):
+            if id(group) not in plans:
+                plans[id(group)] = shared_attention.step_plan(group, slots, lengths)
+            plan = plans[id(group)]
+            if plan is None:
+                continue
+            work = self._page_works.get((id(group), n_heads))
+            if work is None:
+                work = self._page_works[id(group), n_heads] = shared_attention.ReplayedWork(group, n_heads, self.b)
+            if work.refill(plan.lists(n_heads)):
+                self.page_work[id(group), n_heads] = work
+                key.append((i, work.key))
+        self._page_key, self._paged_for = tuple(key), made_for
+
     # ---- what a step launches ---------------------------------------------------------------
     def _begin(self, flags: int, recent=None) -> None:
         c = self.runner.cache
@@ -206,7 +239,15 @@ class DecodeSession:
         self._begin(ops.BEGIN_ADVANCE)
         return r.model.step_logits(self._info(), r.cache)
 
-    def _forward_generate(self, p: SamplingParams) -> torch.Tensor:
+    def _score(self, logits: torch.Tensor, tokens: torch.Tensor, top: int) -> None:
+        """How likely the sampled tokens were, into the session's buffers."""
+        held = self._scores.get(top)
+        if held is None:
+            held = self._scores[top] = TokenScores.empty(self.b, top, logits.device)
+        n = logits.shape[0]
+        log_probs(logits, tokens, top, out=TokenScores(*(v[:n] if v is not None else None for v in held)))
+
+    def _forward_generate(self, p: SamplingParams, top: Optional[int] = None) -> torch.Tensor:
         r = self.runner
         penal = p.rep_penalty != 1.0 and p.repeat_last_n > 0
         recent = None
@@ -221,6 +262,8 @@ class DecodeSession:
         self._begin(flags, recent)
         logits = r.model.step_logits(self._info(), r.cache)
         sample_into(logits, self.sampled, p, self.uniforms, recent, self.recent_len)
+        if top is not None:
+            self._score(logits, self.sampled, top)
         c = r.cache
         ops.slot_end(c.record, c.recent, self.slot, self.meta, self.b, self.sampled)
         return logits
@@ -268,7 +311,7 @@ class DecodeSession:
             self.logits = fn()
             self.launches_per_step = ops.launch_count - before
             return self.logits
-        g, self.logits = self._program(key + (self._planned_len, self._planned_live, self._planned_fill), fn)
+        g, self.logits = self._program(key + (self._planned_len, self._planned_live, self._planned_fill, self._page_key), fn)
         g.replay()
         return self.logits
 
@@ -277,13 +320,13 @@ class DecodeSession:
         vocab] (a view of a static buffer when graphs are on: use it before the next run)."""
         return self._run(("step",), self._forward_step)[: self.n_live]
 
-    def run_generate(self, params: SamplingParams) -> None:
+    def run_generate(self, params: SamplingParams, top: Optional[int] = None) -> None:
         """One step whose input tokens are the ones sampled last; the new ones are sampled on the
-        device (`self.sampled`) and go into the slots' records."""
-        key = ("generate", params.temp, params.top_k, params.top_p, params.rep_penalty, params.repeat_last_n)
-        self._run(key, lambda: self._forward_generate(params))
+        device (`self.sampled`) and go into the slots' records.  `top`: their log probabilities, the entropy and that many alternatives too."""
+        key = ("generate", params.temp, params.top_k, params.top_p, params.rep_penalty, params.repeat_last_n, top)
+        self._run(key, lambda: self._forward_generate(params, top))
 
-    def sample_logits(self, logits: torch.Tensor, params: SamplingParams) -> None:
+    def sample_logits(self, logits: torch.Tensor, params: SamplingParams, top: Optional[int] = None) -> None:
         """Sample from logits [live rows, vocab] of a step that ran elsewhere (the sequences' first
         step), with the records' generators and recent tokens, as run_generate does after its own step."""
         n = logits.shape[0]
@@ -299,24 +342,38 @@ class DecodeSession:
                            self.recent_len if recent is not None else None)
         sample_into(logits, self.sampled[:n], params, self.uniforms[:n], recent[:n] if penal else None,
                     self.recent_len[:n])
+        if top is not None:
+            self._score(logits, self.sampled[:n], top)
         ops.slot_end(c.record, c.recent, self.slot, self.meta, self.b, self.sampled)
 
     # ---- sampled tokens to the host, without waiting --------------------------------------------
-    def fetch_start(self):
-        """Start copying the tokens just sampled to the host; hand the result to fetch_read later."""
+    def fetch_start(self, top: Optional[int] = None):
+        """Start copying the tokens just sampled (and, as run_generate was given `top`, their scores) to the host; hand the result to
+        fetch_read later."""
         turn = self._fetch_turn
         self._fetch_turn = (turn + 1) % len(self._fetch_hosts)
         host = self._fetch_hosts[turn]
         host[: self.b].copy_(self.sampled, non_blocking=True)
+        scores = None
+        if top is not None:
+            scores = self._score_hosts.get((turn, top))
+            if scores is None:
+                scores = self._score_hosts[turn, top] = TokenScores(*(torch.empty_like(v, device="cpu").pin_memory() if v is not None else None
+                                                                      for v in self._scores[top]))
+            for to, v in zip(scores, self._scores[top]):
+                if v is not None:
+                    to.copy_(v, non_blocking=True)
         ev = torch.cuda.Event()
         ev.record()
-        return host, ev, self.n_live
+        return host, ev, self.n_live, scores
 
     @staticmethod
     def fetch_read(handle) -> List[int]:
-        host, ev, n = handle
+        host, ev, n, scores = handle
         ev.synchronize()
         ops.check_errors()            # a kernel that gave up a wait: these tokens are not to be trusted
+        if scores is not None:
+            return scored_tokens(host[:n].tolist(), TokenScores(*(v[:n] if v is not None else None for v in scores)))
         return host[:n].tolist()
 
 

@@ -1,6 +1,7 @@
 """The Python entry point, in the manner of the reference's binding (py/src/lib.rs:12-92):
 `Engine(path)`, `generate(prompt, max_tokens=128, temp=0.0, top_k=40, top_p=0.95,
-rep_penalty=1.1, repeat_last_n=64, seed=42)`, `perplexity`, `bench`, `vocab_size`.
+rep_penalty=1.1, repeat_last_n=64, seed=42)`, `perplexity`, `bench`, `vocab_size`;
+beside them `score` and the log probabilities of generated tokens.
 Prompts and results are token ids (tokenizers are not part of this library): a
 prompt is a list of ids, or a list of such lists, which is run as batches.
 Bad input raises `ValueError` (every `HosError` is one), as the binding does.
@@ -14,8 +15,10 @@ from typing import List, Optional, Sequence, Tuple, Union
 import torch
 
 from ..config.base import ModelConfig
+from .. import ops
 from ..errors import HosError
-from ..sampling import SamplingParams, stream_seed
+from ..sampling import SamplingParams, ScoredToken, scored_tokens, stream_seed
+from ..sampling.scores import MAX_TOP
 from . import generate as gen
 from .runner import Runner
 
@@ -27,9 +30,10 @@ class _DeviceBackend:
     step, then record-driven single-token steps with sampling on the device.  Tokens come back
     through pinned buffers, fetched in the order in which they were sampled."""
 
-    def __init__(self, runner: Runner, params: SamplingParams):
+    def __init__(self, runner: Runner, params: SamplingParams, top: Optional[int] = None):
         self.runner = runner
         self.params = params
+        self.top = top                      # alternatives that come with each token's log probability; None: plain tokens
         self.admit, self.release, self.length = runner.admit, runner.release, runner.length
         self._queue: List[object] = []
         self._stops: Sequence[int] = ()
@@ -47,16 +51,16 @@ class _DeviceBackend:
                         restart=True)
         sess = r.decode_session(len(slots))
         sess.upload(slots, stop_ids=self._stops)
-        sess.sample_logits(logits, p)
-        self._queue.append(sess.fetch_start())
+        sess.sample_logits(logits, p, self.top)
+        self._queue.append(sess.fetch_start(self.top))
 
     def advance(self, slots) -> None:
         r = self.runner
         r.cache.extend_all(slots, [r.cache.lengths[s] + 1 for s in slots])
         sess = r.decode_session(len(slots))
         sess.upload(slots, stop_ids=self._stops, lengths=[r.cache.lengths[s] for s in slots])
-        sess.run_generate(self.params)
-        self._queue.append(sess.fetch_start())
+        sess.run_generate(self.params, self.top)
+        self._queue.append(sess.fetch_start(self.top))
 
     def fetch(self) -> List[int]:
         from .decode import DecodeSession
@@ -80,12 +84,14 @@ class Engine:
     max_tokens  tokens the cache holds (default: max_batch full contexts, at most 8192 each)
     weight_bits 4: attention projections and gated feed-forwards in 4 bits (None: as `dtype` says)
     cache_bits  4: keys and values in 4 bits
+    share_prefix  conversations forked from one another attend over what they share once for all of them, where that pays
+                (bfloat16 keys and values)
     """
 
     def __init__(self, path: Optional[str] = None, gpu: bool = True, dtype: str = "bfloat16",
                  max_batch: int = 8, max_tokens: Optional[int] = None,
                  max_seq_len: Optional[int] = None, weight_bits: Optional[int] = None,
-                 cache_bits: Optional[int] = None, _runner: Optional[Runner] = None):
+                 cache_bits: Optional[int] = None, share_prefix: bool = False, _runner: Optional[Runner] = None):
         self.max_batch = max_batch
         if _runner is not None:
             self.runner = _runner
@@ -99,7 +105,7 @@ class Engine:
             self.runner = Runner.from_folder(path, dtype=dtype, max_seq_len=max_seq_len,
                                              max_tokens=self._default_tokens(cfg, max_batch, max_tokens,
                                                                              max_seq_len),
-                                             weight_bits=weight_bits, cache_bits=cache_bits)
+                                             weight_bits=weight_bits, cache_bits=cache_bits, share_prefix=share_prefix)
         self.config = self.runner.config
         self.stop_ids: Tuple[int, ...] = tuple(self.runner.plan.stop_token_ids)
 
@@ -114,9 +120,10 @@ class Engine:
     def from_config(cls, config: ModelConfig, seed: int = 0, dtype: str = "bfloat16",
                     max_batch: int = 8, max_tokens: Optional[int] = None,
                     max_seq_len: Optional[int] = None, weight_bits: Optional[int] = None,
-                    cache_bits: Optional[int] = None) -> "Engine":
+                    cache_bits: Optional[int] = None, share_prefix: bool = False) -> "Engine":
         """A model with random weights made on the device (no files)."""
         runner = Runner.from_random(config, seed, dtype=dtype, max_seq_len=max_seq_len, weight_bits=weight_bits, cache_bits=cache_bits,
+                                    share_prefix=share_prefix,
                                     max_tokens=cls._default_tokens(config, max_batch, max_tokens,
                                                                    max_seq_len))
         return cls(max_batch=max_batch, _runner=runner)
@@ -124,12 +131,15 @@ class Engine:
     # ---- generation -------------------------------------------------------------------
     def generate(self, prompt: Prompt, max_tokens: int = 128, temp: float = 0.0, top_k: int = 40,
                  top_p: float = 0.95, rep_penalty: float = 1.1, repeat_last_n: int = 64,
-                 seed: int = 42, stop_ids: Optional[Sequence[int]] = None, on_token=None):
+                 seed: int = 42, stop_ids: Optional[Sequence[int]] = None, on_token=None,
+                 logprobs: Optional[int] = None):
         """New token ids for the prompt (a list) or for each prompt (a list of lists).
         A stop token (the model's eos ids unless `stop_ids` is given) ends a sequence
-        and is not returned."""
+        and is not returned.  With `logprobs` (0 to 32) the ids are `sampling.ScoredToken`s: each also has its `logprob` and
+        the `entropy` under the model's softmax (before temperature, penalty, top-k and top-p), and the `top` likeliest
+        `logprobs` tokens there with their log probabilities."""
         params = SamplingParams(temp, top_k, top_p, rep_penalty, repeat_last_n, seed)
-        return self._generate(prompt, max_tokens, params, stop_ids, on_token)
+        return self._generate(prompt, max_tokens, params, stop_ids, on_token, logprobs)
 
     def generate_ids(self, prompt: Prompt, max_tokens: int, temp: float = 0.0, seed: int = 42,
                      stop_ids: Optional[Sequence[int]] = None):
@@ -137,11 +147,18 @@ class Engine:
         is a function of the logits alone (src/lib.rs:458-486)."""
         return self._generate(prompt, max_tokens, SamplingParams.pure(temp, seed), stop_ids, None)
 
-    def _generate(self, prompt, max_tokens, params, stop_ids, on_token):
+    def _top(self, logprobs: Optional[int]) -> Optional[int]:
+        most = min(MAX_TOP, self.vocab_size())
+        if logprobs is not None and not 0 <= int(logprobs) <= most:
+            raise HosError(f"logprobs: {logprobs} alternatives (0 to {most}, or None)")
+        return None if logprobs is None else int(logprobs)
+
+    def _generate(self, prompt, max_tokens, params, stop_ids, on_token, logprobs=None):
+        top = self._top(logprobs)
         batch = _is_batch(prompt)
         prompts = [list(p) for p in prompt] if batch else [list(prompt)]
         stops = self.stop_ids if stop_ids is None else tuple(stop_ids)
-        outs = gen.generate(_DeviceBackend(self.runner, params), prompts, max_tokens, stops,
+        outs = gen.generate(_DeviceBackend(self.runner, params, top), prompts, max_tokens, stops,
                             self.runner.cache.tokens_capacity(), self.max_batch, on_token,
                             page=self.runner.cache.page_tokens)
         return outs if batch else outs[0]
@@ -155,11 +172,13 @@ class Engine:
     def generate_from_ids(self, conversations: Sequence["Conversation"], ids: Sequence[Sequence[int]],
                           max_tokens: int = 128, temp: float = 0.0, top_k: int = 40, top_p: float = 0.95,
                           rep_penalty: float = 1.1, repeat_last_n: int = 64, seed: int = 42,
-                          stop_ids: Optional[Sequence[int]] = None, on_token=None) -> List[List[int]]:
+                          stop_ids: Optional[Sequence[int]] = None, on_token=None,
+                          logprobs: Optional[int] = None) -> List[List[int]]:
         """Feed `ids[i]` to conversation i on top of what it holds and generate, all conversations
         side by side (src/lib.rs:499-503: continues from the current position, does not reset; the
         caller owns the prompt).  Long prompts are fed in pieces by the step function.  A token that
-        the last call returned last is fed first (it was sampled but never run)."""
+        the last call returned last is fed first (it was sampled but never run).  `logprobs`: as for `generate`."""
+        top = self._top(logprobs)
         params = SamplingParams(temp, top_k, top_p, rep_penalty, repeat_last_n, seed)
         stops = self.stop_ids if stop_ids is None else tuple(stop_ids)
         if len(conversations) != len(ids):
@@ -174,13 +193,13 @@ class Engine:
                 raise HosError(f"generate_from_ids: {self.runner.length(c.slot)} tokens held and {len(p)} more are "
                                f"more than the context holds ({self.runner.max_seq_len})")
             prompts.append(p)
-        outs = gen.run_batch(_DeviceBackend(self.runner, params), prompts, list(range(len(prompts))), max_tokens,
+        outs = gen.run_batch(_DeviceBackend(self.runner, params, top), prompts, list(range(len(prompts))), max_tokens,
                              stops, on_token, slots=[c.slot for c in conversations])
         for c, p, o in zip(conversations, prompts, outs):
             # the last returned token has been sampled but not run, unless the context is full
             fed = self.runner.length(c.slot) - c.position - len(p)
             c.position = self.runner.length(c.slot)
-            c.pending = o[-1] if o and fed < len(o) else None
+            c.pending = int(o[-1]) if o and fed < len(o) else None
         return outs
 
     # ---- the step function, for callers that drive it themselves ------------------------
@@ -233,10 +252,59 @@ class Engine:
                 nll += float((lse - logits.gather(1, target[:, None])[:, 0]).sum())
         finally:
             r.release(slot)
-        from .. import ops
         ops.check_errors()
         mean = nll / len(feed)
         return len(feed), mean, math.exp(mean)
+
+    def score(self, prompt: Sequence[int], answers: Sequence[Sequence[int]], top: int = 0) -> List[List[ScoredToken]]:
+        """How likely each of the answers is after the prompt: for every answer its tokens as `sampling.ScoredToken`s, with `logprob`,
+        `entropy` and the `top` likeliest `top` tokens (0 to 32) at each place.  The prompt is run once; the answers are run side by side (up
+        to max_batch) on forks of it, and with share_prefix they read its keys and values once for all of them."""
+        top = self._top(top) or 0
+        prompt, answers = [int(t) for t in prompt], [[int(t) for t in a] for a in answers]
+        r = self.runner
+        if not prompt or any(not a for a in answers):
+            raise HosError("score: the prompt and every answer need a token at least")
+        longest = len(prompt) + max((len(a) for a in answers), default=1) - 1
+        if longest > r.max_seq_len:
+            raise HosError(f"score: {longest} tokens are more than the context holds ({r.max_seq_len})")
+        r._check_ids([prompt] + answers)
+        out: List[List[ScoredToken]] = []
+        held = r.admit(1)
+        try:
+            if len(prompt) > 1:
+                r.step(held, [prompt[:-1]])
+            at = 0
+            while at < len(answers):
+                batch = answers[at:at + self._fitting(len(prompt), [len(a) for a in answers[at:at + self.max_batch]])]
+                forks = r.fork(held[0], len(batch))
+                try:
+                    scores = r.scores(forks, [[prompt[-1]] + a[:-1] for a in batch], batch, top)
+                    tokens = scored_tokens([t for a in batch for t in a], scores)
+                finally:
+                    for s in forks:
+                        r.release(s)
+                ops.check_errors()
+                for a in batch:
+                    out.append(tokens[:len(a)])
+                    tokens = tokens[len(a):]
+                at += len(batch)
+        finally:
+            r.release(held[0])
+        return out
+
+    def _fitting(self, held: int, lengths: Sequence[int]) -> int:
+        """How many of the sequences that go on from `held` tokens by these lengths the cache has room for at once (one at least: the cache says
+        no itself)."""
+        cache = self.runner.cache
+        free = min((g.pages.n_free for g in cache.groups), default=1 << 62)
+        n = 0
+        for length in lengths[:cache.slots.n_free]:
+            free -= -(-(held % cache.page_tokens + length) // cache.page_tokens) + 1
+            if free < 0:
+                break
+            n += 1
+        return max(1, n)
 
     def bench(self, prompt: Prompt, decode_tokens: int = 64):
         """Time the prompt step and greedy decoding separately, after a warm-up of one prompt

@@ -25,8 +25,10 @@ from ..config.base import ModelConfig, read_config_json
 from .. import ops
 from ..errors import ExtensionMissingError, HosError
 from ..model import Model
+from ..parts import shared_attention
 from ..parts.base import FEW_TOKENS, Runtime
 from ..registry import config_from_dict, plan_for
+from ..sampling.scores import MAX_TOP, TokenScores
 from ..weights import RandomSource, SafetensorsFolder, load_tensors
 from .batch import build_step
 
@@ -45,11 +47,13 @@ class Runner:
     def __init__(self, config: ModelConfig, source, dtype: str = "bfloat16", max_tokens: int = 8192,
                  max_seq_len: Optional[int] = None, max_slots: Optional[int] = None,
                  device: Optional[torch.device] = None, chunk_tokens: int = 2048,
-                 weight_bits: Optional[int] = None, cache_bits: Optional[int] = None):
+                 weight_bits: Optional[int] = None, cache_bits: Optional[int] = None, share_prefix: bool = False):
         """`chunk_tokens`: the most tokens a step adds in one pass to a sequence that is under way
         (layers that keep a window of keys make their ring of pages that much longer; a step
         that brings more is run as several passes).  `weight_bits` 4: the projections of softmax attention and the matrices of
-        gated feed-forwards are held in 4 bits; `cache_bits` 4: the keys and values are (every mixer that keeps keys must offer it)."""
+        gated feed-forwards are held in 4 bits; `cache_bits` 4: the keys and values are (every mixer that keeps keys must offer it).  `share_prefix`:
+        steps of sequences that were forked from one another read the pages that they share once for all of them, where that pays
+        (parts/shared_attention.py; bfloat16 keys and values)."""
         if dtype not in DTYPES:
             raise HosError(f"dtype must be one of {sorted(DTYPES)}, found {dtype!r}")
         self.config = config
@@ -71,6 +75,17 @@ class Runner:
         del tensors
         self.cache: CacheManager = self.model.new_cache(max_tokens, max_seq_len, max_slots, chunk_tokens)
         self.vocab_size = self.plan.vocab_size
+        self.share_prefix = bool(share_prefix)
+        # (cache group, query heads) of the mixers that may read shared pages once
+        self.sharers = []
+        if self.share_prefix:
+            for call, store in zip(self.model.schedule, self.cache.stores):
+                mixer = self.model.layers[call.layer].mixer
+                if mixer.shares_pages and store.group is not None and shared_attention.takes(store.group):
+                    if not any(g is store.group and n == mixer.n_heads for g, n in self.sharers):
+                        self.sharers.append((store.group, mixer.n_heads))
+            if not self.sharers:
+                raise HosError("share_prefix: no mixer of this model attends over keys and values in bfloat16 that sequences can share")
         self._sessions = {}
         self.use_sessions = self.model.graph_safe     # single-token steps run through DecodeSession
         self.prompt_sessions = True                   # and short prompt steps through PromptSession
@@ -167,7 +182,7 @@ class Runner:
                     sess.feed(slots, token_lists)
                     out = sess.run()
                 return out.clone() if copy else out
-        if not single and last_only and self.use_sessions and self.prompt_sessions and all(st > 0 for st in starts):
+        if not single and last_only and self.use_sessions and self.prompt_sessions and all(st > 0 for st in starts) and not self._share(slots):
             # a short step of sequences that go on by several tokens (a second turn): replayed too
             from .decode import PromptSession, length_class, prompt_bucket
             bucket = prompt_bucket(sum(len(t) for t in token_lists), len(slots))
@@ -185,6 +200,13 @@ class Runner:
                     out = sess.run()
                 return out.clone() if copy else out
         return self._general(slots, starts, token_lists, want)
+
+    def _share(self, slots: Sequence[int]) -> bool:
+        """Whether some of these sequences hold pages in common that a step would read once for them (such a step of several tokens a
+        sequence is not replayed)."""
+        if len(slots) < 2 or any(s not in self.cache.lengths for s in slots):
+            return False
+        return any(g.shared_runs(slots, [self.cache.lengths[s] for s in slots]) for g, _ in self.sharers)
 
     @contextlib.contextmanager
     def _lengths_back_on_error(self, slots, starts):
@@ -271,6 +293,23 @@ class Runner:
             return self._passes(slots, starts, token_lists, want)
 
     def _passes(self, slots, starts, token_lists, want) -> torch.Tensor:
+        n_out = sum(len(w) for w in want)
+        out = None
+        for x, rows_t, dest in self._each_pass(slots, starts, token_lists, want):
+            if not dest:
+                continue
+            logits = self.model.logits(x, rows_t)
+            if len(dest) == n_out and dest == list(range(n_out)):
+                return logits                 # one pass gave every wanted row, in order
+            if out is None:
+                out = torch.empty((n_out, self.vocab_size), dtype=torch.float32, device=self.device)
+            out[torch.tensor(dest, dtype=torch.long, device=self.device)] = logits
+        if out is None:
+            out = torch.empty((0, self.vocab_size), dtype=torch.float32, device=self.device)
+        return out
+
+    def _each_pass(self, slots, starts, token_lists, want):
+        """Pass after pass: the hidden rows, which of them are wanted (a device tensor), and their places in the result."""
         room = self.cache.chunk_room()
         # stable: the sequences that start come first, the ones that go on by a few tokens last
         order = sorted(range(len(slots)),
@@ -280,9 +319,7 @@ class Runner:
         for i, w in enumerate(want):
             first_row[i] = at
             at += len(w)
-        n_out = at
         done = [0] * len(slots)               # tokens of each sequence already run
-        out = None
         while True:
             part = []                         # (sequence, first token, tokens) of this pass
             for i in order:
@@ -292,7 +329,7 @@ class Runner:
                 take = left if (starts[i] == 0 and done[i] == 0) or room is None else min(left, room)
                 part.append((i, done[i], take))
             if not part:
-                break
+                return
             rows, dest = [], []
             base = 0
             for i, lo, k in part:
@@ -305,16 +342,33 @@ class Runner:
                                      [token_lists[i][lo:lo + k] for i, lo, k in part], rows, extend=False)
             for i, lo, k in part:
                 done[i] = lo + k
-            if not rows:
-                continue
-            logits = self.model.logits(x, rows_t)
-            if len(dest) == n_out and dest == list(range(n_out)):
-                return logits                 # one pass gave every wanted row, in order
-            if out is None:
-                out = torch.empty((n_out, self.vocab_size), dtype=torch.float32, device=self.device)
-            out[torch.tensor(dest, dtype=torch.long, device=self.device)] = logits
-        if out is None:
-            out = torch.empty((0, self.vocab_size), dtype=torch.float32, device=self.device)
+            yield x, rows_t, dest
+
+    def scores(self, slots: Sequence[int], token_lists: Sequence[Sequence[int]], targets: Sequence[Sequence[int]], top: int = 0):
+        """Run `token_lists[i]` as the next tokens of the sequence in `slots[i]` and score `targets[i]`, the token that follows each of them:
+        sampling.TokenScores on the device, rows in the order of the sequences and of their tokens, with the `top` likeliest tokens beside
+        each.  The logits of all rows together are not held."""
+        if len(slots) != len(token_lists) or len(slots) != len(targets) or len(set(slots)) != len(slots):
+            raise HosError("scores: a list of tokens and one of targets for each of different slots are needed")
+        if any(len(t) != len(g) or len(t) == 0 for t, g in zip(token_lists, targets)):
+            raise HosError("scores: a target for each of a sequence's tokens is needed, and a token at least")
+        if not 0 <= top <= min(MAX_TOP, self.vocab_size):
+            raise HosError(f"scores: {top} alternatives (0 to {min(MAX_TOP, self.vocab_size)})")
+        starts = [self.cache.lengths[s] if s in self.cache.lengths else self._no_slot(s) for s in slots]
+        self._check_ids(token_lists)
+        self._check_ids(targets)
+        flat = [int(t) for g in targets for t in g]
+        out = TokenScores.empty(len(flat), top, self.device)
+        self.cache.extend_all(slots, [st + len(t) for st, t in zip(starts, token_lists)])
+        with self._lengths_back_on_error(slots, starts):
+            for x, rows_t, dest in self._each_pass(slots, starts, token_lists, [range(len(t)) for t in token_lists]):
+                # places and targets travel together
+                both = torch.tensor([dest, [flat[d] for d in dest]], dtype=torch.int32).pin_memory().to(self.device, non_blocking=True)
+                got = self.model.log_probs(x, rows_t, both[1], top)
+                at = both[0].long()
+                for to, part in zip(out, got):
+                    if to is not None:
+                        to[at] = part
         return out
 
     def hidden_states(self, slots: Sequence[int], token_lists: Sequence[Sequence[int]]) -> List[torch.Tensor]:
@@ -333,6 +387,7 @@ class Runner:
         """The hidden rows of one pass, and `rows` (indices into them) as a device tensor.  The
         sequences that start at position 0 must come first."""
         info, rows_t = build_step(token_lists, starts, slots, self.device, self.vocab_size, extra=rows)
+        info.share_pages = self.share_prefix
         if extend:
             self.cache.extend_all(slots, [st + len(t) for st, t in zip(starts, token_lists)])
         self.cache.flush()

@@ -114,12 +114,21 @@ class Model:
         """float32 [len(rows), vocab] for the given rows of the residual stream."""
         if rows.shape[0] == 0:
             return torch.empty((0, self.plan.vocab_size), dtype=torch.float32, device=x.device)
+        return self.head.forward(self.final_norm.forward(self._picked(x, rows)))
+
+    def log_probs(self, x: torch.Tensor, rows: torch.Tensor, tokens: torch.Tensor, top: int = 0):
+        """Scores (sampling.TokenScores) of tokens[i] under the logits of row rows[i] of the residual stream."""
+        if rows.shape[0] == 0:
+            from .sampling import TokenScores
+            return TokenScores.empty(0, top, x.device)
+        return self.head.log_probs(self.final_norm.forward(self._picked(x, rows)), tokens, top)
+
+    def _picked(self, x: torch.Tensor, rows: torch.Tensor) -> torch.Tensor:
         if self.streams > 1:
-            picked = ops.stream_sums(x, self.streams, rows)
-        else:
-            picked = torch.empty((rows.shape[0], x.shape[1]), dtype=torch.float32, device=x.device)
-            ops.gather_rows(x, rows, picked)
-        return self.head.forward(self.final_norm.forward(picked))
+            return ops.stream_sums(x, self.streams, rows)
+        picked = torch.empty((rows.shape[0], x.shape[1]), dtype=torch.float32, device=x.device)
+        ops.gather_rows(x, rows, picked)
+        return picked
 
 
 def weight_specs_for(config: ModelConfig) -> List[WeightSpec]:

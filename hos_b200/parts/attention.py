@@ -14,7 +14,8 @@ runtime's `cache_bits` 4 they are held in 4 bits (parts/attention4.py), and with
 A sequence that starts at position 0 attends over its own freshly projected rows
 and only stores to the cache; a sequence that goes on (by one token or by many)
 stores first and then attends over the cache.  One step may hold both kinds: the
-rows of the first kind come first and go to one kernel, the rest to another.  An entry of the run order that reads another entry's cache
+rows of the first kind come first and go to one kernel, the rest to another, which may read the pages that several sequences share
+once for all of them (StepInfo.share_pages; parts/shared_attention.py).  An entry of the run order that reads another entry's cache
 projects q only and always attends over that cache.
 """
 from __future__ import annotations
@@ -26,7 +27,7 @@ import torch
 from .. import ops
 from ..errors import KernelError, SpecError
 from ..registry import part_impl, register_part
-from . import attention4, linear
+from . import attention4, linear, shared_attention
 from .base import CallStore, KVNeed, Mixer, StepInfo, WeightSpec
 from .weights4 import Weight4
 
@@ -34,6 +35,7 @@ from .weights4 import Weight4
 class SoftmaxAttention(Mixer):
     graph_safe = True
     takes_weight_bits = True
+    shares_pages = True
 
     def __init__(self, spec, rt):
         super().__init__(spec, rt)
@@ -142,6 +144,8 @@ class SoftmaxAttention(Mixer):
                             f"keys that the step still reads")
                 if four:
                     attention4.attend(qkv[nf:, :self.q_dim], att[nf:], rest, cache, self.n_heads, self.scale, self.softcap, self.window)
+                    return linear.matmul_or_partials(att, self.w_o) if partial_ok else linear.matmul(att, self.w_o)
+                if rest.share_pages and shared_attention.attend_step(self, qkv[nf:, :self.q_dim], att[nf:], rest, cache, store.group):
                     return linear.matmul_or_partials(att, self.w_o) if partial_ok else linear.matmul(att, self.w_o)
                 # sequences that bring many tokens: a kernel that takes 64 queries per key tile; the few-token
                 # tail (decoding rows that share the step): the kernel that splits one query's keys over the GPU

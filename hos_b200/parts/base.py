@@ -118,6 +118,9 @@ class StepInfo:
     tail_tokens: int = 0             # that many sequences, that many rows (a mixer may send them to another kernel)
     row_offset: int = 0              # of a part of a step (see rows()): its first row and its first sequence in the
     seq_offset: int = 0              # whole step, which cu_seqlens (rows) and token_seq, seq_slot (sequences) still count from
+    share_pages: bool = False        # attention may read pages that several of the step's sequences hold once for all of them
+    page_work: dict = field(default_factory=dict)    # a replayed step's lists of work for that: (cache group, query heads) -> the lists
+                                     # on the device (parts/shared_attention.py), refilled like the step's arrays
     shared: dict = field(default_factory=dict)   # what one part of a step leaves for the parts that run after it in the same
                                      # step (a layer's values that later layers blend into theirs); rows as the step's
 
@@ -168,8 +171,9 @@ class CallStore:
     """The storage of one entry of the run order: its view of the paged cache (or
     of the cache of the entry it reads from) and its per-sequence state tensors."""
 
-    def __init__(self, kv=None, owns_kv: bool = True, state: Optional[Dict[str, torch.Tensor]] = None):
+    def __init__(self, kv=None, owns_kv: bool = True, state: Optional[Dict[str, torch.Tensor]] = None, group=None):
         self.kv = kv                      # ops.PagedKVArgs or None
+        self.group = group                # the cache.KVGroup that the view is of, or None
         self.owns_kv = owns_kv            # False: another entry writes this cache
         self.state = state or {}          # name -> tensor [n_slots, *shape]
 
@@ -183,6 +187,7 @@ class Part:
     # `step.slots_host` or the like leaves it False and is run step by step.
     graph_safe = False
     takes_weight_bits = False       # True if bind() holds its matrices as the runtime's weight_bits says
+    shares_pages = False            # True if it heeds StepInfo.share_pages
 
     def __init__(self, spec: PartSpec, rt: Runtime):
         self.spec = spec

@@ -2,7 +2,8 @@
 common are read once for all of their rows, the others sequence by sequence, and a row's parts are joined (csrc/attention_shared.cu).
 
 `plan` finds what is shared, once a step and group of the cache; `attend` is attention over the group's pages in any of its layers.
-bfloat16 keys and values; heads of a multiple of 16 numbers up to 256; any number of rows a sequence."""
+bfloat16 keys and values; heads of a multiple of 16 numbers up to 256; any number of rows a sequence.  `attend_step` is what a mixer calls
+in a step that may share pages; `ReplayedWork` holds the lists of a replayed step."""
 from __future__ import annotations
 
 import ctypes
@@ -19,6 +20,7 @@ OPEN = 1 << 30                 # a page behind every sequence's last
 ITEM_INTS = 20
 PAIRS, BLOCK = 8, 128          # (row, head) pairs of an item, of a big one
 MOST_PARTS = 64 << 20          # bytes of the parts that wait for the merge
+SHARE_BYTES = 64 << 20         # spared bytes from which on a step shares (SharedPlan.pays)
 
 _libs: Dict[int, ops.Library] = {}
 
@@ -43,14 +45,26 @@ class SharedPlan:
         self.runs, self.rows, self.slots, self.lengths, self.n_rows = runs, rows, slots, lengths, n_rows
         self._work: Dict[int, "Work"] = {}
 
+    def lists(self, n_heads: int) -> "Lists":
+        need = self.group.need
+        return lists(self.runs, self.rows, self.slots, self.lengths, self.n_rows, n_heads // need.n_kv_heads, need.n_kv_heads, need.head_dim,
+                     need.window, has_big(need.head_dim))
+
     def work(self, n_heads: int) -> "Work":
         w = self._work.get(n_heads)
         if w is None:
-            need = self.group.need
-            made = lists(self.runs, self.rows, self.slots, self.lengths, self.n_rows, n_heads // need.n_kv_heads, need.n_kv_heads,
-                         need.head_dim, need.window, has_big(need.head_dim))
-            w = self._work[n_heads] = Work(made, self.group, n_heads)
+            w = self._work[n_heads] = Work(self.lists(n_heads), self.group, n_heads)
         return w
+
+    def pays(self) -> bool:
+        """Whether a step is sooner done with its shared pages read once: if that spares SHARE_BYTES of keys and values.  Besides its bytes
+        attention over shared pages takes 3 to 9 us more than attention sequence by sequence, two kernels for one.  Measured (B200, us shared /
+        sequence by sequence): 16 heads over 32 / 16 kv heads of 128, 4 rows on 1,000 keys (24 MB spared) 10.6 / 9.3, on 2,000 (49 MB) 10.9 / 13.5,
+        16 on 1,000 (118 MB) 14.9 / 23.1, 64 on 4,000 32.6 / 242; 8 heads over 4 of 256, 8 rows on 2,000 (57 MB) 14.7 / 11.1, on 4,000 (114 MB)
+        15.9 / 16.1, 16 on 4,000 16.4 / 27.1; 5 pieces of 37 rows on 3,001 (48 MB) 22.5 / 32.6, 3 of 300 rows on 4,000 (33 MB) 74.6 / 52.7."""
+        need = self.group.need
+        spared = sum((len(members) - 1) * (hi - lo) for members, lo, hi in self.runs)
+        return spared * 4 * ops.PAGE_TOKENS * need.n_kv_heads * need.head_dim >= SHARE_BYTES
 
 
 class Lists:
@@ -71,23 +85,77 @@ class Work:
     """The lists on the device, in one array: the numbers of items, the rows' parts, the items, their rows."""
 
     def __init__(self, made: Lists, group, n_heads: int):
-        table, need = group.table_dev, group.need
+        device, need = group.table_dev.device, group.need
         n = len(made.n_parts)
         at = -(-(4 + n) // 4) * 4
         flat = np.concatenate([np.asarray([len(made.items), len(made.big), 0, 0], dtype=np.int32), made.n_parts, np.zeros(at - 4 - n, dtype=np.int32),
                                made.items.reshape(-1), made.big.reshape(-1), made.rows])
-        host = torch.from_numpy(flat)
-        if table.device.type == "cuda":
-            host = host.pin_memory()
-        self.array = host.to(table.device, non_blocking=True)
-        self._host = host                                   # the copy reads it
+        self.array = torch.from_numpy(flat)
+        self.copied = None                                  # (stream, event) of the copy to the device
+        if device.type == "cuda":
+            if torch.cuda.is_current_stream_capturing():
+                raise KernelError("attention over shared pages: call it once before it is captured, its lists are made then")
+            self._host = self.array.pin_memory()            # the copy reads it
+            self.array = self._host.to(device, non_blocking=True)
+            self.copied = (ops._stream().value, torch.cuda.Event())
+            self.copied[1].record()
         base = self.array.data_ptr()
         items, big = base + 4 * at, base + 4 * (at + made.items.size)
-        self.parts = made.parts
-        self.fields = SharedWork(base, base + 16, items, big, big + 4 * made.big.size, table.data_ptr(), len(made.items), len(made.big), made.sms, made.parts,
-                                 table.shape[1], group.ring_pages, n_heads, need.n_kv_heads, need.window or 0)
+        self.fields = _fields(group, n_heads, made, base, base + 16, items, big, big + 4 * made.big.size)
         self.address = ctypes.addressof(self.fields)
+        self.parts = made.parts
         self.floats = n * n_heads * made.parts * (need.head_dim + 2)
+
+
+def _fields(group, n_heads: int, made: Lists, counts: int, n_parts: int, items: int, big: int, rows: int) -> SharedWork:
+    need = group.need
+    return SharedWork(counts, n_parts, items, big, rows, group.table_dev.data_ptr(), len(made.items), len(made.big), made.sms, made.parts,
+                      group.table_dev.shape[1], group.ring_pages, n_heads, need.n_kv_heads, need.window or 0)
+
+
+class ReplayedWork:
+    """The lists of a replayed step of up to `n` rows: places that stay where they are, refilled before a replay.  What a launch is made for
+    (numbers of items and parts, SMs) is rounded up, so that steps alike share a program: `key`."""
+    MOST_ITEMS, MOST_BIG = 4096, 512
+
+    def __init__(self, group, n_heads: int, n: int):
+        self.group, self.n_heads, self.n = group, n_heads, n
+        self._at = np.cumsum([0, 4, n, self.MOST_ITEMS + 8 * n, ITEM_INTS * self.MOST_BIG, ITEM_INTS * self.MOST_ITEMS])
+        self._at = -(-self._at // 4) * 4
+        self.array = torch.zeros(int(self._at[-1]) + 8, dtype=torch.int32, device=group.table_dev.device)
+        self.fields = None
+        self.key = None
+
+    def refill(self, made: Lists) -> bool:
+        """The lists of the next step; False if they have no room here."""
+        _, n_parts, rows, big, items, _ = self._at
+        if len(made.items) > self.MOST_ITEMS or len(made.big) > self.MOST_BIG or len(made.rows) > big - rows or len(made.n_parts) > self.n:
+            return False
+        end = int(items) + made.items.size
+        host = torch.empty(end, dtype=torch.int32, pin_memory=self.array.is_cuda)
+        flat = host.numpy()
+        flat[:4] = (len(made.items), len(made.big), 0, 0)
+        flat[n_parts:n_parts + len(made.n_parts)] = made.n_parts
+        flat[n_parts + len(made.n_parts):rows] = 0           # padding rows: zeros
+        flat[rows:rows + len(made.rows)] = made.rows
+        flat[big:big + made.big.size] = made.big.reshape(-1)
+        flat[items:end] = made.items.reshape(-1)
+        self.array[:end].copy_(host, non_blocking=True)
+        base = self.array.data_ptr()
+        counts, parts, rows, big, items = (base + 4 * int(x) for x in self._at[:5])
+        f = self.fields = _fields(self.group, self.n_heads, made, counts, parts, items, big, rows)
+        f.most, f.big_most, f.parts = _rounded(f.most), _rounded(f.big_most), _rounded(f.parts)
+        f.sms = f.sms if f.sms == ops.sm_count() else max(1, f.sms // 16 * 16)
+        self.address = ctypes.addressof(f)
+        self.floats = self.n * self.n_heads * f.parts * (self.group.need.head_dim + 2)
+        self.key = (f.most, f.big_most, f.sms, f.parts)
+        return True
+
+
+def _rounded(n: int) -> int:
+    """Up to 4 as it is, then the next of 6, 8, 12, 16, 24, ..."""
+    step = 1 << max(0, n.bit_length() - 2)
+    return n if n <= 4 else -(-n // step) * step
 
 
 def has_big(head_dim: int) -> bool:
@@ -247,7 +315,8 @@ def plan(group, step) -> SharedPlan:
 def attend(q: torch.Tensor, out: torch.Tensor, step, cache: ops.PagedKVArgs, plan: SharedPlan, n_heads: int, scale: float,
            softcap: float = 0.0, window: Optional[int] = None) -> None:
     """out[N, n_heads * head_dim] = softmax attention of the step's rows, each at its own position, over what the cache's pages hold up
-    to and with that position (the last `window` of it).  Padding rows become zeros."""
+    to and with that position (the last `window` of it).  Padding rows become zeros.  To be captured it has to have run once, and the plan
+    has to live as long as the graph."""
     ops._check_here(q, "queries")
     ops._check_rows(q, "queries", torch.bfloat16)
     ops._check_rows(out, "attention output", torch.bfloat16)
@@ -270,6 +339,54 @@ def attend(q: torch.Tensor, out: torch.Tensor, step, cache: ops.PagedKVArgs, pla
     if n == 0:
         return
     work = plan.work(n_heads)
+    if work.copied[0] != ops._stream().value and not torch.cuda.is_current_stream_capturing():
+        stream = torch.cuda.current_stream()                 # the lists were copied on another
+        stream.wait_event(work.copied[1])
+        work.array.record_stream(stream)
+    _run(q, out, step.token_pos, cache, work, scale, softcap)
+
+
+def _run(q, out, token_pos, cache: ops.PagedKVArgs, work, scale: float, softcap: float) -> None:
     ws = torch.empty(work.floats, dtype=torch.float32, device=q.device)
-    lib_for(dim).call("hos_attn_shared", q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), n, step.token_pos.data_ptr(), cache.k_pages.data_ptr(),
-                      cache.v_pages.data_ptr(), cache.k_pages.shape[0], work.address, scale, softcap, ws.data_ptr(), ops._stream())
+    lib_for(cache.head_dim).call("hos_attn_shared", q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), q.shape[0], token_pos.data_ptr(),
+                                 cache.k_pages.data_ptr(), cache.v_pages.data_ptr(), cache.k_pages.shape[0], work.address, scale, softcap, ws.data_ptr(),
+                                 ops._stream())
+
+
+def takes(group) -> bool:
+    """Whether the layers of this group of the cache can attend over shared pages."""
+    need = group.need
+    return (need.bits is None and not need.keys_only and (need.v_head_dim or need.head_dim) == need.head_dim and supports(need.head_dim)
+            and group.k[0].dtype == torch.bfloat16)
+
+
+def step_plan(group, slots: Sequence[int], lengths: Sequence[int]) -> Optional[SharedPlan]:
+    """The plan of a single-token step of sequences of these lengths (with the step's token), if sharing pays."""
+    if not takes(group):
+        return None
+    made = SharedPlan(group, group.shared_runs(slots, lengths), [range(i, i + 1) for i in range(len(slots))], list(slots), list(lengths), len(slots))
+    return made if made.runs and made.pays() else None
+
+
+def attend_step(mixer, q: torch.Tensor, out: torch.Tensor, step, cache: ops.PagedKVArgs, group) -> bool:
+    """A mixer's attention over the cache in a step that may share pages; False where nothing is shared, or too little to pay (the mixer then
+    attends sequence by sequence).  A replayed step finds its lists in step.page_work."""
+    if mixer.scale <= 0.0:
+        return False
+    if step.replayed:
+        work = step.page_work.get((id(group), mixer.n_heads))
+        if work is None:
+            return False
+        _run(q, out, step.token_pos, cache, work, mixer.scale, mixer.softcap)
+        return True
+    key = ("shared pages", id(group), step.row_offset, step.n_tokens)
+    if key not in step.shared:                               # once a step and group
+        made = None
+        if group is not None and takes(group) and len(step.cu_host) == step.n_seqs + 1 and step.cu_host[-1] == step.n_tokens:
+            made = plan(group, step)
+        step.shared[key] = made if made is not None and made.pays() else None
+    made = step.shared[key]
+    if made is None:
+        return False
+    attend(q, out, step, cache, made, mixer.n_heads, mixer.scale, mixer.softcap, mixer.window)
+    return True

@@ -1,2 +1,2 @@
 from .sampler import Sampler, SamplingParams, next_rand, stream_seed  # noqa: F401
-from .scores import TokenScores, log_probs  # noqa: F401
+from .scores import ScoredToken, TokenScores, log_probs, scored_tokens  # noqa: F401

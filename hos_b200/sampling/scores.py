@@ -5,7 +5,7 @@ The distribution is the softmax of the logits as they are: temperature, top-k, t
 business.  All of it is float32."""
 from __future__ import annotations
 
-from typing import NamedTuple, Optional
+from typing import List, NamedTuple, Optional, Sequence
 
 import torch
 
@@ -29,6 +29,25 @@ class TokenScores(NamedTuple):
             return TokenScores(both[0], both[1])
         return TokenScores(both[0], both[1], torch.empty((rows, top), dtype=torch.int32, device=device),
                            torch.empty((rows, top), dtype=torch.float32, device=device))
+
+
+class ScoredToken(int):
+    """A token id that also knows how likely it was: `logprob`, the `entropy` of the distribution it came from, and `top`, the likeliest
+    tokens there as [(id, log probability)]."""
+
+    def __new__(cls, token: int, logprob: float, entropy: float, top=()):
+        t = super().__new__(cls, token)
+        t.logprob, t.entropy, t.top = logprob, entropy, list(top)
+        return t
+
+
+def scored_tokens(tokens: Sequence[int], scores: TokenScores) -> List[ScoredToken]:
+    """The tokens with their scores (which are on the host, or are fetched)."""
+    logprob, entropy = scores.logprob.tolist(), scores.entropy.tolist()
+    tops = [()] * len(tokens)
+    if scores.top_ids is not None:
+        tops = [list(zip(i, p)) for i, p in zip(scores.top_ids.tolist(), scores.top_logprobs.tolist())]
+    return [ScoredToken(t, *rest) for t, *rest in zip(tokens, logprob, entropy, tops)]
 
 
 def log_probs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, out: Optional[TokenScores] = None) -> TokenScores:
