@@ -554,26 +554,30 @@ def log_probs_blocks(rows: int, vocab: int) -> tuple:
 
 
 def log_probs(logits: torch.Tensor, tokens: torch.Tensor, logprob: torch.Tensor, entropy: torch.Tensor,
-              top_ids: Optional[torch.Tensor] = None, top_logprobs: Optional[torch.Tensor] = None) -> None:
+              top_ids: Optional[torch.Tensor] = None, top_logprobs: Optional[torch.Tensor] = None, fresh: bool = False) -> None:
     """Of row b: logprob[b] = logits[b, tokens[b]] - log sum exp, entropy[b], and the likeliest top_ids.shape[1] tokens with their log
-    probabilities (see sampling.log_probs)."""
+    probabilities (see sampling.log_probs).  `fresh`: the outputs were made for these logits and are not looked at."""
     _check_here(logits, "logits")
     _check_rows(logits, "logits", torch.float32)
     b, v = logits.shape
     _check(tokens, "tokens", torch.int32, 1)
-    _check(logprob, "log probabilities", torch.float32, 1)
-    _check(entropy, "entropies", torch.float32, 1)
+    if not fresh:
+        _check(logprob, "log probabilities", torch.float32, 1)
+        _check(entropy, "entropies", torch.float32, 1)
+        if top_ids is not None:
+            _check(top_ids, "likeliest tokens", torch.int32, 2)
+            _check(top_logprobs, "their log probabilities", torch.float32, 2)
+            if top_ids.shape != top_logprobs.shape or top_ids.shape[0] != b:
+                raise KernelError(f"log_probs: {b} rows with likeliest tokens {tuple(top_ids.shape)} and log probabilities {tuple(top_logprobs.shape)}")
+        if any(x is not None and x.device != logits.device for x in (logprob, entropy, top_ids, top_logprobs)):
+            raise KernelError(f"log_probs: scores and logits must be on one device ({logits.device})")
+    if tokens.device != logits.device:
+        raise KernelError(f"log_probs: tokens and logits must be on one device, found {tokens.device} and {logits.device}")
     if tokens.shape[0] != b or logprob.shape[0] != b or entropy.shape[0] != b:
         raise KernelError(f"log_probs: {b} rows of logits for {tokens.shape[0]} tokens, {logprob.shape[0]} and {entropy.shape[0]} scores")
-    top = 0
-    if top_ids is not None:
-        _check(top_ids, "likeliest tokens", torch.int32, 2)
-        _check(top_logprobs, "their log probabilities", torch.float32, 2)
-        top = top_ids.shape[1]
-        if top_ids.shape != top_logprobs.shape or top_ids.shape[0] != b:
-            raise KernelError(f"log_probs: {b} rows with likeliest tokens {tuple(top_ids.shape)} and log probabilities {tuple(top_logprobs.shape)}")
-        if top > min(LOG_PROBS_MAX_TOP, v):
-            raise KernelError(f"log_probs: {top} alternatives of {v} tokens (at most {LOG_PROBS_MAX_TOP})")
+    top = top_ids.shape[1] if top_ids is not None else 0
+    if top > min(LOG_PROBS_MAX_TOP, v):
+        raise KernelError(f"log_probs: {top} alternatives of {v} tokens (at most {LOG_PROBS_MAX_TOP})")
     if b == 0:
         return
     if v == 0:

@@ -100,7 +100,10 @@ def matmul_partials(x, w, k_splits: Optional[int] = None) -> Optional[torch.Tens
     return ws[: used.value]
 
 
-SCORE_MIN_ROWS = PAIR_MIN_ROWS
+# Scores come out of the head's product from so many rows on.  Measured (B200, us by the product / by logits, soft-capped): 64 rows of 2,304 by
+# 256,000 226 / 229, 65 rows 224 / 238, 128 rows 237 / 353; 2,048 by 50,021: 48 rows 51 / 53, 65 rows 51 / 61, 128 rows 51 / 80; 4,096 by 32,000: 33
+# rows 60 / 59, 65 rows 61 / 66; few rows 255 / 251 (24 of 2,304 by 256,000, no cap) to 57 / 49 (24 of 2,048 by 50,021).
+SCORE_MIN_ROWS = NEVER if PAIR_MIN_ROWS == NEVER else 65
 
 
 def can_score(x: torch.Tensor, w: torch.Tensor) -> bool:

@@ -93,17 +93,22 @@ def log_probs(x: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, cap: float
     ops._check_here(x, "hidden rows")
     if x.dim() != 2 or x.dtype not in (torch.float32, torch.bfloat16) or tokens.shape != x.shape[:1]:
         raise KernelError(f"log_probs: one token for each hidden row is needed, found rows {tuple(x.shape)} ({x.dtype}) and tokens {tuple(tokens.shape)}")
+    if not 0 <= top <= ops.LOG_PROBS_MAX_TOP:
+        raise KernelError(f"log_probs: {top} alternatives (0 to {ops.LOG_PROBS_MAX_TOP})")
     m, vocab = x.shape[0], w.n if isinstance(w, Weight4) else w.shape[0]
-    out = TokenScores.empty(m, top, x.device)
     if not top and not _force_plain and not isinstance(w, Weight4) and x.dtype == torch.bfloat16:
         from . import gemm_tc
         if gemm_tc.can_score(x, w):
             ops._check(tokens, "tokens", torch.int32, 1)
             ops._check_here(w, "head")
+            out = TokenScores.empty(m, 0, x.device)
             gemm_tc.log_probs(x, w, tokens, out.logprob, out.entropy, cap)
             return out
     epilogue = ops.EPI_SOFTCAP if cap > 0.0 else ops.EPI_NONE
     each = max(1, LOGITS_BYTES // (4 * vocab))
+    if 0 < m <= each:
+        return from_logits(matmul(x, w, out_dtype=torch.float32, epilogue=epilogue, cap=cap), tokens, top)
+    out = TokenScores.empty(m, top, x.device)
     for lo in range(0, m, each):
         logits = matmul(x[lo:lo + each], w, out_dtype=torch.float32, epilogue=epilogue, cap=cap)
         from_logits(logits, tokens[lo:lo + each], top, out=TokenScores(*(v[lo:lo + each] if v is not None else None for v in out)))

@@ -327,6 +327,8 @@ def attend(q: torch.Tensor, out: torch.Tensor, step, cache: ops.PagedKVArgs, pla
         raise KernelError(f"attend: {n_heads} query heads over {kv} kv heads")
     if not scale > 0.0:
         raise KernelError(f"attend: a scale of {scale}")
+    if out.device != q.device or step.token_pos.device != q.device:
+        raise KernelError(f"attend: queries, output and positions must be on one device, found {q.device}, {out.device} and {step.token_pos.device}")
     if q.shape[1] != n_heads * dim or out.shape != q.shape:
         raise KernelError(f"queries {tuple(q.shape)} and output {tuple(out.shape)} for {n_heads} heads of {dim}")
     if step.n_tokens != n or plan.n_rows != n:
@@ -347,7 +349,7 @@ def attend(q: torch.Tensor, out: torch.Tensor, step, cache: ops.PagedKVArgs, pla
 
 
 def _run(q, out, token_pos, cache: ops.PagedKVArgs, work, scale: float, softcap: float) -> None:
-    ws = torch.empty(work.floats, dtype=torch.float32, device=q.device)
+    ws = token_pos.new_empty(work.floats)                    # (words of 32 bits; a call's own, so that graphs share none)
     lib_for(cache.head_dim).call("hos_attn_shared", q.data_ptr(), q.stride(0), out.data_ptr(), out.stride(0), q.shape[0], token_pos.data_ptr(),
                                  cache.k_pages.data_ptr(), cache.v_pages.data_ptr(), cache.k_pages.shape[0], work.address, scale, softcap, ws.data_ptr(),
                                  ops._stream())

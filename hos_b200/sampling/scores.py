@@ -10,6 +10,7 @@ from typing import List, NamedTuple, Optional, Sequence
 import torch
 
 from .. import ops
+from ..errors import KernelError
 
 MAX_TOP = ops.LOG_PROBS_MAX_TOP
 
@@ -24,11 +25,10 @@ class TokenScores(NamedTuple):
 
     @staticmethod
     def empty(rows: int, top: int, device) -> "TokenScores":
-        both = torch.empty((2, rows), dtype=torch.float32, device=device)
+        first = torch.empty(rows, dtype=torch.float32, device=device)
         if not top:
-            return TokenScores(both[0], both[1])
-        return TokenScores(both[0], both[1], torch.empty((rows, top), dtype=torch.int32, device=device),
-                           torch.empty((rows, top), dtype=torch.float32, device=device))
+            return TokenScores(first, torch.empty_like(first))
+        return TokenScores(first, torch.empty_like(first), torch.empty((rows, top), dtype=torch.int32, device=device), first.new_empty((rows, top)))
 
 
 class ScoredToken(int):
@@ -55,7 +55,10 @@ def log_probs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, out: Opt
     the `top` likeliest tokens beside it (0 to 32).  A token outside the vocabulary marks a padding row: zeros, ids -1.
     -inf rules a token out; a row that holds nothing else, +inf or a number that is none has no distribution, and its scores are no
     numbers.  Among the likeliest a number that is none counts as -inf.  `out`: scores of the same sizes to write into."""
-    if out is None:
+    if not 0 <= top <= MAX_TOP:
+        raise KernelError(f"log_probs: {top} alternatives (0 to {MAX_TOP})")
+    fresh = out is None
+    if fresh:
         out = TokenScores.empty(logits.shape[0] if logits.dim() else 0, top, logits.device)
-    ops.log_probs(logits, tokens, out.logprob, out.entropy, out.top_ids if top else None, out.top_logprobs if top else None)
+    ops.log_probs(logits, tokens, out.logprob, out.entropy, out.top_ids if top else None, out.top_logprobs if top else None, fresh)
     return out

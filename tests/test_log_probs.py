@@ -12,6 +12,12 @@ def test_logits_that_are_not_on_the_gpu_are_refused():
         log_probs(torch.zeros(2, 8), torch.zeros(2, dtype=torch.int32), 1)
 
 
+@pytest.mark.parametrize("top", [-1, 33])
+def test_so_many_alternatives_are_refused(top):
+    with pytest.raises(KernelError, match="alternatives"):
+        log_probs(torch.zeros(2, 64), torch.zeros(2, dtype=torch.int32), top)
+
+
 def test_scores_to_write_into_have_the_sizes_asked_for():
     s = TokenScores.empty(3, 4, "cpu")
     assert s.logprob.shape == s.entropy.shape == (3,) and s.top_ids.shape == s.top_logprobs.shape == (3, 4)
