@@ -100,6 +100,24 @@ def test_rows_apart_another_stream_and_a_replayed_graph(rows):
     check(other, plain(x, w, t, 30.0))
 
 
+@pytest.mark.parametrize("rows", [8, 9, 24, 32, 64, 65, 90])
+@pytest.mark.parametrize("cap,top", [(0.0, 0), (0.0, 2), (30.0, 0)])
+def test_few_rows_and_a_large_vocabulary(rows, cap, top):
+    x, w, t = make(rows, 136, 20011, rows)
+    got, want = linear.log_probs(x, w, t, cap, top), plain(x, w, t, cap)
+    check(got, want)
+    if top:
+        assert ((want[2].gather(1, got.top_ids.long()) - got.top_logprobs.double()).abs() <= 1e-4).all()
+
+
+def test_heads_that_do_not_fit_are_refused():
+    for rows in (4, 20, 200):
+        x, w, t = make(rows, 64, 20000, 1)
+        for head in (w[:, :56], w[:0], w[0], w.cpu()):
+            with pytest.raises(KernelError):
+                linear.log_probs(x, head, t)
+
+
 def test_refusals():
     x, w, t = make(4, 64, 100, 1)
     for bad in ((x, w, t[:2]), (x.half(), w, t), (x[0], w, t[:1]), (x.cpu(), w, t), (x, w, t.long())):
