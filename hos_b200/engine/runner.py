@@ -182,7 +182,7 @@ class Runner:
                     sess.feed(slots, token_lists)
                     out = sess.run()
                 return out.clone() if copy else out
-        if not single and last_only and self.use_sessions and self.prompt_sessions and all(st > 0 for st in starts) and not self._share(slots):
+        if not single and last_only and self.use_sessions and self.prompt_sessions and all(st > 0 for st in starts) and not self._shares(slots):
             # a short step of sequences that go on by several tokens (a second turn): replayed too
             from .decode import PromptSession, length_class, prompt_bucket
             bucket = prompt_bucket(sum(len(t) for t in token_lists), len(slots))
@@ -201,12 +201,13 @@ class Runner:
                 return out.clone() if copy else out
         return self._general(slots, starts, token_lists, want)
 
-    def _share(self, slots: Sequence[int]) -> bool:
+    def _shares(self, slots: Sequence[int]) -> bool:
         """Whether some of these sequences hold pages in common that a step would read once for them (such a step of several tokens a
         sequence is not replayed)."""
-        if len(slots) < 2 or any(s not in self.cache.lengths for s in slots):
+        if len(slots) < 2:
             return False
-        return any(g.shared_runs(slots, [self.cache.lengths[s] for s in slots]) for g, _ in self.sharers)
+        lengths = [self.cache.lengths[s] for s in slots]
+        return any(shared_attention.pays(g, g.shared_runs(slots, lengths)) for g, _ in self.sharers)
 
     @contextlib.contextmanager
     def _lengths_back_on_error(self, slots, starts):

@@ -20,7 +20,7 @@ OPEN = 1 << 30                 # a page behind every sequence's last
 ITEM_INTS = 20
 PAIRS, BLOCK = 8, 128          # (row, head) pairs of an item, of a big one
 MOST_PARTS = 64 << 20          # bytes of the parts that wait for the merge
-SHARE_BYTES = 64 << 20         # spared bytes from which on a step shares (SharedPlan.pays)
+SHARE_BYTES = 64 << 20         # spared bytes from which on a step shares (pays)
 
 _libs: Dict[int, ops.Library] = {}
 
@@ -57,14 +57,17 @@ class SharedPlan:
         return w
 
     def pays(self) -> bool:
-        """Whether a step is sooner done with its shared pages read once: if that spares SHARE_BYTES of keys and values.  Besides its bytes
-        attention over shared pages takes 3 to 9 us more than attention sequence by sequence, two kernels for one.  Measured (B200, us shared /
-        sequence by sequence): 16 heads over 32 / 16 kv heads of 128, 4 rows on 1,000 keys (24 MB spared) 10.6 / 9.3, on 2,000 (49 MB) 10.9 / 13.5,
-        16 on 1,000 (118 MB) 14.9 / 23.1, 64 on 4,000 32.6 / 242; 8 heads over 4 of 256, 8 rows on 2,000 (57 MB) 14.7 / 11.1, on 4,000 (114 MB)
-        15.9 / 16.1, 16 on 4,000 16.4 / 27.1; 5 pieces of 37 rows on 3,001 (48 MB) 22.5 / 32.6, 3 of 300 rows on 4,000 (33 MB) 74.6 / 52.7."""
-        need = self.group.need
-        spared = sum((len(members) - 1) * (hi - lo) for members, lo, hi in self.runs)
-        return spared * 4 * ops.PAGE_TOKENS * need.n_kv_heads * need.head_dim >= SHARE_BYTES
+        return pays(self.group, self.runs)
+
+
+def pays(group, runs) -> bool:
+    """Whether a step is sooner done with its shared pages read once: if that spares SHARE_BYTES of keys and values.  Besides its bytes
+    attention over shared pages takes 3 to 9 us more than attention sequence by sequence, two kernels for one.  Measured (B200, us shared /
+    sequence by sequence): 32 heads over 16 of 128, 4 rows on 1,000 keys (24 MB spared) 10.6 / 9.3, on 2,000 (49 MB) 10.9 / 13.5,
+    16 on 1,000 (118 MB) 14.9 / 23.1, 64 on 4,000 32.6 / 242; 8 heads over 4 of 256, 8 rows on 2,000 (57 MB) 14.7 / 11.1, on 4,000 (114 MB)
+    15.9 / 16.1, 16 on 4,000 16.4 / 27.1; 5 pieces of 37 rows on 3,001 (48 MB) 22.5 / 32.6, 3 of 300 rows on 4,000 (33 MB) 74.6 / 52.7."""
+    spared = sum((len(members) - 1) * (hi - lo) for members, lo, hi in runs)
+    return bool(runs) and spared * 4 * ops.PAGE_TOKENS * group.need.n_kv_heads * group.need.head_dim >= SHARE_BYTES
 
 
 class Lists:
@@ -367,7 +370,7 @@ def step_plan(group, slots: Sequence[int], lengths: Sequence[int]) -> Optional[S
     if not takes(group):
         return None
     made = SharedPlan(group, group.shared_runs(slots, lengths), [range(i, i + 1) for i in range(len(slots))], list(slots), list(lengths), len(slots))
-    return made if made.runs and made.pays() else None
+    return made if made.pays() else None
 
 
 def attend_step(mixer, q: torch.Tensor, out: torch.Tensor, step, cache: ops.PagedKVArgs, group) -> bool:

@@ -1,5 +1,7 @@
 """Several answers to a prompt through the engine: forked conversations that read their common pages once, the log probabilities of what is
 generated, and the scores of given answers; against the plain implementation and against the engine's own steps."""
+import json
+import os
 import random
 
 import pytest
@@ -264,8 +266,25 @@ def test_refusals(tmp_path):
     assert r.cache.lengths[a] == 0
 
 
+@pytest.mark.parametrize("shared_pages", [True, False])
+def test_the_example_ranks_answers(tmp_path, shared_pages, shared, capsys):
+    import importlib.util
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "several_answers.py")
+    spec = importlib.util.spec_from_file_location("several_answers", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    from test_fourbit_engine_gpu import RAW                  # (heads that keys in 4 bits take)
+    config = tmp_path / "config.json"
+    config.write_text(json.dumps(RAW))
+    prompt = ",".join(str(3 + i % 90) for i in range(140))
+    args = ["--random", str(config), "-p", prompt, "--answers", "3", "-n", "5", "--max-seq-len", "256", "--rank"] + (["--shared"] if shared_pages else [])
+    assert example.main(args) == 0
+    got = capsys.readouterr()
+    means = [float(x) for x in [l for l in got.err.splitlines() if "mean log" in l][0].split()[4:]]
+    assert len(got.out.strip().splitlines()) == 3 and means == sorted(means, reverse=True) and bool(shared) == shared_pages
+
+
 def test_the_command_line(tmp_path):
-    import os
     import subprocess
     hos = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "bin", "hos")
     folder = make_folder(tmp_path, "D")
