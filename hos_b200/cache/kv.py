@@ -86,6 +86,7 @@ class KVGroup:
         self._slot_pages: Dict[int, List[int]] = {}
         self._holders: Dict[int, int] = {}             # pages that several slots hold -> how many
         self.version = 0                               # moves on whenever a slot's pages change
+        self.joins = 0                                 # and this whenever they change otherwise than by one more of its own
         self._dirty: set = set()
         self._views: Dict[int, ops.PagedKVArgs] = {}
         # what ops.copy_pages wants of the arrays (the keys', then the values'): address and bytes of a page
@@ -110,6 +111,7 @@ class KVGroup:
             raise CacheError(f"slot {slot} is opened twice")
         self._slot_pages[slot] = []
         self.version += 1
+        self.joins += 1
 
     def shared_before(self, slot: int, old_len: int, new_len: int) -> List[int]:
         """Table entries of the slot that positions old_len..new_len-1 are written to and whose pages others hold too."""
@@ -156,6 +158,7 @@ class KVGroup:
                 self._let_go(old)
             self._dirty.add(slot)
             self.version += 1
+            self.joins += 1
         while len(held) < want:
             page = self.pages.take()
             self.version += 1
@@ -165,6 +168,7 @@ class KVGroup:
 
     def close_slot(self, slot: int) -> None:
         self.version += 1
+        self.joins += 1
         for page in self._slot_pages.pop(slot):
             self._let_go(page)
 
@@ -185,6 +189,7 @@ class KVGroup:
         self._table_np[new_slot, :len(pages)] = pages
         self._dirty.add(new_slot)
         self.version += 1
+        self.joins += 1
 
     def shared_runs(self, slots: Sequence[int], lengths: Sequence[int]) -> List[tuple]:
         """Where sequences of these lengths share pages: [(places in `slots`, first logical page, the page behind the last)], each
@@ -246,6 +251,7 @@ class KVGroup:
             self._copy_listed(olds, news)
             self.pages.exchange(olds, news)
             self.version += 1
+            self.joins += 1
             to = dict(zip(olds, news))
             self._holders = {to.get(p, p): k for p, k in self._holders.items()}
             for slot, held in self._slot_pages.items():

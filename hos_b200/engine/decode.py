@@ -204,12 +204,13 @@ class DecodeSession:
 
     def _share(self, slots: Sequence[int], lengths: Optional[Sequence[int]]) -> None:
         """The lists of work for attention over pages that these sequences share, on the device (where the runner shares pages, the lengths are
-        known and it pays); made anew when the slots or their pages have changed."""
+        known and it pays); made anew when the slots or what they share have changed, or their own pages are many more."""
         sharers = self.runner.sharers
         if not sharers or lengths is None:
             self.page_work, self._page_key, self._paged_for = {}, (), None
             return
-        made_for = (tuple(slots), tuple(g.version for g, _ in sharers))
+        # (a page more of a sequence's own makes the lists no less true, only less even: those are counted together)
+        made_for = (tuple(slots), tuple((g.joins, g.version // max(16, len(slots))) for g, _ in sharers))
         if made_for == self._paged_for:
             return
         self.page_work, key, plans = {}, [], {}
@@ -222,7 +223,7 @@ class DecodeSession:
             work = self._page_works.get((id(group), n_heads))
             if work is None:
                 work = self._page_works[id(group), n_heads] = shared_attention.ReplayedWork(group, n_heads, self.b)
-            if work.refill(plan.lists(n_heads)):
+            if work.refill(plan.lists(n_heads, work.share)):
                 self.page_work[id(group), n_heads] = work
                 key.append((i, work.key))
         self._page_key, self._paged_for = tuple(key), made_for

@@ -182,7 +182,7 @@ class Runner:
                     sess.feed(slots, token_lists)
                     out = sess.run()
                 return out.clone() if copy else out
-        if not single and last_only and self.use_sessions and self.prompt_sessions and all(st > 0 for st in starts) and not self._shares(slots):
+        if not single and last_only and self.use_sessions and self.prompt_sessions and all(st > 0 for st in starts) and not self._shares(slots, token_lists):
             # a short step of sequences that go on by several tokens (a second turn): replayed too
             from .decode import PromptSession, length_class, prompt_bucket
             bucket = prompt_bucket(sum(len(t) for t in token_lists), len(slots))
@@ -201,13 +201,13 @@ class Runner:
                 return out.clone() if copy else out
         return self._general(slots, starts, token_lists, want)
 
-    def _shares(self, slots: Sequence[int]) -> bool:
+    def _shares(self, slots: Sequence[int], token_lists) -> bool:
         """Whether some of these sequences hold pages in common that a step would read once for them (such a step of several tokens a
         sequence is not replayed)."""
         if len(slots) < 2:
             return False
-        lengths = [self.cache.lengths[s] for s in slots]
-        return any(shared_attention.pays(g, g.shared_runs(slots, lengths)) for g, _ in self.sharers)
+        lengths, news = [self.cache.lengths[s] for s in slots], [len(t) for t in token_lists]
+        return any(shared_attention.pays(g, g.shared_runs(slots, lengths), news) for g, _ in self.sharers)
 
     @contextlib.contextmanager
     def _lengths_back_on_error(self, slots, starts):

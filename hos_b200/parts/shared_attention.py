@@ -20,7 +20,7 @@ OPEN = 1 << 30                 # a page behind every sequence's last
 ITEM_INTS = 20
 PAIRS, BLOCK = 8, 128          # (row, head) pairs of an item, of a big one
 MOST_PARTS = 64 << 20          # bytes of the parts that wait for the merge
-SHARE_BYTES = 64 << 20         # spared bytes from which on a step shares (pays)
+SHARE_BYTES, SHARE_ROWS = 64 << 20, 64        # spared bytes from which on, rows of a sequence up to which a step shares (pays)
 
 _libs: Dict[int, ops.Library] = {}
 
@@ -45,10 +45,10 @@ class SharedPlan:
         self.runs, self.rows, self.slots, self.lengths, self.n_rows = runs, rows, slots, lengths, n_rows
         self._work: Dict[int, "Work"] = {}
 
-    def lists(self, n_heads: int) -> "Lists":
+    def lists(self, n_heads: int, keep: Optional[tuple] = None) -> "Lists":
         need = self.group.need
         return lists(self.runs, self.rows, self.slots, self.lengths, self.n_rows, n_heads // need.n_kv_heads, need.n_kv_heads, need.head_dim,
-                     need.window, has_big(need.head_dim))
+                     need.window, has_big(need.head_dim), keep)
 
     def work(self, n_heads: int) -> "Work":
         w = self._work.get(n_heads)
@@ -57,24 +57,32 @@ class SharedPlan:
         return w
 
     def pays(self) -> bool:
-        return pays(self.group, self.runs)
+        return pays(self.group, self.runs, [len(r) for r in self.rows])
 
 
-def pays(group, runs) -> bool:
-    """Whether a step is sooner done with its shared pages read once: if that spares SHARE_BYTES of keys and values.  Besides its bytes
+def pays(group, runs, news: Sequence[int]) -> bool:
+    """Whether a step of sequences that bring so many rows is sooner done with its shared pages read once: if that spares SHARE_BYTES of keys
+    and values, and the sequences bring up to SHARE_ROWS rows in the middle: longer pieces are bound by their products.  Besides its bytes
     attention over shared pages takes 3 to 9 us more than attention sequence by sequence, two kernels for one.  Measured (B200, us shared /
     sequence by sequence): 32 heads over 16 of 128, 4 rows on 1,000 keys (24 MB spared) 10.6 / 9.3, on 2,000 (49 MB) 10.9 / 13.5,
     16 on 1,000 (118 MB) 14.9 / 23.1, 64 on 4,000 32.6 / 242; 8 heads over 4 of 256, 8 rows on 2,000 (57 MB) 14.7 / 11.1, on 4,000 (114 MB)
-    15.9 / 16.1, 16 on 4,000 16.4 / 27.1; 5 pieces of 37 rows on 3,001 (48 MB) 22.5 / 32.6, 3 of 300 rows on 4,000 (33 MB) 74.6 / 52.7."""
+    15.9 / 16.1, 16 on 4,000 16.4 / 27.1; 5 pieces of 37 rows on 3,001 (48 MB) 22.5 / 32.6, 3 of 300 rows on 4,000 (33 MB) 74.6 / 52.7; 16 pieces on 4,000 of 32 rows 49 / 76, of 64 77 / 78, of 100 102 / 81, of 200 179 / 158; 32
+    heads over 16 of 128, of 32 rows 94 / 278, of 64 157 / 279, of 100 248 / 291, 16 of 100 on 1,000 131 / 102.  Lists of work take the host 0.5 to
+    1.4 ms a step and group."""
+    if not runs:
+        return False
+    sharing = {i for members, _, _ in runs for i in members}
+    if sum(news[i] for i in sharing) > SHARE_ROWS * len(sharing):
+        return False
     spared = sum((len(members) - 1) * (hi - lo) for members, lo, hi in runs)
-    return bool(runs) and spared * 4 * ops.PAGE_TOKENS * group.need.n_kv_heads * group.need.head_dim >= SHARE_BYTES
+    return spared * 4 * ops.PAGE_TOKENS * group.need.n_kv_heads * group.need.head_dim >= SHARE_BYTES
 
 
 class Lists:
-    """Items (of up to 8 pairs, then of up to 128), their rows, each row's number of parts, and SMs for the small ones, on the host."""
+    """Items (of up to 8 pairs, then of up to 128), their rows, each row's number of parts, and the cut that they have (`shares`), on the host."""
 
-    def __init__(self, items: np.ndarray, big: np.ndarray, rows: np.ndarray, n_parts: np.ndarray, sms: int):
-        self.items, self.big, self.rows, self.n_parts, self.sms = items, big, rows, n_parts, sms
+    def __init__(self, items: np.ndarray, big: np.ndarray, rows: np.ndarray, n_parts: np.ndarray, share: tuple):
+        self.items, self.big, self.rows, self.n_parts, self.share, self.sms = items, big, rows, n_parts, share, share[2]
         self.parts = int(n_parts.max()) if n_parts.size else 0
 
 
@@ -126,8 +134,7 @@ class ReplayedWork:
         self._at = np.cumsum([0, 4, n, self.MOST_ITEMS + 8 * n, ITEM_INTS * self.MOST_BIG, ITEM_INTS * self.MOST_ITEMS])
         self._at = -(-self._at // 4) * 4
         self.array = torch.zeros(int(self._at[-1]) + 8, dtype=torch.int32, device=group.table_dev.device)
-        self.fields = None
-        self.key = None
+        self.fields, self.key, self.share = None, None, None
 
     def refill(self, made: Lists) -> bool:
         """The lists of the next step; False if they have no room here."""
@@ -148,6 +155,7 @@ class ReplayedWork:
         counts, parts, rows, big, items = (base + 4 * int(x) for x in self._at[:5])
         f = self.fields = _fields(self.group, self.n_heads, made, counts, parts, items, big, rows)
         f.most, f.big_most, f.parts = _rounded(f.most), _rounded(f.big_most), _rounded(f.parts)
+        self.share = made.share
         f.sms = f.sms if f.sms == ops.sm_count() else max(1, f.sms // 16 * 16)
         self.address = ctypes.addressof(f)
         self.floats = self.n * self.n_heads * f.parts * (self.group.need.head_dim + 2)
@@ -191,10 +199,12 @@ def _cuts(pages: np.ndarray):
     return np.asarray(lengths), -(-pages[:, None] // np.asarray(lengths)) if pages.size else np.zeros((0, len(lengths)), dtype=np.int64)
 
 
-def shares(small: np.ndarray, big: np.ndarray, big_pairs: np.ndarray, per_item: int, kv: int, head_dim: int, distinct: int) -> tuple:
+def shares(small: np.ndarray, big: np.ndarray, big_pairs: np.ndarray, per_item: int, kv: int, head_dim: int, distinct: int,
+           keep: Optional[tuple] = None) -> tuple:
     """(pages of a small share, of a big one, SMs for the small ones) for small blocks and big blocks of so many pages, `distinct` pages in all
-    counting shared ones once: the cut that makes the step shortest by the estimate above.  An item is run per_item times (a big one kv
-    times).  Big items have an SM each; the small ones run beside them on the SMs that are left, or after them on all."""
+    counting shared ones once (OPEN: not cut): the cut that makes the step shortest by the estimate above.  An item is run per_item times (a big one kv
+    times).  Big items have an SM each; the small ones run beside them on the SMs that are left, or after them on all.  `keep`: what an
+    earlier step had; it stays where that costs up to a tenth, so that steps replay one program."""
     sms, (small_page, big_page) = ops.sm_count(), _page_us(head_dim)
     at_once = 2 if head_dim <= 128 else 1
     part_us = (head_dim + 2) * 8.0 / PART_BYTES_US
@@ -215,8 +225,13 @@ def shares(small: np.ndarray, big: np.ndarray, big_pairs: np.ndarray, per_item: 
     us = np.maximum(us, tile_us * max(distinct * kv, float(small.sum()) * per_item + float(big.sum()) * kv) + SMALL_US)
     us = us + (big_splits * big_pairs[:, None]).sum(axis=0)[:, None] * kv * part_us + items * 8.0 * part_us
     i, j = divmod(int(np.argmin(us)), len(lengths))
+    if keep is not None:
+        at = min(int(np.searchsorted(big_lengths, keep[1])), len(big_lengths) - 1), min(int(np.searchsorted(lengths, keep[0])), len(lengths) - 1)
+        if us[at] <= 1.1 * us[i, j]:
+            i, j = at
     spare = int(left[i])
-    return int(lengths[j]), int(big_lengths[i]), spare if spare and big.size and max(big_us[i], beside[i, j]) <= after[i, j] else sms
+    uncut = [OPEN if k + 1 == len(of) else int(of[k]) for k, of in ((j, lengths), (i, big_lengths))]
+    return *uncut, spare if spare and big.size and max(big_us[i], beside[i, j]) <= after[i, j] else sms
 
 
 def is_big(pairs: int, pages: int, head_dim: int) -> bool:
@@ -228,7 +243,7 @@ def is_big(pairs: int, pages: int, head_dim: int) -> bool:
 
 
 def lists(runs, rows: Sequence[range], slots: Sequence[int], lengths: Sequence[int], n_rows: int, per: int, kv: int, head_dim: int,
-          window: Optional[int], big: bool) -> Lists:
+          window: Optional[int], big: bool, keep: Optional[tuple] = None) -> Lists:
     """The work: a run's rows in blocks of up to 8 pairs, or of up to 128 where a kernel has such blocks (`big`) and that is faster, over the
     run's pages, each sequence's over the rest of its own."""
     big = big and per <= BLOCK
@@ -267,7 +282,7 @@ def lists(runs, rows: Sequence[range], slots: Sequence[int], lengths: Sequence[i
         else:
             cut(of, slot, 0, OPEN, *lo_hi, n)
     pages = [np.asarray([b[6] for b in of], dtype=np.int64) for of in blocks]
-    share = shares(pages[0], pages[1], np.asarray([len(b[0]) * per for b in blocks[1]], dtype=np.int64), kv * chunks, kv, head_dim, distinct)
+    share = shares(pages[0], pages[1], np.asarray([len(b[0]) * per for b in blocks[1]], dtype=np.int64), kv * chunks, kv, head_dim, distinct, keep)
     most = max(2, MOST_PARTS // max(1, 4 * n_rows * per * kv * (head_dim + 2)))
     n_parts = np.zeros(n_rows, dtype=np.int32)
     listed = []
@@ -293,7 +308,7 @@ def lists(runs, rows: Sequence[range], slots: Sequence[int], lengths: Sequence[i
         rows_of[:, 7] = share_of
         rows_of[:, 9] += share_of.astype(np.int32)
         items.append(rows_of[np.argsort(-rows_of[:, 10], kind="stable")])      # the longest first
-    return Lists(items[0], items[1], np.asarray(listed, dtype=np.int32), n_parts, share[2])
+    return Lists(items[0], items[1], np.asarray(listed, dtype=np.int32), n_parts, share)
 
 
 def plan(group, step) -> SharedPlan:

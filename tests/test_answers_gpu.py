@@ -295,3 +295,48 @@ def test_the_command_line(tmp_path):
     assert p.returncode == 0 and [l.split(" : ")[0] for l in lines] == ["7,8", "9"] and all(float(l.split(" : ")[1]) < 0 for l in lines)
     p = subprocess.run([hos, "-m", folder, "--score", "7,8"], capture_output=True, text=True)
     assert p.returncode == 1 and "one prompt" in p.stderr
+
+
+def test_a_cache_of_another_size_and_a_released_fork(tmp_path, shared):
+    """Lists of work are made anew after the cache was resized, after forks left and others came into their slots."""
+    folder = make_folder(tmp_path, "D")
+    w, cfg = plain_model(folder)
+    rng = random.Random(6)
+    r = runner_for(folder, chunk_tokens=1, max_slots=8)
+    first = random_tokens(rng, 200, 1000)
+    a, = r.admit(1)
+    r.step([a], [first])
+    slots = [a] + r.fork(a, 3)
+    seqs = [list(first) for _ in slots]
+    for t in range(6):
+        if t == 2:
+            r.resize_cache(2048)
+        if t == 4:                                           # a stranger in a fork's slot
+            r.release(slots[2])
+            slots[2], = r.admit(1)
+            seqs[2] = random_tokens(rng, 150, 1000)
+            r.step([slots[2]], [seqs[2]])
+        new = random_tokens(rng, 4, 1000)
+        seqs = [s + [x] for s, x in zip(seqs, new)]
+        got = r.step(slots, [[x] for x in new])
+        for row, s in zip(got, seqs):
+            assert_close(row, P.forward_logits(w, cfg, s)[-1], "bfloat16", f"step {t}, {len(s)} tokens")
+    assert len(shared) > 1
+
+
+def test_sequences_that_grow_by_many_pages(tmp_path, shared):
+    """The lists of a replayed step stay while sequences take pages of their own."""
+    folder = make_folder(tmp_path, "G")
+    w, cfg = plain_model(folder)
+    vocab = TINY["G"][0]["vocab_size"]
+    rng = random.Random(7)
+    r = runner_for(folder, chunk_tokens=1)
+    first = random_tokens(rng, 70, vocab)
+    a, = r.admit(1)
+    r.step([a], [first])
+    slots = [a] + r.fork(a, 1)
+    seqs = [first + random_tokens(rng, 300, vocab) for _ in slots]
+    rows = [r.step(slots, [[s[70 + t]] for s in seqs]) for t in range(300)]
+    assert shared
+    for i, s in enumerate(seqs):
+        assert_close(torch.stack([row[i] for row in rows]), P.forward_logits(w, cfg, s)[70:], "bfloat16", f"sequence {i}")
