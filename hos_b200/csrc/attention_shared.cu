@@ -151,6 +151,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attn_shared_kernel(Share
             const int kvh = work % per_item / chunks, to = round % kGroups * kStages;
             int low, high;
             const Walk w = small_walk(a, it, lane, low, high);
+            const int seen_from = a.window > 0 ? max(0, low + 1 - a.window) : 0;
             const int* table = a.cache.page_table + (size_t)it.slot * a.cache.table_stride;
             for (int i0 = w.begin; i0 < w.end && ok; i0 += 32) {             // 32 pages looked up at a time
                 const int page_l = i0 + lane < w.end ? table[kv_table_entry(a.cache, walk_page(w, i0 + lane))] : 0;
@@ -160,17 +161,19 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attn_shared_kernel(Share
                     if (lane == 0) {
                         const int s = t % kStages;
                         const uint32_t parity = ((t / kStages) - 1) & 1;
-                        const size_t off = kv_tile_offset(a.cache, page, kvh);
-                        unsigned char* dst = ring + (size_t)s * 2 * kTileBytes;
+                        // of the first and the last page the rows that are seen
+                        const int key0 = walk_page(w, i0 + i) * kPageTokens, row0 = max(0, seen_from - key0), rows = min(kPageTokens, high + 1 - key0) - row0;
+                        const size_t off = kv_tile_offset(a.cache, page, kvh) + (size_t)row0 * HD;
+                        unsigned char* dst = ring + (size_t)s * 2 * kTileBytes + row0 * (HD * 2);
                         if (t >= kStages) ok = mbar_wait_cycles(&k_empty[s], parity, kWaitCycles);
                         if (ok) {
-                            mbar_expect_tx(&k_full[to + s], kTileBytes);
-                            bulk_g2s(dst, k_pages + off, kTileBytes, &k_full[to + s]);
+                            mbar_expect_tx(&k_full[to + s], rows * (HD * 2));
+                            bulk_g2s(dst, k_pages + off, rows * (HD * 2), &k_full[to + s]);
                             if (t >= kStages) ok = mbar_wait_cycles(&v_empty[s], parity, kWaitCycles);
                         }
                         if (ok) {
-                            mbar_expect_tx(&v_full[to + s], kTileBytes);
-                            bulk_g2s(dst + kTileBytes, v_pages + off, kTileBytes, &v_full[to + s]);
+                            mbar_expect_tx(&v_full[to + s], rows * (HD * 2));
+                            bulk_g2s(dst + kTileBytes, v_pages + off, rows * (HD * 2), &v_full[to + s]);
                         }
                     }
                     ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
