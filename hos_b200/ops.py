@@ -539,16 +539,17 @@ def _check_here(t: torch.Tensor, what: str) -> None:
 
 def log_probs_blocks(rows: int, vocab: int) -> tuple:
     """(threads of a block, blocks that share a row).  Rows that leave SMs free are cut over clusters of blocks of 1,024 threads, each with
-    a tile of 32,768 numbers or more; clusters of 4 and 8 only as many as run at once beside one another (128 blocks).  Measured (B200,
-    256,000 numbers, 5 alternatives, us by blocks of 1,024 threads a row 1 / 2 / 4 / 8 and of 256 threads 1): 1 row 21.0 / 15.4 / 11.7 / 9.5
-    and 38; 18 rows 23.5 / 17.1 / 13.2 / 19.0 and 49; 148 rows 31.0 / 38.5 / 60 / 90 and 53; 300 rows, 20 alternatives, 80.8 / 93.7 / 127 /
+    a tile of 32,768 numbers or more; clusters of 4 and 8 only as many as run at once beside one another (33 of 4 and 15 of 8 do here; 32 and
+    14 are taken).  Measured (B200, 256,000 numbers, 5 alternatives, us by blocks of 1,024 threads a row 1 / 2 / 4 / 8 and of 256 threads 1): 1
+    row 21.0 / 15.4 / 11.7 / 9.5 and 38; 15 rows 22.1 / 16.1 / 12.2 / 9.9; 16 rows 22.0 / 16.1 / 12.1 / 17.3; 33 rows 24.1 / 17.9 / 15.3 / 27.9; 36
+    rows 24.2 / 18.2 / 24.8 / 28.5; 148 rows 31.0 / 38.5 / 60 / 90 and 53; 300 rows, 20 alternatives, 80.8 / 93.7 / 127 /
     209 and 79.0; 1,500 rows of 2,200: 64 with 1,024 threads, 14.3 with 256, 9.2 with 128."""
     if vocab <= 4096:
         return 128, 1
     if rows > sm_count() or vocab <= 8192:
         return 256, 1
-    blocks = 1
-    while blocks < 8 and vocab > 32768 * blocks and 2 * rows * blocks <= (128 if blocks > 1 else sm_count()):
+    blocks, at_once = 1, {2: sm_count(), 4: 128, 8: 112}
+    while blocks < 8 and vocab > 32768 * blocks and 2 * rows * blocks <= at_once[2 * blocks]:
         blocks *= 2
     return 1024, blocks
 
