@@ -154,10 +154,16 @@ struct RopeEpi {
 // What the epilogue of a head's product leaves instead of the logits (kGEpiScores): an epilogue thread has 128 columns of a row of a tile,
 // and joins their moments (moments.cuh) to those of the tiles of this row that its CTA took before; parts[part][row] are written when
 // the rows change, and `wanted` gets the logit of the row's token from the thread that meets it.
+//
+// A tensor core's sum in 32 bits is cut at every step of 16 products, not rounded: a logit comes out low by 1e-9 of itself per product (measured,
+// B200: 2.4e-6 at K 2,304, 3.8e-6 at 3,584; sums of rounded 32-bit products are off by 4e-7 there).  So K goes in chunks of up to 24 blocks of
+// 64, whose sums the epilogue adds in registers while the next chunk runs.
+constexpr int kScoreBlocks = 24;
 struct ScoreEpi {
     const int* tokens;         // [M]
     float4* parts;             // [parts][rows of m_tiles x 256]: (maximum, sum, weighted sum, unused)
     float* wanted;             // [M]
+    int chunks;                // of K: their sums are added outside the tensor cores, see kScoreBlocks
     int same_rows;             // 1: a pair's tiles are all of the same rows (it leaves one part), 0: one part a tile
 };
 
@@ -584,26 +590,30 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a,     // A: boxes o
             constexpr uint32_t idesc = umma_idesc(2 * GM, BN);
             int it = 0, local_tile = 0;
             bool ok = true;
-            for (int tile = pair; tile < total_tiles && ok; tile += n_pairs, ++local_tile) {
-                const int acc = local_tile & 1;
-                if (local_tile >= 2 && !mbar_wait_timed(&acc_empty[acc], ((local_tile >> 1) - 1) & 1)) { ok = false; break; }
-                tc_fence_after();
-                const uint32_t d_tmem = tmem_base + acc * BN;
+            const int chunks = EPI == kGEpiScores ? p.score.chunks : 1;       // (local_tile counts accumulators: one a tile, or a chunk)
+            for (int tile = pair; tile < total_tiles && ok; tile += n_pairs) {
                 const int ks = tile % p.k_splits;
-                const int kb0 = ks * kb_per_split, kb1 = min(k_blocks, kb0 + kb_per_split);
-                for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                    const int s = it % Cfg::kStages;
-                    if (!mbar_wait_timed(&full[s], (it / Cfg::kStages) & 1)) { ok = false; break; }
+                const int tile_kb0 = ks * kb_per_split, tile_kb1 = min(k_blocks, tile_kb0 + kb_per_split);
+                for (int chunk = 0; chunk < chunks && ok; ++chunk, ++local_tile) {
+                    const int acc = local_tile & 1;
+                    if (local_tile >= 2 && !mbar_wait_timed(&acc_empty[acc], ((local_tile >> 1) - 1) & 1)) { ok = false; break; }
                     tc_fence_after();
-                    const uint32_t a_addr = smem_u32(stages + (size_t)s * Cfg::kStageBytes);
-                    const uint64_t a_desc = umma_desc_sw128(a_addr);
-                    const uint64_t b_desc = umma_desc_sw128(a_addr + Cfg::kABytes);
+                    const uint32_t d_tmem = tmem_base + acc * BN;
+                    const int kb0 = EPI == kGEpiScores ? k_blocks * chunk / chunks : tile_kb0, kb1 = EPI == kGEpiScores ? k_blocks * (chunk + 1) / chunks : tile_kb1;
+                    for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                        const int s = it % Cfg::kStages;
+                        if (!mbar_wait_timed(&full[s], (it / Cfg::kStages) & 1)) { ok = false; break; }
+                        tc_fence_after();
+                        const uint32_t a_addr = smem_u32(stages + (size_t)s * Cfg::kStageBytes);
+                        const uint64_t a_desc = umma_desc_sw128(a_addr);
+                        const uint64_t b_desc = umma_desc_sw128(a_addr + Cfg::kABytes);
 #pragma unroll
-                    for (int k = 0; k < GK / 16; ++k)
-                        umma_bf16_pair(d_tmem, a_desc + 2 * k, b_desc + 2 * k, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
-                    umma_commit_pair(&empty[s]);
+                        for (int k = 0; k < GK / 16; ++k)
+                            umma_bf16_pair(d_tmem, a_desc + 2 * k, b_desc + 2 * k, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+                        umma_commit_pair(&empty[s]);
+                    }
+                    if (ok) umma_commit_pair(&acc_full[acc]);
                 }
-                if (ok) umma_commit_pair(&acc_full[acc]);
             }
             if (!ok) record_give_up();
         }
@@ -759,24 +769,55 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a,     // A: boxes o
             } else if constexpr (EPI == kGEpiScores) {
                 const int m = mt * 2 * GM + (int)rank * GM + quarter * 32 + lane;
                 const int token = m < p.M ? p.score.tokens[m] : -1;
-                if (!mbar_wait_timed(&acc_full[acc], (local_tile >> 1) & 1)) { ok = false; break; }
-                tc_fence_after();
+                const uint32_t mine = tmem_base + ((uint32_t)(quarter * 32) << 16) + col_half * (BN / 2);
+                // the chunks' sums so far: of 96 columns in registers, of the last 32 in shared memory, where the warp has 128 bytes a row
+                // (pieces of 16 permuted by the row)
+                float sums[3][32];
+                unsigned char* mine_s = staging + (size_t)(warp - 2) * 4096 + lane * 128;
+                auto piece = [&](int j) -> float4& { return *reinterpret_cast<float4*>(mine_s + ((j ^ (lane & 7)) << 4)); };
+#pragma unroll
+                for (int j = 0; j < 32; ++j) sums[0][j] = sums[1][j] = sums[2][j] = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) piece(j) = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+                for (int chunk = 0; chunk < p.score.chunks; ++chunk) {
+                    const int use = local_tile * p.score.chunks + chunk, held = use & 1;
+                    ok = ok && mbar_wait_timed(&acc_full[held], (use >> 1) & 1);
+                    if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                    tc_fence_after();
+#pragma unroll
+                    for (int g = 0; g < 8; ++g) {
+                        uint32_t v[16];
+                        tmem_ld_32x16(mine + held * BN + 16 * g, v);
+                        tmem_ld_wait();
+                        if (g < 6) {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) sums[g / 2][g % 2 * 16 + j] += __uint_as_float(v[j]);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                float4& to = piece(g % 2 * 4 + j);
+                                float4 s = to;
+                                s.x += __uint_as_float(v[4 * j]); s.y += __uint_as_float(v[4 * j + 1]);
+                                s.z += __uint_as_float(v[4 * j + 2]); s.w += __uint_as_float(v[4 * j + 3]);
+                                to = s;
+                            }
+                        }
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_leader(&acc_empty[held]);
+                }
+                if (!ok) break;
                 const float twice = p.cap > 0.f ? 2.f * 1.44269504f / p.cap : 0.f;
 #pragma unroll 1
-                for (int c0 = col_half * (BN / 2); c0 < (col_half + 1) * (BN / 2); c0 += 32) {
-                    const int n0 = nt * BN + c0;
+                for (int g = 0; g < 4; ++g) {                      // (one body: the columns move up after each turn)
+                    const int n0 = nt * BN + col_half * (BN / 2) + 32 * g;
                     if (n0 >= p.N) break;
-                    uint32_t v[32];
-                    tmem_ld_32x32(t_lane + c0, v);
-                    tmem_ld_wait();
-                    float f[32];
+                    float (&f)[32] = sums[0];
                     if (p.cap > 0.f) {                         // c tanh(x / c) = c - 2 c / (1 + e^(2 x / c)): off by 2^-22 c at most
 #pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            f[j] = fmaf(-2.f * p.cap, rcp_approx(1.f + ex2_approx(twice * __uint_as_float(v[j]))), p.cap);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
+                        for (int j = 0; j < 32; ++j) f[j] = fmaf(-2.f * p.cap, rcp_approx(1.f + ex2_approx(twice * f[j])), p.cap);
                     }
                     if (n0 + 32 > p.N) {
 #pragma unroll
@@ -792,12 +833,23 @@ gemm_tc_pair_kernel(const __grid_constant__ CUtensorMap map_a,     // A: boxes o
 #pragma unroll
                     for (int j = 1; j < 32; ++j) most = fmaxf(most, f[j]);
                     add_to(row_sums, f, most);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float4 s = piece(j);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            sums[0][4 * j + i] = sums[1][4 * j + i];
+                            sums[1][4 * j + i] = sums[2][4 * j + i];
+                        }
+                        sums[2][4 * j] = s.x; sums[2][4 * j + 1] = s.y; sums[2][4 * j + 2] = s.z; sums[2][4 * j + 3] = s.w;
+                    }
                 }
                 if (!p.score.same_rows || tile + n_pairs >= total_tiles) {
                     const int part = 2 * (p.score.same_rows ? pair / m_tiles : nt) + col_half;
                     p.score.parts[(size_t)part * (m_tiles * 2 * GM) + m] = make_float4(row_sums.m, row_sums.s, row_sums.u, 0.f);
                     row_sums = Moments{-INFINITY, 0.f, 0.f};
                 }
+                continue;                                          // (the accumulators went back above)
             } else {
             if (!mbar_wait_timed(&acc_full[acc], (local_tile >> 1) & 1)) { ok = false; break; }
             tc_fence_after();
@@ -905,24 +957,31 @@ __global__ void splitk_reduce_kernel(const float* __restrict__ part, OutT* __res
 // The parts of kGEpiScores joined: 8 rows a block, 32 threads a row.  A row whose token is outside the vocabulary is padding: zeros.
 __global__ void __launch_bounds__(256) score_merge_kernel(ScoreEpi s, int parts, int stride, int M, int N, float* __restrict__ logprob,
                                                           float* __restrict__ entropy) {
-    __shared__ Moments held[32][8];
+    __shared__ Moments held[8][8];
     pdl_enter();
-    const int r = threadIdx.x & 7, deep = threadIdx.x >> 3, m = blockIdx.x * 8 + r;
+    const int r = threadIdx.x & 7, deep = threadIdx.x >> 3, warp = threadIdx.x >> 5, m = blockIdx.x * 8 + r;
     Moments mine{-INFINITY, 0.f, 0.f};
 #pragma unroll 4
     for (int p = deep; p < parts; p += 32) {
         const float4 v = s.parts[(size_t)p * stride + m];      // (rows behind the last are there too)
         mine = joined(mine, Moments{v.x, v.y, v.z});
     }
-    held[deep][r] = mine;
+    auto beside = [&](int o) {                                 // with the thread of the same row o lanes away
+        mine = joined(mine, Moments{__shfl_xor_sync(0xffffffffu, mine.m, o), __shfl_xor_sync(0xffffffffu, mine.s, o), __shfl_xor_sync(0xffffffffu, mine.u, o)});
+    };
+    beside(8);
+    beside(16);
+    if ((deep & 3) == 0) held[warp][r] = mine;
     __syncthreads();
+    if (warp != 0) return;
+    mine = joined(held[deep][r], held[deep + 4][r]);
+    beside(8);
+    beside(16);
     if (deep == 0 && m < M) {
-        for (int d = 1; d < 32; ++d) mine = joined(mine, held[d][r]);
         const int token = s.tokens[m];
         const bool padding = token < 0 || token >= N;
-        const float log_s = logf(mine.s);
-        logprob[m] = padding ? 0.f : (s.wanted[m] - mine.m) - log_s;
-        entropy[m] = padding ? 0.f : log_s - mine.u / mine.s;
+        logprob[m] = padding ? 0.f : (s.wanted[m] - mine.m) - log_sum(mine);
+        entropy[m] = padding ? 0.f : entropy_of(mine);
     }
 }
 
@@ -1282,7 +1341,8 @@ extern "C" int hos_gemm_tc_scores(const void* A, const void* W, const int* token
     const int parts = 2 * (same ? score_pairs(m_tiles, n_tiles) / m_tiles : n_tiles), stride = m_tiles * 2 * GM;
     GemmParams p = {};
     p.M = M; p.N = N; p.K = K; p.k_splits = 1; p.gate_rows = N; p.cap = cap;
-    p.score = ScoreEpi{tokens, reinterpret_cast<float4*>(workspace), workspace + (size_t)parts * 4 * stride, same ? 1 : 0};
+    const int k_blocks = (K + GK - 1) / GK, chunks = (k_blocks + kScoreBlocks - 1) / kScoreBlocks;
+    p.score = ScoreEpi{tokens, reinterpret_cast<float4*>(workspace), workspace + (size_t)parts * 4 * stride, chunks, same ? 1 : 0};
     CUtensorMap mm, mn;
     int rc;
     if ((rc = make_map(&mm, A, M, K, lda, GM))) return rc;

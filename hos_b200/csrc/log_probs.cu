@@ -1,8 +1,8 @@
 // Log probabilities of given tokens, the entropy, and the likeliest tokens, from rows of logits.
 //
 // Of a row l: M = max l, S = sum e^(l - M), U = sum e^(l - M) (l - M) (moments.cuh).  A thread keeps them of what it has seen and, when
-// its maximum grows by d, takes S to S e^-d and U to (U - S d) e^-d, so the logits are read once.  All of it is held in 32 bits; a
-// thread adds some hundred terms, trees the rest.
+// its maximum grows by d, takes S to S e^-d and U to (U - S d) e^-d, so the logits are read once.  All of it is held in 32 bits, S without the
+// maximum's own 1; a thread adds some hundred terms, trees the rest.
 //
 // The likeliest k tokens in the same pass.  A number and its token make a key of 64 bits, larger for larger numbers and, of equal ones,
 // for lower tokens: keys are all different.  32 groups of threads say what the largest number is that they have had; at least k numbers
@@ -300,10 +300,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) log_probs_kernel(LogP
     }
     __syncthreads();
     const Moments r = sh.all;
-    const float log_s = logf(r.s);
+    const float log_s = log_sum(r);
     if (tid == 0) {
         a.logprob[row] = (l[token] - r.m) - log_s;
-        a.entropy[row] = log_s - r.u / r.s;
+        a.entropy[row] = entropy_of(r);
     }
     if (TOP && tid < a.top) {
         const Key k = sh.best[tid];
@@ -330,11 +330,26 @@ static int launch_log_probs(const LogProbArgs& a, int rows, int blocks, cudaStre
     return check_launch("log_probs");
 }
 
+// Logits soft-capped where they lie: c tanh(l / c).
+__global__ void __launch_bounds__(256) softcap_kernel(float* __restrict__ logits, long long n, float cap) {
+    pdl_enter();
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) logits[i] = softcap_precise(logits[i], cap);
+}
+
 }  // namespace hos
 
 using namespace hos;
 
 extern "C" const char* hos_last_error() { return error_buffer(); }
+
+// n float32 logits, side by side, become c tanh(l / c).  Few rows' alone: a product of many rows does that itself.
+extern "C" int hos_softcap(float* logits, long long n, float cap, cudaStream_t stream) {
+    if (n <= 0) return 0;
+    if (!(cap > 0.f)) HOS_REFUSE("softcap: a cap of %f", cap);
+    const long long blocks = (n + 1023) / 1024, most = 16ll * sm_count_cached();
+    launch_pdl(softcap_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, stream, logits, n, cap);
+    return check_launch("softcap");
+}
 
 // Per row of float32 logits (`stride` numbers from row to row): the log probability of tokens[row] and the entropy; with `top`,
 // the likeliest `top` tokens (of equal ones the lower first) and their log probabilities.  A row whose token is outside the vocabulary

@@ -589,6 +589,15 @@ def log_probs(logits: torch.Tensor, tokens: torch.Tensor, logprob: torch.Tensor,
                   _stream())
 
 
+def softcap(logits: torch.Tensor, cap: float) -> None:
+    """float32 logits, side by side, become cap tanh(logits / cap) where they lie."""
+    _check_here(logits, "logits")
+    _check(logits, "logits", torch.float32)
+    if not cap > 0.0:
+        raise KernelError(f"softcap: a cap of {cap}")
+    scores().call("hos_softcap", logits.data_ptr(), logits.numel(), float(cap), _stream())
+
+
 # ---- the per-slot record (csrc/slot_state.cu) ----------------------------------------------
 SLOT_WORDS, RECENT_MAX, MAX_STOPS = 8, 256, 16
 SLOT_POS, SLOT_LAST, SLOT_FLAGS, SLOT_COUNT, SLOT_RNG_LO, SLOT_RNG_HI, SLOT_LIMIT = range(7)

@@ -100,10 +100,11 @@ def matmul_partials(x, w, k_splits: Optional[int] = None) -> Optional[torch.Tens
     return ws[: used.value]
 
 
-# Scores come out of the head's product from so many rows on.  Measured (B200, us by the product / by logits, soft-capped): 64 rows of 2,304 by
-# 256,000 226 / 229, 65 rows 224 / 238, 128 rows 237 / 353; 2,048 by 50,021: 48 rows 51 / 53, 65 rows 51 / 61, 128 rows 51 / 80; 4,096 by 32,000: 33
-# rows 60 / 59, 65 rows 61 / 66; few rows 255 / 251 (24 of 2,304 by 256,000, no cap) to 57 / 49 (24 of 2,048 by 50,021).
-SCORE_MIN_ROWS = NEVER if PAIR_MIN_ROWS == NEVER else 65
+# Scores come out of the head's product from so many rows on.  Measured (B200, us by the product / by logits, soft-capped): 2,304 by 256,000, 20 rows
+# 240 / 246, 24 rows 236 / 265, 32 rows 233 / 338; 2,048 by 50,021: 20 rows 60 / 54, 24 rows 57 / 57, 32 rows 54 / 70; 4,096 by 32,000: 20 rows 64 / 62, 24
+# rows 63 / 65.  From 33 rows on logits come from tensor cores too, 64 rows of 2,304 by 256,000 without a cap 235 / 212, whose sums are less exact
+# (csrc/gemm_tc.cu, kScoreBlocks).
+SCORE_MIN_ROWS = NEVER if PAIR_MIN_ROWS == NEVER else 24
 
 
 def can_score(x: torch.Tensor, w: torch.Tensor) -> bool:

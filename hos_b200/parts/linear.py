@@ -85,16 +85,12 @@ LOGITS_BYTES = 256 << 20        # of logits that `log_probs` holds at a time
 
 
 def _logits(x: torch.Tensor, w: torch.Tensor, cap: float) -> torch.Tensor:
-    """float32 [rows, vocab].  `matmul`, but for 9 to 32 rows and a vocabulary of 16,384 on always the tensor-core kernel: the product of a
-    handful of rows takes longer with every row.  Measured (B200, us handful / tensor cores): 2,304 by 256,000, 8 rows 179 / 184, 12 rows 200 / 184, 24 rows
-    246 / 186; 2,048 by 50,021, 8 rows 34 / 37, 12 rows 40 / 37, 24 rows 46 / 38; 1,024 by 8,000, 12 rows 5.7 / 6.5."""
-    if not cap > 0.0 and x.shape[0] > 8 and not isinstance(w, Weight4) and w.shape[0] >= 16384 and not _force_plain:
-        from . import gemm_tc
-        out = torch.empty((x.shape[0], w.shape[0]), dtype=torch.float32, device=x.device)
-        if gemm_tc.can_take(x, w, out, ops.EPI_NONE):
-            gemm_tc.matmul(x, w, out)
-            return out
-        return matmul(x, w, out=out)
+    """float32 [rows, vocab].  A handful of bfloat16 rows: the product that streams the head through registers, whose sums are the more exact (see
+    csrc/gemm_tc.cu, kScoreBlocks), and the soft-cap where the logits lie: 2,304 by 256,000, 8 rows 182 us, 16 rows 220, with their scores."""
+    if cap > 0.0 and x.dtype == torch.bfloat16 and x.shape[0] < 24 and not isinstance(w, Weight4) and not _force_plain:
+        out = matmul(x, w, out_dtype=torch.float32)
+        ops.softcap(out, cap)
+        return out
     return matmul(x, w, out_dtype=torch.float32, epilogue=ops.EPI_SOFTCAP if cap > 0.0 else ops.EPI_NONE, cap=cap)
 
 

@@ -110,6 +110,36 @@ def test_few_rows_and_a_large_vocabulary(rows, cap, top):
         assert ((want[2].gather(1, got.top_ids.long()) - got.top_logprobs.double()).abs() <= 1e-4).all()
 
 
+@pytest.mark.parametrize("rows", [3, 40, 300])
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+def test_long_sums_lose_little(rows, cap):
+    """Tensor cores cut their sums at every 16 products: by half of the last bit in the middle, 0.36 * 2^-23 of a sum that has grown to half of its
+    chunk's on average.  3,584 products in three chunks of 75 steps: 75 * 0.36 * 2^-23 / 2 = 1.6e-6 of a logit (all
+    of them in one sum would be 4.8e-6); the scores' own roundings are below 4e-7 of it.  A log probability is the difference of two logits (one
+    of them a mean), each low by such a part of itself, an entropy the difference of a logarithm of sums and a mean: errors are a part of the
+    row's largest logit, not of the score, which may be smaller (a row of logits of 9 and a log probability of -0.3)."""
+    x, w, t = make(rows, 3584, 6000, 5)
+    got, want = linear.log_probs(x, w, t, cap), plain(x, w, t, cap)
+    largest = (x.double() @ w.double().T).abs().amax(1).norm()
+    for a, b, part in zip((got.logprob, got.entropy), want, (2e-6, 4e-6)):
+        assert (a.double() - b).norm() < part * largest, float((a.double() - b).norm() / largest)
+
+
+@pytest.mark.parametrize("rows", [1, 23, 24, 200])
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+def test_a_row_that_is_nearly_sure(rows, cap):
+    """The product's scores keep the digits of small log probabilities, where the logits do: an error e of logits of 25 (2^-20 of them, and of the cap)
+    moves what the others have, and so the log probability, by 5e-5 of itself."""
+    x, w, t = make(rows, 512, 3000, 9)
+    w = torch.cat([w, torch.zeros(8, 512, dtype=w.dtype, device=DEV)])
+    w[t.long()] = (w[t.long()].float() * 4).to(w.dtype)
+    x = (w[t.long()].float() * (25 / (w[t.long()].float() ** 2).sum(1, keepdim=True))).to(w.dtype)
+    got, want = linear.log_probs(x, w, t, cap), plain(x, w, t, cap)
+    assert (want[0] > -1e-2).all() and (want[0] < -1e-8).all()
+    for a, b in zip((got.logprob, got.entropy), want):
+        assert ((a.double() - b).abs() <= 1e-4 * b.abs()).all(), float(((a.double() - b) / b).abs().max())
+
+
 def test_heads_that_do_not_fit_are_refused():
     for rows in (4, 20, 200):
         x, w, t = make(rows, 64, 20000, 1)

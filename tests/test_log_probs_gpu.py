@@ -140,3 +140,52 @@ def test_refusals():
         with pytest.raises(KernelError):
             log_probs(a["logits"], a["tokens"], a["top"], a.get("out"))
     assert log_probs(x[:0], t[:0], 2).top_ids.shape == (0, 2)
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 2), (3, 40), (1, 100), (5, 3000), (2, 9000), (1, 256000), (20, 70001), (70, 130000), (300, 5003)])
+def test_nearly_sure_rows_keep_their_digits(rows, vocab):
+    """A row that is sure of a token to 1e-3 or 1e-12: the log probability and the entropy, which are as small, to 2e-5 of themselves.  With d = l - max
+    down to -40 a weight e^d is off by 2^-24 |d| from d's own rounding, as much from d log2 e's, 1.3e-8 |d| from the constant and 2^-22 from the
+    exponential: 6e-6; sums of positive numbers in trees and of up to some hundred a thread add 1e-6 each; the entropy is the sum of two positive
+    terms of such numbers, one with a factor d."""
+    g = torch.Generator().manual_seed(vocab)
+    for lead in (7.0, 20.0, 28.0):
+        logits = torch.rand(rows, vocab, generator=g) * 3
+        best = torch.randint(0, vocab, (rows,), generator=g)
+        logits[torch.arange(rows), best] = 3 + math.log(vocab) + lead * (0.5 + 0.5 * torch.rand(rows, generator=g))
+        got = log_probs(logits.to(DEV), best.to(torch.int32).to(DEV), 1)
+        x = logits.double()
+        d = x - x.amax(1, keepdim=True)
+        rest = d.exp()
+        rest[torch.arange(rows), best] = 0
+        small = rest.sum(1)
+        lp = -torch.log1p(small)
+        entropy = torch.log1p(small) - (rest * d).sum(1) / (1 + small)
+        assert got.top_ids[:, 0].tolist() == best.tolist()
+        for a, b in ((got.logprob, lp), (got.entropy, entropy), (got.top_logprobs[:, 0], lp)):
+            assert ((a.double().cpu() - b).abs() <= 2e-5 * b.abs()).all(), (lead, float(((a.double().cpu() - b) / b).abs().max()))
+
+
+@pytest.mark.parametrize("vocab", [7, 500, 20000, 256000])
+@pytest.mark.parametrize("equal", [2, 5])
+def test_several_equal_maxima_count_each(vocab, equal):
+    """`equal` tokens 40 above all others: log probabilities -log(equal), entropy log(equal), wherever in the row they lie."""
+    g = torch.Generator().manual_seed(vocab + equal)
+    logits = torch.rand(12, vocab, generator=g) - 40
+    where = torch.stack([torch.randperm(vocab, generator=g)[:equal] if i % 3 else torch.arange(equal) for i in range(12)])
+    logits.scatter_(1, where, 5.0)
+    got = log_probs(logits.to(DEV), where[:, 1].to(torch.int32).to(DEV), equal)
+    assert got.top_ids.tolist() == where.sort(1).values.tolist()
+    assert (got.logprob.cpu() + math.log(equal)).abs().max() < 1e-6 and (got.entropy.cpu() - math.log(equal)).abs().max() < 1e-6
+
+
+def test_softcap_in_place():
+    from hos_b200 import ops
+    x = torch.randn(3, 70001, device=DEV) * 40
+    want = 30 * torch.tanh(x.double() / 30)
+    ops.softcap(x, 30.0)
+    assert (x.double() - want).abs().max() < 4e-6            # 30 times the last bits of a tanh and of its product
+    ops.softcap(x[:0], 30.0)
+    for bad in ((x, 0.0), (x, -1.0), (x.T, 3.0), (x.bfloat16(), 3.0), (x.cpu(), 3.0)):
+        with pytest.raises(KernelError):
+            ops.softcap(*bad)
