@@ -156,9 +156,11 @@ struct RopeEpi {
 // the rows change, and `wanted` gets the logit of the row's token from the thread that meets it.
 //
 // A tensor core's sum in 32 bits is cut at every step of 16 products, not rounded: a logit comes out low by 1e-9 of itself per product (measured,
-// B200: 2.4e-6 at K 2,304, 3.8e-6 at 3,584; sums of rounded 32-bit products are off by 4e-7 there).  So K goes in chunks of up to 24 blocks of
-// 64, whose sums the epilogue adds in registers while the next chunk runs.
-constexpr int kScoreBlocks = 24;
+// B200: 2.4e-6 at K 2,304, 3.8e-6 at 3,584; sums of rounded 32-bit products are off by 4e-7 there).  So K goes in chunks of up to 12 blocks of
+// 64, whose sums the epilogue adds in registers while the next chunk runs: log probabilities at K 3,584 off by 3e-7 of themselves, not 2.5e-6.
+// Reading tensor memory as often costs products: 2,048 rows of 3,584 by 64,000 in one sum 630 us, chunks of 24 blocks 667, of 12 684, of 8 702; 185
+// rows of 2,304 by 256,000 245 / 258 / 261 / 272.
+constexpr int kScoreBlocks = 12;
 struct ScoreEpi {
     const int* tokens;         // [M]
     float4* parts;             // [parts][rows of m_tiles x 256]: (maximum, sum, weighted sum, unused)

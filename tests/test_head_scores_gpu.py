@@ -114,7 +114,7 @@ def test_few_rows_and_a_large_vocabulary(rows, cap, top):
 @pytest.mark.parametrize("cap", [0.0, 30.0])
 def test_long_sums_lose_little(rows, cap):
     """Tensor cores cut their sums at every 16 products: by half of the last bit in the middle, 0.36 * 2^-23 of a sum that has grown to half of its
-    chunk's on average.  3,584 products in three chunks of 75 steps: 75 * 0.36 * 2^-23 / 2 = 1.6e-6 of a logit (all
+    chunk's on average.  3,584 products in chunks of up to 48 steps: 48 * 0.36 * 2^-23 / 2 = 1.0e-6 of a logit (all
     of them in one sum would be 4.8e-6); the scores' own roundings are below 4e-7 of it.  A log probability is the difference of two logits (one
     of them a mean), each low by such a part of itself, an entropy the difference of a logarithm of sums and a mean: errors are a part of the
     row's largest logit, not of the score, which may be smaller (a row of logits of 9 and a log probability of -0.3)."""

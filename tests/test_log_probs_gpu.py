@@ -180,11 +180,13 @@ def test_several_equal_maxima_count_each(vocab, equal):
 
 
 def test_softcap_in_place():
+    """30 tanh(l / 30): tanhf is off by 2 units in the last place at most (2 * 2^-24 below 1), 30 times that is 3.6e-6; the product of up to 30 is rounded
+    by 2^-20, 1.0e-6; the quotient by 2^-24 of itself, which x / cosh^2 x < 0.45 makes 30 * 0.45 * 2^-24 = 0.8e-6: 5.4e-6."""
     from hos_b200 import ops
-    x = torch.randn(3, 70001, device=DEV) * 40
+    x = (torch.randn(3, 70001, generator=torch.Generator().manual_seed(1)) * 40).to(DEV)
     want = 30 * torch.tanh(x.double() / 30)
     ops.softcap(x, 30.0)
-    assert (x.double() - want).abs().max() < 4e-6            # 30 times the last bits of a tanh and of its product
+    assert (x.double() - want).abs().max() < 5.5e-6
     ops.softcap(x[:0], 30.0)
     for bad in ((x, 0.0), (x, -1.0), (x.T, 3.0), (x.bfloat16(), 3.0), (x.cpu(), 3.0)):
         with pytest.raises(KernelError):
