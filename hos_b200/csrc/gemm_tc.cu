@@ -39,7 +39,7 @@ constexpr int kGemmThreads = 192;
 constexpr int kPairThreads = 320;         // the kernel on pairs of SMs: TMA warp, MMA warp, 8 epilogue warps
 constexpr long long kWaitCycles = 1ll << 31;     // about a second
 
-enum { kGEpiNone = 0, kGEpiSoftcap = 1, kGEpiGated = 2, kGEpiBias = 3, kGEpiRope = 4, kGEpiScores = 5 };
+enum { kGEpiNone = 0, kGEpiSoftcap = 1, kGEpiGated = 2, kGEpiBias = 3, kGEpiRope = 4, kGEpiScores = 5, kGEpiLogits = 6 };
 
 __device__ int g_gemm_error = 0;
 __device__ int* g_gemm_error_host = nullptr;     // a word in pinned host memory, if the host gave one
@@ -151,16 +151,16 @@ struct RopeEpi {
     int n_heads, n_kv_heads, write_cache;
 };
 
-// What the epilogue of a head's product leaves instead of the logits (kGEpiScores): an epilogue thread has 128 columns of a row of a tile,
-// and joins their moments (moments.cuh) to those of the tiles of this row that its CTA took before; parts[part][row] are written when
-// the rows change, and `wanted` gets the logit of the row's token from the thread that meets it.
-//
 // A tensor core's sum in 32 bits is cut at every step of 16 products, not rounded: a logit comes out low by 1e-9 of itself per product (measured,
 // B200: 2.4e-6 at K 2,304, 3.8e-6 at 3,584; sums of rounded 32-bit products are off by 4e-7 there).  So K goes in chunks of up to 12 blocks of
 // 64, whose sums the epilogue adds in registers while the next chunk runs: log probabilities at K 3,584 off by 3e-7 of themselves, not 2.5e-6.
 // Reading tensor memory as often costs products: 2,048 rows of 3,584 by 64,000 in one sum 630 us, chunks of 24 blocks 667, of 12 684, of 8 702; 185
 // rows of 2,304 by 256,000 245 / 258 / 261 / 272.
 constexpr int kScoreBlocks = 12;
+
+// What the epilogue of a head's product leaves instead of the logits (kGEpiScores): an epilogue thread has 128 columns of a row of a tile,
+// and joins their moments (moments.cuh) to those of the tiles of this row that its CTA took before; parts[part][row] are written when
+// the rows change, and `wanted` gets the logit of the row's token from the thread that meets it.
 struct ScoreEpi {
     const int* tokens;         // [M]
     float4* parts;             // [parts][rows of m_tiles x 256]: (maximum, sum, weighted sum, unused)
@@ -312,27 +312,31 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap map_m,     // the 128-row ope
             constexpr uint32_t idesc = umma_idesc(GM, BN);
             int it = 0, local_tile = 0;
             bool ok = true;
-            for (int tile = blockIdx.x; tile < total_tiles && ok; tile += gridDim.x, ++local_tile) {
+            const int chunks = EPI == kGEpiLogits ? p.score.chunks : 1;       // (local_tile counts accumulators: one a tile, or a chunk)
+            for (int tile = blockIdx.x; tile < total_tiles && ok; tile += gridDim.x) {
                 int mt, nt, ks;
                 tile_coords(tile, mt, nt, ks);
-                const int kb0 = ks * kb_per_split, kb1 = min(k_blocks, kb0 + kb_per_split);
-                const int acc = local_tile & 1;
-                if (local_tile >= 2 && !mbar_wait_timed(&acc_empty[acc], ((local_tile >> 1) - 1) & 1)) { ok = false; break; }
-                tc_fence_after();
-                const uint32_t d_tmem = tmem_base + acc * BN;
-                for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                    const int s = it % Cfg::kStages;
-                    if (!mbar_wait_timed(&full[s], (it / Cfg::kStages) & 1)) { ok = false; break; }
+                const int tile_kb0 = ks * kb_per_split, tile_kb1 = min(k_blocks, tile_kb0 + kb_per_split);
+                for (int chunk = 0; chunk < chunks && ok; ++chunk, ++local_tile) {
+                    const int acc = local_tile & 1;
+                    if (local_tile >= 2 && !mbar_wait_timed(&acc_empty[acc], ((local_tile >> 1) - 1) & 1)) { ok = false; break; }
                     tc_fence_after();
-                    const uint32_t a_addr = smem_u32(stages + (size_t)s * Cfg::kStageBytes);
-                    const uint64_t a_desc = umma_desc_sw128(a_addr);
-                    const uint64_t b_desc = umma_desc_sw128(a_addr + Cfg::kABytes);
+                    const uint32_t d_tmem = tmem_base + acc * BN;
+                    const int kb0 = EPI == kGEpiLogits ? k_blocks * chunk / chunks : tile_kb0, kb1 = EPI == kGEpiLogits ? k_blocks * (chunk + 1) / chunks : tile_kb1;
+                    for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                        const int s = it % Cfg::kStages;
+                        if (!mbar_wait_timed(&full[s], (it / Cfg::kStages) & 1)) { ok = false; break; }
+                        tc_fence_after();
+                        const uint32_t a_addr = smem_u32(stages + (size_t)s * Cfg::kStageBytes);
+                        const uint64_t a_desc = umma_desc_sw128(a_addr);
+                        const uint64_t b_desc = umma_desc_sw128(a_addr + Cfg::kABytes);
 #pragma unroll
-                    for (int k = 0; k < GK / 16; ++k)     // 32 bytes further along K: +2 in 16-byte units
-                        umma_bf16(d_tmem, a_desc + 2 * k, b_desc + 2 * k, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
-                    umma_commit(&empty[s]);               // the stage is free once these products have read it
+                        for (int k = 0; k < GK / 16; ++k)     // 32 bytes further along K: +2 in 16-byte units
+                            umma_bf16(d_tmem, a_desc + 2 * k, b_desc + 2 * k, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+                        umma_commit(&empty[s]);               // the stage is free once these products have read it
+                    }
+                    if (ok) umma_commit(&acc_full[acc]);      // the accumulator is complete
                 }
-                if (ok) umma_commit(&acc_full[acc]);      // the accumulator is complete
             }
             if (!ok) record_give_up();
         }
@@ -345,6 +349,44 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap map_m,     // the 128-row ope
         for (int tile = blockIdx.x; tile < total_tiles && ok; tile += gridDim.x, ++local_tile) {
             int mt, nt, ks;
             tile_coords(tile, mt, nt, ks);
+            if constexpr (EPI == kGEpiLogits) {
+                // a head's logits of up to 128 rows: the chunks' sums are added here (kScoreBlocks); a thread has a token of the vocabulary, of all rows
+                const uint32_t mine = tmem_base + ((uint32_t)(quarter * 32) << 16);
+                float sums[BN];
+#pragma unroll
+                for (int j = 0; j < BN; ++j) sums[j] = 0.f;
+#pragma unroll 1
+                for (int chunk = 0; chunk < p.score.chunks; ++chunk) {
+                    const int use = local_tile * p.score.chunks + chunk, held = use & 1;
+                    ok = mbar_wait_timed(&acc_full[held], (use >> 1) & 1);
+                    ok = __all_sync(0xffffffffu, ok) != 0;
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int c = 0; c < BN; c += 16) {
+                        uint32_t v[16];
+                        tmem_ld_32x16(mine + held * BN + c, v);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) sums[c + j] += __uint_as_float(v[j]);
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&acc_empty[held]);
+                }
+                if (!ok) break;
+                const int feat = mt * GM + quarter * 32 + lane;
+                const float twice = p.cap > 0.f ? 2.f * 1.44269504f / p.cap : 0.f;
+                float* to = reinterpret_cast<float*>(p.out) + (size_t)nt * BN * p.ldo + feat;
+                if (feat < p.N) {
+#pragma unroll
+                    for (int j = 0; j < BN; ++j) {
+                        const float x = sums[j];                   // c tanh(x / c) = c - 2 c / (1 + e^(2 x / c)): off by 2^-22 c at most
+                        if (nt * BN + j < p.M) to[(size_t)j * p.ldo] = p.cap > 0.f ? fmaf(-2.f * p.cap, rcp_approx(1.f + ex2_approx(twice * x)), p.cap) : x;
+                    }
+                }
+                continue;                                          // (the accumulators went back above)
+            }
             const int acc = local_tile & 1;
             if (!mbar_wait_timed(&acc_full[acc], (local_tile >> 1) & 1)) { ok = false; break; }
             tc_fence_after();
@@ -1319,6 +1361,28 @@ static int score_pairs(int m_tiles, int n_tiles) {
     return tiles < most ? (int)tiles : most;
 }
 static bool score_same_rows(int m_tiles, int n_tiles) { return score_pairs(m_tiles, n_tiles) % m_tiles == 0; }
+
+// float32 out[m][n] = A . W^T of up to 128 rows, soft-capped if cap > 0: as hos_gemm_tc's, but summed in chunks of K (kScoreBlocks).
+extern "C" int hos_gemm_tc_logits(const void* A, const void* W, float* out, int M, int N, int K, int lda, int ldw, int ldo, float cap,
+                                  cudaStream_t stream) {
+    if (M <= 0 || N <= 0) return 0;
+    if (M > kSwapMaxRows) HOS_REFUSE("gemm_tc_logits: %d rows (at most %d)", M, kSwapMaxRows);
+    if (K <= 0 || (K % 8) || (lda % 8) || (ldw % 8) || ((uintptr_t)A % 16) || ((uintptr_t)W % 16))
+        HOS_REFUSE("gemm_tc_logits: K and the leading dimensions must be multiples of 8 elements and the operands "
+                   "16-byte aligned (K %d lda %d ldw %d)", K, lda, ldw);
+    GemmParams p = {};
+    p.out = out; p.M = M; p.N = N; p.K = K; p.ldo = ldo; p.k_splits = 1; p.gate_rows = N; p.cap = cap;
+    p.score.chunks = ((K + GK - 1) / GK + kScoreBlocks - 1) / kScoreBlocks;
+    const int bn = M <= 16 ? 16 : (M <= 32 ? 32 : (M <= 64 ? 64 : 128)), tiles = (N + GM - 1) / GM;
+    CUtensorMap mm, mn;
+    int rc;
+    if ((rc = make_map(&mn, A, M, K, lda, bn))) return rc;
+    if ((rc = make_map(&mm, W, N, K, ldw, GM))) return rc;
+    if (bn == 16) return launch<16, kGEpiLogits, true, float>(mm, mn, p, tiles, stream);
+    if (bn == 32) return launch<32, kGEpiLogits, true, float>(mm, mn, p, tiles, stream);
+    if (bn == 64) return launch<64, kGEpiLogits, true, float>(mm, mn, p, tiles, stream);
+    return launch<128, kGEpiLogits, true, float>(mm, mn, p, tiles, stream);
+}
 
 // Floats of workspace of hos_gemm_tc_scores: the parts, and a wanted logit a row.
 extern "C" long long hos_gemm_tc_scores_workspace(int M, int N) {

@@ -100,18 +100,32 @@ def matmul_partials(x, w, k_splits: Optional[int] = None) -> Optional[torch.Tens
     return ws[: used.value]
 
 
-# Scores come out of the head's product from so many rows on.  Measured (B200, us by the product / by logits, soft-capped): 2,304 by 256,000, 20 rows
-# 240 / 246, 24 rows 236 / 265, 32 rows 233 / 338; 2,048 by 50,021: 20 rows 60 / 54, 24 rows 57 / 57, 32 rows 54 / 70; 4,096 by 32,000: 20 rows 64 / 62, 24
-# rows 63 / 65.  From 33 rows on logits come from tensor cores too, 64 rows of 2,304 by 256,000 without a cap 235 / 212, whose sums are less exact
-# (csrc/gemm_tc.cu, kScoreBlocks).
-SCORE_MIN_ROWS = NEVER if PAIR_MIN_ROWS == NEVER else 24
+# Scores come out of the head's product from so many rows on: below, its tiles of 256 rows are mostly empty, and what they multiply all the same costs
+# clocks under the power limit.  Measured (B200 under load, us by the product / by logits): 2,304 by 256,000, 24 rows 293 / 206, 64 rows 285 / 236, 96
+# rows 288 / 280, 128 rows 295 / 301; 2,048 by 50,021, 24 rows 69 / 47, 64 rows 57 / 52, 96 rows 59 / 61, 128 rows 60 / 67; 1,024 by 8,000, 64 rows
+# 15.5 / 15.5, 128 rows 16 / 20.
+SCORE_MIN_ROWS = NEVER if PAIR_MIN_ROWS == NEVER else 97
+
+
+def logits(x: torch.Tensor, w: torch.Tensor, cap: float) -> torch.Tensor:
+    """float32 [rows, vocab] of up to 128 rows, soft-capped if cap > 0, with sums as exact as `log_probs` has them (csrc/gemm_tc.cu, kScoreBlocks)."""
+    m, k = x.shape
+    out = torch.empty((m, w.shape[0]), dtype=torch.float32, device=x.device)
+    lib().call("hos_gemm_tc_logits", x.data_ptr(), w.data_ptr(), out.data_ptr(), m, w.shape[0], k, x.stride(0), w.stride(0), w.shape[0], float(cap),
+               ops._stream())
+    return out
+
+
+def operands_ok(x: torch.Tensor, w: torch.Tensor) -> bool:
+    """The product's rules for its operands."""
+    return (enabled and x.dtype == torch.bfloat16 and w.dtype == torch.bfloat16 and x.shape[1] == w.shape[1] and x.shape[1] % 8 == 0
+            and x.stride(1) == 1 and w.stride(1) == 1 and x.stride(0) % 8 == 0 and w.stride(0) % 8 == 0
+            and x.data_ptr() % 16 == 0 and w.data_ptr() % 16 == 0)
 
 
 def can_score(x: torch.Tensor, w: torch.Tensor) -> bool:
     """Whether log probabilities come out of the head's product itself: the product's rules, and rows enough."""
-    return (enabled and x.dtype == torch.bfloat16 and w.dtype == torch.bfloat16 and x.shape[0] >= SCORE_MIN_ROWS and x.shape[1] == w.shape[1]
-            and x.shape[1] % 8 == 0 and x.stride(1) == 1 and w.stride(1) == 1 and x.stride(0) % 8 == 0 and w.stride(0) % 8 == 0
-            and x.data_ptr() % 16 == 0 and w.data_ptr() % 16 == 0)
+    return x.shape[0] >= SCORE_MIN_ROWS and operands_ok(x, w)
 
 
 def log_probs(x: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, logprob: torch.Tensor, entropy: torch.Tensor, cap: float) -> None:

@@ -85,12 +85,17 @@ LOGITS_BYTES = 256 << 20        # of logits that `log_probs` holds at a time
 
 
 def _logits(x: torch.Tensor, w: torch.Tensor, cap: float) -> torch.Tensor:
-    """float32 [rows, vocab].  A handful of bfloat16 rows: the product that streams the head through registers, whose sums are the more exact (see
-    csrc/gemm_tc.cu, kScoreBlocks), and the soft-cap where the logits lie: 2,304 by 256,000, 8 rows 182 us, 16 rows 220, with their scores."""
-    if cap > 0.0 and x.dtype == torch.bfloat16 and x.shape[0] < 24 and not isinstance(w, Weight4) and not _force_plain:
-        out = matmul(x, w, out_dtype=torch.float32)
-        ops.softcap(out, cap)
-        return out
+    """float32 [rows, vocab].  A handful of bfloat16 rows: the product that streams the head through registers, and the soft-cap where the logits lie; 9
+    to 128: tensor cores, whose sums are added in chunks (csrc/gemm_tc.cu, kScoreBlocks).  Measured (B200 under load, us handful / tensor cores, with the
+    scores): 2,304 by 256,000, 8 rows 197 / 191, 16 rows 237 / 198, 32 rows 347 / 209; 2,048 by 50,021, 8 rows 40 / 46, 16 rows 47 / 46, 32 rows 64 / 48."""
+    if x.dtype == torch.bfloat16 and not isinstance(w, Weight4) and not _force_plain:
+        from . import gemm_skinny, gemm_tc
+        if x.shape[0] <= 8 and cap > 0.0 and gemm_skinny.operands_ok(x, w):
+            out = matmul(x, w, out_dtype=torch.float32)
+            ops.softcap(out, cap)
+            return out
+        if 8 < x.shape[0] <= gemm_tc.SWAP_MAX_ROWS and gemm_tc.operands_ok(x, w):
+            return gemm_tc.logits(x, w, cap)
     return matmul(x, w, out_dtype=torch.float32, epilogue=ops.EPI_SOFTCAP if cap > 0.0 else ops.EPI_NONE, cap=cap)
 
 

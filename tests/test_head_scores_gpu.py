@@ -100,7 +100,7 @@ def test_rows_apart_another_stream_and_a_replayed_graph(rows):
     check(other, plain(x, w, t, 30.0))
 
 
-@pytest.mark.parametrize("rows", [8, 9, 24, 32, 64, 65, 90])
+@pytest.mark.parametrize("rows", [8, 9, 24, 32, 64, 65, 90, 96, 97, 128])
 @pytest.mark.parametrize("cap,top", [(0.0, 0), (0.0, 2), (30.0, 0)])
 def test_few_rows_and_a_large_vocabulary(rows, cap, top):
     x, w, t = make(rows, 136, 20011, rows)
@@ -110,7 +110,7 @@ def test_few_rows_and_a_large_vocabulary(rows, cap, top):
         assert ((want[2].gather(1, got.top_ids.long()) - got.top_logprobs.double()).abs() <= 1e-4).all()
 
 
-@pytest.mark.parametrize("rows", [3, 40, 300])
+@pytest.mark.parametrize("rows", [3, 12, 30, 60, 96, 110, 300])
 @pytest.mark.parametrize("cap", [0.0, 30.0])
 def test_long_sums_lose_little(rows, cap):
     """Tensor cores cut their sums at every 16 products: by half of the last bit in the middle, 0.36 * 2^-23 of a sum that has grown to half of its
@@ -125,7 +125,7 @@ def test_long_sums_lose_little(rows, cap):
         assert (a.double() - b).norm() < part * largest, float((a.double() - b).norm() / largest)
 
 
-@pytest.mark.parametrize("rows", [1, 23, 24, 200])
+@pytest.mark.parametrize("rows", [1, 8, 9, 24, 64, 97, 200])
 @pytest.mark.parametrize("cap", [0.0, 30.0])
 def test_a_row_that_is_nearly_sure(rows, cap):
     """The product's scores keep the digits of small log probabilities, where the logits do: an error e of logits of 25 (2^-20 of them, and of the cap)
