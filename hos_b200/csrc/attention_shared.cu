@@ -113,6 +113,10 @@ __device__ __forceinline__ Walk small_walk(const SharedArgs& a, const SharedItem
     return walk_of(a, it, low, high);
 }
 
+// Long items are bound by their pages' bytes (B200: 64 rows of 64 pages, 16 kv heads of 128, 167 us, 164 at the copy rate), short ones by the latency of
+// an item's start, 3 us of loads that depend on one another, of which a CTA hides all but the first (64 rows of 7 pages 46 us, 35 at the
+// copy rate: DRAM 55%, issue slots 26%, mma.sync 8%).  16 keys a warp: a page's 64 rows are four warps', whose sums stay in registers over
+// the whole item; pages' 32 or 64 KB leave room for 2 to 6 in flight.
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) attn_shared_kernel(SharedArgs a) {
     extern __shared__ __align__(128) unsigned char smem[];
     unsigned char* ring = smem;                                                 // stage: keys, values
@@ -477,6 +481,10 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
     return ok != 0;
 }
 
+// A page is a chain of products, softmax and products, of which two run beside one another: 0.69 us with heads of 64, 0.80 of 128, 1.06 of 256 (with a
+// soft-cap 0.84 / 0.83 / 1.06), of which the products are 45 to 128 clocks each way; an item is 9 us besides.  Neither unit nor memory is full (32 rows of
+// 4 heads on 65,536 keys, 8 kv heads of 128: 67 us, DRAM 50%, tensor cores 27%, exponentials 27%, issue slots 27%); the warps wait for
+// one another.
 __global__ void __launch_bounds__(kTcThreads, 1)
 attn_shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, SharedArgs a) {
     extern __shared__ unsigned char smem_unaligned[];
@@ -854,7 +862,8 @@ attn_shared_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
 #endif
 
 // A row's parts joined; a row without parts (padding) becomes zeros, and so does one that sees no key.  WARPS warps take a (row, head), a
-// share of its parts each: lanes read the maxima of 32 parts at a time, then the sums of each part together.
+// share of its parts each: lanes read the maxima of 32 parts at a time, then the sums of each part together.  2.1 us with two parts of two rows, 4.2
+// with 18 parts of 32 rows of 32 heads of 128 (10 MB, in L2): a launch's length.
 template <int WARPS>
 __global__ void __launch_bounds__(256) attn_shared_merge_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml,
                                                                 const int* __restrict__ n_parts, int parts, int n_rows, int n_heads, bf16* out,
