@@ -140,7 +140,7 @@ class DecodeSession:
         self._windows = sorted({g.need.window or 0 for g in runner.cache.groups})
         # attention over pages that sequences share: the lists of work by (cache group, query heads), which of them the step at hand uses, and
         # for which slots and pages they were made
-        self._page_works, self.page_work, self._page_key, self._paged_for = {}, {}, (), None
+        self._page_works, self.page_work, self._page_key, self._paged_for, self._floors = {}, {}, (), None, {}
         self.n_live = 0
 
     @property
@@ -211,12 +211,14 @@ class DecodeSession:
             return
         # (a page more of a sequence's own makes the lists no less true, only less even: those are counted together)
         made_for = (tuple(slots), tuple((g.joins, g.version // max(16, len(slots))) for g, _ in sharers))
-        if made_for == self._paged_for:
+        if made_for == self._paged_for and all(lengths[i] > at for i, at in self._floors.items()):      # (a sequence may have been set back)
             return
-        self.page_work, key, plans = {}, [], {}
+        self.page_work, self._floors, key, plans = {}, {}, [], {}
         for i, (group, n_heads) in enumerate(sharers):
             if id(group) not in plans:
-                plans[id(group)] = shared_attention.step_plan(group, slots, lengths)
+                made = plans[id(group)] = shared_attention.step_plan(group, slots, lengths)
+                for at, floor in (made.floors() if made is not None else {}).items():
+                    self._floors[at] = max(floor, self._floors.get(at, 0))
             plan = plans[id(group)]
             if plan is None:
                 continue

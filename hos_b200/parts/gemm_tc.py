@@ -104,6 +104,7 @@ def matmul_partials(x, w, k_splits: Optional[int] = None) -> Optional[torch.Tens
 # clocks under the power limit.  Measured (B200 under load, us by the product / by logits): 2,304 by 256,000, 24 rows 293 / 206, 64 rows 285 / 236, 96
 # rows 288 / 280, 128 rows 295 / 301; 2,048 by 50,021, 24 rows 69 / 47, 64 rows 57 / 52, 96 rows 59 / 61, 128 rows 60 / 67; 1,024 by 8,000, 64 rows
 # 15.5 / 15.5, 128 rows 16 / 20.
+SCORE_BYTES = 256 << 20          # of workspace
 SCORE_MIN_ROWS = NEVER if PAIR_MIN_ROWS == NEVER else 97
 
 
@@ -134,9 +135,13 @@ def log_probs(x: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, logprob: t
     n = w.shape[0]
     f = lib().lib.hos_gemm_tc_scores_workspace
     f.restype, f.argtypes = ctypes.c_longlong, [ctypes.c_int, ctypes.c_int]
-    ws = torch.empty(f(m, n), dtype=torch.float32, device=x.device)
-    lib().call("hos_gemm_tc_scores", x.data_ptr(), w.data_ptr(), tokens.data_ptr(), logprob.data_ptr(), entropy.data_ptr(), m, n, k, x.stride(0),
-               w.stride(0), float(cap), ws.data_ptr(), ops._stream())
+    # up to 2 parts a row and 256 columns: so many rows at a time that they stay within SCORE_BYTES
+    each = max(256, SCORE_BYTES // (32 * ((n + 255) // 256)) // 256 * 256)
+    for lo in range(0, m, each):
+        rows = min(each, m - lo)
+        ws = torch.empty(f(rows, n), dtype=torch.float32, device=x.device)
+        lib().call("hos_gemm_tc_scores", x.data_ptr() + 2 * lo * x.stride(0), w.data_ptr(), tokens.data_ptr() + 4 * lo, logprob.data_ptr() + 4 * lo,
+                   entropy.data_ptr() + 4 * lo, rows, n, k, x.stride(0), w.stride(0), float(cap), ws.data_ptr(), ops._stream())
 
 
 def wait_probe(limit_cycles: int = 1 << 20) -> None:

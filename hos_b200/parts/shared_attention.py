@@ -43,12 +43,27 @@ class SharedPlan:
     def __init__(self, group, runs, rows: Sequence[range], slots: Sequence[int], lengths: Sequence[int], n_rows: int):
         self.group, self.version = group, group.version
         self.runs, self.rows, self.slots, self.lengths, self.n_rows = runs, rows, slots, lengths, n_rows
+        # what a step has to be like for the plan to hold: its sequences, their rows, and rows behind the shared pages
+        self.like = (tuple(slots), tuple(r.start for r in rows) + (n_rows,))
+        self.starts = tuple(n - len(r) for n, r in zip(lengths, rows))
         self._work: Dict[int, "Work"] = {}
 
     def lists(self, n_heads: int, keep: Optional[tuple] = None) -> "Lists":
         need = self.group.need
         return lists(self.runs, self.rows, self.slots, self.lengths, self.n_rows, n_heads // need.n_kv_heads, need.n_kv_heads, need.head_dim,
                      need.window, has_big(need.head_dim), keep)
+
+    def floors(self) -> dict:
+        """{place of a sequence: the first position behind the pages that it shares}: no row may lie lower."""
+        return {i: hi * ops.PAGE_TOKENS for members, _, hi in self.runs for i in members}
+
+    def check(self, step) -> None:
+        """Refuses a step of other sequences or rows than the plan's, or of rows in front of the end of what they share."""
+        if (tuple(step.slots_host), tuple(step.cu_host)) != self.like:
+            raise KernelError("attend: the step's sequences or rows are not those of the plan")
+        starts = tuple(step.starts_host)
+        if starts != self.starts and (len(starts) != len(self.starts) or any(starts[i] < at for i, at in self.floors().items())):
+            raise KernelError("attend: the step's rows lie before the end of the pages that the plan shares")
 
     def work(self, n_heads: int) -> "Work":
         w = self._work.get(n_heads)
@@ -356,6 +371,7 @@ def attend(q: torch.Tensor, out: torch.Tensor, step, cache: ops.PagedKVArgs, pla
         raise KernelError("attend: the plan is of another group of the cache")
     if plan.version != group.version:
         raise KernelError("attend: pages have changed since the plan was made")
+    plan.check(step)
     if n == 0:
         return
     work = plan.work(n_heads)

@@ -60,5 +60,7 @@ def log_probs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, out: Opt
     fresh = out is None
     if fresh:
         out = TokenScores.empty(logits.shape[0] if logits.dim() else 0, top, logits.device)
+    elif top and (out.top_ids is None or out.top_logprobs is None or out.top_ids.shape[-1] != top):
+        raise KernelError(f"log_probs: scores to write into without places for {top} alternatives")
     ops.log_probs(logits, tokens, out.logprob, out.entropy, out.top_ids if top else None, out.top_logprobs if top else None, fresh)
     return out

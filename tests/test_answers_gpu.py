@@ -340,3 +340,27 @@ def test_sequences_that_grow_by_many_pages(tmp_path, shared):
     assert shared
     for i, s in enumerate(seqs):
         assert_close(torch.stack([row[i] for row in rows]), P.forward_logits(w, cfg, s)[70:], "bfloat16", f"sequence {i}")
+
+
+@pytest.mark.parametrize("share", [True, False])
+def test_sequences_that_are_set_back(tmp_path, shared, share, monkeypatch):
+    """Forks set back into the pages that they share (their records and lengths), then stepped on: what lies behind is not seen.  (A window
+    as wide as the sequences: a ring of pages no longer has what lies before a narrow one.)"""
+    monkeypatch.setitem(TINY, "wide", (dict(TINY["D"][0], sliding_window=1000), 3))
+    folder = make_folder(tmp_path, "wide")
+    w, cfg = plain_model(folder)
+    rng = random.Random(9)
+    r = runner_for(folder, chunk_tokens=1, share_prefix=share)
+    first = random_tokens(rng, 250, 1000)
+    a, = r.admit(1)
+    r.step([a], [first])
+    slots = [a] + r.fork(a, 3)
+    seqs = [first + random_tokens(rng, 1, 1000) for _ in slots]
+    got = r.step(slots, [s[250:] for s in seqs])
+    assert bool(shared) == share
+    r.write_records(slots, pos=[100, 250, 140, 70])
+    seqs = [first[:n] + random_tokens(rng, 1, 1000) for n in (100, 250, 140, 70)]
+    got = r.step(slots, [s[-1:] for s in seqs])
+    for row, s in zip(got, seqs):
+        assert_close(row, P.forward_logits(w, cfg, s)[-1], "bfloat16", f"{len(s)} tokens")
+    r.cache.check()

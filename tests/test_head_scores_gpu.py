@@ -110,6 +110,17 @@ def test_few_rows_and_a_large_vocabulary(rows, cap, top):
         assert ((want[2].gather(1, got.top_ids.long()) - got.top_logprobs.double()).abs() <= 1e-4).all()
 
 
+def test_many_rows_go_some_at_a_time(monkeypatch):
+    from hos_b200.parts import gemm_tc
+    x, w, t = make(1300, 128, 3000, 7)
+    whole = linear.log_probs(x, w, t, 30.0)
+    monkeypatch.setattr(gemm_tc, "SCORE_BYTES", 600 * 32 * 12)
+    check(linear.log_probs(x, w, t, 30.0), plain(x, w, t, 30.0))
+    monkeypatch.setattr(linear, "LOGITS_BYTES", 4 * 3000 * 300)
+    some = linear.log_probs(x, w, t, 30.0, 2)
+    assert (some.logprob - whole.logprob).abs().max() < 1e-4 and some.top_ids.shape == (1300, 2)
+
+
 @pytest.mark.parametrize("rows", [3, 12, 30, 60, 96, 110, 300])
 @pytest.mark.parametrize("cap", [0.0, 30.0])
 def test_long_sums_lose_little(rows, cap):

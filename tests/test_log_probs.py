@@ -18,6 +18,12 @@ def test_so_many_alternatives_are_refused(top):
         log_probs(torch.zeros(2, 64), torch.zeros(2, dtype=torch.int32), top)
 
 
+@pytest.mark.parametrize("held", [0, 2])
+def test_scores_to_write_into_need_places_for_the_alternatives(held):
+    with pytest.raises(KernelError, match="places for 3"):
+        log_probs(torch.zeros(2, 64), torch.zeros(2, dtype=torch.int32), 3, TokenScores.empty(2, held, "cpu"))
+
+
 def test_scores_to_write_into_have_the_sizes_asked_for():
     s = TokenScores.empty(3, 4, "cpu")
     assert s.logprob.shape == s.entropy.shape == (3,) and s.top_ids.shape == s.top_logprobs.shape == (3, 4)

@@ -231,3 +231,26 @@ def test_a_nan_that_a_row_sees_is_its_own(dim, forks, cap):
     sa.attend(q, bad, step, t.view, plan, 4, dim ** -0.5, cap, None)
     hit[3, 2 * dim:] = True
     assert bad[hit].isnan().all() and torch.equal(bad[~hit], out[~hit])
+
+
+def test_steps_that_are_not_the_plans_are_refused():
+    from hos_b200.engine.batch import build_step
+    t = Tree(2, 64, seed=4)
+    a = t.new(200)
+    f, = t.fork(a)
+    t.bring([a, f], [5, 5])
+    plan = sa.plan(t.group, t.step([a, f], [2, 2]))
+    q = torch.randn(4, 256, generator=t.gen).to(torch.bfloat16).cuda()
+    for which, news in (([f, a], [2, 2]), ([a, f], [1, 3])):
+        with pytest.raises(KernelError, match="those of the plan"):
+            sa.attend(q, q.clone(), t.step(which, news), t.view, plan, 4, 1.0)
+    slots = [t.slots[a], t.slots[f]]
+    with pytest.raises(KernelError, match="before the end"):
+        sa.attend(q, q.clone(), build_step([[0] * 2] * 2, [203, 100], slots, t.dev, 1), t.view, plan, 4, 1.0)
+    earlier = build_step([[0] * 2] * 2, [201, 202], slots, t.dev, 1)                # before the plan's, behind what is shared: 192 tokens
+    out = torch.empty_like(q)
+    sa.attend(q, out, earlier, t.view, plan, 4, 64 ** -0.5)
+    t.k, t.v = ([x[i][:n] for i, n in ((a, 203), (f, 204))] for x in (t.k, t.v))
+    want = t.exact(q, [0, 1], [2, 2], 4, 64 ** -0.5, 0.0, None)
+    t.v = [v.abs() for v in t.v]
+    assert ((out.double().cpu() - want).abs() <= share_bound(t.exact(q, [0, 1], [2, 2], 4, 64 ** -0.5, 0.0, None), want)).all()
