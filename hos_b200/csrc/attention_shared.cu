@@ -71,6 +71,8 @@ struct SharedArgs {
     float scale, cap;
     int window;
     int beside_big;            // the small items run beside the big ones' kernel, which was launched just before
+    bf16* out;                 // not null: a small item's part is all of its rows' (no merge)
+    int out_stride;
 };
 
 __device__ int* g_shared_error_host = nullptr;
@@ -348,6 +350,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attn_shared_kernel(Share
                 const float4 b = *reinterpret_cast<const float4*>(sums + (size_t)(y * kPairs + p) * (HD + 4) + d);
                 l += v.y * f;
                 acc.x += b.x * f; acc.y += b.y * f; acc.z += b.z * f; acc.w += b.w * f;
+            }
+            if (a.out != nullptr) {                          // (as the merge would)
+                const float r = l > 0.f ? 1.f / l : 0.f;
+                *reinterpret_cast<uint2*>(a.out + (size_t)pair_of[p].x * a.out_stride + (size_t)pair_of[p].y * HD + d) =
+                    make_uint2(pack_bf16(acc.x * r, acc.y * r), pack_bf16(acc.z * r, acc.w * r));
+                continue;
             }
             const size_t at = ((size_t)pair_of[p].x * a.n_heads + pair_of[p].y) * a.parts + part;
             *reinterpret_cast<float4*>(a.part_o + at * HD + d) = acc;
@@ -959,6 +967,7 @@ struct SharedWork {
     int sms;                   // for the small ones
     int parts;                 // places of a (row, head) in the workspace
     int table_stride, ring_pages, n_heads, n_kv_heads, window;
+    int direct;                // 1: every row has one part, of a small item, which leaves the output itself
 };
 
 // out[n_rows, n_heads * head_dim] = softmax(c tanh(scale q . k / c)) v by the items of the work; see the head of this file.  workspace:
@@ -977,7 +986,9 @@ extern "C" int hos_attn_shared(const void* q, int q_stride, void* out, int out_s
     float* part_ml = workspace + (size_t)n_rows * k.n_heads * k.parts * HD;
     SharedArgs a{(const bf16*)q, q_stride, token_pos, reinterpret_cast<const SharedItem*>(k.items), k.counts, k.rows,
                  PagedKV{const_cast<void*>(k_pages), const_cast<void*>(v_pages), k.page_table, k.table_stride, k.ring_pages, k.n_kv_heads, HD},
-                 k.n_heads, k.parts, workspace, reinterpret_cast<float2*>(part_ml), scale, cap, k.window, k.big_most > 0 ? 1 : 0};
+                 k.n_heads, k.parts, workspace, reinterpret_cast<float2*>(part_ml), scale, cap, k.window, k.big_most > 0 ? 1 : 0,
+                 k.direct ? (bf16*)out : nullptr, out_stride};
+    if (k.direct && (k.big_most > 0 || k.most <= 0)) HOS_REFUSE("attn_shared: rows of one part are those of small items");
     int rc;
     if (k.big_most > 0) {
 #if (HOS_HEAD_DIM == 64) || (HOS_HEAD_DIM == 128) || (HOS_HEAD_DIM == 256)
@@ -1014,6 +1025,7 @@ extern "C" int hos_attn_shared(const void* q, int q_stride, void* out, int out_s
         launch_ahead(k.big_most > 0 || pdl_enabled(), attn_shared_kernel, dim3(grid), dim3(kThreads), kShared, stream, a);
         if ((rc = check_launch("attn_shared"))) return rc;
     }
+    if (k.direct) return 0;
     // many parts of few rows: eight warps a (row, head) (8 rows of 8 heads of 256, 33 parts: 6.8 us with one, 3.2 with eight)
     const int merged = n_rows * k.n_heads;
     auto merge = [&](auto kernel, int blocks) {

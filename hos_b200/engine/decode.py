@@ -211,7 +211,7 @@ class DecodeSession:
             return
         # (a page more of a sequence's own makes the lists no less true, only less even: those are counted together)
         made_for = (tuple(slots), tuple((g.joins, g.version // max(16, len(slots))) for g, _ in sharers))
-        if made_for == self._paged_for and all(lengths[i] > at for i, at in self._floors.items()):      # (a sequence may have been set back)
+        if made_for == self._paged_for and all(lengths[i] >= at for i, at in self._floors.items()):      # (a sequence may have been set back)
             return
         self.page_work, self._floors, key, plans = {}, {}, [], {}
         for i, (group, n_heads) in enumerate(sharers):

@@ -42,10 +42,14 @@ class SharedPlan:
 
     def __init__(self, group, runs, rows: Sequence[range], slots: Sequence[int], lengths: Sequence[int], n_rows: int):
         self.group, self.version = group, group.version
-        self.runs, self.rows, self.slots, self.lengths, self.n_rows = runs, rows, slots, lengths, n_rows
+        self.rows, self.slots, self.lengths, self.n_rows = rows, slots, lengths, n_rows
+        starts = [n - len(r) for n, r in zip(lengths, rows)]
+        # pages of which every row sees all (a page that is being written is nobody else's, but a sequence may have been forked since)
+        ends = [(members, lo, min(hi, min((starts[i] + 1) // ops.PAGE_TOKENS for i in members))) for members, lo, hi in runs]
+        self.runs = [(members, lo, hi) for members, lo, hi in ends if lo < hi]
         # what a step has to be like for the plan to hold: its sequences, their rows, and rows behind the shared pages
         self.like = (tuple(slots), tuple(r.start for r in rows) + (n_rows,))
-        self.starts = tuple(n - len(r) for n, r in zip(lengths, rows))
+        self.starts = tuple(starts)
         self._work: Dict[int, "Work"] = {}
 
     def lists(self, n_heads: int, keep: Optional[tuple] = None) -> "Lists":
@@ -54,7 +58,7 @@ class SharedPlan:
                      need.window, has_big(need.head_dim), keep)
 
     def floors(self) -> dict:
-        """{place of a sequence: the first position behind the pages that it shares}: no row may lie lower."""
+        """{place of a sequence: the end of the pages that it shares}: it has to be that long with its first row."""
         return {i: hi * ops.PAGE_TOKENS for members, _, hi in self.runs for i in members}
 
     def check(self, step) -> None:
@@ -62,7 +66,7 @@ class SharedPlan:
         if (tuple(step.slots_host), tuple(step.cu_host)) != self.like:
             raise KernelError("attend: the step's sequences or rows are not those of the plan")
         starts = tuple(step.starts_host)
-        if starts != self.starts and (len(starts) != len(self.starts) or any(starts[i] < at for i, at in self.floors().items())):
+        if starts != self.starts and (len(starts) != len(self.starts) or any(starts[i] + 1 < at for i, at in self.floors().items())):
             raise KernelError("attend: the step's rows lie before the end of the pages that the plan shares")
 
     def work(self, n_heads: int) -> "Work":
@@ -99,12 +103,13 @@ class Lists:
     def __init__(self, items: np.ndarray, big: np.ndarray, rows: np.ndarray, n_parts: np.ndarray, share: tuple):
         self.items, self.big, self.rows, self.n_parts, self.share, self.sms = items, big, rows, n_parts, share, share[2]
         self.parts = int(n_parts.max()) if n_parts.size else 0
+        self.direct = not len(big) and len(items) > 0 and bool((n_parts == 1).all())         # no row waits for a merge
 
 
 class SharedWork(ctypes.Structure):
     """A list of work as csrc/attention_shared.cu takes it."""
     _fields_ = [(name, ctypes.c_void_p) for name in ("counts", "n_parts", "items", "big_items", "rows", "page_table")] + \
-               [(name, ctypes.c_int) for name in ("most", "big_most", "sms", "parts", "table_stride", "ring_pages", "n_heads", "n_kv_heads", "window")]
+               [(name, ctypes.c_int) for name in ("most", "big_most", "sms", "parts", "table_stride", "ring_pages", "n_heads", "n_kv_heads", "window", "direct")]
 
 
 class Work:
@@ -130,13 +135,13 @@ class Work:
         self.fields = _fields(group, n_heads, made, base, base + 16, items, big, big + 4 * made.big.size)
         self.address = ctypes.addressof(self.fields)
         self.parts = made.parts
-        self.floats = n * n_heads * made.parts * (need.head_dim + 2)
+        self.floats = 0 if made.direct else n * n_heads * made.parts * (need.head_dim + 2)
 
 
 def _fields(group, n_heads: int, made: Lists, counts: int, n_parts: int, items: int, big: int, rows: int) -> SharedWork:
     need = group.need
     return SharedWork(counts, n_parts, items, big, rows, group.table_dev.data_ptr(), len(made.items), len(made.big), made.sms, made.parts,
-                      group.table_dev.shape[1], group.ring_pages, n_heads, need.n_kv_heads, need.window or 0)
+                      group.table_dev.shape[1], group.ring_pages, n_heads, need.n_kv_heads, need.window or 0, int(made.direct))
 
 
 class ReplayedWork:
@@ -172,9 +177,10 @@ class ReplayedWork:
         f.most, f.big_most, f.parts = _rounded(f.most), _rounded(f.big_most), _rounded(f.parts)
         self.share = made.share
         f.sms = f.sms if f.sms == ops.sm_count() else max(1, f.sms // 16 * 16)
+        f.direct = int(made.direct and len(made.n_parts) == self.n)          # (padding rows are the merge's to clear)
         self.address = ctypes.addressof(f)
-        self.floats = self.n * self.n_heads * f.parts * (self.group.need.head_dim + 2)
-        self.key = (f.most, f.big_most, f.sms, f.parts)
+        self.floats = 0 if f.direct else self.n * self.n_heads * f.parts * (self.group.need.head_dim + 2)
+        self.key = (f.most, f.big_most, f.sms, f.parts, f.direct)
         return True
 
 
@@ -195,7 +201,7 @@ def has_big(head_dim: int) -> bool:
 # are written and read at 5 TB/s.  Measured (B200), 8 answers on 8,000 keys, 8 heads of 256 over 4, shares of 5 / 8 / 16 / 32 pages of a block of
 # 16 pairs 19.9 / 21.0 / 27.9 / 44.3 us; of 8 / 16 / 32 pages of two blocks of 8 pairs 19.5 / 26.5 / 45.4; 16 heads of 128 over 16, of 4 / 16 / 32 / 64
 # pages of two blocks of 8 pairs 31.3 / 26.4 / 37.4 / 62.4.
-SMALL_US, SMALL_MORE_US, BIG_US = 3.0, 1.0, 9.0
+SMALL_US, SMALL_MORE_US, BIG_US, MERGE_US = 3.0, 1.0, 9.0, 2.1
 BYTES_US, PART_BYTES_US = 5.8e6, 5.0e6
 
 
@@ -214,9 +220,14 @@ def _cuts(pages: np.ndarray):
     return np.asarray(lengths), -(-pages[:, None] // np.asarray(lengths)) if pages.size else np.zeros((0, len(lengths)), dtype=np.int64)
 
 
-def shares(small: np.ndarray, big: np.ndarray, big_pairs: np.ndarray, per_item: int, kv: int, head_dim: int, distinct: int,
+def shares(*sizes, **how) -> tuple:
+    """`estimate`'s cut."""
+    return estimate(*sizes, **how)[0]
+
+
+def estimate(small: np.ndarray, big: np.ndarray, big_pairs: np.ndarray, per_item: int, kv: int, head_dim: int, distinct: int,
            keep: Optional[tuple] = None) -> tuple:
-    """(pages of a small share, of a big one, SMs for the small ones) for small blocks and big blocks of so many pages, `distinct` pages in all
+    """((pages of a small share, of a big one, SMs for the small ones), us) for small blocks and big blocks of so many pages, `distinct` pages in all
     counting shared ones once (OPEN: not cut): the cut that makes the step shortest by the estimate above.  An item is run per_item times (a big one kv
     times).  Big items have an SM each; the small ones run beside them on the SMs that are left, or after them on all.  `keep`: what an
     earlier step had; it stays where that costs up to a tenth, so that steps replay one program."""
@@ -246,7 +257,7 @@ def shares(small: np.ndarray, big: np.ndarray, big_pairs: np.ndarray, per_item: 
             i, j = at
     spare = int(left[i])
     uncut = [OPEN if k + 1 == len(of) else int(of[k]) for k, of in ((j, lengths), (i, big_lengths))]
-    return *uncut, spare if spare and big.size and max(big_us[i], beside[i, j]) <= after[i, j] else sms
+    return (*uncut, spare if spare and big.size and max(big_us[i], beside[i, j]) <= after[i, j] else sms), float(us[i, j])
 
 
 def is_big(pairs: int, pages: int, head_dim: int) -> bool:
@@ -258,9 +269,10 @@ def is_big(pairs: int, pages: int, head_dim: int) -> bool:
 
 
 def lists(runs, rows: Sequence[range], slots: Sequence[int], lengths: Sequence[int], n_rows: int, per: int, kv: int, head_dim: int,
-          window: Optional[int], big: bool, keep: Optional[tuple] = None) -> Lists:
+          window: Optional[int], big: bool, keep: Optional[tuple] = None, alone: Optional[bool] = None) -> Lists:
     """The work: a run's rows in blocks of up to 8 pairs, or of up to 128 where a kernel has such blocks (`big`) and that is faster, over the
-    run's pages, each sequence's over the rest of its own."""
+    run's pages, each sequence's over the rest of its own.  Short sequences with few rows that are as soon done without any of that, an item each and no
+    merge, are (`alone`; measured, B200, 2 sequences of 139 tokens, 8 heads of 256 over 4: two kernels 8.4 us, one AAA)."""
     big = big and per <= BLOCK
     chunks = -(-per // PAIRS)
     n_seqs = len(slots)
@@ -297,7 +309,15 @@ def lists(runs, rows: Sequence[range], slots: Sequence[int], lengths: Sequence[i
         else:
             cut(of, slot, 0, OPEN, *lo_hi, n)
     pages = [np.asarray([b[6] for b in of], dtype=np.int64) for of in blocks]
-    share = shares(pages[0], pages[1], np.asarray([len(b[0]) * per for b in blocks[1]], dtype=np.int64), kv * chunks, kv, head_dim, distinct, keep)
+    share, us = estimate(pages[0], pages[1], np.asarray([len(b[0]) * per for b in blocks[1]], dtype=np.int64), kv * chunks, kv, head_dim, distinct, keep)
+    if alone:
+        share = (OPEN, OPEN, share[2])
+    elif alone is None and chunks == 1 and int(news.max()) * per <= PAIRS:
+        whole, page_us = behind - first, _page_us(head_dim)[0]
+        work = n_seqs * kv * SMALL_MORE_US + int(whole.sum()) * kv * page_us / (2 if head_dim <= 128 else 1)
+        bytes_us = int(whole.sum()) * kv * 256.0 * head_dim / BYTES_US
+        if SMALL_US + max(int(whole.max()) * page_us, work / ops.sm_count(), bytes_us) <= us + MERGE_US:
+            return lists([], rows, slots, lengths, n_rows, per, kv, head_dim, window, big, None, True)
     most = max(2, MOST_PARTS // max(1, 4 * n_rows * per * kv * (head_dim + 2)))
     n_parts = np.zeros(n_rows, dtype=np.int32)
     listed = []
@@ -342,6 +362,8 @@ def plan(group, step) -> SharedPlan:
     for s, n in zip(slots, lengths):
         if s not in group._slot_pages or group.pages_for(n) > len(group._slot_pages[s]):
             raise KernelError(f"slot {s} has no pages for {n} tokens")
+        if s in group._dirty:
+            raise KernelError(f"the pages of slot {s} are not on the device yet (CacheManager.flush)")
     return SharedPlan(group, group.shared_runs(slots, lengths), rows, slots, lengths, step.n_tokens)
 
 

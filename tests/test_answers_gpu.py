@@ -19,6 +19,7 @@ pytestmark = pytest.mark.gpu
 def shared(monkeypatch):
     """Steps share however little that spares; how often attention over shared pages ran."""
     monkeypatch.setattr(sa, "SHARE_BYTES", 0)
+    monkeypatch.setattr(sa, "MERGE_US", -1e9)               # (short sequences share too)
     calls = []
     run = sa._run
 

@@ -11,6 +11,14 @@ from hos_b200.parts import shared_attention as sa
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True, params=["as estimated", "never alone"])
+def merged(request, monkeypatch):
+    """Short sequences are an item each, without a merge, where the estimate says so; all of these tests run with that ruled out too."""
+    if request.param == "never alone":
+        monkeypatch.setattr(sa, "MERGE_US", -1e9)
+    return request.param
+
+
 def compare(t, which, news, heads, cap=0.0, scale=None, plan=None, q=None, out=None):
     step = t.step(which, news)
     plan = plan or sa.plan(t.group, step)
@@ -68,14 +76,14 @@ def test_pieces_of_several_rows(dim, per, window, news):
 
 @pytest.mark.parametrize("dim,kv,per,forks", [(64, 2, 1, 63), (64, 1, 8, 40), (128, 2, 2, 63), (128, 1, 5, 30), (256, 2, 2, 63), (256, 1, 16, 20), (64, 1, 100, 3), (128, 1, 128, 2)])
 @pytest.mark.parametrize("prefix,cap", [(1, 0.0), (700, 50.0), (1500, 0.0)])
-def test_many_forks(dim, kv, per, forks, prefix, cap):
+def test_many_forks(dim, kv, per, forks, prefix, cap, merged):
     t = Tree(kv, dim, seed=forks + prefix)
     a = t.new(prefix)
     all_ = [a] + t.fork(a, forks)
     for j, i in enumerate(all_):
         t.bring([i], [1 + (37 * j) % 130])
     plan = compare(t, all_, [1] * len(all_), per * kv, cap=cap)
-    assert prefix < 64 or plan.work(per * kv).fields.big_most > 0
+    assert prefix < 64 or merged == "as estimated" or plan.work(per * kv).fields.big_most > 0
 
 
 @pytest.mark.parametrize("dim", [64, 128, 256])
@@ -254,3 +262,17 @@ def test_steps_that_are_not_the_plans_are_refused():
     want = t.exact(q, [0, 1], [2, 2], 4, 64 ** -0.5, 0.0, None)
     t.v = [v.abs() for v in t.v]
     assert ((out.double().cpu() - want).abs() <= share_bound(t.exact(q, [0, 1], [2, 2], 4, 64 ** -0.5, 0.0, None), want)).all()
+
+
+def test_short_sequences_need_no_merge(merged):
+    t = Tree(4, 256, seed=2)
+    a = t.new(130)
+    all_ = [a] + t.fork(a)
+    t.bring(all_, [9, 5])
+    plan = compare(t, all_, [1, 1], 8, cap=50.0)
+    assert plan.work(8).fields.direct == (merged == "as estimated") and bool(plan.work(8).floats) == (merged != "as estimated")
+    many = t.fork(t.new(1200), 3)                            # forked, nothing brought yet: rows in a page that all share
+    with pytest.raises(KernelError, match="flush"):
+        sa.plan(t.group, t.step(many, [1, 1, 1]))
+    t.cache.flush()
+    assert compare(t, many + all_, [1] * 5, 8).work(8).fields.direct == 0
