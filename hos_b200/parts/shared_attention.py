@@ -272,7 +272,8 @@ def lists(runs, rows: Sequence[range], slots: Sequence[int], lengths: Sequence[i
           window: Optional[int], big: bool, keep: Optional[tuple] = None, alone: Optional[bool] = None) -> Lists:
     """The work: a run's rows in blocks of up to 8 pairs, or of up to 128 where a kernel has such blocks (`big`) and that is faster, over the
     run's pages, each sequence's over the rest of its own.  Short sequences with few rows that are as soon done without any of that, an item each and no
-    merge, are (`alone`; measured, B200, 2 sequences of 139 tokens, 8 heads of 256 over 4: two kernels 8.4 us, one AAA)."""
+    merge, are (`alone`; measured, B200, us with shared pages and a merge / an item each: 2 sequences of 139 tokens, 8 heads of 256 over 4, 8.4 / 8.0, 16 of
+    them 13.3 / 8.2; 32 heads of 128 over 8, 16 of 139 tokens 12.1 / 7.3, 16 of 340 12.5 / 10.4, 16 of 660 13.6 / 15.3, 16 of 1,100 12.9 / 22.3)."""
     big = big and per <= BLOCK
     chunks = -(-per // PAIRS)
     n_seqs = len(slots)
