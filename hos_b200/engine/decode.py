@@ -34,6 +34,7 @@ from ..parts.base import StepInfo
 from ..sampling.sampler import SamplingParams
 from ..sampling.scores import TokenScores, log_probs, scored_tokens
 
+SHARED_PROGRAMS = 48             # programs of steps that share pages that a session keeps (they differ in how many items there are)
 BUCKETS = (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256)
 META = 2 + ops.MAX_STOPS        # live rows, number of stop ids, the stop ids
 
@@ -279,6 +280,11 @@ class DecodeSession:
         if prog is not None:
             return prog
         c = self.runner.cache
+        # (the first program's pool is everyone's: it stays)
+        sharing = [k for i, k in enumerate(self._programs) if i > 0 and k[-1]] if key[-1] else ()
+        if len(sharing) >= SHARED_PROGRAMS:
+            torch.cuda.synchronize()
+            del self._programs[sharing[0]]
         keep = (c.record.clone(), c.recent.clone())
         state = c.snapshot_state(self.slot[: self.n_live])      # a recurrence must not be moved on twice
         before = ops.launch_count

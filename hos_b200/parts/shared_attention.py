@@ -98,7 +98,7 @@ def pays(group, runs, news: Sequence[int]) -> bool:
 
 
 class Lists:
-    """Items (of up to 8 pairs, then of up to 128), their rows, each row's number of parts, and the cut that they have (`shares`), on the host."""
+    """Items (of up to 8 pairs, then of up to 128), their rows, each row's number of parts, and the cut that they have (`estimate`), on the host."""
 
     def __init__(self, items: np.ndarray, big: np.ndarray, rows: np.ndarray, n_parts: np.ndarray, share: tuple):
         self.items, self.big, self.rows, self.n_parts, self.share, self.sms = items, big, rows, n_parts, share, share[2]
@@ -218,11 +218,6 @@ def _cuts(pages: np.ndarray):
         n = max(n + 1, n * 6 // 5)
     lengths.append(most)
     return np.asarray(lengths), -(-pages[:, None] // np.asarray(lengths)) if pages.size else np.zeros((0, len(lengths)), dtype=np.int64)
-
-
-def shares(*sizes, **how) -> tuple:
-    """`estimate`'s cut."""
-    return estimate(*sizes, **how)[0]
 
 
 def estimate(small: np.ndarray, big: np.ndarray, big_pairs: np.ndarray, per_item: int, kv: int, head_dim: int, distinct: int,

@@ -365,3 +365,27 @@ def test_sequences_that_are_set_back(tmp_path, shared, share, monkeypatch):
     for row, s in zip(got, seqs):
         assert_close(row, P.forward_logits(w, cfg, s)[-1], "bfloat16", f"{len(s)} tokens")
     r.cache.check()
+
+
+def test_few_programs_are_kept(tmp_path, shared, monkeypatch):
+    """Steps whose lists want another program every time: the oldest go, and the steps stay right."""
+    from hos_b200.engine import decode
+    monkeypatch.setattr(decode, "SHARED_PROGRAMS", 2)
+    refill, number = sa.ReplayedWork.refill, iter(range(100))
+
+    def another(self, made):
+        ok = refill(self, made)
+        self.key = self.key + (next(number),)
+        return ok
+    monkeypatch.setattr(sa.ReplayedWork, "refill", another)
+    runners = [runner_for(make_folder(tmp_path / str(share), "D"), chunk_tokens=1, share_prefix=share) for share in (True, False)]
+    slots = []
+    for r in runners:
+        a, = r.admit(1)
+        r.step([a], [[3, 8, 1] * 80])
+        slots.append([a] + r.fork(a, 3))
+    for t in range(8):
+        runners[0].decode_session(4)._paged_for = None       # new lists, and by the above another program
+        got, want = (r.step(s, [[t]] * 4) for r, s in zip(runners, slots))
+        assert_close(got, want.cpu(), "bfloat16", f"step {t}")
+        assert sum(bool(k[-1]) for k in runners[0].decode_session(4)._programs) <= 3

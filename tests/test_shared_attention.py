@@ -165,7 +165,7 @@ def test_refusals():
                                           ([], [46] * 3 + [2] * 5, 4)])
 @pytest.mark.parametrize("dim", [16, 64, 128, 256])
 def test_shares_leave_no_round_of_big_items_nearly_empty(small, big, kv, dim):
-    n_small, n_big, sms = sa.shares(np.asarray(small, dtype=np.int64), np.asarray(big, dtype=np.int64), np.asarray([128] * len(big), dtype=np.int64), kv, kv, dim, sum(small) + sum(big))
+    (n_small, n_big, sms), _ = sa.estimate(np.asarray(small, dtype=np.int64), np.asarray(big, dtype=np.int64), np.asarray([128] * len(big), dtype=np.int64), kv, kv, dim, sum(small) + sum(big))
     assert n_small >= 1 and n_big >= 1 and 1 <= sms <= 148
     items = sum(-(-p // n_big) for p in big) * kv
     assert items <= 148 or len(big) * kv > 148 or items > 2 * 148 - 8 * kv
@@ -177,3 +177,15 @@ def test_blocks_of_few_pairs_and_of_many():
     assert sorted({it[1] for it in made.items.tolist()}) == [1, 4] and {it[1] for it in made.big.tolist()} == {32}
     plain = sa.lists([(list(range(40)), 0, 60)], rows, list(range(40)), [4000] * 40, 40, 2, 4, 128, None, False)
     assert len(plain.big) == 0 and max(it[1] for it in plain.items.tolist()) == 4
+
+
+def test_a_cut_is_kept_while_it_costs_little():
+    small, big = np.asarray([3, 1, 4, 1, 5], dtype=np.int64), np.asarray([125], dtype=np.int64)
+    pairs = np.asarray([16], dtype=np.int64)
+    first, us = sa.estimate(small, big, pairs, 4, 4, 256, 139)
+    for more in range(1, 12):
+        best, least = sa.estimate(small + more, big, pairs, 4, 4, 256, 139 + 5 * more)
+        kept, costs = sa.estimate(small + more, big, pairs, 4, 4, 256, 139 + 5 * more, first)
+        assert least <= costs <= 1.1 * least and (kept == best or kept[1] == first[1])
+    far, _ = sa.estimate(np.asarray([900], dtype=np.int64), big, pairs, 4, 4, 256, 1025, (sa.OPEN, 2, 20))
+    assert far[0] < 900                                      # what costs more is not kept
