@@ -542,13 +542,15 @@ def log_probs_blocks(rows: int, vocab: int) -> tuple:
     a tile of 32,768 numbers or more; clusters of 4 and 8 only as many as run at once beside one another (33 of 4 and 15 of 8 do here; 32 and
     14 are taken).  Measured (B200, 256,000 numbers, 5 alternatives, us by blocks of 1,024 threads a row 1 / 2 / 4 / 8 and of 256 threads 1): 1
     row 21.0 / 15.4 / 11.7 / 9.5 and 38; 15 rows 22.1 / 16.1 / 12.2 / 9.9; 16 rows 22.0 / 16.1 / 12.1 / 17.3; 33 rows 24.1 / 17.9 / 15.3 / 27.9; 36
-    rows 24.2 / 18.2 / 24.8 / 28.5; 148 rows 31.0 / 38.5 / 60 / 90 and 53; 300 rows, 20 alternatives, 80.8 / 93.7 / 127 /
-    209 and 79.0; 1,500 rows of 2,200: 64 with 1,024 threads, 14.3 with 256, 9.2 with 128."""
-    if vocab <= 4096:
+    rows 24.2 / 18.2 / 24.8 / 28.5; 148 rows 31.0 / 38.5 / 60 / 90 and 53.  More rows than SMs, by blocks of 1,024 / 256 / 128 threads: 200 of 256,000
+    numbers 55.5 / 65.0 / 102, 400 83.7 / 82.2 / 113, 1,000 192 / 185 / 176; 200 of 100,003 33.2 / 31.1 / 46.6; 400 of 32,003 23.4 / 16.1 / 20.5, 1,000
+    53.7 / 33.8 / 32.4; 2,000 of 10,000 88 / 34 / 27; 120 of 10,000 7.8 / 6.8 / 8.3; 1,500 of 2,200 64 / 14.3 / 9.2."""
+    sms = sm_count()
+    if vocab <= 4096 or rows > 4 * sms:
         return 128, 1
-    if rows > sm_count() or vocab <= 8192:
+    if vocab <= 16384 or rows > (2 * sms if vocab > 131072 else sms):
         return 256, 1
-    blocks, at_once = 1, {2: sm_count(), 4: 128, 8: 112}
+    blocks, at_once = 1, {2: sms, 4: 128, 8: 112}
     while blocks < 8 and vocab > 32768 * blocks and 2 * rows * blocks <= at_once[2 * blocks]:
         blocks *= 2
     return 1024, blocks
