@@ -389,7 +389,11 @@ __global__ void rope_kv_write_kernel(const TSrc* __restrict__ src, int n_parts, 
     extern __shared__ float2 sincos_tab[];          // [rotary_dim / 2]
     const int n = blockIdx.x;
     const int seq = token_seq[n];
-    if (seq < 0) return;
+    if (seq < 0) {                                   // padding: a row that is formed here becomes zeros (attention reads on behind a
+        if ((const void*)src != (const void*)qkv)    // sequence's last row)
+            for (int e = threadIdx.x; e < (n_heads + 2 * cache.n_kv_heads) * cache.head_dim; e += blockDim.x) qkv[(size_t)n * row_stride + e] = from_float<T>(0.f);
+        return;
+    }
     const int pos = token_pos[n];
     const int hd = cache.head_dim, nkv = cache.n_kv_heads;
     const int half = rotary_dim >> 1;
@@ -482,7 +486,12 @@ rope_kv_write_vec_kernel(const float* __restrict__ parts, int n_parts, size_t pa
     extern __shared__ float2 sincos_tab[];          // [rotary_dim / 2]
     const int n = blockIdx.x;
     const int seq = token_seq[n];
-    if (seq < 0) return;
+    if (seq < 0) {
+        if (PARTS)
+            for (int e = (blockIdx.y * blockDim.x + threadIdx.x) * 8; e < (n_heads + 2 * cache.n_kv_heads) * cache.head_dim; e += gridDim.y * blockDim.x * 8)
+                *reinterpret_cast<uint4*>(qkv + (size_t)n * row_stride + e) = make_uint4(0, 0, 0, 0);
+        return;
+    }
     const int pos = token_pos[n];
     const int hd = cache.head_dim, nkv = cache.n_kv_heads;
     const int half = rotary_dim >> 1;

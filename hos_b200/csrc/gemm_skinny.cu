@@ -302,8 +302,11 @@ qkv_rope_skinny_kernel(const bf16* __restrict__ A, const bf16* __restrict__ W, b
 #pragma unroll
         for (int w = 0; w < kSkinnyWarps; ++w) { v0 += part[w][m][r][tt]; v1 += part[w][m][r + 8][tt]; }
         const int seq = q.token_seq[tok];
-        if (seq < 0) continue;                                   // padding: nothing is stored
         const int fa_ = f_lo + step * r, fb_ = f_hi + step * r;
+        if (seq < 0) {                                           // padding: zeros, as attention reads on behind a sequence's last row (with a
+            out[(size_t)tok * ldo + fa_] = out[(size_t)tok * ldo + fb_] = __float2bfloat16_rn(0.f);      // weight of 0, which makes no number of NaN)
+            continue;
+        }
         if (rotated) {
             const int i = 8 * t + r;                             // index of the pair within the head
             float sn, cs;
